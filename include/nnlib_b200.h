@@ -344,6 +344,136 @@ NNLIB_B200_API int nnlib_b200_batched_gemm(const nnlib_b200_gemm_params* p, void
 /* NNLIB_B200_PATH_* that batched_gemm would take for p, or a negative error */
 NNLIB_B200_API int nnlib_b200_batched_gemm_path(const nnlib_b200_gemm_params* p);
 
+/* RMS norm of every query and key head followed by the rotation of its features by position, in one pass:
+     r = 1 / sqrt(mean(x^2) + eps),   n = x * r * g,   y = n with its feature pairs turned,
+   for the d features x of each head of q (weights gq) and of k (weights gk).  Pair p < rot / 2 is turned by the angle
+   position * freqs[p]: (a, b) -> (a cos - b sin, a sin + b cos); a and b are features p and p + rot / 2 of the head,
+   or 2p and 2p + 1 with interleaved = 1.  Features rot .. d - 1 are normalised only.  Angles are Float64 until they are
+   reduced to one turn, everything else Float32; results are rounded once.  The reference has no counterpart. */
+typedef struct nnlib_b200_norm_rope_params {
+  size_t struct_size;        /* = sizeof(nnlib_b200_norm_rope_params) */
+  int32_t dtype;             /* element type of q, k and of the results */
+  int32_t wdtype;            /* element type of gq, gk and of their gradients: dtype or NNLIB_B200_F32 */
+  int32_t interleaved;
+  int32_t reserved;
+  int64_t d, rot;            /* features of a head (even, at most 256); rotated ones (even, at most d) */
+  int64_t Hq, Hk, L, B;      /* query heads, key heads, tokens, batch; one of Hq and Hk may be 0 */
+  const void* q;             /* (Hq*d, L, B), feature stride 1 */
+  const void* k;             /* (Hk*d, L, B) */
+  int64_t q_stride_l, q_stride_b, k_stride_l, k_stride_b;   /* elements, 0 = dense */
+  const void* gq;            /* (d) */
+  const void* gk;
+  const double* freqs;       /* (rot / 2): angle per position */
+  const int32_t* positions;  /* position of token (l, b) at positions[l*s[0] + b*s[1]]; NULL: start */
+  int64_t positions_stride[2];
+  const int32_t* start;      /* (B): token l of sequence b is at start[b] + l; NULL: start0 + l */
+  int64_t start0;
+  float eps;
+  void* yq;                  /* forward: results, dense (Hq*d, L, B) and (Hk*d, L, B); backward: ignored */
+  void* yk;
+  const void* dyq;           /* backward: cotangents of yq and yk, feature stride 1 */
+  const void* dyk;
+  int64_t dyq_stride_l, dyq_stride_b, dyk_stride_l, dyk_stride_b;
+  void* dq;                  /* backward: written dense */
+  void* dk;
+  void* dgq;                 /* backward: (d), summed over tokens and heads in Float32 in a fixed order */
+  void* dgk;
+} nnlib_b200_norm_rope_params;
+
+NNLIB_B200_API int nnlib_b200_norm_rope(const nnlib_b200_norm_rope_params* p, void* stream);
+/* Its pullback, from q and k themselves (nothing is kept of the forward call).  workspace: device memory, 16-byte
+   aligned, at least nnlib_b200_norm_rope_bwd_workspace_bytes(p) bytes; it need not be cleared. */
+NNLIB_B200_API size_t nnlib_b200_norm_rope_bwd_workspace_bytes(const nnlib_b200_norm_rope_params* p);
+NNLIB_B200_API int nnlib_b200_norm_rope_bwd(const nnlib_b200_norm_rope_params* p, void* workspace, size_t workspace_bytes,
+                                            void* stream);
+
+/* Key / value cache held in 8 bits: a pool of pages of `page` tokens each, with one scale for every page and head, of
+   keys and of values.  An element stands for code * scale.
+     k_codes, v_codes  (d*H, page, pages)  element (e, t, p) at [e + d*H*(t + page*p)], one byte
+     k_scale, v_scale  (H, pages)          Float32, at [h + H*p]
+   Token number l of sequence b lives in slot l % page of page table[l / page + table_stride*b]; without a table in page
+   (pages / B)*b + l / page.  A sequence has at most `rows` pages, rows * page tokens are its capacity.
+   A page number outside 0 .. pages - 1 is never followed: a write leaves its tokens out, a read and attention give NaN.
+   Codes: NNLIB_B200_INT8, -127 .. 127, scale = largest magnitude / 127; NNLIB_B200_E4M3 (four bits of exponent, three of
+   mantissa, no infinities), scale = the smallest power of two that brings the largest magnitude to 448 or less.  A
+   scale below 2^-126 is stored as 0, with codes of zero.  A block that is given a NaN or an infinity gets the scale
+   NaN: all of its tokens read as NaN until the page is begun anew. */
+enum {
+  NNLIB_B200_INT8 = 0,
+  NNLIB_B200_E4M3 = 1
+};
+
+typedef struct nnlib_b200_cache {
+  size_t struct_size;        /* = sizeof(nnlib_b200_cache) */
+  int32_t code;              /* NNLIB_B200_INT8 / NNLIB_B200_E4M3 */
+  int32_t reserved;
+  int64_t d, H;              /* features of a head (a multiple of 16, at most 256), heads */
+  int64_t page, pages;       /* tokens of a page (a power of two, 16 .. 256), pages of the pool */
+  void* k_codes;             /* 16-byte aligned */
+  void* v_codes;
+  float* k_scale;
+  float* v_scale;
+  int64_t B;                 /* sequences */
+  const int32_t* table;      /* (rows, B) page numbers, or NULL */
+  int64_t table_stride;      /* elements between two sequences, 0 = rows */
+  int64_t rows;              /* pages of a sequence; without a table pages / B */
+} nnlib_b200_cache;
+
+/* Tokens on their way into or out of a cache. */
+typedef struct nnlib_b200_cache_tokens {
+  size_t struct_size;        /* = sizeof(nnlib_b200_cache_tokens) */
+  int32_t dtype;             /* element type of k and v */
+  int32_t reserved;
+  int64_t L;                 /* tokens of a sequence */
+  void* k;                   /* (d*H, L, B), feature stride 1; read by cache_write, written by cache_read */
+  void* v;
+  int64_t k_stride_l, k_stride_b, v_stride_l, v_stride_b;   /* elements, 0 = dense */
+  const int32_t* start;      /* (B): token l of sequence b has number start[b] + l; NULL: start0 + l */
+  int64_t start0;
+  const int32_t* count;      /* cache_write: (B), the first count[b] tokens of sequence b are written; NULL: all L */
+  const int32_t* lens;       /* cache_read: (B), tokens from number lens[b] on come back as zeros; NULL: none do */
+} nnlib_b200_cache_tokens;
+
+/* Quantises new tokens into the cache behind the start[b] tokens that sequence b holds; tokens from start[b] on are
+   overwritten or, in the slots behind the new ones, left as they are.  A page that held tokens before keeps the larger
+   of its scale and the one that the new tokens ask for; where that grows, the older codes are rounded to it anew,
+   code * (old scale / new scale).  Tokens at a negative number or beyond the capacity are left out.  A page that is
+   written by two sequences of one call ends with either's tokens. */
+NNLIB_B200_API int nnlib_b200_cache_write(const nnlib_b200_cache* c, const nnlib_b200_cache_tokens* t, void* stream);
+/* code * scale of tokens start[b] .. start[b] + L - 1, rounded to dtype; zeros at a negative number, from lens[b] on and
+   beyond the capacity. */
+NNLIB_B200_API int nnlib_b200_cache_read(const nnlib_b200_cache* c, const nnlib_b200_cache_tokens* t, void* stream);
+
+/* Attention of new queries over such a cache: x = sum_j softmax_j(scale * q . k_j) v_j over the tokens j < lens[b] of
+   the query's own sequence and, causal, j <= start[b] + i for query i.  Hq query heads share H cache heads: query head h
+   reads cache head h / (Hq / H).  Products run on codes, which 16-bit floating point holds exactly, with Float32 sums;
+   Float32 arrays take two 16-bit terms of each query element and weight (about 22 bits).  A scale of values below 2^-100
+   counts as 2^-100.  A query that sees no token gives NaN (or zeros), one that sees a token of a page with a NaN scale
+   gives NaN, and one that does not is not touched by it. */
+typedef struct nnlib_b200_cache_attn_params {
+  size_t struct_size;        /* = sizeof(nnlib_b200_cache_attn_params) */
+  int32_t dtype;             /* element type of q and x */
+  int32_t causal;
+  int32_t nan_on_fully_masked;
+  int32_t reserved;
+  int64_t Hq, L;             /* query heads (a multiple of H), queries of a sequence */
+  const void* q;             /* (d*Hq, L, B), feature stride 1 */
+  void* x;                   /* (d*Hq, L, B), feature stride 1 */
+  int64_t q_stride_l, q_stride_b, x_stride_l, x_stride_b;   /* elements, 0 = dense */
+  const int32_t* lens;       /* (B): tokens in the cache, clamped to 0 .. capacity; NULL: len0 for all */
+  int64_t len0;
+  const int32_t* start;      /* (B): position of query 0; NULL: lens[b] - L */
+  float scale;               /* 0 means 1/sqrt(d) */
+  float* lse;                /* optional, (L, Hq, B) Float32: natural-log sum of exponentials, -Inf where nothing is seen */
+  int32_t* status;           /* optional device int32, as in nnlib_b200_attn_params */
+} nnlib_b200_cache_attn_params;
+
+/* workspace: device memory, 16-byte aligned, at least nnlib_b200_cache_attn_workspace_bytes(c, p) bytes (which may be 0);
+   it need not be cleared and is free again when the call's kernels have run. */
+NNLIB_B200_API size_t nnlib_b200_cache_attn_workspace_bytes(const nnlib_b200_cache* c, const nnlib_b200_cache_attn_params* p);
+NNLIB_B200_API int nnlib_b200_cache_attn(const nnlib_b200_cache* c, const nnlib_b200_cache_attn_params* p, void* workspace,
+                                         size_t workspace_bytes, void* stream);
+
 /* make_causal_mask (src/attention.jl:149-153): fill an (L, L) byte matrix
    with m[i + L*j] = (i <= j). */
 NNLIB_B200_API int nnlib_b200_causal_fill(uint8_t* mask, int64_t L, void* stream);

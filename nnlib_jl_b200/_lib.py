@@ -13,6 +13,7 @@ import os
 from pathlib import Path
 
 F16, BF16, F32 = 0, 1, 2
+INT8, E4M3 = 0, 1
 
 OK = 0
 INVALID_ARG = -1
@@ -55,6 +56,13 @@ EXPORTS = (
     "nnlib_b200_attn_path",
     "nnlib_b200_softmax_fwd",
     "nnlib_b200_softmax_bwd",
+    "nnlib_b200_norm_rope",
+    "nnlib_b200_norm_rope_bwd",
+    "nnlib_b200_norm_rope_bwd_workspace_bytes",
+    "nnlib_b200_cache_write",
+    "nnlib_b200_cache_read",
+    "nnlib_b200_cache_attn",
+    "nnlib_b200_cache_attn_workspace_bytes",
     "nnlib_b200_device_health",
     "nnlib_b200_selftest_wait_runout",
     "nnlib_b200_strerror",
@@ -152,6 +160,88 @@ class SoftmaxParams(C.Structure):
         self.struct_size = C.sizeof(SoftmaxParams)
 
 
+class NormRopeParams(C.Structure):
+    """Mirror of ``nnlib_b200_norm_rope_params``."""
+
+    _fields_ = [
+        ("struct_size", C.c_size_t),
+        ("dtype", C.c_int32), ("wdtype", C.c_int32), ("interleaved", C.c_int32), ("reserved", C.c_int32),
+        ("d", C.c_int64), ("rot", C.c_int64),
+        ("Hq", C.c_int64), ("Hk", C.c_int64), ("L", C.c_int64), ("B", C.c_int64),
+        ("q", C.c_void_p), ("k", C.c_void_p),
+        ("q_stride_l", C.c_int64), ("q_stride_b", C.c_int64), ("k_stride_l", C.c_int64), ("k_stride_b", C.c_int64),
+        ("gq", C.c_void_p), ("gk", C.c_void_p),
+        ("freqs", C.c_void_p),
+        ("positions", C.c_void_p), ("positions_stride", C.c_int64 * 2),
+        ("start", C.c_void_p), ("start0", C.c_int64),
+        ("eps", C.c_float),
+        ("yq", C.c_void_p), ("yk", C.c_void_p),
+        ("dyq", C.c_void_p), ("dyk", C.c_void_p),
+        ("dyq_stride_l", C.c_int64), ("dyq_stride_b", C.c_int64), ("dyk_stride_l", C.c_int64), ("dyk_stride_b", C.c_int64),
+        ("dq", C.c_void_p), ("dk", C.c_void_p), ("dgq", C.c_void_p), ("dgk", C.c_void_p),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__(**kw)
+        self.struct_size = C.sizeof(NormRopeParams)
+
+
+class Cache(C.Structure):
+    """Mirror of ``nnlib_b200_cache``."""
+
+    _fields_ = [
+        ("struct_size", C.c_size_t),
+        ("code", C.c_int32), ("reserved", C.c_int32),
+        ("d", C.c_int64), ("H", C.c_int64), ("page", C.c_int64), ("pages", C.c_int64),
+        ("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("B", C.c_int64),
+        ("table", C.c_void_p), ("table_stride", C.c_int64), ("rows", C.c_int64),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__(**kw)
+        self.struct_size = C.sizeof(Cache)
+
+
+class CacheTokens(C.Structure):
+    """Mirror of ``nnlib_b200_cache_tokens``."""
+
+    _fields_ = [
+        ("struct_size", C.c_size_t),
+        ("dtype", C.c_int32), ("reserved", C.c_int32),
+        ("L", C.c_int64),
+        ("k", C.c_void_p), ("v", C.c_void_p),
+        ("k_stride_l", C.c_int64), ("k_stride_b", C.c_int64), ("v_stride_l", C.c_int64), ("v_stride_b", C.c_int64),
+        ("start", C.c_void_p), ("start0", C.c_int64),
+        ("count", C.c_void_p), ("lens", C.c_void_p),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__(**kw)
+        self.struct_size = C.sizeof(CacheTokens)
+
+
+class CacheAttnParams(C.Structure):
+    """Mirror of ``nnlib_b200_cache_attn_params``."""
+
+    _fields_ = [
+        ("struct_size", C.c_size_t),
+        ("dtype", C.c_int32), ("causal", C.c_int32), ("nan_on_fully_masked", C.c_int32), ("reserved", C.c_int32),
+        ("Hq", C.c_int64), ("L", C.c_int64),
+        ("q", C.c_void_p), ("x", C.c_void_p),
+        ("q_stride_l", C.c_int64), ("q_stride_b", C.c_int64), ("x_stride_l", C.c_int64), ("x_stride_b", C.c_int64),
+        ("lens", C.c_void_p), ("len0", C.c_int64), ("start", C.c_void_p),
+        ("scale", C.c_float),
+        ("lse", C.c_void_p), ("status", C.c_void_p),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__(**kw)
+        self.struct_size = C.sizeof(CacheAttnParams)
+        if "nan_on_fully_masked" not in kw:
+            self.nan_on_fully_masked = 1
+
+
 _lib = None
 
 
@@ -212,6 +302,21 @@ def load() -> C.CDLL:
     lib.nnlib_b200_softmax_fwd.restype = C.c_int
     lib.nnlib_b200_softmax_bwd.argtypes = [C.POINTER(SoftmaxParams), C.c_void_p]
     lib.nnlib_b200_softmax_bwd.restype = C.c_int
+    NR, CP, CT, CA = (C.POINTER(t) for t in (NormRopeParams, Cache, CacheTokens, CacheAttnParams))
+    lib.nnlib_b200_norm_rope.argtypes = [NR, C.c_void_p]
+    lib.nnlib_b200_norm_rope.restype = C.c_int
+    lib.nnlib_b200_norm_rope_bwd.argtypes = [NR, C.c_void_p, C.c_size_t, C.c_void_p]
+    lib.nnlib_b200_norm_rope_bwd.restype = C.c_int
+    lib.nnlib_b200_norm_rope_bwd_workspace_bytes.argtypes = [NR]
+    lib.nnlib_b200_norm_rope_bwd_workspace_bytes.restype = C.c_size_t
+    for name in ("nnlib_b200_cache_write", "nnlib_b200_cache_read"):
+        fn = getattr(lib, name)
+        fn.argtypes = [CP, CT, C.c_void_p]
+        fn.restype = C.c_int
+    lib.nnlib_b200_cache_attn.argtypes = [CP, CA, C.c_void_p, C.c_size_t, C.c_void_p]
+    lib.nnlib_b200_cache_attn.restype = C.c_int
+    lib.nnlib_b200_cache_attn_workspace_bytes.argtypes = [CP, CA]
+    lib.nnlib_b200_cache_attn_workspace_bytes.restype = C.c_size_t
     lib.nnlib_b200_attn_path.argtypes = [P]
     lib.nnlib_b200_attn_path.restype = C.c_int
     lib.nnlib_b200_device_health.argtypes = [C.c_void_p]

@@ -29,6 +29,8 @@ bool force_simt() {
   return v;
 }
 
+}  // namespace
+
 // NNLIB_B200_LOG=1: one line per call on stderr (entry point, sizes, options, kernel family and, when the
 // tensor-core kernels were not taken, why) so that a call that silently runs on the CUDA-core kernels —
 // an unaligned pointer, a stride that is not a multiple of 8 elements — can be found.
@@ -61,6 +63,14 @@ bool on_current_device(const void* ptr, int dev) {
   if (at.type == cudaMemoryTypeManaged) return true;
   return at.type == cudaMemoryTypeDevice && at.device == dev;
 }
+
+int finish(cudaError_t e) {
+  if (e == cudaSuccess) return NNLIB_B200_OK;
+  set_last_cuda_error(e);
+  return NNLIB_B200_CUDA_ERROR;
+}
+
+namespace {
 
 // The caller's arrays must live on the current device: the kernels are launched there and the library
 // never switches devices.  q and x are always looked up (a result written to another GPU's memory, or a
@@ -175,12 +185,6 @@ int resolve(const nnlib_b200_attn_params* p, unsigned need, AttnArgs* out, bool 
   }
   *out = a;
   return NNLIB_B200_OK;
-}
-
-int finish(cudaError_t e) {
-  if (e == cudaSuccess) return NNLIB_B200_OK;
-  set_last_cuda_error(e);
-  return NNLIB_B200_CUDA_ERROR;
 }
 
 // the two-tile tensor-core kernels: 16-bit arrays with d = dv <= 128 a multiple of 8

@@ -1,0 +1,463 @@
+// Attention over the 8-bit cache by streamed warp-level products: generated tokens, short runs of them, Float32 arrays.
+//
+// A key or value element is code * scale, the scale one number per page and head, so both products run on the codes
+// themselves, which 16-bit floating point holds exactly:
+//   logit_ij = (q_i . kcode_j) * scale * ks(page of j)
+//   x_i = sum_j w_ij vcode_j / sum_j w_ij / vs(page of j),   w_ij = 2^(log2e * logit_ij + log2 vs(page of j) - m_i)
+// i.e. a page's value scale goes into the exponent, where the running maximum m_i takes it up: no product is scaled, no
+// accumulator has a page's scale in it, and a weight's size is the size of what it adds to x.  q_i is brought to a
+// largest element in [2^13, 2^14) by a power of two of its own; w is rounded to 16 bits after a factor of 2^14, so that
+// weights keep 11 bits down to 2^-28 of the largest.  Float32 arrays: q and w as the sum of two 16-bit terms each.
+//
+// HBM is the bound (2 d bytes per key and head for up to 16 rows), so what counts is bytes in flight: nothing is staged,
+// a warp streams 16 keys at a time straight into the fragments of m16n8k16 products.  Rows of a tile: the query heads of
+// a group and the queries, row r = query r / G, head r % G of the group.
+//   S: lane (g, c) = (lane / 4, lane % 4) takes 16 consecutive features 64 G + 16 c .. of key g: word t of its 16 bytes is
+//      what it owes to k-step t, two codes to each register; Q's fragments are loaded in the same order.
+//   O: columns may be any features: column g of product j is feature g * (D/8) + j, so a lane loads D/8 consecutive bytes
+//      of each of its four keys 2c, 2c+1, 2c+8, 2c+9 and pairs the codes of two keys up.
+// Int8 to 16 bits: (code ^ 0x80) under 0x64 is 1024 + 128 + code, less 1152.  E4M3: the conversion instruction.
+// A unit's keys (sequence, cache head, row tile) are dealt to `splits` blocks in equal runs of 64; the four warps of a
+// block alternate.  attn_split_reduce_kernel merges the blocks' running maxima, sums and outputs.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "cache_codes.cuh"
+#include "split_reduce.cuh"
+
+namespace nb200 {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kStep = 16;                 // keys a warp takes at a time
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kValueFloor = 7.8886090522101181e-31f;    // 2^-100
+constexpr float kWeightBits = 14.f;
+
+__device__ __forceinline__ float ninf() { return __int_as_float(0xff800000); }
+__device__ __forceinline__ float qnan() { return __int_as_float(0x7fc00000); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  uint32_t u;
+  memcpy(&u, &v, 4);
+  return u;
+}
+
+// two codes in the low bytes of the halves of u (as they are: int8) to two 16-bit numbers
+__device__ __forceinline__ uint32_t int8_pair(uint32_t biased, uint32_t sel) {
+  const uint32_t v = __byte_perm(biased, 0x64646464u, sel);
+  uint32_t r;
+  asm("sub.f16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(0x64806480u));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t two) {
+  uint32_t r;
+  asm("{ .reg .b16 t; cvt.u16.u32 t, %1; cvt.rn.f16x2.e4m3x2 %0, t; }" : "=r"(r) : "r"(two));
+  return r;
+}
+// bytes 0, 1 and 2, 3 of a word as two pairs
+template <int CODE>
+__device__ __forceinline__ void word_pairs(uint32_t w, uint32_t& p0, uint32_t& p1) {
+  if (CODE == NNLIB_B200_INT8) {
+    const uint32_t u = w ^ 0x80808080u;
+    p0 = int8_pair(u, 0x4140u);
+    p1 = int8_pair(u, 0x4342u);
+  } else {
+    p0 = e4m3_pair(w);
+    p1 = e4m3_pair(w >> 16);
+  }
+}
+
+template <bool ROWS8>
+__device__ __forceinline__ void mma(float (&c)[ROWS8 ? 2 : 4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                    uint32_t b0, uint32_t b1) {
+  if constexpr (ROWS8) {
+    float u, v;
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %10, %10};"
+        : "+f"(c[0]), "+f"(c[1]), "=f"(u), "=f"(v) : "r"(a0), "r"(0u), "r"(a2), "r"(0u), "r"(b0), "r"(b1), "f"(0.f));
+  } else {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+}
+
+// BYTES codes of a lane, as words
+template <int BYTES>
+__device__ __forceinline__ void load_codes(const unsigned char* p, uint32_t (&w)[BYTES / 4]) {
+  if constexpr (BYTES == 8) {
+    asm("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+  } else {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i)
+      asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+          : "=r"(w[4 * i]), "=r"(w[4 * i + 1]), "=r"(w[4 * i + 2]), "=r"(w[4 * i + 3]) : "l"(p + 16 * i));
+  }
+}
+
+__device__ __forceinline__ int seq_len(const CacheAttnArgs& a, int b) {
+  const long long cap = a.c.rows << a.c.log_page;
+  const long long n = a.lens ? (long long)a.lens[b] : a.len0;
+  return (int)(n < 0 ? 0 : (n < cap ? n : cap));
+}
+// position of query 0 of a sequence of len tokens
+__device__ __forceinline__ long long seq_start(const CacheAttnArgs& a, int b, int len) {
+  return a.start ? (long long)a.start[b] : (long long)len - a.L;
+}
+// the last key that query i sees
+__device__ __forceinline__ int last_key(const CacheAttnArgs& a, long long start, int i, int len) {
+  if (!a.causal) return len - 1;
+  const long long e = start + i;
+  return e < 0 ? -1 : (e < len ? (int)e : len - 1);
+}
+
+template <int D, bool ROWS8> struct Cfg { static constexpr int kCtas = D <= 64 ? 4 : (D <= 128 ? (ROWS8 ? 4 : 3) : 2); };
+
+// T: element type of q and x; HILO: two 16-bit terms for an element of q and for a weight (T = float)
+template <typename T, int D, int CODE, bool ROWS8>
+__global__ void __launch_bounds__(kWarps * 32, Cfg<D, ROWS8>::kCtas)
+cache_attn_kernel(const CacheAttnArgs a, const int splits) {
+  constexpr bool HILO = sizeof(T) == 4;
+  constexpr int R = ROWS8 ? 1 : 2, ROWS = 8 * R, KS = D / 16, GK = D / 64, VB = D / 8;
+  __shared__ float sm_o[kWarps][ROWS][D];
+  __shared__ float sm_m[kWarps][ROWS], sm_l[kWarps][ROWS];
+  const CacheArgs& cc = a.c;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int G = a.Hq / cc.H, rows = a.L * G, tiles = (rows + ROWS - 1) / ROWS;
+  // blocks of one sequence's cache heads side by side: they read whole rows of the cache together
+  int item = blockIdx.x;
+  const int h = item % cc.H;
+  item /= cc.H;
+  const int split = item % splits;
+  item /= splits;
+  const int tile = item % tiles, b = item / tiles;
+  const int row0 = tile * ROWS;
+  const int len = seq_len(a, b);
+  const long long start = seq_start(a, b, len);
+  const int kend = last_key(a, start, (min(row0 + ROWS, rows) - 1) / G, len) + 1;
+  // this block's keys: whole groups of 64
+  const int groups = (kend + 63) / 64, share = (groups + splits - 1) / splits;
+  const int key_lo = min(split * share, groups) * 64, key_hi = min(min((split + 1) * share, groups) * 64, kend);
+  const unsigned char* kbase = cc.codes[0] + (long long)h * cc.d;
+  const unsigned char* vbase = cc.codes[1] + (long long)h * cc.d;
+
+  // Q's fragments, brought to a largest element in [2^13, 2^14)
+  uint32_t qa[R][KS][2], qlo[HILO ? R : 1][HILO ? KS : 1][2];
+  float crow[R];                               // what a row's products are multiplied by, but for the page's scale
+  int lim[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int row = row0 + g + 8 * r, i = row / G, hq = h * G + row % G;
+    const bool live = row < rows;
+    lim[r] = live ? last_key(a, start, i, len) : -1;
+    const T* qp = reinterpret_cast<const T*>(a.q) + (live ? (long long)i * a.q_sl + (long long)b * a.q_sb + (long long)hq * cc.d : 0);
+    float top = 0.f;
+#pragma unroll
+    for (int G4 = 0; G4 < GK; ++G4)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int f = 64 * G4 + 16 * c + e;
+        if (live && f < cc.d) top = fmaxf(top, fabsf(Elem<T>::to_f(qp[f])));
+      }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int ex = (top > 0.f && top <= 3.402823466e38f) ? 13 - ilogbf(top) : 0;
+    crow[r] = scalbnf(a.scale * kLog2e, -ex);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int f = 64 * (ks / 4) + 16 * c + 4 * (ks % 4) + e;
+        v[e] = (live && f < cc.d) ? scalbnf(Elem<T>::to_f(qp[f]), ex) : 0.f;
+      }
+      qa[r][ks][0] = half2_bits(v[0], v[1]);
+      qa[r][ks][1] = half2_bits(v[2], v[3]);
+      if constexpr (HILO) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] -= __half2float(__float2half_rn(v[e]));
+        qlo[r][ks][0] = half2_bits(v[0], v[1]);
+        qlo[r][ks][1] = half2_bits(v[2], v[3]);
+      }
+    }
+  }
+
+  // Pages, 32 of a warp's steps at a time: lane n looks up step n's page and scales
+  int pg = 0;
+  float ksc = 0.f, vsc = 0.f;
+  auto look_up = [&](int key) {
+    const bool in = key < key_hi;
+    const long long page = in ? cache_page(cc, b, (long long)key >> cc.log_page) : -1;
+    pg = page < 0 ? 0 : (int)page;
+    ksc = page < 0 ? qnan() : cc.scale[0][page * cc.H + h];
+    vsc = page < 0 ? qnan() : cc.scale[1][page * cc.H + h];
+  };
+  uint32_t kf[2][GK][4], vf[4][VB / 4];
+  auto load_k = [&](int key0, int page) {
+    const long long slot = ((long long)page << cc.log_page) + (key0 & ((1 << cc.log_page) - 1));
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+      for (int G4 = 0; G4 < GK; ++G4) {
+        const int f = 64 * G4 + 16 * c;
+        if (f < cc.d) load_codes<16>(kbase + (slot + nt * 8 + g) * cc.row + f, kf[nt][G4]);
+      }
+  };
+  auto load_v = [&](int key0, int page) {
+    const long long slot = ((long long)page << cc.log_page) + (key0 & ((1 << cc.log_page) - 1));
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (VB * g < cc.d) load_codes<VB>(vbase + (slot + 2 * c + (u & 1) + (u >> 1) * 8) * cc.row + VB * g, vf[u]);
+  };
+#pragma unroll
+  for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+    for (int G4 = 0; G4 < GK; ++G4)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) kf[nt][G4][w] = 0u;
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+#pragma unroll
+    for (int w = 0; w < VB / 4; ++w) vf[u][w] = 0u;
+
+  float m[R], l[R], o[D / 8][2 * R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) m[r] = ninf(), l[r] = 0.f;
+#pragma unroll
+  for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+    for (int e = 0; e < 2 * R; ++e) o[j][e] = 0.f;
+
+  const int stride = kWarps * kStep;
+  int key0 = key_lo + warp * kStep;
+  if (key0 < key_hi) {
+    look_up(key0 + lane * stride);
+    const int page = __shfl_sync(0xffffffffu, pg, 0);
+    load_k(key0, page);
+    load_v(key0, page);
+  }
+  for (int n = 0; key0 < key_hi; key0 += stride, ++n) {
+    const float ks = __shfl_sync(0xffffffffu, ksc, n & 31), vs = __shfl_sync(0xffffffffu, vsc, n & 31);
+    const int next = key0 + stride;
+    if ((n & 31) == 31 && next < key_hi) look_up(next + lane * stride);
+    const int page = __shfl_sync(0xffffffffu, pg, (n + 1) & 31);
+
+    float sc[2][2 * R];
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 2 * R; ++e) sc[nt][e] = 0.f;
+#pragma unroll
+      for (int k2 = 0; k2 < KS; ++k2) {
+        uint32_t b0, b1;
+        word_pairs<CODE>(kf[nt][k2 / 4][k2 % 4], b0, b1);
+        mma<ROWS8>(sc[nt], qa[0][k2][0], qa[R - 1][k2][0], qa[0][k2][1], qa[R - 1][k2][1], b0, b1);
+        if constexpr (HILO) mma<ROWS8>(sc[nt], qlo[0][k2][0], qlo[R - 1][k2][0], qlo[0][k2][1], qlo[R - 1][k2][1], b0, b1);
+      }
+    }
+    if (next < key_hi) load_k(next, page);
+
+    // scales of this step's page (16 keys never cross one)
+    const float vse = vs >= kValueFloor ? vs : ((vs >= 0.f) ? kValueFloor : qnan());
+    const float lvs = log2f(vse) + kWeightBits, ivs = __fdiv_rn(1.f, vse);
+    uint32_t pa[R][2], plo[HILO ? R : 1][2];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float f = crow[r] * ks;
+      float t[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        t[u] = fmaf(sc[u >> 1][2 * r + (u & 1)], f, lvs);
+        if (key0 + 2 * c + (u & 1) + (u >> 1) * 8 > lim[r]) t[u] = ninf();
+      }
+      float mx = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float mn = fmaxf(m[r], mx - kWeightBits);
+      if (__any_sync(0xffffffffu, mn > m[r])) {
+        const float fo = (m[r] == ninf()) ? 0.f : ex2(m[r] - mn);
+        l[r] *= fo;
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) {
+          o[j][2 * r] *= fo;
+          o[j][2 * r + 1] *= fo;
+        }
+        m[r] = mn;
+      }
+      const float ref = (mn == ninf()) ? 0.f : mn;
+      float p[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) p[u] = ex2(t[u] - ref);
+      const float sum = (p[0] + p[1]) + (p[2] + p[3]);
+      // this lane's keys only; a page that the row does not see adds nothing, whatever its scale is
+      if (!(sum == 0.f)) l[r] = fmaf(sum, ivs, l[r]);
+      pa[r][0] = half2_bits(p[0], p[1]);
+      pa[r][1] = half2_bits(p[2], p[3]);
+      if constexpr (HILO) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) p[u] -= __half2float(__float2half_rn(p[u]));
+        plo[r][0] = half2_bits(p[0], p[1]);
+        plo[r][1] = half2_bits(p[2], p[3]);
+      }
+    }
+    // E4M3 has a NaN; a slot behind the last token may hold anything
+    if (CODE == NNLIB_B200_E4M3 && key0 + kStep > kend) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (key0 + 2 * c + (u & 1) + (u >> 1) * 8 >= kend)
+#pragma unroll
+          for (int w = 0; w < VB / 4; ++w) vf[u][w] = 0u;
+    }
+#pragma unroll
+    for (int w = 0; w < VB / 4; ++w) {
+      // the codes of keys 2c and 2c + 1 side by side, features 4w .. 4w + 3
+      const uint32_t a01 = __byte_perm(vf[0][w], vf[1][w], 0x5140), a23 = __byte_perm(vf[0][w], vf[1][w], 0x7362);
+      const uint32_t b01 = __byte_perm(vf[2][w], vf[3][w], 0x5140), b23 = __byte_perm(vf[2][w], vf[3][w], 0x7362);
+      uint32_t b0[4], b1[4];
+      word_pairs<CODE>(a01, b0[0], b0[1]);
+      word_pairs<CODE>(a23, b0[2], b0[3]);
+      word_pairs<CODE>(b01, b1[0], b1[1]);
+      word_pairs<CODE>(b23, b1[2], b1[3]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        mma<ROWS8>(o[4 * w + e], pa[0][0], pa[R - 1][0], pa[0][1], pa[R - 1][1], b0[e], b1[e]);
+        if constexpr (HILO) mma<ROWS8>(o[4 * w + e], plo[0][0], plo[R - 1][0], plo[0][1], plo[R - 1][1], b0[e], b1[e]);
+      }
+    }
+    if (next < key_hi) load_v(next, page);
+  }
+
+  // merge the four warps
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int row = g + 8 * r;
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    if (c == 0) {
+      sm_m[warp][row] = m[r];
+      sm_l[warp][row] = l[r];
+    }
+    // columns 2c and 2c + 1 of product j: features VB (2c) + j and VB (2c + 1) + j
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int j = 0; j < D / 8; j += 4)
+        *reinterpret_cast<float4*>(&sm_o[warp][row][VB * (2 * c + e) + j]) =
+            make_float4(o[j][2 * r + e], o[j + 1][2 * r + e], o[j + 2][2 * r + e], o[j + 3][2 * r + e]);
+  }
+  __syncthreads();
+  for (int idx = threadIdx.x; idx < ROWS * D; idx += kWarps * 32) {
+    const int rr = idx / D, e = idx % D, row = row0 + rr;
+    if (row >= rows) break;
+    const int i = row / G, hq = h * G + row % G;
+    float M = ninf(), L = 0.f, acc = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm_m[w][rr]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float mw = sm_m[w][rr], f = mw == ninf() ? (sm_l[w][rr] == 0.f ? 0.f : 1.f) : ex2(mw - M);
+      L = fmaf(sm_l[w][rr], f, L);
+      if (f != 0.f) acc = fmaf(sm_o[w][rr][e], f, acc);
+    }
+    if (splits > 1) {
+      const long long unit = hq + (long long)a.Hq * b, at = (unit * splits + split) * a.L + i;
+      if (e < cc.d) a.ws[((((long long)a.Hq * cc.B * splits * a.L * 2) + 3) & ~3LL) + at * cc.d + e] = acc;
+      if (e == 0) {
+        a.ws[at * 2] = M - kWeightBits;              // (L has that factor)
+        a.ws[at * 2 + 1] = L;
+      }
+    } else {
+      const bool dead = L == 0.f;
+      if (e < cc.d) {
+        const float out = dead ? (a.nan_fm ? qnan() : 0.f) : acc / L;
+        reinterpret_cast<T*>(a.x)[(long long)i * a.x_sl + (long long)b * a.x_sb + (long long)hq * cc.d + e] = Elem<T>::from_f(out);
+      }
+      if (e == 0 && a.lse) a.lse[i + (long long)a.L * (hq + (long long)a.Hq * b)] = dead ? ninf() : fmaf(M - kWeightBits, 0.6931471805599453f, logf(L));
+    }
+  }
+}
+
+int row_tile(const CacheAttnArgs& a, int dtype) {
+  // (two 16-bit terms, or a head of 256 features, leave registers for eight rows only)
+  return (dtype == NNLIB_B200_F32 || a.c.d > 128 || (long long)a.L * (a.Hq / a.c.H) <= 8) ? 8 : 16;
+}
+
+// Blocks of a unit: enough for four blocks on each SM, but no fewer than 256 keys each where the cache is full.
+int split_count(const CacheAttnArgs& a, int dtype) {
+  const long long rows = (long long)a.L * (a.Hq / a.c.H), tile = row_tile(a, dtype);
+  const long long units = (long long)a.c.B * a.c.H * ((rows + tile - 1) / tile);
+  long long cap = a.c.rows << a.c.log_page;
+  if (!a.lens) cap = std::min(cap, std::max(a.len0, 0LL));
+  const long long n = std::min((4 * 148 + units - 1) / units, (cap + 255) / 256);
+  return (int)std::max(1LL, std::min(n, 1024LL));
+}
+
+AttnArgs reduce_args(const CacheAttnArgs& a) {
+  AttnArgs r;
+  std::memset(&r, 0, sizeof(r));
+  r.x = a.x;
+  r.x_sl = a.x_sl;
+  r.x_sb = a.x_sb;
+  r.lse = a.lse;
+  r.lse_sb = (long long)a.L * a.Hq;
+  r.ws = a.ws;
+  r.inv_keep = 1.f;
+  r.nan_fm = a.nan_fm;
+  r.dv = a.c.d;
+  r.H = a.Hq;
+  r.B = a.c.B;
+  r.Lq = a.L;
+  return r;
+}
+
+template <typename T, int D, int CODE, bool ROWS8>
+cudaError_t launch(const CacheAttnArgs& a, int splits, cudaStream_t st) {
+  const long long rows = (long long)a.L * (a.Hq / a.c.H), tile = ROWS8 ? 8 : 16;
+  const long long blocks = (long long)a.c.B * a.c.H * ((rows + tile - 1) / tile) * splits;
+  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  cache_attn_kernel<T, D, CODE, ROWS8><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a, splits);
+  count_launch();
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || splits == 1) return e;
+  const AttnArgs r = reduce_args(a);
+  attn_split_reduce_kernel<T, false><<<(unsigned)((long long)a.Hq * a.c.B * a.L), 128, 0, st>>>(r, splits);
+  count_launch();
+  return cudaGetLastError();
+}
+
+template <typename T, int CODE>
+cudaError_t launch_d(const CacheAttnArgs& a, int rows, int splits, cudaStream_t st) {
+  if (a.c.d > 128) return launch<T, 256, CODE, true>(a, splits, st);
+  if constexpr (sizeof(T) == 2) {
+    if (rows == 16) return a.c.d <= 64 ? launch<T, 64, CODE, false>(a, splits, st) : launch<T, 128, CODE, false>(a, splits, st);
+  }
+  return a.c.d <= 64 ? launch<T, 64, CODE, true>(a, splits, st) : launch<T, 128, CODE, true>(a, splits, st);
+}
+
+template <typename T>
+cudaError_t launch_c(const CacheAttnArgs& a, int rows, int splits, cudaStream_t st) {
+  return a.c.code == NNLIB_B200_INT8 ? launch_d<T, NNLIB_B200_INT8>(a, rows, splits, st) : launch_d<T, NNLIB_B200_E4M3>(a, rows, splits, st);
+}
+
+}  // namespace
+
+size_t cache_attn_workspace_bytes(const CacheAttnArgs& a, int dtype) {
+  const int n = split_count(a, dtype);
+  return n == 1 ? 0 : sizeof(float) * (size_t)split_ws_floats(reduce_args(a), n);
+}
+
+cudaError_t cache_attn(const CacheAttnArgs& a, int dtype, cudaStream_t st) {
+  const int n = split_count(a, dtype), rows = row_tile(a, dtype);
+  if (dtype == NNLIB_B200_F16) return launch_c<__half>(a, rows, n, st);
+  if (dtype == NNLIB_B200_BF16) return launch_c<__nv_bfloat16>(a, rows, n, st);
+  return launch_c<float>(a, rows, n, st);
+}
+
+}  // namespace nb200

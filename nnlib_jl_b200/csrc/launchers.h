@@ -95,4 +95,75 @@ cudaError_t softmax_forward(int dtype, bool log, const void* x, void* y, long lo
 cudaError_t softmax_backward(int dtype, bool log, const void* dy, const void* y, void* dx, long long inner, long long n,
                              long long outer, cudaStream_t st);
 
+// helpers of the C ABI (api.cu)
+int finish(cudaError_t e);                                // a return code, remembering what failed
+bool on_current_device(const void* ptr, int dev);         // NULL passes
+bool check_all_pointers();
+bool log_calls();
+
+// norm and rotation of heads (norm_rope.cu); a side is the queries or the keys
+struct NormRopeSide {
+  const void* x;
+  const void* dy;            // pullback: the cotangent
+  void* out;                 // forward: the result, pullback: the gradient of x; dense
+  const void* g;
+  void* dg;
+  long long sl, sb, dsl, dsb;
+  int heads;
+};
+struct NormRopeArgs {
+  NormRopeSide side[2];
+  const double* freqs;
+  const int* positions;
+  long long pos_sl, pos_sb;
+  const int* start;
+  long long start0;
+  long long tokens;          // L * B
+  float* ws;                 // pullback: d floats for each block
+  float eps;
+  int d, rot, L, interleaved, wdtype;
+  int lanes, tok, blocks_q;  // filled in by the launcher
+};
+size_t norm_rope_workspace_bytes(NormRopeArgs a, int esize);
+cudaError_t norm_rope(NormRopeArgs a, int dtype, bool bwd, cudaStream_t st);
+
+// 8-bit cache (cache.cu): what nnlib_b200_cache says, checked
+struct CacheArgs {
+  unsigned char* codes[2];   // keys, values
+  float* scale[2];
+  const int* table;
+  long long table_stride, pages, row;   // row: bytes of a token, d * H
+  long long rows;            // pages of a sequence
+  int code, d, H, B, log_page;
+};
+struct CacheTokens {
+  void* x[2];
+  long long sl[2], sb[2];
+  const int* start;
+  long long start0;
+  const int* count;
+  const int* lens;
+  int L;
+};
+cudaError_t cache_write(const CacheArgs& c, const CacheTokens& t, int dtype, cudaStream_t st);
+cudaError_t cache_read(const CacheArgs& c, const CacheTokens& t, int dtype, cudaStream_t st);
+
+// attention over it
+struct CacheAttnArgs {
+  CacheArgs c;
+  const void* q;
+  void* x;
+  long long q_sl, q_sb, x_sl, x_sb;
+  const int* lens;
+  const int* start;
+  long long len0;
+  float* lse;
+  float* ws;
+  int* status;
+  float scale;
+  int causal, nan_fm, Hq, L;
+};
+size_t cache_attn_workspace_bytes(const CacheAttnArgs& a, int dtype);   // (cache_attn.cu)
+cudaError_t cache_attn(const CacheAttnArgs& a, int dtype, cudaStream_t st);   // a.ws holds the workspace
+
 }  // namespace nb200

@@ -265,3 +265,103 @@ def test_decode_entry_and_new_fields_without_a_gpu(lib):
     assert lib.nnlib_b200_attn_path(C.byref(_params(dtype=_lib.F32, allow_tf32=1))) in (_lib.PATH_TILE, _lib.PATH_SIMT)
     assert lib.nnlib_b200_selftest_wait_runout(0, None, None) == _lib.INVALID_ARG
     assert lib.nnlib_b200_static_scratch(None, None) == _lib.INVALID_ARG
+
+
+def test_cache_and_norm_struct_layouts_match_the_header(tmp_path):
+    names = {"nnlib_b200_norm_rope_params": (_lib.NormRopeParams, ["q", "gq", "freqs", "positions_stride", "start0", "eps", "yq", "dyk_stride_b", "dgk"]),
+             "nnlib_b200_cache": (_lib.Cache, ["d", "pages", "k_codes", "B", "table", "rows"]),
+             "nnlib_b200_cache_tokens": (_lib.CacheTokens, ["L", "k", "v_stride_b", "start0", "count", "lens"]),
+             "nnlib_b200_cache_attn_params": (_lib.CacheAttnParams, ["Hq", "q", "x_stride_b", "lens", "len0", "start", "scale", "lse", "status"])}
+    body = "".join(f'printf("%zu\\n", sizeof({t}));' + "".join(f'printf("%zu\\n", offsetof({t}, {f}));' for f in fields)
+                   for t, (_, fields) in names.items())
+    src = tmp_path / "sz.c"
+    src.write_text('#include "nnlib_b200.h"\n#include <stdio.h>\n#include <stddef.h>\nint main(void){' + body + "return 0;}\n")
+    exe = tmp_path / "sz"
+    subprocess.run(["gcc", "-std=c99", "-I", str(ROOT / "include"), str(src), "-o", str(exe)], check=True)
+    got = [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    want = [n for t, fields in names.values() for n in [C.sizeof(t)] + [getattr(t, f).offset for f in fields]]
+    assert got == want
+
+
+def _norm_rope(**kw):
+    p = _lib.NormRopeParams(dtype=_lib.BF16, wdtype=_lib.BF16, d=64, rot=64, Hq=4, Hk=2, L=3, B=2, eps=1e-6)
+    for f in ("q", "k", "gq", "gk", "freqs", "yq", "yk", "dyq", "dyk", "dq", "dk", "dgq", "dgk"):
+        setattr(p, f, 0x1000)
+    for k, v in kw.items():
+        setattr(p, k, v)
+    return p
+
+
+def test_norm_rope_argument_checks_without_a_gpu(lib):
+    fwd = lambda **kw: lib.nnlib_b200_norm_rope(C.byref(_norm_rope(**kw)), None)
+    bwd = lambda ws=None, n=0, **kw: lib.nnlib_b200_norm_rope_bwd(C.byref(_norm_rope(**kw)), ws, n, None)
+    for bad in (dict(struct_size=8), dict(dtype=3), dict(wdtype=_lib.F16), dict(d=63), dict(d=0), dict(rot=66), dict(rot=3), dict(rot=-2),
+                dict(Hq=0, Hk=0), dict(Hq=-1), dict(L=-1), dict(q=None), dict(yk=None), dict(gq=None), dict(freqs=None),
+                dict(q=0x1001), dict(freqs=0x1004), dict(start=0x1002), dict(eps=-1.0), dict(eps=float("inf")), dict(eps=float("nan")),
+                dict(q_stride_l=100), dict(k_stride_b=-1), dict(start0=2 ** 40), dict(positions=0x1000, positions_stride=(C.c_int64 * 2)(-1, 0))):
+        assert fwd(**bad) == _lib.INVALID_ARG, bad
+        assert bwd(**bad) == _lib.INVALID_ARG or set(bad) <= {"yk"}, bad
+    for bad in (dict(dq=None), dict(dyk=None), dict(dgq=None), dict(dyq_stride_l=3)):
+        assert bwd(**bad) == _lib.INVALID_ARG, bad
+    assert fwd(d=258, rot=2) == _lib.UNSUPPORTED_SHAPE
+    assert lib.nnlib_b200_norm_rope(None, None) == _lib.INVALID_ARG
+    # one row of partial sums for each block: six tokens of queries and of keys
+    assert lib.nnlib_b200_norm_rope_bwd_workspace_bytes(C.byref(_norm_rope())) == 4 * 64 * 12
+    assert lib.nnlib_b200_norm_rope_bwd_workspace_bytes(C.byref(_norm_rope(d=63))) == 0
+    assert bwd(0x1000, 4 * 64 * 12 - 1) == _lib.WORKSPACE_TOO_SMALL and bwd(0x1008, 1 << 20) == _lib.WORKSPACE_TOO_SMALL
+    before = lib.nnlib_b200_launch_count()
+    assert fwd(L=0) == _lib.OK and fwd(B=0, q=None) == _lib.OK
+    assert lib.nnlib_b200_launch_count() == before
+
+
+def _cache(**kw):
+    c = _lib.Cache(code=_lib.INT8, d=64, H=2, page=32, pages=8, k_codes=0x1000, v_codes=0x1000, k_scale=0x1000, v_scale=0x1000, B=2, rows=4)
+    for k, v in kw.items():
+        setattr(c, k, v)
+    return c
+
+
+def _tokens(**kw):
+    t = _lib.CacheTokens(dtype=_lib.BF16, L=3, k=0x1000, v=0x1000)
+    for k, v in kw.items():
+        setattr(t, k, v)
+    return t
+
+
+def _cache_attn(**kw):
+    p = _lib.CacheAttnParams(dtype=_lib.BF16, causal=1, Hq=4, L=1, q=0x1000, x=0x1000, len0=100)
+    for k, v in kw.items():
+        setattr(p, k, v)
+    return p
+
+
+def test_cache_argument_checks_without_a_gpu(lib):
+    def calls(c, t=None, p=None):
+        t, p = C.byref(t or _tokens()), C.byref(p or _cache_attn())
+        return (lib.nnlib_b200_cache_write(C.byref(c), t, None), lib.nnlib_b200_cache_read(C.byref(c), t, None),
+                lib.nnlib_b200_cache_attn(C.byref(c), p, None, 0, None))
+    for bad in (dict(struct_size=8), dict(code=2), dict(d=0), dict(H=0), dict(page=8), dict(page=48), dict(page=512), dict(pages=-1),
+                dict(rows=-1), dict(B=-1), dict(rows=5), dict(table=0x1000, table_stride=3), dict(table=0x1002), dict(k_codes=None),
+                dict(v_scale=None), dict(k_codes=0x1008), dict(k_scale=0x1002), dict(B=65536, table=0x1000), dict(H=32768),
+                dict(table=0x1000, rows=2 ** 27), dict(table_stride=-1)):
+        assert calls(_cache(**bad)) == (_lib.INVALID_ARG,) * 3, bad
+    for bad in (dict(d=24), dict(d=272)):
+        assert calls(_cache(**bad)) == (_lib.UNSUPPORTED_SHAPE,) * 3, bad
+    for bad in (dict(struct_size=8), dict(dtype=5), dict(L=-1), dict(k=None), dict(v=None), dict(k=0x1001), dict(start=0x1001), dict(count=0x1002),
+                dict(lens=0x1003), dict(k_stride_l=127), dict(v_stride_b=-1), dict(start0=2 ** 40)):
+        assert calls(_cache(), t=_tokens(**bad))[:2] == (_lib.INVALID_ARG,) * 2, bad
+    for bad in (dict(struct_size=8), dict(dtype=5), dict(Hq=3), dict(Hq=0), dict(L=-1), dict(q=None), dict(x=None), dict(q=0x1001),
+                dict(lens=0x1002), dict(lse=0x1002), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(q_stride_l=255),
+                dict(x_stride_b=-1), dict(L=2 ** 30)):
+        assert calls(_cache(), p=_cache_attn(**bad))[2] == _lib.INVALID_ARG, bad
+    assert lib.nnlib_b200_cache_write(None, C.byref(_tokens()), None) == _lib.INVALID_ARG
+    assert lib.nnlib_b200_cache_read(C.byref(_cache()), None, None) == _lib.INVALID_ARG
+    assert lib.nnlib_b200_cache_attn(C.byref(_cache()), None, None, 0, None) == _lib.INVALID_ARG
+    assert lib.nnlib_b200_cache_attn_workspace_bytes(None, C.byref(_cache_attn())) == 0
+    # nothing to do
+    before = lib.nnlib_b200_launch_count()
+    assert calls(_cache(B=0)) == (_lib.OK,) * 3
+    assert calls(_cache(), _tokens(L=0), _cache_attn(L=0)) == (_lib.OK,) * 3
+    assert lib.nnlib_b200_cache_write(C.byref(_cache(rows=0, pages=0, k_codes=None, v_codes=None, k_scale=None, v_scale=None)),
+                                      C.byref(_tokens(L=0)), None) == _lib.OK
+    assert lib.nnlib_b200_launch_count() == before
