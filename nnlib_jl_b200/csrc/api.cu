@@ -656,7 +656,7 @@ int nnlib_b200_attn_path(const nnlib_b200_attn_params* p) {
 }
 
 int nnlib_b200_device_health(void* stream) {
-  int v = 0, w = 0, u = 0, t = 0, s = 0, f = 0;
+  int v = 0, w = 0, u = 0, t = 0, s = 0, f = 0, c = 0;
   cudaError_t e = short_take_abort(&s, (cudaStream_t)stream);
   v = 0;
   if (e == cudaSuccess) e = umma_take_abort(&v, (cudaStream_t)stream);
@@ -664,8 +664,9 @@ int nnlib_b200_device_health(void* stream) {
   if (e == cudaSuccess) e = umma_bwd_fused_take_abort(&f, (cudaStream_t)stream);
   if (e == cudaSuccess) e = gemm_take_abort(&u, (cudaStream_t)stream);
   if (e == cudaSuccess) e = tile_take_abort(&t, (cudaStream_t)stream);
+  if (e == cudaSuccess) e = cache_umma_take_abort(&c, (cudaStream_t)stream);
   if (e != cudaSuccess) return finish(e);
-  return (v || w || u || t || s || f) ? NNLIB_B200_TIMEOUT : NNLIB_B200_OK;
+  return (v || w || u || t || s || f || c) ? NNLIB_B200_TIMEOUT : NNLIB_B200_OK;
 }
 
 int nnlib_b200_selftest_wait_runout(uint64_t limit_ns, int32_t* status, void* stream) {

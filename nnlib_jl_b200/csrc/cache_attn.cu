@@ -34,6 +34,7 @@ constexpr int kStep = 16;                 // keys a warp takes at a time
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kValueFloor = 7.8886090522101181e-31f;    // 2^-100
 constexpr float kWeightBits = 14.f;
+constexpr int kUmmaRows = 48;
 
 __device__ __forceinline__ float ninf() { return __int_as_float(0xff800000); }
 __device__ __forceinline__ float qnan() { return __int_as_float(0x7fc00000); }
@@ -417,6 +418,19 @@ AttnArgs reduce_args(const CacheAttnArgs& a) {
   return r;
 }
 
+// Many rows go to the tensor cores.
+bool use_umma(const CacheAttnArgs& a, int dtype) {
+  return cache_umma_supports(a, dtype) && (long long)a.L * (a.Hq / a.c.H) > kUmmaRows;
+}
+
+template <typename T>
+cudaError_t reduce(const CacheAttnArgs& a, int splits, cudaStream_t st) {
+  const AttnArgs r = reduce_args(a);
+  attn_split_reduce_kernel<T, false><<<(unsigned)((long long)a.Hq * a.c.B * a.L), 128, 0, st>>>(r, splits);
+  count_launch();
+  return cudaGetLastError();
+}
+
 template <typename T, int D, int CODE, bool ROWS8>
 cudaError_t launch(const CacheAttnArgs& a, int splits, cudaStream_t st) {
   const long long rows = (long long)a.L * (a.Hq / a.c.H), tile = ROWS8 ? 8 : 16;
@@ -424,12 +438,8 @@ cudaError_t launch(const CacheAttnArgs& a, int splits, cudaStream_t st) {
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
   cache_attn_kernel<T, D, CODE, ROWS8><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a, splits);
   count_launch();
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || splits == 1) return e;
-  const AttnArgs r = reduce_args(a);
-  attn_split_reduce_kernel<T, false><<<(unsigned)((long long)a.Hq * a.c.B * a.L), 128, 0, st>>>(r, splits);
-  count_launch();
-  return cudaGetLastError();
+  const cudaError_t e = cudaGetLastError();
+  return e != cudaSuccess || splits == 1 ? e : reduce<T>(a, splits, st);
 }
 
 template <typename T, int CODE>
@@ -449,11 +459,17 @@ cudaError_t launch_c(const CacheAttnArgs& a, int rows, int splits, cudaStream_t 
 }  // namespace
 
 size_t cache_attn_workspace_bytes(const CacheAttnArgs& a, int dtype) {
-  const int n = split_count(a, dtype);
+  const int n = use_umma(a, dtype) ? cache_umma_splits(a) : split_count(a, dtype);
   return n == 1 ? 0 : sizeof(float) * (size_t)split_ws_floats(reduce_args(a), n);
 }
 
 cudaError_t cache_attn(const CacheAttnArgs& a, int dtype, cudaStream_t st) {
+  if (use_umma(a, dtype)) {
+    const int n = cache_umma_splits(a);
+    const cudaError_t e = cache_umma(a, dtype, n, st);
+    if (e != cudaSuccess || n == 1) return e;
+    return dtype == NNLIB_B200_F16 ? reduce<__half>(a, n, st) : reduce<__nv_bfloat16>(a, n, st);
+  }
   const int n = split_count(a, dtype), rows = row_tile(a, dtype);
   if (dtype == NNLIB_B200_F16) return launch_c<__half>(a, rows, n, st);
   if (dtype == NNLIB_B200_BF16) return launch_c<__nv_bfloat16>(a, rows, n, st);

@@ -1,0 +1,617 @@
+// Attention over the 8-bit cache on the tensor cores: many queries at a time (parts of prompts, prompts).
+//
+// The arithmetic is that of cache_attn.cu: products of codes, which Float16 holds exactly, with the page's key scale on the
+// logits and its value scale in the exponent.  Here the products are tcgen05.mma: a block owns 256 rows (two tiles of 128) of
+// one sequence and cache head, row = query * G + head of the group, so that query heads that share keys share their tiles,
+// and walks over the keys in tiles of 128:
+//
+//   warp 0       pages and scales of the next tiles, into shared memory
+//   warp 1       issues every tcgen05.mma:  S_t = Q_t K_j^T (smem x smem -> TMEM),  O_t += W_t V_j (TMEM x smem -> TMEM)
+//   warp 2       allocates / frees the 512 TMEM columns
+//   warps 4-11   softmax of the two tiles (a thread owns a row), before that Q: rounded to Float16 after a power of two of
+//                the row's own, after that x
+//   warps 12-15  codes to Float16: K by two warps, V by two, from global memory through registers into the 128-byte
+//                swizzled tiles the products read; both operands have a key's features in a row, so the code is the same
+//
+// Bound by the tensor pipe and the softmax warps' issue slots, like the forward kernel for 16-bit arrays.  A conversion is
+// five instructions for four codes (Int8), 32768 codes a round, some 450 issue slots of each scheduler's 3100, which is why
+// it has warps of its own: the loads of a warp's next batch are under way while it converts one.  The copy engine could
+// bring codes only, which would cost another pass through shared memory.
+// A scale serves 16 keys at least (64 where the pages allow: SG), so a thread scales and sums by groups of SG keys.
+// Weights leave with a factor of 2^10 and the running maximum is raised when it grew by more than 2^4: they are below 2^14
+// and keep 11 bits down to 2^-24 of the largest.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "cache_codes.cuh"
+#include "split_reduce.cuh"
+#include "umma_shared.cuh"
+
+namespace nb200 {
+
+__device__ int g_cache_attn_abort = 0;   // sticky: a bounded wait ran out somewhere
+
+namespace {
+
+constexpr int kThreadsC = 512, kTiles = 2;
+constexpr float kGap = 4.f, kBits = 10.f;
+constexpr float kValueFloorU = 7.8886090522101181e-31f;   // 2^-100
+constexpr int kMetaTiles = 8;
+
+struct __align__(16) PageMeta {
+  float ks, lvs, ivs;     // key scale; log2(value scale) + kBits; 1 / value scale
+  int page;               // -1: no tokens here
+};
+
+template <int D>
+struct CfgC {
+  static constexpr int kChunks = D / 64;
+  static constexpr int kTileBytes = kChunks * kChunkBytes;
+  static constexpr int kStagesK = D == 128 ? 2 : 4, kStagesV = D == 128 ? 3 : 4;
+  static constexpr int kKOff = kTiles * kTileBytes, kVOff = kKOff + kStagesK * kTileBytes;
+  static constexpr int kMetaOff = kVOff + kStagesV * kTileBytes;
+  static constexpr int kBarOff = kMetaOff + kMetaTiles * 8 * (int)sizeof(PageMeta);
+  static constexpr int kSmemBytes = kBarOff + 256 + 1024;
+};
+static_assert(CfgC<128>::kSmemBytes <= 232448, "shared memory budget");
+
+struct BarsC {
+  uint64_t q_full[kTiles], s_full[kTiles], p_half[kTiles][2], o_full[kTiles];
+  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
+  uint64_t meta_full[2], meta_free[2];     // four tiles each
+  uint32_t tmem_base;
+  int abort_flag;
+};
+static_assert(sizeof(BarsC) <= 256, "barrier block");
+
+template <int CODE>
+__device__ __forceinline__ void codes4(uint32_t w, uint32_t& p0, uint32_t& p1) {
+  if (CODE == NNLIB_B200_INT8) {
+    const uint32_t u = w ^ 0x80808080u;
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(p0) : "r"(__byte_perm(u, 0x64646464u, 0x4140u)), "r"(0x64806480u));
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(p1) : "r"(__byte_perm(u, 0x64646464u, 0x4342u)), "r"(0x64806480u));
+  } else {
+    asm("{ .reg .b16 lo, hi; mov.b32 {lo, hi}, %2; cvt.rn.f16x2.e4m3x2 %0, lo; cvt.rn.f16x2.e4m3x2 %1, hi; }"
+        : "=r"(p0), "=r"(p1) : "r"(w));
+  }
+}
+
+// One side's tiles: keys 128 (j_lo + j) .. of sequence b, head h, into the ring at `ring`.  Two warps, each one chunk of 64
+// features (D = 128) or one half of the keys (D = 64); lane = (key of eight, piece of 16 features of four), which puts the
+// stores of eight lanes, two neighbouring keys, on all banks.
+template <int D, int CODE, int STAGES>
+__device__ __forceinline__ void convert_tiles(const CacheArgs& cc, const unsigned char* base, uint8_t* ring, const PageMeta* meta,
+                                              uint64_t* full, uint64_t* empty, uint64_t* meta_full, volatile int* abort_flag,
+                                              int w, int lane, int j_lo, int n_kv, int len) {
+  constexpr int N = D == 128 ? 16 : 8, BATCH = 4, NB = N / BATCH;
+  constexpr int kTileBytes = CfgC<D>::kTileBytes;
+  const int key8 = lane >> 2, piece = lane & 3;
+  const int feat = (D == 128 ? w * 64 : 0) + piece * 16;
+  const int n0 = D == 128 ? 0 : w * 8;
+  const bool feat_ok = feat < cc.d;
+  uint8_t* out = ring + (D == 128 ? w * kChunkBytes : 0) + n0 * 1024 + key8 * 128;
+  const int u0 = ((2 * piece) ^ key8) << 4, u1 = ((2 * piece + 1) ^ key8) << 4;
+  const int T1 = (1 << cc.log_page) - 1;
+  base += feat;
+  uint4 raw[2][BATCH];
+  auto load = [&](uint4 (&r)[BATCH], int j, int bt) {
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int n = n0 + bt * BATCH + i, key = (j_lo + j) * kBN + n * 8 + key8;
+      r[i] = make_uint4(0u, 0u, 0u, 0u);
+      const int page = meta[(j & (kMetaTiles - 1)) * 8 + (n >> 1)].page;
+      if (feat_ok && key < len && page >= 0)
+        r[i] = __ldg(reinterpret_cast<const uint4*>(base + (((long long)page << cc.log_page) + (key & T1)) * cc.row));
+    }
+  };
+  bool ok = n_kv > 0 && mbar_wait_warp(&meta_full[0], 0, abort_flag);
+  if (ok) load(raw[0], 0, 0);
+  for (int j = 0; j < n_kv && ok; ++j) {
+    const int s = j % STAGES;
+#pragma unroll
+    for (int bt = 0; bt < NB; ++bt) {
+      // the next batch, of this tile or the next one
+      if (bt + 1 < NB) {
+        load(raw[(bt + 1) & 1], j, bt + 1);
+      } else if (j + 1 < n_kv) {
+        const int jn = j + 1;
+        if ((jn & 3) == 0) ok = mbar_wait_warp(&meta_full[(jn >> 2) & 1], (jn >> 3) & 1, abort_flag);
+        if (!ok) break;
+        load(raw[(bt + 1) & 1], jn, 0);
+      }
+      if (bt == 0 && j >= STAGES) {
+        ok = mbar_wait_warp(&empty[s], ((j / STAGES) - 1) & 1, abort_flag);
+        if (!ok) break;
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const uint4 r = raw[bt & 1][i];
+        uint4 a, b;
+        codes4<CODE>(r.x, a.x, a.y);
+        codes4<CODE>(r.y, a.z, a.w);
+        codes4<CODE>(r.z, b.x, b.y);
+        codes4<CODE>(r.w, b.z, b.w);
+        uint8_t* p = out + s * kTileBytes + (bt * BATCH + i) * 1024;
+        *reinterpret_cast<uint4*>(p + u0) = a;
+        *reinterpret_cast<uint4*>(p + u1) = b;
+      }
+    }
+    if (!ok) break;
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&full[s]);
+  }
+}
+
+// SG: keys that certainly share a scale
+template <typename T, int D, int CODE, int SG>
+__global__ void __launch_bounds__(kThreadsC, 1) cache_attn_umma_kernel(const CacheAttnArgs a, const int splits, const int vec) {
+  using C = CfgC<D>;
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  BarsC* bars = reinterpret_cast<BarsC*>(smem + C::kBarOff);
+  PageMeta* meta = reinterpret_cast<PageMeta*>(smem + C::kMetaOff);
+  volatile int* abort_flag = &bars->abort_flag;
+  const CacheArgs& cc = a.c;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = a.Hq / cc.H, rows = a.L * G, blocks = (rows + kTiles * kBM - 1) / (kTiles * kBM);
+  // the longest blocks of all units first; heads of a sequence side by side
+  int item = blockIdx.x;
+  const int h = item % cc.H;
+  item /= cc.H;
+  const int b = item % cc.B;
+  item /= cc.B;
+  const int split = item % splits, row0 = (blocks - 1 - item / splits) * (kTiles * kBM);
+
+  const long long cap = cc.rows << cc.log_page;
+  const long long n_len = a.lens ? (long long)a.lens[b] : a.len0;
+  const int len = (int)(n_len < 0 ? 0 : (n_len < cap ? n_len : cap));
+  const long long start = a.start ? (long long)a.start[b] : (long long)len - a.L;
+  auto last_key = [&](int row) {      // the last key that a row sees, -1: none
+    if (row >= rows) return -1;
+    if (!a.causal) return len - 1;
+    const long long e = start + row / G;
+    return e < 0 ? -1 : (e < len ? (int)e : len - 1);
+  };
+  // this block's key tiles, and where each of its row tiles stops
+  int n_t[kTiles], j_lo;
+  {
+    int most = 0, n[kTiles];
+    for (int t = 0; t < kTiles; ++t) {
+      const int lo = row0 + t * kBM;
+      n[t] = lo < rows ? (last_key(min(lo + kBM, rows) - 1) + kBN) / kBN : 0;
+      most = max(most, n[t]);
+    }
+    const int share = (most + splits - 1) / splits;
+    j_lo = split * share;
+    for (int t = 0; t < kTiles; ++t) n_t[t] = max(0, min(n[t], j_lo + share) - j_lo);
+  }
+  const int n_kv = max(n_t[0], n_t[1]);
+
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < kTiles; ++t) {
+      mbar_init(&bars->q_full[t], 4);
+      mbar_init(&bars->s_full[t], 1);
+      mbar_init(&bars->p_half[t][0], 4);
+      mbar_init(&bars->p_half[t][1], 4);
+      mbar_init(&bars->o_full[t], 1);
+      mbar_init(&bars->meta_full[t], 1);
+      mbar_init(&bars->meta_free[t], 1);
+    }
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(&bars->k_full[s], 2);
+      mbar_init(&bars->k_empty[s], 1);
+      mbar_init(&bars->v_full[s], 2);
+      mbar_init(&bars->v_empty[s], 1);
+    }
+    bars->abort_flag = *reinterpret_cast<volatile int*>(&g_cache_attn_abort);
+    fence_mbar_init();
+  }
+  if (warp == 2) {
+    tmem_alloc(&bars->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  const bool start_ok = (*abort_flag == 0);
+
+  // registers: 128 x 40 + 256 x 208 + 128 x 56 = the 512 x 128 launched
+  if (warp < 4) {
+    setmaxnreg_dec<40>();
+    if (start_ok && warp == 0) {
+      // ---------------------------------------------------- pages and scales, four tiles at a time
+      bool ok = true;
+      for (int q = 0; 4 * q < n_kv && ok; ++q) {
+        if (q >= 2) ok = mbar_wait_warp(&bars->meta_free[q & 1], ((q >> 1) - 1) & 1, abort_flag);
+        if (!ok) break;
+        const int j = 4 * q + (lane >> 3);
+        const long long key = (long long)(j_lo + j) * kBN + (lane & 7) * 16;
+        PageMeta m = {1.f, 0.f, 0.f, -1};
+        if (key < len) {
+          const long long page = cache_page(cc, b, key >> cc.log_page);
+          float ks = __int_as_float(0x7fc00000), vs = ks;
+          if (page >= 0) {
+            ks = cc.scale[0][page * cc.H + h];
+            vs = cc.scale[1][page * cc.H + h];
+          }
+          const float vse = vs >= kValueFloorU ? vs : (vs >= 0.f ? kValueFloorU : __int_as_float(0x7fc00000));
+          m.ks = ks >= 0.f ? ks : __int_as_float(0x7fc00000);
+          m.lvs = log2f(vse) + kBits;
+          m.ivs = __fdiv_rn(1.f, vse);
+          m.page = (int)page;
+        }
+        meta[(j & (kMetaTiles - 1)) * 8 + (lane & 7)] = m;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->meta_full[q & 1]);
+      }
+    } else if (start_ok && warp == 1 && lane == 0 && n_kv > 0) {
+      // ---------------------------------------------------- MMA issuer (descriptors as in attn_umma.cu)
+      constexpr uint32_t idesc_qk = make_idesc_f16(false, kBM, kBN, false, false);
+      constexpr uint32_t idesc_pv = make_idesc_f16(false, kBM, D, false, true);
+      constexpr uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+      constexpr uint32_t lbo_k = (16u >> 4) << 16, lbo_v = (static_cast<uint32_t>(kChunkBytes) >> 4) << 16;
+      constexpr uint32_t tile16 = C::kTileBytes >> 4;
+      const uint32_t q_lo = (smem_u32(smem) >> 4) | lbo_k;
+      const uint32_t k_lo = (smem_u32(smem + C::kKOff) >> 4) | lbo_k;
+      const uint32_t v_lo = (smem_u32(smem + C::kVOff) >> 4) | lbo_v;
+      auto issue_qk = [&](int t, int stage) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * (kChunkBytes >> 4) + (kk & 3) * 2;
+          umma_ss_lohi(tmem + t * kBN, q_lo + t * tile16 + off, k_lo + stage * tile16 + off, desc_hi, idesc_qk, kk > 0 ? 1u : 0u);
+        }
+      };
+      auto issue_pv = [&](int t, int stage, int half, bool first) {
+#pragma unroll
+        for (int kk = 0; kk < kBN / 32; ++kk) {
+          const int k = half * (kBN / 32) + kk;
+          umma_ts_lohi(tmem + kTiles * kBN + t * D, tmem + t * kBN + k * 8, v_lo + stage * tile16 + k * (2048 >> 4), desc_hi,
+                       idesc_pv, (first && k == 0) ? 0u : 1u);
+        }
+      };
+      bool ok = true;
+      for (int t = 0; t < kTiles; ++t)
+        if (ok && n_t[t] > 0) ok = mbar_wait(&bars->q_full[t], 0, abort_flag);
+      if (ok) ok = mbar_wait(&bars->k_full[0], 0, abort_flag);
+      if (ok) {
+        tc_fence_after();
+        for (int t = 0; t < kTiles; ++t)
+          if (n_t[t] > 0) {
+            issue_qk(t, 0);
+            umma_commit(&bars->s_full[t]);
+          }
+        umma_commit(&bars->k_empty[0]);
+      }
+      for (int j = 0; j < n_kv && ok; ++j) {
+        const int sv = j % C::kStagesV, sk = (j + 1) % C::kStagesK;
+        const uint32_t par = j & 1;
+        ok = mbar_wait(&bars->v_full[sv], (j / C::kStagesV) & 1, abort_flag);
+        if (ok && j + 1 < n_kv) ok = mbar_wait(&bars->k_full[sk], ((j + 1) / C::kStagesK) & 1, abort_flag);
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+          const int nt = t == 0 ? n_t[0] : n_t[1];
+          if (!ok || j >= nt) continue;
+          ok = mbar_wait(&bars->p_half[t][0], par, abort_flag);
+          if (!ok) continue;
+          tc_fence_after();
+          issue_pv(t, sv, 0, j == 0);
+          ok = mbar_wait(&bars->p_half[t][1], par, abort_flag);
+          if (!ok) continue;
+          tc_fence_after();
+          issue_pv(t, sv, 1, false);
+          if (j + 1 < nt) {
+            issue_qk(t, sk);
+            umma_commit(&bars->s_full[t]);
+          } else {
+            umma_commit(&bars->o_full[t]);
+          }
+        }
+        if (!ok) break;
+        umma_commit(&bars->v_empty[sv]);
+        if (j + 1 < n_kv) umma_commit(&bars->k_empty[sk]);
+        // everything of tiles up to j is done with: the pages and scales of j - 3 .. j may go
+        if ((j & 3) == 3) umma_commit(&bars->meta_free[(j >> 2) & 1]);
+      }
+    }
+  } else if (warp >= 12) {
+    setmaxnreg_dec<56>();
+    if (start_ok) {
+      const int w = (warp - 12) & 1;
+      if (warp < 14)
+        convert_tiles<D, CODE, C::kStagesK>(cc, cc.codes[0] + (long long)h * cc.d, smem + C::kKOff, meta, bars->k_full,
+                                            bars->k_empty, bars->meta_full, abort_flag, w, lane, j_lo, n_kv, len);
+      else
+        convert_tiles<D, CODE, C::kStagesV>(cc, cc.codes[1] + (long long)h * cc.d, smem + C::kVOff, meta, bars->v_full,
+                                            bars->v_empty, bars->meta_full, abort_flag, w, lane, j_lo, n_kv, len);
+    }
+  } else {
+    setmaxnreg_inc<208>();
+    const int t = (warp - 4) >> 2, nt = t == 0 ? n_t[0] : n_t[1];
+    const int wq = warp & 3, r = wq * 32 + lane, row = row0 + t * kBM + r;
+    const bool row_ok = row < rows;
+    const int i = row_ok ? row / G : 0, hq = h * G + (row_ok ? row % G : 0);
+    if (start_ok && row0 + t * kBM < rows) {
+      const uint32_t lane_base = tmem + (static_cast<uint32_t>(wq * 32) << 16);
+      const uint32_t tS = lane_base + t * kBN, tO = lane_base + kTiles * kBN + t * D;
+      const int lim = last_key(row);
+      float crow = 0.f;
+      if (nt > 0) {
+        // ------------------------------------------------ this row of Q, by a power of two to a largest element in [2^13, 2^14)
+        const T* qp = reinterpret_cast<const T*>(a.q) + (long long)i * a.q_sl + (long long)b * a.q_sb + (long long)hq * cc.d;
+        auto load8 = [&](int f, float (&v)[8]) {
+          T e[8];
+          if (vec) {
+            const uint4 raw = __ldg(reinterpret_cast<const uint4*>(qp + f));
+            memcpy(e, &raw, 16);
+          } else {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) e[u] = qp[f + u];
+          }
+#pragma unroll
+          for (int u = 0; u < 8; ++u) v[u] = Elem<T>::to_f(e[u]);
+        };
+        float top = 0.f;
+#pragma unroll
+        for (int f = 0; f < D; f += 8)
+          if (row_ok && f < cc.d) {
+            float v[8];
+            load8(f, v);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) top = fmaxf(top, fabsf(v[u]));
+          }
+        const int ex = (top > 0.f && top <= 3.402823466e38f) ? 13 - ilogbf(top) : 0;
+        crow = scalbnf(a.scale * kLog2e, -ex);
+        uint8_t* qrow = smem + t * C::kTileBytes + r * 128;
+#pragma unroll
+        for (int f = 0; f < D; f += 8) {
+          uint4 p = make_uint4(0u, 0u, 0u, 0u);
+          if (row_ok && f < cc.d) {
+            float v[8];
+            load8(f, v);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = scalbnf(v[u], ex);
+            p = make_uint4(pack2<false>(v[0], v[1]), pack2<false>(v[2], v[3]), pack2<false>(v[4], v[5]), pack2<false>(v[6], v[7]));
+          }
+          *reinterpret_cast<uint4*>(qrow + (f / 64) * kChunkBytes + ((((f / 8) & 7) ^ (r & 7)) << 4)) = p;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->q_full[t]);
+      }
+
+      float m_used = neg_inf(), l = 0.f;
+      bool ok = true;
+      for (int j = 0; j < nt; ++j) {
+        if ((j & 3) == 0) ok = mbar_wait_warp(&bars->meta_full[(j >> 2) & 1], (j >> 3) & 1, abort_flag);
+        if (!ok) break;
+        // scales: a group of SG keys has factor fg, offset cg
+        constexpr int NG = kBN / SG;
+        const PageMeta* pm = meta + (j & (kMetaTiles - 1)) * 8;
+        float fg[NG], cg[NG];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          fg[g] = crow * pm[g * (SG / 16)].ks;
+          cg[g] = pm[g * (SG / 16)].lvs;
+        }
+        ok = mbar_wait(&bars->s_full[t], j & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t sr[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, sr[c]);
+        tmem_wait_ld();
+        const int j0 = (j_lo + j) * kBN;
+        if (__any_sync(0xffffffffu, j0 + kBN - 1 > lim)) {
+          // the scaled logits themselves, -Inf where the row does not look
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const int g = (c * 32 + e) / SG;
+              const float v = fmaf(__uint_as_float(sr[c][e]), fg[g], cg[g]);
+              sr[c][e] = j0 + c * 32 + e > lim ? 0xff800000u : __float_as_uint(v);
+            }
+#pragma unroll
+          for (int g = 0; g < NG; ++g) fg[g] = 1.f, cg[g] = 0.f;
+        }
+
+        uint32_t pk[32];
+        float sums[NG];
+        // weights of 64 keys relative to REF
+        auto weights = [&](int hf, float ref) {
+#pragma unroll
+          for (int gg = 0; gg < 64 / SG; ++gg) {
+            const int g = hf * (64 / SG) + gg;
+            const unsigned long long f2 = pair_of(fg[g]), c2 = pair_of(cg[g] - ref);
+            unsigned long long s2[2] = {0ull, 0ull};
+#pragma unroll
+            for (int e = 0; e < SG; e += 2) {
+              const int at = gg * SG + e, c = hf * 2 + at / 32;
+              float x0, x1;
+              fma2(x0, x1, __uint_as_float(sr[c][at & 31]), __uint_as_float(sr[c][(at & 31) + 1]), f2, c2);
+              x0 = ex2_approx(x0);
+              x1 = ex2_approx(x1);
+              add2(s2[(e >> 1) & 1], x0, x1);
+              pk[at >> 1] = pack2<false>(x0, x1);
+            }
+            sums[g] = pair_sum(s2[0]) + pair_sum(s2[1]);
+          }
+        };
+        float mx = neg_inf();
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          float m0 = neg_inf(), m1 = neg_inf();
+#pragma unroll
+          for (int e = 0; e < SG; e += 4) {
+            const int c = (g * SG + e) / 32, at = (g * SG + e) & 31;
+            m0 = max3(m0, __uint_as_float(sr[c][at]), __uint_as_float(sr[c][at + 1]));
+            m1 = max3(m1, __uint_as_float(sr[c][at + 2]), __uint_as_float(sr[c][at + 3]));
+          }
+          mx = fmaxf(mx, fmaf(fmaxf(m0, m1), fg[g], cg[g]));
+        }
+        const float m_new = fmaxf(m_used, mx - kBits);
+        const bool raise = m_new > m_used + kGap;      // also true for m_used = -Inf < m_new
+        // the first half against the running reference while the maximum is being found; redone where that moves it
+        const bool guess = j > 0;
+        if (guess) weights(0, m_used == neg_inf() ? 0.f : m_used);
+        if (!guess || __any_sync(0xffffffffu, raise)) {
+          if (j > 0) {
+            const float f = raise ? ex2_approx(m_used - m_new) : 1.f;
+            l *= f;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32(tO + c * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st32(tO + c * 32, o);
+            }
+          }
+          if (raise) m_used = m_new;
+          weights(0, m_used == neg_inf() ? 0.f : m_used);
+        }
+        const float ref = m_used == neg_inf() ? 0.f : m_used;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          if (hf == 1) weights(1, ref);
+          tmem_st32(tS + hf * 32, pk);
+          // a page that the row does not see adds nothing, whatever its scale is
+#pragma unroll
+          for (int g = hf * NG / 2; g < (hf + 1) * NG / 2; ++g)
+            if (!(sums[g] == 0.f)) l = fmaf(sums[g], pm[g * (SG / 16)].ivs, l);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->p_half[t][hf]);
+        }
+      }
+
+      // -------------------------------------------------- epilogue
+      if (ok && nt > 0) {
+        ok = mbar_wait(&bars->o_full[t], 0, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+      }
+      if (ok) {
+        tc_fence_after();
+        const bool dead = l == 0.f;
+        const long long unit = hq + (long long)a.Hq * b, at = (unit * splits + split) * a.L + i;
+        float* wrow = nullptr;
+        T* xrow = nullptr;
+        float inv = 1.f;
+        if (splits > 1) {
+          wrow = a.ws + ((((long long)a.Hq * cc.B * splits * a.L * 2) + 3) & ~3LL) + at * cc.d;
+          if (row_ok) {
+            a.ws[at * 2] = m_used - kBits;              // (l has that factor)
+            a.ws[at * 2 + 1] = l;
+          }
+        } else {
+          xrow = reinterpret_cast<T*>(a.x) + (long long)i * a.x_sl + (long long)b * a.x_sb + (long long)hq * cc.d;
+          inv = dead ? (a.nan_fm ? __int_as_float(0x7fc00000) : 0.f) : 1.f / l;
+          if (row_ok && a.lse) a.lse[i + (long long)a.L * unit] = dead ? neg_inf() : (m_used - kBits + log2f(l)) * kLn2;
+        }
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          if (nt > 0) {
+            tmem_ld32(tO + c * 32, o);
+            tmem_wait_ld();
+          }
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            if (!row_ok || c * 32 + e >= cc.d) continue;
+            float f[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) f[u] = dead ? (splits > 1 ? 0.f : inv) : __uint_as_float(o[e + u]) * inv;
+            if (splits > 1) {
+              *reinterpret_cast<float4*>(wrow + c * 32 + e) = make_float4(f[0], f[1], f[2], f[3]);
+              *reinterpret_cast<float4*>(wrow + c * 32 + e + 4) = make_float4(f[4], f[5], f[6], f[7]);
+            } else if (vec) {
+              *reinterpret_cast<uint4*>(xrow + c * 32 + e) =
+                  make_uint4(pack2<BF16>(f[0], f[1]), pack2<BF16>(f[2], f[3]), pack2<BF16>(f[4], f[5]), pack2<BF16>(f[6], f[7]));
+            } else {
+#pragma unroll
+              for (int u = 0; u < 8; ++u) xrow[c * 32 + e + u] = Elem<T>::from_f(f[u]);
+            }
+          }
+        }
+      }
+    }
+  }
+
+  // ---------------------------------------------------------------- teardown
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+  if (threadIdx.x == 0 && *abort_flag) {
+    atomicExch(&g_cache_attn_abort, 1);
+    if (a.status) atomicExch(a.status, NNLIB_B200_TIMEOUT);
+  }
+}
+
+template <typename T, int D, int CODE, int SG>
+cudaError_t launch(const CacheAttnArgs& a, int splits, cudaStream_t st) {
+  const long long rows = (long long)a.L * (a.Hq / a.c.H);
+  const long long blocks = (rows + kTiles * kBM - 1) / (kTiles * kBM) * a.c.B * a.c.H * splits;
+  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const bool vec = aligned16(a.q) && aligned16(a.x) && a.q_sl % 8 == 0 && a.q_sb % 8 == 0 && a.x_sl % 8 == 0 && a.x_sb % 8 == 0;
+  auto kernel = cache_attn_umma_kernel<T, D, CODE, SG>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, CfgC<D>::kSmemBytes);
+  if (e != cudaSuccess) return e;
+  kernel<<<(unsigned)blocks, kThreadsC, CfgC<D>::kSmemBytes, st>>>(a, splits, vec ? 1 : 0);
+  count_launch();
+  return cudaGetLastError();
+}
+
+template <typename T, int CODE>
+cudaError_t launch_d(const CacheAttnArgs& a, int splits, cudaStream_t st) {
+  if (a.c.log_page >= 6) return a.c.d <= 64 ? launch<T, 64, CODE, 64>(a, splits, st) : launch<T, 128, CODE, 64>(a, splits, st);
+  return a.c.d <= 64 ? launch<T, 64, CODE, 16>(a, splits, st) : launch<T, 128, CODE, 16>(a, splits, st);
+}
+
+template <typename T>
+cudaError_t launch_c(const CacheAttnArgs& a, int splits, cudaStream_t st) {
+  return a.c.code == NNLIB_B200_INT8 ? launch_d<T, NNLIB_B200_INT8>(a, splits, st) : launch_d<T, NNLIB_B200_E4M3>(a, splits, st);
+}
+
+}  // namespace
+
+bool cache_umma_supports(const CacheAttnArgs& a, int dtype) { return dtype != NNLIB_B200_F32 && a.c.d <= 128; }
+
+// Blocks of keys of a unit: where there are too few blocks of rows to fill the GPU, with eight tiles of keys each at least.
+int cache_umma_splits(const CacheAttnArgs& a) {
+  const long long rows = (long long)a.L * (a.Hq / a.c.H);
+  const long long blocks = (rows + kTiles * kBM - 1) / (kTiles * kBM) * a.c.B * a.c.H;
+  long long cap = a.c.rows << a.c.log_page;
+  if (!a.lens) cap = std::min(cap, std::max(a.len0, 0LL));
+  const long long n = std::min(148 / std::max(blocks, 1LL), cap / (8 * kBN));
+  return (int)std::max(1LL, std::min(n, 64LL));
+}
+
+cudaError_t cache_umma(const CacheAttnArgs& a, int dtype, int splits, cudaStream_t st) {
+  return dtype == NNLIB_B200_F16 ? launch_c<__half>(a, splits, st) : launch_c<__nv_bfloat16>(a, splits, st);
+}
+
+cudaError_t cache_umma_take_abort(int* out, cudaStream_t st) {
+  int v = 0;
+  cudaError_t e = cudaStreamSynchronize(st);
+  if (e != cudaSuccess) return e;
+  e = cudaMemcpyFromSymbol(&v, g_cache_attn_abort, sizeof(int));
+  if (e != cudaSuccess) return e;
+  if (v) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_cache_attn_abort, &zero, sizeof(int));
+  }
+  *out = v;
+  return e;
+}
+
+}  // namespace nb200
