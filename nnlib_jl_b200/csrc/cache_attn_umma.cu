@@ -80,11 +80,15 @@ __device__ __forceinline__ void codes4(uint32_t w, uint32_t& p0, uint32_t& p1) {
 // One side's tiles: keys 128 (j_lo + j) .. of sequence b, head h, into the ring at `ring`.  Two warps, each one chunk of 64
 // features (D = 128) or one half of the keys (D = 64); lane = (key of eight, piece of 16 features of four), which puts the
 // stores of eight lanes, two neighbouring keys, on all banks.
-template <int D, int CODE, int STAGES>
+// Keys that are not there, behind the last one or on pages that the pool does not have, read zeros (a NaN among E4M3's codes
+// would spoil rows that give them no weight) or, behind the last one of a group of SG keys, that one once more.
+__device__ const uint4 g_zero_codes[16] = {};
+
+template <int D, int CODE, int STAGES, int SG>
 __device__ __forceinline__ void convert_tiles(const CacheArgs& cc, const unsigned char* base, uint8_t* ring, const PageMeta* meta,
                                               uint64_t* full, uint64_t* empty, uint64_t* meta_full, volatile int* abort_flag,
                                               int w, int lane, int j_lo, int n_kv, int len) {
-  constexpr int N = D == 128 ? 16 : 8, BATCH = 4, NB = N / BATCH;
+  constexpr int N = D == 128 ? 16 : 8, AHEAD = 8;     // loads of a tile, and how many are under way
   constexpr int kTileBytes = CfgC<D>::kTileBytes;
   const int key8 = lane >> 2, piece = lane & 3;
   const int feat = (D == 128 ? w * 64 : 0) + piece * 16;
@@ -94,50 +98,52 @@ __device__ __forceinline__ void convert_tiles(const CacheArgs& cc, const unsigne
   const int u0 = ((2 * piece) ^ key8) << 4, u1 = ((2 * piece + 1) ^ key8) << 4;
   const int T1 = (1 << cc.log_page) - 1;
   base += feat;
-  uint4 raw[2][BATCH];
-  auto load = [&](uint4 (&r)[BATCH], int j, int bt) {
-#pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
-      const int n = n0 + bt * BATCH + i, key = (j_lo + j) * kBN + n * 8 + key8;
-      r[i] = make_uint4(0u, 0u, 0u, 0u);
-      const int page = meta[(j & (kMetaTiles - 1)) * 8 + (n >> 1)].page;
-      if (feat_ok && key < len && page >= 0)
-        r[i] = __ldg(reinterpret_cast<const uint4*>(base + (((long long)page << cc.log_page) + (key & T1)) * cc.row));
+  uint4 raw[AHEAD];
+  // 64 keys from number 64 hh of tile j on: where a group of SG of them begins, and its distance from key to key
+  const unsigned char* group;
+  int row, most;
+  auto load = [&](uint4& r, int j, int hh, int i) {
+    if (i % (SG / 8) == 0) {
+      const int key = (j_lo + j) * kBN + hh * 64 + i * 8;
+      const int page = meta[(j & (kMetaTiles - 1)) * 8 + hh * 4 + i / 2].page;
+      const bool in = feat_ok && page >= 0;
+      group = in ? base + (((long long)page << cc.log_page) + (key & T1)) * cc.row : reinterpret_cast<const unsigned char*>(g_zero_codes);
+      row = in ? (int)cc.row : 0;
+      most = len - 1 - key;
     }
+    // (what little of L1 shared memory leaves is for the stack)
+    asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+        : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(group + (long long)min((i % (SG / 8)) * 8 + key8, most) * row));
   };
   bool ok = n_kv > 0 && mbar_wait_warp(&meta_full[0], 0, abort_flag);
-  if (ok) load(raw[0], 0, 0);
+  if (ok) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) load(raw[i], 0, n0 / 8, i);
+  }
+#pragma unroll 1
   for (int j = 0; j < n_kv && ok; ++j) {
     const int s = j % STAGES;
+    if (j >= STAGES) ok = mbar_wait_warp(&empty[s], ((j / STAGES) - 1) & 1, abort_flag);
+    if (ok && j + 1 < n_kv && ((j + 1) & 3) == 0) ok = mbar_wait_warp(&meta_full[((j + 1) >> 2) & 1], ((j + 1) >> 3) & 1, abort_flag);
+    if (!ok) break;
+#pragma unroll 1
+    for (int h = 0; h < N / AHEAD; ++h) {
+      const bool last = h + 1 == N / AHEAD;
+      const int jn = last ? j + 1 : j, hn = last ? n0 / 8 : n0 / 8 + h + 1;      // what is fetched meanwhile
+      uint8_t* p = out + s * kTileBytes + h * (AHEAD * 1024);
 #pragma unroll
-    for (int bt = 0; bt < NB; ++bt) {
-      // the next batch, of this tile or the next one
-      if (bt + 1 < NB) {
-        load(raw[(bt + 1) & 1], j, bt + 1);
-      } else if (j + 1 < n_kv) {
-        const int jn = j + 1;
-        if ((jn & 3) == 0) ok = mbar_wait_warp(&meta_full[(jn >> 2) & 1], (jn >> 3) & 1, abort_flag);
-        if (!ok) break;
-        load(raw[(bt + 1) & 1], jn, 0);
-      }
-      if (bt == 0 && j >= STAGES) {
-        ok = mbar_wait_warp(&empty[s], ((j / STAGES) - 1) & 1, abort_flag);
-        if (!ok) break;
-      }
-#pragma unroll
-      for (int i = 0; i < BATCH; ++i) {
-        const uint4 r = raw[bt & 1][i];
+      for (int i = 0; i < AHEAD; ++i) {
+        const uint4 r = raw[i];
         uint4 a, b;
         codes4<CODE>(r.x, a.x, a.y);
         codes4<CODE>(r.y, a.z, a.w);
         codes4<CODE>(r.z, b.x, b.y);
         codes4<CODE>(r.w, b.z, b.w);
-        uint8_t* p = out + s * kTileBytes + (bt * BATCH + i) * 1024;
-        *reinterpret_cast<uint4*>(p + u0) = a;
-        *reinterpret_cast<uint4*>(p + u1) = b;
+        if (jn < n_kv) load(raw[i], jn, hn, i);
+        *reinterpret_cast<uint4*>(p + i * 1024 + u0) = a;
+        *reinterpret_cast<uint4*>(p + i * 1024 + u1) = b;
       }
     }
-    if (!ok) break;
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(&full[s]);
@@ -176,19 +182,12 @@ __global__ void __launch_bounds__(kThreadsC, 1) cache_attn_umma_kernel(const Cac
     return e < 0 ? -1 : (e < len ? (int)e : len - 1);
   };
   // this block's key tiles, and where each of its row tiles stops
-  int n_t[kTiles], j_lo;
-  {
-    int most = 0, n[kTiles];
-    for (int t = 0; t < kTiles; ++t) {
-      const int lo = row0 + t * kBM;
-      n[t] = lo < rows ? (last_key(min(lo + kBM, rows) - 1) + kBN) / kBN : 0;
-      most = max(most, n[t]);
-    }
-    const int share = (most + splits - 1) / splits;
-    j_lo = split * share;
-    for (int t = 0; t < kTiles; ++t) n_t[t] = max(0, min(n[t], j_lo + share) - j_lo);
-  }
-  const int n_kv = max(n_t[0], n_t[1]);
+  // (named, not an array: an index that is not a constant would put it into local memory)
+  const int end0 = (last_key(min(row0 + kBM, rows) - 1) + kBN) / kBN;
+  const int end1 = row0 + kBM < rows ? (last_key(min(row0 + 2 * kBM, rows) - 1) + kBN) / kBN : 0;
+  const int share = (max(end0, end1) + splits - 1) / splits, j_lo = split * share;
+  const int n_t0 = max(0, min(end0, j_lo + share) - j_lo), n_t1 = max(0, min(end1, j_lo + share) - j_lo);
+  const int n_kv = max(n_t0, n_t1);
 
   if (threadIdx.x == 0) {
     for (int t = 0; t < kTiles; ++t) {
@@ -219,9 +218,9 @@ __global__ void __launch_bounds__(kThreadsC, 1) cache_attn_umma_kernel(const Cac
   const uint32_t tmem = bars->tmem_base;
   const bool start_ok = (*abort_flag == 0);
 
-  // registers: 128 x 40 + 256 x 208 + 128 x 56 = the 512 x 128 launched
+  // registers: 128 x 64 + 256 x 168 + 128 x 112 = the 512 x 128 launched
   if (warp < 4) {
-    setmaxnreg_dec<40>();
+    setmaxnreg_dec<64>();
     if (start_ok && warp == 0) {
       // ---------------------------------------------------- pages and scales, four tiles at a time
       bool ok = true;
@@ -258,88 +257,98 @@ __global__ void __launch_bounds__(kThreadsC, 1) cache_attn_umma_kernel(const Cac
       const uint32_t q_lo = (smem_u32(smem) >> 4) | lbo_k;
       const uint32_t k_lo = (smem_u32(smem + C::kKOff) >> 4) | lbo_k;
       const uint32_t v_lo = (smem_u32(smem + C::kVOff) >> 4) | lbo_v;
+      // (the bases are made opaque, or the compiler keeps every descriptor of the loop in a register and spills them:
+      // this thread's local loads then take longer than the products)
       auto issue_qk = [&](int t, int stage) {
+        uint32_t ql = q_lo + t * tile16, kl = k_lo + stage * tile16, ts = tmem + t * kBN;
+        asm volatile("" : "+r"(ql), "+r"(kl), "+r"(ts));
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = (kk >> 2) * (kChunkBytes >> 4) + (kk & 3) * 2;
-          umma_ss_lohi(tmem + t * kBN, q_lo + t * tile16 + off, k_lo + stage * tile16 + off, desc_hi, idesc_qk, kk > 0 ? 1u : 0u);
+          umma_ss_lohi(ts, ql + off, kl + off, desc_hi, idesc_qk, kk > 0 ? 1u : 0u);
         }
       };
       auto issue_pv = [&](int t, int stage, int half, bool first) {
+        uint32_t to = tmem + kTiles * kBN + t * D, tw = tmem + t * kBN + half * (kBN / 4), vl = v_lo + stage * tile16 + half * ((kBN / 32) * (2048 >> 4));
+        asm volatile("" : "+r"(to), "+r"(tw), "+r"(vl));
 #pragma unroll
-        for (int kk = 0; kk < kBN / 32; ++kk) {
-          const int k = half * (kBN / 32) + kk;
-          umma_ts_lohi(tmem + kTiles * kBN + t * D, tmem + t * kBN + k * 8, v_lo + stage * tile16 + k * (2048 >> 4), desc_hi,
-                       idesc_pv, (first && k == 0) ? 0u : 1u);
-        }
+        for (int kk = 0; kk < kBN / 32; ++kk)
+          umma_ts_lohi(to, tw + kk * 8, vl + kk * (2048 >> 4), desc_hi, idesc_pv, (first && half == 0 && kk == 0) ? 0u : 1u);
       };
       bool ok = true;
-      for (int t = 0; t < kTiles; ++t)
-        if (ok && n_t[t] > 0) ok = mbar_wait(&bars->q_full[t], 0, abort_flag);
+      if (n_t0 > 0) ok = mbar_wait(&bars->q_full[0], 0, abort_flag);
+      if (ok && n_t1 > 0) ok = mbar_wait(&bars->q_full[1], 0, abort_flag);
       if (ok) ok = mbar_wait(&bars->k_full[0], 0, abort_flag);
       if (ok) {
         tc_fence_after();
-        for (int t = 0; t < kTiles; ++t)
-          if (n_t[t] > 0) {
-            issue_qk(t, 0);
-            umma_commit(&bars->s_full[t]);
-          }
+        if (n_t0 > 0) {
+          issue_qk(0, 0);
+          umma_commit(&bars->s_full[0]);
+        }
+        if (n_t1 > 0) {
+          issue_qk(1, 0);
+          umma_commit(&bars->s_full[1]);
+        }
         umma_commit(&bars->k_empty[0]);
       }
+#pragma unroll 1
       for (int j = 0; j < n_kv && ok; ++j) {
+        BarsC* bb = bars;
+        asm volatile("" : "+l"(bb));         // (nor every barrier's address)
         const int sv = j % C::kStagesV, sk = (j + 1) % C::kStagesK;
         const uint32_t par = j & 1;
-        ok = mbar_wait(&bars->v_full[sv], (j / C::kStagesV) & 1, abort_flag);
-        if (ok && j + 1 < n_kv) ok = mbar_wait(&bars->k_full[sk], ((j + 1) / C::kStagesK) & 1, abort_flag);
+        ok = mbar_wait(&bb->v_full[sv], (j / C::kStagesV) & 1, abort_flag);
+        if (ok && j + 1 < n_kv) ok = mbar_wait(&bb->k_full[sk], ((j + 1) / C::kStagesK) & 1, abort_flag);
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
-          const int nt = t == 0 ? n_t[0] : n_t[1];
+          const int nt = t == 0 ? n_t0 : n_t1;
           if (!ok || j >= nt) continue;
-          ok = mbar_wait(&bars->p_half[t][0], par, abort_flag);
+          ok = mbar_wait(&bb->p_half[t][0], par, abort_flag);
           if (!ok) continue;
           tc_fence_after();
           issue_pv(t, sv, 0, j == 0);
-          ok = mbar_wait(&bars->p_half[t][1], par, abort_flag);
+          ok = mbar_wait(&bb->p_half[t][1], par, abort_flag);
           if (!ok) continue;
           tc_fence_after();
           issue_pv(t, sv, 1, false);
           if (j + 1 < nt) {
             issue_qk(t, sk);
-            umma_commit(&bars->s_full[t]);
+            umma_commit(&bb->s_full[t]);
           } else {
-            umma_commit(&bars->o_full[t]);
+            umma_commit(&bb->o_full[t]);
           }
         }
         if (!ok) break;
-        umma_commit(&bars->v_empty[sv]);
-        if (j + 1 < n_kv) umma_commit(&bars->k_empty[sk]);
+        umma_commit(&bb->v_empty[sv]);
+        if (j + 1 < n_kv) umma_commit(&bb->k_empty[sk]);
         // everything of tiles up to j is done with: the pages and scales of j - 3 .. j may go
-        if ((j & 3) == 3) umma_commit(&bars->meta_free[(j >> 2) & 1]);
+        if ((j & 3) == 3) umma_commit(&bb->meta_free[(j >> 2) & 1]);
       }
     }
   } else if (warp >= 12) {
-    setmaxnreg_dec<56>();
+    setmaxnreg_dec<112>();
     if (start_ok) {
       const int w = (warp - 12) & 1;
       if (warp < 14)
-        convert_tiles<D, CODE, C::kStagesK>(cc, cc.codes[0] + (long long)h * cc.d, smem + C::kKOff, meta, bars->k_full,
+        convert_tiles<D, CODE, C::kStagesK, SG>(cc, cc.codes[0] + (long long)h * cc.d, smem + C::kKOff, meta, bars->k_full,
                                             bars->k_empty, bars->meta_full, abort_flag, w, lane, j_lo, n_kv, len);
       else
-        convert_tiles<D, CODE, C::kStagesV>(cc, cc.codes[1] + (long long)h * cc.d, smem + C::kVOff, meta, bars->v_full,
+        convert_tiles<D, CODE, C::kStagesV, SG>(cc, cc.codes[1] + (long long)h * cc.d, smem + C::kVOff, meta, bars->v_full,
                                             bars->v_empty, bars->meta_full, abort_flag, w, lane, j_lo, n_kv, len);
     }
   } else {
-    setmaxnreg_inc<208>();
-    const int t = (warp - 4) >> 2, nt = t == 0 ? n_t[0] : n_t[1];
-    const int wq = warp & 3, r = wq * 32 + lane, row = row0 + t * kBM + r;
-    const bool row_ok = row < rows;
-    const int i = row_ok ? row / G : 0, hq = h * G + (row_ok ? row % G : 0);
+    setmaxnreg_inc<168>();
+    const int t = (warp - 4) >> 2, nt = t == 0 ? n_t0 : n_t1;
+    const int wq = warp & 3;
     if (start_ok && row0 + t * kBM < rows) {
       const uint32_t lane_base = tmem + (static_cast<uint32_t>(wq * 32) << 16);
       const uint32_t tS = lane_base + t * kBN, tO = lane_base + kTiles * kBN + t * D;
-      const int lim = last_key(row);
+      const int lim = last_key(row0 + t * kBM + wq * 32 + lane);
       float crow = 0.f;
       if (nt > 0) {
+        const int r = wq * 32 + lane, row = row0 + t * kBM + r;
+        const bool row_ok = row < rows;
+        const int i = row_ok ? row / G : 0, hq = h * G + (row_ok ? row % G : 0);
         // ------------------------------------------------ this row of Q, by a power of two to a largest element in [2^13, 2^14)
         const T* qp = reinterpret_cast<const T*>(a.q) + (long long)i * a.q_sl + (long long)b * a.q_sb + (long long)hq * cc.d;
         auto load8 = [&](int f, float (&v)[8]) {
@@ -385,85 +394,69 @@ __global__ void __launch_bounds__(kThreadsC, 1) cache_attn_umma_kernel(const Cac
 
       float m_used = neg_inf(), l = 0.f;
       bool ok = true;
+#pragma unroll 1
       for (int j = 0; j < nt; ++j) {
-        if ((j & 3) == 0) ok = mbar_wait_warp(&bars->meta_full[(j >> 2) & 1], (j >> 3) & 1, abort_flag);
+        uint8_t* sm = smem;
+        asm volatile("" : "+l"(sm));         // (no barrier's address in a register for good)
+        BarsC* bb = reinterpret_cast<BarsC*>(sm + C::kBarOff);
+        volatile int* abort_flag = &bb->abort_flag;
+        if ((j & 3) == 0) ok = mbar_wait_warp(&bb->meta_full[(j >> 2) & 1], (j >> 3) & 1, abort_flag);
         if (!ok) break;
-        // scales: a group of SG keys has factor fg, offset cg
-        constexpr int NG = kBN / SG;
-        const PageMeta* pm = meta + (j & (kMetaTiles - 1)) * 8;
-        float fg[NG], cg[NG];
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          fg[g] = crow * pm[g * (SG / 16)].ks;
-          cg[g] = pm[g * (SG / 16)].lvs;
-        }
-        ok = mbar_wait(&bars->s_full[t], j & 1, abort_flag);
+        // scales: a group of SG keys has a factor and an offset
+        const PageMeta* pm = reinterpret_cast<const PageMeta*>(sm + C::kMetaOff) + (j & (kMetaTiles - 1)) * 8;
+        ok = mbar_wait(&bb->s_full[t], j & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        uint32_t sr[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, sr[c]);
-        tmem_wait_ld();
+        // Twice over the scores, 64 keys at a time: once for the maximum, once for the weights, which overwrite them.  (Held
+        // whole in registers, as the 16-bit forward does, a row leaves none for the converting warps, and the longer code
+        // keeps every warp waiting for instructions: TODO us.)
         const int j0 = (j_lo + j) * kBN;
-        if (__any_sync(0xffffffffu, j0 + kBN - 1 > lim)) {
-          // the scaled logits themselves, -Inf where the row does not look
+        const bool edge = __any_sync(0xffffffffu, j0 + kBN - 1 > lim);
+        constexpr int HG = 64 / SG;             // scales of 64 keys
+        uint32_t sr[2][32];
+        auto fetch = [&](int hf) {
+          tmem_ld32(tS + hf * 64, sr[0]);
+          tmem_ld32(tS + hf * 64 + 32, sr[1]);
+          tmem_wait_ld();
+          if (edge) {
+            // the scaled logits themselves, -Inf where the row does not look
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+            for (int g = 0; g < HG; ++g) {
+              const float f = crow * pm[hf * 4 + g * (SG / 16)].ks, o = pm[hf * 4 + g * (SG / 16)].lvs;
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const int g = (c * 32 + e) / SG;
-              const float v = fmaf(__uint_as_float(sr[c][e]), fg[g], cg[g]);
-              sr[c][e] = j0 + c * 32 + e > lim ? 0xff800000u : __float_as_uint(v);
+              for (int e = g * SG; e < (g + 1) * SG; ++e) {
+                const float v = fmaf(__uint_as_float(sr[e / 32][e & 31]), f, o);
+                sr[e / 32][e & 31] = j0 + hf * 64 + e > lim ? 0xff800000u : __float_as_uint(v);
+              }
             }
-#pragma unroll
-          for (int g = 0; g < NG; ++g) fg[g] = 1.f, cg[g] = 0.f;
-        }
-
-        uint32_t pk[32];
-        float sums[NG];
-        // weights of 64 keys relative to REF
-        auto weights = [&](int hf, float ref) {
-#pragma unroll
-          for (int gg = 0; gg < 64 / SG; ++gg) {
-            const int g = hf * (64 / SG) + gg;
-            const unsigned long long f2 = pair_of(fg[g]), c2 = pair_of(cg[g] - ref);
-            unsigned long long s2[2] = {0ull, 0ull};
-#pragma unroll
-            for (int e = 0; e < SG; e += 2) {
-              const int at = gg * SG + e, c = hf * 2 + at / 32;
-              float x0, x1;
-              fma2(x0, x1, __uint_as_float(sr[c][at & 31]), __uint_as_float(sr[c][(at & 31) + 1]), f2, c2);
-              x0 = ex2_approx(x0);
-              x1 = ex2_approx(x1);
-              add2(s2[(e >> 1) & 1], x0, x1);
-              pk[at >> 1] = pack2<false>(x0, x1);
-            }
-            sums[g] = pair_sum(s2[0]) + pair_sum(s2[1]);
           }
         };
+        auto factor = [&](int hf, int g) { return edge ? 1.f : crow * pm[hf * 4 + g * (SG / 16)].ks; };
+        auto offset = [&](int hf, int g) { return edge ? 0.f : pm[hf * 4 + g * (SG / 16)].lvs; };
+
         float mx = neg_inf();
+#pragma unroll 1
+        for (int hf = 0; hf < 2; ++hf) {
+          fetch(hf);
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          float m0 = neg_inf(), m1 = neg_inf();
+          for (int g = 0; g < HG; ++g) {
+            float m0 = neg_inf(), m1 = neg_inf();
 #pragma unroll
-          for (int e = 0; e < SG; e += 4) {
-            const int c = (g * SG + e) / 32, at = (g * SG + e) & 31;
-            m0 = max3(m0, __uint_as_float(sr[c][at]), __uint_as_float(sr[c][at + 1]));
-            m1 = max3(m1, __uint_as_float(sr[c][at + 2]), __uint_as_float(sr[c][at + 3]));
+            for (int e = g * SG; e < (g + 1) * SG; e += 4) {
+              m0 = max3(m0, __uint_as_float(sr[e / 32][e & 31]), __uint_as_float(sr[e / 32][(e & 31) + 1]));
+              m1 = max3(m1, __uint_as_float(sr[e / 32][(e & 31) + 2]), __uint_as_float(sr[e / 32][(e & 31) + 3]));
+            }
+            mx = fmaxf(mx, fmaf(fmaxf(m0, m1), factor(hf, g), offset(hf, g)));
           }
-          mx = fmaxf(mx, fmaf(fmaxf(m0, m1), fg[g], cg[g]));
         }
         const float m_new = fmaxf(m_used, mx - kBits);
         const bool raise = m_new > m_used + kGap;      // also true for m_used = -Inf < m_new
-        // the first half against the running reference while the maximum is being found; redone where that moves it
-        const bool guess = j > 0;
-        if (guess) weights(0, m_used == neg_inf() ? 0.f : m_used);
-        if (!guess || __any_sync(0xffffffffu, raise)) {
+        if (__any_sync(0xffffffffu, raise)) {
           if (j > 0) {
             const float f = raise ? ex2_approx(m_used - m_new) : 1.f;
             l *= f;
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               uint32_t o[32];
               tmem_ld32(tO + c * 32, o);
@@ -474,21 +467,34 @@ __global__ void __launch_bounds__(kThreadsC, 1) cache_attn_umma_kernel(const Cac
             }
           }
           if (raise) m_used = m_new;
-          weights(0, m_used == neg_inf() ? 0.f : m_used);
         }
         const float ref = m_used == neg_inf() ? 0.f : m_used;
-#pragma unroll
+#pragma unroll 1
         for (int hf = 0; hf < 2; ++hf) {
-          if (hf == 1) weights(1, ref);
-          tmem_st32(tS + hf * 32, pk);
-          // a page that the row does not see adds nothing, whatever its scale is
+          fetch(hf);
+          uint32_t pk[32];
 #pragma unroll
-          for (int g = hf * NG / 2; g < (hf + 1) * NG / 2; ++g)
-            if (!(sums[g] == 0.f)) l = fmaf(sums[g], pm[g * (SG / 16)].ivs, l);
+          for (int g = 0; g < HG; ++g) {
+            const unsigned long long f2 = pair_of(factor(hf, g)), c2 = pair_of(offset(hf, g) - ref);
+            unsigned long long s2[2] = {0ull, 0ull};
+#pragma unroll
+            for (int e = g * SG; e < (g + 1) * SG; e += 2) {
+              float x0, x1;
+              fma2(x0, x1, __uint_as_float(sr[e / 32][e & 31]), __uint_as_float(sr[e / 32][(e & 31) + 1]), f2, c2);
+              x0 = ex2_approx(x0);
+              x1 = ex2_approx(x1);
+              add2(s2[(e >> 1) & 1], x0, x1);
+              pk[e >> 1] = pack2<false>(x0, x1);
+            }
+            // a page that the row does not see adds nothing, whatever its scale is
+            const float sum = pair_sum(s2[0]) + pair_sum(s2[1]);
+            if (!(sum == 0.f)) l = fmaf(sum, pm[hf * 4 + g * (SG / 16)].ivs, l);
+          }
+          tmem_st32(tS + hf * 32, pk);
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->p_half[t][hf]);
+          if (lane == 0) mbar_arrive(&bb->p_half[t][hf]);
         }
       }
 
@@ -500,6 +506,11 @@ __global__ void __launch_bounds__(kThreadsC, 1) cache_attn_umma_kernel(const Cac
       if (ok) {
         tc_fence_after();
         const bool dead = l == 0.f;
+        // (worked out anew, so that nothing of it lives in registers beside a score row)
+        int tid = threadIdx.x;
+        asm volatile("" : "+r"(tid));
+        const int row = row0 + ((tid - 128) & 255), i = row < rows ? row / G : 0, hq = h * G + (row < rows ? row % G : 0);
+        const bool row_ok = row < rows;
         const long long unit = hq + (long long)a.Hq * b, at = (unit * splits + split) * a.L + i;
         float* wrow = nullptr;
         T* xrow = nullptr;
