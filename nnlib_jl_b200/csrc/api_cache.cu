@@ -1,5 +1,6 @@
 // The C ABI of what stands around attention in a decoder layer (include/nnlib_b200.h): norm and rotation of heads, the
 // 8-bit key / value cache and attention over it.  Argument checks and defaults, as in api.cu.
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <cstdio>
@@ -43,7 +44,7 @@ int resolve_norm_rope(const nnlib_b200_norm_rope_params* p, bool bwd, NormRopeAr
   if (p->d < 2 || p->d % 2 || p->rot < 0 || p->rot % 2 || p->rot > p->d) return NNLIB_B200_INVALID_ARG;
   if (p->Hq < 0 || p->Hk < 0 || p->Hq + p->Hk < 1 || p->L < 0 || p->B < 0) return NNLIB_B200_INVALID_ARG;
   if (p->d > 256) return NNLIB_B200_UNSUPPORTED_SHAPE;
-  if (p->Hq > kMost / p->d || p->Hk > kMost / p->d || p->L > kMost || p->B > kMost || (p->L && p->B > (kMost << 8) / p->L))
+  if (p->Hq > kMost / p->d || p->Hk > kMost / p->d || p->L > kMost || p->B > kMost || (p->L && p->B > kMost / p->L / std::max<int64_t>(1, std::max(p->Hq, p->Hk))))
     return NNLIB_B200_INVALID_ARG;
   if (!(p->eps >= 0.f) || std::isinf(p->eps)) return NNLIB_B200_INVALID_ARG;
   if (p->start0 < -kMost || p->start0 > kMost) return NNLIB_B200_INVALID_ARG;
@@ -102,7 +103,7 @@ int resolve_cache(const nnlib_b200_cache* c, CacheArgs* out) {
   if (c->d < 1 || c->H < 1 || c->pages < 0 || c->B < 0 || c->rows < 0 || c->table_stride < 0) return NNLIB_B200_INVALID_ARG;
   if (c->page < 16 || c->page > 256 || (c->page & (c->page - 1))) return NNLIB_B200_INVALID_ARG;
   if (c->d % 16 || c->d > 256) return NNLIB_B200_UNSUPPORTED_SHAPE;
-  if (c->H > 32767 || c->B > 65535 || c->pages > kMost) return NNLIB_B200_INVALID_ARG;
+  if (c->H > 32767 || c->B > 32767 || c->pages > kMost) return NNLIB_B200_INVALID_ARG;
   if (c->rows > (kMost - 4095) / c->page) return NNLIB_B200_INVALID_ARG;
   CacheArgs a;
   std::memset(&a, 0, sizeof(a));

@@ -1,9 +1,12 @@
 // Tokens into and out of the 8-bit key / value cache (nnlib_b200.h: pages, scales, codes).
 //
+// Both are bound by HBM: an element is two bytes (or four) on one side and one on the other.
 // Write: one block for a page that a sequence's new tokens touch, a head, and keys or values.  It is the only one that
 // touches this page's scale and codes of this head, so there is nothing to order: it finds the new tokens' largest
-// magnitude, settles the scale, rounds the older codes anew where the scale has grown, and writes the new ones.
-// Read: 16 codes to a thread.  Both are bound by HBM: an element is two bytes on one side and one on the other.
+// magnitude, settles the scale, rounds the older codes anew where the scale has grown, and writes the new ones.  A thread
+// works on 16 elements at a time, one 16-byte store of codes, and keeps the first HELD such pieces in registers between
+// the two steps; blocks of more (pages of more than 8192 elements of a head) read the rest again, from L2.
+// Read: eight codes to a thread and store, so that a warp's stores of 16-bit results are whole lines.
 #include <algorithm>
 
 #include "cache_codes.cuh"
@@ -11,133 +14,225 @@
 namespace nb200 {
 namespace {
 
-constexpr int kWrThreads = 256;
+constexpr int kHeld = 2;
 
-template <typename T, int CODE>
-__global__ void __launch_bounds__(kWrThreads) cache_write_kernel(const CacheArgs c, const CacheTokens t) {
-  __shared__ float sm[kWrThreads / 32];
-  const int kv = blockIdx.y / c.H, h = blockIdx.y % c.H, b = blockIdx.z, tid = threadIdx.x;
-  const int T_ = 1 << c.log_page;
+// 16 elements; VEC: 16-byte loads
+template <typename T, bool VEC>
+__device__ __forceinline__ void load16(const T* p, T (&v)[16]) {
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(v) / 16; ++i) {
+      const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+      memcpy(reinterpret_cast<char*>(v) + 16 * i, &raw, 16);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = p[i];
+  }
+}
+
+// The largest magnitude of 16 elements and what came before, as bits: a NaN is larger than all others.
+__device__ __forceinline__ uint32_t magnitude(uint32_t top, const float (&v)[16]) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+  return top;
+}
+template <typename T2, typename T>
+__device__ __forceinline__ uint32_t magnitude16(uint32_t top, const T (&v)[16]) {
+  T2 m[8];
+  memcpy(m, v, sizeof(m));
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m[e] = __habs2(m[e]);
+#pragma unroll
+  for (int n = 4; n > 0; n >>= 1)
+#pragma unroll
+    for (int e = 0; e < n; ++e) m[e] = __hmax2_nan(m[e], m[e + n]);
+  const float lo = __low2float(m[0]), hi = __high2float(m[0]);
+  return max(top, max(__float_as_uint(lo) & 0x7fffffffu, __float_as_uint(hi) & 0x7fffffffu));
+}
+__device__ __forceinline__ uint32_t magnitude(uint32_t top, const __half (&v)[16]) { return magnitude16<__half2>(top, v); }
+__device__ __forceinline__ uint32_t magnitude(uint32_t top, const __nv_bfloat16 (&v)[16]) { return magnitude16<__nv_bfloat162>(top, v); }
+
+template <typename T, int CODE, bool VEC>
+__global__ void __launch_bounds__(256, 4) cache_write_kernel(const CacheArgs c, const CacheTokens t) {
+  __shared__ uint32_t sm[8];
+  // heads side by side: what runs at one time reads whole tokens
+  const int h = blockIdx.x % c.H, kv = (blockIdx.x / c.H) & 1, b = blockIdx.y, tid = threadIdx.x, nt = blockDim.x;
   const long long start = t.start ? (long long)t.start[b] : t.start0;
   const long long n_new = t.count ? min(max(t.count[b], 0), t.L) : t.L;
   if (start < 0) return;
-  const long long p = (start >> c.log_page) + blockIdx.x;              // page of the sequence
+  const long long p = (start >> c.log_page) + blockIdx.x / (2 * c.H);  // page of the sequence
   if (p >= c.rows) return;
   const long long lo = max(start, p << c.log_page), hi = min(start + n_new, (p + 1) << c.log_page);
   if (lo >= hi) return;
+  const int fill = (int)(lo - (p << c.log_page));                      // older tokens of the page
+  const unsigned pieces = c.d / 16, n = (unsigned)(hi - lo) * pieces;  // new ones, in pieces
+  const long long sl = t.sl[kv];
+  const T* x = reinterpret_cast<const T*>(t.x[kv]) + (lo - start) * sl + b * t.sb[kv] + (long long)h * c.d;
+  auto source = [&](unsigned i) { return x + (long long)(i / pieces) * sl + (i % pieces) * 16; };
+
+  T held[kHeld][16];
+#pragma unroll
+  for (int r = 0; r < kHeld; ++r)
+    if (tid + r * nt < n) load16<T, VEC>(source(tid + r * nt), held[r]);
   const long long page = cache_page(c, b, p);
   if (page < 0) return;
-  const int fill = (int)(lo - (p << c.log_page)), n = (int)(hi - lo);  // older tokens of the page, new ones
-  const T* x = reinterpret_cast<const T*>(t.x[kv]) + (lo - start) * t.sl[kv] + b * t.sb[kv] + (long long)h * c.d;
-  unsigned char* codes = c.codes[kv] + (page * T_) * c.row + (long long)h * c.d;
+  unsigned char* codes = c.codes[kv] + (page << c.log_page) * c.row + (long long)h * c.d;
   float* scale = c.scale[kv] + page * c.H + h;
-
-  float amax = 0.f;
-  bool bad = false;
-  for (int i = tid; i < n * c.d; i += kWrThreads) {
-    const int l = i / c.d, e = i - l * c.d;
-    const float v = fabsf(Elem<T>::to_f(x[l * t.sl[kv] + e]));
-    bad |= !(v <= 3.402823466e38f);
-    amax = fmaxf(amax, v);
-  }
-  if (bad) amax = __int_as_float(0x7f800000);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-  if ((tid & 31) == 0) sm[tid >> 5] = amax;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWrThreads / 32; ++w) amax = fmaxf(amax, sm[w]);
-
   const float old = fill > 0 ? *scale : 0.f;
-  const float asked = block_scale<CODE>(amax);
+
+  uint32_t top = 0u;
+#pragma unroll
+  for (int r = 0; r < kHeld; ++r)
+    if (tid + r * nt < n) top = magnitude(top, held[r]);
+  for (unsigned i = tid + kHeld * nt; i < n; i += nt) {
+    T v[16];
+    load16<T, VEC>(source(i), v);
+    top = magnitude(top, v);
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (nt > 32) {
+    if ((tid & 31) == 0) sm[tid >> 5] = top;
+    __syncthreads();
+    for (int w = 0; w < nt / 32; ++w) top = max(top, sm[w]);
+  }
+
+  const float asked = block_scale<CODE>(__uint_as_float(top));
   const float s = (old != old || asked != asked) ? __int_as_float(0x7fc00000) : fmaxf(old, asked);
   const float inv = inverse_scale(s);
   if (fill > 0 && s > old) {
     const float f = __fdiv_rn(old, s);
-    for (int i = tid; i < fill * c.d; i += kWrThreads) {
-      const int l = i / c.d, e = i - l * c.d;
-      unsigned char* q = codes + l * c.row + e;
-      *q = (unsigned char)to_code<CODE>(from_code<CODE>(*q), f);
+    for (unsigned i = tid; i < fill * pieces; i += nt) {
+      uint4* q = reinterpret_cast<uint4*>(codes + (long long)(i / pieces) * c.row + (i % pieces) * 16);
+      uint4 v = *q;
+      auto again = [&](uint32_t w) {
+        float g[4];
+        from_codes4<CODE>(w, g);
+        return to_codes4<CODE>(g[0], g[1], g[2], g[3], f);
+      };
+      *q = make_uint4(again(v.x), again(v.y), again(v.z), again(v.w));
     }
   }
-  for (int i = tid; i < n * c.d; i += kWrThreads) {
-    const int l = i / c.d, e = i - l * c.d;
-    codes[(fill + l) * c.row + e] = (unsigned char)to_code<CODE>(code_input(Elem<T>::to_f(x[l * t.sl[kv] + e]), inv), inv);
+  auto quantise = [&](unsigned i, const T (&v)[16]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      w[e] = to_codes4<CODE>(Elem<T>::to_f(v[4 * e]), Elem<T>::to_f(v[4 * e + 1]), Elem<T>::to_f(v[4 * e + 2]), Elem<T>::to_f(v[4 * e + 3]), inv);
+    *reinterpret_cast<uint4*>(codes + (long long)(fill + i / pieces) * c.row + (i % pieces) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+  };
+#pragma unroll
+  for (int r = 0; r < kHeld; ++r)
+    if (tid + r * nt < n) quantise(tid + r * nt, held[r]);
+  for (unsigned i = tid + kHeld * nt; i < n; i += nt) {
+    T v[16];
+    load16<T, VEC>(source(i), v);
+    quantise(i, v);
   }
-  __syncthreads();                                                     // every thread has read the old scale
+  // (every thread has read the old scale: it came before the barrier, or the block is one warp)
   if (tid == 0) *scale = s;
 }
 
-template <typename T, int CODE>
+constexpr int kReadTokens = 16;            // tokens of a block: never more than a page's
+
+// VEC: results may be stored 16 bytes at a time
+template <typename T, int CODE, bool VEC>
 __global__ void __launch_bounds__(256) cache_read_kernel(const CacheArgs c, const CacheTokens t) {
-  const int kv = blockIdx.y, b = blockIdx.z;
-  const long long parts = c.row / 16, i = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long l = i / parts;
-  if (l >= t.L) return;
-  const int e0 = (int)(i - l * parts) * 16, h = e0 / c.d;
-  const long long pos = l + (t.start ? (long long)t.start[b] : t.start0);
-  T out[16];
-  uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-  float s = 0.f;
-  if (pos >= 0 && pos < (c.rows << c.log_page) && !(t.lens && pos >= t.lens[b])) {
-    const long long page = cache_page(c, b, pos >> c.log_page);
-    s = __int_as_float(0x7fc00000);
-    if (page >= 0) {
-      const long long slot = (page << c.log_page) + (pos & ((1 << c.log_page) - 1));
-      raw = __ldcs(reinterpret_cast<const uint4*>(c.codes[kv] + slot * c.row + e0));
-      s = c.scale[kv][page * c.H + h];
+  const int kv = blockIdx.y & 1, b = blockIdx.y >> 1;
+  const int parts = (int)(c.row / 8), width = min(parts, 256), rows = 256 / width;   // eight codes to a thread, tokens side by side
+  const int col = threadIdx.x % width, first = threadIdx.x / width;
+  const long long start = t.start ? (long long)t.start[b] : t.start0;
+  // the block's tokens are those of one aligned sixteen, so one page's (below zero, too)
+  const long long p16 = (start >> 4) + blockIdx.x, lo = max(p16 << 4, start), hi = min((p16 + 1) << 4, start + t.L);
+  const long long cap = c.rows << c.log_page, end = t.lens ? min(cap, (long long)t.lens[b]) : cap;
+  const bool inside = lo >= 0 && lo < end;
+  const long long page = inside ? cache_page(c, b, lo >> c.log_page) : -1;
+  const unsigned char* codes = c.codes[kv] + (page < 0 ? 0 : ((page << c.log_page) + (lo & ((1 << c.log_page) - 1))) * c.row);
+  T* y = reinterpret_cast<T*>(t.x[kv]) + (lo - start) * t.sl[kv] + b * t.sb[kv];
+  const int n = (int)(hi - lo), n_in = inside ? (int)min((long long)n, end - lo) : 0;
+  if (first >= rows) return;
+  for (int part = col; part < parts; part += width) {
+    float s = __int_as_float(0x7fc00000);
+    if (page >= 0) s = c.scale[kv][page * c.H + part * 8 / c.d];
+#pragma unroll 4
+    for (int l = first; l < n; l += rows) {
+      uint2 raw = make_uint2(0u, 0u);
+      if (l < n_in && page >= 0) raw = __ldcs(reinterpret_cast<const uint2*>(codes + l * c.row + part * 8));
+      const float sl = l < n_in ? s : 0.f;
+      float f[8];
+      {
+        float lo4[4], hi4[4];
+        from_codes4<CODE>(raw.x, lo4);
+        from_codes4<CODE>(raw.y, hi4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f[e] = lo4[e] * sl;
+          f[4 + e] = hi4[e] * sl;
+        }
+      }
+      T out[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) out[e] = Elem<T>::from_f(f[e]);
+      T* to = y + l * t.sl[kv] + part * 8;
+      if constexpr (VEC) {
+#pragma unroll
+        for (int e = 0; e < (int)sizeof(out) / 16; ++e) {
+          uint4 v;
+          memcpy(&v, reinterpret_cast<const char*>(out) + 16 * e, 16);
+          __stcs(reinterpret_cast<uint4*>(to) + e, v);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) to[e] = out[e];
+      }
     }
-  }
-  const unsigned int w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-  for (int j = 0; j < 16; ++j) out[j] = Elem<T>::from_f(from_code<CODE>(w[j >> 2] >> (8 * (j & 3))) * s);
-  T* y = reinterpret_cast<T*>(t.x[kv]) + l * t.sl[kv] + b * t.sb[kv] + e0;
-  if (((reinterpret_cast<uintptr_t>(y) & 15u) == 0)) {
-#pragma unroll
-    for (int j = 0; j < (int)sizeof(out) / 16; ++j) {
-      uint4 v;
-      memcpy(&v, reinterpret_cast<const char*>(out) + 16 * j, 16);
-      reinterpret_cast<uint4*>(y)[j] = v;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) y[j] = out[j];
   }
 }
 
-template <typename T>
+// may elements be moved 16 bytes at a time?
+bool vectors(const CacheTokens& t, int esize) {
+  for (int i = 0; i < 2; ++i)
+    if (reinterpret_cast<uintptr_t>(t.x[i]) % 16 || t.sl[i] * esize % 16 || t.sb[i] * esize % 16) return false;
+  return true;
+}
+
+template <typename T, int CODE>
 cudaError_t write_t(const CacheArgs& c, const CacheTokens& t, cudaStream_t st) {
   const int T_ = 1 << c.log_page;
   const long long pages = std::min<long long>((t.L + T_ - 2) / T_ + 1, c.rows);    // that L tokens can touch
-  const dim3 grid((unsigned)pages, 2 * c.H, c.B);
-  if (c.code == NNLIB_B200_INT8) cache_write_kernel<T, NNLIB_B200_INT8><<<grid, kWrThreads, 0, st>>>(c, t);
-  else cache_write_kernel<T, NNLIB_B200_E4M3><<<grid, kWrThreads, 0, st>>>(c, t);
+  if (pages * 2 * c.H > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+  const dim3 grid((unsigned)(pages * 2 * c.H), c.B);
+  const int pieces = std::min(t.L, T_) * (c.d / 16);
+  const int threads = std::min(256, std::max(32, (pieces / kHeld + 31) & ~31));
+  if (vectors(t, sizeof(T))) cache_write_kernel<T, CODE, true><<<grid, threads, 0, st>>>(c, t);
+  else cache_write_kernel<T, CODE, false><<<grid, threads, 0, st>>>(c, t);
+  count_launch();
+  return cudaGetLastError();
+}
+
+template <typename T, int CODE>
+cudaError_t read_t(const CacheArgs& c, const CacheTokens& t, cudaStream_t st) {
+  const dim3 grid((unsigned)((t.L + kReadTokens - 2) / kReadTokens + 1), 2 * c.B);   // aligned sixteens that L tokens touch
+  if (vectors(t, sizeof(T))) cache_read_kernel<T, CODE, true><<<grid, 256, 0, st>>>(c, t);
+  else cache_read_kernel<T, CODE, false><<<grid, 256, 0, st>>>(c, t);
   count_launch();
   return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t read_t(const CacheArgs& c, const CacheTokens& t, cudaStream_t st) {
-  const long long items = (long long)t.L * (c.row / 16);
-  const dim3 grid((unsigned)((items + 255) / 256), 2, c.B);
-  if (c.code == NNLIB_B200_INT8) cache_read_kernel<T, NNLIB_B200_INT8><<<grid, 256, 0, st>>>(c, t);
-  else cache_read_kernel<T, NNLIB_B200_E4M3><<<grid, 256, 0, st>>>(c, t);
-  count_launch();
-  return cudaGetLastError();
+cudaError_t move_t(const CacheArgs& c, const CacheTokens& t, bool in, cudaStream_t st) {
+  if (c.code == NNLIB_B200_INT8) return in ? write_t<T, NNLIB_B200_INT8>(c, t, st) : read_t<T, NNLIB_B200_INT8>(c, t, st);
+  return in ? write_t<T, NNLIB_B200_E4M3>(c, t, st) : read_t<T, NNLIB_B200_E4M3>(c, t, st);
+}
+
+cudaError_t move(const CacheArgs& c, const CacheTokens& t, int dtype, bool in, cudaStream_t st) {
+  if (dtype == NNLIB_B200_F16) return move_t<__half>(c, t, in, st);
+  if (dtype == NNLIB_B200_BF16) return move_t<__nv_bfloat16>(c, t, in, st);
+  return move_t<float>(c, t, in, st);
 }
 
 }  // namespace
 
-cudaError_t cache_write(const CacheArgs& c, const CacheTokens& t, int dtype, cudaStream_t st) {
-  if (dtype == NNLIB_B200_F16) return write_t<__half>(c, t, st);
-  if (dtype == NNLIB_B200_BF16) return write_t<__nv_bfloat16>(c, t, st);
-  return write_t<float>(c, t, st);
-}
-
-cudaError_t cache_read(const CacheArgs& c, const CacheTokens& t, int dtype, cudaStream_t st) {
-  if (dtype == NNLIB_B200_F16) return read_t<__half>(c, t, st);
-  if (dtype == NNLIB_B200_BF16) return read_t<__nv_bfloat16>(c, t, st);
-  return read_t<float>(c, t, st);
-}
+cudaError_t cache_write(const CacheArgs& c, const CacheTokens& t, int dtype, cudaStream_t st) { return move(c, t, dtype, true, st); }
+cudaError_t cache_read(const CacheArgs& c, const CacheTokens& t, int dtype, cudaStream_t st) { return move(c, t, dtype, false, st); }
 
 }  // namespace nb200

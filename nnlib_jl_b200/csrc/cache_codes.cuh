@@ -1,8 +1,6 @@
 // The 8-bit cache's pages, scales and codes (nnlib_b200.h), as its kernels see them.
 #pragma once
 
-#include <cuda_fp8.h>
-
 #include "common.cuh"
 #include "launchers.h"
 
@@ -33,20 +31,45 @@ __device__ __forceinline__ float block_scale(float amax) {
   return (amax > 0.f && s >= kScaleTiny) ? s : 0.f;
 }
 
-// x / scale, given 1 / scale (0 for the scales 0 and NaN), as a code's bits
+// Four x / scale as codes, given 1 / scale (0 for the scales 0 and NaN: then all codes are 0, also of an x that is not
+// finite).  Int8: rounded by adding 1.5 * 2^23, whose last byte is then the code (the conversion instruction runs at a
+// quarter of the rate).
 template <int CODE>
-__device__ __forceinline__ unsigned int to_code(float x, float inv) {
-  const float t = x * inv;
-  if (CODE == NNLIB_B200_INT8) return (unsigned int)__float2int_rn(fminf(fmaxf(t, -127.f), 127.f)) & 0xffu;
-  return __nv_cvt_float_to_fp8(t, __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ uint32_t to_codes4(float a, float b, float c, float d, float inv) {
+  if (inv == 0.f) return 0u;
+  if (CODE == NNLIB_B200_INT8) {
+    auto bits = [&](float x) { return __float_as_uint(__fadd_rn(fminf(fmaxf(__fmul_rn(x, inv), -127.f), 127.f), 12582912.f)); };
+    return __byte_perm(__byte_perm(bits(a), bits(b), 0x0040u), __byte_perm(bits(c), bits(d), 0x0040u), 0x5410u);
+  }
+  auto pair = [&](float x, float y) {
+    unsigned short r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(__fmul_rn(y, inv)), "f"(__fmul_rn(x, inv)));
+    return (uint32_t)r;
+  };
+  return pair(a, b) | (pair(c, d) << 16);
 }
-// (a product with 0 that is NaN, from an infinity in a block whose scale is NaN, becomes code 0)
-__device__ __forceinline__ float code_input(float x, float inv) { return inv == 0.f ? 0.f : x; }
 
+// the four numbers that the codes of a word are
 template <int CODE>
-__device__ __forceinline__ float from_code(unsigned int bits) {
-  if (CODE == NNLIB_B200_INT8) return (float)(signed char)(bits & 0xffu);
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)(bits & 0xffu), __NV_E4M3)));
+__device__ __forceinline__ void from_codes4(uint32_t w, float (&f)[4]) {
+  if (CODE == NNLIB_B200_INT8) {
+    // code + 128 as the last byte of 2^23
+    const uint32_t u = w ^ 0x80808080u;
+    f[0] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440u)) - 8388736.f;
+    f[1] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441u)) - 8388736.f;
+    f[2] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442u)) - 8388736.f;
+    f[3] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443u)) - 8388736.f;
+  } else {
+    uint32_t lo, hi;
+    asm("{ .reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b; }" : "=r"(lo), "=r"(hi) : "r"(w));
+    __half2 h;
+    memcpy(&h, &lo, 4);
+    f[0] = __low2float(h);
+    f[1] = __high2float(h);
+    memcpy(&h, &hi, 4);
+    f[2] = __low2float(h);
+    f[3] = __high2float(h);
+  }
 }
 
 __device__ __forceinline__ float inverse_scale(float s) { return s > 0.f ? __fdiv_rn(1.f, s) : 0.f; }

@@ -110,6 +110,7 @@ struct NormRopeSide {
   void* dg;
   long long sl, sb, dsl, dsb;
   int heads;
+  int chunk;                 // filled in by the launcher: heads that a warp takes of a token
 };
 struct NormRopeArgs {
   NormRopeSide side[2];
@@ -122,7 +123,7 @@ struct NormRopeArgs {
   float* ws;                 // pullback: d floats for each block
   float eps;
   int d, rot, L, interleaved, wdtype;
-  int lanes, tok, blocks_q;  // filled in by the launcher
+  int lanes, blocks_q;       // filled in by the launcher
 };
 size_t norm_rope_workspace_bytes(NormRopeArgs a, int esize);
 cudaError_t norm_rope(NormRopeArgs a, int dtype, bool bwd, cudaStream_t st);
