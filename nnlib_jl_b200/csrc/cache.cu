@@ -1,11 +1,13 @@
 // Tokens into and out of the 8-bit key / value cache (nnlib_b200.h: pages, scales, codes).
 //
-// Both are bound by HBM: an element is two bytes (or four) on one side and one on the other.
+// Both are bound by HBM: an element is two bytes (or four) on one side and one on the other.  (32768 bf16 tokens of 8 heads of
+// 128 into pages of 64: written in 36 us, 5.5 TB/s, read back in 40 us, 5.0 TB/s.  More in flight to a thread, half the
+// blocks: 46 and 49.)
 // Write: one block for a page that a sequence's new tokens touch, a head, and keys or values.  It is the only one that
 // touches this page's scale and codes of this head, so there is nothing to order: it finds the new tokens' largest
 // magnitude, settles the scale, rounds the older codes anew where the scale has grown, and writes the new ones.  A thread
-// works on 16 elements at a time, one 16-byte store of codes, and keeps the first HELD such pieces in registers between
-// the two steps; blocks of more (pages of more than 8192 elements of a head) read the rest again, from L2.
+// works on 16 bytes of elements at a time and keeps the first kHeld such pieces in registers between the two steps; blocks
+// of more (pages of more than 16384 16-bit elements of a head) read the rest again, from L2.
 // Read: eight codes to a thread and store, so that a warp's stores of 16-bit results are whole lines.
 #include <algorithm>
 
@@ -14,47 +16,53 @@
 namespace nb200 {
 namespace {
 
-constexpr int kHeld = 2;
+constexpr int kHeld = 8;                  // pieces of 16 bytes that a thread keeps
 
-// 16 elements; VEC: 16-byte loads
+// 16 bytes of elements; VEC: in one load
 template <typename T, bool VEC>
-__device__ __forceinline__ void load16(const T* p, T (&v)[16]) {
-  if constexpr (VEC) {
+__device__ __forceinline__ uint4 load_piece(const T* p) {
+  if constexpr (VEC) return __ldcs(reinterpret_cast<const uint4*>(p));
+  uint32_t w[4];
+  if constexpr (sizeof(T) == 2) {
+    const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(v) / 16; ++i) {
-      const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(p) + i);
-      memcpy(reinterpret_cast<char*>(v) + 16 * i, &raw, 16);
-    }
+    for (int i = 0; i < 4; ++i) w[i] = q[2 * i] | ((uint32_t)q[2 * i + 1] << 16);
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = p[i];
+    for (int i = 0; i < 4; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The largest magnitude so far, as bits: of Float32, or two by two of 16-bit numbers.  As whole numbers magnitudes keep their
+// order, and a NaN is larger than all others.
+template <typename T>
+__device__ __forceinline__ uint32_t magnitude(uint32_t top, const uint4& v) {
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t m = 0x7fff7fffu;
+    return __vmaxu2(top, __vmaxu2(__vmaxu2(v.x & m, v.y & m), __vmaxu2(v.z & m, v.w & m)));
+  } else {
+    const uint32_t m = 0x7fffffffu;
+    return max(top, max(max(v.x & m, v.y & m), max(v.z & m, v.w & m)));
   }
 }
 
-// The largest magnitude of 16 elements and what came before, as bits: a NaN is larger than all others.
-__device__ __forceinline__ uint32_t magnitude(uint32_t top, const float (&v)[16]) {
-#pragma unroll
-  for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
-  return top;
+__device__ __forceinline__ float2 two_floats(uint32_t w, __nv_bfloat16) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
-template <typename T2, typename T>
-__device__ __forceinline__ uint32_t magnitude16(uint32_t top, const T (&v)[16]) {
-  T2 m[8];
-  memcpy(m, v, sizeof(m));
-#pragma unroll
-  for (int e = 0; e < 8; ++e) m[e] = __habs2(m[e]);
-#pragma unroll
-  for (int n = 4; n > 0; n >>= 1)
-#pragma unroll
-    for (int e = 0; e < n; ++e) m[e] = __hmax2_nan(m[e], m[e + n]);
-  const float lo = __low2float(m[0]), hi = __high2float(m[0]);
-  return max(top, max(__float_as_uint(lo) & 0x7fffffffu, __float_as_uint(hi) & 0x7fffffffu));
+__device__ __forceinline__ float2 two_floats(uint32_t w, __half) {
+  __half2 h;
+  memcpy(&h, &w, 4);
+  return __half22float2(h);
 }
-__device__ __forceinline__ uint32_t magnitude(uint32_t top, const __half (&v)[16]) { return magnitude16<__half2>(top, v); }
-__device__ __forceinline__ uint32_t magnitude(uint32_t top, const __nv_bfloat16 (&v)[16]) { return magnitude16<__nv_bfloat162>(top, v); }
+
+// (an argument indexed by a number that is not a constant would be copied to local memory whole)
+template <typename X>
+__device__ __forceinline__ X pick(const X (&v)[2], int kv) { return kv ? v[1] : v[0]; }
 
 template <typename T, int CODE, bool VEC>
-__global__ void __launch_bounds__(256, 4) cache_write_kernel(const CacheArgs c, const CacheTokens t) {
+__global__ void __launch_bounds__(256, 3) cache_write_kernel(const CacheArgs c, const CacheTokens t) {
+  constexpr int U = 16 / sizeof(T);        // elements of a piece: as many bytes of codes
   __shared__ uint32_t sm[8];
   // heads side by side: what runs at one time reads whole tokens
   const int h = blockIdx.x % c.H, kv = (blockIdx.x / c.H) & 1, b = blockIdx.y, tid = threadIdx.x, nt = blockDim.x;
@@ -66,29 +74,39 @@ __global__ void __launch_bounds__(256, 4) cache_write_kernel(const CacheArgs c, 
   const long long lo = max(start, p << c.log_page), hi = min(start + n_new, (p + 1) << c.log_page);
   if (lo >= hi) return;
   const int fill = (int)(lo - (p << c.log_page));                      // older tokens of the page
-  const unsigned pieces = c.d / 16, n = (unsigned)(hi - lo) * pieces;  // new ones, in pieces
-  const long long sl = t.sl[kv];
-  const T* x = reinterpret_cast<const T*>(t.x[kv]) + (lo - start) * sl + b * t.sb[kv] + (long long)h * c.d;
-  auto source = [&](unsigned i) { return x + (long long)(i / pieces) * sl + (i % pieces) * 16; };
+  const unsigned pieces = c.d / U, n = (unsigned)(hi - lo) * pieces;   // new ones, in pieces
+  const long long sl = pick(t.sl, kv);
+  const T* x = reinterpret_cast<const T*>(pick(t.x, kv)) + (lo - start) * sl + b * pick(t.sb, kv) + (long long)h * c.d;
+  // where pieces tid, tid + nt, ... are: token, piece of the token
+  const unsigned l0 = tid / pieces, e0 = tid - l0 * pieces, dl = nt / pieces, de = nt - dl * pieces;
+  auto advance = [&](unsigned& l, unsigned& e) {
+    l += dl;
+    e += de;
+    if (e >= pieces) e -= pieces, ++l;
+  };
+  auto source = [&](unsigned l, unsigned e) { return x + (long long)l * sl + e * U; };
 
-  T held[kHeld][16];
+  uint4 held[kHeld];
+  unsigned l = l0, e = e0;
 #pragma unroll
-  for (int r = 0; r < kHeld; ++r)
-    if (tid + r * nt < n) load16<T, VEC>(source(tid + r * nt), held[r]);
+  for (int r = 0; r < kHeld; ++r) {
+    held[r] = make_uint4(0u, 0u, 0u, 0u);
+    if (tid + r * nt < n) held[r] = load_piece<T, VEC>(source(l, e));
+    advance(l, e);
+  }
   const long long page = cache_page(c, b, p);
   if (page < 0) return;
-  unsigned char* codes = c.codes[kv] + (page << c.log_page) * c.row + (long long)h * c.d;
-  float* scale = c.scale[kv] + page * c.H + h;
+  unsigned char* codes = pick(c.codes, kv) + (page << c.log_page) * c.row + (long long)h * c.d;
+  float* scale = pick(c.scale, kv) + page * c.H + h;
   const float old = fill > 0 ? *scale : 0.f;
 
   uint32_t top = 0u;
 #pragma unroll
-  for (int r = 0; r < kHeld; ++r)
-    if (tid + r * nt < n) top = magnitude(top, held[r]);
-  for (unsigned i = tid + kHeld * nt; i < n; i += nt) {
-    T v[16];
-    load16<T, VEC>(source(i), v);
-    top = magnitude(top, v);
+  for (int r = 0; r < kHeld; ++r) top = magnitude<T>(top, held[r]);
+  for (unsigned i = tid + kHeld * nt; i < n; i += nt, advance(l, e)) top = magnitude<T>(top, load_piece<T, VEC>(source(l, e)));
+  if constexpr (sizeof(T) == 2) {
+    top = max(top >> 16, top & 0xffffu);
+    top = __float_as_uint(two_floats(top, T()).x);
   }
   top = __reduce_max_sync(0xffffffffu, top);
   if (nt > 32) {
@@ -101,9 +119,10 @@ __global__ void __launch_bounds__(256, 4) cache_write_kernel(const CacheArgs c, 
   const float s = (old != old || asked != asked) ? __int_as_float(0x7fc00000) : fmaxf(old, asked);
   const float inv = inverse_scale(s);
   if (fill > 0 && s > old) {
-    const float f = __fdiv_rn(old, s);
-    for (unsigned i = tid; i < fill * pieces; i += nt) {
-      uint4* q = reinterpret_cast<uint4*>(codes + (long long)(i / pieces) * c.row + (i % pieces) * 16);
+    const float f = __fdiv_rn(old, s);               // (0 where the older codes are all 0)
+    const unsigned per = c.d / 16;
+    for (unsigned i = tid; i < fill * per; i += nt) {
+      uint4* q = reinterpret_cast<uint4*>(codes + (long long)(i / per) * c.row + (i % per) * 16);
       uint4 v = *q;
       auto again = [&](uint32_t w) {
         float g[4];
@@ -113,21 +132,30 @@ __global__ void __launch_bounds__(256, 4) cache_write_kernel(const CacheArgs c, 
       *q = make_uint4(again(v.x), again(v.y), again(v.z), again(v.w));
     }
   }
-  auto quantise = [&](unsigned i, const T (&v)[16]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      w[e] = to_codes4<CODE>(Elem<T>::to_f(v[4 * e]), Elem<T>::to_f(v[4 * e + 1]), Elem<T>::to_f(v[4 * e + 2]), Elem<T>::to_f(v[4 * e + 3]), inv);
-    *reinterpret_cast<uint4*>(codes + (long long)(fill + i / pieces) * c.row + (i % pieces) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+  unsigned char* to0 = codes + (long long)fill * c.row;
+  auto quantise = [&](const uint4& v) {
+    unsigned char* to = to0 + (long long)l * c.row + e * U;
+    if constexpr (sizeof(T) == 2) {
+      const float2 a = two_floats(v.x, T()), b2 = two_floats(v.y, T()), c2 = two_floats(v.z, T()), d2 = two_floats(v.w, T());
+      *reinterpret_cast<uint2*>(to) = make_uint2(to_codes4<CODE>(a.x, a.y, b2.x, b2.y, inv), to_codes4<CODE>(c2.x, c2.y, d2.x, d2.y, inv));
+    } else {
+      *reinterpret_cast<uint32_t*>(to) = to_codes4<CODE>(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w), inv);
+    }
   };
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  if (inv == 0.f) {                      // a scale of 0 or NaN: all codes are 0, also of what is not finite
 #pragma unroll
-  for (int r = 0; r < kHeld; ++r)
-    if (tid + r * nt < n) quantise(tid + r * nt, held[r]);
-  for (unsigned i = tid + kHeld * nt; i < n; i += nt) {
-    T v[16];
-    load16<T, VEC>(source(i), v);
-    quantise(i, v);
+    for (int r = 0; r < kHeld; ++r) held[r] = zero;
   }
+  l = l0;
+  e = e0;
+#pragma unroll
+  for (int r = 0; r < kHeld; ++r) {
+    if (tid + r * nt < n) quantise(held[r]);
+    advance(l, e);
+  }
+  for (unsigned i = tid + kHeld * nt; i < n; i += nt, advance(l, e))
+    quantise(inv == 0.f ? zero : load_piece<T, VEC>(source(l, e)));
   // (every thread has read the old scale: it came before the barrier, or the block is one warp)
   if (tid == 0) *scale = s;
 }
@@ -146,13 +174,15 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const CacheArgs c, cons
   const long long cap = c.rows << c.log_page, end = t.lens ? min(cap, (long long)t.lens[b]) : cap;
   const bool inside = lo >= 0 && lo < end;
   const long long page = inside ? cache_page(c, b, lo >> c.log_page) : -1;
-  const unsigned char* codes = c.codes[kv] + (page < 0 ? 0 : ((page << c.log_page) + (lo & ((1 << c.log_page) - 1))) * c.row);
-  T* y = reinterpret_cast<T*>(t.x[kv]) + (lo - start) * t.sl[kv] + b * t.sb[kv];
+  const unsigned char* codes = pick(c.codes, kv) + (page < 0 ? 0 : ((page << c.log_page) + (lo & ((1 << c.log_page) - 1))) * c.row);
+  T* y = reinterpret_cast<T*>(pick(t.x, kv)) + (lo - start) * pick(t.sl, kv) + b * pick(t.sb, kv);
+  const float* scale = pick(c.scale, kv);
+  const long long sl_y = pick(t.sl, kv);
   const int n = (int)(hi - lo), n_in = inside ? (int)min((long long)n, end - lo) : 0;
   if (first >= rows) return;
   for (int part = col; part < parts; part += width) {
     float s = __int_as_float(0x7fc00000);
-    if (page >= 0) s = c.scale[kv][page * c.H + part * 8 / c.d];
+    if (page >= 0) s = scale[page * c.H + part * 8 / c.d];
 #pragma unroll 4
     for (int l = first; l < n; l += rows) {
       uint2 raw = make_uint2(0u, 0u);
@@ -172,7 +202,7 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const CacheArgs c, cons
       T out[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) out[e] = Elem<T>::from_f(f[e]);
-      T* to = y + l * t.sl[kv] + part * 8;
+      T* to = y + l * sl_y + part * 8;
       if constexpr (VEC) {
 #pragma unroll
         for (int e = 0; e < (int)sizeof(out) / 16; ++e) {
@@ -201,7 +231,7 @@ cudaError_t write_t(const CacheArgs& c, const CacheTokens& t, cudaStream_t st) {
   const long long pages = std::min<long long>((t.L + T_ - 2) / T_ + 1, c.rows);    // that L tokens can touch
   if (pages * 2 * c.H > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   const dim3 grid((unsigned)(pages * 2 * c.H), c.B);
-  const int pieces = std::min(t.L, T_) * (c.d / 16);
+  const int pieces = std::min(t.L, T_) * c.d / (16 / (int)sizeof(T));
   const int threads = std::min(256, std::max(32, (pieces / kHeld + 31) & ~31));
   if (vectors(t, sizeof(T))) cache_write_kernel<T, CODE, true><<<grid, threads, 0, st>>>(c, t);
   else cache_write_kernel<T, CODE, false><<<grid, threads, 0, st>>>(c, t);

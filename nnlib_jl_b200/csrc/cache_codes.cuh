@@ -31,14 +31,13 @@ __device__ __forceinline__ float block_scale(float amax) {
   return (amax > 0.f && s >= kScaleTiny) ? s : 0.f;
 }
 
-// Four x / scale as codes, given 1 / scale (0 for the scales 0 and NaN: then all codes are 0, also of an x that is not
-// finite).  Int8: rounded by adding 1.5 * 2^23, whose last byte is then the code (the conversion instruction runs at a
-// quarter of the rate).
+// Four x / scale as codes, given 1 / scale.  No x is larger than 127 or 448 scales but for the rounding of the inverse, less
+// than half a code.  Int8: rounded by adding 1.5 * 2^23, whose last byte is then the code (the conversion instruction runs
+// at a quarter of the rate).
 template <int CODE>
 __device__ __forceinline__ uint32_t to_codes4(float a, float b, float c, float d, float inv) {
-  if (inv == 0.f) return 0u;
   if (CODE == NNLIB_B200_INT8) {
-    auto bits = [&](float x) { return __float_as_uint(__fadd_rn(fminf(fmaxf(__fmul_rn(x, inv), -127.f), 127.f), 12582912.f)); };
+    auto bits = [&](float x) { return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.f)); };
     return __byte_perm(__byte_perm(bits(a), bits(b), 0x0040u), __byte_perm(bits(c), bits(d), 0x0040u), 0x5410u);
   }
   auto pair = [&](float x, float y) {
