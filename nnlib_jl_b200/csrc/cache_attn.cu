@@ -10,14 +10,16 @@
 // weights keep 11 bits down to 2^-28 of the largest.  Float32 arrays: q and w as the sum of two 16-bit terms each.
 //
 // HBM is the bound (2 d bytes per key and head for up to 16 rows), so what counts is bytes in flight: nothing is staged,
-// a warp streams 16 keys at a time straight into the fragments of m16n8k16 products.  Rows of a tile: the query heads of
-// a group and the queries, row r = query r / G, head r % G of the group.
-//   S: lane (g, c) = (lane / 4, lane % 4) takes 16 consecutive features 64 G + 16 c .. of key g: word t of its 16 bytes is
-//      what it owes to k-step t, two codes to each register; Q's fragments are loaded in the same order.
-//   O: columns may be any features: column g of product j is feature g * (D/8) + j, so a lane loads D/8 consecutive bytes
-//      of each of its four keys 2c, 2c+1, 2c+8, 2c+9 and pairs the codes of two keys up.
+// a warp streams 16 keys at a time straight into the fragments of m16n8k16 products.  Keys and the features of values are
+// the products' sixteen rows, queries their eight columns, so that one query costs half of what it would as a row:
+//   S^T = K Q^T   lane (g, c) = (lane / 4, lane % 4) takes 16 consecutive features 64 G + 16 c .. of keys g and g + 8: word t
+//                 of 16 bytes is what it owes to k-step t, two codes to each register; Q's fragments in the same order.
+//   O^T += V^T W^T  rows may be any features: rows g and g + 8 of product j are features g (D/8) + 2j and the next, so a lane
+//                 loads D/8 consecutive bytes of each of its four keys 2c, 2c+1, 2c+8, 2c+9 and pairs the codes of two keys
+//                 up.  W^T comes from S^T's layout by transposing 8 x 8 blocks.
+// Columns: the query heads of a group and the queries, column r = query r / G, head r % G of the group; NT blocks of eight.
 // Int8 to 16 bits: (code ^ 0x80) under 0x64 is 1024 + 128 + code, less 1152.  E4M3: the conversion instruction.
-// A unit's keys (sequence, cache head, row tile) are dealt to `splits` blocks in equal runs of 64; the four warps of a
+// A unit's keys (sequence, cache head, tile of columns) are dealt to `splits` blocks in equal runs of 64; the four warps of a
 // block alternate.  attn_split_reduce_kernel merges the blocks' running maxima, sums and outputs.
 #include <algorithm>
 #include <cmath>
@@ -77,17 +79,15 @@ __device__ __forceinline__ void word_pairs(uint32_t w, uint32_t& p0, uint32_t& p
   }
 }
 
-template <bool ROWS8>
-__device__ __forceinline__ void mma(float (&c)[ROWS8 ? 2 : 4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                    uint32_t b0, uint32_t b1) {
-  if constexpr (ROWS8) {
-    float u, v;
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %10, %10};"
-        : "+f"(c[0]), "+f"(c[1]), "=f"(u), "=f"(v) : "r"(a0), "r"(0u), "r"(a2), "r"(0u), "r"(b0), "r"(b1), "f"(0.f));
-  } else {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// an 8 x 8 block of 16-bit values: row i / columns 2j, 2j + 1 in lane 4i + j becomes column i / rows 2j, 2j + 1
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 
 // BYTES codes of a lane, as words
@@ -119,14 +119,15 @@ __device__ __forceinline__ int last_key(const CacheAttnArgs& a, long long start,
   return e < 0 ? -1 : (e < len ? (int)e : len - 1);
 }
 
-template <int D, bool ROWS8> struct Cfg { static constexpr int kCtas = D <= 64 ? 4 : (D <= 128 ? (ROWS8 ? 4 : 3) : 2); };
+// blocks of an SM: what registers allow without spilling the codes in flight
+template <typename T, int D, int NT> struct Cfg { static constexpr int kCtas = D <= 64 ? 4 : (D <= 128 ? (sizeof(T) == 4 || NT == 2 ? 3 : 4) : 2); };
 
 // T: element type of q and x; HILO: two 16-bit terms for an element of q and for a weight (T = float)
-template <typename T, int D, int CODE, bool ROWS8>
-__global__ void __launch_bounds__(kWarps * 32, Cfg<D, ROWS8>::kCtas)
-cache_attn_kernel(const CacheAttnArgs a, const int splits) {
+template <typename T, int D, int CODE, int NT>
+__global__ void __launch_bounds__(kWarps * 32, Cfg<T, D, NT>::kCtas)
+cache_attn_kernel(const CacheAttnArgs a, const int splits, const int vec) {
   constexpr bool HILO = sizeof(T) == 4;
-  constexpr int R = ROWS8 ? 1 : 2, ROWS = 8 * R, KS = D / 16, GK = D / 64, VB = D / 8;
+  constexpr int ROWS = 8 * NT, KS = D / 16, GK = D / 64, VB = D / 8, HL = HILO ? 2 : 1;
   __shared__ float sm_o[kWarps][ROWS][D];
   __shared__ float sm_m[kWarps][ROWS], sm_l[kWarps][ROWS];
   const CacheArgs& cc = a.c;
@@ -146,49 +147,8 @@ cache_attn_kernel(const CacheAttnArgs a, const int splits) {
   // this block's keys: whole groups of 64
   const int groups = (kend + 63) / 64, share = (groups + splits - 1) / splits;
   const int key_lo = min(split * share, groups) * 64, key_hi = min(min((split + 1) * share, groups) * 64, kend);
-  const unsigned char* kbase = cc.codes[0] + (long long)h * cc.d;
-  const unsigned char* vbase = cc.codes[1] + (long long)h * cc.d;
-
-  // Q's fragments, brought to a largest element in [2^13, 2^14)
-  uint32_t qa[R][KS][2], qlo[HILO ? R : 1][HILO ? KS : 1][2];
-  float crow[R];                               // what a row's products are multiplied by, but for the page's scale
-  int lim[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int row = row0 + g + 8 * r, i = row / G, hq = h * G + row % G;
-    const bool live = row < rows;
-    lim[r] = live ? last_key(a, start, i, len) : -1;
-    const T* qp = reinterpret_cast<const T*>(a.q) + (live ? (long long)i * a.q_sl + (long long)b * a.q_sb + (long long)hq * cc.d : 0);
-    float top = 0.f;
-#pragma unroll
-    for (int G4 = 0; G4 < GK; ++G4)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int f = 64 * G4 + 16 * c + e;
-        if (live && f < cc.d) top = fmaxf(top, fabsf(Elem<T>::to_f(qp[f])));
-      }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const int ex = (top > 0.f && top <= 3.402823466e38f) ? 13 - ilogbf(top) : 0;
-    crow[r] = scalbnf(a.scale * kLog2e, -ex);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      float v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int f = 64 * (ks / 4) + 16 * c + 4 * (ks % 4) + e;
-        v[e] = (live && f < cc.d) ? scalbnf(Elem<T>::to_f(qp[f]), ex) : 0.f;
-      }
-      qa[r][ks][0] = half2_bits(v[0], v[1]);
-      qa[r][ks][1] = half2_bits(v[2], v[3]);
-      if constexpr (HILO) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] -= __half2float(__float2half_rn(v[e]));
-        qlo[r][ks][0] = half2_bits(v[0], v[1]);
-        qlo[r][ks][1] = half2_bits(v[2], v[3]);
-      }
-    }
-  }
+  const unsigned char* kbase = cc.codes[0] + (long long)h * cc.d + 16 * c;
+  const unsigned char* vbase = cc.codes[1] + (long long)h * cc.d + VB * g;
 
   // Pages, 32 of a warp's steps at a time: lane n looks up step n's page and scales
   int pg = 0;
@@ -201,21 +161,20 @@ cache_attn_kernel(const CacheAttnArgs a, const int splits) {
     vsc = page < 0 ? qnan() : cc.scale[1][page * cc.H + h];
   };
   uint32_t kf[2][GK][4], vf[4][VB / 4];
+  const int T1 = (1 << cc.log_page) - 1;
   auto load_k = [&](int key0, int page) {
-    const long long slot = ((long long)page << cc.log_page) + (key0 & ((1 << cc.log_page) - 1));
+    const unsigned char* p = kbase + (((long long)page << cc.log_page) + (key0 & T1) + g) * cc.row;
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-      for (int G4 = 0; G4 < GK; ++G4) {
-        const int f = 64 * G4 + 16 * c;
-        if (f < cc.d) load_codes<16>(kbase + (slot + nt * 8 + g) * cc.row + f, kf[nt][G4]);
-      }
+      for (int G4 = 0; G4 < GK; ++G4)
+        if (64 * G4 + 16 * c < cc.d) load_codes<16>(p + nt * 8 * cc.row + 64 * G4, kf[nt][G4]);
   };
   auto load_v = [&](int key0, int page) {
-    const long long slot = ((long long)page << cc.log_page) + (key0 & ((1 << cc.log_page) - 1));
+    const unsigned char* p = vbase + (((long long)page << cc.log_page) + (key0 & T1) + 2 * c) * cc.row;
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (VB * g < cc.d) load_codes<VB>(vbase + (slot + 2 * c + (u & 1) + (u >> 1) * 8) * cc.row + VB * g, vf[u]);
+      if (VB * g < cc.d) load_codes<VB>(p + ((u & 1) + (u >> 1) * 8) * cc.row, vf[u]);
   };
 #pragma unroll
   for (int nt = 0; nt < 2; ++nt)
@@ -227,85 +186,163 @@ cache_attn_kernel(const CacheAttnArgs a, const int splits) {
   for (int u = 0; u < 4; ++u)
 #pragma unroll
     for (int w = 0; w < VB / 4; ++w) vf[u][w] = 0u;
-
-  float m[R], l[R], o[D / 8][2 * R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) m[r] = ninf(), l[r] = 0.f;
-#pragma unroll
-  for (int j = 0; j < D / 8; ++j)
-#pragma unroll
-    for (int e = 0; e < 2 * R; ++e) o[j][e] = 0.f;
-
   const int stride = kWarps * kStep;
   int key0 = key_lo + warp * kStep;
+  // the first keys are on their way while Q is prepared
   if (key0 < key_hi) {
     look_up(key0 + lane * stride);
     const int page = __shfl_sync(0xffffffffu, pg, 0);
     load_k(key0, page);
     load_v(key0, page);
   }
+
+  // Q's fragments, brought to a largest element in [2^13, 2^14)
+  uint32_t qb[NT][HL][KS][2];
+  float crow[NT][2];                           // what a column's products are multiplied by, but for the page's scale
+  int lim[NT][2];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int row = row0 + 8 * t + g, i = row / G, hq = h * G + row % G;
+    const bool live = row < rows;
+    const T* qp = reinterpret_cast<const T*>(a.q) + (live ? (long long)i * a.q_sl + (long long)b * a.q_sb + (long long)hq * cc.d : 0) + 16 * c;
+    float top = 0.f, q[GK][16];
+#pragma unroll
+    for (int G4 = 0; G4 < GK; ++G4) {
+      if (live && 64 * G4 + 16 * c < cc.d) {
+        if (vec) {
+#pragma unroll
+          for (int w = 0; w < (int)sizeof(T); ++w) {
+            constexpr int U = 16 / sizeof(T);
+            const uint4 raw = __ldg(reinterpret_cast<const uint4*>(qp + 64 * G4) + w);
+            T e[U];
+            memcpy(e, &raw, 16);
+#pragma unroll
+            for (int u = 0; u < U; ++u) q[G4][w * U + u] = Elem<T>::to_f(e[u]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) q[G4][e] = Elem<T>::to_f(qp[64 * G4 + e]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) q[G4][e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(q[G4][e]));
+    }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int ex = (top > 0.f && top <= 3.402823466e38f) ? 13 - ilogbf(top) : 0;
+    const float cr = scalbnf(a.scale * kLog2e, -ex);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      crow[t][u] = __shfl_sync(0xffffffffu, cr, 4 * (2 * c + u));
+      const int mine = row0 + 8 * t + 2 * c + u;
+      lim[t][u] = mine < rows ? last_key(a, start, mine / G, len) : -1;
+    }
+    // a power of two in two factors, each a normal number
+    const float fa = scalbnf(1.f, ex / 2), fb = scalbnf(1.f, ex - ex / 2);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = q[ks / 4][4 * (ks % 4) + e] * fa * fb;
+      qb[t][0][ks][0] = half2_bits(v[0], v[1]);
+      qb[t][0][ks][1] = half2_bits(v[2], v[3]);
+      if constexpr (HILO) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] -= __half2float(__float2half_rn(v[e]));
+        qb[t][1][ks][0] = half2_bits(v[0], v[1]);
+        qb[t][1][ks][1] = half2_bits(v[2], v[3]);
+      }
+    }
+  }
+
+  float m[NT][2], l[NT][2], o[NT][D / 16][4];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) m[t][u] = ninf(), l[t][u] = 0.f;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[t][j][e] = 0.f;
+  }
+
   for (int n = 0; key0 < key_hi; key0 += stride, ++n) {
     const float ks = __shfl_sync(0xffffffffu, ksc, n & 31), vs = __shfl_sync(0xffffffffu, vsc, n & 31);
     const int next = key0 + stride;
     if ((n & 31) == 31 && next < key_hi) look_up(next + lane * stride);
     const int page = __shfl_sync(0xffffffffu, pg, (n + 1) & 31);
 
-    float sc[2][2 * R];
+    // (two chains of sums)
+    float sc[NT][4], sd[NT][4];
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int e = 0; e < 2 * R; ++e) sc[nt][e] = 0.f;
+      for (int e = 0; e < 4; ++e) sc[t][e] = sd[t][e] = 0.f;
 #pragma unroll
-      for (int k2 = 0; k2 < KS; ++k2) {
-        uint32_t b0, b1;
-        word_pairs<CODE>(kf[nt][k2 / 4][k2 % 4], b0, b1);
-        mma<ROWS8>(sc[nt], qa[0][k2][0], qa[R - 1][k2][0], qa[0][k2][1], qa[R - 1][k2][1], b0, b1);
-        if constexpr (HILO) mma<ROWS8>(sc[nt], qlo[0][k2][0], qlo[R - 1][k2][0], qlo[0][k2][1], qlo[R - 1][k2][1], b0, b1);
-      }
+    for (int k2 = 0; k2 < KS; ++k2) {
+      uint32_t a0, a1, a2, a3;
+      word_pairs<CODE>(kf[0][k2 / 4][k2 % 4], a0, a2);
+      word_pairs<CODE>(kf[1][k2 / 4][k2 % 4], a1, a3);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int hl = 0; hl < HL; ++hl) mma(k2 & 1 ? sd[t] : sc[t], a0, a1, a2, a3, qb[t][hl][k2][0], qb[t][hl][k2][1]);
     }
     if (next < key_hi) load_k(next, page);
 
     // scales of this step's page (16 keys never cross one)
     const float vse = vs >= kValueFloor ? vs : ((vs >= 0.f) ? kValueFloor : qnan());
-    const float lvs = log2f(vse) + kWeightBits, ivs = __fdiv_rn(1.f, vse);
-    uint32_t pa[R][2], plo[HILO ? R : 1][2];
+    const float lvs = __log2f(vse) + kWeightBits, ivs = __fdividef(1.f, vse);
+    uint32_t pb[NT][HL][2];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const float f = crow[r] * ks;
-      float t[4];
+    for (int t = 0; t < NT; ++t) {
+      // w[e]: key g (+ 8 for e >= 2), column 2c (+ 1 for odd e)
+      float w[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        t[u] = fmaf(sc[u >> 1][2 * r + (u & 1)], f, lvs);
-        if (key0 + 2 * c + (u & 1) + (u >> 1) * 8 > lim[r]) t[u] = ninf();
+      for (int e = 0; e < 4; ++e) {
+        w[e] = fmaf(sc[t][e] + sd[t][e], crow[t][e & 1] * ks, lvs);
+        if (key0 + g + (e >> 1) * 8 > lim[t][e & 1]) w[e] = ninf();
       }
-      float mx = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float mn = fmaxf(m[r], mx - kWeightBits);
-      if (__any_sync(0xffffffffu, mn > m[r])) {
-        const float fo = (m[r] == ninf()) ? 0.f : ex2(m[r] - mn);
-        l[r] *= fo;
+      float mn[2];
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j) {
-          o[j][2 * r] *= fo;
-          o[j][2 * r + 1] *= fo;
+      for (int u = 0; u < 2; ++u) {
+        float mx = fmaxf(w[u], w[2 + u]);
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+        mn[u] = fmaxf(m[t][u], mx - kWeightBits);
+      }
+      if (__any_sync(0xffffffffu, mn[0] > m[t][0] || mn[1] > m[t][1])) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float fo = (m[t][u] == ninf()) ? 0.f : ex2(m[t][u] - mn[u]);
+          l[t][u] *= fo;
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) {
+            o[t][j][u] *= fo;
+            o[t][j][2 + u] *= fo;
+          }
+          m[t][u] = mn[u];
         }
-        m[r] = mn;
       }
-      const float ref = (mn == ninf()) ? 0.f : mn;
-      float p[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) p[u] = ex2(t[u] - ref);
-      const float sum = (p[0] + p[1]) + (p[2] + p[3]);
-      // this lane's keys only; a page that the row does not see adds nothing, whatever its scale is
-      if (!(sum == 0.f)) l[r] = fmaf(sum, ivs, l[r]);
-      pa[r][0] = half2_bits(p[0], p[1]);
-      pa[r][1] = half2_bits(p[2], p[3]);
-      if constexpr (HILO) {
+      for (int e = 0; e < 4; ++e) w[e] = ex2(w[e] - (mn[e & 1] == ninf() ? 0.f : mn[e & 1]));
+      // this lane's keys only; a page that the query does not see adds nothing, whatever its scale is
 #pragma unroll
-        for (int u = 0; u < 4; ++u) p[u] -= __half2float(__float2half_rn(p[u]));
-        plo[r][0] = half2_bits(p[0], p[1]);
-        plo[r][1] = half2_bits(p[2], p[3]);
+      for (int u = 0; u < 2; ++u) {
+        const float sum = w[u] + w[2 + u];
+        if (!(sum == 0.f)) l[t][u] = fmaf(sum, ivs, l[t][u]);
+      }
+#pragma unroll
+      for (int hl = 0; hl < HL; ++hl) {
+        pb[t][hl][0] = transposed(half2_bits(w[0], w[1]));
+        pb[t][hl][1] = transposed(half2_bits(w[2], w[3]));
+        if (HILO && hl == 0) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] -= __half2float(__float2half_rn(w[e]));
+        }
       }
     }
     // E4M3 has a NaN; a slot behind the last token may hold anything
@@ -321,38 +358,40 @@ cache_attn_kernel(const CacheAttnArgs a, const int splits) {
       // the codes of keys 2c and 2c + 1 side by side, features 4w .. 4w + 3
       const uint32_t a01 = __byte_perm(vf[0][w], vf[1][w], 0x5140), a23 = __byte_perm(vf[0][w], vf[1][w], 0x7362);
       const uint32_t b01 = __byte_perm(vf[2][w], vf[3][w], 0x5140), b23 = __byte_perm(vf[2][w], vf[3][w], 0x7362);
-      uint32_t b0[4], b1[4];
-      word_pairs<CODE>(a01, b0[0], b0[1]);
-      word_pairs<CODE>(a23, b0[2], b0[3]);
-      word_pairs<CODE>(b01, b1[0], b1[1]);
-      word_pairs<CODE>(b23, b1[2], b1[3]);
+      uint32_t lo[4], hi[4];
+      word_pairs<CODE>(a01, lo[0], lo[1]);
+      word_pairs<CODE>(a23, lo[2], lo[3]);
+      word_pairs<CODE>(b01, hi[0], hi[1]);
+      word_pairs<CODE>(b23, hi[2], hi[3]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        mma<ROWS8>(o[4 * w + e], pa[0][0], pa[R - 1][0], pa[0][1], pa[R - 1][1], b0[e], b1[e]);
-        if constexpr (HILO) mma<ROWS8>(o[4 * w + e], plo[0][0], plo[R - 1][0], plo[0][1], plo[R - 1][1], b0[e], b1[e]);
-      }
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int hl = 0; hl < HL; ++hl)
+            mma(o[t][2 * w + j], lo[2 * j], lo[2 * j + 1], hi[2 * j], hi[2 * j + 1], pb[t][hl][0], pb[t][hl][1]);
     }
     if (next < key_hi) load_v(next, page);
   }
 
   // merge the four warps
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int row = g + 8 * r;
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    if (c == 0) {
-      sm_m[warp][row] = m[r];
-      sm_l[warp][row] = l[r];
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int row = 8 * t + 2 * c + u;
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) l[t][u] += __shfl_xor_sync(0xffffffffu, l[t][u], off);
+      if (g == 0) {
+        sm_m[warp][row] = m[t][u];
+        sm_l[warp][row] = l[t][u];
+      }
+      // rows g and g + 8 of product j: features VB g + 2j and the next
+#pragma unroll
+      for (int j = 0; j < D / 16; j += 2)
+        *reinterpret_cast<float4*>(&sm_o[warp][row][VB * g + 2 * j]) =
+            make_float4(o[t][j][u], o[t][j][2 + u], o[t][j + 1][u], o[t][j + 1][2 + u]);
     }
-    // columns 2c and 2c + 1 of product j: features VB (2c) + j and VB (2c + 1) + j
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-#pragma unroll
-      for (int j = 0; j < D / 8; j += 4)
-        *reinterpret_cast<float4*>(&sm_o[warp][row][VB * (2 * c + e) + j]) =
-            make_float4(o[j][2 * r + e], o[j + 1][2 * r + e], o[j + 2][2 * r + e], o[j + 3][2 * r + e]);
-  }
   __syncthreads();
   for (int idx = threadIdx.x; idx < ROWS * D; idx += kWarps * 32) {
     const int rr = idx / D, e = idx % D, row = row0 + rr;
@@ -386,17 +425,17 @@ cache_attn_kernel(const CacheAttnArgs a, const int splits) {
 }
 
 int row_tile(const CacheAttnArgs& a, int dtype) {
-  // (two 16-bit terms, or a head of 256 features, leave registers for eight rows only)
+  // (two 16-bit terms, or a head of 256 features, leave registers for eight columns only)
   return (dtype == NNLIB_B200_F32 || a.c.d > 128 || (long long)a.L * (a.Hq / a.c.H) <= 8) ? 8 : 16;
 }
 
-// Blocks of a unit: enough for four blocks on each SM, but no fewer than 256 keys each where the cache is full.
+// Blocks of a unit: enough for four blocks on each SM, but no fewer than 64 keys, a step for each warp, where the cache is full.
 int split_count(const CacheAttnArgs& a, int dtype) {
   const long long rows = (long long)a.L * (a.Hq / a.c.H), tile = row_tile(a, dtype);
   const long long units = (long long)a.c.B * a.c.H * ((rows + tile - 1) / tile);
   long long cap = a.c.rows << a.c.log_page;
   if (!a.lens) cap = std::min(cap, std::max(a.len0, 0LL));
-  const long long n = std::min((4 * 148 + units - 1) / units, (cap + 255) / 256);
+  const long long n = std::min((4 * 148 + units - 1) / units, (cap + 63) / 64);
   return (int)std::max(1LL, std::min(n, 1024LL));
 }
 
@@ -431,12 +470,13 @@ cudaError_t reduce(const CacheAttnArgs& a, int splits, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-template <typename T, int D, int CODE, bool ROWS8>
+template <typename T, int D, int CODE, int NT>
 cudaError_t launch(const CacheAttnArgs& a, int splits, cudaStream_t st) {
-  const long long rows = (long long)a.L * (a.Hq / a.c.H), tile = ROWS8 ? 8 : 16;
+  const long long rows = (long long)a.L * (a.Hq / a.c.H), tile = 8 * NT;
   const long long blocks = (long long)a.c.B * a.c.H * ((rows + tile - 1) / tile) * splits;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-  cache_attn_kernel<T, D, CODE, ROWS8><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a, splits);
+  const bool vec = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_sl * sizeof(T) % 16 == 0 && a.q_sb * sizeof(T) % 16 == 0;
+  cache_attn_kernel<T, D, CODE, NT><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a, splits, vec ? 1 : 0);
   count_launch();
   const cudaError_t e = cudaGetLastError();
   return e != cudaSuccess || splits == 1 ? e : reduce<T>(a, splits, st);
@@ -444,11 +484,11 @@ cudaError_t launch(const CacheAttnArgs& a, int splits, cudaStream_t st) {
 
 template <typename T, int CODE>
 cudaError_t launch_d(const CacheAttnArgs& a, int rows, int splits, cudaStream_t st) {
-  if (a.c.d > 128) return launch<T, 256, CODE, true>(a, splits, st);
+  if (a.c.d > 128) return launch<T, 256, CODE, 1>(a, splits, st);
   if constexpr (sizeof(T) == 2) {
-    if (rows == 16) return a.c.d <= 64 ? launch<T, 64, CODE, false>(a, splits, st) : launch<T, 128, CODE, false>(a, splits, st);
+    if (rows == 16) return a.c.d <= 64 ? launch<T, 64, CODE, 2>(a, splits, st) : launch<T, 128, CODE, 2>(a, splits, st);
   }
-  return a.c.d <= 64 ? launch<T, 64, CODE, true>(a, splits, st) : launch<T, 128, CODE, true>(a, splits, st);
+  return a.c.d <= 64 ? launch<T, 64, CODE, 1>(a, splits, st) : launch<T, 128, CODE, 1>(a, splits, st);
 }
 
 template <typename T>
