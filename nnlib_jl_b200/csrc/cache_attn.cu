@@ -32,7 +32,6 @@ namespace nb200 {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kStep = 16;                 // keys a warp takes at a time
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kValueFloor = 7.8886090522101181e-31f;    // 2^-100
 constexpr float kWeightBits = 14.f;
@@ -119,15 +118,20 @@ __device__ __forceinline__ int last_key(const CacheAttnArgs& a, long long start,
   return e < 0 ? -1 : (e < len ? (int)e : len - 1);
 }
 
-// blocks of an SM: what registers allow without spilling the codes in flight
-template <typename T, int D, int NT> struct Cfg { static constexpr int kCtas = D <= 64 ? 4 : (D <= 128 ? (sizeof(T) == 4 || NT == 2 ? 3 : 4) : 2); };
+// KG: sixteens of keys that a warp takes at a time, two where registers allow (what a step costs beside its products is then
+// shared); blocks of an SM: as many as do not spill the codes in flight
+template <typename T, int D, int NT>
+struct Cfg {
+  static constexpr int kKG = sizeof(T) == 2 && NT == 1 && D <= 128 ? 2 : 1;
+  static constexpr int kCtas = D <= 64 ? 4 : (D <= 128 ? 3 : 2);
+};
 
 // T: element type of q and x; HILO: two 16-bit terms for an element of q and for a weight (T = float)
 template <typename T, int D, int CODE, int NT>
 __global__ void __launch_bounds__(kWarps * 32, Cfg<T, D, NT>::kCtas)
 cache_attn_kernel(const CacheAttnArgs a, const int splits, const int vec) {
   constexpr bool HILO = sizeof(T) == 4;
-  constexpr int ROWS = 8 * NT, KS = D / 16, GK = D / 64, VB = D / 8, HL = HILO ? 2 : 1;
+  constexpr int ROWS = 8 * NT, KS = D / 16, GK = D / 64, VB = D / 8, HL = HILO ? 2 : 1, KG = Cfg<T, D, NT>::kKG, kStep = 16 * KG;
   __shared__ float sm_o[kWarps][ROWS][D];
   __shared__ float sm_m[kWarps][ROWS], sm_l[kWarps][ROWS];
   const CacheArgs& cc = a.c;
@@ -147,53 +151,73 @@ cache_attn_kernel(const CacheAttnArgs a, const int splits, const int vec) {
   // this block's keys: whole groups of 64
   const int groups = (kend + 63) / 64, share = (groups + splits - 1) / splits;
   const int key_lo = min(split * share, groups) * 64, key_hi = min(min((split + 1) * share, groups) * 64, kend);
-  const unsigned char* kbase = cc.codes[0] + (long long)h * cc.d + 16 * c;
-  const unsigned char* vbase = cc.codes[1] + (long long)h * cc.d + VB * g;
+  const unsigned char* kbase = cc.codes[0] + (long long)h * cc.d + 16 * c + g * cc.row;
+  const unsigned char* vbase = cc.codes[1] + (long long)h * cc.d + VB * g + 2 * c * cc.row;
 
-  // Pages, 32 of a warp's steps at a time: lane n looks up step n's page and scales
+  // Pages, 32 sixteens of keys at a time: the warp's sixteen number n (of its steps, one after the other) by lane n
+  const int stride = kWarps * kStep;
+  int key0 = key_lo + warp * kStep;
   int pg = 0;
   float ksc = 0.f, vsc = 0.f;
-  auto look_up = [&](int key) {
+  auto look_up = [&](int first) {
+    const int key = first + (lane / KG) * stride + (lane % KG) * 16;
     const bool in = key < key_hi;
     const long long page = in ? cache_page(cc, b, (long long)key >> cc.log_page) : -1;
     pg = page < 0 ? 0 : (int)page;
     ksc = page < 0 ? qnan() : cc.scale[0][page * cc.H + h];
     vsc = page < 0 ? qnan() : cc.scale[1][page * cc.H + h];
   };
-  uint32_t kf[2][GK][4], vf[4][VB / 4];
+  uint32_t kf[KG][2][GK][4], vf[KG][4][VB / 4];
   const int T1 = (1 << cc.log_page) - 1;
-  auto load_k = [&](int key0, int page) {
-    const unsigned char* p = kbase + (((long long)page << cc.log_page) + (key0 & T1) + g) * cc.row;
+  const int row8 = 8 * (int)cc.row;
+  long long at[KG];                                // where the sixteens of the step under way begin
+  auto place = [&](int key, int n) {
+#pragma unroll
+    for (int kg = 0; kg < KG; ++kg) {
+      const int page = __shfl_sync(0xffffffffu, pg, (n * KG + kg) & 31);
+      at[kg] = (((long long)page << cc.log_page) + ((key + 16 * kg) & T1)) * cc.row;
+    }
+  };
+  // (a step may reach behind the block's last key, onto a page that is not looked up: page 0 then)
+  auto load_k = [&]() {
+#pragma unroll
+    for (int kg = 0; kg < KG; ++kg) {
+      const unsigned char* p = kbase + at[kg];
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int G4 = 0; G4 < GK; ++G4)
+          if (64 * G4 + 16 * c < cc.d) load_codes<16>(p + nt * row8 + 64 * G4, kf[kg][nt][G4]);
+    }
+  };
+  auto load_v = [&]() {
+#pragma unroll
+    for (int kg = 0; kg < KG; ++kg) {
+      const unsigned char* p = vbase + at[kg];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (VB * g < cc.d) load_codes<VB>(p + (u & 1) * (int)cc.row + (u >> 1) * row8, vf[kg][u]);
+    }
+  };
+#pragma unroll
+  for (int kg = 0; kg < KG; ++kg) {
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
       for (int G4 = 0; G4 < GK; ++G4)
-        if (64 * G4 + 16 * c < cc.d) load_codes<16>(p + nt * 8 * cc.row + 64 * G4, kf[nt][G4]);
-  };
-  auto load_v = [&](int key0, int page) {
-    const unsigned char* p = vbase + (((long long)page << cc.log_page) + (key0 & T1) + 2 * c) * cc.row;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) kf[kg][nt][G4][w] = 0u;
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (VB * g < cc.d) load_codes<VB>(p + ((u & 1) + (u >> 1) * 8) * cc.row, vf[u]);
-  };
 #pragma unroll
-  for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-    for (int G4 = 0; G4 < GK; ++G4)
-#pragma unroll
-      for (int w = 0; w < 4; ++w) kf[nt][G4][w] = 0u;
-#pragma unroll
-  for (int u = 0; u < 4; ++u)
-#pragma unroll
-    for (int w = 0; w < VB / 4; ++w) vf[u][w] = 0u;
-  const int stride = kWarps * kStep;
-  int key0 = key_lo + warp * kStep;
+      for (int w = 0; w < VB / 4; ++w) vf[kg][u][w] = 0u;
+  }
   // the first keys are on their way while Q is prepared
   if (key0 < key_hi) {
-    look_up(key0 + lane * stride);
-    const int page = __shfl_sync(0xffffffffu, pg, 0);
-    load_k(key0, page);
-    load_v(key0, page);
+    look_up(key0);
+    place(key0, 0);
+    load_k();
+    load_v();
   }
 
   // Q's fragments, brought to a largest element in [2^13, 2^14)
@@ -269,47 +293,76 @@ cache_attn_kernel(const CacheAttnArgs a, const int splits, const int vec) {
       for (int e = 0; e < 4; ++e) o[t][j][e] = 0.f;
   }
 
-  for (int n = 0; key0 < key_hi; key0 += stride, ++n) {
-    const float ks = __shfl_sync(0xffffffffu, ksc, n & 31), vs = __shfl_sync(0xffffffffu, vsc, n & 31);
-    const int next = key0 + stride;
-    if ((n & 31) == 31 && next < key_hi) look_up(next + lane * stride);
-    const int page = __shfl_sync(0xffffffffu, pg, (n + 1) & 31);
+  int lim_all = 0x7fffffff;                    // up to here every column of the tile sees every key
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) lim_all = min(lim_all, lim[t][u]);
+  lim_all = __reduce_min_sync(0xffffffffu, lim_all);
 
-    // (two chains of sums)
-    float sc[NT][4], sd[NT][4];
+  for (int n = 0; key0 < key_hi; key0 += stride, ++n) {
+    float ks[KG], vs[KG];
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int kg = 0; kg < KG; ++kg) {
+      ks[kg] = __shfl_sync(0xffffffffu, ksc, (n * KG + kg) & 31);
+      vs[kg] = __shfl_sync(0xffffffffu, vsc, (n * KG + kg) & 31);
+    }
+    const int next = key0 + stride;
+    if (next < key_hi) {
+      if (((n + 1) * KG & 31) == 0) look_up(next);
+      place(next, n + 1);
+    }
+
+    float sc[KG][NT][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sc[t][e] = sd[t][e] = 0.f;
-#pragma unroll
-    for (int k2 = 0; k2 < KS; ++k2) {
-      uint32_t a0, a1, a2, a3;
-      word_pairs<CODE>(kf[0][k2 / 4][k2 % 4], a0, a2);
-      word_pairs<CODE>(kf[1][k2 / 4][k2 % 4], a1, a3);
+    for (int kg = 0; kg < KG; ++kg) {
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int hl = 0; hl < HL; ++hl) mma(k2 & 1 ? sd[t] : sc[t], a0, a1, a2, a3, qb[t][hl][k2][0], qb[t][hl][k2][1]);
+        for (int e = 0; e < 4; ++e) sc[kg][t][e] = 0.f;
+#pragma unroll
+      for (int k2 = 0; k2 < KS; ++k2) {
+        uint32_t a0, a1, a2, a3;
+        word_pairs<CODE>(kf[kg][0][k2 / 4][k2 % 4], a0, a2);
+        word_pairs<CODE>(kf[kg][1][k2 / 4][k2 % 4], a1, a3);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int hl = 0; hl < HL; ++hl) mma(sc[kg][t], a0, a1, a2, a3, qb[t][hl][k2][0], qb[t][hl][k2][1]);
+      }
     }
-    if (next < key_hi) load_k(next, page);
+    if (next < key_hi) load_k();
 
-    // scales of this step's page (16 keys never cross one)
-    const float vse = vs >= kValueFloor ? vs : ((vs >= 0.f) ? kValueFloor : qnan());
-    const float lvs = __log2f(vse) + kWeightBits, ivs = __fdividef(1.f, vse);
-    uint32_t pb[NT][HL][2];
+    // scales of this step's pages (sixteen keys never cross one)
+    float lvs[KG], ivs[KG];
+#pragma unroll
+    for (int kg = 0; kg < KG; ++kg) {
+      const float vse = vs[kg] >= kValueFloor ? vs[kg] : ((vs[kg] >= 0.f) ? kValueFloor : qnan());
+      lvs[kg] = __log2f(vse) + kWeightBits;
+      ivs[kg] = __fdividef(1.f, vse);
+    }
+    const bool edge = key0 + kStep - 1 > lim_all;
+    uint32_t pb[KG][NT][HL][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      // w[e]: key g (+ 8 for e >= 2), column 2c (+ 1 for odd e)
-      float w[4];
+      // w[.][e]: key g (+ 8 for e >= 2), column 2c (+ 1 for odd e)
+      float w[KG][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        w[e] = fmaf(sc[t][e] + sd[t][e], crow[t][e & 1] * ks, lvs);
-        if (key0 + g + (e >> 1) * 8 > lim[t][e & 1]) w[e] = ninf();
+      for (int kg = 0; kg < KG; ++kg)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[kg][e] = fmaf(sc[kg][t][e], crow[t][e & 1] * ks[kg], lvs[kg]);
+      if (edge) {
+#pragma unroll
+        for (int kg = 0; kg < KG; ++kg)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (key0 + 16 * kg + g + (e >> 1) * 8 > lim[t][e & 1]) w[kg][e] = ninf();
       }
       float mn[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        float mx = fmaxf(w[u], w[2 + u]);
+        float mx = fmaxf(w[0][u], w[0][2 + u]);
+        if (KG == 2) mx = fmaxf(mx, fmaxf(w[KG - 1][u], w[KG - 1][2 + u]));
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
         mn[u] = fmaxf(m[t][u], mx - kWeightBits);
@@ -327,51 +380,58 @@ cache_attn_kernel(const CacheAttnArgs a, const int splits, const int vec) {
           m[t][u] = mn[u];
         }
       }
+      const float ref[2] = {mn[0] == ninf() ? 0.f : mn[0], mn[1] == ninf() ? 0.f : mn[1]};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = ex2(w[e] - (mn[e & 1] == ninf() ? 0.f : mn[e & 1]));
-      // this lane's keys only; a page that the query does not see adds nothing, whatever its scale is
+      for (int kg = 0; kg < KG; ++kg) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const float sum = w[u] + w[2 + u];
-        if (!(sum == 0.f)) l[t][u] = fmaf(sum, ivs, l[t][u]);
-      }
+        for (int e = 0; e < 4; ++e) w[kg][e] = ex2(w[kg][e] - ref[e & 1]);
+        // this lane's keys only; a page that the query does not see adds nothing, whatever its scale is
 #pragma unroll
-      for (int hl = 0; hl < HL; ++hl) {
-        pb[t][hl][0] = transposed(half2_bits(w[0], w[1]));
-        pb[t][hl][1] = transposed(half2_bits(w[2], w[3]));
-        if (HILO && hl == 0) {
+        for (int u = 0; u < 2; ++u) {
+          const float sum = w[kg][u] + w[kg][2 + u];
+          if (!(sum == 0.f)) l[t][u] = fmaf(sum, ivs[kg], l[t][u]);
+        }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] -= __half2float(__float2half_rn(w[e]));
+        for (int hl = 0; hl < HL; ++hl) {
+          pb[kg][t][hl][0] = transposed(half2_bits(w[kg][0], w[kg][1]));
+          pb[kg][t][hl][1] = transposed(half2_bits(w[kg][2], w[kg][3]));
+          if (HILO && hl == 0) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[kg][e] -= __half2float(__float2half_rn(w[kg][e]));
+          }
         }
       }
     }
-    // E4M3 has a NaN; a slot behind the last token may hold anything
-    if (CODE == NNLIB_B200_E4M3 && key0 + kStep > kend) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (key0 + 2 * c + (u & 1) + (u >> 1) * 8 >= kend)
+    for (int kg = 0; kg < KG; ++kg) {
+      // E4M3 has a NaN; a slot behind the last token may hold anything
+      if (CODE == NNLIB_B200_E4M3 && key0 + kStep > kend) {
 #pragma unroll
-          for (int w = 0; w < VB / 4; ++w) vf[u][w] = 0u;
+        for (int u = 0; u < 4; ++u)
+          if (key0 + 16 * kg + 2 * c + (u & 1) + (u >> 1) * 8 >= kend)
+#pragma unroll
+            for (int w = 0; w < VB / 4; ++w) vf[kg][u][w] = 0u;
+      }
+#pragma unroll
+      for (int w = 0; w < VB / 4; ++w) {
+        // the codes of keys 2c and 2c + 1 side by side, features 4w .. 4w + 3
+        const uint32_t a01 = __byte_perm(vf[kg][0][w], vf[kg][1][w], 0x5140), a23 = __byte_perm(vf[kg][0][w], vf[kg][1][w], 0x7362);
+        const uint32_t b01 = __byte_perm(vf[kg][2][w], vf[kg][3][w], 0x5140), b23 = __byte_perm(vf[kg][2][w], vf[kg][3][w], 0x7362);
+        uint32_t lo[4], hi[4];
+        word_pairs<CODE>(a01, lo[0], lo[1]);
+        word_pairs<CODE>(a23, lo[2], lo[3]);
+        word_pairs<CODE>(b01, hi[0], hi[1]);
+        word_pairs<CODE>(b23, hi[2], hi[3]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int hl = 0; hl < HL; ++hl)
+              mma(o[t][2 * w + j], lo[2 * j], lo[2 * j + 1], hi[2 * j], hi[2 * j + 1], pb[kg][t][hl][0], pb[kg][t][hl][1]);
+      }
     }
-#pragma unroll
-    for (int w = 0; w < VB / 4; ++w) {
-      // the codes of keys 2c and 2c + 1 side by side, features 4w .. 4w + 3
-      const uint32_t a01 = __byte_perm(vf[0][w], vf[1][w], 0x5140), a23 = __byte_perm(vf[0][w], vf[1][w], 0x7362);
-      const uint32_t b01 = __byte_perm(vf[2][w], vf[3][w], 0x5140), b23 = __byte_perm(vf[2][w], vf[3][w], 0x7362);
-      uint32_t lo[4], hi[4];
-      word_pairs<CODE>(a01, lo[0], lo[1]);
-      word_pairs<CODE>(a23, lo[2], lo[3]);
-      word_pairs<CODE>(b01, hi[0], hi[1]);
-      word_pairs<CODE>(b23, hi[2], hi[3]);
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int hl = 0; hl < HL; ++hl)
-            mma(o[t][2 * w + j], lo[2 * j], lo[2 * j + 1], hi[2 * j], hi[2 * j + 1], pb[t][hl][0], pb[t][hl][1]);
-    }
-    if (next < key_hi) load_v(next, page);
+    if (next < key_hi) load_v();
   }
 
   // merge the four warps
@@ -429,13 +489,15 @@ int row_tile(const CacheAttnArgs& a, int dtype) {
   return (dtype == NNLIB_B200_F32 || a.c.d > 128 || (long long)a.L * (a.Hq / a.c.H) <= 8) ? 8 : 16;
 }
 
-// Blocks of a unit: enough for four blocks on each SM, but no fewer than 64 keys, a step for each warp, where the cache is full.
+// Blocks of a unit: as many as fit the GPU at once (one more wave of them, however small, costs as much as the first), but no
+// fewer than 64 keys, a step for each warp, where the cache is full.
 int split_count(const CacheAttnArgs& a, int dtype) {
   const long long rows = (long long)a.L * (a.Hq / a.c.H), tile = row_tile(a, dtype);
   const long long units = (long long)a.c.B * a.c.H * ((rows + tile - 1) / tile);
   long long cap = a.c.rows << a.c.log_page;
   if (!a.lens) cap = std::min(cap, std::max(a.len0, 0LL));
-  const long long n = std::min((4 * 148 + units - 1) / units, (cap + 63) / 64);
+  const int fit = a.c.d <= 64 ? 4 : (a.c.d <= 128 ? 3 : 2);      // blocks of an SM (Cfg)
+  const long long n = std::min(fit * 148 / units, (cap + 63) / 64);
   return (int)std::max(1LL, std::min(n, 1024LL));
 }
 
