@@ -305,10 +305,11 @@ def test_norm_rope_argument_checks_without_a_gpu(lib):
         assert bwd(**bad) == _lib.INVALID_ARG, bad
     assert fwd(d=258, rot=2) == _lib.UNSUPPORTED_SHAPE
     assert lib.nnlib_b200_norm_rope(None, None) == _lib.INVALID_ARG
-    # one row of partial sums for each block: six tokens of queries and of keys
-    assert lib.nnlib_b200_norm_rope_bwd_workspace_bytes(C.byref(_norm_rope())) == 4 * 64 * 12
+    # one row of partial sums for each block: four warps of it take one of the six tokens' queries or keys each
+    need = lib.nnlib_b200_norm_rope_bwd_workspace_bytes(C.byref(_norm_rope()))
+    assert need == 4 * 64 * 4
     assert lib.nnlib_b200_norm_rope_bwd_workspace_bytes(C.byref(_norm_rope(d=63))) == 0
-    assert bwd(0x1000, 4 * 64 * 12 - 1) == _lib.WORKSPACE_TOO_SMALL and bwd(0x1008, 1 << 20) == _lib.WORKSPACE_TOO_SMALL
+    assert bwd(0x1000, need - 1) == _lib.WORKSPACE_TOO_SMALL and bwd(0x1008, 1 << 20) == _lib.WORKSPACE_TOO_SMALL
     before = lib.nnlib_b200_launch_count()
     assert fwd(L=0) == _lib.OK and fwd(B=0, q=None) == _lib.OK
     assert lib.nnlib_b200_launch_count() == before
