@@ -20,7 +20,7 @@ import torch
 from . import _lib
 from .attention import _DTYPES, ArgumentError, _check, _empty3, _on_device, _status_word, _stream
 from .layout import is_column_major, jl_empty
-from .rotary import _int32, _require_rows
+from .rotary import _dense, _int32, _require_rows
 
 __all__ = ["QuantizedCache", "cache_write_", "cache_read", "cached_attention"]
 
@@ -82,10 +82,9 @@ class QuantizedCache:
         E, T, P = k.shape
         H = k_scale.shape[0]
         codes, scales = (1, E, E * T), (1, H)
-        if (k.stride() != codes and not is_column_major(k)) or (v.stride() != codes and not is_column_major(v)) or \
-                (k_scale.stride() != scales and not is_column_major(k_scale)) or \
-                (v_scale.stride() != scales and not is_column_major(v_scale)):
-            raise TypeError("a cache's arrays must be dense and column-major")
+        for t, strides in ((k, codes), (v, codes), (k_scale, scales), (v_scale, scales)):
+            if t.stride() != strides and not is_column_major(t):       # (the first says it at a glance)
+                raise TypeError("a cache's arrays must be dense and column-major")
         if T < 16 or T > 256 or T & (T - 1):
             raise ArgumentError(f"a page holds a power of two from 16 to 256 tokens, got {T}")
         if batch < 0:
@@ -136,7 +135,7 @@ class QuantizedCache:
 
 def _starts(p, start, B, dev):
     if isinstance(start, torch.Tensor):
-        p.start = _int32("start", start, (B,), dev)
+        p.start = _int32("start", start, B, dev)
     else:
         p.start0 = int(start)
 
@@ -168,7 +167,7 @@ def cache_write_(cache: QuantizedCache, k: torch.Tensor, v: torch.Tensor, *, sta
     p.v_stride_l, p.v_stride_b = vst
     _starts(p, start, B, k.device)
     if count is not None:
-        p.count = _int32("count", count, (B,), k.device)
+        p.count = _int32("count", count, B, k.device)
     with _on_device(k.device):
         _check(_lib.load().nnlib_b200_cache_write(C.byref(c), C.byref(p), _stream()), "cache_write")
     return cache
@@ -199,7 +198,7 @@ def cache_read(cache: QuantizedCache, length: int, *, start: Union[int, torch.Te
     p = _lib.CacheTokens.from_buffer_copy(_blank_tokens)
     _starts(p, start, B, dev)
     if lens is not None:
-        p.lens = _int32("lens", lens, (B,), dev)
+        p.lens = _int32("lens", lens, B, dev)
     k, v = _empty3(E, length, B, dtype, dev), _empty3(E, length, B, dtype, dev)
     p.dtype, p.L, p.k, p.v = _DTYPES[dtype], length, k.data_ptr(), v.data_ptr()
     with _on_device(dev):
@@ -232,16 +231,16 @@ def cached_attention(q: torch.Tensor, cache: QuantizedCache, lens: Union[int, to
     p.dtype, p.causal = _DTYPES[q.dtype], 1 if causal else 0
     p.Hq, p.L = nheads, L
     if isinstance(lens, torch.Tensor):
-        p.lens = _int32("lens", lens, (B,), dev)
+        p.lens = _int32("lens", lens, B, dev)
     else:
         p.len0 = int(lens)
     if start is not None:
-        p.start = _int32("start", start, (B,), dev)
+        p.start = _int32("start", start, B, dev)
     if scale is not None:
         if not scale > 0:
             raise ArgumentError(f"scale = {scale}")
         p.scale = scale
-    x = _empty3(E, L, B, q.dtype, dev)
+    x = _dense(q, E, L, B)
     p.q, p.x = q.data_ptr(), x.data_ptr()
     p.q_stride_l, p.q_stride_b = qst
     lse = None

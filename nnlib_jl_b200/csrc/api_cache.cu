@@ -90,11 +90,12 @@ int resolve_norm_rope(const nnlib_b200_norm_rope_params* p, bool bwd, NormRopeAr
 }
 
 int check_norm_rope_arrays(const NormRopeArgs& a) {
-  const void* all[] = {a.side[0].heads ? a.side[0].x : nullptr, a.side[1].heads ? a.side[1].x : nullptr,
+  const NormRopeSide& s = a.side[a.side[0].heads ? 0 : 1];
+  const void* all[] = {s.x, s.out, a.side[0].heads ? a.side[0].x : nullptr, a.side[1].heads ? a.side[1].x : nullptr,
                        a.side[0].heads ? a.side[0].out : nullptr, a.side[1].heads ? a.side[1].out : nullptr,
                        a.side[0].dy, a.side[1].dy, a.side[0].g, a.side[1].g, a.side[0].dg, a.side[1].dg,
                        a.freqs, a.positions, a.start};
-  return check_arrays(all, 4, 13);
+  return check_arrays(all, 2, 15);
 }
 
 int resolve_cache(const nnlib_b200_cache* c, CacheArgs* out) {
@@ -149,8 +150,8 @@ int resolve_tokens(const CacheArgs& c, const nnlib_b200_cache_tokens* p, CacheTo
     return NNLIB_B200_INVALID_ARG;
   if (t.L > 0 && c.B > 0) {
     if (!p->k || !p->v) return NNLIB_B200_INVALID_ARG;
-    const void* all[] = {p->k, p->v, c.codes[0], c.codes[1], c.scale[0], c.scale[1], c.table, p->start, p->count, p->lens};
-    const int rc = check_arrays(all, 4, 10);
+    const void* all[] = {p->k, c.codes[0], p->v, c.codes[1], c.scale[0], c.scale[1], c.table, p->start, p->count, p->lens};
+    const int rc = check_arrays(all, 2, 10);
     if (rc) return rc;
   }
   *out = t;
@@ -187,7 +188,7 @@ int resolve_attn(const CacheArgs& c, const nnlib_b200_cache_attn_params* p, bool
     if (!p->q || !p->x) return NNLIB_B200_INVALID_ARG;
     if (launching) {
       const void* all[] = {p->q, p->x, c.codes[0], c.codes[1], c.scale[0], c.scale[1], c.table, p->lens, p->start, p->lse, p->status};
-      const int rc = check_arrays(all, 4, 11);
+      const int rc = check_arrays(all, 2, 11);
       if (rc) return rc;
     }
   }

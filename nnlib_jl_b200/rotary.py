@@ -13,7 +13,7 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from .attention import _DTYPES, ArgumentError, _check, _empty3, _on_device, _stream
+from .attention import _DTYPES, ArgumentError, _check, _on_device, _stream
 
 __all__ = ["rope_frequencies", "qk_norm_rope", "qk_norm_rope_pullback"]
 
@@ -37,63 +37,78 @@ def _require_rows(name: str, t: torch.Tensor, like: Optional[torch.Tensor] = Non
         raise TypeError(f"{name} lives on {t.device}: this method is defined for CUDA arrays only")
     if t.dtype not in _DTYPES:
         raise TypeError(f"{name} has eltype {t.dtype}; supported: Float16, BFloat16, Float32")
-    if t.ndim != 3:
+    size = t.shape
+    if len(size) != 3:
         raise TypeError(f"{name} must be a 3-d (features, length, batch) array")
     if like is not None and (t.dtype != like.dtype or t.device != like.device):
         raise TypeError(f"{name} must have the eltype and device of the other arrays")
-    (E, L, B), (s0, sl, sb) = t.shape, t.stride()
+    E, L, B = size
+    s0, sl, sb = t.stride()
     if (E > 1 and s0 != 1) or (L > 1 and sl < E) or (B > 1 and sb < 1):
-        raise TypeError(f"{name}: features must be adjacent and tokens apart (strides {t.stride()} for size {tuple(t.shape)})")
+        raise TypeError(f"{name}: features must be adjacent and tokens apart (strides {t.stride()} for size {tuple(size)})")
     return (sl if L > 1 else 0), (sb if B > 1 else 0)
 
 
-def _int32(name: str, t: torch.Tensor, shape: tuple, dev: torch.device) -> int:
-    """Address of a dense Int32 vector."""
+def _dense(t: torch.Tensor, E: int, L: int, B: int) -> torch.Tensor:
+    """A dense column-major (E, L, B) array of the type and on the device of ``t``."""
+    s1 = E or 1
+    return t.new_empty_strided((E, L, B), (1, s1, s1 * (L or 1)))
+
+
+def _int32(name: str, t: torch.Tensor, n: int, dev: torch.device) -> int:
+    """Address of a dense Int32 vector of n elements."""
     if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != dev:
         raise TypeError(f"{name} must be an Int32 CUDA tensor on the device of the arrays")
-    if tuple(t.shape) != shape or (t.numel() > 1 and t.stride(0) != 1):
-        raise ArgumentError(f"{name} must be a dense array of size {shape}, got {tuple(t.shape)}")
+    if t.ndim != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+        raise ArgumentError(f"{name} must be a dense vector of {n} elements, got size {tuple(t.shape)}")
     return t.data_ptr()
+
+
+def _weights(name: str, g, d: int, q, dtype) -> int:
+    if not isinstance(g, torch.Tensor) or g.dtype != dtype or g.device != q.device or (dtype != q.dtype and dtype != torch.float32):
+        raise TypeError(f"the {name} weights must be a CUDA vector of the arrays' eltype, or Float32, both alike")
+    if g.ndim != 1 or g.shape[0] != d or (d > 1 and g.stride(0) != 1):
+        raise ArgumentError(f"the {name} weights must be a dense vector of {d} elements")
+    return g.data_ptr()
 
 
 def _params(q, k, gq, gk, freqs, nheads, start, positions, eps, interleaved):
     qs = _require_rows("query", q)
     ks = _require_rows("key", k, q)
     Eq, L, B = q.shape
+    Ek, Lk, Bk = k.shape
     nheads = int(nheads)
     if nheads < 1 or Eq % nheads != 0 or Eq == 0:
         raise ArgumentError(f"First dimension of query must be divisible by `nheads`: size {tuple(q.shape)}, nheads {nheads}")
     d = Eq // nheads
-    if tuple(k.shape[1:]) != (L, B) or k.shape[0] % d != 0 or k.shape[0] == 0:
+    if Lk != L or Bk != B or Ek % d != 0 or Ek == 0:
         raise ArgumentError(f"query of size {tuple(q.shape)} and key of size {tuple(k.shape)} do not match for heads of {d} features")
     p = _lib.NormRopeParams.from_buffer_copy(_blank)
-    for name, g in (("query", gq), ("key", gk)):
-        if not isinstance(g, torch.Tensor) or g.device != q.device or g.dtype not in (q.dtype, torch.float32) or g.dtype != gq.dtype:
-            raise TypeError(f"the {name} weights must be a CUDA vector of the arrays' eltype, or Float32, both alike")
-        if tuple(g.shape) != (d,) or (d > 1 and g.stride(0) != 1):
-            raise ArgumentError(f"the {name} weights must be a dense vector of {d} elements")
-    if not isinstance(freqs, torch.Tensor) or freqs.dtype != torch.float64 or freqs.device != q.device:
+    wdtype = getattr(gq, "dtype", None)
+    p.gq, p.gk = _weights("query", gq, d, q, wdtype), _weights("key", gk, d, q, wdtype)
+    dev = q.device
+    if not isinstance(freqs, torch.Tensor) or freqs.dtype != torch.float64 or freqs.device != dev:
         raise TypeError("freqs must be a Float64 CUDA vector (rope_frequencies makes one)")
-    if freqs.ndim != 1 or 2 * freqs.shape[0] > d or (freqs.shape[0] > 1 and freqs.stride(0) != 1):
+    n = freqs.shape[0] if freqs.ndim == 1 else -1
+    if n < 0 or 2 * n > d or (n > 1 and freqs.stride(0) != 1):
         raise ArgumentError(f"freqs must be a dense vector of at most {d // 2} elements, got {tuple(freqs.shape)}")
-    p.dtype, p.wdtype = _DTYPES[q.dtype], _DTYPES[gq.dtype]
-    p.interleaved = 1 if interleaved else 0
-    p.d, p.rot = d, 2 * freqs.shape[0]
-    p.Hq, p.Hk, p.L, p.B = nheads, k.shape[0] // d, L, B
-    p.q, p.k = q.data_ptr(), k.data_ptr()
+    p.dtype, p.wdtype = _DTYPES[q.dtype], _DTYPES[wdtype]
+    if interleaved:
+        p.interleaved = 1
+    p.d, p.rot, p.Hq, p.Hk, p.L, p.B = d, 2 * n, nheads, Ek // d, L, B
+    p.q, p.k, p.freqs = q.data_ptr(), k.data_ptr(), freqs.data_ptr()
     p.q_stride_l, p.q_stride_b = qs
     p.k_stride_l, p.k_stride_b = ks
-    p.gq, p.gk, p.freqs = gq.data_ptr(), gk.data_ptr(), freqs.data_ptr()
     p.eps = eps
     if positions is not None:
-        if not isinstance(positions, torch.Tensor) or positions.dtype != torch.int32 or positions.device != q.device:
+        if not isinstance(positions, torch.Tensor) or positions.dtype != torch.int32 or positions.device != dev:
             raise TypeError("positions must be an Int32 CUDA tensor on the device of the arrays")
-        if tuple(positions.shape) not in ((L, B), (L,)) or min(positions.stride(), default=0) < 0:
+        if tuple(positions.shape) not in ((L, B), (L,)):
             raise ArgumentError(f"positions must be of size {(L, B)} or {(L,)}, got {tuple(positions.shape)}")
         p.positions = positions.data_ptr()
         p.positions_stride = (C.c_int64 * 2)(positions.stride(0), positions.stride(1) if positions.ndim == 2 else 0)
     elif isinstance(start, torch.Tensor):
-        p.start = _int32("start", start, (B,), q.device)
+        p.start = _int32("start", start, B, dev)
     else:
         p.start0 = int(start)
     return p
@@ -111,8 +126,7 @@ def qk_norm_rope(q, k, gq, gk, freqs, *, nheads: int, start: Union[int, torch.Te
     ``positions[l, b]`` (Int32; ``(len,)`` serves every sequence).  ``k`` has as many heads as its size says.  Arithmetic
     is Float32 (angles Float64), results are rounded once; head sizes are even, up to 256."""
     p = _params(q, k, gq, gk, freqs, nheads, start, positions, eps, interleaved)
-    yq = _empty3(*q.shape, q.dtype, q.device)
-    yk = _empty3(*k.shape, k.dtype, k.device)
+    yq, yk = _dense(q, *q.shape), _dense(k, *k.shape)
     p.yq, p.yk = yq.data_ptr(), yk.data_ptr()
     with _on_device(q.device):
         _check(_lib.load().nnlib_b200_norm_rope(C.byref(p), _stream()), "norm_rope")
@@ -136,8 +150,7 @@ def qk_norm_rope_pullback(q, k, gq, gk, freqs, *, nheads: int, start: Union[int,
                 p.dyq, (p.dyq_stride_l, p.dyq_stride_b) = t.data_ptr(), strides
             else:
                 p.dyk, (p.dyk_stride_l, p.dyk_stride_b) = t.data_ptr(), strides
-        dq = _empty3(*q.shape, q.dtype, q.device)
-        dk = _empty3(*k.shape, k.dtype, k.device)
+        dq, dk = _dense(q, *q.shape), _dense(k, *k.shape)
         dgq, dgk = torch.empty_like(gq), torch.empty_like(gk)
         p.dq, p.dk, p.dgq, p.dgk = dq.data_ptr(), dk.data_ptr(), dgq.data_ptr(), dgk.data_ptr()
         lib = _lib.load()
