@@ -407,16 +407,16 @@ typedef struct nnlib_b200_cache {
   size_t struct_size;        /* = sizeof(nnlib_b200_cache) */
   int32_t code;              /* NNLIB_B200_INT8 / NNLIB_B200_E4M3 */
   int32_t reserved;
-  int64_t d, H;              /* features of a head (a multiple of 16, at most 256), heads */
+  int64_t d, H;              /* features of a head (a multiple of 16, at most 256), heads (at most 32767) */
   int64_t page, pages;       /* tokens of a page (a power of two, 16 .. 256), pages of the pool */
   void* k_codes;             /* 16-byte aligned */
   void* v_codes;
   float* k_scale;
   float* v_scale;
-  int64_t B;                 /* sequences */
+  int64_t B;                 /* sequences (at most 32767) */
   const int32_t* table;      /* (rows, B) page numbers, or NULL */
   int64_t table_stride;      /* elements between two sequences, 0 = rows */
-  int64_t rows;              /* pages of a sequence; without a table pages / B */
+  int64_t rows;              /* pages of a sequence, rows * page < 2^31 - 4096; without a table at most pages / B */
 } nnlib_b200_cache;
 
 /* Tokens on their way into or out of a cache. */
@@ -437,7 +437,7 @@ typedef struct nnlib_b200_cache_tokens {
 /* Quantises new tokens into the cache behind the start[b] tokens that sequence b holds; tokens from start[b] on are
    overwritten or, in the slots behind the new ones, left as they are.  A page that held tokens before keeps the larger
    of its scale and the one that the new tokens ask for; where that grows, the older codes are rounded to it anew,
-   code * (old scale / new scale).  Tokens at a negative number or beyond the capacity are left out.  A page that is
+   code * (old scale / new scale).  A sequence whose start is negative and tokens beyond the capacity are left out.  A page that is
    written by two sequences of one call ends with either's tokens. */
 NNLIB_B200_API int nnlib_b200_cache_write(const nnlib_b200_cache* c, const nnlib_b200_cache_tokens* t, void* stream);
 /* code * scale of tokens start[b] .. start[b] + L - 1, rounded to dtype; zeros at a negative number, from lens[b] on and
@@ -449,7 +449,10 @@ NNLIB_B200_API int nnlib_b200_cache_read(const nnlib_b200_cache* c, const nnlib_
    reads cache head h / (Hq / H).  Products run on codes, which 16-bit floating point holds exactly, with Float32 sums;
    Float32 arrays take two 16-bit terms of each query element and weight (about 22 bits).  A scale of values below 2^-100
    counts as 2^-100.  A query that sees no token gives NaN (or zeros), one that sees a token of a page with a NaN scale
-   gives NaN, and one that does not is not touched by it. */
+   gives NaN, and one that does not is not touched by it; codes of tokens in use must be numbers (cache_write makes no
+   others).  Many queries run on the tensor cores (tcgen05), few, Float32 arrays and heads of more than 128 features on
+   streamed warp-level products.  The same call gives the same bits each time; the cuts of the keys that sums are taken in
+   depend on the lengths of all sequences of the call, so a sequence's last bits may differ in another batch. */
 typedef struct nnlib_b200_cache_attn_params {
   size_t struct_size;        /* = sizeof(nnlib_b200_cache_attn_params) */
   int32_t dtype;             /* element type of q and x */

@@ -148,8 +148,8 @@ def cache_write_(cache: QuantizedCache, k: torch.Tensor, v: torch.Tensor, *, sta
 
     A page begun by this call gets the scale that its tokens ask for; one that holds tokens before ``start`` keeps its own
     unless the new tokens need a larger one, in which case the older codes are rounded to that.  What a page holds behind the
-    new tokens is left as it is, and tokens beyond the capacity, at negative numbers or on pages that the pool does not have
-    are left out.  A block that is given a NaN or an infinity reads as NaN until its page is begun anew.  Pages that are
+    new tokens is left as it is; tokens beyond the capacity or on pages that the pool does not have are left out, like a
+    sequence whose start is negative.  A block that is given a NaN or an infinity reads as NaN until its page is begun anew.  Pages that are
     written must be one sequence's alone."""
     kst = _require_rows("key", k)
     vst = _require_rows("value", v, k)

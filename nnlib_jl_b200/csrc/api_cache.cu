@@ -166,6 +166,7 @@ int resolve_attn(const CacheArgs& c, const nnlib_b200_cache_attn_params* p, bool
   CacheAttnArgs a;
   std::memset(&a, 0, sizeof(a));
   a.c = c;
+  if (c.pages == 0) a.c.rows = 0;            // a pool without a page has no address to read in a page's place
   a.q = p->q;
   a.x = p->x;
   if (!strides(p->Hq * c.d, p->L, p->q_stride_l, p->q_stride_b, &a.q_sl, &a.q_sb) ||

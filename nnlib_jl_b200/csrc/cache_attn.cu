@@ -24,8 +24,9 @@
 // sequences and tiles of columns, laid end to end in groups of one step of the block's four warps, are dealt to the teams in
 // equal runs.  A tile that one team has whole it also finishes; of others each team leaves running maxima, sums and outputs,
 // two pieces at most (its first tile's and its last one's), and cache_merge_kernel merges what a tile's first team says
-// there is.  (One query each, 8 sequences of 8192 tokens, 32 / 8 heads of 128: TODO us, with the keys of each sequence cut
-// into equal parts and one wave of blocks 39.)
+// there is.  One query each, 32 / 8 heads of 128, Int8: 4 sequences of 131072 tokens 212 us, 5.1 TB/s; 8 of 8192 41 us, of which
+// some 14 are the way to the first keys, the end and the merging, and 2.8 each step at 5 TB/s; 64 of 2048 73 us (each
+// sequence's keys cut into parts by themselves: 86).
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -40,7 +41,6 @@ constexpr int kWarps = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kValueFloor = 7.8886090522101181e-31f;    // 2^-100
 constexpr float kWeightBits = 14.f;
-constexpr int kUmmaRows = 48;
 
 __device__ __forceinline__ float ninf() { return __int_as_float(0xff800000); }
 __device__ __forceinline__ float qnan() { return __int_as_float(0x7fc00000); }
@@ -651,9 +651,16 @@ AttnArgs reduce_args(const CacheAttnArgs& a) {
   return r;
 }
 
-// Many rows go to the tensor cores.
+// Many columns go to the tensor cores, whose blocks take 256 of them at once but some 12 us to begin: more than 16 columns, and
+// more than five groups of keys to a team here.  Measured (us; here / there), 32 / 8 heads of 128: 4 x 16384 tokens, 16 columns
+// 69 / 88, 32 103 / 90, 64 184 / 97; 32 x 2048 tokens, 32 columns 133 / 100; 8 / 8 heads, 8 x 4096 tokens, 16 columns 47 / 55,
+// 24 65 / 56; 16 / 2 heads, 1 x 8192 tokens (3.5 groups) 96 columns 32 / 34, 192 (6.9) 45 / 33.
 bool use_umma(const CacheAttnArgs& a, int dtype) {
-  return cache_umma_supports(a, dtype) && (long long)a.L * (a.Hq / a.c.H) > kUmmaRows;
+  const long long rows = (long long)a.L * (a.Hq / a.c.H);
+  if (!cache_umma_supports(a, dtype) || rows <= 16) return false;
+  long long cap = a.c.rows << a.c.log_page;
+  if (!a.lens) cap = std::min(cap, std::max(a.len0, 0LL));
+  return (rows + 15) / 16 * a.c.B * ((cap + 63) / 64) > 5LL * team_count(a);
 }
 
 template <typename T>

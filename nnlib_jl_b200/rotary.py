@@ -124,7 +124,7 @@ def qk_norm_rope(q, k, gq, gk, freqs, *, nheads: int, start: Union[int, torch.Te
     ``p + length(freqs)``, or ``2p`` and ``2p + 1`` where ``interleaved``; the others stay as they are.  Token ``l`` of
     sequence ``b`` is at position ``start + l``, ``start`` an integer or an Int32 tensor of one per sequence, or at
     ``positions[l, b]`` (Int32; ``(len,)`` serves every sequence).  ``k`` has as many heads as its size says.  Arithmetic
-    is Float32 (angles Float64), results are rounded once; head sizes are even, up to 256."""
+    is Float32 (angles in 64 bits until they are less than a turn), results are rounded once; head sizes are even, up to 256."""
     p = _params(q, k, gq, gk, freqs, nheads, start, positions, eps, interleaved)
     yq, yk = _dense(q, *q.shape), _dense(k, *k.shape)
     p.yq, p.yk = yq.data_ptr(), yk.data_ptr()
