@@ -476,6 +476,8 @@ typedef struct nnlib_b200_cache_attn_params {
 NNLIB_B200_API size_t nnlib_b200_cache_attn_workspace_bytes(const nnlib_b200_cache* c, const nnlib_b200_cache_attn_params* p);
 NNLIB_B200_API int nnlib_b200_cache_attn(const nnlib_b200_cache* c, const nnlib_b200_cache_attn_params* p, void* workspace,
                                          size_t workspace_bytes, void* stream);
+/* NNLIB_B200_PATH_UMMA or NNLIB_B200_PATH_SIMT (warp-level products), what cache_attn would take, or a negative error */
+NNLIB_B200_API int nnlib_b200_cache_attn_path(const nnlib_b200_cache* c, const nnlib_b200_cache_attn_params* p);
 
 /* make_causal_mask (src/attention.jl:149-153): fill an (L, L) byte matrix
    with m[i + L*j] = (i <= j). */

@@ -63,6 +63,7 @@ EXPORTS = (
     "nnlib_b200_cache_read",
     "nnlib_b200_cache_attn",
     "nnlib_b200_cache_attn_workspace_bytes",
+    "nnlib_b200_cache_attn_path",
     "nnlib_b200_device_health",
     "nnlib_b200_selftest_wait_runout",
     "nnlib_b200_strerror",
@@ -315,6 +316,8 @@ def load() -> C.CDLL:
         fn.restype = C.c_int
     lib.nnlib_b200_cache_attn.argtypes = [CP, CA, C.c_void_p, C.c_size_t, C.c_void_p]
     lib.nnlib_b200_cache_attn.restype = C.c_int
+    lib.nnlib_b200_cache_attn_path.argtypes = [CP, CA]
+    lib.nnlib_b200_cache_attn_path.restype = C.c_int
     lib.nnlib_b200_cache_attn_workspace_bytes.argtypes = [CP, CA]
     lib.nnlib_b200_cache_attn_workspace_bytes.restype = C.c_size_t
     lib.nnlib_b200_attn_path.argtypes = [P]

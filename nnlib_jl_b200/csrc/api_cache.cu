@@ -259,6 +259,15 @@ size_t nnlib_b200_cache_attn_workspace_bytes(const nnlib_b200_cache* c, const nn
   return cache_attn_workspace_bytes(a, p->dtype);
 }
 
+int nnlib_b200_cache_attn_path(const nnlib_b200_cache* c, const nnlib_b200_cache_attn_params* p) {
+  CacheArgs k;
+  CacheAttnArgs a;
+  int rc = resolve_cache(c, &k);
+  if (!rc) rc = resolve_attn(k, p, false, &a);
+  if (rc) return rc;
+  return cache_attn_umma_path(a, p->dtype) ? NNLIB_B200_PATH_UMMA : NNLIB_B200_PATH_SIMT;
+}
+
 int nnlib_b200_cache_attn(const nnlib_b200_cache* c, const nnlib_b200_cache_attn_params* p, void* workspace,
                           size_t workspace_bytes, void* stream) {
   CacheArgs k;
@@ -270,6 +279,9 @@ int nnlib_b200_cache_attn(const nnlib_b200_cache* c, const nnlib_b200_cache_attn
   const size_t need = cache_attn_workspace_bytes(a, p->dtype);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return NNLIB_B200_WORKSPACE_TOO_SMALL;
   a.ws = static_cast<float*>(workspace);
+  if (log_calls())
+    std::fprintf(stderr, "[nnlib_b200] cache_attn d=%d H=%d Hq=%d L=%d B=%d causal=%d -> %s\n", k.d, k.H, a.Hq, a.L, k.B, a.causal,
+                 cache_attn_umma_path(a, p->dtype) ? "tcgen05" : "streamed keys");
   return finish(cache_attn(a, p->dtype, (cudaStream_t)stream));
 }
 

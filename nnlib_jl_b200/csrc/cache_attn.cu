@@ -709,6 +709,8 @@ cudaError_t launch_c(const CacheAttnArgs& a, int rows, cudaStream_t st) {
 
 }  // namespace
 
+bool cache_attn_umma_path(const CacheAttnArgs& a, int dtype) { return use_umma(a, dtype); }
+
 size_t cache_attn_workspace_bytes(const CacheAttnArgs& a, int dtype) {
   if (use_umma(a, dtype)) {
     const int n = cache_umma_splits(a);

@@ -109,22 +109,26 @@ def attention(q, kc, vc, ks, vs, lens, nheads, *, start=None, causal=True, scale
         at = np.zeros(B, int)
         vscale = np.array([vs[:, max(pages_of(table, rows, P, b, j // T), 0)] for j in range(n)], np.float64).reshape(n, H)
         k, v = (read(c, s, n, at, B, table=table)[:, :, b].astype(np.float64) if n else np.zeros((E, 0)) for c, s in ((kc, ks), (vc, vs)))
-        for i in range(L):
-            m = n if not causal else min(max(s0 + i + 1, 0), n)
-            if m == 0:
+        seen = np.arange(n)[None] <= (s0 + np.arange(L)[:, None] if causal else np.full((L, 1), n))
+        some = seen.any(1)
+        for h in range(nheads):
+            r, c = slice(h * d, (h + 1) * d), slice(h // G * d, (h // G + 1) * d)
+            with np.errstate(invalid="ignore"):
+                t = np.where(seen, scale * (q[r, :, b].T.astype(np.float64) @ k[c]), -np.inf)
+            bad = (np.isnan(t) | (seen & np.isnan(v[c]).any(0)[None])).any(1)       # a NaN among what the query sees
+            ok = some & ~bad
+            lse[bad, h, b] = np.nan
+            if not ok.any():
                 continue
-            for h in range(nheads):
-                r, c = slice(h * d, (h + 1) * d), slice(h // G * d, (h // G + 1) * d)
-                t = scale * (k[c, :m].T @ q[r, i, b].astype(np.float64))
-                if np.isnan(t).any() or np.isnan(v[c, :m]).any():
-                    lse[i, h, b] = np.nan
-                    continue
-                w = np.exp(t - t.max())
-                lse[i, h, b] = t.max() + np.log(w.sum())
-                w /= w.sum()
-                x[r, i, b] = v[c, :m] @ w
-                size[r, i, b] = np.abs(v[c, :m]) @ w
-                s = vscale[:m, h // G]
-                codes = np.abs(v[c, :m]) / np.where(s > 0, s, 1)
-                grid[r, i, b] = (w * s).max() * codes.sum(1)
+            t = t[ok]
+            top = t.max(1, keepdims=True)
+            w = np.exp(t - top)
+            sums = w.sum(1, keepdims=True)
+            lse[ok, h, b] = (top + np.log(sums))[:, 0]
+            w /= sums
+            val = np.where(np.isnan(v[c]), 0.0, v[c])                              # (weight 0 in these rows)
+            s = vscale[:, h // G]
+            codes = np.abs(val) / np.where(s > 0, s, 1)
+            x[r, ok, b], size[r, ok, b] = val @ w.T, np.abs(val) @ w.T
+            grid[r, ok, b] = (w * np.where(np.isnan(s), 0, s)).max(1) * (codes @ seen[ok].T)
     return x, lse, size, grid

@@ -9,6 +9,8 @@ relatively by that, and x by twice that times ``size``; exponentials, page scale
 Products of a weight and a value scale are multiples of 2^-34 of the largest one (2^-38 where queries are few), so each is off
 by 2^-35 of that at least, and x by 2^-35 times ``grid``.  With N(0, 1) inputs sum |q||k| scale <= 0.7 d / sqrt(d) <= 12.  So |x - x64| <= (W + 2 * 12 * 2^-18 + 2^-19) size + 2^-35 grid +
 half a step of the result: 2^-11 + 2^-13 for 16-bit arrays, 2^-13 for Float32 ones (which stay far below it)."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
@@ -207,6 +209,96 @@ def test_attention_matches_the_oracle(code, dtype, d, Hq, H, L, cap, page, paged
     q = _array(gen, (d * Hq, L, B), dtype)
     c.attend(q, [cap, max(L, cap // 2 + 1)], Hq)
     c.attend(q, [cap - 1, 1], Hq, causal=False, scale=0.3)
+
+
+def _path(c, q, nheads):
+    """Which kernels a call with lengths on the device takes."""
+    k = c.dev._call(q.shape[2], c.t)
+    p = nb._lib.CacheAttnParams(dtype=nb.attention._DTYPES[q.dtype], causal=1, Hq=nheads, L=q.shape[1], q=0x1000, x=0x1000, lens=0x1000)
+    return nb._lib.load().nnlib_b200_cache_attn_path(C.byref(k), C.byref(p))
+
+
+@gpu
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d,Hq,H,L,cap,page,paged", [
+    (16, 64, 64, 60, 380, 16, True),       # heads enough that few queries and keys make a large call
+    (64, 64, 64, 33, 530, 64, False),
+    (64, 96, 48, 33, 400, 32, True),
+    (80, 64, 64, 30, 490, 16, False),
+    (112, 64, 32, 300, 300, 128, True),    # 600 rows: three blocks, the last one's second tile empty
+    (128, 64, 64, 129, 1100, 64, True),    # keys cut into parts
+    (128, 48, 16, 90, 520, 32, True),
+])
+def test_attention_on_the_tensor_cores_matches_the_oracle(code, dtype, d, Hq, H, L, cap, page, paged):
+    gen = np.random.default_rng(15)
+    B = 2 if L < 200 else 1
+    c = _filled(gen, d * H, cap, B, H, page, code, paged)
+    q = _array(gen, (d * Hq, L, B), dtype)
+    assert _path(c, q, Hq) == nb._lib.PATH_UMMA
+    c.attend(q, [cap, max(L, cap // 2 + 1)][:B], Hq)
+    c.attend(q, [cap - 1, 1][:B], Hq, causal=False, scale=0.3)
+    nb.device_health()
+
+
+@gpu
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("page", [16, 64])
+def test_tensor_cores_with_lengths_of_every_kind(code, page):
+    gen = np.random.default_rng(16)
+    d, H, L, cap, B = 16, 64, 45, 200, 7
+    c = _filled(gen, d * H, cap, B, H, page, code, True)
+    q = _array(gen, (d * H, L, B), BF16)
+    assert _path(c, q, H) == nb._lib.PATH_UMMA
+    lens = [0, 1, 31, 33, 10 ** 9, -5, 150]
+    c.attend(q, lens, H)
+    c.attend(q, lens, H, causal=False)
+    x, lse = c.attend(q, lens, H, start=[0, -2, 40, 2, 190, 0, -L - 3])
+    assert torch.isnan(x[:, :, 6].float()).all() and torch.isneginf(lse[:, :, 6]).all()
+
+
+@gpu
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_tensor_cores_and_what_a_query_does_not_see(code):
+    """Poisoned and missing pages, E4M3's NaN behind the last token, as in the test for few queries below."""
+    gen = np.random.default_rng(17)
+    d, H, L, T = 32, 64, 50, 16
+    c = _filled(gen, d * H, 320, 3, H, T, code, True)
+    c.dev.v_scale[:, c.table[18, 0]], c.scale[1][:, c.table[18, 0]] = NAN, NAN
+    c.dev.k_scale[:, c.table[17, 1]], c.scale[0][:, c.table[17, 1]] = NAN, NAN
+    c.table[19, 2] = -1
+    if code == "e4m3":
+        for n, t in enumerate((c.dev.k, c.dev.v)):
+            t.view(torch.uint8)[:, 9:, c.table[18, 1]] = 0x7f
+            c.codes[n][:, 9:, c.table[18, 1]] = NAN
+    q = _array(gen, (d * H, L, 3), F16)
+    assert _path(c, q, H) == nb._lib.PATH_UMMA
+    x, _ = c.attend(q, [304, 297, 319], H)               # queries 254 .., 247 .. and 269 ..
+    assert torch.isfinite(x[:, 0].float()).all() and torch.isnan(x[:, -1, 0].float()).all()
+    c.attend(q, [288, 16 * 17, 304], H)
+
+
+@gpu
+def test_tensor_cores_captured_with_lengths_that_change():
+    gen = np.random.default_rng(18)
+    d, H, L, B = 64, 64, 40, 2
+    c = _filled(gen, d * H, 700, B, H, 64, "int8", True)
+    q, lens, t = _array(gen, (d * H, L, B), BF16), _i32([60, 700]), c.t
+    assert _path(c, q, H) == nb._lib.PATH_UMMA
+    want = nb.cached_attention(q, c.dev, lens, nheads=H, table=t)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        x = nb.cached_attention(q, c.dev, lens, nheads=H, table=t)
+    for n in ([60, 700], [40, 333], [699, 41]):
+        lens.copy_(_i32(n))
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(x, nb.cached_attention(q, c.dev, lens, nheads=H, table=t))
+    lens.copy_(_i32([60, 700]))
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(x, want)
 
 
 @gpu
@@ -468,3 +560,4 @@ def test_empty_calls():
     nb.cache_write_(nothing, k, k)
     assert not nb.cache_read(nothing, 2)[0].any()
     assert torch.isnan(nb.cached_attention(k, nothing, 3, nheads=2).float()).all()
+    assert torch.isnan(nb.cached_attention(k, nothing, 3, nheads=2, table=nb.jl_zeros((4, 2), torch.int32, DEV)).float()).all()
