@@ -437,8 +437,8 @@ typedef struct nnlib_b200_cache_tokens {
 /* Quantises new tokens into the cache behind the start[b] tokens that sequence b holds; tokens from start[b] on are
    overwritten or, in the slots behind the new ones, left as they are.  A page that held tokens before keeps the larger
    of its scale and the one that the new tokens ask for; where that grows, the older codes are rounded to it anew,
-   code * (old scale / new scale).  A sequence whose start is negative and tokens beyond the capacity are left out.  A page that is
-   written by two sequences of one call ends with either's tokens. */
+   code * (old scale / new scale).  A sequence whose start is negative and tokens beyond the capacity are left out.  A page that
+   one call writes from two places of its table ends as a mixture of both. */
 NNLIB_B200_API int nnlib_b200_cache_write(const nnlib_b200_cache* c, const nnlib_b200_cache_tokens* t, void* stream);
 /* code * scale of tokens start[b] .. start[b] + L - 1, rounded to dtype; zeros at a negative number, from lens[b] on and
    beyond the capacity. */

@@ -177,7 +177,11 @@ cache_attn_kernel(const CacheAttnArgs a, const int teams, const int vec) {
   // this team's run of groups: lo .. hi - 1 of all of them, from tile v on, whose first group is number base
   long long lo, hi, total, base;
   int v, n_teams;
-  {
+  if (a.ws == nullptr) {                         // short sequences: a team for each tile, which has it whole
+    v = n_teams = team;
+    lo = base = 0;
+    hi = total = 1;
+  } else {
     const int per = (n_tiles + kWarps * 32 - 1) / (kWarps * 32), v0 = min((int)threadIdx.x * per, n_tiles), v1 = min(v0 + per, n_tiles);
     long long mine = 0;
     for (int i = v0; i < v1; ++i) {
@@ -224,7 +228,8 @@ cache_attn_kernel(const CacheAttnArgs a, const int teams, const int vec) {
   for (bool first = true;; ++v) {
     const TileKeys tk = tile_keys(a, v, tiles, ROWS, rows, G);
     const int n_groups = (tk.kend + GS - 1) / GS;
-    if (n_groups == 0) continue;
+    if (a.ws == nullptr) hi = n_groups;
+    else if (n_groups == 0) continue;
     const int b = tk.b, row0 = tk.row0, len = tk.len, kend = tk.kend;
     const long long start = tk.start;
     const int g_lo = (int)max(lo - base, 0LL), g_hi = (int)min(hi - base, (long long)n_groups);
@@ -533,7 +538,7 @@ cache_attn_kernel(const CacheAttnArgs a, const int teams, const int vec) {
     __syncthreads();
     const bool whole = g_lo == 0 && g_hi == n_groups;
     const int piece = 2 * team + (first ? 0 : 1);
-    if (g_lo == 0 && h == 0 && threadIdx.x == 0) {
+    if (a.ws != nullptr && g_lo == 0 && h == 0 && threadIdx.x == 0) {
       // the last team of this tile: the last one whose run begins at or before its last group
       const int last = (int)quotient((base + n_groups) * n_teams - 1, total);
       ws_meta[v] = make_int2(piece, last - team + 1);
@@ -633,6 +638,15 @@ int team_count(const CacheAttnArgs& a) {
   return std::max(1, fit * 148 / a.c.H);
 }
 
+// At most 512 tokens to a sequence, and blocks enough for a whole tile each: nothing is merged, one launch and no workspace.
+// (500 tokens of 12 heads of 64: TODO us a call, dealt out and merged 19.4)
+bool one_launch(const CacheAttnArgs& a, int dtype) {
+  long long cap = a.c.rows << a.c.log_page;
+  if (!a.lens) cap = std::min(cap, std::max(a.len0, 0LL));
+  const int width = row_tile(a, dtype), rows = a.L * (a.Hq / a.c.H);
+  return cap <= 512 && (long long)((rows + width - 1) / width) * a.c.B <= team_count(a);
+}
+
 AttnArgs reduce_args(const CacheAttnArgs& a) {
   AttnArgs r;
   std::memset(&r, 0, sizeof(r));
@@ -673,12 +687,13 @@ cudaError_t reduce(const CacheAttnArgs& a, int splits, cudaStream_t st) {
 
 template <typename T, int D, int CODE, int NT>
 cudaError_t launch(const CacheAttnArgs& a, cudaStream_t st) {
-  const int teams = team_count(a);
+  const bool one = a.ws == nullptr;
+  const int teams = one ? (a.L * (a.Hq / a.c.H) + 8 * NT - 1) / (8 * NT) * a.c.B : team_count(a);
   const bool vec = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_sl * sizeof(T) % 16 == 0 && a.q_sb * sizeof(T) % 16 == 0;
   cache_attn_kernel<T, D, CODE, NT><<<(unsigned)(teams * a.c.H), kWarps * 32, 0, st>>>(a, teams, vec ? 1 : 0);
   count_launch();
   cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || one) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((long long)a.Hq * a.c.B * a.L));
   cfg.blockDim = dim3(128);
@@ -716,18 +731,20 @@ size_t cache_attn_workspace_bytes(const CacheAttnArgs& a, int dtype) {
     const int n = cache_umma_splits(a);
     return n == 1 ? 0 : sizeof(float) * (size_t)split_ws_floats(reduce_args(a), n);
   }
+  if (one_launch(a, dtype)) return 0;
   const int width = row_tile(a, dtype), rows = a.L * (a.Hq / a.c.H);
   return sizeof(float) * (size_t)(piece_slots(team_count(a), a.c.H, width) * (2 + a.c.d)) +
          sizeof(int2) * (size_t)((rows + width - 1) / width) * a.c.B;
 }
 
-cudaError_t cache_attn(const CacheAttnArgs& a, int dtype, cudaStream_t st) {
+cudaError_t cache_attn(CacheAttnArgs a, int dtype, cudaStream_t st) {
   if (use_umma(a, dtype)) {
     const int n = cache_umma_splits(a);
     const cudaError_t e = cache_umma(a, dtype, n, st);
     if (e != cudaSuccess || n == 1) return e;
     return dtype == NNLIB_B200_F16 ? reduce<__half>(a, n, st) : reduce<__nv_bfloat16>(a, n, st);
   }
+  if (one_launch(a, dtype)) a.ws = nullptr;
   const int rows = row_tile(a, dtype);
   if (dtype == NNLIB_B200_F16) return launch_c<__half>(a, rows, st);
   if (dtype == NNLIB_B200_BF16) return launch_c<__nv_bfloat16>(a, rows, st);

@@ -165,7 +165,7 @@ struct CacheAttnArgs {
   int causal, nan_fm, Hq, L;
 };
 size_t cache_attn_workspace_bytes(const CacheAttnArgs& a, int dtype);   // (cache_attn.cu)
-cudaError_t cache_attn(const CacheAttnArgs& a, int dtype, cudaStream_t st);   // a.ws holds the workspace
+cudaError_t cache_attn(CacheAttnArgs a, int dtype, cudaStream_t st);          // a.ws holds the workspace
 bool cache_attn_umma_path(const CacheAttnArgs& a, int dtype);                 // which of the two it takes
 bool cache_umma_supports(const CacheAttnArgs& a, int dtype);                  // tcgen05 (cache_attn_umma.cu): 16-bit, d <= 128
 int cache_umma_splits(const CacheAttnArgs& a);
