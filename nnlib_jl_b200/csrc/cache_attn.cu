@@ -24,7 +24,8 @@
 // sequences and tiles of columns, laid end to end in groups of one step of the block's four warps, are dealt to the teams in
 // equal runs.  A tile that one team has whole it also finishes; of others each team leaves running maxima, sums and outputs,
 // two pieces at most (its first tile's and its last one's), and cache_merge_kernel merges what a tile's first team says
-// there is.  One query each, 32 / 8 heads of 128, Int8: 4 sequences of 131072 tokens 212 us, 5.1 TB/s; 8 of 8192 41 us, of which
+// there is.  (Runs cut so that none reaches into a second tile, where tiles are few: 8 x 1024 tokens 16 us instead of 20, but 8 x
+// 8192 43 instead of 42 and 4 x 131072 218 instead of 212, for the registers that it takes.)  One query each, 32 / 8 heads of 128, Int8: 4 sequences of 131072 tokens 212 us, 5.1 TB/s; 8 of 8192 41 us, of which
 // some 14 are the way to the first keys, the end and the merging, and 2.8 each step at 5 TB/s; 64 of 2048 73 us (each
 // sequence's keys cut into parts by themselves: 86).
 #include <algorithm>
@@ -639,7 +640,7 @@ int team_count(const CacheAttnArgs& a) {
 }
 
 // At most 512 tokens to a sequence, and blocks enough for a whole tile each: nothing is merged, one launch and no workspace.
-// (500 tokens of 12 heads of 64: TODO us a call, dealt out and merged 19.4)
+// (500 tokens of 12 heads of 64: 15.8 us a call, dealt out and merged 19.4.)
 bool one_launch(const CacheAttnArgs& a, int dtype) {
   long long cap = a.c.rows << a.c.log_page;
   if (!a.lens) cap = std::min(cap, std::max(a.len0, 0LL));
