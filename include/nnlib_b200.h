@@ -397,7 +397,7 @@ NNLIB_B200_API int nnlib_b200_norm_rope_bwd(const nnlib_b200_norm_rope_params* p
    Codes: NNLIB_B200_INT8, -127 .. 127, scale = largest magnitude / 127; NNLIB_B200_E4M3 (four bits of exponent, three of
    mantissa, no infinities), scale = the smallest power of two that brings the largest magnitude to 448 or less.  A
    scale below 2^-126 is stored as 0, with codes of zero.  A block that is given a NaN or an infinity gets the scale
-   NaN: all of its tokens read as NaN until the page is begun anew. */
+   NaN: all of its tokens read as NaN until the page is begun anew.  No scale is negative. */
 enum {
   NNLIB_B200_INT8 = 0,
   NNLIB_B200_E4M3 = 1

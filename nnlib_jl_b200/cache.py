@@ -25,6 +25,7 @@ from .rotary import _dense, _int32, _require_rows
 __all__ = ["QuantizedCache", "cache_write_", "cache_read", "cached_attention"]
 
 _CODES = {torch.int8: _lib.INT8, torch.float8_e4m3fn: _lib.E4M3}
+_blank_cache = bytes(_lib.Cache())
 _blank_tokens = bytes(_lib.CacheTokens())
 _blank_attn = bytes(_lib.CacheAttnParams())
 
@@ -90,7 +91,7 @@ class QuantizedCache:
         if batch < 0:
             raise ArgumentError(f"batch = {batch}")
         self.k, self.v, self.k_scale, self.v_scale, self.batch = k, v, k_scale, v_scale, batch
-        p = _lib.Cache()
+        p = _lib.Cache.from_buffer_copy(_blank_cache)
         p.code = _CODES[k.dtype]
         p.d, p.H, p.page, p.pages = E // H, H, T, P
         p.k_codes, p.v_codes = k.data_ptr(), v.data_ptr()
@@ -199,7 +200,8 @@ def cache_read(cache: QuantizedCache, length: int, *, start: Union[int, torch.Te
     _starts(p, start, B, dev)
     if lens is not None:
         p.lens = _int32("lens", lens, B, dev)
-    k, v = _empty3(E, length, B, dtype, dev), _empty3(E, length, B, dtype, dev)
+    size, strides = (E, length, B), (1, E, E * (length or 1))
+    k, v = (cache.k_scale.new_empty_strided(size, strides, dtype=dtype) for _ in range(2))
     p.dtype, p.L, p.k, p.v = _DTYPES[dtype], length, k.data_ptr(), v.data_ptr()
     with _on_device(dev):
         _check(_lib.load().nnlib_b200_cache_read(C.byref(c), C.byref(p), _stream()), "cache_read")
