@@ -394,7 +394,7 @@ NNLIB_B200_API int nnlib_b200_norm_rope_bwd(const nnlib_b200_norm_rope_params* p
    Token number l of sequence b lives in slot l % page of page table[l / page + table_stride*b]; without a table in page
    (pages / B)*b + l / page.  A sequence has at most `rows` pages, rows * page tokens are its capacity.
    A page number outside 0 .. pages - 1 is never followed: a write leaves its tokens out, a read and attention give NaN.
-   Codes: NNLIB_B200_INT8, -127 .. 127, scale = largest magnitude / 127; NNLIB_B200_E4M3 (four bits of exponent, three of
+   Codes: NNLIB_B200_INT8, -127 .. 127, scale = largest magnitude * (1 / 127) in Float32; NNLIB_B200_E4M3 (four bits of exponent, three of
    mantissa, no infinities), scale = the smallest power of two that brings the largest magnitude to 448 or less.  A
    scale below 2^-126 is stored as 0, with codes of zero.  A block that is given a NaN or an infinity gets the scale
    NaN: all of its tokens read as NaN until the page is begun anew.  No scale is negative. */

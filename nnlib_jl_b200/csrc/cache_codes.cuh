@@ -21,7 +21,7 @@ __device__ __forceinline__ float block_scale(float amax) {
   if (!(amax <= 3.402823466e38f)) return __int_as_float(0x7fc00000);
   float s;
   if (CODE == NNLIB_B200_INT8) {
-    s = __fdiv_rn(amax, 127.f);
+    s = __fmul_rn(amax, 1.f / 127.f);    // (the constant rounded to Float32)
   } else {
     // 2^e with 448 * 2^e >= amax, 448 = 0.875 * 2^9
     int e;

@@ -23,7 +23,7 @@ def block_scale(amax, code: str):
     if not np.isfinite(amax):
         return F32(np.nan)
     if code == "int8":
-        s = F32(amax) / F32(127)
+        s = F32(F32(amax) * (F32(1) / F32(127)))
     else:
         m, e = np.frexp(F32(amax))
         s = F32(np.ldexp(1.0, int(e) - 9 + int(m > 0.875)))
