@@ -509,10 +509,20 @@ cache_attn_kernel(const CacheAttnArgs a, const int teams, const int vec) {
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < NT; ++t) {
+              if constexpr (HL == 1) {
+                mma(o[t][2 * w + j], lo[2 * j], lo[2 * j + 1], hi[2 * j], hi[2 * j + 1], pb[kg][t][0][0], pb[kg][t][0][1]);
+              } else {
+                // The products' own addition cuts off instead of rounding: over a long run the sum shrinks by a part of
+                // 2^-24 a step (2e-5 of x behind 99163 keys).  Float32 sums are added up with rounded additions.
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-              for (int hl = 0; hl < HL; ++hl)
-                mma(o[t][2 * w + j], lo[2 * j], lo[2 * j + 1], hi[2 * j], hi[2 * j + 1], pb[kg][t][hl][0], pb[kg][t][hl][1]);
+                for (int hl = 0; hl < HL; ++hl)
+                  mma(part, lo[2 * j], lo[2 * j + 1], hi[2 * j], hi[2 * j + 1], pb[kg][t][hl][0], pb[kg][t][hl][1]);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) o[t][2 * w + j][u] += part[u];
+              }
+            }
         }
       }
       if (next < key_hi) load_v();

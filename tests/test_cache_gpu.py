@@ -432,6 +432,31 @@ def test_a_long_history():
 
 
 @gpu
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_float32_sums_of_a_long_history_are_rounded(code):
+    """Positive values behind 131072 keys: a warp adds up to N = 131072 / 64 steps to a sum, and each addition that rounds is off
+    by at most 2^-24 of it, to either side: 5 sqrt(N / 3) 2^-24 at five standard deviations, once for x and once for the sum of
+    the weights; 8 2^-24 for the weights' two terms, a step's products and what the read values are rounded by.  Additions
+    that cut off would shrink every element alike, by up to N 2^-23.  The logits' own error, 2 * 2^-18 sum |q||k| scale at
+    most, moves elements to both sides; q is small, so that this stays below 8 2^-24 too."""
+    d, Hq, L, n = 32, 8, 1024, 131072
+    gen = np.random.default_rng(77)
+    c = nb.QuantizedCache(d, n, 1, nheads=1, page=64, eltype=CODE[code], device=DEV)
+    k, v = _array(gen, (d, n, 1), F32), _array(gen, (d, n, 1), F32)
+    nb.cache_write_(c, k, v.abs() + 0.5)
+    q = _array(gen, (d * Hq, L, 1), F32, 2.0 ** -7)
+    x = nb.cached_attention(q, c, n, nheads=Hq, causal=False)
+    kr, vr = (t[:, :, 0].double() for t in nb.cache_read(c, n, dtype=F32))
+    at = torch.arange(0, L, 33, device=DEV)
+    rows = q[:, at, 0].double().reshape(Hq, d, -1)
+    want = torch.stack([torch.softmax(r.T @ kr / d ** 0.5, 1) @ vr.T for r in rows])            # (Hq, rows, d)
+    got = x[:, at, 0].double().reshape(Hq, d, -1).transpose(1, 2)
+    lim = (2 * 5 * (n / 64 / 3) ** 0.5 + 16) * 2.0 ** -24
+    off = got / want - 1
+    assert off.abs().max().item() <= lim, (off.abs().max().item(), off.mean().item(), lim)
+
+
+@gpu
 def test_capture_replay_streams_and_repeatability():
     gen = np.random.default_rng(13)
     d, H, Hq, B = 64, 2, 8, 3
