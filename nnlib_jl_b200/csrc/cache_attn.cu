@@ -739,7 +739,7 @@ bool cache_attn_umma_path(const CacheAttnArgs& a, int dtype) { return use_umma(a
 
 size_t cache_attn_workspace_bytes(const CacheAttnArgs& a, int dtype) {
   if (use_umma(a, dtype)) {
-    const int n = cache_umma_splits(a);
+    const int n = cache_umma_splits(a, dtype);
     return n == 1 ? 0 : sizeof(float) * (size_t)split_ws_floats(reduce_args(a), n);
   }
   if (one_launch(a, dtype)) return 0;
@@ -750,7 +750,7 @@ size_t cache_attn_workspace_bytes(const CacheAttnArgs& a, int dtype) {
 
 cudaError_t cache_attn(CacheAttnArgs a, int dtype, cudaStream_t st) {
   if (use_umma(a, dtype)) {
-    const int n = cache_umma_splits(a);
+    const int n = cache_umma_splits(a, dtype);
     const cudaError_t e = cache_umma(a, dtype, n, st);
     if (e != cudaSuccess || n == 1) return e;
     return dtype == NNLIB_B200_F16 ? reduce<__half>(a, n, st) : reduce<__nv_bfloat16>(a, n, st);

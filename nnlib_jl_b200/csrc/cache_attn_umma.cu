@@ -642,14 +642,19 @@ cudaError_t launch_c(const CacheAttnArgs& a, int splits, cudaStream_t st) {
 
 bool cache_umma_supports(const CacheAttnArgs& a, int dtype) { return dtype != NNLIB_B200_F32 && a.c.d <= 128; }
 
-// Blocks of keys of a unit: where there are too few blocks of rows to fill the GPU, with four tiles of keys each at least.
-int cache_umma_splits(const CacheAttnArgs& a) {
+// Blocks of keys of a unit: where there are too few blocks of rows to fill the GPU, with four tiles of keys each at least; and
+// so many that a block's sums stay short.  The products' additions cut off instead of rounding, and behind n keys of a block x is
+// short by some n 2^-27.2 where all values have one sign (1024 queries, values 0.5 and above: 2.1e-4 with 32768 keys a block,
+// 8.7e-4 with 131072; half a step of Float16 is 4.9e-4).  32768 keys a block, 262144 for BFloat16, whose step is eight times as
+// large, keep that below half of half a step; joining the parts moves 8 bytes where a block did 4 * 32768 operations or more.
+int cache_umma_splits(const CacheAttnArgs& a, int dtype) {
   const long long rows = (long long)a.L * (a.Hq / a.c.H);
   const long long blocks = (rows + kTiles * kBM - 1) / (kTiles * kBM) * a.c.B * a.c.H;
+  const long long most = dtype == NNLIB_B200_F16 ? 32768 : 262144;
   long long cap = a.c.rows << a.c.log_page;
   if (!a.lens) cap = std::min(cap, std::max(a.len0, 0LL));
   const long long n = std::min(148 / std::max(blocks, 1LL), cap / (4 * kBN));
-  return (int)std::max(1LL, std::min(n, 64LL));
+  return (int)std::max(std::max(1LL, std::min(n, 64LL)), (cap + most - 1) / most);
 }
 
 cudaError_t cache_umma(const CacheAttnArgs& a, int dtype, int splits, cudaStream_t st) {

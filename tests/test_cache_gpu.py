@@ -457,6 +457,31 @@ def test_float32_sums_of_a_long_history_are_rounded(code):
 
 
 @gpu
+@pytest.mark.parametrize("L", [3, 1024])
+def test_float16_sums_of_a_very_long_history(L):
+    """Positive values behind 524288 keys: sum p |v| is x itself here.  Weights' roundings fall to both sides and cancel
+    over so many; 2^-12 for the sums (blocks of 32768 keys, each key's part of a cut-off addition 2^-27), half a step of the result, 2^-11."""
+    d, Hq, n = 32, 8, 524288
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    c = nb.QuantizedCache(d, n, 1, nheads=1, page=64, eltype=torch.int8, device=DEV)
+    k, v = (nb.jl_empty((d, n, 1), F16, DEV).normal_(generator=gen) for _ in range(2))
+    nb.cache_write_(c, k, v.abs() + 0.5)
+    q = nb.jl_empty((d * Hq, L, 1), F16, DEV).normal_(generator=gen) * 2.0 ** -7
+    x = nb.cached_attention(q, c, n, nheads=Hq, causal=False)
+    kr, vr = (t[:, :, 0].double() for t in nb.cache_read(c, n, dtype=F32))
+    at = torch.arange(0, L, 61, device=DEV)
+    rows = q[:, at, 0].double().reshape(Hq, d, -1)
+    want = torch.stack([torch.softmax(r.T @ kr / d ** 0.5, 1) @ vr.T for r in rows])
+    off = x[:, at, 0].double().reshape(Hq, d, -1).transpose(1, 2) / want - 1
+    # what is common to all elements is what the sums lose, 32768 2^-27 at most; the results' roundings, 32 different ones
+    # where queries are nearly alike, leave 2^-11 / sqrt(3 * 32) at one standard deviation
+    far = off.abs().max().item()
+    assert far <= 2.0 ** -11 + 2.0 ** -12
+    mean = abs(off.mean().item())
+    assert mean <= 2.0 ** -12 + 3 * 2.0 ** -11 / 96 ** 0.5
+
+
+@gpu
 def test_capture_replay_streams_and_repeatability():
     gen = np.random.default_rng(13)
     d, H, Hq, B = 64, 2, 8, 3
