@@ -7,7 +7,9 @@
 // i.e. a page's value scale goes into the exponent, where the running maximum m_i takes it up: no product is scaled, no
 // accumulator has a page's scale in it, and a weight's size is the size of what it adds to x.  q_i is brought to a
 // largest element in [2^13, 2^14) by a power of two of its own; w is rounded to 16 bits after a factor of 2^14, so that
-// weights keep 11 bits down to 2^-28 of the largest.  Float32 arrays: q and w as the sum of two 16-bit terms each.
+// weights keep 11 bits down to 2^-28 of the largest.  Float32 arrays: q and w as the sum of two 16-bit terms
+// each, sums over the keys by rounded additions (drawn cases 7.4e-7 off at most instead of 2.3e-5; 16 x 8192 tokens, Int8 86.0 us
+// and 87.0, E4M3 84.9 and 89.0; 256 queries of 4 sequences of 8192, heads of 64, 568 and 604).
 //
 // HBM is the bound (2 d bytes per key and head for up to 16 rows), so what counts is bytes in flight: nothing is staged,
 // a warp streams 16 keys at a time straight into the fragments of m16n8k16 products.  Keys and the features of values are
