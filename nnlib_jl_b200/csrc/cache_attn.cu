@@ -99,16 +99,36 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
 
 // BYTES codes of a lane, as words
 template <int BYTES>
-__device__ __forceinline__ void load_codes(const unsigned char* p, uint32_t (&w)[BYTES / 4]) {
-  if constexpr (BYTES == 8) {
+__device__ __forceinline__ void load_codes(const unsigned char* p, uint32_t* w) {
+  static_assert(BYTES == 8 || BYTES == 16, "one load");
+  if constexpr (BYTES == 8)
     asm("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
-  } else {
-#pragma unroll
-    for (int i = 0; i < BYTES / 16; ++i)
-      asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-          : "=r"(w[4 * i]), "=r"(w[4 * i + 1]), "=r"(w[4 * i + 2]), "=r"(w[4 * i + 3]) : "l"(p + 16 * i));
-  }
+  else
+    asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
 }
+
+// The features of a value row that lane group g of eight takes, D / 8 of them, in loads of at most 16: whether it makes its
+// load number i for a head of d features (a multiple of 16, at most D, which need not be one of D / 8).
+template <int D>
+struct ValueLoads {
+  static constexpr int kLane = D / 8, kBytes = kLane < 16 ? kLane : 16, kLoads = kLane / kBytes;
+  __host__ __device__ static constexpr bool made(int d, int g, int i) { return kLane * g + kBytes * i < d; }
+  // every feature of a head is loaded and none behind it
+  static constexpr bool exact() {
+    for (int d = 16; d <= D; d += 16) {
+      int n = 0;
+      for (int g = 0; g < 8; ++g)
+        for (int i = 0; i < kLoads; ++i)
+          if (made(d, g, i)) {
+            if (kLane * g + kBytes * (i + 1) > d) return false;
+            n += kBytes;
+          }
+      if (n != d) return false;
+    }
+    return true;
+  }
+};
+static_assert(ValueLoads<64>::exact() && ValueLoads<128>::exact() && ValueLoads<256>::exact(), "loads of value rows stay in their head");
 
 __device__ __forceinline__ int seq_len(const CacheAttnArgs& a, int b) {
   const long long cap = a.c.rows << a.c.log_page;
@@ -282,7 +302,10 @@ cache_attn_kernel(const CacheAttnArgs a, const int teams, const int vec) {
         const unsigned char* p = vbase + at[kg];
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-          if (VB * g < cc.d) load_codes<VB>(p + (u & 1) * (int)cc.row + (u >> 1) * row8, vf[kg][u]);
+#pragma unroll
+          for (int i = 0; i < ValueLoads<D>::kLoads; ++i)
+            if (ValueLoads<D>::made(cc.d, g, i))
+              load_codes<ValueLoads<D>::kBytes>(p + (u & 1) * (int)cc.row + (u >> 1) * row8 + 16 * i, vf[kg][u] + 4 * i);
       }
     };
 #pragma unroll

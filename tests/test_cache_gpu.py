@@ -611,3 +611,24 @@ def test_empty_calls():
     assert not nb.cache_read(nothing, 2)[0].any()
     assert torch.isnan(nb.cached_attention(k, nothing, 3, nheads=2).float()).all()
     assert torch.isnan(nb.cached_attention(k, nothing, 3, nheads=2, table=nb.jl_zeros((4, 2), torch.int32, DEV)).float()).all()
+
+
+# ------------------------------------------------------------------------------------------------ found later
+@gpu
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("d", [144, 176, 208, 240])
+def test_heads_whose_last_features_are_half_of_a_lanes_share(code, dtype, d):
+    """Heads of more than 128 features that are no multiple of 32; the last token of the pool's last page, with arrays that
+    lie inside larger ones whose bytes behind are no numbers.  (The kernel's loads are checked when it is compiled.)"""
+    gen = np.random.default_rng(31)
+    H, Hq, B, T, cap = 2, 4, 2, 16, 64
+    c = Pair(d * H, cap, B, H, T, code, gen, False)
+    wide = [torch.full((c.dev.k.numel() + 4096,), 0x7f, dtype=torch.uint8, device=DEV) for _ in range(2)]
+    inner = [nb.jl_reshape(w[:c.dev.k.numel()].view(c.dev.k.dtype), c.dev.k.shape) for w in wide]
+    c.dev = nb.QuantizedCache.from_arrays(*inner, c.dev.k_scale, c.dev.v_scale, batch=B)
+    c.write(_array(gen, (d * H, cap, B), dtype), _array(gen, (d * H, cap, B), dtype, 0.5), 0)
+    c.same()
+    for L in (1, 3, 20):
+        c.attend(_array(gen, (d * Hq, L, B), dtype), [cap, cap - 7], Hq)
+    assert all((w[c.dev.k.numel():] == 0x7f).all() for w in wide)
