@@ -649,9 +649,10 @@ __global__ void __launch_bounds__(128) cache_merge_kernel(const CacheAttnArgs a,
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float fj = __shfl_sync(0xffffffffu, f, j0 + j), lj = __shfl_sync(0xffffffffu, ml.y, j0 + j);
-          if (j0 + j < cnt && fj != 0.f) {
+          // (a sum that is NaN, of a query that sees such a page, counts however small its piece's weight is)
+          if (j0 + j < cnt) {
             L = fmaf(fj, lj, L);
-            acc = fmaf(fj, o[j], acc);
+            if (fj != 0.f) acc = fmaf(fj, o[j], acc);
           }
         }
       }

@@ -632,3 +632,25 @@ def test_heads_whose_last_features_are_half_of_a_lanes_share(code, dtype, d):
     for L in (1, 3, 20):
         c.attend(_array(gen, (d * Hq, L, B), dtype), [cap, cap - 7], Hq)
     assert all((w[c.dev.k.numel():] == 0x7f).all() for w in wide)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("what", ["value scale", "key scale", "page"])
+def test_a_bad_page_counts_beside_a_dominating_logit(what, dtype):
+    """The bad page in one block's share of the keys; in another's, logits some 400 above all in the first, whose weight
+    beside them is 0 in Float32.  Few tokens to a share: a step of four warps."""
+    gen = np.random.default_rng(32)
+    d, T, n = 32, 32, 2560
+    c = _filled(gen, d, n, 1, 1, T, "int8", True)
+    loud, bad = c.table[60, 0], c.table[0, 0]
+    c.scale[0][:, loud] *= 200
+    c.dev.k_scale[:, loud] *= 200
+    if what == "page":
+        c.table[0, 0] = -1
+    else:
+        side = 1 if what == "value scale" else 0
+        (c.dev.k_scale, c.dev.v_scale)[side][:, bad], c.scale[side][:, bad] = NAN, NAN
+    for L in (1, 3):
+        x, lse = c.attend(_array(gen, (d, L, 1), dtype), [n], 1)
+        assert torch.isnan(x.float()).all() and torch.isnan(lse).all()
