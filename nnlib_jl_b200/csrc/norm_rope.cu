@@ -305,7 +305,8 @@ __global__ void __launch_bounds__(kNrThreads, V == 1 ? 3 : (BWD && V == 8 ? 4 : 
       }
       const float sum = group_sum(pair_sum(sum2), lanes, lane, wl - lane);
       // (the approximation's error, two units in the last place, is little beside the sum's)
-      const float r = rsqrtf(fmaf(sum, inv_d, a.eps));
+      // A group that has no row this time must add nothing to the weights' gradient: with eps = 0 its r would be infinite.
+      const float r = live || !BWD ? rsqrtf(fmaf(sum, inv_d, a.eps)) : 0.f;
       const Two r2 = pair_of(r);
       Two back2 = 0ull;
       if (BWD) back2 = pair_of(-group_sum(pair_sum(dot2), lanes, lane, wl - lane) * inv_d * r * r);

@@ -243,3 +243,22 @@ def test_the_oracles_pullback_agrees_with_differences():
         h = 1e-5
         num = ((R.norm_rope(x + h * v, g + h * vg, pos, f, 1e-3, inter) - R.norm_rope(x - h * v, g - h * vg, pos, f, 1e-3, inter)) * dy).sum() / (2 * h)
         np.testing.assert_allclose(num, (dx * v).sum() + (dg * vg).sum(), rtol=1e-7)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("case", [
+    # d, rotated, neighbours, query heads, key heads, L, B
+    (128, 128, False, 1, 2, 9, 2),        # fewer heads than a warp has groups
+    (128, 128, True, 6, 3, 5, 1),         # heads that its groups do not divide
+    (80, 80, False, 8, 7, 700, 6),        # six groups, tokens enough that a warp takes all of a token's heads
+    (34, 34, False, 3, 2, 6, 2),          # single pairs
+    (64, 64, False, 12, 1, 1, 1),         # one token, its heads cut up
+])
+def test_without_eps(dtype, case):
+    """eps = 0: r = 1 / sqrt(mean x^2) of every row that is not all zero, and no trace of rows that a warp does not have."""
+    d, rot, inter, H, Hk, L, B = case
+    gen = np.random.default_rng(33)
+    q, k, dyq, dyk = (_array(gen, (h * d, L, B), dtype) for h in (H, Hk, H, Hk))
+    gq, gk = (1 + 0.2 * _array(gen, (d,), F32)).to(dtype), (1 + 0.2 * _array(gen, (d,), F32)).to(dtype)
+    _check(q, k, gq, gk, nb.rope_frequencies(rot), H, dyq, dyk, inter, eps=0.0, start=3)
