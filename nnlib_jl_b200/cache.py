@@ -5,7 +5,7 @@ A :class:`QuantizedCache` is a pool of pages of ``page`` tokens; one scale for e
 says what a code stands for.  :func:`cache_write_` quantises new tokens into it, :func:`cache_read` reads tokens back,
 :func:`cached_attention` attends to it without doing so.  Sequences find their pages through a table
 (``table[l // page, b]`` is the page of token ``l`` of sequence ``b``); without one, sequence ``b`` of ``batch`` owns the
-``b``-th run of ``pages / batch`` pages.
+``b``-th run of ``pages / batch`` pages, and calls are for ``batch`` sequences.
 
 All of it is asynchronous on the current stream, allocates through torch and reads lengths, starts and tables on the device,
 so that a captured call follows what they hold when it is replayed.  NNlib.jl has no counterpart.
@@ -33,7 +33,8 @@ _blank_attn = bytes(_lib.CacheAttnParams())
 class QuantizedCache:
     """Keys and values of ``nheads`` heads of ``dim / nheads`` features in 8 bits: ``capacity`` tokens (rounded up to whole
     pages) for each of ``batch`` sequences, or, for programs that hand pages out themselves, ``batch=1`` and as many tokens
-    as the pool is to hold.
+    as the pool is to hold.  A call without a table is for exactly ``batch`` sequences, or refused; with a table it is for as
+    many as that has.
 
     ``eltype``: ``torch.int8`` (a block's largest magnitude becomes 127) or ``torch.float8_e4m3fn`` (its scale is a power of
     two, the smallest that brings the largest magnitude to 448 or less).  ``page``: tokens of a page, a power of two from 16
@@ -62,10 +63,11 @@ class QuantizedCache:
         self._set(k, v, k_scale, v_scale, batch)
 
     @classmethod
-    def from_arrays(cls, k, v, k_scale, v_scale, *, batch: int = 1) -> "QuantizedCache":
-        """The cache that these arrays make up (no copy)."""
+    def from_arrays(cls, k, v, k_scale, v_scale, *, batch: Optional[int] = None) -> "QuantizedCache":
+        """The cache that these arrays make up (no copy).  Without ``batch`` it is a pool: a call without a table deals its
+        pages out in equal runs to however many sequences the call is for."""
         c = cls.__new__(cls)
-        c._set(k, v, k_scale, v_scale, int(batch))
+        c._set(k, v, k_scale, v_scale, None if batch is None else int(batch))
         return c
 
     def _set(self, k, v, k_scale, v_scale, batch):
@@ -88,7 +90,7 @@ class QuantizedCache:
                 raise TypeError("a cache's arrays must be dense and column-major")
         if T < 16 or T > 256 or T & (T - 1):
             raise ArgumentError(f"a page holds a power of two from 16 to 256 tokens, got {T}")
-        if batch < 0:
+        if batch is not None and batch < 0:
             raise ArgumentError(f"batch = {batch}")
         self.k, self.v, self.k_scale, self.v_scale, self.batch = k, v, k_scale, v_scale, batch
         p = _lib.Cache.from_buffer_copy(_blank_cache)
@@ -122,6 +124,9 @@ class QuantizedCache:
         p = _lib.Cache.from_buffer_copy(self._template)
         p.B = B
         if table is None:
+            # (a call for no sequence touches nothing)
+            if B != self.batch and self.batch is not None and B:
+                raise ArgumentError(f"a call for {B} sequences, without a table, on a cache of {self.batch}")
             p.rows = self.k.shape[2] // B if B else 0
             return p
         if not isinstance(table, torch.Tensor) or table.dtype != torch.int32 or table.device != self.k.device:
@@ -179,13 +184,13 @@ def cache_read(cache: QuantizedCache, length: int, *, start: Union[int, torch.Te
     """``(k, v)``: tokens ``start[b] .. start[b] + length - 1`` of every sequence as dense ``(dim, length, batch)`` arrays of
     ``dtype``, ``code * scale`` rounded once.  Tokens from ``lens[b]`` on (Int32; without it, from the capacity on) come as
     zeros, tokens on pages that the pool does not have as NaN.  The batch is the table's, else that of ``start`` or ``lens``,
-    else the cache's own."""
+    else the cache's own, or one of a pool that has none."""
     length = int(length)
     if length < 0:
         raise ArgumentError(f"length = {length}")
     if dtype not in _DTYPES:
         raise TypeError(f"eltype {dtype}; supported: Float16, BFloat16, Float32")
-    B = cache.batch
+    B = 1 if cache.batch is None else cache.batch
     if table is not None:
         if not isinstance(table, torch.Tensor) or table.ndim != 2:
             raise TypeError("table must be a 2-d Int32 CUDA tensor")

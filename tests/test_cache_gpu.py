@@ -654,3 +654,42 @@ def test_a_bad_page_counts_beside_a_dominating_logit(what, dtype):
     for L in (1, 3):
         x, lse = c.attend(_array(gen, (d, L, 1), dtype), [n], 1)
         assert torch.isnan(x.float()).all() and torch.isnan(lse).all()
+
+
+@gpu
+def test_a_call_without_a_table_is_for_the_caches_own_sequences():
+    gen = np.random.default_rng(34)
+    dim, H, T, B, cap = 64, 2, 16, 4, 48
+    c = Pair(dim, cap, B, H, T, "int8", gen, False)
+    c.write(_array(gen, (dim, cap, B), BF16), _array(gen, (dim, cap, B), BF16), 0)
+    for n in (1, 2, 3, 5, 8):
+        k = _array(gen, (dim, 5, n), BF16)
+        with pytest.raises(nb.ArgumentError):
+            nb.cache_write_(c.dev, k, k)
+        with pytest.raises(nb.ArgumentError):
+            nb.cached_attention(k, c.dev, 5, nheads=H)
+        for how in (dict(start=_i32([0] * n)), dict(lens=_i32([1] * n))):
+            with pytest.raises(nb.ArgumentError):
+                nb.cache_read(c.dev, 3, **how)
+    c.same()
+    # one sequence does not reach its neighbour's pages
+    one = _array(gen, (dim, 20, 4), BF16)
+    c.write(one, one, 40)
+    c.same()
+    # with a table a call is for as many as that has
+    k, t = _array(gen, (dim, 5, 1), BF16), nb.jl_from_numpy(np.array([[7], [0]], np.int32), device=DEV)
+    nb.cache_write_(c.dev, k, k, table=t)
+    assert torch.equal(nb.cache_read(c.dev, 5, table=t)[0], nb.cache_read(c.dev, 5, start=_i32([0, 0, 16, 0]))[0][:, :, 2:3])
+    # a pool without a batch of its own goes by the call's
+    pool = nb.QuantizedCache.from_arrays(c.dev.k, c.dev.v, c.dev.k_scale, c.dev.v_scale)
+    assert pool.batch is None and nb.QuantizedCache.from_arrays(c.dev.k, c.dev.v, c.dev.k_scale, c.dev.v_scale, batch=B).batch == B
+    k = _array(gen, (dim, 5, 2), BF16)
+    nb.cache_write_(pool, k, k, start=90)
+    at, halves = _i32([90, 90]), nb.jl_from_numpy(np.arange(12, dtype=np.int32).reshape(2, 6).T.copy(), device=DEV)
+    assert torch.equal(nb.cache_read(pool, 5, start=at)[0], nb.cache_read(pool, 5, start=at, table=halves)[0])
+    assert tuple(nb.cache_read(pool, 4)[0].shape) == (dim, 4, 1)
+    held = nb.QuantizedCache.from_arrays(c.dev.k, c.dev.v, c.dev.k_scale, c.dev.v_scale, batch=B)
+    with pytest.raises(nb.ArgumentError):
+        nb.cache_write_(held, k, k)
+    with pytest.raises(nb.ArgumentError):
+        nb.QuantizedCache.from_arrays(c.dev.k, c.dev.v, c.dev.k_scale, c.dev.v_scale, batch=-1)
