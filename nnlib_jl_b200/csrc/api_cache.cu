@@ -116,6 +116,7 @@ int resolve_cache(const nnlib_b200_cache* c, CacheArgs* out) {
   a.table = c->table;
   a.table_stride = c->table_stride ? c->table_stride : c->rows;
   a.rows = c->rows;
+  a.run = c->B > 0 ? c->pages / c->B : 0;
   if (!c->table && c->B > 0 && c->rows > c->pages / c->B) return NNLIB_B200_INVALID_ARG;
   if (c->table && a.table_stride < c->rows && c->B > 1) return NNLIB_B200_INVALID_ARG;
   a.codes[0] = static_cast<unsigned char*>(c->k_codes);

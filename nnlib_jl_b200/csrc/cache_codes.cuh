@@ -11,7 +11,7 @@ constexpr float kScaleTiny = 1.17549435e-38f;     // 2^-126: a smaller scale is 
 
 // Page number p of sequence b; -1: none, or one that the pool does not have.
 __device__ __forceinline__ long long cache_page(const CacheArgs& c, int b, long long p) {
-  const long long n = c.table ? (long long)c.table[p + c.table_stride * b] : c.rows * b + p;
+  const long long n = c.table ? (long long)c.table[p + c.table_stride * b] : c.run * b + p;
   return (n >= 0 && n < c.pages) ? n : -1;
 }
 

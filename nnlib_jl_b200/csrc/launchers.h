@@ -135,6 +135,7 @@ struct CacheArgs {
   const int* table;
   long long table_stride, pages, row;   // row: bytes of a token, d * H
   long long rows;            // pages of a sequence
+  long long run;             // without a table: pages from one sequence's first to the next one's
   int code, d, H, B, log_page;
 };
 struct CacheTokens {

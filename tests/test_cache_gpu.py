@@ -693,3 +693,29 @@ def test_a_call_without_a_table_is_for_the_caches_own_sequences():
         nb.cache_write_(held, k, k)
     with pytest.raises(nb.ArgumentError):
         nb.QuantizedCache.from_arrays(c.dev.k, c.dev.v, c.dev.k_scale, c.dev.v_scale, batch=-1)
+
+
+@gpu
+def test_a_capacity_below_the_run_of_pages():
+    """A sequence's pages begin at (pages / B) * b also where the struct's rows, its capacity, are fewer than pages / B."""
+    gen = np.random.default_rng(35)
+    d, H, T, B = 32, 2, 16, 3
+    c = nb.QuantizedCache(d * H, 64, B, nheads=H, page=T, device=DEV)             # four pages each
+    k, q = _array(gen, (d * H, 50, B), BF16), _array(gen, (d * H, 1, B), BF16)
+    lib, L = nb._lib.load(), nb._lib
+    s = c._call(B, None)
+    s.rows = 2
+    p = L.CacheTokens(dtype=L.BF16, L=50, k=k.data_ptr(), v=k.data_ptr())
+    assert lib.nnlib_b200_cache_write(C.byref(s), C.byref(p), None) == L.OK
+    torch.cuda.synchronize()
+    back = nb.cache_read(c, 50, dtype=F32)[0]
+    assert (back[:, :32] - k[:, :32].float()).abs().max().item() <= 5 / 254 and not back[:, 32:].any()
+    got = nb.jl_zeros((d * H, 50, B), F32, DEV)
+    p = L.CacheTokens(dtype=L.F32, L=50, k=got.data_ptr(), v=got.data_ptr())
+    assert lib.nnlib_b200_cache_read(C.byref(s), C.byref(p), None) == L.OK
+    x = nb.jl_zeros((d * H, 1, B), BF16, DEV)
+    a = L.CacheAttnParams(dtype=L.BF16, causal=0, Hq=H, L=1, q=q.data_ptr(), x=x.data_ptr(), len0=60)
+    assert lib.nnlib_b200_cache_attn_workspace_bytes(C.byref(s), C.byref(a)) == 0
+    assert lib.nnlib_b200_cache_attn(C.byref(s), C.byref(a), None, 0, None) == L.OK
+    torch.cuda.synchronize()
+    assert torch.equal(got, back) and torch.equal(x, nb.cached_attention(q, c, 32, nheads=H, causal=False))
