@@ -513,11 +513,12 @@ cache_attn_kernel(const CacheAttnArgs a, const int teams, const int vec) {
       }
 #pragma unroll
       for (int kg = 0; kg < KG; ++kg) {
-        // E4M3 has a NaN; a slot behind the last token may hold anything
-        if (CODE == NNLIB_B200_E4M3 && key0 + kStep > kend) {
+        // E4M3 has a NaN; a slot behind the last token may hold anything, and so may page 0, which is read in the place of a
+        // page that the pool does not have (its scale is NaN here)
+        if (CODE == NNLIB_B200_E4M3 && (key0 + kStep > kend || !(vs[kg] >= 0.f))) {
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            if (key0 + 16 * kg + 2 * c + (u & 1) + (u >> 1) * 8 >= kend)
+            if (key0 + 16 * kg + 2 * c + (u & 1) + (u >> 1) * 8 >= kend || !(vs[kg] >= 0.f))
 #pragma unroll
               for (int w = 0; w < VB / 4; ++w) vf[kg][u][w] = 0u;
         }
@@ -650,9 +651,9 @@ __global__ void __launch_bounds__(128) cache_merge_kernel(const CacheAttnArgs a,
         for (int j = 0; j < 8; ++j) {
           const float fj = __shfl_sync(0xffffffffu, f, j0 + j), lj = __shfl_sync(0xffffffffu, ml.y, j0 + j);
           // (a sum that is NaN, of a query that sees such a page, counts however small its piece's weight is)
-          if (j0 + j < cnt) {
+          if (j0 + j < cnt && (fj != 0.f || lj != lj)) {
             L = fmaf(fj, lj, L);
-            if (fj != 0.f) acc = fmaf(fj, o[j], acc);
+            acc = fmaf(fj, o[j], acc);
           }
         }
       }

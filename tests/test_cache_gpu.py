@@ -719,3 +719,30 @@ def test_a_capacity_below_the_run_of_pages():
     assert lib.nnlib_b200_cache_attn(C.byref(s), C.byref(a), None, 0, None) == L.OK
     torch.cuda.synchronize()
     assert torch.equal(got, back) and torch.equal(x, nb.cached_attention(q, c, 32, nheads=H, causal=False))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("L", [2, 20, 40])
+def test_a_missing_page_and_a_pool_whose_first_page_holds_no_numbers(dtype, L):
+    """Queries that do not see the missing page are finite, although page 0, which no sequence has, is all NaN codes."""
+    gen = np.random.default_rng(36)
+    d, H, Hq, T, B = 64, 1, 2, 16, 2
+    c = _filled(gen, d * H, 96, B, H, T, "e4m3", True)
+    spare = [p for p in range(c.dev.pages) if p not in c.table][0]
+    if (c.table == 0).any():                                     # page 0 gives its place to one that is not used
+        for t, host in zip((c.dev.k.view(torch.uint8), c.dev.v.view(torch.uint8)), c.codes):
+            t[:, :, spare] = t[:, :, 0]
+            host[:, :, spare] = host[:, :, 0]
+        for t, host in zip((c.dev.k_scale, c.dev.v_scale), c.scale):
+            t[:, spare] = t[:, 0]
+            host[:, spare] = host[:, 0]
+        c.table[c.table == 0] = spare
+    for t, host in zip((c.dev.k, c.dev.v), c.codes):
+        t.view(torch.uint8)[:, :, 0] = 0x7f
+        host[:, :, 0] = NAN
+    c.table[5, 0], c.table[3, 1] = -1, 10 ** 6
+    q = _array(gen, (d * Hq, L, B), dtype)
+    lens = [80 + min(L // 2, 16), 48 + min(L // 2, 16)]
+    x, _ = c.attend(q, lens, Hq)
+    assert torch.isfinite(x[:, 0].float()).all() and torch.isnan(x[:, -1].float()).all()
