@@ -766,8 +766,8 @@ bool cache_attn_umma_path(const CacheAttnArgs& a, int dtype) { return use_umma(a
 
 size_t cache_attn_workspace_bytes(const CacheAttnArgs& a, int dtype) {
   if (use_umma(a, dtype)) {
-    const int n = cache_umma_splits(a, dtype);
-    return n == 1 ? 0 : sizeof(float) * (size_t)split_ws_floats(reduce_args(a), n);
+    const int n = cache_umma_splits(a);
+    return cache_umma_parts(a, dtype, n) ? sizeof(float) * (size_t)split_ws_floats(reduce_args(a), n) : 0;
   }
   if (one_launch(a, dtype)) return 0;
   const int width = row_tile(a, dtype), rows = a.L * (a.Hq / a.c.H);
@@ -777,7 +777,7 @@ size_t cache_attn_workspace_bytes(const CacheAttnArgs& a, int dtype) {
 
 cudaError_t cache_attn(CacheAttnArgs a, int dtype, cudaStream_t st) {
   if (use_umma(a, dtype)) {
-    const int n = cache_umma_splits(a, dtype);
+    const int n = cache_umma_splits(a);
     const cudaError_t e = cache_umma(a, dtype, n, st);
     if (e != cudaSuccess || n == 1) return e;
     return dtype == NNLIB_B200_F16 ? reduce<__half>(a, n, st) : reduce<__nv_bfloat16>(a, n, st);

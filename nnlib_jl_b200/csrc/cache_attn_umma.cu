@@ -20,6 +20,11 @@
 // sequences, 32 / 8 heads of 128, bf16 over Int8: 2.30 ms, 719 TFLOP/s.  With sixteen softmax warps, two threads to a row, 2.26,
 // but 512 queries over up to 16384 tokens in E4M3 0.75 instead of 0.64; with eight converting warps 2.50 and 0.75.
 // A scale serves 16 keys at least (64 where the pages allow: SG), so a thread scales and sums by groups of SG keys.
+// The products' additions cut off instead of rounding, always towards zero: behind n keys that one accumulator has summed x is
+// short by some n 2^-27.2 where all values have one sign (1024 queries, values 0.5 and above: 2.1e-4 behind 32768 keys, 8.7e-4
+// behind 131072; half a step of Float16 is 4.9e-4).  So every 32768 keys (BFloat16, whose step is eight times as large: 262144)
+// the tensor memory's sums are added, rounded, to a Float32 row of the block's own in the workspace and begun anew, which
+// keeps that below half of half a step for histories of any length.
 // Weights leave with a factor of 2^10 and the running maximum is raised when it grew by more than 2^4: they are below 2^14
 // and keep 11 bits down to 2^-24 of the largest.
 #include <algorithm>
@@ -40,6 +45,8 @@ constexpr int kThreadsC = 512, kTiles = 2;
 constexpr float kGap = 4.f, kBits = 10.f;
 constexpr float kValueFloorU = 7.8886090522101181e-31f;   // 2^-100
 constexpr int kMetaTiles = 8;
+template <typename T>
+constexpr int kFoldTiles = std::is_same<T, __half>::value ? 256 : 2048;      // tiles of keys that tensor memory sums up (a power of two)
 constexpr int kWaves = 6;                // fewer waves of blocks than these are put in order by their lengths
 
 struct __align__(16) PageMeta {
@@ -87,10 +94,10 @@ __device__ __forceinline__ void codes4(uint32_t w, uint32_t& p0, uint32_t& p1) {
 // would spoil rows that give them no weight) or, behind the last one of a group of SG keys, that one once more.
 __device__ const uint4 g_zero_codes[16] = {};
 
-template <int D, int CODE, int STAGES, int SG>
+template <int D, int CODE, int SG>
 __device__ __forceinline__ void convert_tiles(const CacheArgs& cc, const unsigned char* base, uint8_t* ring, const PageMeta* meta,
                                               uint64_t* full, uint64_t* empty, uint64_t* meta_full, volatile int* abort_flag,
-                                              int w, int lane, int j_lo, int n_kv, int len) {
+                                              int stages, int w, int lane, int j_lo, int n_kv, int len) {
   constexpr int N = D == 128 ? 16 : 8, AHEAD = 8;     // loads of a tile, and how many are under way
   constexpr int kTileBytes = CfgC<D>::kTileBytes;
   const int key8 = lane >> 2, piece = lane & 3;
@@ -123,10 +130,11 @@ __device__ __forceinline__ void convert_tiles(const CacheArgs& cc, const unsigne
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) load(raw[i], 0, n0 / 8, i);
   }
+  int s = 0;
+  uint32_t phase = 1;                        // of the stage's last release: none is waited for in the first round
 #pragma unroll 1
   for (int j = 0; j < n_kv && ok; ++j) {
-    const int s = j % STAGES;
-    if (j >= STAGES) ok = mbar_wait_warp(&empty[s], ((j / STAGES) - 1) & 1, abort_flag);
+    if (j >= stages) ok = mbar_wait_warp(&empty[s], phase, abort_flag);
     if (ok && j + 1 < n_kv && ((j + 1) & 3) == 0) ok = mbar_wait_warp(&meta_full[((j + 1) >> 2) & 1], ((j + 1) >> 3) & 1, abort_flag);
     if (!ok) break;
 #pragma unroll 1
@@ -150,6 +158,10 @@ __device__ __forceinline__ void convert_tiles(const CacheArgs& cc, const unsigne
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(&full[s]);
+    if (++s == stages) {
+      s = 0;
+      phase ^= 1;
+    }
   }
 }
 
@@ -158,6 +170,7 @@ template <typename T, int D, int CODE, int SG>
 __global__ void __launch_bounds__(kThreadsC, 1) cache_attn_umma_kernel(const CacheAttnArgs a, const int splits, const int vec) {
   using C = CfgC<D>;
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kFold = kFoldTiles<T>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   BarsC* bars = reinterpret_cast<BarsC*>(smem + C::kBarOff);
@@ -340,7 +353,7 @@ __global__ void __launch_bounds__(kThreadsC, 1) cache_attn_umma_kernel(const Cac
           ok = mbar_wait(&bb->p_half[t][0], par, abort_flag);
           if (!ok) continue;
           tc_fence_after();
-          issue_pv(t, sv, 0, j == 0);
+          issue_pv(t, sv, 0, (j & (kFold - 1)) == 0);
           ok = mbar_wait(&bb->p_half[t][1], par, abort_flag);
           if (!ok) continue;
           tc_fence_after();
@@ -362,13 +375,11 @@ __global__ void __launch_bounds__(kThreadsC, 1) cache_attn_umma_kernel(const Cac
   } else if (warp >= 12) {
     setmaxnreg_dec<112>();
     if (start_ok) {
-      const int w = (warp - 12) & 1;
-      if (warp < 14)
-        convert_tiles<D, CODE, C::kStagesK, SG>(cc, cc.codes[0] + (long long)h * cc.d, smem + C::kKOff, meta, bars->k_full,
-                                            bars->k_empty, bars->meta_full, abort_flag, w, lane, j_lo, n_kv, len);
-      else
-        convert_tiles<D, CODE, C::kStagesV, SG>(cc, cc.codes[1] + (long long)h * cc.d, smem + C::kVOff, meta, bars->v_full,
-                                            bars->v_empty, bars->meta_full, abort_flag, w, lane, j_lo, n_kv, len);
+      // (one piece of code for both sides: two keep every warp waiting for instructions)
+      const bool v = warp >= 14;
+      convert_tiles<D, CODE, SG>(cc, (v ? cc.codes[1] : cc.codes[0]) + (long long)h * cc.d, smem + (v ? C::kVOff : C::kKOff), meta,
+                                 v ? bars->v_full : bars->k_full, v ? bars->v_empty : bars->k_empty, bars->meta_full, abort_flag,
+                                 v ? C::kStagesV : C::kStagesK, (warp - 12) & 1, lane, j_lo, n_kv, len);
     }
   } else {
     setmaxnreg_inc<168>();
@@ -430,10 +441,73 @@ __global__ void __launch_bounds__(kThreadsC, 1) cache_attn_umma_kernel(const Cac
         if (lane == 0) mbar_arrive(&bars->q_full[t]);
       }
 
+      // Where this thread's row has its partial results in the workspace: (maximum, sum) and, behind all of these, outputs.  What
+      // tensor memory had summed up so far is there, too, with the maximum that it refers to.  (The row is worked out anew, so that
+      // nothing of it lives in registers beside a score row.)
+      struct Part {
+        float *ml, *o;
+        int row, i, hq;
+        long long unit;
+      };
+      auto part = [&]() {
+        int tid = threadIdx.x;
+        asm volatile("" : "+r"(tid));
+        Part p;
+        p.row = row0 + ((tid - 128) & 255);
+        const int r = p.row < rows ? p.row : 0;
+        p.i = r / G;
+        p.hq = h * G + r % G;
+        p.unit = p.hq + (long long)a.Hq * b;
+        const long long at = (p.unit * splits + split) * a.L + p.i;
+        p.ml = a.ws + at * 2;
+        p.o = a.ws + ((((long long)a.Hq * cc.B * splits * a.L * 2) + 3) & ~3LL) + at * cc.d;
+        return p;
+      };
+      // what such sums are multiplied by beside a maximum that has grown to m
+      auto since = [](float then, float m) { return then == m ? 1.f : ex2_approx(then - m); };
+
       float m_used = neg_inf(), l = 0.f;
       bool ok = true;
+      // (a loop around the loop over the tiles: a step that is rarely taken inside it costs its code 4 % and more)
 #pragma unroll 1
-      for (int j = 0; j < nt; ++j) {
+      for (int j_from = 0; j_from < nt && ok; j_from += kFold) {
+      if (j_from > 0) {
+        // the products of the tiles so far are done when the scores of the next one are; that one's begin the sums anew
+        ok = mbar_wait(&bars->s_full[t], 0, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        if (!idle) {
+          const Part p = part();
+          const bool row_ok = p.row < rows, more = j_from > kFold;
+          float f = 0.f;
+          if (row_ok) {
+            if (more) f = since(p.ml[0], m_used);
+            p.ml[0] = m_used;
+          }
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(tO + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              if (!row_ok || c * 32 + e >= cc.d) continue;
+              float4* to = reinterpret_cast<float4*>(p.o + c * 32 + e);
+              float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (more) s = *to;
+              s.x = fmaf(s.x, f, __uint_as_float(o[e]));
+              s.y = fmaf(s.y, f, __uint_as_float(o[e + 1]));
+              s.z = fmaf(s.z, f, __uint_as_float(o[e + 2]));
+              s.w = fmaf(s.w, f, __uint_as_float(o[e + 3]));
+              *to = s;
+            }
+          }
+        }
+      }
+      const int j_to = min(nt, j_from + kFold);
+#pragma unroll 1
+      for (int j = j_from; j < j_to; ++j) {
         uint8_t* sm = smem;
         asm volatile("" : "+l"(sm));         // (no barrier's address in a register for good)
         BarsC* bb = reinterpret_cast<BarsC*>(sm + C::kBarOff);
@@ -542,6 +616,7 @@ __global__ void __launch_bounds__(kThreadsC, 1) cache_attn_umma_kernel(const Cac
           if (lane == 0) mbar_arrive(&bb->p_half[t][hf]);
         }
       }
+      }
 
       // -------------------------------------------------- epilogue
       if (ok && nt > 0) {
@@ -551,25 +626,21 @@ __global__ void __launch_bounds__(kThreadsC, 1) cache_attn_umma_kernel(const Cac
       if (ok) {
         tc_fence_after();
         const bool dead = l == 0.f;
-        // (worked out anew, so that nothing of it lives in registers beside a score row)
-        int tid = threadIdx.x;
-        asm volatile("" : "+r"(tid));
-        const int row = row0 + ((tid - 128) & 255), i = row < rows ? row / G : 0, hq = h * G + (row < rows ? row % G : 0);
-        const bool row_ok = row < rows;
-        const long long unit = hq + (long long)a.Hq * b, at = (unit * splits + split) * a.L + i;
-        float* wrow = nullptr;
+        const Part p = part();
+        const bool row_ok = p.row < rows, folded = nt > kFold;
+        float f_since = 0.f;
+        if (folded && row_ok) f_since = since(p.ml[0], m_used);
         T* xrow = nullptr;
         float inv = 1.f;
         if (splits > 1) {
-          wrow = a.ws + ((((long long)a.Hq * cc.B * splits * a.L * 2) + 3) & ~3LL) + at * cc.d;
           if (row_ok) {
-            a.ws[at * 2] = m_used - kBits;              // (l has that factor)
-            a.ws[at * 2 + 1] = l;
+            p.ml[0] = m_used - kBits;              // (l has that factor)
+            p.ml[1] = l;
           }
         } else {
-          xrow = reinterpret_cast<T*>(a.x) + (long long)i * a.x_sl + (long long)b * a.x_sb + (long long)hq * cc.d;
+          xrow = reinterpret_cast<T*>(a.x) + (long long)p.i * a.x_sl + (long long)b * a.x_sb + (long long)p.hq * cc.d;
           inv = dead ? (a.nan_fm ? __int_as_float(0x7fc00000) : 0.f) : 1.f / l;
-          if (row_ok && a.lse) a.lse[i + (long long)a.L * unit] = dead ? neg_inf() : (m_used - kBits + log2f(l)) * kLn2;
+          if (row_ok && a.lse) a.lse[p.i + (long long)a.L * p.unit] = dead ? neg_inf() : (m_used - kBits + log2f(l)) * kLn2;
         }
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
@@ -582,11 +653,15 @@ __global__ void __launch_bounds__(kThreadsC, 1) cache_attn_umma_kernel(const Cac
           for (int e = 0; e < 32; e += 8) {
             if (!row_ok || c * 32 + e >= cc.d) continue;
             float f[8];
+            if (folded) {
+#pragma unroll
+              for (int u = 0; u < 8; ++u) o[e + u] = __float_as_uint(fmaf(p.o[c * 32 + e + u], f_since, __uint_as_float(o[e + u])));
+            }
 #pragma unroll
             for (int u = 0; u < 8; ++u) f[u] = dead ? (splits > 1 ? 0.f : inv) : __uint_as_float(o[e + u]) * inv;
             if (splits > 1) {
-              *reinterpret_cast<float4*>(wrow + c * 32 + e) = make_float4(f[0], f[1], f[2], f[3]);
-              *reinterpret_cast<float4*>(wrow + c * 32 + e + 4) = make_float4(f[4], f[5], f[6], f[7]);
+              *reinterpret_cast<float4*>(p.o + c * 32 + e) = make_float4(f[0], f[1], f[2], f[3]);
+              *reinterpret_cast<float4*>(p.o + c * 32 + e + 4) = make_float4(f[4], f[5], f[6], f[7]);
             } else if (vec) {
               *reinterpret_cast<uint4*>(xrow + c * 32 + e) =
                   make_uint4(pack2<BF16>(f[0], f[1]), pack2<BF16>(f[2], f[3]), pack2<BF16>(f[4], f[5]), pack2<BF16>(f[6], f[7]));
@@ -638,23 +713,29 @@ cudaError_t launch_c(const CacheAttnArgs& a, int splits, cudaStream_t st) {
   return a.c.code == NNLIB_B200_INT8 ? launch_d<T, NNLIB_B200_INT8>(a, splits, st) : launch_d<T, NNLIB_B200_E4M3>(a, splits, st);
 }
 
+// keys of a sequence at most
+long long most_keys(const CacheAttnArgs& a) {
+  const long long cap = a.c.rows << a.c.log_page;
+  return a.lens ? cap : std::min(cap, std::max(a.len0, 0LL));
+}
+
 }  // namespace
 
 bool cache_umma_supports(const CacheAttnArgs& a, int dtype) { return dtype != NNLIB_B200_F32 && a.c.d <= 128; }
 
-// Blocks of keys of a unit: where there are too few blocks of rows to fill the GPU, with four tiles of keys each at least; and
-// so many that a block's sums stay short.  The products' additions cut off instead of rounding, and behind n keys of a block x is
-// short by some n 2^-27.2 where all values have one sign (1024 queries, values 0.5 and above: 2.1e-4 with 32768 keys a block,
-// 8.7e-4 with 131072; half a step of Float16 is 4.9e-4).  32768 keys a block, 262144 for BFloat16, whose step is eight times as
-// large, keep that below half of half a step; joining the parts moves 8 bytes where a block did 4 * 32768 operations or more.
-int cache_umma_splits(const CacheAttnArgs& a, int dtype) {
+// Blocks of keys of a unit: where there are too few blocks of rows to fill the GPU, with four tiles of keys each at least.
+// What the host knows of the lengths is the capacity, or len0.
+int cache_umma_splits(const CacheAttnArgs& a) {
   const long long rows = (long long)a.L * (a.Hq / a.c.H);
   const long long blocks = (rows + kTiles * kBM - 1) / (kTiles * kBM) * a.c.B * a.c.H;
-  const long long most = dtype == NNLIB_B200_F16 ? 32768 : 262144;
-  long long cap = a.c.rows << a.c.log_page;
-  if (!a.lens) cap = std::min(cap, std::max(a.len0, 0LL));
-  const long long n = std::min(148 / std::max(blocks, 1LL), cap / (4 * kBN));
-  return (int)std::max(std::max(1LL, std::min(n, 64LL)), (cap + most - 1) / most);
+  const long long n = std::min(148 / std::max(blocks, 1LL), most_keys(a) / (4 * kBN));
+  return (int)std::max(1LL, std::min(n, 64LL));
+}
+
+// Does a block have, or may it have, partial results in the workspace?
+bool cache_umma_parts(const CacheAttnArgs& a, int dtype, int splits) {
+  const long long tiles = ((most_keys(a) + kBN - 1) / kBN + splits - 1) / splits;
+  return splits > 1 || tiles > (dtype == NNLIB_B200_F16 ? kFoldTiles<__half> : kFoldTiles<__nv_bfloat16>);
 }
 
 cudaError_t cache_umma(const CacheAttnArgs& a, int dtype, int splits, cudaStream_t st) {

@@ -169,7 +169,8 @@ size_t cache_attn_workspace_bytes(const CacheAttnArgs& a, int dtype);   // (cach
 cudaError_t cache_attn(CacheAttnArgs a, int dtype, cudaStream_t st);          // a.ws holds the workspace
 bool cache_attn_umma_path(const CacheAttnArgs& a, int dtype);                 // which of the two it takes
 bool cache_umma_supports(const CacheAttnArgs& a, int dtype);                  // tcgen05 (cache_attn_umma.cu): 16-bit, d <= 128
-int cache_umma_splits(const CacheAttnArgs& a, int dtype);
+int cache_umma_splits(const CacheAttnArgs& a);
+bool cache_umma_parts(const CacheAttnArgs& a, int dtype, int splits);         // it needs a workspace
 cudaError_t cache_umma(const CacheAttnArgs& a, int dtype, int splits, cudaStream_t st);   // partial results only, if splits > 1
 cudaError_t cache_umma_take_abort(int* out, cudaStream_t st);
 

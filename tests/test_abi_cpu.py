@@ -366,3 +366,20 @@ def test_cache_argument_checks_without_a_gpu(lib):
     assert lib.nnlib_b200_cache_write(C.byref(_cache(rows=0, pages=0, k_codes=None, v_codes=None, k_scale=None, v_scale=None)),
                                       C.byref(_tokens(L=0)), None) == _lib.OK
     assert lib.nnlib_b200_launch_count() == before
+
+
+def test_cache_attention_workspace_does_not_grow_with_the_table(lib):
+    """A table has the rows of the longest history that a server serves.  Many queries: at most one Float32 row of partial
+    outputs, with a maximum and a sum, for each row of x (or, where few blocks share the GPU, for two rows to each of its SMs)."""
+    def need(tokens, dtype, B, L, Hq=32, H=8, d=128, **kw):
+        c = _cache(code=_lib.INT8, d=d, H=H, page=64, pages=1 << 20, B=B, rows=tokens // 64, table=0x1000, table_stride=1 << 24)
+        p = _cache_attn(dtype=dtype, Hq=Hq, L=L, lens=0x1000, **kw)
+        assert lib.nnlib_b200_cache_attn_path(C.byref(c), C.byref(p)) == _lib.PATH_UMMA
+        return lib.nnlib_b200_cache_attn_workspace_bytes(C.byref(c), C.byref(p))
+    for dtype, most in ((_lib.F16, 1 << 15), (_lib.BF16, 1 << 18)):
+        for B, L in ((4, 4096), (8, 1024), (3, 777)):
+            rows = 32 * B * L * (128 + 2) * 4 + 16
+            assert need(most, dtype, B, L) == 0
+            assert 0 < need(2 * most, dtype, B, L) <= rows
+            assert need(2 * most, dtype, B, L) == need(1 << 20, dtype, B, L) == need(1 << 24, dtype, B, L)
+        assert 0 < need(1 << 20, dtype, 1, 64, Hq=8, H=1) <= 2 * 148 * 256 * (128 + 2) * 4

@@ -746,3 +746,52 @@ def test_a_missing_page_and_a_pool_whose_first_page_holds_no_numbers(dtype, L):
     lens = [80 + min(L // 2, 16), 48 + min(L // 2, 16)]
     x, _ = c.attend(q, lens, Hq)
     assert torch.isfinite(x[:, 0].float()).all() and torch.isnan(x[:, -1].float()).all()
+
+
+@gpu
+@pytest.mark.parametrize("loud", [1, 200])
+@pytest.mark.parametrize("dtype,n", [(F16, 300032), (BF16, 600064)])
+def test_sums_of_a_very_long_history_that_one_block_walks_over(dtype, n, loud):
+    """Rows enough that no block's keys are cut into parts; positive values, so that additions that cut off shrink every
+    element alike, by 2^-27 of it for each key that the products sum up by themselves: 32768 (Float16), 262144 (BFloat16).
+    ``loud``: the last third's logits are that much larger, so that a maximum rises behind sums that have been put aside;
+    there sum |q||k| scale <= 9 (0.64 * 200 * 2^-7 * 32 / sqrt(32), half as much again), which moves weights by 2 * 9 * 2^-18 < 2^-13.
+    The results' roundings leave half a step / sqrt(3 * 32) in the mean, as in the test above."""
+    d, Hq, L = 32, 8, 2400
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    c = nb.QuantizedCache(d, n, 1, nheads=1, page=64, eltype=torch.int8, device=DEV)
+    k, v = (nb.jl_empty((d, n, 1), F16, DEV).normal_(generator=gen) for _ in range(2))
+    nb.cache_write_(c, k, v.abs() + 0.5)
+    c.k_scale[:, n // 96:] *= loud
+    q = (nb.jl_empty((d * Hq, L, 1), F32, DEV).normal_(generator=gen) * 2.0 ** -7).to(dtype)
+    x = nb.cached_attention(q, c, n, nheads=Hq, causal=False)
+    nb.device_health()
+    kr, vr = (t[:, :, 0].double() for t in nb.cache_read(c, n, dtype=F32))
+    at = torch.arange(0, L, 61, device=DEV)
+    rows = q[:, at, 0].double().reshape(Hq, d, -1)
+    want = torch.stack([torch.softmax(r.T @ kr / d ** 0.5, 1) @ vr.T for r in rows])
+    off = x[:, at, 0].double().reshape(Hq, d, -1).transpose(1, 2) / want - 1
+    half, sums = (2.0 ** -11, 2.0 ** -12) if dtype == F16 else (2.0 ** -8, 2.0 ** -9)
+    logits = 2.0 ** -13 if loud > 1 else 0
+    assert off.abs().max().item() <= half + sums + logits, (off.abs().max().item(), off.mean().item())
+    assert abs(off.mean().item()) <= sums + logits + 3 * half / 96 ** 0.5, off.mean().item()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_short_histories_in_a_table_for_long_ones(dtype):
+    """The same bits as with a table that just fits (blocks enough that keys are not cut into parts)."""
+    gen = np.random.default_rng(37)
+    d, H, L, cap, B, T = 16, 64, 45, 640, 2, 64
+    c = _filled(gen, d * H, cap, B, H, T, "int8", True)
+    q = _array(gen, (d * H, L, B), dtype)
+    wide = nb.jl_empty(((1 << 20) // T, B), torch.int32, DEV)
+    wide.fill_(-1)
+    wide[:c.table.shape[0]] = c.t
+    assert _path(c, q, H) == nb._lib.PATH_UMMA           # (also with the small table)
+    for lens in ([640, 100], [45, 0]):
+        want = nb.cached_attention(q, c.dev, _i32(lens), nheads=H, table=c.t, return_lse=True)
+        got = nb.cached_attention(q, c.dev, _i32(lens), nheads=H, table=wide, return_lse=True)
+        for g, w in zip(got, want):
+            assert torch.equal(torch.nan_to_num(g, nan=7.0), torch.nan_to_num(w, nan=7.0))
+    c.attend(q, [640, 100], H)
