@@ -19,6 +19,9 @@
 //   O^T += V^T W^T  rows may be any features: rows g and g + 8 of product j are features g (D/8) + 2j and the next, so a lane
 //                 loads D/8 consecutive bytes of each of its four keys 2c, 2c+1, 2c+8, 2c+9 and pairs the codes of two keys
 //                 up.  W^T comes from S^T's layout by transposing 8 x 8 blocks.
+// The products' additions cut off instead of rounding, by up to 2^-23 of the sum behind sixteen keys.  So a warp of a 16-bit
+// call adds what it has to its part of shared memory, rounded, every 32768 keys, which leaves 2^-12 however long the history
+// is (nine sequences of 1048576 tokens, a team to each: Float16 1.5e-3 off before).
 // Columns: the query heads of a group and the queries, column r = query r / G, head r % G of the group; NT blocks of eight.
 // Int8 to 16 bits: (code ^ 0x80) under 0x64 is 1024 + 128 + code, less 1152.  E4M3: the conversion instruction.
 // Lengths are known on the device only, and a block more than fit at once costs a second wave.  So the blocks, as many as
@@ -409,150 +412,178 @@ cache_attn_kernel(const CacheAttnArgs a, const int teams, const int vec) {
       for (int u = 0; u < 2; ++u) lim_all = min(lim_all, lim[t][u]);
     lim_all = __reduce_min_sync(0xffffffffu, lim_all);
 
-    for (int n = 0; key0 < key_hi; key0 += stride, ++n) {
-      float ks[KG], vs[KG];
+    // Products' additions cut off (below), so a warp of a 16-bit call sums up 32768 keys by them; what it has is then added,
+    // rounded, to its part of shared memory, with the maximum that it refers to, and begun anew.
+    constexpr int kFold = 32768 / kStep;
+    auto since = [](float then, float now) { return then == now ? 1.f : ex2(then - now); };
+    int n = 0;
+    for (;;) {
+      const int key_stop = HL == 1 && key_hi - key0 > kFold * stride ? key0 + kFold * stride : key_hi;
+      for (; key0 < key_stop; key0 += stride, ++n) {
+        float ks[KG], vs[KG];
 #pragma unroll
-      for (int kg = 0; kg < KG; ++kg) {
-        ks[kg] = __shfl_sync(0xffffffffu, ksc, (n * KG + kg) & 31);
-        vs[kg] = __shfl_sync(0xffffffffu, vsc, (n * KG + kg) & 31);
-      }
-      const int next = key0 + stride;
-      if (next < key_hi) {
-        if (((n + 1) * KG & 31) == 0) look_up(next);
-        place(next, n + 1);
-      }
+        for (int kg = 0; kg < KG; ++kg) {
+          ks[kg] = __shfl_sync(0xffffffffu, ksc, (n * KG + kg) & 31);
+          vs[kg] = __shfl_sync(0xffffffffu, vsc, (n * KG + kg) & 31);
+        }
+        const int next = key0 + stride;
+        if (next < key_hi) {
+          if (((n + 1) * KG & 31) == 0) look_up(next);
+          place(next, n + 1);
+        }
 
-      float sc[KG][NT][4];
-#pragma unroll
-      for (int kg = 0; kg < KG; ++kg) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[kg][t][e] = 0.f;
-#pragma unroll
-        for (int k2 = 0; k2 < KS; ++k2) {
-          uint32_t a0, a1, a2, a3;
-          word_pairs<CODE>(kf[kg][0][k2 / 4][k2 % 4], a0, a2);
-          word_pairs<CODE>(kf[kg][1][k2 / 4][k2 % 4], a1, a3);
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int hl = 0; hl < HL; ++hl) mma(sc[kg][t], a0, a1, a2, a3, qb[t][hl][k2][0], qb[t][hl][k2][1]);
-        }
-      }
-      if (next < key_hi) load_k();
-
-      // scales of this step's pages (sixteen keys never cross one)
-      float lvs[KG], ivs[KG];
-#pragma unroll
-      for (int kg = 0; kg < KG; ++kg) {
-        const float vse = vs[kg] >= kValueFloor ? vs[kg] : ((vs[kg] >= 0.f) ? kValueFloor : qnan());
-        lvs[kg] = __log2f(vse) + kWeightBits;
-        ivs[kg] = __fdividef(1.f, vse);
-      }
-      const bool edge = key0 + kStep - 1 > lim_all;
-      uint32_t pb[KG][NT][HL][2];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        // w[.][e]: key g (+ 8 for e >= 2), column 2c (+ 1 for odd e)
-        float w[KG][4];
-#pragma unroll
-        for (int kg = 0; kg < KG; ++kg)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w[kg][e] = fmaf(sc[kg][t][e], crow[t][e & 1] * ks[kg], lvs[kg]);
-        if (edge) {
-#pragma unroll
-          for (int kg = 0; kg < KG; ++kg)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (key0 + 16 * kg + g + (e >> 1) * 8 > lim[t][e & 1]) w[kg][e] = ninf();
-        }
-        float mn[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          float mx = fmaxf(w[0][u], w[0][2 + u]);
-          if (KG == 2) mx = fmaxf(mx, fmaxf(w[KG - 1][u], w[KG - 1][2 + u]));
-#pragma unroll
-          for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-          mn[u] = fmaxf(m[t][u], mx - kWeightBits);
-        }
-        if (__any_sync(0xffffffffu, mn[0] > m[t][0] || mn[1] > m[t][1])) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const float fo = (m[t][u] == ninf()) ? 0.f : ex2(m[t][u] - mn[u]);
-            l[t][u] *= fo;
-#pragma unroll
-            for (int j = 0; j < D / 16; ++j) {
-              o[t][j][u] *= fo;
-              o[t][j][2 + u] *= fo;
-            }
-            m[t][u] = mn[u];
-          }
-        }
-        const float ref[2] = {mn[0] == ninf() ? 0.f : mn[0], mn[1] == ninf() ? 0.f : mn[1]};
+        float sc[KG][NT][4];
 #pragma unroll
         for (int kg = 0; kg < KG; ++kg) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[kg][e] = ex2(w[kg][e] - ref[e & 1]);
-          // this lane's keys only; a page that the query does not see adds nothing, whatever its scale is
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[kg][t][e] = 0.f;
+#pragma unroll
+          for (int k2 = 0; k2 < KS; ++k2) {
+            uint32_t a0, a1, a2, a3;
+            word_pairs<CODE>(kf[kg][0][k2 / 4][k2 % 4], a0, a2);
+            word_pairs<CODE>(kf[kg][1][k2 / 4][k2 % 4], a1, a3);
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int hl = 0; hl < HL; ++hl) mma(sc[kg][t], a0, a1, a2, a3, qb[t][hl][k2][0], qb[t][hl][k2][1]);
+          }
+        }
+        if (next < key_hi) load_k();
+
+        // scales of this step's pages (sixteen keys never cross one)
+        float lvs[KG], ivs[KG];
+#pragma unroll
+        for (int kg = 0; kg < KG; ++kg) {
+          const float vse = vs[kg] >= kValueFloor ? vs[kg] : ((vs[kg] >= 0.f) ? kValueFloor : qnan());
+          lvs[kg] = __log2f(vse) + kWeightBits;
+          ivs[kg] = __fdividef(1.f, vse);
+        }
+        const bool edge = key0 + kStep - 1 > lim_all;
+        uint32_t pb[KG][NT][HL][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          // w[.][e]: key g (+ 8 for e >= 2), column 2c (+ 1 for odd e)
+          float w[KG][4];
+#pragma unroll
+          for (int kg = 0; kg < KG; ++kg)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[kg][e] = fmaf(sc[kg][t][e], crow[t][e & 1] * ks[kg], lvs[kg]);
+          if (edge) {
+#pragma unroll
+            for (int kg = 0; kg < KG; ++kg)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (key0 + 16 * kg + g + (e >> 1) * 8 > lim[t][e & 1]) w[kg][e] = ninf();
+          }
+          float mn[2];
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const float sum = w[kg][u] + w[kg][2 + u];
-            if (!(sum == 0.f)) l[t][u] = fmaf(sum, ivs[kg], l[t][u]);
+            float mx = fmaxf(w[0][u], w[0][2 + u]);
+            if (KG == 2) mx = fmaxf(mx, fmaxf(w[KG - 1][u], w[KG - 1][2 + u]));
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+            mn[u] = fmaxf(m[t][u], mx - kWeightBits);
           }
+          if (__any_sync(0xffffffffu, mn[0] > m[t][0] || mn[1] > m[t][1])) {
 #pragma unroll
-          for (int hl = 0; hl < HL; ++hl) {
-            pb[kg][t][hl][0] = transposed(half2_bits(w[kg][0], w[kg][1]));
-            pb[kg][t][hl][1] = transposed(half2_bits(w[kg][2], w[kg][3]));
-            if (HILO && hl == 0) {
+            for (int u = 0; u < 2; ++u) {
+              const float fo = (m[t][u] == ninf()) ? 0.f : ex2(m[t][u] - mn[u]);
+              l[t][u] *= fo;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) w[kg][e] -= __half2float(__float2half_rn(w[kg][e]));
+              for (int j = 0; j < D / 16; ++j) {
+                o[t][j][u] *= fo;
+                o[t][j][2 + u] *= fo;
+              }
+              m[t][u] = mn[u];
             }
           }
-        }
-      }
+          const float ref[2] = {mn[0] == ninf() ? 0.f : mn[0], mn[1] == ninf() ? 0.f : mn[1]};
 #pragma unroll
-      for (int kg = 0; kg < KG; ++kg) {
-        // E4M3 has a NaN; a slot behind the last token may hold anything, and so may page 0, which is read in the place of a
-        // page that the pool does not have (its scale is NaN here)
-        if (CODE == NNLIB_B200_E4M3 && (key0 + kStep > kend || !(vs[kg] >= 0.f))) {
+          for (int kg = 0; kg < KG; ++kg) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (key0 + 16 * kg + 2 * c + (u & 1) + (u >> 1) * 8 >= kend || !(vs[kg] >= 0.f))
+            for (int e = 0; e < 4; ++e) w[kg][e] = ex2(w[kg][e] - ref[e & 1]);
+            // this lane's keys only; a page that the query does not see adds nothing, whatever its scale is
 #pragma unroll
-              for (int w = 0; w < VB / 4; ++w) vf[kg][u][w] = 0u;
-        }
+            for (int u = 0; u < 2; ++u) {
+              const float sum = w[kg][u] + w[kg][2 + u];
+              if (!(sum == 0.f)) l[t][u] = fmaf(sum, ivs[kg], l[t][u]);
+            }
 #pragma unroll
-        for (int w = 0; w < VB / 4; ++w) {
-          // the codes of keys 2c and 2c + 1 side by side, features 4w .. 4w + 3
-          const uint32_t a01 = __byte_perm(vf[kg][0][w], vf[kg][1][w], 0x5140), a23 = __byte_perm(vf[kg][0][w], vf[kg][1][w], 0x7362);
-          const uint32_t b01 = __byte_perm(vf[kg][2][w], vf[kg][3][w], 0x5140), b23 = __byte_perm(vf[kg][2][w], vf[kg][3][w], 0x7362);
-          uint32_t lo[4], hi[4];
-          word_pairs<CODE>(a01, lo[0], lo[1]);
-          word_pairs<CODE>(a23, lo[2], lo[3]);
-          word_pairs<CODE>(b01, hi[0], hi[1]);
-          word_pairs<CODE>(b23, hi[2], hi[3]);
+            for (int hl = 0; hl < HL; ++hl) {
+              pb[kg][t][hl][0] = transposed(half2_bits(w[kg][0], w[kg][1]));
+              pb[kg][t][hl][1] = transposed(half2_bits(w[kg][2], w[kg][3]));
+              if (HILO && hl == 0) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              if constexpr (HL == 1) {
-                mma(o[t][2 * w + j], lo[2 * j], lo[2 * j + 1], hi[2 * j], hi[2 * j + 1], pb[kg][t][0][0], pb[kg][t][0][1]);
-              } else {
-                // The products' own addition cuts off instead of rounding: over a long run the sum shrinks by a part of
-                // 2^-24 a step (2e-5 of x behind 99163 keys).  Float32 sums are added up with rounded additions.
-                float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int hl = 0; hl < HL; ++hl)
-                  mma(part, lo[2 * j], lo[2 * j + 1], hi[2 * j], hi[2 * j + 1], pb[kg][t][hl][0], pb[kg][t][hl][1]);
-#pragma unroll
-                for (int u = 0; u < 4; ++u) o[t][2 * w + j][u] += part[u];
+                for (int e = 0; e < 4; ++e) w[kg][e] -= __half2float(__float2half_rn(w[kg][e]));
               }
             }
+          }
         }
+#pragma unroll
+        for (int kg = 0; kg < KG; ++kg) {
+          // E4M3 has a NaN; a slot behind the last token may hold anything, and so may page 0, which is read in the place of a
+          // page that the pool does not have (its scale is NaN here)
+          if (CODE == NNLIB_B200_E4M3 && (key0 + kStep > kend || !(vs[kg] >= 0.f))) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              if (key0 + 16 * kg + 2 * c + (u & 1) + (u >> 1) * 8 >= kend || !(vs[kg] >= 0.f))
+#pragma unroll
+                for (int w = 0; w < VB / 4; ++w) vf[kg][u][w] = 0u;
+          }
+#pragma unroll
+          for (int w = 0; w < VB / 4; ++w) {
+            // the codes of keys 2c and 2c + 1 side by side, features 4w .. 4w + 3
+            const uint32_t a01 = __byte_perm(vf[kg][0][w], vf[kg][1][w], 0x5140), a23 = __byte_perm(vf[kg][0][w], vf[kg][1][w], 0x7362);
+            const uint32_t b01 = __byte_perm(vf[kg][2][w], vf[kg][3][w], 0x5140), b23 = __byte_perm(vf[kg][2][w], vf[kg][3][w], 0x7362);
+            uint32_t lo[4], hi[4];
+            word_pairs<CODE>(a01, lo[0], lo[1]);
+            word_pairs<CODE>(a23, lo[2], lo[3]);
+            word_pairs<CODE>(b01, hi[0], hi[1]);
+            word_pairs<CODE>(b23, hi[2], hi[3]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int t = 0; t < NT; ++t) {
+                if constexpr (HL == 1) {
+                  mma(o[t][2 * w + j], lo[2 * j], lo[2 * j + 1], hi[2 * j], hi[2 * j + 1], pb[kg][t][0][0], pb[kg][t][0][1]);
+                } else {
+                  // The products' own addition cuts off instead of rounding: over a long run the sum shrinks by a part of
+                  // 2^-24 a step (2e-5 of x behind 99163 keys).  Float32 sums are added up with rounded additions.
+                  float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                  for (int hl = 0; hl < HL; ++hl)
+                    mma(part, lo[2 * j], lo[2 * j + 1], hi[2 * j], hi[2 * j + 1], pb[kg][t][hl][0], pb[kg][t][hl][1]);
+#pragma unroll
+                  for (int u = 0; u < 4; ++u) o[t][2 * w + j][u] += part[u];
+                }
+              }
+          }
+        }
+        if (next < key_hi) load_v();
       }
-      if (next < key_hi) load_v();
+      if (HL != 1 || key0 >= key_hi) break;
+      const bool more = n > kFold;                   // (what the warp put there itself)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int row = 8 * t + 2 * c + u;
+          const float f = more ? since(sm_m[warp][row], m[t][u]) : 0.f;
+#pragma unroll
+          for (int j = 0; j < D / 16; j += 2) {
+            float4* to = reinterpret_cast<float4*>(&sm_o[warp][row][VB * g + 2 * j]);
+            const float4 s = more ? *to : make_float4(0.f, 0.f, 0.f, 0.f);
+            *to = make_float4(fmaf(s.x, f, o[t][j][u]), fmaf(s.y, f, o[t][j][2 + u]), fmaf(s.z, f, o[t][j + 1][u]), fmaf(s.w, f, o[t][j + 1][2 + u]));
+            o[t][j][u] = o[t][j][2 + u] = o[t][j + 1][u] = o[t][j + 1][2 + u] = 0.f;
+          }
+          __syncwarp();
+          if (g == 0) sm_m[warp][row] = m[t][u];
+          __syncwarp();
+        }
     }
+    const bool folded = HL == 1 && n > kFold;
 
     // merge the four warps
 #pragma unroll
@@ -562,6 +593,18 @@ cache_attn_kernel(const CacheAttnArgs a, const int teams, const int vec) {
         const int row = 8 * t + 2 * c + u;
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) l[t][u] += __shfl_xor_sync(0xffffffffu, l[t][u], off);
+        if (folded) {
+          const float f = since(sm_m[warp][row], m[t][u]);
+#pragma unroll
+          for (int j = 0; j < D / 16; j += 2) {
+            const float4 s = *reinterpret_cast<const float4*>(&sm_o[warp][row][VB * g + 2 * j]);
+            o[t][j][u] = fmaf(s.x, f, o[t][j][u]);
+            o[t][j][2 + u] = fmaf(s.y, f, o[t][j][2 + u]);
+            o[t][j + 1][u] = fmaf(s.z, f, o[t][j + 1][u]);
+            o[t][j + 1][2 + u] = fmaf(s.w, f, o[t][j + 1][2 + u]);
+          }
+          __syncwarp();
+        }
         if (g == 0) {
           sm_m[warp][row] = m[t][u];
           sm_l[warp][row] = l[t][u];

@@ -471,151 +471,151 @@ __global__ void __launch_bounds__(kThreadsC, 1) cache_attn_umma_kernel(const Cac
       // (a loop around the loop over the tiles: a step that is rarely taken inside it costs its code 4 % and more)
 #pragma unroll 1
       for (int j_from = 0; j_from < nt && ok; j_from += kFold) {
-      if (j_from > 0) {
-        // the products of the tiles so far are done when the scores of the next one are; that one's begin the sums anew
-        ok = mbar_wait(&bars->s_full[t], 0, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
-        if (!idle) {
-          const Part p = part();
-          const bool row_ok = p.row < rows, more = j_from > kFold;
-          float f = 0.f;
-          if (row_ok) {
-            if (more) f = since(p.ml[0], m_used);
-            p.ml[0] = m_used;
-          }
-#pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(tO + c * 32, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              if (!row_ok || c * 32 + e >= cc.d) continue;
-              float4* to = reinterpret_cast<float4*>(p.o + c * 32 + e);
-              float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-              if (more) s = *to;
-              s.x = fmaf(s.x, f, __uint_as_float(o[e]));
-              s.y = fmaf(s.y, f, __uint_as_float(o[e + 1]));
-              s.z = fmaf(s.z, f, __uint_as_float(o[e + 2]));
-              s.w = fmaf(s.w, f, __uint_as_float(o[e + 3]));
-              *to = s;
+        if (j_from > 0) {
+          // the products of the tiles so far are done when the scores of the next one are; that one's begin the sums anew
+          ok = mbar_wait(&bars->s_full[t], 0, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          if (!idle) {
+            const Part p = part();
+            const bool row_ok = p.row < rows, more = j_from > kFold;
+            float f = 0.f;
+            if (row_ok) {
+              if (more) f = since(p.ml[0], m_used);
+              p.ml[0] = m_used;
             }
-          }
-        }
-      }
-      const int j_to = min(nt, j_from + kFold);
-#pragma unroll 1
-      for (int j = j_from; j < j_to; ++j) {
-        uint8_t* sm = smem;
-        asm volatile("" : "+l"(sm));         // (no barrier's address in a register for good)
-        BarsC* bb = reinterpret_cast<BarsC*>(sm + C::kBarOff);
-        volatile int* abort_flag = &bb->abort_flag;
-        if ((j & 3) == 0) ok = mbar_wait_warp(&bb->meta_full[(j >> 2) & 1], (j >> 3) & 1, abort_flag);
-        if (!ok) break;
-        // scales: a group of SG keys has a factor and an offset
-        const PageMeta* pm = reinterpret_cast<const PageMeta*>(sm + C::kMetaOff) + (j & (kMetaTiles - 1)) * 8;
-        ok = mbar_wait(&bb->s_full[t], j & 1, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
-        if (idle) {
-          if (lane == 0) {
-            mbar_arrive(&bb->p_half[t][0]);
-            mbar_arrive(&bb->p_half[t][1]);
-          }
-          continue;
-        }
-        // Twice over the scores, 64 keys at a time: once for the maximum, once for the weights, which overwrite them.  (Held
-        // whole in registers, as the 16-bit forward does, a row leaves none for the converting warps, and the longer code
-        // keeps every warp waiting for instructions: 2.56 ms instead of 2.34 for 4096 queries over 8192 tokens of 4 sequences.)
-        const int j0 = (j_lo + j) * kBN;
-        const bool edge = __any_sync(0xffffffffu, j0 + kBN - 1 > lim);
-        constexpr int HG = 64 / SG;             // scales of 64 keys
-        uint32_t sr[2][32];
-        auto fetch = [&](int hf) {
-          tmem_ld32(tS + hf * 64, sr[0]);
-          tmem_ld32(tS + hf * 64 + 32, sr[1]);
-          tmem_wait_ld();
-          if (edge) {
-            // the scaled logits themselves, -Inf where the row does not look
-#pragma unroll
-            for (int g = 0; g < HG; ++g) {
-              const float f = crow * pm[hf * 4 + g * (SG / 16)].ks, o = pm[hf * 4 + g * (SG / 16)].lvs;
-#pragma unroll
-              for (int e = g * SG; e < (g + 1) * SG; ++e) {
-                const float v = fmaf(__uint_as_float(sr[e / 32][e & 31]), f, o);
-                sr[e / 32][e & 31] = j0 + hf * 64 + e > lim ? 0xff800000u : __float_as_uint(v);
-              }
-            }
-          }
-        };
-        auto factor = [&](int hf, int g) { return edge ? 1.f : crow * pm[hf * 4 + g * (SG / 16)].ks; };
-        auto offset = [&](int hf, int g) { return edge ? 0.f : pm[hf * 4 + g * (SG / 16)].lvs; };
-
-        float mx = neg_inf();
-#pragma unroll 1
-        for (int hf = 0; hf < 2; ++hf) {
-          fetch(hf);
-#pragma unroll
-          for (int g = 0; g < HG; ++g) {
-            float m0 = neg_inf(), m1 = neg_inf();
-#pragma unroll
-            for (int e = g * SG; e < (g + 1) * SG; e += 4) {
-              m0 = max3(m0, __uint_as_float(sr[e / 32][e & 31]), __uint_as_float(sr[e / 32][(e & 31) + 1]));
-              m1 = max3(m1, __uint_as_float(sr[e / 32][(e & 31) + 2]), __uint_as_float(sr[e / 32][(e & 31) + 3]));
-            }
-            mx = fmaxf(mx, fmaf(fmaxf(m0, m1), factor(hf, g), offset(hf, g)));
-          }
-        }
-        const float m_new = fmaxf(m_used, mx - kBits);
-        const bool raise = m_new > m_used + kGap;      // also true for m_used = -Inf < m_new
-        if (__any_sync(0xffffffffu, raise)) {
-          if (j > 0) {
-            const float f = raise ? ex2_approx(m_used - m_new) : 1.f;
-            l *= f;
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               uint32_t o[32];
               tmem_ld32(tO + c * 32, o);
               tmem_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tmem_st32(tO + c * 32, o);
+              for (int e = 0; e < 32; e += 4) {
+                if (!row_ok || c * 32 + e >= cc.d) continue;
+                float4* to = reinterpret_cast<float4*>(p.o + c * 32 + e);
+                float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (more) s = *to;
+                s.x = fmaf(s.x, f, __uint_as_float(o[e]));
+                s.y = fmaf(s.y, f, __uint_as_float(o[e + 1]));
+                s.z = fmaf(s.z, f, __uint_as_float(o[e + 2]));
+                s.w = fmaf(s.w, f, __uint_as_float(o[e + 3]));
+                *to = s;
+              }
             }
           }
-          if (raise) m_used = m_new;
         }
-        const float ref = m_used == neg_inf() ? 0.f : m_used;
+        const int j_to = min(nt, j_from + kFold);
 #pragma unroll 1
-        for (int hf = 0; hf < 2; ++hf) {
-          fetch(hf);
-          uint32_t pk[32];
-#pragma unroll
-          for (int g = 0; g < HG; ++g) {
-            const unsigned long long f2 = pair_of(factor(hf, g)), c2 = pair_of(offset(hf, g) - ref);
-            unsigned long long s2[2] = {0ull, 0ull};
-#pragma unroll
-            for (int e = g * SG; e < (g + 1) * SG; e += 2) {
-              float x0, x1;
-              fma2(x0, x1, __uint_as_float(sr[e / 32][e & 31]), __uint_as_float(sr[e / 32][(e & 31) + 1]), f2, c2);
-              x0 = ex2_approx(x0);
-              x1 = ex2_approx(x1);
-              add2(s2[(e >> 1) & 1], x0, x1);
-              pk[e >> 1] = pack2<false>(x0, x1);
+        for (int j = j_from; j < j_to; ++j) {
+          uint8_t* sm = smem;
+          asm volatile("" : "+l"(sm));         // (no barrier's address in a register for good)
+          BarsC* bb = reinterpret_cast<BarsC*>(sm + C::kBarOff);
+          volatile int* abort_flag = &bb->abort_flag;
+          if ((j & 3) == 0) ok = mbar_wait_warp(&bb->meta_full[(j >> 2) & 1], (j >> 3) & 1, abort_flag);
+          if (!ok) break;
+          // scales: a group of SG keys has a factor and an offset
+          const PageMeta* pm = reinterpret_cast<const PageMeta*>(sm + C::kMetaOff) + (j & (kMetaTiles - 1)) * 8;
+          ok = mbar_wait(&bb->s_full[t], j & 1, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          if (idle) {
+            if (lane == 0) {
+              mbar_arrive(&bb->p_half[t][0]);
+              mbar_arrive(&bb->p_half[t][1]);
             }
-            // a page that the row does not see adds nothing, whatever its scale is
-            const float sum = pair_sum(s2[0]) + pair_sum(s2[1]);
-            if (!(sum == 0.f)) l = fmaf(sum, pm[hf * 4 + g * (SG / 16)].ivs, l);
+            continue;
           }
-          tmem_st32(tS + hf * 32, pk);
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bb->p_half[t][hf]);
+          // Twice over the scores, 64 keys at a time: once for the maximum, once for the weights, which overwrite them.  (Held
+          // whole in registers, as the 16-bit forward does, a row leaves none for the converting warps, and the longer code
+          // keeps every warp waiting for instructions: 2.56 ms instead of 2.34 for 4096 queries over 8192 tokens of 4 sequences.)
+          const int j0 = (j_lo + j) * kBN;
+          const bool edge = __any_sync(0xffffffffu, j0 + kBN - 1 > lim);
+          constexpr int HG = 64 / SG;             // scales of 64 keys
+          uint32_t sr[2][32];
+          auto fetch = [&](int hf) {
+            tmem_ld32(tS + hf * 64, sr[0]);
+            tmem_ld32(tS + hf * 64 + 32, sr[1]);
+            tmem_wait_ld();
+            if (edge) {
+              // the scaled logits themselves, -Inf where the row does not look
+#pragma unroll
+              for (int g = 0; g < HG; ++g) {
+                const float f = crow * pm[hf * 4 + g * (SG / 16)].ks, o = pm[hf * 4 + g * (SG / 16)].lvs;
+#pragma unroll
+                for (int e = g * SG; e < (g + 1) * SG; ++e) {
+                  const float v = fmaf(__uint_as_float(sr[e / 32][e & 31]), f, o);
+                  sr[e / 32][e & 31] = j0 + hf * 64 + e > lim ? 0xff800000u : __float_as_uint(v);
+                }
+              }
+            }
+          };
+          auto factor = [&](int hf, int g) { return edge ? 1.f : crow * pm[hf * 4 + g * (SG / 16)].ks; };
+          auto offset = [&](int hf, int g) { return edge ? 0.f : pm[hf * 4 + g * (SG / 16)].lvs; };
+
+          float mx = neg_inf();
+#pragma unroll 1
+          for (int hf = 0; hf < 2; ++hf) {
+            fetch(hf);
+#pragma unroll
+            for (int g = 0; g < HG; ++g) {
+              float m0 = neg_inf(), m1 = neg_inf();
+#pragma unroll
+              for (int e = g * SG; e < (g + 1) * SG; e += 4) {
+                m0 = max3(m0, __uint_as_float(sr[e / 32][e & 31]), __uint_as_float(sr[e / 32][(e & 31) + 1]));
+                m1 = max3(m1, __uint_as_float(sr[e / 32][(e & 31) + 2]), __uint_as_float(sr[e / 32][(e & 31) + 3]));
+              }
+              mx = fmaxf(mx, fmaf(fmaxf(m0, m1), factor(hf, g), offset(hf, g)));
+            }
+          }
+          const float m_new = fmaxf(m_used, mx - kBits);
+          const bool raise = m_new > m_used + kGap;      // also true for m_used = -Inf < m_new
+          if (__any_sync(0xffffffffu, raise)) {
+            if (j > 0) {
+              const float f = raise ? ex2_approx(m_used - m_new) : 1.f;
+              l *= f;
+#pragma unroll 1
+              for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld32(tO + c * 32, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tmem_st32(tO + c * 32, o);
+              }
+            }
+            if (raise) m_used = m_new;
+          }
+          const float ref = m_used == neg_inf() ? 0.f : m_used;
+#pragma unroll 1
+          for (int hf = 0; hf < 2; ++hf) {
+            fetch(hf);
+            uint32_t pk[32];
+#pragma unroll
+            for (int g = 0; g < HG; ++g) {
+              const unsigned long long f2 = pair_of(factor(hf, g)), c2 = pair_of(offset(hf, g) - ref);
+              unsigned long long s2[2] = {0ull, 0ull};
+#pragma unroll
+              for (int e = g * SG; e < (g + 1) * SG; e += 2) {
+                float x0, x1;
+                fma2(x0, x1, __uint_as_float(sr[e / 32][e & 31]), __uint_as_float(sr[e / 32][(e & 31) + 1]), f2, c2);
+                x0 = ex2_approx(x0);
+                x1 = ex2_approx(x1);
+                add2(s2[(e >> 1) & 1], x0, x1);
+                pk[e >> 1] = pack2<false>(x0, x1);
+              }
+              // a page that the row does not see adds nothing, whatever its scale is
+              const float sum = pair_sum(s2[0]) + pair_sum(s2[1]);
+              if (!(sum == 0.f)) l = fmaf(sum, pm[hf * 4 + g * (SG / 16)].ivs, l);
+            }
+            tmem_st32(tS + hf * 32, pk);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bb->p_half[t][hf]);
+          }
         }
-      }
       }
 
       // -------------------------------------------------- epilogue

@@ -795,3 +795,39 @@ def test_short_histories_in_a_table_for_long_ones(dtype):
         for g, w in zip(got, want):
             assert torch.equal(torch.nan_to_num(g, nan=7.0), torch.nan_to_num(w, nan=7.0))
     c.attend(q, [640, 100], H)
+
+
+@gpu
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("loud", [1, 64])
+def test_sums_of_a_very_long_history_that_one_team_of_blocks_walks_over(dtype, code, loud):
+    """Single queries of as many sequences as there are teams, so that a warp has a quarter of a history of 1048576 tokens;
+    positive values.  Each addition of the products cuts off less than 2^-23 of the sum behind 16 keys, 2^-27 a key, and a warp
+    adds 32768 keys that way: 2^-12; 2^-16 for all else (logits below 1, Float32 sums, weights' roundings that cancel over so
+    many).  Rounding keeps order, so a result lies between the rounded ends of that range.  (Nothing is said of the mean of what
+    is left: means of 1048576 values of a spread near 2 differ by 2 / 1024, less than a step, so their roundings are not
+    independent, and 128 of them may be off by up to half a step together.)  ``loud``: the last third's logits are that much
+    larger, so that maxima rise behind sums that have been put aside (sum |q||k| scale <= 8: 2 * 8 * 2^-18 = 2^-14 for weights)."""
+    d, H, n, B = 16, 64, 1 << 20, 9
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    c = nb.QuantizedCache(d * H, n, 1, nheads=H, page=64, eltype=CODE[code], device=DEV)
+    lo, hi = ((-127, 128), (40, 128)) if code == "int8" else ((0x20, 0x58), (0x38, 0x50))     # (E4M3: 0.125 .. 15 and 1 .. 7.5)
+    for t, (a, b) in ((c.k, lo), (c.v, hi)):
+        (t if code == "int8" else t.view(torch.uint8)).random_(a, b, generator=gen)
+    c.k_scale.fill_(2.0 ** -7 if code == "int8" else 2.0 ** -4)
+    c.v_scale.fill_(2.0 ** -7 if code == "int8" else 2.0 ** -3)
+    c.k_scale[:, n // 96:] *= loud
+    t = nb.jl_empty((n // 64, B), torch.int32, DEV)
+    t.copy_(torch.arange(n // 64, dtype=torch.int32, device=DEV)[:, None].expand(-1, B))
+    q = (nb.jl_empty((d * H, 1, B), F32, DEV).normal_(generator=gen) * 2.0 ** -5).to(dtype)
+    x = nb.cached_attention(q, c, n, nheads=H, table=t)
+    off = 2.0 ** -12 + 2.0 ** -16 + (2.0 ** -14 if loud > 1 else 0)
+    for h in range(0, H, 8):
+        s = slice(h * d, (h + 1) * d)
+        kr, vr = ((z[s].float() if code == "int8" else z[s].view(torch.uint8).contiguous().view(z.dtype).float()).double().permute(2, 1, 0).reshape(n, d)
+                  * f[0].double().repeat_interleave(64)[:, None] for z, f in ((c.k, c.k_scale), (c.v, c.v_scale)))
+        want = torch.softmax(q[s, 0].double().T @ kr.T / d ** 0.5, 1) @ vr                    # (B, d)
+        got = x[s, 0].double().T
+        low, high = ((want * (1 + e)).to(dtype).double() for e in (-off, off))
+        assert (low <= got).all() and (got <= high).all(), ((got - low).min().item(), (high - got).min().item())
