@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(kNrThreads, V == 1 ? 3 : (BWD && V == 8 ? 4 : 
   const NormRopeSide& s = a.side[second ? 1 : 0];
   const int bid = second ? blockIdx.x - a.blocks_q : blockIdx.x, nblk = second ? gridDim.x - a.blocks_q : a.blocks_q;
   const float inv_d = 1.f / (float)a.d;
+  const bool whole = a.rot == a.d;                       // every feature is turned
 
   Two gw[NS][V], acc[NS][V];
   int f0[NS], f1[NS];
@@ -247,6 +248,21 @@ __global__ void __launch_bounds__(kNrThreads, V == 1 ? 3 : (BWD && V == 8 ? 4 : 
       }
     }
     auto partner = [&](const Two (&v)[V], int e) { return ADJ ? swapped(v[e]) : v[e < H2 ? e + H2 : e - H2]; };
+    // The rotation of slot n.  Features that are not turned meet no other: the sine of 0 would make NaN of an infinity there.
+    // (plain: every feature is turned, or v holds none)
+    auto turned = [&](const Two (&v)[V], int n, bool plain, Two (&t)[V]) {
+      if (plain) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) t[e] = pair_fma(v[e], f1c[n][e], pair_mul(partner(v, e), f2s[n][e]));
+      } else {
+        const int left = a.rot / 2 - (lane + n * lanes) * V;      // pairs of this slot that are turned
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const Two other = (ADJ ? e < left : left > 0) ? partner(v, e) : 0ull;
+          t[e] = pair_fma(v[e], f1c[n][e], pair_mul(other, f2s[n][e]));
+        }
+      }
+    };
     const int h_end = h_hi;
     T* const out = orow;
     for (int h = h_lo; h < h_end; h += per_warp) {       // (the same for all of a warp's lanes: they shuffle)
@@ -293,8 +309,7 @@ __global__ void __launch_bounds__(kNrThreads, V == 1 ? 3 : (BWD && V == 8 ? 4 : 
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
           Two t[V];
-#pragma unroll
-          for (int e = 0; e < V; ++e) t[e] = pair_fma(u[n][e], f1c[n][e], pair_mul(partner(u[n], e), f2s[n][e]));
+          turned(u[n], n, whole, t);
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             u[n][e] = t[e];
@@ -313,6 +328,7 @@ __global__ void __launch_bounds__(kNrThreads, V == 1 ? 3 : (BWD && V == 8 ? 4 : 
 #pragma unroll
       for (int n = 0; n < NS; ++n) {
         Two y[V];
+        if (!BWD) turned(x[n], n, sum <= 3.402823466e38f, y);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           if (BWD) {
@@ -320,7 +336,7 @@ __global__ void __launch_bounds__(kNrThreads, V == 1 ? 3 : (BWD && V == 8 ? 4 : 
             acc[n][e] = pair_fma(u[n][e], xs, acc[n][e]);
             y[e] = pair_fma(xs, back2, pair_mul(w[n][e], r2));
           } else {
-            y[e] = pair_mul(r2, pair_fma(x[n][e], f1c[n][e], pair_mul(partner(x[n], e), f2s[n][e])));
+            y[e] = pair_mul(r2, y[e]);
           }
         }
         if (live && on[n]) {

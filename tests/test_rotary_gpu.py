@@ -262,3 +262,30 @@ def test_without_eps(dtype, case):
     q, k, dyq, dyk = (_array(gen, (h * d, L, B), dtype) for h in (H, Hk, H, Hk))
     gq, gk = (1 + 0.2 * _array(gen, (d,), F32)).to(dtype), (1 + 0.2 * _array(gen, (d,), F32)).to(dtype)
     _check(q, k, gq, gk, nb.rope_frequencies(rot), H, dyq, dyk, inter, eps=0.0, start=3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("d,rot,inter", [(64, 32, False), (64, 32, True), (64, 20, True), (34, 10, False), (254, 20, True), (48, 0, False)])
+def test_features_that_are_not_turned_meet_no_others(dtype, d, rot, inter):
+    """An infinity in a feature behind the rotated ones: r is 0 and so is every other feature of y; in the cotangent it
+    reaches dx of its row, through the mean, and the gradient of its own weight only."""
+    H, L, B = 3, 5, 2
+    gen = np.random.default_rng(38)
+    g, f = (1 + 0.2 * _array(gen, (d,), F32)).to(dtype), nb.rope_frequencies(rot)
+    for at in {rot, (rot + d) // 2, d - 1}:
+        q, dy = _array(gen, (H * d, L, B), dtype), _array(gen, (H * d, L, B), dtype)
+        want = nb.qk_norm_rope(q, q, g, g, f, nheads=H, interleaved=inter, start=4)[0]
+        bad = q.clone()
+        bad[d + at, 2, 1] = float("inf")
+        y, _, back = nb.qk_norm_rope_pullback(bad, bad, g, g, f, nheads=H, interleaved=inter, start=4)
+        row = y[d:2 * d, 2, 1]
+        assert torch.isnan(row[at]) and not torch.cat((row[:at], row[at + 1:])).float().abs().any()
+        same = torch.ones_like(y, dtype=torch.bool)
+        same[d:2 * d, 2, 1] = False
+        assert torch.equal(y[same], want[same])
+        loud = dy.clone()
+        loud[d + at, 2, 1] = float("inf")
+        dgq = nb.qk_norm_rope_pullback(q, q, g, g, f, nheads=H, interleaved=inter, start=4)[2](loud, dy)[2]
+        hit = ~torch.isfinite(dgq.float())
+        assert hit[at] and hit.sum().item() == 1
