@@ -244,9 +244,9 @@ def cached_attention(q: torch.Tensor, cache: QuantizedCache, lens: Union[int, to
     if start is not None:
         p.start = _int32("start", start, B, dev)
     if scale is not None:
-        if not scale > 0:
-            raise ArgumentError(f"scale = {scale}")
         p.scale = scale
+        if not p.scale > 0:            # (as Float32, where 0 would stand for the default)
+            raise ArgumentError(f"scale = {scale}")
     x = _dense(q, E, L, B)
     p.q, p.x = q.data_ptr(), x.data_ptr()
     p.q_stride_l, p.q_stride_b = qst

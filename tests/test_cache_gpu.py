@@ -831,3 +831,18 @@ def test_sums_of_a_very_long_history_that_one_team_of_blocks_walks_over(dtype, c
         got = x[s, 0].double().T
         low, high = ((want * (1 + e)).to(dtype).double() for e in (-off, off))
         assert (low <= got).all() and (got <= high).all(), ((got - low).min().item(), (high - got).min().item())
+
+
+@gpu
+def test_a_scale_that_is_none_in_float32():
+    """1e-46 is 0 in Float32, which the C ABI takes for 1 / sqrt(d); the smallest number that is not is taken as it is."""
+    gen = np.random.default_rng(39)
+    d, H = 64, 2
+    c = _filled(gen, d * H, 50, 1, H, 16, "int8", False)
+    q = _array(gen, (d * H, 1, 1), F32)
+    for scale in (1e-46, 1e-300, 0.0, -1e-46, 1e39):
+        with pytest.raises(nb.ArgumentError):
+            nb.cached_attention(q, c.dev, 50, nheads=H, scale=scale)
+    x = nb.cached_attention(q, c.dev, 50, nheads=H, scale=1e-44)
+    v = nb.cache_read(c.dev, 50, dtype=F32)[1].double()
+    assert (x[:, 0].double() - v.mean(1)).abs().max().item() <= 2.0 ** -20 * v.abs().max().item()
