@@ -13,6 +13,7 @@ so that a captured call follows what they hold when it is replayed.  NNlib.jl ha
 from __future__ import annotations
 
 import ctypes as C
+import operator
 from typing import Optional, Union
 
 import torch
@@ -30,6 +31,16 @@ _blank_tokens = bytes(_lib.CacheTokens())
 _blank_attn = bytes(_lib.CacheAttnParams())
 
 
+def _fixed(slot: str) -> property:
+    """An attribute of a cache: calls go by the addresses that the first arrays had, so it cannot be replaced."""
+    get = operator.attrgetter(slot)
+
+    def put(self, value):
+        if value is not get(self):                     # (`cache.k_scale *= 2` assigns the same array)
+            raise AttributeError(f"{slot[1:]} of a cache cannot be replaced; from_arrays makes another cache")
+    return property(get, put)
+
+
 class QuantizedCache:
     """Keys and values of ``nheads`` heads of ``dim / nheads`` features in 8 bits: ``capacity`` tokens (rounded up to whole
     pages) for each of ``batch`` sequences, or, for programs that hand pages out themselves, ``batch=1`` and as many tokens
@@ -41,9 +52,12 @@ class QuantizedCache:
     to 256.  The head size is a multiple of 16, at most 256.
 
     Arrays, all column-major: ``k`` and ``v`` codes ``(dim, page, pages)``, ``k_scale`` and ``v_scale`` Float32
-    ``(nheads, pages)``; an element stands for ``code * scale``.  :meth:`from_arrays` takes them from elsewhere."""
+    ``(nheads, pages)``; an element stands for ``code * scale``.  They can be written to, not replaced.  :meth:`from_arrays`
+    takes them from elsewhere."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "batch", "_template")
+    __slots__ = ("_k", "_v", "_k_scale", "_v_scale", "_batch", "_template")
+
+    k, v, k_scale, v_scale, batch = (_fixed(name) for name in ("_k", "_v", "_k_scale", "_v_scale", "_batch"))
 
     def __init__(self, dim: int, capacity: int, batch: int = 1, *, nheads: int, page: int = 64, eltype=torch.int8,
                  device="cuda"):
@@ -92,7 +106,7 @@ class QuantizedCache:
             raise ArgumentError(f"a page holds a power of two from 16 to 256 tokens, got {T}")
         if batch is not None and batch < 0:
             raise ArgumentError(f"batch = {batch}")
-        self.k, self.v, self.k_scale, self.v_scale, self.batch = k, v, k_scale, v_scale, batch
+        self._k, self._v, self._k_scale, self._v_scale, self._batch = k, v, k_scale, v_scale, batch
         p = _lib.Cache.from_buffer_copy(_blank_cache)
         p.code = _CODES[k.dtype]
         p.d, p.H, p.page, p.pages = E // H, H, T, P
@@ -102,22 +116,22 @@ class QuantizedCache:
 
     @property
     def device(self):
-        return self.k.device
+        return self._k.device
 
     @property
     def nheads(self) -> int:
-        return self.k_scale.shape[0]
+        return self._k_scale.shape[0]
 
     @property
     def page(self) -> int:
-        return self.k.shape[1]
+        return self._k.shape[1]
 
     @property
     def pages(self) -> int:
-        return self.k.shape[2]
+        return self._k.shape[2]
 
     def __repr__(self):
-        return f"QuantizedCache(dim={self.k.shape[0]}, nheads={self.nheads}, {self.pages} pages of {self.page} tokens, {self.k.dtype})"
+        return f"QuantizedCache(dim={self._k.shape[0]}, nheads={self.nheads}, {self.pages} pages of {self.page} tokens, {self._k.dtype})"
 
     def _call(self, B: int, table: Optional[torch.Tensor]):
         """The struct of a call for B sequences."""
@@ -125,11 +139,11 @@ class QuantizedCache:
         p.B = B
         if table is None:
             # (a call for no sequence touches nothing)
-            if B != self.batch and self.batch is not None and B:
-                raise ArgumentError(f"a call for {B} sequences, without a table, on a cache of {self.batch}")
-            p.rows = self.k.shape[2] // B if B else 0
+            if B != self._batch and self._batch is not None and B:
+                raise ArgumentError(f"a call for {B} sequences, without a table, on a cache of {self._batch}")
+            p.rows = self._k.shape[2] // B if B else 0
             return p
-        if not isinstance(table, torch.Tensor) or table.dtype != torch.int32 or table.device != self.k.device:
+        if not isinstance(table, torch.Tensor) or table.dtype != torch.int32 or table.device != self._k.device:
             raise TypeError("table must be an Int32 CUDA tensor on the cache's device")
         rows = table.shape[0]
         if table.ndim != 2 or table.shape[1] != B or (rows > 1 and table.stride(0) != 1) or (B > 1 and table.stride(1) < max(rows, 1)):
@@ -159,11 +173,11 @@ def cache_write_(cache: QuantizedCache, k: torch.Tensor, v: torch.Tensor, *, sta
     written must be one sequence's alone."""
     kst = _require_rows("key", k)
     vst = _require_rows("value", v, k)
-    if k.device != cache.device:
-        raise TypeError(f"key lives on {k.device}, the cache on {cache.device}")
+    if k.device != cache._k.device:
+        raise TypeError(f"key lives on {k.device}, the cache on {cache._k.device}")
     E, L, B = k.shape
-    if E != cache.k.shape[0] or v.shape != k.shape:
-        raise ArgumentError(f"key and value must both be ({cache.k.shape[0]}, len, batch) arrays. Instead:\n"
+    if E != cache._k.shape[0] or v.shape != k.shape:
+        raise ArgumentError(f"key and value must both be ({cache._k.shape[0]}, len, batch) arrays. Instead:\n"
                             f"- size(k): {tuple(k.shape)}\n- size(v): {tuple(v.shape)}")
     c = cache._call(B, table)
     p = _lib.CacheTokens.from_buffer_copy(_blank_tokens)
@@ -190,7 +204,7 @@ def cache_read(cache: QuantizedCache, length: int, *, start: Union[int, torch.Te
         raise ArgumentError(f"length = {length}")
     if dtype not in _DTYPES:
         raise TypeError(f"eltype {dtype}; supported: Float16, BFloat16, Float32")
-    B = 1 if cache.batch is None else cache.batch
+    B = 1 if cache._batch is None else cache._batch
     if table is not None:
         if not isinstance(table, torch.Tensor) or table.ndim != 2:
             raise TypeError("table must be a 2-d Int32 CUDA tensor")
@@ -199,14 +213,14 @@ def cache_read(cache: QuantizedCache, length: int, *, start: Union[int, torch.Te
         B = start.numel()
     elif isinstance(lens, torch.Tensor):
         B = lens.numel()
-    dev, E = cache.device, cache.k.shape[0]
+    dev, E = cache._k.device, cache._k.shape[0]
     c = cache._call(B, table)
     p = _lib.CacheTokens.from_buffer_copy(_blank_tokens)
     _starts(p, start, B, dev)
     if lens is not None:
         p.lens = _int32("lens", lens, B, dev)
     size, strides = (E, length, B), (1, E, E * (length or 1))
-    k, v = (cache.k_scale.new_empty_strided(size, strides, dtype=dtype) for _ in range(2))
+    k, v = (cache._k_scale.new_empty_strided(size, strides, dtype=dtype) for _ in range(2))
     p.dtype, p.L, p.k, p.v = _DTYPES[dtype], length, k.data_ptr(), v.data_ptr()
     with _on_device(dev):
         _check(_lib.load().nnlib_b200_cache_read(C.byref(c), C.byref(p), _stream()), "cache_read")
@@ -227,8 +241,8 @@ def cached_attention(q: torch.Tensor, cache: QuantizedCache, lens: Union[int, to
     was given a NaN."""
     qst = _require_rows("query", q)
     dev = q.device
-    if dev != cache.device:
-        raise TypeError(f"query lives on {dev}, the cache on {cache.device}")
+    if dev != cache._k.device:
+        raise TypeError(f"query lives on {dev}, the cache on {cache._k.device}")
     E, L, B = q.shape
     nheads, t = int(nheads), cache._template
     if nheads < 1 or nheads % t.H != 0 or E != nheads * t.d:

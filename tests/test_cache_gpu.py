@@ -846,3 +846,18 @@ def test_a_scale_that_is_none_in_float32():
     x = nb.cached_attention(q, c.dev, 50, nheads=H, scale=1e-44)
     v = nb.cache_read(c.dev, 50, dtype=F32)[1].double()
     assert (x[:, 0].double() - v.mean(1)).abs().max().item() <= 2.0 ** -20 * v.abs().max().item()
+
+
+@gpu
+def test_a_caches_arrays_are_written_to_not_replaced():
+    c = nb.QuantizedCache(32, 32, 2, nheads=2, page=16, device=DEV)
+    for name in ("k", "v", "k_scale", "v_scale"):
+        with pytest.raises(AttributeError):
+            setattr(c, name, getattr(c, name).clone())
+    with pytest.raises(AttributeError):
+        c.batch = 1
+    k = _array(np.random.default_rng(40), (32, 5, 2), F32)
+    nb.cache_write_(c, k, k)
+    before = nb.cache_read(c, 5, dtype=F32)[0]
+    c.k_scale *= 2
+    assert torch.equal(nb.cache_read(c, 5, dtype=F32)[0], 2 * before)
