@@ -348,8 +348,9 @@ NNLIB_B200_API int nnlib_b200_batched_gemm_path(const nnlib_b200_gemm_params* p)
      r = 1 / sqrt(mean(x^2) + eps),   n = x * r * g,   y = n with its feature pairs turned,
    for the d features x of each head of q (weights gq) and of k (weights gk).  Pair p < rot / 2 is turned by the angle
    position * freqs[p]: (a, b) -> (a cos - b sin, a sin + b cos); a and b are features p and p + rot / 2 of the head,
-   or 2p and 2p + 1 with interleaved = 1.  Features rot .. d - 1 are normalised only.  Angles are Float64 until they are
-   reduced to one turn, everything else Float32; results are rounded once.  The reference has no counterpart. */
+   or 2p and 2p + 1 with interleaved = 1.  Features rot .. d - 1 are normalised only.  Angles are reduced to one turn in 64
+   bits, everything else is Float32, for 16-bit arrays with sines and cosines to 2^-21 (also in the gradients of Float32
+   weights); results are rounded once.  The reference has no counterpart. */
 typedef struct nnlib_b200_norm_rope_params {
   size_t struct_size;        /* = sizeof(nnlib_b200_norm_rope_params) */
   int32_t dtype;             /* element type of q, k and of the results */
@@ -451,8 +452,9 @@ NNLIB_B200_API int nnlib_b200_cache_read(const nnlib_b200_cache* c, const nnlib_
    counts as 2^-100.  A query that sees no token gives NaN (or zeros), one that sees a token of a page with a NaN scale
    gives NaN, and one that does not is not touched by it; codes of tokens in use must be numbers (cache_write makes no
    others).  Many queries run on the tensor cores (tcgen05), few, Float32 arrays and heads of more than 128 features on
-   streamed warp-level products.  The same call gives the same bits each time; the cuts of the keys that sums are taken in
-   depend on the lengths of all sequences of the call, so a sequence's last bits may differ in another batch. */
+   streamed warp-level products; where lens is on the device, the choice goes by the capacity, rows * page.  The same call gives
+   the same bits each time; the cuts of the keys that sums are taken in depend on the lengths of all sequences of the call (and on
+   the capacity), so a sequence's last bits may differ in another batch. */
 typedef struct nnlib_b200_cache_attn_params {
   size_t struct_size;        /* = sizeof(nnlib_b200_cache_attn_params) */
   int32_t dtype;             /* element type of q and x */
@@ -472,7 +474,9 @@ typedef struct nnlib_b200_cache_attn_params {
 } nnlib_b200_cache_attn_params;
 
 /* workspace: device memory, 16-byte aligned, at least nnlib_b200_cache_attn_workspace_bytes(c, p) bytes (which may be 0);
-   it need not be cleared and is free again when the call's kernels have run. */
+   it need not be cleared and is free again when the call's kernels have run.  Its size depends on the sizes of the call and on
+   the capacity (or len0), not on what lens holds; on the tensor cores it is at most d + 2 floats for each query and head, or
+   for 148 * 256 of them where that is more. */
 NNLIB_B200_API size_t nnlib_b200_cache_attn_workspace_bytes(const nnlib_b200_cache* c, const nnlib_b200_cache_attn_params* p);
 NNLIB_B200_API int nnlib_b200_cache_attn(const nnlib_b200_cache* c, const nnlib_b200_cache_attn_params* p, void* workspace,
                                          size_t workspace_bytes, void* stream);

@@ -231,14 +231,18 @@ def cached_attention(q: torch.Tensor, cache: QuantizedCache, lens: Union[int, to
                      table: Optional[torch.Tensor] = None, start: Optional[torch.Tensor] = None, causal: bool = True,
                      scale: Optional[float] = None, return_lse: bool = False):
     """Attention of ``q``, ``(nheads * d, len, batch)`` with adjacent features, over the first ``lens[b]`` tokens of each
-    sequence in ``cache`` (an integer, or Int32, one per sequence): ``x`` of the size of ``q``, and with ``return_lse`` the
-    Float32 ``(len, nheads, batch)`` log-sum-exp of each query's logits.
+    sequence in ``cache`` (an integer, or Int32, one per sequence; at most the capacity counts): ``x`` of the size of ``q``, and
+    with ``return_lse`` the Float32 ``(len, nheads, batch)`` log-sum-exp of each query's logits.
 
     Causal: query ``i`` of sequence ``b`` is at position ``start[b] + i`` (Int32; by default ``lens[b] - len + i``, the
     queries of the last tokens) and sees the tokens up to its own.  ``nheads`` is a multiple of the cache's heads; a group of
     ``nheads / cache.nheads`` query heads shares one.  ``scale`` multiplies the logits, ``1/sqrt(d)`` by default.  A query
     that sees nothing gives NaN, like one with a token among those it sees whose page the pool does not have, or whose block
-    was given a NaN."""
+    was given a NaN.
+
+    What the call knows of lengths in a tensor is the capacity, the table's rows or the cache's: kernels are chosen and the
+    workspace is sized by it.  A program that holds little in a table for much gets the kernels for much; an integer ``lens``, or a
+    table of the rows in use, tells."""
     qst = _require_rows("query", q)
     dev = q.device
     if dev != cache._k.device:

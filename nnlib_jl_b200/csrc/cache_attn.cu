@@ -8,8 +8,9 @@
 // accumulator has a page's scale in it, and a weight's size is the size of what it adds to x.  q_i is brought to a
 // largest element in [2^13, 2^14) by a power of two of its own; w is rounded to 16 bits after a factor of 2^14, so that
 // weights keep 11 bits down to 2^-28 of the largest.  Float32 arrays: q and w as the sum of two 16-bit terms
-// each, sums over the keys by rounded additions (drawn cases 7.4e-7 off at most instead of 2.3e-5; 16 x 8192 tokens, Int8 86.0 us
-// and 87.0, E4M3 84.9 and 89.0; 256 queries of 4 sequences of 8192, heads of 64, 568 and 604).
+// each, sums over the keys by rounded additions (over 246 random shapes 7.4e-7 off at most instead of 2.3e-5; one query each, 32 / 8
+// heads of 128, 16 sequences of 8192 tokens, Int8 84.6 us, E4M3 86.3, 1 % and 5 % more than without; 256 queries of 4 sequences
+// of 8192, 16 / 4 heads of 64, 555 us).
 //
 // HBM is the bound (2 d bytes per key and head for up to 16 rows), so what counts is bytes in flight: nothing is staged,
 // a warp streams 16 keys at a time straight into the fragments of m16n8k16 products.  Keys and the features of values are
@@ -30,9 +31,9 @@
 // equal runs.  A tile that one team has whole it also finishes; of others each team leaves running maxima, sums and outputs,
 // two pieces at most (its first tile's and its last one's), and cache_merge_kernel merges what a tile's first team says
 // there is.  (Runs cut so that none reaches into a second tile, where tiles are few: 8 x 1024 tokens 16 us instead of 20, but 8 x
-// 8192 43 instead of 42 and 4 x 131072 218 instead of 212, for the registers that it takes.)  One query each, 32 / 8 heads of 128, Int8: 4 sequences of 131072 tokens 212 us, 5.1 TB/s; 8 of 8192 41 us, of which
-// some 14 are the way to the first keys, the end and the merging, and 2.8 each step at 5 TB/s; 64 of 2048 73 us (each
-// sequence's keys cut into parts by themselves: 86).
+// 8192 43 instead of 42 and 4 x 131072 218 instead of 212, for the registers that it takes.)  One query each, 32 / 8 heads of 128,
+// Int8: 4 sequences of 131072 tokens 206 us, 5.2 TB/s; 8 of 8192 42 to 43 us, of which some 14 are the way to the first keys, the
+// end and the merging, and 2.8 each step at 5 TB/s; 64 of 2048 71 to 73 us (each sequence's keys cut into parts by themselves: 86).
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -720,7 +721,10 @@ int team_count(const CacheAttnArgs& a) {
 }
 
 // At most 512 tokens to a sequence, and blocks enough for a whole tile each: nothing is merged, one launch and no workspace.
-// (500 tokens of 12 heads of 64: 15.8 us a call, dealt out and merged 19.4.)
+// Measured (us on the device, one launch / dealt out and merged; an eager call, which its caller bounds, 11 and 15): 16-bit, 12
+// heads of 64, 1 sequence, 256 tokens 5.5 / 8.4, 512 7.4 / 8.6, 640 8.6 / 8.7, 1024 11.5 / 8.8; 32 / 8 heads of 128, 1 sequence,
+// 256 8.5 / 10.6, 512 11.5 / 10.8, 1024 17.5 / 11.2, 8 sequences, 512 11.7 / 12.7, 640 13.1 / 13.4, 1024 17.6 / 20.1; heads
+// of 256, 256 12.2 / 12.5, 512 17.1 / 13.0; Float32, heads of 64, 256 6.7 / 7.7, 512 10.0 / 8.3.
 bool one_launch(const CacheAttnArgs& a, int dtype) {
   long long cap = a.c.rows << a.c.log_page;
   if (!a.lens) cap = std::min(cap, std::max(a.len0, 0LL));
@@ -748,8 +752,9 @@ AttnArgs reduce_args(const CacheAttnArgs& a) {
 
 // Many columns go to the tensor cores, whose blocks take 256 of them at once but some 12 us to begin: more than 16 columns, and
 // more than five groups of keys to a team here.  Measured (us; here / there), 32 / 8 heads of 128: 4 x 16384 tokens, 16 columns
-// 69 / 88, 32 103 / 90, 64 184 / 97; 32 x 2048 tokens, 32 columns 133 / 100; 8 / 8 heads, 8 x 4096 tokens, 16 columns 47 / 55,
-// 24 65 / 56; 16 / 2 heads, 1 x 8192 tokens (3.5 groups) 96 columns 32 / 34, 192 (6.9) 45 / 33.
+// 67 / 89, 32 99 / 90, 64 177 / 93; 32 x 2048 tokens, 16 columns 74 / 100, 32 129 / 101; 8 / 8 heads, 8 x 4096 tokens, 16
+// columns 46 / 53, 24 62 / 55; 16 / 2 heads, 1 x 8192 tokens (3.5 groups) 96 columns 30 / 28, 192 (6.9) 44 / 33; 12 heads of 64,
+// 2 x 1000 tokens (1.3 groups), 24 columns 17 / 19.  Where lengths are on the device the capacity stands for them.
 bool use_umma(const CacheAttnArgs& a, int dtype) {
   const long long rows = (long long)a.L * (a.Hq / a.c.H);
   if (!cache_umma_supports(a, dtype) || rows <= 16) return false;

@@ -13,12 +13,15 @@
 //   warps 12-15  codes to Float16: K by two warps, V by two, from global memory through registers into the 128-byte
 //                swizzled tiles the products read; both operands have a key's features in a row, so the code is the same
 //
-// Bound by the chain of a tile, its scores through the softmax (some 3300 cycles for 128 keys) and back into the products
-// (1000): 4300 cycles a round for 2048 of tensor work.  A conversion is five instructions for four codes (Int8), 32768 codes a
-// round, which is why it has warps of its own: the loads of a warp's next keys are under way while it converts some.  The
-// copy engine could bring codes only, which would cost another pass through shared memory.  4096 queries over 8192 tokens of 4
-// sequences, 32 / 8 heads of 128, bf16 over Int8: 2.30 ms, 719 TFLOP/s.  With sixteen softmax warps, two threads to a row, 2.26,
-// but 512 queries over up to 16384 tokens in E4M3 0.75 instead of 0.64; with eight converting warps 2.50 and 0.75.
+// Bound by the chain of a tile, its scores through the softmax and back into the products: 2.46 us a round of 128 keys (1024
+// queries over 131072 tokens, 128 blocks of 1020 rounds) for 2048 cycles, 1.07 us, of tensor work.  A conversion is five
+// instructions for four codes (Int8), 32768 codes a round, which is why it has warps of its own: the loads of a warp's next
+// keys are under way while it converts some.  The copy engine could bring codes only, which would cost another pass through
+// shared memory.  The length of the code counts: with the conversion of keys and of values written out each for itself every
+// warp waited for instructions (2.30 ms, and 2.07 to 2.37 for changes that did no more work).  4096 queries over 8192 tokens of
+// 4 sequences, 32 / 8 heads of 128, bf16 over Int8: 2.01 ms, 822 TFLOP/s; call after call for seconds 2.14 ms, at the power
+// limit (994 W, 1.83 to 1.92 GHz).  (At 2.30 ms: sixteen softmax warps, two threads to a row, 2.26, but 512 queries over up to
+// 16384 tokens in E4M3 0.75 instead of 0.64; eight converting warps 2.50 and 0.75.)
 // A scale serves 16 keys at least (64 where the pages allow: SG), so a thread scales and sums by groups of SG keys.
 // The products' additions cut off instead of rounding, always towards zero: behind n keys that one accumulator has summed x is
 // short by some n 2^-27.2 where all values have one sign (1024 queries, values 0.5 and above: 2.1e-4 behind 32768 keys, 8.7e-4
@@ -529,7 +532,7 @@ __global__ void __launch_bounds__(kThreadsC, 1) cache_attn_umma_kernel(const Cac
           }
           // Twice over the scores, 64 keys at a time: once for the maximum, once for the weights, which overwrite them.  (Held
           // whole in registers, as the 16-bit forward does, a row leaves none for the converting warps, and the longer code
-          // keeps every warp waiting for instructions: 2.56 ms instead of 2.34 for 4096 queries over 8192 tokens of 4 sequences.)
+          // keeps every warp waiting for instructions: 2.56 ms when this form took 2.34, 4096 queries over 8192 tokens of 4 sequences.)
           const int j0 = (j_lo + j) * kBN;
           const bool edge = __any_sync(0xffffffffu, j0 + kBN - 1 > lim);
           constexpr int HG = 64 / SG;             // scales of 64 keys

@@ -9,9 +9,11 @@
 // holds as many groups as fit (six of five lanes for a head of 80 features) and works by itself: it takes a token, or some of
 // a token's heads where tokens are few, works out its angles, and walks over the heads, the next rows, then the next token's,
 // always under way.  Queries and keys are two ranges of blocks of one launch.
-// bf16, 32768 tokens, heads of 128: 32 + 8 heads 135 us (5.0 TB/s), pullback 271 (3.7); 32 + 32 heads 197 (5.4) and 386 (4.2);
-// Float32, 16384 tokens, 32 + 8 heads 124 (5.4) and 179 (5.6): what bounds the 16-bit pullback is the number of rows under
-// way, 64 to an SM at 128 registers a thread, and the issue slots that a row takes however many bytes it has.
+// bf16, 32768 tokens, heads of 128: 32 + 8 heads 135 us (5.0 TB/s), pullback 270 (3.7); 32 + 32 heads 196 (5.5) and 381 (4.2);
+// Float32, 16384 tokens, 32 + 8 heads 122 (5.5) and 168 (6.0): what bounds the 16-bit pullback is the number of rows under
+// way, 64 to an SM at 128 registers a thread, and the issue slots that a row takes however many bytes it has.  Float16, 6000
+// tokens, 8 + 8 heads of 80: 13.5 and 29.4 (2.3 and 1.6 TB/s): four or five tokens to a warp, each a chain of angles, shared
+// memory and rows, and eight heads are six rows and two for its six groups.
 // The weights' gradient: a thread's pairs are the same in every row it meets, so it sums in registers; the block adds its
 // groups in a fixed order and leaves one row of partial sums in the workspace, norm_rope_reduce_kernel adds those in order.
 #include <algorithm>
@@ -152,8 +154,9 @@ __global__ void __launch_bounds__(kNrThreads, V == 1 ? 3 : (BWD && V == 8 ? 4 : 
   }
 
   // Frequencies in turns per position, the fraction as 64 bits: a position times that, whose overflow are whole turns, is the
-  // angle to 2^-32 of a turn or better wherever the position is (a Float32 product near 10^6 would be off by 0.06, and
-  // Float64 arithmetic for every token and pair costs more issue slots than the row)
+  // angle to 2^-32 of a turn for frequencies up to 1 and positions below 2^23, to 2^-24 at 2^31, where the frequency's own last
+  // bits count (a Float32 product near 10^6 would be off by 0.06, and Float64 arithmetic for every token and pair costs more
+  // issue slots than the row)
   __shared__ unsigned long long sm_freq[kNrMaxPairs];
   __shared__ float2 sm_turn[kNrWarps][kNrMaxPairs];
   __shared__ float sm_one[kNrMaxPairs];                  // NaN for a frequency that is not finite
@@ -206,7 +209,8 @@ __global__ void __launch_bounds__(kNrThreads, V == 1 ? 3 : (BWD && V == 8 ? 4 : 
     for (int p = wl; p < pairs; p += 32) {
       const float one = sm_one[p], turns = (float)(int)((sm_freq[p] * (unsigned long long)pos) >> 32) * 2.3283064365386963e-10f;
       float tc, ts;
-      // (16-bit results: sine and cosine to 2^-21)
+      // (16-bit results: sine and cosine to 2^-21, also where the weights and their gradients are Float32: half a step of what
+      // they are multiplied by is 2^-12 or more)
       if (sizeof(T) == 2) __sincosf(6.283185307179586f * turns, &ts, &tc);
       else sincospif(2.f * turns, &ts, &tc);
       sm_turn[warp][p] = make_float2(tc * one, ts * one);

@@ -123,8 +123,9 @@ def qk_norm_rope(q, k, gq, gk, freqs, *, nheads: int, start: Union[int, torch.Te
     ``2 * length(freqs)`` features is turned by the angle ``position * freqs[p]`` — features ``p`` and
     ``p + length(freqs)``, or ``2p`` and ``2p + 1`` where ``interleaved``; the others stay as they are.  Token ``l`` of
     sequence ``b`` is at position ``start + l``, ``start`` an integer or an Int32 tensor of one per sequence, or at
-    ``positions[l, b]`` (Int32; ``(len,)`` serves every sequence).  ``k`` has as many heads as its size says.  Arithmetic
-    is Float32 (angles in 64 bits until they are less than a turn), results are rounded once; head sizes are even, up to 256."""
+    ``positions[l, b]`` (Int32; ``(len,)`` serves every sequence; ``start`` is not looked at then).  ``k`` has as many heads as
+    its size says.  Arithmetic is Float32 (angles in 64 bits until they are less than a turn; sines and cosines of 16-bit calls
+    to 2^-21), results are rounded once; head sizes are even, up to 256."""
     p = _params(q, k, gq, gk, freqs, nheads, start, positions, eps, interleaved)
     yq, yk = _dense(q, *q.shape), _dense(k, *k.shape)
     p.yq, p.yk = yq.data_ptr(), yk.data_ptr()
@@ -136,7 +137,8 @@ def qk_norm_rope(q, k, gq, gk, freqs, *, nheads: int, start: Union[int, torch.Te
 def qk_norm_rope_pullback(q, k, gq, gk, freqs, *, nheads: int, start: Union[int, torch.Tensor] = 0,
                           positions: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False):
     """``rrule``-style forward of :func:`qk_norm_rope`: returns ``(q', k', back)`` where ``back(dq', dk')`` gives
-    ``(dq, dk, dgq, dgk)``.  Nothing but the arguments is kept, so ``q`` and ``k`` must not be written to in between.
+    ``(dq, dk, dgq, dgk)``.  Nothing but the arguments is kept, so none of them (``start`` and ``positions`` among them) may
+    be written to in between.
     The gradients of the weights are summed in Float32 in a fixed order and rounded to the weights' element type."""
     yq, yk = qk_norm_rope(q, k, gq, gk, freqs, nheads=nheads, start=start, positions=positions, eps=eps, interleaved=interleaved)
 
