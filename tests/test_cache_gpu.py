@@ -861,3 +861,47 @@ def test_a_caches_arrays_are_written_to_not_replaced():
     before = nb.cache_read(c, 5, dtype=F32)[0]
     c.k_scale *= 2
     assert torch.equal(nb.cache_read(c, 5, dtype=F32)[0], 2 * before)
+
+
+@gpu
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_lengths_about_the_point_where_sums_are_put_aside(code):
+    """256 tiles of 128 keys exactly, one key more, fewer, some more; queries on both sides of it; a poisoned page among the
+    first, and a missing one that only the last queries see.  One table of pages for all sequences."""
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    d, H, L, n, T = 16, 16, 45, 33024, 64
+    c = nb.QuantizedCache(d * H, n + T, 1, nheads=H, page=T, eltype=CODE[code], device=DEV)
+    k, v = (nb.jl_empty((d * H, n + T, 1), F16, DEV).normal_(generator=gen) for _ in range(2))
+    nb.cache_write_(c, k, v)
+    c.v_scale[:, n // T] = NAN                                   # page 516, which no healthy sequence has
+    lens = [32768, 32769, 32640, 33000, 5, 32790, 32800]
+    B = len(lens)
+    t = nb.jl_empty((n // T, B), torch.int32, DEV)
+    t.copy_(torch.arange(n // T, dtype=torch.int32, device=DEV)[:, None].expand(-1, B))
+    t[3, 5], t[512, 6] = n // T, -1                              # tokens 192 .. 255; 32768 .. 32831
+    q = nb.jl_empty((d * H, L, B), F16, DEV).normal_(generator=gen)
+    s = c._call(B, t)
+    p = nb._lib.CacheAttnParams(dtype=nb._lib.F16, causal=1, Hq=H, L=L, q=0x1000, x=0x1000, lens=0x1000)
+    lib = nb._lib.load()
+    assert lib.nnlib_b200_cache_attn_path(C.byref(s), C.byref(p)) == nb._lib.PATH_UMMA
+    assert lib.nnlib_b200_cache_attn_workspace_bytes(C.byref(s), C.byref(p)) >= 4 * d * H * L * B      # one part, with a row for sums
+    x, lse = nb.cached_attention(q, c, _i32(lens), nheads=H, table=t, return_lse=True)
+    nb.device_health()
+    kr, vr = (z[:, :n, 0].double() for z in nb.cache_read(c, n, dtype=F32))
+    for b, m in enumerate(lens):
+        sees = torch.arange(n, device=DEV)[None] <= (m - L + torch.arange(L, device=DEV))[:, None]
+        none = ~sees.any(1)
+        bad = sees[:, 32768:32832].any(1) if b == 6 else torch.full((L,), b == 5, device=DEV)
+        assert torch.equal(torch.isnan(x[:, :, b].float()).all(0), none | bad) and torch.equal(torch.isnan(x[:, :, b].float()).any(0), none | bad)
+        assert torch.equal(torch.isneginf(lse[:, 0, b]), none)
+        ok = ~(none | bad)
+        if not ok.any():
+            continue
+        for h in range(H):
+            r = slice(h * d, (h + 1) * d)
+            logits = (q[r, ok, b].double().T @ kr[r] / d ** 0.5).masked_fill(~sees[ok], -INF)
+            w = torch.softmax(logits, 1)
+            want, size = w @ vr[r].T, w @ vr[r].abs().T
+            lim = (2.0 ** -11 + 2.0 ** -13) * size + 2.0 ** -11 * want.abs() * 1.001 + 2.0 ** -25
+            assert ((x[r, ok, b].double().T - want).abs() <= lim).all()
+            torch.testing.assert_close(lse[ok, h, b].double(), torch.logsumexp(logits, 1), atol=2 * 12 * 2.0 ** -18, rtol=2.0 ** -20)
