@@ -349,8 +349,8 @@ NNLIB_B200_API int nnlib_b200_batched_gemm_path(const nnlib_b200_gemm_params* p)
    for the d features x of each head of q (weights gq) and of k (weights gk).  Pair p < rot / 2 is turned by the angle
    position * freqs[p]: (a, b) -> (a cos - b sin, a sin + b cos); a and b are features p and p + rot / 2 of the head,
    or 2p and 2p + 1 with interleaved = 1.  Features rot .. d - 1 are normalised only.  Angles are reduced to one turn in 64
-   bits, everything else is Float32, for 16-bit arrays with sines and cosines to 2^-21 (also in the gradients of Float32
-   weights); results are rounded once.  The reference has no counterpart. */
+   bits, everything else is Float32, where all results are 16-bit with sines and cosines to 2^-21; results are rounded once.
+   The reference has no counterpart. */
 typedef struct nnlib_b200_norm_rope_params {
   size_t struct_size;        /* = sizeof(nnlib_b200_norm_rope_params) */
   int32_t dtype;             /* element type of q, k and of the results */

@@ -9,7 +9,8 @@
 // holds as many groups as fit (six of five lanes for a head of 80 features) and works by itself: it takes a token, or some of
 // a token's heads where tokens are few, works out its angles, and walks over the heads, the next rows, then the next token's,
 // always under way.  Queries and keys are two ranges of blocks of one launch.
-// bf16, 32768 tokens, heads of 128: 32 + 8 heads 135 us (5.0 TB/s), pullback 270 (3.7); 32 + 32 heads 196 (5.5) and 381 (4.2);
+// bf16, 32768 tokens, heads of 128: 32 + 8 heads 135 us (5.0 TB/s), pullback 273 (3.7; Float32 weights, whose
+// gradients ask for better sines, 275); 32 + 32 heads 196 (5.5) and 381 (4.2; 387);
 // Float32, 16384 tokens, 32 + 8 heads 122 (5.5) and 168 (6.0): what bounds the 16-bit pullback is the number of rows under
 // way, 64 to an SM at 128 registers a thread, and the issue slots that a row takes however many bytes it has.  Float16, 6000
 // tokens, 8 + 8 heads of 80: 13.5 and 29.4 (2.3 and 1.6 TB/s): four or five tokens to a warp, each a chain of angles, shared
@@ -209,9 +210,8 @@ __global__ void __launch_bounds__(kNrThreads, V == 1 ? 3 : (BWD && V == 8 ? 4 : 
     for (int p = wl; p < pairs; p += 32) {
       const float one = sm_one[p], turns = (float)(int)((sm_freq[p] * (unsigned long long)pos) >> 32) * 2.3283064365386963e-10f;
       float tc, ts;
-      // (16-bit results: sine and cosine to 2^-21, also where the weights and their gradients are Float32: half a step of what
-      // they are multiplied by is 2^-12 or more)
-      if (sizeof(T) == 2) __sincosf(6.283185307179586f * turns, &ts, &tc);
+      // (16-bit results: sine and cosine to 2^-21; not where the weights' gradients are Float32)
+      if (sizeof(T) == 2 && !(BWD && a.wdtype == NNLIB_B200_F32)) __sincosf(6.283185307179586f * turns, &ts, &tc);
       else sincospif(2.f * turns, &ts, &tc);
       sm_turn[warp][p] = make_float2(tc * one, ts * one);
     }
@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(kNrThreads, V == 1 ? 3 : (BWD && V == 8 ? 4 : 
       const float sum = group_sum(pair_sum(sum2), lanes, lane, wl - lane);
       // (the approximation's error, two units in the last place, is little beside the sum's)
       // A group that has no row this time must add nothing to the weights' gradient: with eps = 0 its r would be infinite.
-      const float r = live || !BWD ? rsqrtf(fmaf(sum, inv_d, a.eps)) : 0.f;
+      const float r = rsqrtf(fmaf(sum, inv_d, live || !BWD ? a.eps : 1.f));
       const Two r2 = pair_of(r);
       Two back2 = 0ull;
       if (BWD) back2 = pair_of(-group_sum(pair_sum(dot2), lanes, lane, wl - lane) * inv_d * r * r);

@@ -124,8 +124,8 @@ def qk_norm_rope(q, k, gq, gk, freqs, *, nheads: int, start: Union[int, torch.Te
     ``p + length(freqs)``, or ``2p`` and ``2p + 1`` where ``interleaved``; the others stay as they are.  Token ``l`` of
     sequence ``b`` is at position ``start + l``, ``start`` an integer or an Int32 tensor of one per sequence, or at
     ``positions[l, b]`` (Int32; ``(len,)`` serves every sequence; ``start`` is not looked at then).  ``k`` has as many heads as
-    its size says.  Arithmetic is Float32 (angles in 64 bits until they are less than a turn; sines and cosines of 16-bit calls
-    to 2^-21), results are rounded once; head sizes are even, up to 256."""
+    its size says.  Arithmetic is Float32 (angles in 64 bits until they are less than a turn; sines and cosines to
+    2^-21 where all results are 16-bit), results are rounded once; head sizes are even, up to 256."""
     p = _params(q, k, gq, gk, freqs, nheads, start, positions, eps, interleaved)
     yq, yk = _dense(q, *q.shape), _dense(k, *k.shape)
     p.yq, p.yk = yq.data_ptr(), yk.data_ptr()

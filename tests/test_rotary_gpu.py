@@ -289,3 +289,28 @@ def test_features_that_are_not_turned_meet_no_others(dtype, d, rot, inter):
         dgq = nb.qk_norm_rope_pullback(q, q, g, g, f, nheads=H, interleaved=inter, start=4)[2](loud, dy)[2]
         hit = ~torch.isfinite(dgq.float())
         assert hit[at] and hit.sum().item() == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("inter", [False, True])
+def test_float32_gradients_of_the_weights_of_16_bit_arrays(dtype, inter):
+    """One row, so that nothing averages out: dg = u x r with u = a cos + b sin of two elements of the cotangent.  The turn is a
+    Float32 below 1/2 (2^-26 of a turn, 2^-23.35 as an angle), sine and cosine are within one unit, 2^-24 below 1, and one product
+    is rounded: u is off by (|a| + |b|) (2^-23.35 + 2^-24 + 2^-24) < 2^-22.1 (|a| + |b|).  The sum u, r (two units, and the sum
+    of squares) and the products by it: 2^-24 + 2^-22 + 2^-23 + 2 * 2^-24 < 2^-21 of the result."""
+    d = 128
+    gen = np.random.default_rng(41)
+    f, g = nb.rope_frequencies(d), 1 + 0.2 * _array(gen, (d,), F32)
+    g64, f64 = _f64(g), f.cpu().numpy()
+    for at in list(range(40)) + [1000, 77777]:
+        x, dy = _array(gen, (d, 1, 1), dtype), _array(gen, (d, 1, 1), dtype)
+        got = nb.qk_norm_rope_pullback(x, x, g, g, f, nheads=1, interleaved=inter, start=at)[2](dy, dy)
+        pos = np.full((1, 1), float(at))
+        _, dg = R.pullback(_f64(x), g64, pos, f64, 1e-6, inter, _f64(dy))
+        a = np.abs(_f64(dy)[:, 0, 0])
+        both = a + (a.reshape(-1, 2)[:, ::-1].reshape(-1) if inter else np.roll(a, d // 2))
+        xr = np.abs(_f64(x)[:, 0, 0]) / np.sqrt((_f64(x) ** 2).mean() + 1e-6)
+        for s in got[2:]:
+            over = np.abs(_f64(s) - dg) - 2.0 ** -22.1 * both * xr - 2.0 ** -21 * np.abs(dg)
+            assert over.max() <= 0, (at, over.max())
