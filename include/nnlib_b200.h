@@ -483,6 +483,135 @@ NNLIB_B200_API int nnlib_b200_cache_attn(const nnlib_b200_cache* c, const nnlib_
 /* NNLIB_B200_PATH_UMMA or NNLIB_B200_PATH_SIMT (warp-level products), what cache_attn would take, or a negative error */
 NNLIB_B200_API int nnlib_b200_cache_attn_path(const nnlib_b200_cache* c, const nnlib_b200_cache_attn_params* p);
 
+/* Products of ragged groups of columns: what a router, its experts and the low-rank pairs of many requests need.  Sizes of
+   groups are on the device only: offsets (runs + 1) says that run g is columns offsets[g] .. offsets[g+1] - 1.  An offset
+   outside 0 .. R counts as the nearer of the two, a run that ends before it begins as empty; runs that overlap leave their
+   common columns undefined. */
+
+/* Each token's k best of G experts (1 <= k <= min(G, 32), G <= 1024) and the tokens' order by expert.
+   Chosen are the k largest of logits + bias (in Float32; ties: the lower expert first; a NaN is below everything), in falling order; their
+   weights are softmax(logits) over the chosen (normalize) or over all experts: equal shares for +Inf, NaN where a NaN or
+   nothing but -Inf is among those that the softmax is over.  A token whose mask byte is 0 takes no part: experts and
+   position -1, weights 0.  The chosen (token, expert) pairs are numbered by expert, then by token:
+     offsets  (G + 1)  expert g has numbers offsets[g] .. offsets[g+1] - 1
+     columns  (k*N)    the token of each number, -1 from offsets[G] on
+     position (k, N)   the number of each pair
+   N * k < 2^31. */
+typedef struct nnlib_b200_route_params {
+  size_t struct_size;        /* = sizeof(nnlib_b200_route_params) */
+  int32_t dtype;             /* element type of logits and dlogits */
+  int32_t normalize;
+  int64_t G, N, k;
+  const void* logits;        /* (G, N), expert stride 1 */
+  int64_t logits_stride;     /* elements between two tokens, 0 = G */
+  const float* bias;         /* (G), for the choice alone; NULL: none */
+  const uint8_t* mask;       /* (N), 0: takes no part; NULL: all do */
+  float* weights;            /* (k, N); route_bwd: read */
+  int32_t* experts;          /* (k, N); route_bwd: read */
+  int32_t* offsets;
+  int32_t* columns;
+  int32_t* position;
+  const float* dweights;     /* route_bwd: (k, N) */
+  void* dlogits;             /* route_bwd: (G, N), dense */
+} nnlib_b200_route_params;
+
+/* workspace: device memory, 16-byte aligned, at least nnlib_b200_route_workspace_bytes(p) bytes (which may be 0), not cleared */
+NNLIB_B200_API size_t nnlib_b200_route_workspace_bytes(const nnlib_b200_route_params* p);
+NNLIB_B200_API int nnlib_b200_route(const nnlib_b200_route_params* p, void* workspace, size_t workspace_bytes, void* stream);
+/* Gradient of the logits from the forward call's logits, experts and weights; the choice and the bias have none. */
+NNLIB_B200_API int nnlib_b200_route_bwd(const nnlib_b200_route_params* p, void* stream);
+
+/* C[:, i] = A[:, :, g] * X[:, columns[i]] for the columns i of run g: batched_gemm with ragged, gathered batches.  Columns
+   of C in no run become zeros (zero_rest) or are left as they are; one whose column of X does not exist becomes zeros.
+   Sums are Float32, rounded once. */
+typedef struct nnlib_b200_grouped_params {
+  size_t struct_size;        /* = sizeof(nnlib_b200_grouped_params) */
+  int32_t dtype;
+  int32_t transA;            /* 1: A is stored as (K, M, G) */
+  int32_t zero_rest;
+  int32_t reserved;
+  int64_t M, K, G;
+  int64_t N, R;              /* columns of X and of C */
+  void* A;                   /* (M, K, G); written by grouped_gemm_grad */
+  int64_t lda, strideA;      /* elements between columns and between matrices */
+  const void* X;             /* (K, N) */
+  int64_t ldx;
+  void* C;                   /* (M, R); read by grouped_gemm_grad */
+  int64_t ldc;
+  const int32_t* offsets;    /* (G + 1) */
+  const int32_t* columns;    /* (R); NULL: column i of C is of column i of X, R <= N */
+  int32_t* status;           /* optional device int32, as in nnlib_b200_attn_params */
+} nnlib_b200_grouped_params;
+
+/* workspace: device memory, 16-byte aligned, at least the matching _workspace_bytes(p) bytes (which may be 0), not cleared */
+NNLIB_B200_API size_t nnlib_b200_grouped_gemm_workspace_bytes(const nnlib_b200_grouped_params* p);
+NNLIB_B200_API int nnlib_b200_grouped_gemm(const nnlib_b200_grouped_params* p, void* workspace, size_t workspace_bytes,
+                                           void* stream);
+/* The matrices' gradient: A[:, :, g] = sum over the columns i of run g of C[:, i] * X[:, columns[i]]^T, zeros for an empty
+   run.  Columns of X that do not exist are left out. */
+NNLIB_B200_API size_t nnlib_b200_grouped_gemm_grad_workspace_bytes(const nnlib_b200_grouped_params* p);
+NNLIB_B200_API int nnlib_b200_grouped_gemm_grad(const nnlib_b200_grouped_params* p, void* workspace, size_t workspace_bytes,
+                                                void* stream);
+
+/* y[:, t] = sum_j weights[j, t] * Y[:, position[j, t]], j ascending, in Float32; positions outside 0 .. R - 1 add nothing. */
+typedef struct nnlib_b200_combine_params {
+  size_t struct_size;        /* = sizeof(nnlib_b200_combine_params) */
+  int32_t dtype;
+  int32_t reserved;
+  int64_t E, N, R, k;        /* 1 <= k <= 32 */
+  const void* Y;             /* (E, R), feature stride 1 */
+  int64_t Y_stride;          /* elements, 0 = E */
+  const int32_t* position;   /* (k, N) */
+  const float* weights;      /* (k, N); NULL: ones */
+  void* y;                   /* (E, N), feature stride 1 */
+  int64_t y_stride;
+  const int32_t* columns;    /* combine_bwd: (R), the token of each column, the inverse of position */
+  const void* dy;            /* combine_bwd: (E, N), feature stride 1 */
+  int64_t dy_stride;
+  void* dY;                  /* combine_bwd: (E, R), dense; zeros where columns and position name no pair */
+  float* dweights;           /* combine_bwd: (k, N); NULL: not wanted */
+} nnlib_b200_combine_params;
+
+NNLIB_B200_API int nnlib_b200_combine(const nnlib_b200_combine_params* p, void* stream);
+NNLIB_B200_API int nnlib_b200_combine_bwd(const nnlib_b200_combine_params* p, void* stream);
+
+/* C = W * X + scale[a] * B[:, :, a] * (A[:, :, a] * X) for the columns of the runs whose id a is a pair's number; a run with
+   another id, and a column in no run, gets W * X alone.  scale * A * X is rounded to two terms of the element type (Float32: not
+   at all) and multiplied by B into the same Float32 sum as W * X. */
+typedef struct nnlib_b200_adapter_params {
+  size_t struct_size;        /* = sizeof(nnlib_b200_adapter_params) */
+  int32_t dtype;
+  int32_t transW, transA, transB;   /* 1: stored as (K, M), (K, r, n), (r, M, n) */
+  int64_t M, K, N;
+  int64_t r, n;              /* rank (1 .. 128) and number of pairs */
+  int64_t runs;
+  const void* W; int64_t ldw;                      /* (M, K) */
+  const void* A; int64_t lda, strideA;             /* (r, K, n) */
+  const void* B; int64_t ldb, strideB;             /* (M, r, n) */
+  const void* X; int64_t ldx;                      /* (K, N) */
+  void* C; int64_t ldc;                            /* (M, N) */
+  const int32_t* offsets;    /* (runs + 1); NULL: run b is columns run_len*b .. run_len*(b+1) - 1 */
+  int64_t run_len;
+  const int32_t* ids;        /* (runs) */
+  const float* scale;        /* (n); NULL: scale0 for all */
+  float scale0;
+  int32_t reserved;
+  const void* dC; int64_t lddc;                    /* adapter_bwd: the cotangent, (M, N) */
+  void* dX;                  /* adapter_bwd: (K, N), dense */
+  void* dA;                  /* adapter_bwd: stored like A, dense; zeros for a pair that no run names.  dA and dB may both be NULL */
+  void* dB;
+  int32_t* status;           /* optional device int32, as in nnlib_b200_attn_params */
+} nnlib_b200_adapter_params;
+
+/* workspace: device memory, 16-byte aligned, at least the matching _workspace_bytes(p) bytes, not cleared */
+NNLIB_B200_API size_t nnlib_b200_adapter_gemm_workspace_bytes(const nnlib_b200_adapter_params* p);
+NNLIB_B200_API int nnlib_b200_adapter_gemm(const nnlib_b200_adapter_params* p, void* workspace, size_t workspace_bytes,
+                                           void* stream);
+/* Gradients of X, A and B; W has none here (it is what adapters leave as it is). */
+NNLIB_B200_API size_t nnlib_b200_adapter_bwd_workspace_bytes(const nnlib_b200_adapter_params* p);
+NNLIB_B200_API int nnlib_b200_adapter_bwd(const nnlib_b200_adapter_params* p, void* workspace, size_t workspace_bytes,
+                                          void* stream);
+
 /* make_causal_mask (src/attention.jl:149-153): fill an (L, L) byte matrix
    with m[i + L*j] = (i <= j). */
 NNLIB_B200_API int nnlib_b200_causal_fill(uint8_t* mask, int64_t L, void* stream);

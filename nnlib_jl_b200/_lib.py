@@ -64,6 +64,19 @@ EXPORTS = (
     "nnlib_b200_cache_attn",
     "nnlib_b200_cache_attn_workspace_bytes",
     "nnlib_b200_cache_attn_path",
+    "nnlib_b200_route",
+    "nnlib_b200_route_workspace_bytes",
+    "nnlib_b200_route_bwd",
+    "nnlib_b200_grouped_gemm",
+    "nnlib_b200_grouped_gemm_workspace_bytes",
+    "nnlib_b200_grouped_gemm_grad",
+    "nnlib_b200_grouped_gemm_grad_workspace_bytes",
+    "nnlib_b200_combine",
+    "nnlib_b200_combine_bwd",
+    "nnlib_b200_adapter_gemm",
+    "nnlib_b200_adapter_gemm_workspace_bytes",
+    "nnlib_b200_adapter_bwd",
+    "nnlib_b200_adapter_bwd_workspace_bytes",
     "nnlib_b200_device_health",
     "nnlib_b200_selftest_wait_runout",
     "nnlib_b200_strerror",
@@ -243,6 +256,86 @@ class CacheAttnParams(C.Structure):
             self.nan_on_fully_masked = 1
 
 
+class RouteParams(C.Structure):
+    """Mirror of ``nnlib_b200_route_params``."""
+
+    _fields_ = [
+        ("struct_size", C.c_size_t),
+        ("dtype", C.c_int32), ("normalize", C.c_int32),
+        ("G", C.c_int64), ("N", C.c_int64), ("k", C.c_int64),
+        ("logits", C.c_void_p), ("logits_stride", C.c_int64),
+        ("bias", C.c_void_p), ("mask", C.c_void_p),
+        ("weights", C.c_void_p), ("experts", C.c_void_p), ("offsets", C.c_void_p), ("columns", C.c_void_p), ("position", C.c_void_p),
+        ("dweights", C.c_void_p), ("dlogits", C.c_void_p),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__(**kw)
+        self.struct_size = C.sizeof(RouteParams)
+
+
+class GroupedParams(C.Structure):
+    """Mirror of ``nnlib_b200_grouped_params``."""
+
+    _fields_ = [
+        ("struct_size", C.c_size_t),
+        ("dtype", C.c_int32), ("transA", C.c_int32), ("zero_rest", C.c_int32), ("reserved", C.c_int32),
+        ("M", C.c_int64), ("K", C.c_int64), ("G", C.c_int64), ("N", C.c_int64), ("R", C.c_int64),
+        ("A", C.c_void_p), ("lda", C.c_int64), ("strideA", C.c_int64),
+        ("X", C.c_void_p), ("ldx", C.c_int64),
+        ("C", C.c_void_p), ("ldc", C.c_int64),
+        ("offsets", C.c_void_p), ("columns", C.c_void_p), ("status", C.c_void_p),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__(**kw)
+        self.struct_size = C.sizeof(GroupedParams)
+
+
+class CombineParams(C.Structure):
+    """Mirror of ``nnlib_b200_combine_params``."""
+
+    _fields_ = [
+        ("struct_size", C.c_size_t),
+        ("dtype", C.c_int32), ("reserved", C.c_int32),
+        ("E", C.c_int64), ("N", C.c_int64), ("R", C.c_int64), ("k", C.c_int64),
+        ("Y", C.c_void_p), ("Y_stride", C.c_int64),
+        ("position", C.c_void_p), ("weights", C.c_void_p),
+        ("y", C.c_void_p), ("y_stride", C.c_int64),
+        ("columns", C.c_void_p),
+        ("dy", C.c_void_p), ("dy_stride", C.c_int64),
+        ("dY", C.c_void_p), ("dweights", C.c_void_p),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__(**kw)
+        self.struct_size = C.sizeof(CombineParams)
+
+
+class AdapterParams(C.Structure):
+    """Mirror of ``nnlib_b200_adapter_params``."""
+
+    _fields_ = [
+        ("struct_size", C.c_size_t),
+        ("dtype", C.c_int32), ("transW", C.c_int32), ("transA", C.c_int32), ("transB", C.c_int32),
+        ("M", C.c_int64), ("K", C.c_int64), ("N", C.c_int64), ("r", C.c_int64), ("n", C.c_int64), ("runs", C.c_int64),
+        ("W", C.c_void_p), ("ldw", C.c_int64),
+        ("A", C.c_void_p), ("lda", C.c_int64), ("strideA", C.c_int64),
+        ("B", C.c_void_p), ("ldb", C.c_int64), ("strideB", C.c_int64),
+        ("X", C.c_void_p), ("ldx", C.c_int64),
+        ("C", C.c_void_p), ("ldc", C.c_int64),
+        ("offsets", C.c_void_p), ("run_len", C.c_int64), ("ids", C.c_void_p),
+        ("scale", C.c_void_p), ("scale0", C.c_float), ("reserved", C.c_int32),
+        ("dC", C.c_void_p), ("lddc", C.c_int64),
+        ("dX", C.c_void_p), ("dA", C.c_void_p), ("dB", C.c_void_p),
+        ("status", C.c_void_p),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__(**kw)
+        self.struct_size = C.sizeof(AdapterParams)
+
+
 _lib = None
 
 
@@ -320,6 +413,16 @@ def load() -> C.CDLL:
     lib.nnlib_b200_cache_attn_path.restype = C.c_int
     lib.nnlib_b200_cache_attn_workspace_bytes.argtypes = [CP, CA]
     lib.nnlib_b200_cache_attn_workspace_bytes.restype = C.c_size_t
+    for name, of, works in (("route", RouteParams, True), ("route_bwd", RouteParams, False), ("grouped_gemm", GroupedParams, True),
+                            ("grouped_gemm_grad", GroupedParams, True), ("combine", CombineParams, False),
+                            ("combine_bwd", CombineParams, False), ("adapter_gemm", AdapterParams, True), ("adapter_bwd", AdapterParams, True)):
+        fn = getattr(lib, "nnlib_b200_" + name)
+        fn.argtypes = [C.POINTER(of), C.c_void_p, C.c_size_t, C.c_void_p] if works else [C.POINTER(of), C.c_void_p]
+        fn.restype = C.c_int
+        if works:
+            fn = getattr(lib, f"nnlib_b200_{name}_workspace_bytes")
+            fn.argtypes = [C.POINTER(of)]
+            fn.restype = C.c_size_t
     lib.nnlib_b200_attn_path.argtypes = [P]
     lib.nnlib_b200_attn_path.restype = C.c_int
     lib.nnlib_b200_device_health.argtypes = [C.c_void_p]

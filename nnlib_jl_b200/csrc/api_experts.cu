@@ -1,0 +1,353 @@
+// The C ABI of products of ragged groups of columns (include/nnlib_b200.h): the router, its experts' products, their weighted
+// sum, low-rank adapters.  Argument checks and defaults, as in api.cu.
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <cstdio>
+#include <cstring>
+
+#include "common.cuh"
+#include "launchers.h"
+
+namespace nb200 {
+namespace {
+
+constexpr int64_t kMost = 0x7fffffffLL;
+
+bool dtype_ok(int dt) { return dt == NNLIB_B200_F16 || dt == NNLIB_B200_BF16 || dt == NNLIB_B200_F32; }
+int esize(int dt) { return dt == NNLIB_B200_F32 ? 4 : 2; }
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+bool extent(int64_t n) { return n >= 0 && n <= kMost; }
+
+// the arrays of a call: the first `always` are looked up on every call, the rest under NNLIB_B200_CHECK_POINTERS
+int check_arrays(const void* const* ptrs, int always, int n) {
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    return NNLIB_B200_CUDA_ERROR;
+  }
+  const int m = check_all_pointers() ? n : always;
+  for (int i = 0; i < m; ++i)
+    if (!on_current_device(ptrs[i], dev)) return NNLIB_B200_INVALID_ARG;
+  return NNLIB_B200_OK;
+}
+
+// `count` matrices of rows x cols, stored as they are or transposed
+bool matrix_ok(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t stride, int64_t count, bool trans, int z) {
+  if (rows == 0 || cols == 0 || count == 0) return true;
+  return p && aligned(p, z) && ld >= (trans ? cols : rows) && stride >= 0 && ld < (1ll << 40) && stride < (1ll << 40);
+}
+
+// ------------------------------------------------------------------------------------------------- router
+int resolve_route(const nnlib_b200_route_params* p, bool bwd, RouteArgs* out) {
+  if (!p || p->struct_size != sizeof(*p) || !dtype_ok(p->dtype)) return NNLIB_B200_INVALID_ARG;
+  if (p->G < 1 || p->N < 0 || p->k < 1 || p->k > p->G || p->logits_stride < 0) return NNLIB_B200_INVALID_ARG;
+  if (p->G > 1024 || p->k > 32) return NNLIB_B200_UNSUPPORTED_SHAPE;
+  if (p->N > kMost / p->k) return NNLIB_B200_INVALID_ARG;
+  RouteArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.logits = p->logits;
+  a.stride = p->logits_stride ? p->logits_stride : p->G;
+  if (a.stride < p->G) return NNLIB_B200_INVALID_ARG;
+  a.bias = p->bias;
+  a.mask = p->mask;
+  a.weights = p->weights;
+  a.experts = p->experts;
+  a.offsets = p->offsets;
+  a.columns = p->columns;
+  a.position = p->position;
+  a.dweights = p->dweights;
+  a.dlogits = p->dlogits;
+  a.G = (int)p->G; a.N = (int)p->N; a.k = (int)p->k;
+  a.normalize = p->normalize ? 1 : 0;
+  const int z = esize(p->dtype);
+  if (!aligned(p->logits, z) || !aligned(p->bias, 4) || !aligned(p->weights, 4) || !aligned(p->experts, 4) || !aligned(p->offsets, 4) ||
+      !aligned(p->columns, 4) || !aligned(p->position, 4) || !aligned(p->dweights, 4) || !aligned(p->dlogits, z))
+    return NNLIB_B200_INVALID_ARG;
+  if (a.N && (!p->logits || !p->weights || !p->experts)) return NNLIB_B200_INVALID_ARG;
+  if (bwd) {
+    if (a.N && (!p->dweights || !p->dlogits)) return NNLIB_B200_INVALID_ARG;
+  } else if (!p->offsets || (a.N && (!p->columns || !p->position))) {
+    return NNLIB_B200_INVALID_ARG;
+  }
+  *out = a;
+  return NNLIB_B200_OK;
+}
+
+// ------------------------------------------------------------------------------------------------- grouped products
+int resolve_grouped(const nnlib_b200_grouped_params* p, GroupedArgs* out) {
+  if (!p || p->struct_size != sizeof(*p) || !dtype_ok(p->dtype)) return NNLIB_B200_INVALID_ARG;
+  if (!extent(p->M) || !extent(p->K) || !extent(p->N) || !extent(p->R) || p->G < 0) return NNLIB_B200_INVALID_ARG;
+  if (p->G > 32767 || p->R > kMost - 65536) return NNLIB_B200_UNSUPPORTED_SHAPE;
+  const int z = esize(p->dtype);
+  if (!matrix_ok(p->A, p->M, p->K, p->lda, p->strideA, p->G, p->transA != 0, z) || !matrix_ok(p->X, p->K, p->N, p->ldx, 0, 1, false, z) ||
+      !matrix_ok(p->C, p->M, p->R, p->ldc, 0, 1, false, z))
+    return NNLIB_B200_INVALID_ARG;
+  if ((p->G > 0 && !p->offsets) || (!p->columns && p->R > p->N)) return NNLIB_B200_INVALID_ARG;
+  if (!aligned(p->offsets, 4) || !aligned(p->columns, 4) || !aligned(p->status, 4)) return NNLIB_B200_INVALID_ARG;
+  GroupedArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.A = p->A; a.X = p->X; a.C = p->C;
+  a.lda = p->lda; a.strideA = p->strideA; a.ldx = p->ldx; a.ldc = p->ldc;
+  a.offsets = p->offsets;
+  a.columns = p->columns;
+  a.scale0 = 1.f;
+  a.transA = p->transA ? 1 : 0;
+  a.zero_rest = p->zero_rest ? 1 : 0;
+  a.M = (int)p->M; a.K = (int)p->K; a.G = (int)p->G; a.N = (int)p->N; a.R = (int)p->R;
+  a.mats = a.G;
+  a.status = p->status;
+  *out = a;
+  return NNLIB_B200_OK;
+}
+GroupedGradArgs grad_of(const GroupedArgs& a) {
+  GroupedGradArgs g;
+  std::memset(&g, 0, sizeof(g));
+  g.A = const_cast<void*>(a.A); g.X = a.X; g.C = a.C;
+  g.lda = a.lda; g.strideA = a.strideA; g.ldx = a.ldx; g.ldc = a.ldc;
+  g.offsets = a.offsets; g.ids = a.ids; g.columns = a.columns; g.run_len = a.run_len;
+  g.transA = a.transA;
+  g.M = a.M; g.K = a.K; g.G = a.G; g.N = a.N; g.R = a.R; g.mats = a.mats;
+  g.status = a.status;
+  return g;
+}
+int check_grouped_arrays(const GroupedArgs& a) {
+  const void* all[] = {a.C, a.X, a.A, a.offsets, a.columns, a.status};
+  return check_arrays(all, 2, 6);
+}
+
+// ------------------------------------------------------------------------------------------------- combine
+int resolve_combine(const nnlib_b200_combine_params* p, bool bwd, CombineArgs* out) {
+  if (!p || p->struct_size != sizeof(*p) || !dtype_ok(p->dtype)) return NNLIB_B200_INVALID_ARG;
+  if (p->E < 1 || !extent(p->E) || !extent(p->N) || !extent(p->R) || p->k < 1) return NNLIB_B200_INVALID_ARG;
+  if (p->k > 32) return NNLIB_B200_UNSUPPORTED_SHAPE;
+  if (p->N > kMost / p->k || p->R > kMost - 8) return NNLIB_B200_INVALID_ARG;
+  CombineArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.Y = p->Y; a.y = p->y; a.dy = p->dy; a.dY = p->dY;
+  a.position = p->position;
+  a.weights = p->weights;
+  a.columns = p->columns;
+  a.dweights = p->dweights;
+  a.Y_stride = p->Y_stride ? p->Y_stride : p->E;
+  a.y_stride = p->y_stride ? p->y_stride : p->E;
+  a.dy_stride = p->dy_stride ? p->dy_stride : p->E;
+  a.E = (int)p->E; a.N = (int)p->N; a.R = (int)p->R; a.k = (int)p->k;
+  const int z = esize(p->dtype);
+  if (a.Y_stride < p->E || a.y_stride < p->E || a.dy_stride < p->E) return NNLIB_B200_INVALID_ARG;
+  if (!aligned(p->Y, z) || !aligned(p->y, z) || !aligned(p->dy, z) || !aligned(p->dY, z) || !aligned(p->position, 4) ||
+      !aligned(p->weights, 4) || !aligned(p->columns, 4) || !aligned(p->dweights, 4))
+    return NNLIB_B200_INVALID_ARG;
+  if (a.N && !p->position) return NNLIB_B200_INVALID_ARG;
+  if (a.R && !p->Y && (!bwd || p->dweights)) return NNLIB_B200_INVALID_ARG;
+  if (bwd) {
+    if ((a.R && (!p->dY || !p->columns)) || (a.N && !p->dy)) return NNLIB_B200_INVALID_ARG;
+  } else if (a.N && !p->y) {
+    return NNLIB_B200_INVALID_ARG;
+  }
+  *out = a;
+  return NNLIB_B200_OK;
+}
+
+// ------------------------------------------------------------------------------------------------- adapters
+struct Adapters {
+  GroupedArgs main;          // W X with the low-rank term; for the gradient of X W^T dC
+  GroupedArgs first;         // the factor next to the columns: A X; for the gradient of X B^T dC
+};
+
+int resolve_adapter(const nnlib_b200_adapter_params* p, bool bwd, Adapters* out) {
+  if (!p || p->struct_size != sizeof(*p) || !dtype_ok(p->dtype)) return NNLIB_B200_INVALID_ARG;
+  if (!extent(p->M) || !extent(p->K) || !extent(p->N) || p->r < 1 || p->n < 0 || p->runs < 0 || p->run_len < 0) return NNLIB_B200_INVALID_ARG;
+  if (p->r > 128 || p->n > 32767 || p->runs > (1 << 20) || p->N > kMost - 65536) return NNLIB_B200_UNSUPPORTED_SHAPE;
+  if (p->run_len > kMost) return NNLIB_B200_INVALID_ARG;
+  const int z = esize(p->dtype);
+  if (!matrix_ok(p->W, p->M, p->K, p->ldw, 0, 1, p->transW != 0, z) || !matrix_ok(p->A, p->r, p->K, p->lda, p->strideA, p->n, p->transA != 0, z) ||
+      !matrix_ok(p->B, p->M, p->r, p->ldb, p->strideB, p->n, p->transB != 0, z))
+    return NNLIB_B200_INVALID_ARG;
+  if (p->runs > 0 && !p->ids) return NNLIB_B200_INVALID_ARG;
+  if (!aligned(p->offsets, 4) || !aligned(p->ids, 4) || !aligned(p->scale, 4) || !aligned(p->status, 4)) return NNLIB_B200_INVALID_ARG;
+  if (!bwd) {
+    if (!matrix_ok(p->X, p->K, p->N, p->ldx, 0, 1, false, z) || !matrix_ok(p->C, p->M, p->N, p->ldc, 0, 1, false, z)) return NNLIB_B200_INVALID_ARG;
+  } else {
+    if (!matrix_ok(p->dC, p->M, p->N, p->lddc, 0, 1, false, z) || !matrix_ok(p->dX, p->K, p->N, p->K, 0, 1, false, z)) return NNLIB_B200_INVALID_ARG;
+    if ((p->dA == nullptr) != (p->dB == nullptr) && p->M && p->K && p->n) return NNLIB_B200_INVALID_ARG;
+    if (p->dA && !matrix_ok(p->X, p->K, p->N, p->ldx, 0, 1, false, z)) return NNLIB_B200_INVALID_ARG;
+    if (!aligned(p->dA, z) || !aligned(p->dB, z)) return NNLIB_B200_INVALID_ARG;
+  }
+  Adapters a;
+  std::memset(&a, 0, sizeof(a));
+  GroupedArgs& m = a.main;
+  GroupedArgs& f = a.first;
+  f.offsets = p->offsets;
+  f.ids = p->ids;
+  f.run_len = p->run_len;
+  f.scale = p->scale;
+  f.scale0 = p->scale0;
+  f.G = (int)p->runs; f.mats = (int)p->n;
+  f.M = (int)p->r;
+  f.N = f.R = m.N = m.R = (int)p->N;
+  f.status = m.status = p->status;
+  m.A = p->W; m.lda = p->ldw;
+  m.G = m.mats = 1;
+  m.run_len = p->N;
+  m.scale0 = 1.f;
+  LowRank& l = m.low;
+  l.offsets = p->offsets;
+  l.ids = p->ids;
+  l.run_len = p->run_len;
+  l.r = (int)p->r; l.n = (int)p->n; l.runs = (int)p->runs;
+  if (!bwd) {
+    m.M = (int)p->M; m.K = f.K = (int)p->K;
+    m.transA = p->transW ? 1 : 0;
+    m.X = f.X = p->X; m.ldx = f.ldx = p->ldx;
+    m.C = p->C; m.ldc = p->ldc;
+    f.A = p->A; f.lda = p->lda; f.strideA = p->strideA; f.transA = p->transA ? 1 : 0;
+    l.B = p->B; l.ldb = p->ldb; l.strideB = p->strideB; l.transB = p->transB ? 1 : 0;
+  } else {
+    m.M = (int)p->K; m.K = f.K = (int)p->M;
+    m.transA = p->transW ? 0 : 1;
+    m.X = f.X = p->dC; m.ldx = f.ldx = p->lddc;
+    m.C = p->dX; m.ldc = p->K;
+    f.A = p->B; f.lda = p->ldb; f.strideA = p->strideB; f.transA = p->transB ? 0 : 1;
+    l.B = p->A; l.ldb = p->lda; l.strideB = p->strideA; l.transB = p->transA ? 0 : 1;
+  }
+  *out = a;
+  return NNLIB_B200_OK;
+}
+size_t low_bytes(const nnlib_b200_adapter_params* p) { return ((size_t)p->r * (size_t)p->N * 4 + 255) / 256 * 256; }
+
+}  // namespace
+}  // namespace nb200
+
+using namespace nb200;
+
+extern "C" {
+
+size_t nnlib_b200_route_workspace_bytes(const nnlib_b200_route_params* p) {
+  RouteArgs a;
+  if (resolve_route(p, false, &a)) return 0;
+  return route_workspace_bytes(a);
+}
+int nnlib_b200_route(const nnlib_b200_route_params* p, void* workspace, size_t workspace_bytes, void* stream) {
+  RouteArgs a;
+  int rc = resolve_route(p, false, &a);
+  if (rc) return rc;
+  const size_t need = route_workspace_bytes(a);
+  if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return NNLIB_B200_WORKSPACE_TOO_SMALL;
+  const void* all[] = {a.offsets, a.logits, a.bias, a.mask, a.weights, a.experts, a.columns, a.position};
+  if ((rc = check_arrays(all, 2, 8))) return rc;
+  a.ws = static_cast<int*>(workspace);
+  return finish(route(a, p->dtype, (cudaStream_t)stream));
+}
+int nnlib_b200_route_bwd(const nnlib_b200_route_params* p, void* stream) {
+  RouteArgs a;
+  int rc = resolve_route(p, true, &a);
+  if (rc || a.N == 0) return rc;
+  const void* all[] = {a.dlogits, a.logits, a.weights, a.experts, a.dweights};
+  if ((rc = check_arrays(all, 2, 5))) return rc;
+  return finish(route_bwd(a, p->dtype, (cudaStream_t)stream));
+}
+
+size_t nnlib_b200_grouped_gemm_workspace_bytes(const nnlib_b200_grouped_params* p) {
+  GroupedArgs a;
+  if (resolve_grouped(p, &a)) return 0;
+  return 0;
+}
+int nnlib_b200_grouped_gemm(const nnlib_b200_grouped_params* p, void* workspace, size_t workspace_bytes, void* stream) {
+  GroupedArgs a;
+  int rc = resolve_grouped(p, &a);
+  if (rc || a.M == 0 || a.R == 0) return rc;
+  if ((rc = check_grouped_arrays(a))) return rc;
+  return finish(grouped_fma(a, p->dtype, false, (cudaStream_t)stream));
+}
+size_t nnlib_b200_grouped_gemm_grad_workspace_bytes(const nnlib_b200_grouped_params* p) {
+  GroupedArgs a;
+  if (resolve_grouped(p, &a)) return 0;
+  return 0;
+}
+int nnlib_b200_grouped_gemm_grad(const nnlib_b200_grouped_params* p, void* workspace, size_t workspace_bytes, void* stream) {
+  GroupedArgs a;
+  int rc = resolve_grouped(p, &a);
+  if (rc || a.M == 0 || a.K == 0 || a.G == 0) return rc;
+  if ((rc = check_grouped_arrays(a))) return rc;
+  return finish(grouped_fma_grad(grad_of(a), p->dtype, false, false, (cudaStream_t)stream));
+}
+
+int nnlib_b200_combine(const nnlib_b200_combine_params* p, void* stream) {
+  CombineArgs a;
+  int rc = resolve_combine(p, false, &a);
+  if (rc || a.N == 0) return rc;
+  const void* all[] = {a.y, a.Y, a.position, a.weights};
+  if ((rc = check_arrays(all, 2, 4))) return rc;
+  return finish(combine(a, p->dtype, (cudaStream_t)stream));
+}
+int nnlib_b200_combine_bwd(const nnlib_b200_combine_params* p, void* stream) {
+  CombineArgs a;
+  int rc = resolve_combine(p, true, &a);
+  if (rc || (a.N == 0 && a.R == 0)) return rc;
+  const void* all[] = {a.dY, a.dy, a.Y, a.position, a.weights, a.columns, a.dweights};
+  if ((rc = check_arrays(all, 2, 7))) return rc;
+  return finish(combine_bwd(a, p->dtype, (cudaStream_t)stream));
+}
+
+size_t nnlib_b200_adapter_gemm_workspace_bytes(const nnlib_b200_adapter_params* p) {
+  Adapters a;
+  if (resolve_adapter(p, false, &a)) return 0;
+  return low_bytes(p);
+}
+int nnlib_b200_adapter_gemm(const nnlib_b200_adapter_params* p, void* workspace, size_t workspace_bytes, void* stream) {
+  Adapters a;
+  int rc = resolve_adapter(p, false, &a);
+  if (rc || a.main.M == 0 || a.main.N == 0) return rc;
+  const size_t need = low_bytes(p);
+  if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return NNLIB_B200_WORKSPACE_TOO_SMALL;
+  const void* all[] = {p->C, p->X, p->W, p->A, p->B, p->offsets, p->ids, p->scale, p->status};
+  if ((rc = check_arrays(all, 2, 9))) return rc;
+  a.first.C = workspace;
+  a.first.ldc = p->r;
+  a.main.low.T = workspace;
+  a.main.low.ldt = p->r;
+  if ((rc = finish(grouped_fma(a.first, p->dtype, true, (cudaStream_t)stream)))) return rc;
+  return finish(grouped_fma(a.main, p->dtype, false, (cudaStream_t)stream));
+}
+size_t nnlib_b200_adapter_bwd_workspace_bytes(const nnlib_b200_adapter_params* p) {
+  Adapters a;
+  if (resolve_adapter(p, true, &a)) return 0;
+  return 2 * low_bytes(p);
+}
+int nnlib_b200_adapter_bwd(const nnlib_b200_adapter_params* p, void* workspace, size_t workspace_bytes, void* stream) {
+  Adapters a;
+  int rc = resolve_adapter(p, true, &a);
+  if (rc) return rc;
+  const size_t need = 2 * low_bytes(p);
+  if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return NNLIB_B200_WORKSPACE_TOO_SMALL;
+  const void* all[] = {p->dX, p->dC, p->X, p->W, p->A, p->B, p->offsets, p->ids, p->scale, p->status, p->dA, p->dB};
+  if ((rc = check_arrays(all, 2, 12))) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  float* of_dC = static_cast<float*>(workspace);                                          // scale * B^T dC
+  float* of_X = reinterpret_cast<float*>(static_cast<char*>(workspace) + low_bytes(p));   // scale * A X
+  a.first.C = of_dC;
+  a.first.ldc = p->r;
+  a.main.low.T = of_dC;
+  a.main.low.ldt = p->r;
+  if ((rc = finish(grouped_fma(a.first, p->dtype, true, st)))) return rc;
+  if ((rc = finish(grouped_fma(a.main, p->dtype, false, st)))) return rc;
+  if (!p->dA || !p->dB) return NNLIB_B200_OK;
+  GroupedArgs f = a.first;
+  f.A = p->A; f.lda = p->lda; f.strideA = p->strideA; f.transA = p->transA ? 1 : 0;
+  f.K = (int)p->K;
+  f.X = p->X; f.ldx = p->ldx;
+  f.C = of_X;
+  if ((rc = finish(grouped_fma(f, p->dtype, true, st)))) return rc;
+  GroupedGradArgs g = grad_of(f);                       // dA = (scale B^T dC) X^T
+  g.A = p->dA; g.lda = p->transA ? p->K : p->r; g.strideA = p->r * p->K;
+  g.C = of_dC;
+  if ((rc = finish(grouped_fma_grad(g, p->dtype, true, false, st)))) return rc;
+  g.A = p->dB; g.transA = p->transB ? 1 : 0; g.lda = p->transB ? p->r : p->M; g.strideA = p->M * p->r;
+  g.M = (int)p->M; g.K = (int)p->r;
+  g.C = p->dC; g.ldc = p->lddc;                         // dB = dC (scale A X)^T
+  g.X = of_X; g.ldx = p->r;
+  return finish(grouped_fma_grad(g, p->dtype, false, true, st));
+}
+
+}  // extern "C"

@@ -174,4 +174,84 @@ bool cache_umma_parts(const CacheAttnArgs& a, int dtype, int splits);         //
 cudaError_t cache_umma(const CacheAttnArgs& a, int dtype, int splits, cudaStream_t st);   // partial results only, if splits > 1
 cudaError_t cache_umma_take_abort(int* out, cudaStream_t st);
 
+// ---- ragged groups of columns (api_experts.cu checks, experts.cu and grouped_*.cu compute) ----
+struct RouteArgs {
+  const void* logits;
+  long long stride;
+  const float* bias;
+  const unsigned char* mask;
+  float* weights;
+  int* experts;
+  int* offsets;
+  int* columns;
+  int* position;
+  const float* dweights;
+  void* dlogits;
+  int* ws;                   // counts (G, blocks), totals (G)
+  int G, N, k, normalize;
+  int blocks, per_block;     // filled in by the launcher
+};
+size_t route_workspace_bytes(const RouteArgs& a);
+cudaError_t route(RouteArgs a, int dtype, cudaStream_t st);
+cudaError_t route_bwd(const RouteArgs& a, int dtype, cudaStream_t st);
+
+struct CombineArgs {
+  const void* Y;
+  const int* position;
+  const float* weights;
+  void* y;
+  const int* columns;
+  const void* dy;
+  void* dY;
+  float* dweights;
+  long long Y_stride, y_stride, dy_stride;
+  int E, N, R, k;
+};
+cudaError_t combine(const CombineArgs& a, int dtype, cudaStream_t st);
+cudaError_t combine_bwd(const CombineArgs& a, int dtype, cudaStream_t st);
+
+// C[:, i] = scale * A[:, :, id(g)] X[:, columns[i]] for the columns i of run g, and, with `low`, what a low-rank pair adds
+struct LowRank {
+  const void* B;             // (M, r, n), or (r, M, n)
+  long long ldb, strideB;
+  const void* T;             // scale * A X: (r, N) Float32 (grouped_fma.cu), or as grouped_umma.cu lays it out
+  long long ldt;
+  const int* offsets;        // runs; NULL: of run_len columns each
+  const int* ids;
+  long long run_len;
+  int transB, r, n, runs;
+};
+struct GroupedArgs {
+  const void* A;
+  const void* X;
+  void* C;
+  long long lda, strideA, ldx, ldc;
+  const int* offsets;        // NULL: runs of run_len columns each
+  const int* ids;            // matrix of each run, outside 0 .. mats - 1: none (zeros); NULL: its own number
+  const int* columns;
+  const float* scale;        // of each matrix; NULL: scale0
+  long long run_len;
+  float scale0;
+  int transA, zero_rest;
+  int M, K, G, N, R, mats;   // G: runs, N: columns of X, R: columns of C
+  LowRank low;               // r = 0: none
+  int* status;
+};
+// Gradient of the matrices: A[:, :, a] = sum over the columns i of the runs of matrix a of C[:, i] X[:, columns[i]]^T
+struct GroupedGradArgs {
+  void* A;
+  const void* X;
+  const void* C;
+  long long lda, strideA, ldx, ldc;
+  const int* offsets;
+  const int* ids;
+  const int* columns;
+  long long run_len;
+  int transA;
+  int M, K, G, N, R, mats;
+  int* status;
+};
+cudaError_t grouped_fma(const GroupedArgs& g, int dtype, bool f32_out, cudaStream_t st);
+cudaError_t grouped_fma_grad(const GroupedGradArgs& g, int dtype, bool f32_rows, bool f32_cols, cudaStream_t st);
+
 }  // namespace nb200
