@@ -19,8 +19,6 @@ static thread_local int t_last_cuda_error = 0;
 void count_launch(int n) { g_launches.fetch_add((unsigned long long)n, std::memory_order_relaxed); }
 void set_last_cuda_error(cudaError_t e) { t_last_cuda_error = (int)e; }
 
-namespace {
-
 bool force_simt() {
   static const bool v = [] {
     const char* e = std::getenv("NNLIB_B200_FORCE_SIMT");
@@ -28,8 +26,6 @@ bool force_simt() {
   }();
   return v;
 }
-
-}  // namespace
 
 // NNLIB_B200_LOG=1: one line per call on stderr (entry point, sizes, options, kernel family and, when the
 // tensor-core kernels were not taken, why) so that a call that silently runs on the CUDA-core kernels —
@@ -656,7 +652,7 @@ int nnlib_b200_attn_path(const nnlib_b200_attn_params* p) {
 }
 
 int nnlib_b200_device_health(void* stream) {
-  int v = 0, w = 0, u = 0, t = 0, s = 0, f = 0, c = 0;
+  int v = 0, w = 0, u = 0, t = 0, s = 0, f = 0, c = 0, g = 0;
   cudaError_t e = short_take_abort(&s, (cudaStream_t)stream);
   v = 0;
   if (e == cudaSuccess) e = umma_take_abort(&v, (cudaStream_t)stream);
@@ -665,8 +661,9 @@ int nnlib_b200_device_health(void* stream) {
   if (e == cudaSuccess) e = gemm_take_abort(&u, (cudaStream_t)stream);
   if (e == cudaSuccess) e = tile_take_abort(&t, (cudaStream_t)stream);
   if (e == cudaSuccess) e = cache_umma_take_abort(&c, (cudaStream_t)stream);
+  if (e == cudaSuccess) e = grouped_take_abort(&g, (cudaStream_t)stream);
   if (e != cudaSuccess) return finish(e);
-  return (v || w || u || t || s || f || c) ? NNLIB_B200_TIMEOUT : NNLIB_B200_OK;
+  return (v || w || u || t || s || f || c || g) ? NNLIB_B200_TIMEOUT : NNLIB_B200_OK;
 }
 
 int nnlib_b200_selftest_wait_runout(uint64_t limit_ns, int32_t* status, void* stream) {

@@ -111,6 +111,14 @@ GroupedGradArgs grad_of(const GroupedArgs& a) {
   g.status = a.status;
   return g;
 }
+// Float16 / BFloat16 on the tensor cores, unless there are more runs than a block's table of them holds
+bool on_umma(const GroupedArgs& a, int dtype) { return !force_simt() && grouped_umma_supports(a, dtype); }
+bool on_umma(const GroupedGradArgs& a, int dtype) { return !force_simt() && grouped_umma_grad_supports(a, dtype); }
+int workspace_ok(const void* ws, size_t bytes, size_t need) {
+  return need && (!ws || bytes < need || !aligned(ws, 16)) ? NNLIB_B200_WORKSPACE_TOO_SMALL : NNLIB_B200_OK;
+}
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
 int check_grouped_arrays(const GroupedArgs& a) {
   const void* all[] = {a.C, a.X, a.A, a.offsets, a.columns, a.status};
   return check_arrays(all, 2, 6);
@@ -214,7 +222,56 @@ int resolve_adapter(const nnlib_b200_adapter_params* p, bool bwd, Adapters* out)
   *out = a;
   return NNLIB_B200_OK;
 }
-size_t low_bytes(const nnlib_b200_adapter_params* p) { return ((size_t)p->r * (size_t)p->N * 4 + 255) / 256 * 256; }
+// on the tensor cores both products are, or neither: T is theirs
+bool adapter_on_umma(const Adapters& a, int dtype) {
+  GroupedArgs f = a.first;
+  f.G = std::max(1, f.G);
+  f.mats = std::max(1, f.mats);
+  return on_umma(a.main, dtype) && on_umma(f, dtype);
+}
+bool has_pairs(const Adapters& a) { return a.first.G > 0 && a.first.mats > 0 && a.first.K > 0; }
+size_t low_bytes(const Adapters& a, bool umma) {
+  return round256((size_t)a.first.R * (umma ? 2 * (size_t)low_width(a.first.M) : 4 * (size_t)a.first.M));
+}
+// A X (or B^T dC) into `low`, then the product that adds B times it (A^T times it); `ws`: for both
+cudaError_t adapter_products(Adapters& a, int dtype, bool umma, void* low, void* ws, cudaStream_t st) {
+  a.first.C = low;
+  a.first.ldc = a.first.M;
+  a.main.low.T = low;
+  a.main.low.ldt = umma ? low_width(a.first.M) : a.first.M;
+  if (!has_pairs(a)) a.main.low.r = 0;
+  if (has_pairs(a)) {
+    const cudaError_t e = umma ? grouped_umma(a.first, dtype, true, ws, st) : grouped_fma(a.first, dtype, true, st);
+    if (e != cudaSuccess) return e;
+  }
+  return umma ? grouped_umma(a.main, dtype, false, ws, st) : grouped_fma(a.main, dtype, false, st);
+}
+size_t adapter_ws(const Adapters& a, bool umma) {
+  return umma ? std::max(grouped_umma_workspace_bytes(a.first), grouped_umma_workspace_bytes(a.main)) : 0;
+}
+
+// Gradients of the pairs: dA = (scale B^T dC) X^T, dB = dC (scale A X)^T.  `other`: A X for them.
+struct PairGrads {
+  GroupedArgs first;         // A X
+  GroupedGradArgs a, b;
+};
+PairGrads pair_grads(const nnlib_b200_adapter_params* p, const Adapters& a, bool umma) {
+  PairGrads o;
+  o.first = a.first;
+  o.first.A = p->A; o.first.lda = p->lda; o.first.strideA = p->strideA; o.first.transA = p->transA ? 1 : 0;
+  o.first.K = (int)p->K;
+  o.first.X = p->X; o.first.ldx = p->ldx;
+  const long long wide = umma ? low_width((int)p->r) : p->r;
+  o.a = grad_of(o.first);
+  o.a.A = p->dA; o.a.lda = p->transA ? p->K : p->r; o.a.strideA = p->r * p->K;
+  o.a.C = nullptr; o.a.ldc = wide;
+  o.b = grad_of(o.first);
+  o.b.A = p->dB; o.b.transA = p->transB ? 1 : 0; o.b.lda = p->transB ? p->r : p->M; o.b.strideA = p->M * p->r;
+  o.b.M = (int)p->M; o.b.K = (int)p->r;
+  o.b.C = p->dC; o.b.ldc = p->lddc;
+  o.b.X = nullptr; o.b.ldx = wide;
+  return o;
+}
 
 }  // namespace
 }  // namespace nb200
@@ -251,26 +308,35 @@ int nnlib_b200_route_bwd(const nnlib_b200_route_params* p, void* stream) {
 size_t nnlib_b200_grouped_gemm_workspace_bytes(const nnlib_b200_grouped_params* p) {
   GroupedArgs a;
   if (resolve_grouped(p, &a)) return 0;
-  return 0;
+  return on_umma(a, p->dtype) ? grouped_umma_workspace_bytes(a) : 0;
 }
 int nnlib_b200_grouped_gemm(const nnlib_b200_grouped_params* p, void* workspace, size_t workspace_bytes, void* stream) {
   GroupedArgs a;
   int rc = resolve_grouped(p, &a);
   if (rc || a.M == 0 || a.R == 0) return rc;
+  const bool umma = on_umma(a, p->dtype);
+  if (umma && (rc = workspace_ok(workspace, workspace_bytes, grouped_umma_workspace_bytes(a)))) return rc;
   if ((rc = check_grouped_arrays(a))) return rc;
-  return finish(grouped_fma(a, p->dtype, false, (cudaStream_t)stream));
+  if (log_calls())
+    std::fprintf(stderr, "[nnlib_b200] grouped_gemm M=%d K=%d G=%d N=%d R=%d -> %s\n", a.M, a.K, a.G, a.N, a.R, umma ? "tcgen05" : "cuda-core");
+  return finish(umma ? grouped_umma(a, p->dtype, false, workspace, (cudaStream_t)stream) : grouped_fma(a, p->dtype, false, (cudaStream_t)stream));
 }
 size_t nnlib_b200_grouped_gemm_grad_workspace_bytes(const nnlib_b200_grouped_params* p) {
   GroupedArgs a;
   if (resolve_grouped(p, &a)) return 0;
-  return 0;
+  const GroupedGradArgs g = grad_of(a);
+  return on_umma(g, p->dtype) ? grouped_umma_grad_workspace_bytes(g, 0) : 0;
 }
 int nnlib_b200_grouped_gemm_grad(const nnlib_b200_grouped_params* p, void* workspace, size_t workspace_bytes, void* stream) {
   GroupedArgs a;
   int rc = resolve_grouped(p, &a);
   if (rc || a.M == 0 || a.K == 0 || a.G == 0) return rc;
+  const GroupedGradArgs g = grad_of(a);
+  const bool umma = on_umma(g, p->dtype);
+  if (umma && (rc = workspace_ok(workspace, workspace_bytes, grouped_umma_grad_workspace_bytes(g, 0)))) return rc;
   if ((rc = check_grouped_arrays(a))) return rc;
-  return finish(grouped_fma_grad(grad_of(a), p->dtype, false, false, (cudaStream_t)stream));
+  return finish(umma ? grouped_umma_grad(g, p->dtype, 0, workspace, (cudaStream_t)stream)
+                     : grouped_fma_grad(g, p->dtype, false, false, (cudaStream_t)stream));
 }
 
 int nnlib_b200_combine(const nnlib_b200_combine_params* p, void* stream) {
@@ -293,61 +359,61 @@ int nnlib_b200_combine_bwd(const nnlib_b200_combine_params* p, void* stream) {
 size_t nnlib_b200_adapter_gemm_workspace_bytes(const nnlib_b200_adapter_params* p) {
   Adapters a;
   if (resolve_adapter(p, false, &a)) return 0;
-  return low_bytes(p);
+  const bool umma = adapter_on_umma(a, p->dtype);
+  return low_bytes(a, umma) + adapter_ws(a, umma);
 }
 int nnlib_b200_adapter_gemm(const nnlib_b200_adapter_params* p, void* workspace, size_t workspace_bytes, void* stream) {
   Adapters a;
   int rc = resolve_adapter(p, false, &a);
   if (rc || a.main.M == 0 || a.main.N == 0) return rc;
-  const size_t need = low_bytes(p);
-  if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return NNLIB_B200_WORKSPACE_TOO_SMALL;
+  const bool umma = adapter_on_umma(a, p->dtype);
+  const size_t low = low_bytes(a, umma);
+  if ((rc = workspace_ok(workspace, workspace_bytes, low + adapter_ws(a, umma)))) return rc;
   const void* all[] = {p->C, p->X, p->W, p->A, p->B, p->offsets, p->ids, p->scale, p->status};
   if ((rc = check_arrays(all, 2, 9))) return rc;
-  a.first.C = workspace;
-  a.first.ldc = p->r;
-  a.main.low.T = workspace;
-  a.main.low.ldt = p->r;
-  if ((rc = finish(grouped_fma(a.first, p->dtype, true, (cudaStream_t)stream)))) return rc;
-  return finish(grouped_fma(a.main, p->dtype, false, (cudaStream_t)stream));
+  if (log_calls())
+    std::fprintf(stderr, "[nnlib_b200] adapter_gemm M=%d K=%d N=%d r=%d runs=%d -> %s\n", a.main.M, a.main.K, a.main.N, a.first.M, a.first.G,
+                 umma ? "tcgen05" : "cuda-core");
+  return finish(adapter_products(a, p->dtype, umma, workspace, static_cast<char*>(workspace) + low, (cudaStream_t)stream));
 }
 size_t nnlib_b200_adapter_bwd_workspace_bytes(const nnlib_b200_adapter_params* p) {
   Adapters a;
   if (resolve_adapter(p, true, &a)) return 0;
-  return 2 * low_bytes(p);
+  const bool umma = adapter_on_umma(a, p->dtype);
+  size_t rest = adapter_ws(a, umma);
+  if (umma && p->dA) {
+    const PairGrads g = pair_grads(p, a, true);
+    rest = std::max({rest, grouped_umma_workspace_bytes(g.first), grouped_umma_grad_workspace_bytes(g.a, 1), grouped_umma_grad_workspace_bytes(g.b, 2)});
+  }
+  return 2 * low_bytes(a, umma) + rest;
 }
 int nnlib_b200_adapter_bwd(const nnlib_b200_adapter_params* p, void* workspace, size_t workspace_bytes, void* stream) {
   Adapters a;
   int rc = resolve_adapter(p, true, &a);
   if (rc) return rc;
-  const size_t need = 2 * low_bytes(p);
-  if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return NNLIB_B200_WORKSPACE_TOO_SMALL;
+  const bool umma = adapter_on_umma(a, p->dtype);
+  const size_t low = low_bytes(a, umma);
+  if ((rc = workspace_ok(workspace, workspace_bytes, nnlib_b200_adapter_bwd_workspace_bytes(p)))) return rc;
   const void* all[] = {p->dX, p->dC, p->X, p->W, p->A, p->B, p->offsets, p->ids, p->scale, p->status, p->dA, p->dB};
   if ((rc = check_arrays(all, 2, 12))) return rc;
   cudaStream_t st = (cudaStream_t)stream;
-  float* of_dC = static_cast<float*>(workspace);                                          // scale * B^T dC
-  float* of_X = reinterpret_cast<float*>(static_cast<char*>(workspace) + low_bytes(p));   // scale * A X
-  a.first.C = of_dC;
-  a.first.ldc = p->r;
-  a.main.low.T = of_dC;
-  a.main.low.ldt = p->r;
-  if ((rc = finish(grouped_fma(a.first, p->dtype, true, st)))) return rc;
-  if ((rc = finish(grouped_fma(a.main, p->dtype, false, st)))) return rc;
-  if (!p->dA || !p->dB) return NNLIB_B200_OK;
-  GroupedArgs f = a.first;
-  f.A = p->A; f.lda = p->lda; f.strideA = p->strideA; f.transA = p->transA ? 1 : 0;
-  f.K = (int)p->K;
-  f.X = p->X; f.ldx = p->ldx;
-  f.C = of_X;
-  if ((rc = finish(grouped_fma(f, p->dtype, true, st)))) return rc;
-  GroupedGradArgs g = grad_of(f);                       // dA = (scale B^T dC) X^T
-  g.A = p->dA; g.lda = p->transA ? p->K : p->r; g.strideA = p->r * p->K;
-  g.C = of_dC;
-  if ((rc = finish(grouped_fma_grad(g, p->dtype, true, false, st)))) return rc;
-  g.A = p->dB; g.transA = p->transB ? 1 : 0; g.lda = p->transB ? p->r : p->M; g.strideA = p->M * p->r;
-  g.M = (int)p->M; g.K = (int)p->r;
-  g.C = p->dC; g.ldc = p->lddc;                         // dB = dC (scale A X)^T
-  g.X = of_X; g.ldx = p->r;
-  return finish(grouped_fma_grad(g, p->dtype, false, true, st));
+  char* of_dC = static_cast<char*>(workspace);             // scale * B^T dC
+  char* of_X = of_dC + low;                                // scale * A X
+  char* ws = of_X + low;
+  if ((rc = finish(adapter_products(a, p->dtype, umma, of_dC, ws, st)))) return rc;
+  if (!p->dA || !p->dB || a.first.mats == 0) return NNLIB_B200_OK;
+  PairGrads g = pair_grads(p, a, umma);
+  g.first.C = of_X;
+  g.a.C = of_dC;
+  g.b.X = of_X;
+  if (!umma) {
+    if ((rc = finish(grouped_fma(g.first, p->dtype, true, st)))) return rc;
+    if ((rc = finish(grouped_fma_grad(g.a, p->dtype, true, false, st)))) return rc;
+    return finish(grouped_fma_grad(g.b, p->dtype, false, true, st));
+  }
+  if (has_pairs(a) && (rc = finish(grouped_umma(g.first, p->dtype, true, ws, st)))) return rc;
+  if ((rc = finish(grouped_umma_grad(g.a, p->dtype, 1, ws, st)))) return rc;
+  return finish(grouped_umma_grad(g.b, p->dtype, 2, ws, st));
 }
 
 }  // extern "C"

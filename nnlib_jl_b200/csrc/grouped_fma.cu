@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(256) grouped_grad_kernel(const GroupedGradArgs
   const Runs of{g.offsets, g.run_len, g.G, g.R};
   Tile<BT> t;
   t.clear();
-  for (int b = g.ids ? 0 : a; b < (g.ids ? g.G : a + 1); ++b) {
+  for (int b = g.ids ? 0 : a; b < (g.ids ? g.G : min(a + 1, g.G)); ++b) {
     if (g.ids && g.ids[b] != a) continue;
     const int lo = of.begin(b), n = of.end(b) - lo;
     contract<BT>(t, st, n, false, false,

@@ -1,0 +1,999 @@
+// Products of ragged groups of columns on the sm_100a tensor cores (Float16 / BFloat16), run sizes on the device:
+//
+//     C[:, i] = A_g X[:, columns[i]]            for the columns i of run g
+//             + B_a T[:, i]                     for low-rank pairs, T = scale * A_a X in two 16-bit terms
+//
+// The tensor core computes D[m, i] = sum_k P[m, k] Q[i, k]: rows of a matrix in the 128 lanes of tensor memory, a run's
+// columns along its columns.  That way round a tile's number of columns can be any multiple of 16 (the instruction's N is its own), so
+// that a run of 300 is two tiles of 160 and 140 and not 256 and 44, and one of 3 is padded to 16 and not to 128.
+//
+// One CTA owns an (MH*128 rows) x (at most NT columns) tile and walks over K in blocks of 64; the grid is persistent.
+//   prologue    every CTA counts the tiles of all runs (at most kMaxRuns: 4 KB of prefix sums in shared memory)
+//   warp 0      TMA producer: a ring of stages, each a K block of the matrix (K- or MN-major, as it is stored) and of the
+//               columns (K-major); gathered columns arrive four at a time (tile::gather4), their numbers in the lanes' registers
+//   warp 1      allocates tensor memory, issues every tcgen05.mma; for low-rank pairs it clears the rows of T that belong to
+//               other runs before it multiplies
+//   warps 2-9   epilogue: tensor memory -> registers -> C; two lanes exchange halves so that a store is two rows of a column
+// With MH*NT <= 256 two accumulators alternate, so that the epilogue of one tile overlaps the products of the next.
+#include <cuda.h>
+
+#include <algorithm>
+#include <cstring>
+
+#include "common.cuh"
+#include "grouped_runs.cuh"
+#include "launchers.h"
+#include "umma.cuh"
+#include "umma_shared.cuh"
+
+namespace nb200 {
+
+__device__ int g_grouped_abort = 0;  // sticky: a bounded wait of one of these kernels ran out
+
+namespace {
+
+constexpr int kThreads = 320;
+constexpr int kBK = 64;                  // K elements per stage: one 128-byte swizzle row
+constexpr int kHalfBytes = 128 * 128;    // 128 rows x 64 K elements, either layout
+constexpr int kMaxRuns = 1024;
+constexpr int kAhead = 8;                // column tiles that a band of row tiles shares
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);   // 8-row groups 1024 bytes apart, 128-byte swizzle
+
+template <int MH, int NT>
+struct Cfg {
+  static constexpr int kA = MH * kHalfBytes, kX = NT * 128, kStage = kA + kX;
+  static constexpr int kRoom = 226 * 1024 - 4 * (kMaxRuns + 8) - 512;
+  static constexpr int kStages = kRoom / kStage > 10 ? 10 : kRoom / kStage;
+  static constexpr int kAccCols = MH * NT, kAccBufs = kAccCols <= 256 ? 2 : 1;
+  static constexpr int kTmemCols = kAccCols * kAccBufs < 32 ? 32 : kAccCols * kAccBufs;
+  static constexpr int kBox = NT >= 128 ? 64 : 16;       // columns of X that one copy brings
+  static constexpr int kCumOff = kStages * kStage, kBarOff = kCumOff + 4 * (kMaxRuns + 8);
+  static constexpr int kSmem = kBarOff + 512 + 1024;
+};
+static_assert(Cfg<2, 256>::kStages == 3 && Cfg<1, 256>::kStages == 4 && Cfg<1, 32>::kStages == 10, "ring depth");
+static_assert(Cfg<2, 256>::kSmem <= 232448 && Cfg<1, 256>::kSmem <= 232448 && Cfg<1, 128>::kSmem <= 232448 && Cfg<1, 64>::kSmem <= 232448 &&
+              Cfg<1, 32>::kSmem <= 232448, "shared memory budget");
+
+struct Bars {
+  uint64_t full[10], empty[10], acc_full[2], acc_empty[2];
+  unsigned long long there[10];          // gradient: which of a stage's 64 columns take part
+  uint32_t tmem_base;
+  int abort_flag;
+  RunSearch search;
+};
+static_assert(sizeof(Bars) <= 512, "barrier block");
+
+enum { kToC, kToParts, kToLow };         // what the epilogue writes
+
+struct FwdArgs {
+  Runs runs;
+  const int* ids;
+  const int* columns;
+  void* C;                               // kToParts: Float32 (M, R, splits); kToLow: T, 16-bit
+  long long ldc;
+  const float* scale;
+  float scale0;
+  int M, K, G, N, mats;
+  int a_kmaj, a_same, zero_rest, splits, tiles_m, to, pairs;
+  int low_width, low_step;               // kToLow: elements of T for a column, from the first term to the second
+  Runs low_runs;                         // kToC: low-rank pairs, r = 0: none
+  const int* low_ids;
+  int r, n, low_kmaj;
+  int* status;
+};
+
+// four rows of a 2-d tensor map, 64 elements each
+__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, int4 r) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+               "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr) { return ((addr & 0x3FFFFu) >> 4) | ((uint32_t)((kHalfBytes / 2) >> 4) << 16); }
+__device__ __forceinline__ uint32_t idesc_of(bool bf16, int n, bool a_mn, bool b_mn) {
+  return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
+         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+__device__ __forceinline__ int round16(int n) { return (n + 15) & ~15; }
+
+// tiles of a run of n columns, and their width: as even as multiples of 16 allow
+template <int NT>
+__device__ __forceinline__ int tile_width(int n) {
+  const int c = (n + NT - 1) / NT;
+  return c > 0 ? round16((n + c - 1) / c) : 16;
+}
+template <int NT>
+__device__ __forceinline__ int tile_count(int n) {
+  const int w = tile_width<NT>(n);
+  return (n + w - 1) / w;
+}
+
+// cum[i]: column tiles of the runs before run i (runs of one length need no table).  By the whole block.
+template <int NT>
+__device__ void count_tiles(const FwdArgs& g, int* cum, RunSearch& s) {
+  if (!g.runs.offsets) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int carry = 0;
+  for (int i0 = 0; i0 < g.G; i0 += kThreads) {
+    const int i = i0 + (int)threadIdx.x;
+    int own = 0;
+    if (i < g.G) {
+      const int mat = g.ids ? g.ids[i] : i;
+      if (mat >= 0 && mat < g.mats) own = tile_count<NT>(g.runs.end(i) - g.runs.begin(i));
+    }
+    int sum = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += u;
+    }
+    if (lane == 31) s.part[warp] = sum;
+    __syncthreads();
+    int before = carry, all = carry;
+    for (int q = 0; q < kThreads / 32; ++q) {
+      if (q < warp) before += s.part[q];
+      all += s.part[q];
+    }
+    if (i < g.G) cum[i] = before + sum - own;
+    carry = all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) cum[g.G] = carry;
+  __syncthreads();
+}
+
+struct Tile {
+  int run, mat, n0, nt, m0, kb0, kb1, split;
+};
+// Tile number t of this CTA's growing sequence; `run` is where the last one was.
+template <int MH, int NT>
+__device__ __forceinline__ Tile tile_of(const FwdArgs& g, const int* cum, long long t, int nkb, int& run) {
+  Tile o;
+  o.split = (int)(t % g.splits);
+  const long long q = t / g.splits;
+  int tiles;
+  long long at;
+  if (g.runs.offsets) {
+    while ((long long)cum[run + 1] * g.tiles_m <= q) ++run;
+    tiles = cum[run + 1] - cum[run];
+    at = q - (long long)cum[run] * g.tiles_m;
+  } else {
+    tiles = tile_count<NT>((int)g.runs.len);
+    run = (int)(q / ((long long)tiles * g.tiles_m));
+    at = q - (long long)run * tiles * g.tiles_m;
+  }
+  // bands of kAhead column tiles: what runs at the same time shares the matrix's rows and the columns
+  const int band = (int)(at / (kAhead * g.tiles_m)), in = (int)(at - (long long)band * kAhead * g.tiles_m), wide = min(kAhead, tiles - band * kAhead);
+  const int begin = g.runs.begin(run), end = g.runs.end(run), w = tile_width<NT>(end - begin);
+  o.run = run;
+  o.mat = g.ids ? g.ids[run] : run;
+  o.m0 = (in / wide) * (MH * 128);
+  o.n0 = begin + (band * kAhead + in % wide) * w;
+  o.nt = o.mat >= 0 && o.mat < g.mats ? min(w, end - o.n0) : 0;      // (0: nothing to do)
+  o.kb0 = (int)((long long)nkb * o.split / g.splits);
+  o.kb1 = (int)((long long)nkb * (o.split + 1) / g.splits);
+  return o;
+}
+
+// Runs of low-rank pairs that have columns in a tile, neighbours of the same pair as one.
+struct Pairs {
+  int b, end, id, lo, hi;
+  __device__ __forceinline__ Pairs(const FwdArgs& g, int n0, int nt) : end(n0 + nt) {
+    int a = 0, c = g.low_runs.runs;                        // the first run that ends behind n0
+    while (a < c) {
+      const int mid = (a + c) >> 1;
+      if (g.low_runs.end(mid) > n0) c = mid; else a = mid + 1;
+    }
+    b = a;
+  }
+  __device__ __forceinline__ bool next(const FwdArgs& g, int n0) {
+    for (; b < g.low_runs.runs; ++b) {
+      lo = max(g.low_runs.begin(b), n0);
+      if (lo >= end) return false;
+      hi = min(g.low_runs.end(b), end);
+      id = g.low_ids[b];
+      if (lo >= hi || id < 0 || id >= g.n) continue;
+      for (++b; b < g.low_runs.runs && hi < end && g.low_ids[b] == id && g.low_runs.begin(b) == hi; ++b) hi = max(hi, min(g.low_runs.end(b), end));
+      return true;
+    }
+    return false;
+  }
+};
+// K blocks that a pair adds: rank up to 32: both terms of T in one; above: the first terms' blocks, then the second ones'
+__device__ __forceinline__ int low_blocks(int r) { return r <= 32 ? 1 : 2 * ((r + 63) / 64); }
+
+template <bool BF16, int MH, int NT>
+__global__ void __launch_bounds__(kThreads, 1)
+grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_b,
+                    const __grid_constant__ CUtensorMap tm_t, const __grid_constant__ FwdArgs g) {
+  using C = Cfg<MH, NT>;
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  int* cum = reinterpret_cast<int*>(smem + C::kCumOff);
+  Bars* bars = reinterpret_cast<Bars*>(smem + C::kBarOff);
+  volatile int* abort_flag = &bars->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int nkb = (g.K + kBK - 1) / kBK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars->acc_full[s], 1);
+      mbar_init(&bars->acc_empty[s], 8);
+    }
+    bars->abort_flag = *reinterpret_cast<volatile int*>(&g_grouped_abort);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&bars->tmem_base, C::kTmemCols);
+    tmem_relinquish();
+  }
+  count_tiles<NT>(g, cum, bars->search);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  const bool start_ok = (*abort_flag == 0);
+  const long long columns = g.runs.offsets ? cum[g.G] : (long long)g.G * tile_count<NT>((int)g.runs.len);
+  const long long tiles = columns * g.tiles_m * g.splits;
+
+  if (start_ok && warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      prefetch_tensormap(&tm_a);
+      prefetch_tensormap(&tm_x);
+    }
+    bool ok = true;
+    long long it = 0;
+    int run = 0;
+    // one stage: the boxes of the matrix (map ma, block ka of matrix za) and of the columns (map mx, block kx), a lane each
+    auto fill = [&](const CUtensorMap* ma, int ka, int za, bool kmaj, const CUtensorMap* mx, int kx, const Tile& o, bool gather, const int4 (&at)[2]) {
+      const int s = (int)(it % C::kStages);
+      int good = 1;
+      if (it >= C::kStages && lane == 0) good = mbar_wait(&bars->empty[s], (uint32_t)((it / C::kStages) - 1) & 1u, abort_flag) ? 1 : 0;
+      if (!__shfl_sync(0xffffffffu, good, 0)) return false;
+      uint8_t* da = smem + s * C::kStage;
+      uint8_t* dx = da + C::kA;
+      const int boxes = gather ? 0 : (o.nt + C::kBox - 1) / C::kBox;
+      if (lane == 0) mbar_arrive_expect_tx(&bars->full[s], C::kA + (gather ? round16(o.nt) * 128 : boxes * C::kBox * 128));
+      __syncwarp();
+      const int na = kmaj ? MH : 2 * MH;
+      if (lane < na) {
+        if (kmaj) tma_load_3d(da + lane * kHalfBytes, ma, &bars->full[s], ka, o.m0 + lane * 128, za);
+        else tma_load_3d(da + lane * (kHalfBytes / 2), ma, &bars->full[s], o.m0 + lane * 64, ka, za);
+      } else if (lane - na < boxes) {
+        const int i = lane - na;
+        tma_load_2d(dx + i * C::kBox * 128, mx, &bars->full[s], kx, o.n0 + i * C::kBox);
+      }
+      if (gather) {
+#pragma unroll
+        for (int i = 0; i < (NT > 128 ? 2 : 1); ++i) {
+          const int q = lane + 32 * i;
+          if (q * 4 < round16(o.nt)) tma_gather4(dx + q * 512, mx, &bars->full[s], kx, at[i]);
+        }
+      }
+      ++it;
+      return true;
+    };
+    for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const Tile o = tile_of<MH, NT>(g, cum, t, nkb, run);
+      if (o.nt <= 0) continue;
+      int4 at[2] = {};
+      if (g.columns) {
+#pragma unroll
+        for (int i = 0; i < (NT > 128 ? 2 : 1); ++i) {
+          int c[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int n = (lane + 32 * i) * 4 + e;
+            c[e] = n < o.nt ? g.columns[o.n0 + n] : 0;
+            if ((unsigned)c[e] >= (unsigned)g.N) c[e] = 0;     // (its column of C becomes zeros)
+          }
+          at[i] = make_int4(c[0], c[1], c[2], c[3]);
+        }
+      }
+      for (int kb = o.kb0; kb < o.kb1 && ok; ++kb)
+        ok = fill(&tm_a, kb * kBK, g.a_same ? 0 : o.mat, g.a_kmaj != 0, &tm_x, kb * kBK, o, g.columns != nullptr, at);
+      if (g.r > 0 && ok) {
+        Pairs p(g, o.n0, o.nt);
+        const int blocks = low_blocks(g.r), half = blocks / 2;
+        while (ok && p.next(g, o.n0))
+          for (int q = 0; q < blocks && ok; ++q) ok = fill(&tm_b, (half ? q % half : 0) * kBK, p.id, g.low_kmaj != 0, &tm_t, q * kBK, o, false, at);
+      }
+    }
+    if (lane == 0 && *abort_flag) {
+      // give copies still in flight a bounded chance to land before the CTA leaves
+      for (long long jj = (it > C::kStages ? it - C::kStages : 0); jj < it; ++jj)
+        mbar_wait_drain(&bars->full[jj % C::kStages], (uint32_t)(jj / C::kStages) & 1u, kDrainNs);
+    }
+  } else if (start_ok && warp == 1) {
+    // -------------------------------------------------------------- MMA issuer
+    bool ok = true;
+    long long it = 0;
+    int ti = 0, run = 0;
+    for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const Tile o = tile_of<MH, NT>(g, cum, t, nkb, run);
+      if (o.nt <= 0) continue;
+      const int ab = ti % C::kAccBufs;
+      const uint32_t acc = tmem + ab * C::kAccCols;
+      const uint32_t id_main = idesc_of(BF16, round16(o.nt), !g.a_kmaj, false);
+      int good = 1;
+      if (lane == 0) {
+        if (ti >= C::kAccBufs) good = mbar_wait(&bars->acc_empty[ab], (uint32_t)((ti / C::kAccBufs) - 1) & 1u, abort_flag) ? 1 : 0;
+        tc_fence_after();
+        const uint32_t step = g.a_kmaj ? 32 >> 4 : 2048 >> 4;
+        for (int kb = o.kb0; kb < o.kb1 && good; ++kb) {
+          const long long i = it + (kb - o.kb0);
+          const int s = (int)(i % C::kStages);
+          if (!mbar_wait(&bars->full[s], (uint32_t)(i / C::kStages) & 1u, abort_flag)) { good = 0; break; }
+          tc_fence_after();
+          const uint32_t a = desc_lo(smem_u32(smem + s * C::kStage)), x = desc_lo(smem_u32(smem + s * C::kStage + C::kA));
+          const int steps = min(4, (g.K - kb * kBK + 15) >> 4);
+          for (int kk = 0; kk < steps; ++kk) {
+#pragma unroll
+            for (int h = 0; h < MH; ++h)
+              umma_ss_lohi(acc + h * NT, a + h * (kHalfBytes >> 4) + kk * step, x + kk * 2, kDescHi, id_main, (kb > o.kb0 || kk > 0) ? 1u : 0u);
+          }
+          umma_commit(&bars->empty[s]);
+        }
+      }
+      it += o.kb1 - o.kb0;
+      ok = __shfl_sync(0xffffffffu, good, 0) != 0;
+      if (g.r > 0 && ok) {
+        Pairs p(g, o.n0, o.nt);
+        const int blocks = low_blocks(g.r), half = blocks / 2;
+        const uint32_t id_low = idesc_of(BF16, round16(o.nt), !g.low_kmaj, false), step = g.low_kmaj ? 32 >> 4 : 2048 >> 4;
+        while (ok && p.next(g, o.n0)) {
+          const int lo = p.lo - o.n0, hi = p.hi - o.n0, all = round16(o.nt);
+          for (int q = 0; q < blocks; ++q, ++it) {
+            const int s = (int)(it % C::kStages);
+            ok = mbar_wait_warp(&bars->full[s], (uint32_t)(it / C::kStages) & 1u, abort_flag);
+            if (!ok) break;
+            __syncwarp();
+            uint8_t* tx = smem + s * C::kStage + C::kA;
+            if (lo > 0 || hi < all) {                      // columns of other runs take no part
+              for (int i = lane; i < all * 8; i += 32)
+                if ((i >> 3) < lo || (i >> 3) >= hi) *reinterpret_cast<uint4*>(tx + i * 16) = make_uint4(0, 0, 0, 0);
+              fence_proxy_async_smem();
+              __syncwarp();
+            }
+            if (lane == 0) {
+              tc_fence_after();
+              const uint32_t a = desc_lo(smem_u32(smem + s * C::kStage)), x = desc_lo(smem_u32(tx));
+              const int left = half ? g.r - (q % half) * kBK : g.r, steps = min(4, (left + 15) >> 4);
+              for (int kk = 0; kk < steps; ++kk) {
+#pragma unroll
+                for (int h = 0; h < MH; ++h) {
+                  umma_ss_lohi(acc + h * NT, a + h * (kHalfBytes >> 4) + kk * step, x + kk * 2, kDescHi, id_low, 1u);
+                  if (!half) umma_ss_lohi(acc + h * NT, a + h * (kHalfBytes >> 4) + kk * step, x + kk * 2 + 4, kDescHi, id_low, 1u);
+                }
+              }
+              umma_commit(&bars->empty[s]);
+            }
+            __syncwarp();
+          }
+        }
+      }
+      if (ok && lane == 0) umma_commit(&bars->acc_full[ab]);
+      ++ti;
+    }
+  } else if (start_ok && warp >= 2) {
+    // ----------------------------------------------------------------- epilogue
+    const int wq = warp & 3, part = (warp - 2) >> 2;       // TMEM lane quarter; MH = 2: half of the rows, 1: every other 32 columns
+    constexpr int kStep = MH == 2 ? 1 : 2;
+    bool ok = true;
+    int ti = 0, run = 0;
+    for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const Tile o = tile_of<MH, NT>(g, cum, t, nkb, run);
+      if (o.nt <= 0) continue;
+      const int ab = ti % C::kAccBufs;
+      ok = mbar_wait_warp(&bars->acc_full[ab], (uint32_t)(ti / C::kAccBufs) & 1u, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      const int m = o.m0 + (MH == 2 ? part * 128 : 0) + wq * 32 + lane;
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(wq * 32) << 16) + ab * C::kAccCols + (MH == 2 ? part * NT : 0);
+      const int chunks = (o.nt + 31) / 32;
+      float scale = 1.f;
+      if (g.to == kToLow) scale = g.scale ? g.scale[o.mat] : g.scale0;
+      for (int c = MH == 2 ? 0 : part; c < chunks; c += kStep) {
+        uint32_t acc[32];
+        tmem_ld32(taddr + c * 32, acc);
+        tmem_wait_ld();
+        if (c + kStep >= chunks) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->acc_empty[ab]);
+        }
+        const int nc = min(32, o.nt - c * 32), n = o.n0 + c * 32;
+        if (g.to == kToC) {
+          uint32_t valid = 0xffffffffu;
+          if (g.columns) valid = __ballot_sync(0xffffffffu, lane < nc && (unsigned)g.columns[n + min(lane, nc - 1)] < (unsigned)g.N);
+          T* out = reinterpret_cast<T*>(g.C) + (long long)n * g.ldc;
+          if (g.pairs) {
+            const int mp = m & ~1;
+            const bool odd = lane & 1;
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              const uint32_t mine = pack2<BF16>(__uint_as_float(acc[j]), __uint_as_float(acc[j + 1]));
+              const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
+              // even lane: column j of rows m, m + 1; odd lane: column j + 1 of rows m - 1, m
+              uint32_t v = odd ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
+              const int col = j + (odd ? 1 : 0);
+              if (col < nc && mp < g.M) {
+                if (!((valid >> col) & 1u)) v = 0u;
+                T* dst = out + (long long)col * g.ldc + mp;
+                if (mp + 1 < g.M) *reinterpret_cast<uint32_t*>(dst) = v;
+                else *reinterpret_cast<unsigned short*>(dst) = (unsigned short)v;
+              }
+            }
+          } else if (m < g.M) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < nc) out[(long long)j * g.ldc + m] = Elem<T>::from_f(((valid >> j) & 1u) ? __uint_as_float(acc[j]) : 0.f);
+          }
+        } else if (g.to == kToParts) {
+          float* out = reinterpret_cast<float*>(g.C) + ((long long)o.split * g.runs.R + n) * g.M + m;
+          if (m < g.M) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < nc) out[(long long)j * g.M] = __uint_as_float(acc[j]);
+          }
+        } else if (m < g.low_step) {
+          // T: what is left after rounding to 16 bits is the second term; zeros behind the rank
+          T* out = reinterpret_cast<T*>(g.C) + (long long)n * g.low_width + m;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float v = m < g.M ? scale * __uint_as_float(acc[j]) : 0.f;
+            const T first = Elem<T>::from_f(v);
+            if (j < nc) {
+              out[(long long)j * g.low_width] = first;
+              out[(long long)j * g.low_width + g.low_step] = Elem<T>::from_f(v - Elem<T>::to_f(first));
+            }
+          }
+        }
+      }
+      if (MH == 1 && part >= chunks) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->acc_empty[ab]);
+      }
+      ++ti;
+    }
+    if (g.zero_rest && ok) {
+      // columns in no run
+      const int first = g.G > 0 ? g.runs.at(0) : g.runs.R, last = g.G > 0 ? g.runs.at(g.G) : g.runs.R;
+      const int rest = first + g.runs.R - last;
+      for (int i = blockIdx.x * 8 + warp - 2; i < rest; i += gridDim.x * 8) {
+        T* out = reinterpret_cast<T*>(g.C) + (long long)(i < first ? i : last + i - first) * g.ldc;
+        for (int m = lane; m < g.M; m += 32) out[m] = Elem<T>::from_f(0.f);
+      }
+    }
+  }
+
+  // ---------------------------------------------------------------- teardown
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kTmemCols);
+  }
+  if (threadIdx.x == 0 && *abort_flag) {
+    atomicExch(&g_grouped_abort, 1);
+    if (g.status) atomicExch(g.status, NNLIB_B200_TIMEOUT);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------- gradient
+//     A_a[row, col] = sum over the columns i of the runs of matrix a of P[row, i] Q[col, i]
+// rows and columns of the matrix being features of dC and X, or of X and dC: the one that is stored contiguously is the rows'.  Both
+// operands are MN-major, the contraction runs over a run's columns in blocks of 64; what a block holds behind the run's end, or of a
+// column that is none, is cleared in shared memory before it is multiplied (another run's infinity times zero would be a NaN).
+struct GradArgs {
+  Runs runs;
+  const int* ids;
+  const int* columns;
+  void* A;
+  long long ld, stride;                  // between columns and matrices of the result
+  int rows, cols, G, N, mats;
+  int gather;                            // 1: the rows' operand is gathered, 2: the columns' is
+  int tiles_r, tiles_c, pairs;
+  int fold, fold_step, along;            // fold: columns fold_step apart are the two terms of one; along: a row's columns are contiguous
+  int* status;
+};
+
+template <bool BF16, int MH, int NT>
+__global__ void __launch_bounds__(kThreads, 1)
+grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_constant__ CUtensorMap tm_c, const __grid_constant__ GradArgs g) {
+  using C = Cfg<MH, NT>;
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  Bars* bars = reinterpret_cast<Bars*>(smem + C::kBarOff);
+  volatile int* abort_flag = &bars->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars->acc_full[s], 1);
+      mbar_init(&bars->acc_empty[s], 8);
+    }
+    bars->abort_flag = *reinterpret_cast<volatile int*>(&g_grouped_abort);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&bars->tmem_base, C::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  const bool start_ok = (*abort_flag == 0);
+  const long long each = (long long)g.tiles_r * g.tiles_c, tiles = each * g.mats;
+  // blocks of a tile, run by run: begin(b), end(b) of the runs b of matrix a
+  auto first_run = [&](int a) { return g.ids ? 0 : a; };
+  auto last_run = [&](int a) { return g.ids ? g.G : min(a + 1, g.G); };
+
+  if (start_ok && warp == 0) {
+    bool ok = true;
+    long long it = 0;
+    if (lane == 0) {
+      prefetch_tensormap(&tm_r);
+      prefetch_tensormap(&tm_c);
+    }
+    constexpr int kBoxesR = 2 * MH, kBoxesC = NT / 64;
+    for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const int a = (int)(t / each), q = (int)(t % each);
+      const int r0 = (q % g.tiles_r) * (MH * 128), c0 = (q / g.tiles_r) * NT;
+      for (int b = first_run(a); b < last_run(a) && ok; ++b) {
+        if (g.ids && g.ids[b] != a) continue;
+        const int end = g.runs.end(b);
+        for (int i0 = g.runs.begin(b); i0 < end && ok; i0 += kBK, ++it) {
+          const int s = (int)(it % C::kStages);
+          int4 at = make_int4(0, 0, 0, 0);
+          unsigned long long there = end - i0 >= 64 ? ~0ull : (1ull << (end - i0)) - 1;
+          if (g.gather) {
+            int c[4];
+            unsigned have = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int i = i0 + (lane & 15) * 4 + e;
+              c[e] = i < end ? g.columns[i] : -1;
+              if ((unsigned)c[e] < (unsigned)g.N) have |= 1u << e; else c[e] = 0;
+            }
+            at = make_int4(c[0], c[1], c[2], c[3]);
+            unsigned lo = have << ((lane & 7) * 4);
+#pragma unroll
+            for (int x = 1; x < 8; x <<= 1) lo |= __shfl_xor_sync(0xffffffffu, lo, x);
+            there = (unsigned long long)__shfl_sync(0xffffffffu, lo, 0) | (unsigned long long)__shfl_sync(0xffffffffu, lo, 8) << 32;
+          }
+          int good = 1;
+          if (it >= C::kStages && lane == 0) good = mbar_wait(&bars->empty[s], (uint32_t)((it / C::kStages) - 1) & 1u, abort_flag) ? 1 : 0;
+          ok = __shfl_sync(0xffffffffu, good, 0) != 0;
+          if (!ok) break;
+          uint8_t* dr = smem + s * C::kStage;
+          uint8_t* dc = dr + C::kA;
+          if (lane == 0) {
+            bars->there[s] = there;
+            mbar_arrive_expect_tx(&bars->full[s], C::kStage);
+          }
+          __syncwarp();
+          if (g.gather == 1) {
+            for (int x = lane >> 4; x < kBoxesR; x += 2) tma_gather4(dr + x * (kHalfBytes / 2) + (lane & 15) * 512, &tm_r, &bars->full[s], r0 + x * 64, at);
+          } else if (lane < kBoxesR) {
+            tma_load_2d(dr + lane * (kHalfBytes / 2), &tm_r, &bars->full[s], r0 + lane * 64, i0);
+          }
+          if (g.gather == 2) {
+            for (int x = lane >> 4; x < kBoxesC; x += 2) tma_gather4(dc + x * (kHalfBytes / 2) + (lane & 15) * 512, &tm_c, &bars->full[s], c0 + x * 64, at);
+          } else if (lane >= 8 && lane - 8 < kBoxesC) {
+            tma_load_2d(dc + (lane - 8) * (kHalfBytes / 2), &tm_c, &bars->full[s], c0 + (lane - 8) * 64, i0);
+          }
+        }
+      }
+    }
+    if (lane == 0 && *abort_flag) {
+      for (long long jj = (it > C::kStages ? it - C::kStages : 0); jj < it; ++jj)
+        mbar_wait_drain(&bars->full[jj % C::kStages], (uint32_t)(jj / C::kStages) & 1u, kDrainNs);
+    }
+  } else if (start_ok && warp == 1) {
+    bool ok = true;
+    long long it = 0;
+    int ti = 0;
+    for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++ti) {
+      const int a = (int)(t / each), left = g.cols - (int)((t % each) / g.tiles_r) * NT;
+      const int ab = ti % C::kAccBufs;
+      const uint32_t acc = tmem + ab * C::kAccCols;
+      const uint32_t idesc = idesc_of(BF16, g.fold || left > NT ? NT : round16(left), true, true);
+      if (ti >= C::kAccBufs) {
+        ok = mbar_wait_warp(&bars->acc_empty[ab], (uint32_t)((ti / C::kAccBufs) - 1) & 1u, abort_flag);
+        if (!ok) break;
+      }
+      tc_fence_after();
+      bool begun = false;
+      for (int b = first_run(a); b < last_run(a) && ok; ++b) {
+        if (g.ids && g.ids[b] != a) continue;
+        const int end = g.runs.end(b);
+        for (int i0 = g.runs.begin(b); i0 < end; i0 += kBK, ++it) {
+          const int s = (int)(it % C::kStages);
+          ok = mbar_wait_warp(&bars->full[s], (uint32_t)(it / C::kStages) & 1u, abort_flag);
+          if (!ok) break;
+          __syncwarp();
+          const int steps = min(4, (end - i0 + 15) >> 4);
+          const unsigned long long missing = ~*reinterpret_cast<volatile unsigned long long*>(&bars->there[s]) & (steps == 4 ? ~0ull : (1ull << (steps * 16)) - 1);
+          if (missing) {
+            for (int i = lane; i < steps * 16 * 8; i += 32) {
+              if (!((missing >> (i >> 3)) & 1ull)) continue;
+#pragma unroll
+              for (int x = 0; x < C::kStage / (kHalfBytes / 2); ++x)
+                *reinterpret_cast<uint4*>(smem + s * C::kStage + x * (kHalfBytes / 2) + i * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          if (lane == 0) {
+            tc_fence_after();
+            const uint32_t r = desc_lo(smem_u32(smem + s * C::kStage)), c = desc_lo(smem_u32(smem + s * C::kStage + C::kA));
+            for (int kk = 0; kk < steps; ++kk) {
+#pragma unroll
+              for (int h = 0; h < MH; ++h)
+                umma_ss_lohi(acc + h * NT, r + h * (kHalfBytes >> 4) + kk * (2048 >> 4), c + kk * (2048 >> 4), kDescHi, idesc, (begun || kk > 0) ? 1u : 0u);
+            }
+            umma_commit(&bars->empty[s]);
+          }
+          begun = true;
+          __syncwarp();
+        }
+      }
+      if (ok && lane == 0) umma_commit(&bars->acc_full[ab]);
+    }
+  } else if (start_ok && warp >= 2) {
+    const int wq = warp & 3, part = (warp - 2) >> 2;
+    constexpr int kStep = MH == 2 ? 1 : 2;
+    bool ok = true;
+    int ti = 0;
+    for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++ti) {
+      const int a = (int)(t / each), q = (int)(t % each);
+      const int r0 = (q % g.tiles_r) * (MH * 128), c0 = (q / g.tiles_r) * NT;
+      const int ab = ti % C::kAccBufs;
+      bool some = false;                                   // a matrix that no column met is zeros
+      for (int b = first_run(a); b < last_run(a) && !some; ++b) some = (!g.ids || g.ids[b] == a) && g.runs.end(b) > g.runs.begin(b);
+      ok = mbar_wait_warp(&bars->acc_full[ab], (uint32_t)(ti / C::kAccBufs) & 1u, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      const int m = r0 + (MH == 2 ? part * 128 : 0) + wq * 32 + lane;
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(wq * 32) << 16) + ab * C::kAccCols + (MH == 2 ? part * NT : 0);
+      T* base = reinterpret_cast<T*>(g.A) + (long long)a * g.stride;
+      const int width = g.fold ? g.fold_step : NT, chunks = width / 32;
+      for (int c = MH == 2 ? 0 : part; c < chunks; c += kStep) {
+        uint32_t acc[32];
+        tmem_ld32(taddr + c * 32, acc);
+        if (g.fold) {
+          uint32_t more[32];
+          tmem_ld32(taddr + g.fold_step + c * 32, more);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[j] = __float_as_uint(__uint_as_float(acc[j]) + __uint_as_float(more[j]));
+        }
+        tmem_wait_ld();
+        if (c + kStep >= chunks) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->acc_empty[ab]);
+        }
+        if (!some) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[j] = 0u;
+        }
+        const int n = c0 + c * 32, nc = min(32, g.cols - n);
+        if (g.along) {
+          if (m < g.rows) {
+            T* out = base + (long long)m * g.ld + n;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < nc) out[j] = Elem<T>::from_f(__uint_as_float(acc[j]));
+          }
+          continue;
+        }
+        T* out = base + (long long)n * g.ld;
+        if (g.pairs) {
+          const int mp = m & ~1;
+          const bool odd = lane & 1;
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const uint32_t mine = pack2<BF16>(__uint_as_float(acc[j]), __uint_as_float(acc[j + 1]));
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
+            const uint32_t v = odd ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
+            const int col = j + (odd ? 1 : 0);
+            if (col < nc && mp < g.rows) {
+              T* dst = out + (long long)col * g.ld + mp;
+              if (mp + 1 < g.rows) *reinterpret_cast<uint32_t*>(dst) = v;
+              else *reinterpret_cast<unsigned short*>(dst) = (unsigned short)v;
+            }
+          }
+        } else if (m < g.rows) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (j < nc) out[(long long)j * g.ld + m] = Elem<T>::from_f(__uint_as_float(acc[j]));
+        }
+      }
+      if (MH == 1 && part >= chunks) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->acc_empty[ab]);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kTmemCols);
+  }
+  if (threadIdx.x == 0 && *abort_flag) {
+    atomicExch(&g_grouped_abort, 1);
+    if (g.status) atomicExch(g.status, NNLIB_B200_TIMEOUT);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------- copies, host
+// `count` matrices of wide x deep 16-bit elements to rows that the copy engine can address; with `offsets`, only those of runs
+// that have columns.
+__global__ void __launch_bounds__(256) aligned_copy_kernel(const unsigned short* src, long long ld, long long stride, uint4* dst, int wide, long long deep,
+                                                           int ld8, Runs of) {
+  const int mat = blockIdx.z;
+  if (of.offsets && of.end(mat) <= of.begin(mat)) return;
+  const unsigned short* s = src + (long long)mat * stride;
+  uint4* d = dst + (long long)mat * deep * ld8;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < deep * ld8; i += (long long)gridDim.x * 256) {
+    const long long row = i / ld8;
+    const int c = (int)(i % ld8) * 8;
+    const unsigned short* p = s + row * ld + c;
+    unsigned short v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c + e < wide ? p[e] : (unsigned short)0;
+    d[i] = make_uint4(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16, v[4] | (uint32_t)v[5] << 16, v[6] | (uint32_t)v[7] << 16);
+  }
+}
+
+// A matrix (or several) that is read: where it lies, contiguous extent first.
+struct Operand {
+  const void* p;
+  long long wide, deep, ld, stride, count;
+  bool fits() const { return aligned16(p) && stride_ok(ld) && (count <= 1 || stride == 0 || stride_ok(stride)); }
+  size_t copy_bytes() const { return fits() || wide == 0 || deep == 0 || count == 0 ? 0 : (size_t)((wide + 7) / 8 * 16) * deep * count; }
+};
+cudaError_t align_operand(Operand& o, char*& ws, const Runs* of, cudaStream_t st) {
+  const size_t bytes = o.copy_bytes();
+  if (!bytes) return cudaSuccess;
+  const int ld8 = (int)((o.wide + 7) / 8);
+  const long long blocks = std::min<long long>((o.deep * ld8 + 255) / 256, 65535);
+  aligned_copy_kernel<<<dim3((unsigned)blocks, 1, (unsigned)o.count), 256, 0, st>>>(static_cast<const unsigned short*>(o.p), o.ld, o.stride,
+                                                                                    reinterpret_cast<uint4*>(ws), (int)o.wide, o.deep, ld8,
+                                                                                    of ? *of : Runs{nullptr, 0, 0, 0});
+  count_launch();
+  o.p = ws;
+  o.ld = (long long)ld8 * 8;
+  o.stride = o.ld * o.deep;
+  ws += (bytes + 255) / 256 * 256;
+  return cudaGetLastError();
+}
+size_t padded(size_t n) { return (n + 255) / 256 * 256; }
+
+bool encode(CUtensorMap* m, int dtype, int rank, const Operand& o, const cuuint32_t* box) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return false;
+  const long long stride = o.count > 1 && o.stride ? o.stride : o.ld * o.deep;
+  const cuuint64_t dims[3] = {(cuuint64_t)o.wide, (cuuint64_t)o.deep, (cuuint64_t)(o.stride ? o.count : 1)};
+  const cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)stride * 2};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return fn(m, dtype == NNLIB_B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(o.p), dims, strides,
+            box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+bool encode_matrix(CUtensorMap* m, int dtype, const Operand& o, bool kmaj) {
+  const cuuint32_t box[3] = {64, kmaj ? 128u : 64u, 1};
+  return encode(m, dtype, 3, o, box);
+}
+bool encode_columns(CUtensorMap* m, int dtype, const Operand& o, int rows) {
+  const cuuint32_t box[2] = {64, (cuuint32_t)rows};
+  return encode(m, dtype, 2, o, box);
+}
+
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) n = 148;
+  return n;
+}
+
+template <bool BF16, int MH, int NT>
+cudaError_t launch_fwd(const CUtensorMap& a, const CUtensorMap& x, const CUtensorMap& b, const CUtensorMap& t, FwdArgs g, long long most, cudaStream_t st) {
+  using C = Cfg<MH, NT>;
+  auto kern = grouped_umma_kernel<BF16, MH, NT>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  if (e != cudaSuccess) return e;
+  g.tiles_m = (g.M + MH * 128 - 1) / (MH * 128);
+  const long long grid = std::max<long long>(1, std::min<long long>(most * g.tiles_m * g.splits, sm_count()));
+  kern<<<(unsigned)grid, kThreads, C::kSmem, st>>>(a, x, b, t, g);
+  count_launch();
+  return cudaGetLastError();
+}
+template <bool BF16, int MH, int NT>
+cudaError_t launch_bwd(const CUtensorMap& r, const CUtensorMap& c, GradArgs g, cudaStream_t st) {
+  using C = Cfg<MH, NT>;
+  auto kern = grouped_grad_umma_kernel<BF16, MH, NT>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  if (e != cudaSuccess) return e;
+  g.tiles_r = (g.rows + MH * 128 - 1) / (MH * 128);
+  g.tiles_c = g.fold ? 1 : (g.cols + NT - 1) / NT;
+  const long long grid = std::min<long long>((long long)g.tiles_r * g.tiles_c * g.mats, sm_count());
+  kern<<<(unsigned)grid, kThreads, C::kSmem, st>>>(r, c, g);
+  count_launch();
+  return cudaGetLastError();
+}
+
+struct Shape {
+  int mh, nt;
+  long long most;                        // column tiles that there can be
+};
+// Rows and columns of a tile.  As many columns as the average run has (a tile is cut to a multiple of 16 at run time, so that
+// too wide a tile costs ring depth only); 256 rows where K is long enough to hide an epilogue that nothing overlaps with, and where
+// that still leaves every SM a tile.
+Shape shape_of(int M, int K, int R, int runs) {
+  const long long each = R / std::max(1, runs);
+  Shape s;
+  s.mh = 1;
+  s.nt = each > 128 ? 256 : each > 64 ? 128 : each > 32 ? 64 : 32;
+  auto most = [&](int nt) { return (long long)R / nt + std::min(R, runs) + 1; };
+  while (s.nt > 32 && most(s.nt) * ((M + 127) / 128) < 120) s.nt /= 2;
+  if (s.nt == 256 && M > 128 && K > 512 && (R / 256) * ((M + 255) / 256) >= 148) s.mh = 2;
+  s.most = most(s.nt);
+  return s;
+}
+
+template <bool BF16>
+cudaError_t fwd(const Shape& s, const CUtensorMap& a, const CUtensorMap& x, const CUtensorMap& b, const CUtensorMap& t, const FwdArgs& g, cudaStream_t st) {
+  if (s.mh == 2) return launch_fwd<BF16, 2, 256>(a, x, b, t, g, s.most, st);
+  if (s.nt == 256) return launch_fwd<BF16, 1, 256>(a, x, b, t, g, s.most, st);
+  if (s.nt == 128) return launch_fwd<BF16, 1, 128>(a, x, b, t, g, s.most, st);
+  if (s.nt == 64) return launch_fwd<BF16, 1, 64>(a, x, b, t, g, s.most, st);
+  return launch_fwd<BF16, 1, 32>(a, x, b, t, g, s.most, st);
+}
+int box_of(const Shape& s) { return s.nt >= 128 ? 64 : 16; }
+
+Operand matrices(const void* p, bool trans, int M, int K, long long ld, long long stride, int count) {
+  return trans ? Operand{p, K, M, ld, stride, count} : Operand{p, M, K, ld, stride, count};
+}
+
+}  // namespace
+
+int low_width(int r) { return r <= 32 ? 64 : 128 * ((r + 63) / 64); }
+
+bool grouped_umma_supports(const GroupedArgs& g, int dtype) {
+  return (dtype == NNLIB_B200_F16 || dtype == NNLIB_B200_BF16) && g.M > 0 && g.K > 0 && g.N > 0 && g.R > 0 && g.G > 0 && (g.G <= kMaxRuns || !g.offsets) &&
+         g.mats > 0 && encode_tiled_fn() != nullptr;
+}
+size_t grouped_umma_workspace_bytes(const GroupedArgs& g) {
+  const Operand a = matrices(g.A, g.transA != 0, g.M, g.K, g.lda, g.strideA, g.mats), x{g.X, g.K, g.N, g.ldx, 0, 1};
+  size_t n = padded(a.copy_bytes()) + padded(x.copy_bytes());
+  if (g.low.r > 0) n += padded(matrices(g.low.B, g.low.transB != 0, g.M, g.low.r, g.low.ldb, g.low.strideB, g.low.n).copy_bytes());
+  return n;
+}
+// to_low: C is T of a following product, low_width(M) elements for each column
+cudaError_t grouped_umma(const GroupedArgs& g, int dtype, bool to_low, void* workspace, cudaStream_t st) {
+  char* ws = static_cast<char*>(workspace);
+  Operand a = matrices(g.A, g.transA != 0, g.M, g.K, g.lda, g.strideA, g.mats), x{g.X, g.K, g.N, g.ldx, 0, 1};
+  const Runs runs{g.offsets, g.run_len, g.G, g.R};
+  cudaError_t e = align_operand(a, ws, g.ids || !g.offsets ? nullptr : &runs, st);
+  if (e == cudaSuccess) e = align_operand(x, ws, nullptr, st);
+  if (e != cudaSuccess) return e;
+  FwdArgs f;
+  std::memset(&f, 0, sizeof(f));
+  f.runs = runs;
+  f.ids = g.ids;
+  f.columns = g.columns;
+  f.C = g.C;
+  f.ldc = g.ldc;
+  f.scale = g.scale;
+  f.scale0 = g.scale0;
+  f.M = g.M; f.K = g.K; f.G = g.G; f.N = g.N; f.mats = g.mats;
+  f.a_kmaj = g.transA;
+  f.a_same = g.mats > 1 && g.strideA == 0;
+  f.zero_rest = g.zero_rest;
+  f.splits = 1;
+  f.to = to_low ? kToLow : kToC;
+  f.pairs = (reinterpret_cast<uintptr_t>(g.C) & 3u) == 0 && g.ldc % 2 == 0;
+  f.low_width = low_width(g.M);
+  f.low_step = f.low_width / 2;
+  f.status = g.status;
+  const Shape s = shape_of(g.M, g.K, g.R, g.G);
+  CUtensorMap ma, mx, mb, mt;
+  if (!encode_matrix(&ma, dtype, a, g.transA != 0) || !encode_columns(&mx, dtype, x, g.columns ? 1 : box_of(s))) return cudaErrorInvalidValue;
+  mb = ma;
+  mt = mx;
+  if (g.low.r > 0 && g.low.n > 0 && g.low.runs > 0) {
+    Operand b = matrices(g.low.B, g.low.transB != 0, g.M, g.low.r, g.low.ldb, g.low.strideB, g.low.n);
+    if ((e = align_operand(b, ws, nullptr, st)) != cudaSuccess) return e;
+    const Operand t{g.low.T, low_width(g.low.r), g.R, g.low.ldt, 0, 1};
+    if (!encode_matrix(&mb, dtype, b, g.low.transB != 0) || !encode_columns(&mt, dtype, t, box_of(s))) return cudaErrorInvalidValue;
+    f.low_runs = Runs{g.low.offsets, g.low.run_len, g.low.runs, g.R};
+    f.low_ids = g.low.ids;
+    f.r = g.low.r; f.n = g.low.n;
+    f.low_kmaj = g.low.transB;
+  }
+  return dtype == NNLIB_B200_BF16 ? fwd<true>(s, ma, mx, mb, mt, f, st) : fwd<false>(s, ma, mx, mb, mt, f, st);
+}
+
+size_t grouped_umma_grad_workspace_bytes(const GroupedGradArgs& g, int fold) {
+  const Operand c{g.C, g.M, g.R, g.ldc, 0, 1}, x{g.X, g.K, g.N, g.ldx, 0, 1};
+  return (fold == 1 ? 0 : padded(c.copy_bytes())) + (fold == 2 ? 0 : padded(x.copy_bytes()));
+}
+bool grouped_umma_grad_supports(const GroupedGradArgs& g, int dtype) {
+  return (dtype == NNLIB_B200_F16 || dtype == NNLIB_B200_BF16) && g.M > 0 && g.K > 0 && g.N > 0 && g.R > 0 && g.mats > 0 && encode_tiled_fn() != nullptr;
+}
+// fold: 0: none; 1: C is T, M its rank; 2: X is T, K its rank
+cudaError_t grouped_umma_grad(const GroupedGradArgs& g, int dtype, int fold, void* workspace, cudaStream_t st) {
+  char* ws = static_cast<char*>(workspace);
+  Operand c{g.C, fold == 1 ? low_width(g.M) : g.M, g.R, g.ldc, 0, 1}, x{g.X, fold == 2 ? low_width(g.K) : g.K, g.N, g.ldx, 0, 1};
+  cudaError_t e = align_operand(c, ws, nullptr, st);
+  if (e == cudaSuccess) e = align_operand(x, ws, nullptr, st);
+  if (e != cudaSuccess) return e;
+  GradArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.runs = Runs{g.offsets, g.run_len, g.G, g.R};
+  a.ids = g.ids;
+  a.columns = g.columns;
+  a.A = g.A;
+  a.ld = g.lda; a.stride = g.strideA;
+  a.G = g.G; a.N = g.N; a.mats = g.mats;
+  a.status = g.status;
+  // the folded side's terms are neighbours in a row of tensor memory; otherwise the side that is contiguous in the result is in its lanes
+  const bool x_rows = fold ? fold == 1 : g.transA != 0;
+  a.rows = x_rows ? g.K : g.M;
+  a.cols = x_rows ? g.M : g.K;
+  a.fold = fold != 0;
+  a.fold_step = fold ? low_width(a.cols) / 2 : 0;
+  a.along = fold && (fold == 1) == (g.transA == 0);
+  a.gather = !g.columns ? 0 : (x_rows ? 1 : 2);
+  a.pairs = (reinterpret_cast<uintptr_t>(g.A) & 3u) == 0 && g.lda % 2 == 0 && g.strideA % 2 == 0;
+  const int nt = fold ? low_width(a.cols) : 256;
+  // 256 rows where the runs are long enough to hide an epilogue that nothing overlaps with
+  const int mh = !fold && a.rows > 128 && g.R / std::max(1, g.mats) > 1024 ? 2 : 1;
+  CUtensorMap mc, mx;
+  if (!encode_columns(&mc, dtype, c, 64) || !encode_columns(&mx, dtype, x, g.columns ? 1 : 64)) return cudaErrorInvalidValue;
+  const CUtensorMap& r = x_rows ? mx : mc;
+  const CUtensorMap& q = x_rows ? mc : mx;
+  const bool bf16 = dtype == NNLIB_B200_BF16;
+  if (mh == 2) return bf16 ? launch_bwd<true, 2, 256>(r, q, a, st) : launch_bwd<false, 2, 256>(r, q, a, st);
+  if (nt == 256) return bf16 ? launch_bwd<true, 1, 256>(r, q, a, st) : launch_bwd<false, 1, 256>(r, q, a, st);
+  if (nt == 128) return bf16 ? launch_bwd<true, 1, 128>(r, q, a, st) : launch_bwd<false, 1, 128>(r, q, a, st);
+  return bf16 ? launch_bwd<true, 1, 64>(r, q, a, st) : launch_bwd<false, 1, 64>(r, q, a, st);
+}
+
+// Reads and clears the sticky "a bounded wait ran out" flag of these kernels on the current device.
+cudaError_t grouped_take_abort(int* out, cudaStream_t st) {
+  int v = 0;
+  cudaError_t e = cudaStreamSynchronize(st);
+  if (e != cudaSuccess) return e;
+  e = cudaMemcpyFromSymbol(&v, g_grouped_abort, sizeof(int));
+  if (e != cudaSuccess) return e;
+  if (v) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_grouped_abort, &zero, sizeof(int));
+  }
+  *out = v;
+  return e;
+}
+
+}  // namespace nb200

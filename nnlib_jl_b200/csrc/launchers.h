@@ -100,6 +100,7 @@ int finish(cudaError_t e);                                // a return code, reme
 bool on_current_device(const void* ptr, int dev);         // NULL passes
 bool check_all_pointers();
 bool log_calls();
+bool force_simt();
 
 // norm and rotation of heads (norm_rope.cu); a side is the queries or the keys
 struct NormRopeSide {
@@ -253,5 +254,14 @@ struct GroupedGradArgs {
 };
 cudaError_t grouped_fma(const GroupedArgs& g, int dtype, bool f32_out, cudaStream_t st);
 cudaError_t grouped_fma_grad(const GroupedGradArgs& g, int dtype, bool f32_rows, bool f32_cols, cudaStream_t st);
+// tcgen05 (grouped_umma.cu): 16-bit arrays
+bool grouped_umma_supports(const GroupedArgs& g, int dtype);
+size_t grouped_umma_workspace_bytes(const GroupedArgs& g);
+cudaError_t grouped_umma(const GroupedArgs& g, int dtype, bool to_low, void* workspace, cudaStream_t st);
+int low_width(int r);                                     // 16-bit elements of T for a column
+bool grouped_umma_grad_supports(const GroupedGradArgs& g, int dtype);
+size_t grouped_umma_grad_workspace_bytes(const GroupedGradArgs& g, int fold);
+cudaError_t grouped_umma_grad(const GroupedGradArgs& g, int dtype, int fold, void* workspace, cudaStream_t st);   // fold: C (1) or X (2) is T
+cudaError_t grouped_take_abort(int* out, cudaStream_t st);
 
 }  // namespace nb200
