@@ -548,7 +548,7 @@ NNLIB_B200_API size_t nnlib_b200_grouped_gemm_workspace_bytes(const nnlib_b200_g
 NNLIB_B200_API int nnlib_b200_grouped_gemm(const nnlib_b200_grouped_params* p, void* workspace, size_t workspace_bytes,
                                            void* stream);
 /* The matrices' gradient: A[:, :, g] = sum over the columns i of run g of C[:, i] * X[:, columns[i]]^T, zeros for an empty
-   run.  Columns of X that do not exist are left out. */
+   run.  Columns of X that do not exist count as zeros. */
 NNLIB_B200_API size_t nnlib_b200_grouped_gemm_grad_workspace_bytes(const nnlib_b200_grouped_params* p);
 NNLIB_B200_API int nnlib_b200_grouped_gemm_grad(const nnlib_b200_grouped_params* p, void* workspace, size_t workspace_bytes,
                                                 void* stream);

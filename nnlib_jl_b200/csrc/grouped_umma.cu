@@ -56,7 +56,6 @@ static_assert(Cfg<2, 256>::kSmem <= 232448 && Cfg<1, 256>::kSmem <= 232448 && Cf
 
 struct Bars {
   uint64_t full[10], empty[10], acc_full[2], acc_empty[2];
-  unsigned long long there[10];          // gradient: which of a stage's 64 columns take part
   uint32_t tmem_base;
   int abort_flag;
   RunSearch search;
@@ -74,7 +73,7 @@ struct FwdArgs {
   const float* scale;
   float scale0;
   int M, K, G, N, mats;
-  int a_kmaj, a_same, zero_rest, splits, tiles_m, to, pairs;
+  int a_kmaj, a_same, zero_rest, splits, tiles_m, to, pairs, gather;
   int low_width, low_step;               // kToLow: elements of T for a column, from the first term to the second
   Runs low_runs;                         // kToC: low-rank pairs, r = 0: none
   const int* low_ids;
@@ -146,6 +145,15 @@ __device__ void count_tiles(const FwdArgs& g, int* cum, RunSearch& s) {
   if (threadIdx.x == 0) cum[g.G] = carry;
   __syncthreads();
 }
+
+// Place in a ring of N stages: no divisions, which cost as much as a stage's copies do.
+template <int N>
+struct Ring {
+  int s = 0, round = 0;
+  __device__ __forceinline__ void next() {
+    if (++s == N) { s = 0; ++round; }
+  }
+};
 
 struct Tile {
   int run, mat, n0, nt, m0, kb0, kb1, split;
@@ -253,73 +261,78 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
       prefetch_tensormap(&tm_x);
     }
     bool ok = true;
-    long long it = 0;
+    Ring<C::kStages> at;
     int run = 0;
-    // one stage: the boxes of the matrix (map ma, block ka of matrix za) and of the columns (map mx, block kx), a lane each
-    auto fill = [&](const CUtensorMap* ma, int ka, int za, bool kmaj, const CUtensorMap* mx, int kx, const Tile& o, bool gather, const int4 (&at)[2]) {
-      const int s = (int)(it % C::kStages);
-      int good = 1;
-      if (it >= C::kStages && lane == 0) good = mbar_wait(&bars->empty[s], (uint32_t)((it / C::kStages) - 1) & 1u, abort_flag) ? 1 : 0;
-      if (!__shfl_sync(0xffffffffu, good, 0)) return false;
+    // One stage: the boxes of the matrix (map ma, block ka of matrix za) and of the columns (map mx, block kx).  Lane 0 issues them all;
+    // gathered columns are the other lanes' too, four each.
+    auto fill = [&](const CUtensorMap* ma, int ka, int za, bool kmaj, const CUtensorMap* mx, int kx, const Tile& o, bool gather, const int4& four) {
+      const int s = at.s;
       uint8_t* da = smem + s * C::kStage;
       uint8_t* dx = da + C::kA;
-      const int boxes = gather ? 0 : (o.nt + C::kBox - 1) / C::kBox;
-      if (lane == 0) mbar_arrive_expect_tx(&bars->full[s], C::kA + (gather ? round16(o.nt) * 128 : boxes * C::kBox * 128));
-      __syncwarp();
-      const int na = kmaj ? MH : 2 * MH;
-      if (lane < na) {
-        if (kmaj) tma_load_3d(da + lane * kHalfBytes, ma, &bars->full[s], ka, o.m0 + lane * 128, za);
-        else tma_load_3d(da + lane * (kHalfBytes / 2), ma, &bars->full[s], o.m0 + lane * 64, ka, za);
-      } else if (lane - na < boxes) {
-        const int i = lane - na;
-        tma_load_2d(dx + i * C::kBox * 128, mx, &bars->full[s], kx, o.n0 + i * C::kBox);
-      }
-      if (gather) {
+      int good = 1;
+      if (lane == 0) {
+        if (at.round > 0) good = mbar_wait(&bars->empty[s], (uint32_t)(at.round - 1) & 1u, abort_flag) ? 1 : 0;
+        if (good) {
+          const int boxes = (o.nt + C::kBox - 1) / C::kBox;
+          mbar_arrive_expect_tx(&bars->full[s], C::kA + (gather ? round16(o.nt) * 128 : boxes * C::kBox * 128));
+          if (kmaj) {
 #pragma unroll
-        for (int i = 0; i < (NT > 128 ? 2 : 1); ++i) {
-          const int q = lane + 32 * i;
-          if (q * 4 < round16(o.nt)) tma_gather4(dx + q * 512, mx, &bars->full[s], kx, at[i]);
+            for (int i = 0; i < MH; ++i) tma_load_3d(da + i * kHalfBytes, ma, &bars->full[s], ka, o.m0 + i * 128, za);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 2 * MH; ++i) tma_load_3d(da + i * (kHalfBytes / 2), ma, &bars->full[s], o.m0 + i * 64, ka, za);
+          }
+          if (!gather)
+            for (int i = 0; i < boxes; ++i) tma_load_2d(dx + i * C::kBox * 128, mx, &bars->full[s], kx, o.n0 + i * C::kBox);
         }
       }
-      ++it;
-      return true;
+      at.next();
+      if (gather) {
+        good = __shfl_sync(0xffffffffu, good, 0);
+        if (good && lane * 4 < round16(o.nt)) tma_gather4(dx + lane * 512, mx, &bars->full[s], kx, four);
+      }
+      return good != 0;
     };
-    for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const Tile o = tile_of<MH, NT>(g, cum, t, nkb, run);
-      if (o.nt <= 0) continue;
-      int4 at[2] = {};
-      if (g.columns) {
-#pragma unroll
-        for (int i = 0; i < (NT > 128 ? 2 : 1); ++i) {
+    // (all lanes stay together where columns are gathered; elsewhere the others have nothing to do)
+    if (g.gather || lane == 0) {
+      for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        const Tile o = tile_of<MH, NT>(g, cum, t, nkb, run);
+        if (o.nt <= 0) continue;
+        int4 four = make_int4(0, 0, 0, 0);
+        if (g.gather) {
           int c[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int n = (lane + 32 * i) * 4 + e;
+            const int n = lane * 4 + e;
             c[e] = n < o.nt ? g.columns[o.n0 + n] : 0;
             if ((unsigned)c[e] >= (unsigned)g.N) c[e] = 0;     // (its column of C becomes zeros)
           }
-          at[i] = make_int4(c[0], c[1], c[2], c[3]);
+          four = make_int4(c[0], c[1], c[2], c[3]);
+        }
+        for (int kb = o.kb0; kb < o.kb1 && ok; ++kb)
+          ok = fill(&tm_a, kb * kBK, g.a_same ? 0 : o.mat, g.a_kmaj != 0, &tm_x, kb * kBK, o, g.gather != 0, four);
+        if (g.r > 0 && ok) {
+          Pairs p(g, o.n0, o.nt);
+          const int blocks = low_blocks(g.r), half = blocks / 2;
+          while (ok && p.next(g, o.n0))
+            for (int q = 0; q < blocks && ok; ++q) ok = fill(&tm_b, (half ? q % half : 0) * kBK, p.id, g.low_kmaj != 0, &tm_t, q * kBK, o, false, four);
         }
       }
-      for (int kb = o.kb0; kb < o.kb1 && ok; ++kb)
-        ok = fill(&tm_a, kb * kBK, g.a_same ? 0 : o.mat, g.a_kmaj != 0, &tm_x, kb * kBK, o, g.columns != nullptr, at);
-      if (g.r > 0 && ok) {
-        Pairs p(g, o.n0, o.nt);
-        const int blocks = low_blocks(g.r), half = blocks / 2;
-        while (ok && p.next(g, o.n0))
-          for (int q = 0; q < blocks && ok; ++q) ok = fill(&tm_b, (half ? q % half : 0) * kBK, p.id, g.low_kmaj != 0, &tm_t, q * kBK, o, false, at);
-      }
     }
+    __syncwarp();
     if (lane == 0 && *abort_flag) {
       // give copies still in flight a bounded chance to land before the CTA leaves
-      for (long long jj = (it > C::kStages ? it - C::kStages : 0); jj < it; ++jj)
-        mbar_wait_drain(&bars->full[jj % C::kStages], (uint32_t)(jj / C::kStages) & 1u, kDrainNs);
+      for (int i = 0; i < C::kStages; ++i) {
+        const int rounds = at.round - (i < at.s ? 0 : 1);
+        if (rounds >= 0) mbar_wait_drain(&bars->full[i], (uint32_t)rounds & 1u, kDrainNs);
+      }
     }
   } else if (start_ok && warp == 1) {
     // -------------------------------------------------------------- MMA issuer
     bool ok = true;
-    long long it = 0;
+    Ring<C::kStages> at;
     int ti = 0, run = 0;
+    const uint32_t base = desc_lo(smem_u32(smem));
     for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
       const Tile o = tile_of<MH, NT>(g, cum, t, nkb, run);
       if (o.nt <= 0) continue;
@@ -328,35 +341,39 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
       const uint32_t id_main = idesc_of(BF16, round16(o.nt), !g.a_kmaj, false);
       int good = 1;
       if (lane == 0) {
-        if (ti >= C::kAccBufs) good = mbar_wait(&bars->acc_empty[ab], (uint32_t)((ti / C::kAccBufs) - 1) & 1u, abort_flag) ? 1 : 0;
+        if (ti >= C::kAccBufs) good = mbar_wait(&bars->acc_empty[ab], (uint32_t)((ti / C::kAccBufs) + 1) & 1u, abort_flag) ? 1 : 0;
         tc_fence_after();
         const uint32_t step = g.a_kmaj ? 32 >> 4 : 2048 >> 4;
         for (int kb = o.kb0; kb < o.kb1 && good; ++kb) {
-          const long long i = it + (kb - o.kb0);
-          const int s = (int)(i % C::kStages);
-          if (!mbar_wait(&bars->full[s], (uint32_t)(i / C::kStages) & 1u, abort_flag)) { good = 0; break; }
+          const int s = at.s;
+          if (!mbar_wait(&bars->full[s], (uint32_t)at.round & 1u, abort_flag)) { good = 0; break; }
           tc_fence_after();
-          const uint32_t a = desc_lo(smem_u32(smem + s * C::kStage)), x = desc_lo(smem_u32(smem + s * C::kStage + C::kA));
+          const uint32_t a = base + s * (C::kStage >> 4), x = a + (C::kA >> 4);
           const int steps = min(4, (g.K - kb * kBK + 15) >> 4);
-          for (int kk = 0; kk < steps; ++kk) {
 #pragma unroll
-            for (int h = 0; h < MH; ++h)
-              umma_ss_lohi(acc + h * NT, a + h * (kHalfBytes >> 4) + kk * step, x + kk * 2, kDescHi, id_main, (kb > o.kb0 || kk > 0) ? 1u : 0u);
+          for (int kk = 0; kk < 4; ++kk) {
+            if (kk < steps) {
+#pragma unroll
+              for (int h = 0; h < MH; ++h)
+                umma_ss_lohi(acc + h * NT, a + h * (kHalfBytes >> 4) + kk * step, x + kk * 2, kDescHi, id_main, (kb > o.kb0 || kk > 0) ? 1u : 0u);
+            }
           }
           umma_commit(&bars->empty[s]);
+          at.next();
         }
       }
-      it += o.kb1 - o.kb0;
       ok = __shfl_sync(0xffffffffu, good, 0) != 0;
+      at.s = __shfl_sync(0xffffffffu, at.s, 0);
+      at.round = __shfl_sync(0xffffffffu, at.round, 0);
       if (g.r > 0 && ok) {
         Pairs p(g, o.n0, o.nt);
         const int blocks = low_blocks(g.r), half = blocks / 2;
         const uint32_t id_low = idesc_of(BF16, round16(o.nt), !g.low_kmaj, false), step = g.low_kmaj ? 32 >> 4 : 2048 >> 4;
         while (ok && p.next(g, o.n0)) {
           const int lo = p.lo - o.n0, hi = p.hi - o.n0, all = round16(o.nt);
-          for (int q = 0; q < blocks; ++q, ++it) {
-            const int s = (int)(it % C::kStages);
-            ok = mbar_wait_warp(&bars->full[s], (uint32_t)(it / C::kStages) & 1u, abort_flag);
+          for (int q = 0; q < blocks; ++q, at.next()) {
+            const int s = at.s;
+            ok = mbar_wait_warp(&bars->full[s], (uint32_t)at.round & 1u, abort_flag);
             if (!ok) break;
             __syncwarp();
             uint8_t* tx = smem + s * C::kStage + C::kA;
@@ -495,16 +512,14 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
 // ------------------------------------------------------------------------------------------------- gradient
 //     A_a[row, col] = sum over the columns i of the runs of matrix a of P[row, i] Q[col, i]
 // rows and columns of the matrix being features of dC and X, or of X and dC: the one that is stored contiguously is the rows'.  Both
-// operands are MN-major, the contraction runs over a run's columns in blocks of 64; what a block holds behind the run's end, or of a
-// column that is none, is cleared in shared memory before it is multiplied (another run's infinity times zero would be a NaN).
+// operands are MN-major, the contraction runs over a run's columns in blocks of 64; what a block holds behind the run's end is
+// cleared in shared memory before it is multiplied (another run's infinity times zero would be a NaN).
 struct GradArgs {
   Runs runs;
   const int* ids;
-  const int* columns;
   void* A;
   long long ld, stride;                  // between columns and matrices of the result
-  int rows, cols, G, N, mats;
-  int gather;                            // 1: the rows' operand is gathered, 2: the columns' is
+  int rows, cols, G, mats;
   int tiles_r, tiles_c, pairs;
   int fold, fold_step, along;            // fold: columns fold_step apart are the two terms of one; along: a row's columns are contiguous
   int* status;
@@ -547,77 +562,49 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
   auto last_run = [&](int a) { return g.ids ? g.G : min(a + 1, g.G); };
 
   if (start_ok && warp == 0) {
-    bool ok = true;
-    long long it = 0;
     if (lane == 0) {
       prefetch_tensormap(&tm_r);
       prefetch_tensormap(&tm_c);
-    }
-    constexpr int kBoxesR = 2 * MH, kBoxesC = NT / 64;
-    for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const int a = (int)(t / each), q = (int)(t % each);
-      const int r0 = (q % g.tiles_r) * (MH * 128), c0 = (q / g.tiles_r) * NT;
-      for (int b = first_run(a); b < last_run(a) && ok; ++b) {
-        if (g.ids && g.ids[b] != a) continue;
-        const int end = g.runs.end(b);
-        for (int i0 = g.runs.begin(b); i0 < end && ok; i0 += kBK, ++it) {
-          const int s = (int)(it % C::kStages);
-          int4 at = make_int4(0, 0, 0, 0);
-          unsigned long long there = end - i0 >= 64 ? ~0ull : (1ull << (end - i0)) - 1;
-          if (g.gather) {
-            int c[4];
-            unsigned have = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int i = i0 + (lane & 15) * 4 + e;
-              c[e] = i < end ? g.columns[i] : -1;
-              if ((unsigned)c[e] < (unsigned)g.N) have |= 1u << e; else c[e] = 0;
-            }
-            at = make_int4(c[0], c[1], c[2], c[3]);
-            unsigned lo = have << ((lane & 7) * 4);
-#pragma unroll
-            for (int x = 1; x < 8; x <<= 1) lo |= __shfl_xor_sync(0xffffffffu, lo, x);
-            there = (unsigned long long)__shfl_sync(0xffffffffu, lo, 0) | (unsigned long long)__shfl_sync(0xffffffffu, lo, 8) << 32;
-          }
-          int good = 1;
-          if (it >= C::kStages && lane == 0) good = mbar_wait(&bars->empty[s], (uint32_t)((it / C::kStages) - 1) & 1u, abort_flag) ? 1 : 0;
-          ok = __shfl_sync(0xffffffffu, good, 0) != 0;
-          if (!ok) break;
-          uint8_t* dr = smem + s * C::kStage;
-          uint8_t* dc = dr + C::kA;
-          if (lane == 0) {
-            bars->there[s] = there;
+      bool ok = true;
+      Ring<C::kStages> at;
+      for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        const int a = (int)(t / each), q = (int)(t % each);
+        const int r0 = (q % g.tiles_r) * (MH * 128), c0 = (q / g.tiles_r) * NT;
+        for (int b = first_run(a); b < last_run(a) && ok; ++b) {
+          if (g.ids && g.ids[b] != a) continue;
+          const int end = g.runs.end(b);
+          for (int i0 = g.runs.begin(b); i0 < end; i0 += kBK, at.next()) {
+            const int s = at.s;
+            if (at.round > 0) ok = mbar_wait(&bars->empty[s], (uint32_t)(at.round - 1) & 1u, abort_flag);
+            if (!ok) break;
+            uint8_t* d = smem + s * C::kStage;
             mbar_arrive_expect_tx(&bars->full[s], C::kStage);
-          }
-          __syncwarp();
-          if (g.gather == 1) {
-            for (int x = lane >> 4; x < kBoxesR; x += 2) tma_gather4(dr + x * (kHalfBytes / 2) + (lane & 15) * 512, &tm_r, &bars->full[s], r0 + x * 64, at);
-          } else if (lane < kBoxesR) {
-            tma_load_2d(dr + lane * (kHalfBytes / 2), &tm_r, &bars->full[s], r0 + lane * 64, i0);
-          }
-          if (g.gather == 2) {
-            for (int x = lane >> 4; x < kBoxesC; x += 2) tma_gather4(dc + x * (kHalfBytes / 2) + (lane & 15) * 512, &tm_c, &bars->full[s], c0 + x * 64, at);
-          } else if (lane >= 8 && lane - 8 < kBoxesC) {
-            tma_load_2d(dc + (lane - 8) * (kHalfBytes / 2), &tm_c, &bars->full[s], c0 + (lane - 8) * 64, i0);
+#pragma unroll
+            for (int x = 0; x < 2 * MH; ++x) tma_load_2d(d + x * (kHalfBytes / 2), &tm_r, &bars->full[s], r0 + x * 64, i0);
+#pragma unroll
+            for (int x = 0; x < NT / 64; ++x) tma_load_2d(d + C::kA + x * (kHalfBytes / 2), &tm_c, &bars->full[s], c0 + x * 64, i0);
           }
         }
       }
-    }
-    if (lane == 0 && *abort_flag) {
-      for (long long jj = (it > C::kStages ? it - C::kStages : 0); jj < it; ++jj)
-        mbar_wait_drain(&bars->full[jj % C::kStages], (uint32_t)(jj / C::kStages) & 1u, kDrainNs);
+      if (*abort_flag) {
+        for (int i = 0; i < C::kStages; ++i) {
+          const int rounds = at.round - (i < at.s ? 0 : 1);
+          if (rounds >= 0) mbar_wait_drain(&bars->full[i], (uint32_t)rounds & 1u, kDrainNs);
+        }
+      }
     }
   } else if (start_ok && warp == 1) {
     bool ok = true;
-    long long it = 0;
+    Ring<C::kStages> at;
     int ti = 0;
+    const uint32_t base = desc_lo(smem_u32(smem));
     for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++ti) {
       const int a = (int)(t / each), left = g.cols - (int)((t % each) / g.tiles_r) * NT;
       const int ab = ti % C::kAccBufs;
       const uint32_t acc = tmem + ab * C::kAccCols;
       const uint32_t idesc = idesc_of(BF16, g.fold || left > NT ? NT : round16(left), true, true);
       if (ti >= C::kAccBufs) {
-        ok = mbar_wait_warp(&bars->acc_empty[ab], (uint32_t)((ti / C::kAccBufs) - 1) & 1u, abort_flag);
+        ok = mbar_wait_warp(&bars->acc_empty[ab], (uint32_t)((ti / C::kAccBufs) + 1) & 1u, abort_flag);
         if (!ok) break;
       }
       tc_fence_after();
@@ -625,16 +612,13 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
       for (int b = first_run(a); b < last_run(a) && ok; ++b) {
         if (g.ids && g.ids[b] != a) continue;
         const int end = g.runs.end(b);
-        for (int i0 = g.runs.begin(b); i0 < end; i0 += kBK, ++it) {
-          const int s = (int)(it % C::kStages);
-          ok = mbar_wait_warp(&bars->full[s], (uint32_t)(it / C::kStages) & 1u, abort_flag);
+        for (int i0 = g.runs.begin(b); i0 < end; i0 += kBK, at.next()) {
+          const int s = at.s, here = min(kBK, end - i0), steps = (here + 15) >> 4;
+          ok = mbar_wait_warp(&bars->full[s], (uint32_t)at.round & 1u, abort_flag);
           if (!ok) break;
-          __syncwarp();
-          const int steps = min(4, (end - i0 + 15) >> 4);
-          const unsigned long long missing = ~*reinterpret_cast<volatile unsigned long long*>(&bars->there[s]) & (steps == 4 ? ~0ull : (1ull << (steps * 16)) - 1);
-          if (missing) {
-            for (int i = lane; i < steps * 16 * 8; i += 32) {
-              if (!((missing >> (i >> 3)) & 1ull)) continue;
+          if (here & 15) {                                 // another run's columns, or nobody's
+            __syncwarp();
+            for (int i = here * 8 + lane; i < steps * 16 * 8; i += 32) {
 #pragma unroll
               for (int x = 0; x < C::kStage / (kHalfBytes / 2); ++x)
                 *reinterpret_cast<uint4*>(smem + s * C::kStage + x * (kHalfBytes / 2) + i * 16) = make_uint4(0, 0, 0, 0);
@@ -644,11 +628,14 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
           }
           if (lane == 0) {
             tc_fence_after();
-            const uint32_t r = desc_lo(smem_u32(smem + s * C::kStage)), c = desc_lo(smem_u32(smem + s * C::kStage + C::kA));
-            for (int kk = 0; kk < steps; ++kk) {
+            const uint32_t r = base + s * (C::kStage >> 4), c = r + (C::kA >> 4);
 #pragma unroll
-              for (int h = 0; h < MH; ++h)
-                umma_ss_lohi(acc + h * NT, r + h * (kHalfBytes >> 4) + kk * (2048 >> 4), c + kk * (2048 >> 4), kDescHi, idesc, (begun || kk > 0) ? 1u : 0u);
+            for (int kk = 0; kk < 4; ++kk) {
+              if (kk < steps) {
+#pragma unroll
+                for (int h = 0; h < MH; ++h)
+                  umma_ss_lohi(acc + h * NT, r + h * (kHalfBytes >> 4) + kk * (2048 >> 4), c + kk * (2048 >> 4), kDescHi, idesc, (begun || kk > 0) ? 1u : 0u);
+              }
             }
             umma_commit(&bars->empty[s]);
           }
@@ -748,22 +735,44 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
 }
 
 // ------------------------------------------------------------------------------------------------- copies, host
-// `count` matrices of wide x deep 16-bit elements to rows that the copy engine can address; with `offsets`, only those of runs
-// that have columns.
-__global__ void __launch_bounds__(256) aligned_copy_kernel(const unsigned short* src, long long ld, long long stride, uint4* dst, int wide, long long deep,
-                                                           int ld8, Runs of) {
+// `count` matrices of wide x deep 16-bit elements to rows that the copy engine can address; with `of`, only those of runs that have
+// columns; with `columns`, row i from row columns[i] of `rows`, zeros where there is none.
+struct CopyArgs {
+  const unsigned short* src;
+  long long ld, stride, deep;
+  uint4* dst;
+  int wide, ld8, vec, rows;              // ld8: 16-byte packets of a row; vec: the source has them too
+  const int* columns;
+  Runs of;
+};
+__global__ void __launch_bounds__(256) copy_rows_kernel(const __grid_constant__ CopyArgs g) {
   const int mat = blockIdx.z;
-  if (of.offsets && of.end(mat) <= of.begin(mat)) return;
-  const unsigned short* s = src + (long long)mat * stride;
-  uint4* d = dst + (long long)mat * deep * ld8;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < deep * ld8; i += (long long)gridDim.x * 256) {
-    const long long row = i / ld8;
-    const int c = (int)(i % ld8) * 8;
-    const unsigned short* p = s + row * ld + c;
-    unsigned short v[8];
+  if (g.of.offsets && g.of.end(mat) <= g.of.begin(mat)) return;
+  const unsigned short* s = g.src + (long long)mat * g.stride;
+  uint4* d = g.dst + (long long)mat * g.deep * g.ld8;
+  // four packets of a row at a time under way
+  for (long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); row < g.deep; row += (long long)gridDim.x * 8) {
+    long long from = row;
+    if (g.columns) {
+      const int c = g.columns[row];
+      from = (unsigned)c < (unsigned)g.rows ? c : -1;
+    }
+    const unsigned short* p = s + from * g.ld;
+#pragma unroll 4
+    for (int i = threadIdx.x & 31; i < g.ld8; i += 32) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (from >= 0) {
+        if (g.vec) {
+          v = *reinterpret_cast<const uint4*>(p + i * 8);
+        } else {
+          unsigned short e[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = c + e < wide ? p[e] : (unsigned short)0;
-    d[i] = make_uint4(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16, v[4] | (uint32_t)v[5] << 16, v[6] | (uint32_t)v[7] << 16);
+          for (int u = 0; u < 8; ++u) e[u] = i * 8 + u < g.wide ? p[i * 8 + u] : (unsigned short)0;
+          v = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
+        }
+      }
+      d[row * g.ld8 + i] = v;
+    }
   }
 }
 
@@ -771,21 +780,31 @@ __global__ void __launch_bounds__(256) aligned_copy_kernel(const unsigned short*
 struct Operand {
   const void* p;
   long long wide, deep, ld, stride, count;
+  const int* columns;                    // rows `deep` of them are gathered from these of `rows`; NULL: as they lie
+  long long rows;
   bool fits() const { return aligned16(p) && stride_ok(ld) && (count <= 1 || stride == 0 || stride_ok(stride)); }
-  size_t copy_bytes() const { return fits() || wide == 0 || deep == 0 || count == 0 ? 0 : (size_t)((wide + 7) / 8 * 16) * deep * count; }
+  size_t copy_bytes() const { return (fits() && !columns) || wide == 0 || deep == 0 || count == 0 ? 0 : (size_t)((wide + 7) / 8 * 16) * deep * count; }
 };
 cudaError_t align_operand(Operand& o, char*& ws, const Runs* of, cudaStream_t st) {
   const size_t bytes = o.copy_bytes();
   if (!bytes) return cudaSuccess;
-  const int ld8 = (int)((o.wide + 7) / 8);
-  const long long blocks = std::min<long long>((o.deep * ld8 + 255) / 256, 65535);
-  aligned_copy_kernel<<<dim3((unsigned)blocks, 1, (unsigned)o.count), 256, 0, st>>>(static_cast<const unsigned short*>(o.p), o.ld, o.stride,
-                                                                                    reinterpret_cast<uint4*>(ws), (int)o.wide, o.deep, ld8,
-                                                                                    of ? *of : Runs{nullptr, 0, 0, 0});
+  CopyArgs c;
+  c.src = static_cast<const unsigned short*>(o.p);
+  c.ld = o.ld; c.stride = o.stride; c.deep = o.deep;
+  c.dst = reinterpret_cast<uint4*>(ws);
+  c.wide = (int)o.wide;
+  c.ld8 = (int)((o.wide + 7) / 8);
+  c.vec = o.fits() && o.wide % 8 == 0;
+  c.rows = (int)o.rows;
+  c.columns = o.columns;
+  c.of = of ? *of : Runs{nullptr, 0, 0, 0};
+  const long long blocks = std::min<long long>((o.deep + 7) / 8, 1 << 20);
+  copy_rows_kernel<<<dim3((unsigned)blocks, 1, (unsigned)o.count), 256, 0, st>>>(c);
   count_launch();
   o.p = ws;
-  o.ld = (long long)ld8 * 8;
+  o.ld = (long long)c.ld8 * 8;
   o.stride = o.ld * o.deep;
+  o.columns = nullptr;
   ws += (bytes + 255) / 256 * 256;
   return cudaGetLastError();
 }
@@ -873,7 +892,16 @@ cudaError_t fwd(const Shape& s, const CUtensorMap& a, const CUtensorMap& x, cons
 int box_of(const Shape& s) { return s.nt >= 128 ? 64 : 16; }
 
 Operand matrices(const void* p, bool trans, int M, int K, long long ld, long long stride, int count) {
-  return trans ? Operand{p, K, M, ld, stride, count} : Operand{p, M, K, ld, stride, count};
+  return trans ? Operand{p, K, M, ld, stride, count, nullptr, 0} : Operand{p, M, K, ld, stride, count, nullptr, 0};
+}
+// the columns of a product's result, gathered where they are not its own
+Operand columns_of(const void* X, int K, int N, long long ld, const int* columns, int R) {
+  return columns ? Operand{X, K, R, ld, 0, 1, columns, N} : Operand{X, K, N, ld, 0, 1, nullptr, 0};
+}
+// Whether the copy engine gathers: it takes some 65 cycles for every four columns and 64 features, for each tile of rows anew, so
+// only while all columns are few; a copy of them, gathered once, costs a launch (8192 tokens twice, 14336 x 4096: 4.5 ms, 1.5 with the copy).
+bool gathers_in_place(const Operand& x, const Shape& s) {
+  return s.nt <= 32 && Operand{x.p, x.wide, x.deep, x.ld, x.stride, x.count, nullptr, 0}.fits();
 }
 
 }  // namespace
@@ -885,16 +913,19 @@ bool grouped_umma_supports(const GroupedArgs& g, int dtype) {
          g.mats > 0 && encode_tiled_fn() != nullptr;
 }
 size_t grouped_umma_workspace_bytes(const GroupedArgs& g) {
-  const Operand a = matrices(g.A, g.transA != 0, g.M, g.K, g.lda, g.strideA, g.mats), x{g.X, g.K, g.N, g.ldx, 0, 1};
-  size_t n = padded(a.copy_bytes()) + padded(x.copy_bytes());
+  const Operand a = matrices(g.A, g.transA != 0, g.M, g.K, g.lda, g.strideA, g.mats), x = columns_of(g.X, g.K, g.N, g.ldx, g.columns, g.R);
+  size_t n = padded(a.copy_bytes()) + (gathers_in_place(x, shape_of(g.M, g.K, g.R, g.G)) ? 0 : padded(x.copy_bytes()));
   if (g.low.r > 0) n += padded(matrices(g.low.B, g.low.transB != 0, g.M, g.low.r, g.low.ldb, g.low.strideB, g.low.n).copy_bytes());
   return n;
 }
 // to_low: C is T of a following product, low_width(M) elements for each column
 cudaError_t grouped_umma(const GroupedArgs& g, int dtype, bool to_low, void* workspace, cudaStream_t st) {
   char* ws = static_cast<char*>(workspace);
-  Operand a = matrices(g.A, g.transA != 0, g.M, g.K, g.lda, g.strideA, g.mats), x{g.X, g.K, g.N, g.ldx, 0, 1};
+  Operand a = matrices(g.A, g.transA != 0, g.M, g.K, g.lda, g.strideA, g.mats), x = columns_of(g.X, g.K, g.N, g.ldx, g.columns, g.R);
   const Runs runs{g.offsets, g.run_len, g.G, g.R};
+  const Shape s = shape_of(g.M, g.K, g.R, g.G);
+  const bool in_place = g.columns && gathers_in_place(x, s);
+  if (in_place) x = columns_of(g.X, g.K, g.N, g.ldx, nullptr, 0);
   cudaError_t e = align_operand(a, ws, g.ids || !g.offsets ? nullptr : &runs, st);
   if (e == cudaSuccess) e = align_operand(x, ws, nullptr, st);
   if (e != cudaSuccess) return e;
@@ -903,6 +934,7 @@ cudaError_t grouped_umma(const GroupedArgs& g, int dtype, bool to_low, void* wor
   f.runs = runs;
   f.ids = g.ids;
   f.columns = g.columns;
+  f.gather = in_place;
   f.C = g.C;
   f.ldc = g.ldc;
   f.scale = g.scale;
@@ -917,15 +949,14 @@ cudaError_t grouped_umma(const GroupedArgs& g, int dtype, bool to_low, void* wor
   f.low_width = low_width(g.M);
   f.low_step = f.low_width / 2;
   f.status = g.status;
-  const Shape s = shape_of(g.M, g.K, g.R, g.G);
   CUtensorMap ma, mx, mb, mt;
-  if (!encode_matrix(&ma, dtype, a, g.transA != 0) || !encode_columns(&mx, dtype, x, g.columns ? 1 : box_of(s))) return cudaErrorInvalidValue;
+  if (!encode_matrix(&ma, dtype, a, g.transA != 0) || !encode_columns(&mx, dtype, x, in_place ? 1 : box_of(s))) return cudaErrorInvalidValue;
   mb = ma;
   mt = mx;
   if (g.low.r > 0 && g.low.n > 0 && g.low.runs > 0) {
     Operand b = matrices(g.low.B, g.low.transB != 0, g.M, g.low.r, g.low.ldb, g.low.strideB, g.low.n);
     if ((e = align_operand(b, ws, nullptr, st)) != cudaSuccess) return e;
-    const Operand t{g.low.T, low_width(g.low.r), g.R, g.low.ldt, 0, 1};
+    const Operand t{g.low.T, low_width(g.low.r), g.R, g.low.ldt, 0, 1, nullptr, 0};
     if (!encode_matrix(&mb, dtype, b, g.low.transB != 0) || !encode_columns(&mt, dtype, t, box_of(s))) return cudaErrorInvalidValue;
     f.low_runs = Runs{g.low.offsets, g.low.run_len, g.low.runs, g.R};
     f.low_ids = g.low.ids;
@@ -936,7 +967,7 @@ cudaError_t grouped_umma(const GroupedArgs& g, int dtype, bool to_low, void* wor
 }
 
 size_t grouped_umma_grad_workspace_bytes(const GroupedGradArgs& g, int fold) {
-  const Operand c{g.C, g.M, g.R, g.ldc, 0, 1}, x{g.X, g.K, g.N, g.ldx, 0, 1};
+  const Operand c = columns_of(g.C, g.M, g.R, g.ldc, nullptr, 0), x = columns_of(g.X, g.K, g.N, g.ldx, g.columns, g.R);
   return (fold == 1 ? 0 : padded(c.copy_bytes())) + (fold == 2 ? 0 : padded(x.copy_bytes()));
 }
 bool grouped_umma_grad_supports(const GroupedGradArgs& g, int dtype) {
@@ -945,7 +976,8 @@ bool grouped_umma_grad_supports(const GroupedGradArgs& g, int dtype) {
 // fold: 0: none; 1: C is T, M its rank; 2: X is T, K its rank
 cudaError_t grouped_umma_grad(const GroupedGradArgs& g, int dtype, int fold, void* workspace, cudaStream_t st) {
   char* ws = static_cast<char*>(workspace);
-  Operand c{g.C, fold == 1 ? low_width(g.M) : g.M, g.R, g.ldc, 0, 1}, x{g.X, fold == 2 ? low_width(g.K) : g.K, g.N, g.ldx, 0, 1};
+  Operand c = columns_of(g.C, fold == 1 ? low_width(g.M) : g.M, g.R, g.ldc, nullptr, 0),
+          x = columns_of(g.X, fold == 2 ? low_width(g.K) : g.K, g.N, g.ldx, g.columns, g.R);
   cudaError_t e = align_operand(c, ws, nullptr, st);
   if (e == cudaSuccess) e = align_operand(x, ws, nullptr, st);
   if (e != cudaSuccess) return e;
@@ -953,10 +985,9 @@ cudaError_t grouped_umma_grad(const GroupedGradArgs& g, int dtype, int fold, voi
   std::memset(&a, 0, sizeof(a));
   a.runs = Runs{g.offsets, g.run_len, g.G, g.R};
   a.ids = g.ids;
-  a.columns = g.columns;
   a.A = g.A;
   a.ld = g.lda; a.stride = g.strideA;
-  a.G = g.G; a.N = g.N; a.mats = g.mats;
+  a.G = g.G; a.mats = g.mats;
   a.status = g.status;
   // the folded side's terms are neighbours in a row of tensor memory; otherwise the side that is contiguous in the result is in its lanes
   const bool x_rows = fold ? fold == 1 : g.transA != 0;
@@ -965,13 +996,12 @@ cudaError_t grouped_umma_grad(const GroupedGradArgs& g, int dtype, int fold, voi
   a.fold = fold != 0;
   a.fold_step = fold ? low_width(a.cols) / 2 : 0;
   a.along = fold && (fold == 1) == (g.transA == 0);
-  a.gather = !g.columns ? 0 : (x_rows ? 1 : 2);
   a.pairs = (reinterpret_cast<uintptr_t>(g.A) & 3u) == 0 && g.lda % 2 == 0 && g.strideA % 2 == 0;
   const int nt = fold ? low_width(a.cols) : 256;
   // 256 rows where the runs are long enough to hide an epilogue that nothing overlaps with
   const int mh = !fold && a.rows > 128 && g.R / std::max(1, g.mats) > 1024 ? 2 : 1;
   CUtensorMap mc, mx;
-  if (!encode_columns(&mc, dtype, c, 64) || !encode_columns(&mx, dtype, x, g.columns ? 1 : 64)) return cudaErrorInvalidValue;
+  if (!encode_columns(&mc, dtype, c, 64) || !encode_columns(&mx, dtype, x, 64)) return cudaErrorInvalidValue;
   const CUtensorMap& r = x_rows ? mx : mc;
   const CUtensorMap& q = x_rows ? mc : mx;
   const bool bf16 = dtype == NNLIB_B200_BF16;
