@@ -9,8 +9,10 @@
 //
 // One CTA owns an (MH*128 rows) x (at most NT columns) tile and walks over K in blocks of 64; the grid is persistent.
 //   prologue    every CTA counts the tiles of all runs (at most kMaxRuns: 4 KB of prefix sums in shared memory)
-//   warp 0      TMA producer: a ring of stages, each a K block of the matrix (K- or MN-major, as it is stored) and of the
-//               columns (K-major); gathered columns arrive four at a time (tile::gather4), their numbers in the lanes' registers
+//   warps 0, 10, 11  TMA producers, every third stage each: a ring of stages, each a K block of the matrix (K- or MN-major, as it
+//               is stored) and of the columns (K-major); gathered columns arrive four at a time (tile::gather4), their numbers in
+//               the lanes' registers.  One thread takes some 125 cycles for a copy: with a single producer a stage took 765 cycles,
+//               148 of them 4.2 TB/s
 //   warp 1      allocates tensor memory, issues every tcgen05.mma; for low-rank pairs it clears the rows of T that belong to
 //               other runs before it multiplies
 //   warps 2-9   epilogue: tensor memory -> registers -> C; two lanes exchange halves so that a store is two rows of a column
@@ -32,7 +34,8 @@ __device__ int g_grouped_abort = 0;  // sticky: a bounded wait of one of these k
 
 namespace {
 
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;
+constexpr int kProducers = 3;              // warps 0, 10, 11: a copy costs its thread some 125 cycles, a stage has up to eight
 constexpr int kBK = 64;                  // K elements per stage: one 128-byte swizzle row
 constexpr int kHalfBytes = 128 * 128;    // 128 rows x 64 K elements, either layout
 constexpr int kMaxRuns = 1024;
@@ -254,18 +257,25 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
   const long long columns = g.runs.offsets ? cum[g.G] : (long long)g.G * tile_count<NT>((int)g.runs.len);
   const long long tiles = columns * g.tiles_m * g.splits;
 
-  if (start_ok && warp == 0) {
-    // ------------------------------------------------------------ TMA producer
+  if (start_ok && (warp == 0 || warp >= 10)) {
+    // ----------------------------------------------------------- TMA producers
+    const int me = warp == 0 ? 0 : warp - 9;
     if (lane == 0) {
       prefetch_tensormap(&tm_a);
       prefetch_tensormap(&tm_x);
     }
     bool ok = true;
     Ring<C::kStages> at;
-    int run = 0;
-    // One stage: the boxes of the matrix (map ma, block ka of matrix za) and of the columns (map mx, block kx).  Lane 0 issues them all;
+    int run = 0, turn = 0;
+    // One stage, if it is this warp's turn: the boxes of the matrix (map ma, block ka of matrix za) and of the columns (map mx, block kx).  Lane 0 issues them all;
     // gathered columns are the other lanes' too, four each.
     auto fill = [&](const CUtensorMap* ma, int ka, int za, bool kmaj, const CUtensorMap* mx, int kx, const Tile& o, bool gather, const int4& four) {
+      const bool mine = turn == me;
+      if (++turn == kProducers) turn = 0;
+      if (!mine) {
+        at.next();
+        return true;
+      }
       const int s = at.s;
       uint8_t* da = smem + s * C::kStage;
       uint8_t* dx = da + C::kA;
@@ -320,7 +330,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
       }
     }
     __syncwarp();
-    if (lane == 0 && *abort_flag) {
+    if (warp == 0 && lane == 0 && *abort_flag) {
       // give copies still in flight a bounded chance to land before the CTA leaves
       for (int i = 0; i < C::kStages; ++i) {
         const int rounds = at.round - (i < at.s ? 0 : 1);
@@ -403,7 +413,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
       if (ok && lane == 0) umma_commit(&bars->acc_full[ab]);
       ++ti;
     }
-  } else if (start_ok && warp >= 2) {
+  } else if (start_ok && warp >= 2 && warp < 10) {
     // ----------------------------------------------------------------- epilogue
     const int wq = warp & 3, part = (warp - 2) >> 2;       // TMEM lane quarter; MH = 2: half of the rows, 1: every other 32 columns
     constexpr int kStep = MH == 2 ? 1 : 2;
@@ -561,12 +571,14 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
   auto first_run = [&](int a) { return g.ids ? 0 : a; };
   auto last_run = [&](int a) { return g.ids ? g.G : min(a + 1, g.G); };
 
-  if (start_ok && warp == 0) {
+  if (start_ok && (warp == 0 || warp >= 10)) {
+    const int me = warp == 0 ? 0 : warp - 9;
     if (lane == 0) {
       prefetch_tensormap(&tm_r);
       prefetch_tensormap(&tm_c);
       bool ok = true;
       Ring<C::kStages> at;
+      int turn = 0;
       for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
         const int a = (int)(t / each), q = (int)(t % each);
         const int r0 = (q % g.tiles_r) * (MH * 128), c0 = (q / g.tiles_r) * NT;
@@ -574,6 +586,9 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
           if (g.ids && g.ids[b] != a) continue;
           const int end = g.runs.end(b);
           for (int i0 = g.runs.begin(b); i0 < end; i0 += kBK, at.next()) {
+            const bool mine = turn == me;
+            if (++turn == kProducers) turn = 0;
+            if (!mine) continue;
             const int s = at.s;
             if (at.round > 0) ok = mbar_wait(&bars->empty[s], (uint32_t)(at.round - 1) & 1u, abort_flag);
             if (!ok) break;
@@ -586,7 +601,7 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
           }
         }
       }
-      if (*abort_flag) {
+      if (me == 0 && *abort_flag) {
         for (int i = 0; i < C::kStages; ++i) {
           const int rounds = at.round - (i < at.s ? 0 : 1);
           if (rounds >= 0) mbar_wait_drain(&bars->full[i], (uint32_t)rounds & 1u, kDrainNs);
@@ -645,7 +660,7 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
       }
       if (ok && lane == 0) umma_commit(&bars->acc_full[ab]);
     }
-  } else if (start_ok && warp >= 2) {
+  } else if (start_ok && warp >= 2 && warp < 10) {
     const int wq = warp & 3, part = (warp - 2) >> 2;
     constexpr int kStep = MH == 2 ? 1 : 2;
     bool ok = true;
