@@ -8,7 +8,7 @@
 // that a run of 300 is two tiles of 160 and 140 and not 256 and 44, and one of 3 is padded to 16 and not to 128.
 //
 // One CTA owns an (MH*128 rows) x (at most NT columns) tile and walks over K in blocks of 64; the grid is persistent.
-//   prologue    every CTA counts the tiles of all runs (at most kMaxRuns: 4 KB of prefix sums in shared memory)
+//   prologue    every CTA counts the tiles of all runs (at most kMaxRuns) into a table in shared memory
 //   warps 0, 10, 11  TMA producers, every third stage each: a ring of stages, each a K block of the matrix (K- or MN-major, as it
 //               is stored) and of the columns (K-major); gathered columns arrive four at a time (tile::gather4), their numbers in
 //               the lanes' registers.  One thread takes some 125 cycles for a copy: with a single producer a stage took 765 cycles,
@@ -42,15 +42,21 @@ constexpr int kMaxRuns = 1024;
 constexpr int kAhead = 8;                // column tiles that a band of row tiles shares
 constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);   // 8-row groups 1024 bytes apart, 128-byte swizzle
 
+// The runs of a call with offsets, in shared memory: column tiles of the runs before run i, its first column, the column behind it.
+struct Table {
+  int cum[kMaxRuns + 8], begin[kMaxRuns], end[kMaxRuns];
+};
+constexpr int kTableBytes = sizeof(Table);
+
 template <int MH, int NT>
 struct Cfg {
   static constexpr int kA = MH * kHalfBytes, kX = NT * 128, kStage = kA + kX;
-  static constexpr int kRoom = 226 * 1024 - 4 * (kMaxRuns + 8) - 512;
+  static constexpr int kRoom = 226 * 1024 - kTableBytes - 512;
   static constexpr int kStages = kRoom / kStage > 10 ? 10 : kRoom / kStage;
   static constexpr int kAccCols = MH * NT, kAccBufs = kAccCols <= 256 ? 2 : 1;
   static constexpr int kTmemCols = kAccCols * kAccBufs < 32 ? 32 : kAccCols * kAccBufs;
   static constexpr int kBox = NT >= 128 ? 64 : 16;       // columns of X that one copy brings
-  static constexpr int kCumOff = kStages * kStage, kBarOff = kCumOff + 4 * (kMaxRuns + 8);
+  static constexpr int kTableOff = kStages * kStage, kBarOff = kTableOff + kTableBytes;
   static constexpr int kSmem = kBarOff + 512 + 1024;
 };
 static_assert(Cfg<2, 256>::kStages == 3 && Cfg<1, 256>::kStages == 4 && Cfg<1, 32>::kStages == 10, "ring depth");
@@ -115,9 +121,9 @@ __device__ __forceinline__ int tile_count(int n) {
   return (n + w - 1) / w;
 }
 
-// cum[i]: column tiles of the runs before run i (runs of one length need no table).  By the whole block.
+// Fills the table (runs of one length need none).  By the whole block.
 template <int NT>
-__device__ void count_tiles(const FwdArgs& g, int* cum, RunSearch& s) {
+__device__ void count_tiles(const FwdArgs& g, Table& tab, RunSearch& s) {
   if (!g.runs.offsets) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int carry = 0;
@@ -125,8 +131,10 @@ __device__ void count_tiles(const FwdArgs& g, int* cum, RunSearch& s) {
     const int i = i0 + (int)threadIdx.x;
     int own = 0;
     if (i < g.G) {
-      const int mat = g.ids ? g.ids[i] : i;
-      if (mat >= 0 && mat < g.mats) own = tile_count<NT>(g.runs.end(i) - g.runs.begin(i));
+      const int mat = g.ids ? g.ids[i] : i, begin = g.runs.begin(i), end = g.runs.end(i);
+      if (mat >= 0 && mat < g.mats) own = tile_count<NT>(end - begin);
+      tab.begin[i] = begin;
+      tab.end[i] = end;
     }
     int sum = own;
 #pragma unroll
@@ -141,11 +149,11 @@ __device__ void count_tiles(const FwdArgs& g, int* cum, RunSearch& s) {
       if (q < warp) before += s.part[q];
       all += s.part[q];
     }
-    if (i < g.G) cum[i] = before + sum - own;
+    if (i < g.G) tab.cum[i] = before + sum - own;
     carry = all;
     __syncthreads();
   }
-  if (threadIdx.x == 0) cum[g.G] = carry;
+  if (threadIdx.x == 0) tab.cum[g.G] = carry;
   __syncthreads();
 }
 
@@ -161,26 +169,35 @@ struct Ring {
 struct Tile {
   int run, mat, n0, nt, m0, kb0, kb1, split;
 };
-// Tile number t of this CTA's growing sequence; `run` is where the last one was.
 template <int MH, int NT>
-__device__ __forceinline__ Tile tile_of(const FwdArgs& g, const int* cum, long long t, int nkb, int& run) {
+__device__ __forceinline__ Tile tile_of(const FwdArgs& g, const Table& tab, long long t, int nkb) {
   Tile o;
   o.split = (int)(t % g.splits);
   const long long q = t / g.splits;
-  int tiles;
+  int tiles, run, begin, end;
   long long at;
   if (g.runs.offsets) {
-    while ((long long)cum[run + 1] * g.tiles_m <= q) ++run;
-    tiles = cum[run + 1] - cum[run];
-    at = q - (long long)cum[run] * g.tiles_m;
+    const int col = (int)(q / g.tiles_m);                  // the last run with cum[run] <= col
+    int lo = 0, hi = g.G;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (tab.cum[mid] <= col) lo = mid; else hi = mid;
+    }
+    run = lo;
+    tiles = tab.cum[run + 1] - tab.cum[run];
+    at = q - (long long)tab.cum[run] * g.tiles_m;
+    begin = tab.begin[run];
+    end = tab.end[run];
   } else {
     tiles = tile_count<NT>((int)g.runs.len);
     run = (int)(q / ((long long)tiles * g.tiles_m));
     at = q - (long long)run * tiles * g.tiles_m;
+    begin = g.runs.begin(run);
+    end = g.runs.end(run);
   }
   // bands of kAhead column tiles: what runs at the same time shares the matrix's rows and the columns
   const int band = (int)(at / (kAhead * g.tiles_m)), in = (int)(at - (long long)band * kAhead * g.tiles_m), wide = min(kAhead, tiles - band * kAhead);
-  const int begin = g.runs.begin(run), end = g.runs.end(run), w = tile_width<NT>(end - begin);
+  const int w = tile_width<NT>(end - begin);
   o.run = run;
   o.mat = g.ids ? g.ids[run] : run;
   o.m0 = (in / wide) * (MH * 128);
@@ -226,7 +243,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  int* cum = reinterpret_cast<int*>(smem + C::kCumOff);
+  Table& tab = *reinterpret_cast<Table*>(smem + C::kTableOff);
   Bars* bars = reinterpret_cast<Bars*>(smem + C::kBarOff);
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -248,13 +265,13 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     tmem_alloc(&bars->tmem_base, C::kTmemCols);
     tmem_relinquish();
   }
-  count_tiles<NT>(g, cum, bars->search);
+  count_tiles<NT>(g, tab, bars->search);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
   const bool start_ok = (*abort_flag == 0);
-  const long long columns = g.runs.offsets ? cum[g.G] : (long long)g.G * tile_count<NT>((int)g.runs.len);
+  const long long columns = g.runs.offsets ? tab.cum[g.G] : (long long)g.G * tile_count<NT>((int)g.runs.len);
   const long long tiles = columns * g.tiles_m * g.splits;
 
   if (start_ok && (warp == 0 || warp >= 10)) {
@@ -266,7 +283,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     }
     bool ok = true;
     Ring<C::kStages> at;
-    int run = 0, turn = 0;
+    int turn = 0;
     // One stage, if it is this warp's turn: the boxes of the matrix (map ma, block ka of matrix za) and of the columns (map mx, block kx).  Lane 0 issues them all;
     // gathered columns are the other lanes' too, four each.
     auto fill = [&](const CUtensorMap* ma, int ka, int za, bool kmaj, const CUtensorMap* mx, int kx, const Tile& o, bool gather, const int4& four) {
@@ -306,7 +323,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     // (all lanes stay together where columns are gathered; elsewhere the others have nothing to do)
     if (g.gather || lane == 0) {
       for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-        const Tile o = tile_of<MH, NT>(g, cum, t, nkb, run);
+        const Tile o = tile_of<MH, NT>(g, tab, t, nkb);
         if (o.nt <= 0) continue;
         int4 four = make_int4(0, 0, 0, 0);
         if (g.gather) {
@@ -341,10 +358,10 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     // -------------------------------------------------------------- MMA issuer
     bool ok = true;
     Ring<C::kStages> at;
-    int ti = 0, run = 0;
+    int ti = 0;
     const uint32_t base = desc_lo(smem_u32(smem));
     for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const Tile o = tile_of<MH, NT>(g, cum, t, nkb, run);
+      const Tile o = tile_of<MH, NT>(g, tab, t, nkb);
       if (o.nt <= 0) continue;
       const int ab = ti % C::kAccBufs;
       const uint32_t acc = tmem + ab * C::kAccCols;
@@ -418,9 +435,9 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     const int wq = warp & 3, part = (warp - 2) >> 2;       // TMEM lane quarter; MH = 2: half of the rows, 1: every other 32 columns
     constexpr int kStep = MH == 2 ? 1 : 2;
     bool ok = true;
-    int ti = 0, run = 0;
+    int ti = 0;
     for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const Tile o = tile_of<MH, NT>(g, cum, t, nkb, run);
+      const Tile o = tile_of<MH, NT>(g, tab, t, nkb);
       if (o.nt <= 0) continue;
       const int ab = ti % C::kAccBufs;
       ok = mbar_wait_warp(&bars->acc_full[ab], (uint32_t)(ti / C::kAccBufs) & 1u, abort_flag);
@@ -497,7 +514,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     }
     if (g.zero_rest && ok) {
       // columns in no run
-      const int first = g.G > 0 ? g.runs.at(0) : g.runs.R, last = g.G > 0 ? g.runs.at(g.G) : g.runs.R;
+      const int first = tab.begin[0], last = g.runs.at(g.G);
       const int rest = first + g.runs.R - last;
       for (int i = blockIdx.x * 8 + warp - 2; i < rest; i += gridDim.x * 8) {
         T* out = reinterpret_cast<T*>(g.C) + (long long)(i < first ? i : last + i - first) * g.ldc;
