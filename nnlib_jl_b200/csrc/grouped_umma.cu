@@ -235,6 +235,50 @@ struct Pairs {
 // K blocks that a pair adds: rank up to 32: both terms of T in one; above: the first terms' blocks, then the second ones'
 __device__ __forceinline__ int low_blocks(int r) { return r <= 32 ? 1 : 2 * ((r + 63) / 64); }
 
+// 32 columns of row m (32 neighbouring rows to a warp) to a column-major array: out + column * ld + row.  `pairs`: an even number of rows
+// at 4-byte addresses, two lanes exchange halves: the even one has a column of rows m, m + 1, the odd one the next column.  Nothing
+// but predicates between the stores: with a branch for each a tile of 256 x 256 took 17000 cycles to write.
+template <bool BF16>
+__device__ __forceinline__ void store_columns(const uint32_t (&acc)[32], void* out_, long long ld, int m, int rows, int nc, bool pairs, uint32_t valid) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  T* out = reinterpret_cast<T*>(out_);
+  const bool odd = threadIdx.x & 1;
+  uint32_t v[16];
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    float lo = __uint_as_float(acc[j]), hi = __uint_as_float(acc[j + 1]);
+    if (valid != 0xffffffffu) {
+      if (!((valid >> j) & 1u)) lo = 0.f;
+      if (!((valid >> (j + 1)) & 1u)) hi = 0.f;
+    }
+    v[j / 2] = pack2<BF16>(lo, hi);
+  }
+  if (pairs) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, v[j], 1);
+      v[j] = odd ? __byte_perm(other, v[j], 0x7632) : __byte_perm(v[j], other, 0x5410);
+    }
+    if (m < rows) {
+      T* dst = out + (m & ~1) + (odd ? ld : 0);
+      if (nc >= 32) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j, dst += 2 * ld) *reinterpret_cast<uint32_t*>(dst) = v[j];
+      } else {
+        const int last = nc - (odd ? 1 : 0);
+#pragma unroll
+        for (int j = 0; j < 16; ++j, dst += 2 * ld)
+          if (2 * j < last) *reinterpret_cast<uint32_t*>(dst) = v[j];
+      }
+    }
+  } else if (m < rows) {
+    unsigned short* dst = reinterpret_cast<unsigned short*>(out) + m;
+#pragma unroll
+    for (int j = 0; j < 32; ++j, dst += ld)
+      if (j < nc) *dst = (unsigned short)(v[j / 2] >> (j & 1 ? 16 : 0));
+  }
+}
+
 template <bool BF16, int MH, int NT>
 __global__ void __launch_bounds__(kThreads, 1)
 grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_b,
@@ -460,30 +504,8 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         const int nc = min(32, o.nt - c * 32), n = o.n0 + c * 32;
         if (g.to == kToC) {
           uint32_t valid = 0xffffffffu;
-          if (g.columns) valid = __ballot_sync(0xffffffffu, lane < nc && (unsigned)g.columns[n + min(lane, nc - 1)] < (unsigned)g.N);
-          T* out = reinterpret_cast<T*>(g.C) + (long long)n * g.ldc;
-          if (g.pairs) {
-            const int mp = m & ~1;
-            const bool odd = lane & 1;
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              const uint32_t mine = pack2<BF16>(__uint_as_float(acc[j]), __uint_as_float(acc[j + 1]));
-              const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
-              // even lane: column j of rows m, m + 1; odd lane: column j + 1 of rows m - 1, m
-              uint32_t v = odd ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
-              const int col = j + (odd ? 1 : 0);
-              if (col < nc && mp < g.M) {
-                if (!((valid >> col) & 1u)) v = 0u;
-                T* dst = out + (long long)col * g.ldc + mp;
-                if (mp + 1 < g.M) *reinterpret_cast<uint32_t*>(dst) = v;
-                else *reinterpret_cast<unsigned short*>(dst) = (unsigned short)v;
-              }
-            }
-          } else if (m < g.M) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j < nc) out[(long long)j * g.ldc + m] = Elem<T>::from_f(((valid >> j) & 1u) ? __uint_as_float(acc[j]) : 0.f);
-          }
+          if (g.columns) valid = __ballot_sync(0xffffffffu, lane >= nc || (unsigned)g.columns[n + min(lane, nc - 1)] < (unsigned)g.N);
+          store_columns<BF16>(acc, reinterpret_cast<T*>(g.C) + (long long)n * g.ldc, g.ldc, m, g.M, nc, g.pairs != 0, valid);
         } else if (g.to == kToParts) {
           float* out = reinterpret_cast<float*>(g.C) + ((long long)o.split * g.runs.R + n) * g.M + m;
           if (m < g.M) {
@@ -725,27 +747,7 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
           }
           continue;
         }
-        T* out = base + (long long)n * g.ld;
-        if (g.pairs) {
-          const int mp = m & ~1;
-          const bool odd = lane & 1;
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const uint32_t mine = pack2<BF16>(__uint_as_float(acc[j]), __uint_as_float(acc[j + 1]));
-            const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
-            const uint32_t v = odd ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
-            const int col = j + (odd ? 1 : 0);
-            if (col < nc && mp < g.rows) {
-              T* dst = out + (long long)col * g.ld + mp;
-              if (mp + 1 < g.rows) *reinterpret_cast<uint32_t*>(dst) = v;
-              else *reinterpret_cast<unsigned short*>(dst) = (unsigned short)v;
-            }
-          }
-        } else if (m < g.rows) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (j < nc) out[(long long)j * g.ld + m] = Elem<T>::from_f(__uint_as_float(acc[j]));
-        }
+        store_columns<BF16>(acc, base + (long long)n * g.ld, g.ld, m, g.rows, nc, g.pairs != 0, 0xffffffffu);
       }
       if (MH == 1 && part >= chunks) {
         tc_fence_before();
@@ -977,7 +979,7 @@ cudaError_t grouped_umma(const GroupedArgs& g, int dtype, bool to_low, void* wor
   f.zero_rest = g.zero_rest;
   f.splits = 1;
   f.to = to_low ? kToLow : kToC;
-  f.pairs = (reinterpret_cast<uintptr_t>(g.C) & 3u) == 0 && g.ldc % 2 == 0;
+  f.pairs = (reinterpret_cast<uintptr_t>(g.C) & 3u) == 0 && g.ldc % 2 == 0 && g.M % 2 == 0;
   f.low_width = low_width(g.M);
   f.low_step = f.low_width / 2;
   f.status = g.status;
@@ -1028,7 +1030,7 @@ cudaError_t grouped_umma_grad(const GroupedGradArgs& g, int dtype, int fold, voi
   a.fold = fold != 0;
   a.fold_step = fold ? low_width(a.cols) / 2 : 0;
   a.along = fold && (fold == 1) == (g.transA == 0);
-  a.pairs = (reinterpret_cast<uintptr_t>(g.A) & 3u) == 0 && g.lda % 2 == 0 && g.strideA % 2 == 0;
+  a.pairs = (reinterpret_cast<uintptr_t>(g.A) & 3u) == 0 && g.lda % 2 == 0 && g.strideA % 2 == 0 && a.rows % 2 == 0;
   const int nt = fold ? low_width(a.cols) : 256;
   // 256 rows where the runs are long enough to hide an epilogue that nothing overlaps with
   const int mh = !fold && a.rows > 128 && g.R / std::max(1, g.mats) > 1024 ? 2 : 1;
