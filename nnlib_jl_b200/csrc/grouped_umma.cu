@@ -20,6 +20,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 
 #include "common.cuh"
@@ -82,6 +83,7 @@ struct FwdArgs {
   const float* scale;
   float scale0;
   int M, K, G, N, mats;
+  int cap;                               // columns of a tile, at most NT
   int a_kmaj, a_same, zero_rest, splits, tiles_m, to, pairs, gather;
   int low_width, low_step;               // kToLow: elements of T for a column, from the first term to the second
   Runs low_runs;                         // kToC: low-rank pairs, r = 0: none
@@ -109,20 +111,17 @@ __device__ __forceinline__ uint32_t idesc_of(bool bf16, int n, bool a_mn, bool b
 }
 __device__ __forceinline__ int round16(int n) { return (n + 15) & ~15; }
 
-// tiles of a run of n columns, and their width: as even as multiples of 16 allow
-template <int NT>
-__device__ __forceinline__ int tile_width(int n) {
-  const int c = (n + NT - 1) / NT;
-  return c > 0 ? round16((n + c - 1) / c) : 16;
+// Width of the tiles of a run of n columns, and their number: at most cap (a multiple of 16) and as even as multiples of 16 allow.
+__host__ __device__ __forceinline__ int tile_width(int n, int cap) {
+  const int c = (n + cap - 1) / cap;
+  return c > 0 ? ((n + c - 1) / c + 15) & ~15 : 16;
 }
-template <int NT>
-__device__ __forceinline__ int tile_count(int n) {
-  const int w = tile_width<NT>(n);
+__host__ __device__ __forceinline__ int tile_count(int n, int cap) {
+  const int w = tile_width(n, cap);
   return (n + w - 1) / w;
 }
 
 // Fills the table (runs of one length need none).  By the whole block.
-template <int NT>
 __device__ void count_tiles(const FwdArgs& g, Table& tab, RunSearch& s) {
   if (!g.runs.offsets) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -132,7 +131,7 @@ __device__ void count_tiles(const FwdArgs& g, Table& tab, RunSearch& s) {
     int own = 0;
     if (i < g.G) {
       const int mat = g.ids ? g.ids[i] : i, begin = g.runs.begin(i), end = g.runs.end(i);
-      if (mat >= 0 && mat < g.mats) own = tile_count<NT>(end - begin);
+      if (mat >= 0 && mat < g.mats) own = tile_count(end - begin, g.cap);
       tab.begin[i] = begin;
       tab.end[i] = end;
     }
@@ -169,7 +168,7 @@ struct Ring {
 struct Tile {
   int run, mat, n0, nt, m0, kb0, kb1, split;
 };
-template <int MH, int NT>
+template <int MH>
 __device__ __forceinline__ Tile tile_of(const FwdArgs& g, const Table& tab, long long t, int nkb) {
   Tile o;
   o.split = (int)(t % g.splits);
@@ -189,7 +188,7 @@ __device__ __forceinline__ Tile tile_of(const FwdArgs& g, const Table& tab, long
     begin = tab.begin[run];
     end = tab.end[run];
   } else {
-    tiles = tile_count<NT>((int)g.runs.len);
+    tiles = tile_count((int)g.runs.len, g.cap);
     run = (int)(q / ((long long)tiles * g.tiles_m));
     at = q - (long long)run * tiles * g.tiles_m;
     begin = g.runs.begin(run);
@@ -197,7 +196,7 @@ __device__ __forceinline__ Tile tile_of(const FwdArgs& g, const Table& tab, long
   }
   // bands of kAhead column tiles: what runs at the same time shares the matrix's rows and the columns
   const int band = (int)(at / (kAhead * g.tiles_m)), in = (int)(at - (long long)band * kAhead * g.tiles_m), wide = min(kAhead, tiles - band * kAhead);
-  const int w = tile_width<NT>(end - begin);
+  const int w = tile_width(end - begin, g.cap);
   o.run = run;
   o.mat = g.ids ? g.ids[run] : run;
   o.m0 = (in / wide) * (MH * 128);
@@ -309,13 +308,13 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     tmem_alloc(&bars->tmem_base, C::kTmemCols);
     tmem_relinquish();
   }
-  count_tiles<NT>(g, tab, bars->search);
+  count_tiles(g, tab, bars->search);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
   const bool start_ok = (*abort_flag == 0);
-  const long long columns = g.runs.offsets ? tab.cum[g.G] : (long long)g.G * tile_count<NT>((int)g.runs.len);
+  const long long columns = g.runs.offsets ? tab.cum[g.G] : (long long)g.G * tile_count((int)g.runs.len, g.cap);
   const long long tiles = columns * g.tiles_m * g.splits;
 
   if (start_ok && (warp == 0 || warp >= 10)) {
@@ -367,7 +366,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     // (all lanes stay together where columns are gathered; elsewhere the others have nothing to do)
     if (g.gather || lane == 0) {
       for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-        const Tile o = tile_of<MH, NT>(g, tab, t, nkb);
+        const Tile o = tile_of<MH>(g, tab, t, nkb);
         if (o.nt <= 0) continue;
         int4 four = make_int4(0, 0, 0, 0);
         if (g.gather) {
@@ -405,7 +404,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     int ti = 0;
     const uint32_t base = desc_lo(smem_u32(smem));
     for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const Tile o = tile_of<MH, NT>(g, tab, t, nkb);
+      const Tile o = tile_of<MH>(g, tab, t, nkb);
       if (o.nt <= 0) continue;
       const int ab = ti % C::kAccBufs;
       const uint32_t acc = tmem + ab * C::kAccCols;
@@ -481,9 +480,16 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     bool ok = true;
     int ti = 0;
     for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const Tile o = tile_of<MH, NT>(g, tab, t, nkb);
+      const Tile o = tile_of<MH>(g, tab, t, nkb);
       if (o.nt <= 0) continue;
       const int ab = ti % C::kAccBufs;
+      uint32_t none[NT / 32];                              // columns whose column of X does not exist, a bit each
+#pragma unroll
+      for (int c = 0; c < NT / 32; ++c) {
+        none[c] = 0u;
+        if (g.columns && c * 32 < o.nt)
+          none[c] = __ballot_sync(0xffffffffu, c * 32 + lane < o.nt && (unsigned)g.columns[o.n0 + min(c * 32 + lane, o.nt - 1)] >= (unsigned)g.N);
+      }
       ok = mbar_wait_warp(&bars->acc_full[ab], (uint32_t)(ti / C::kAccBufs) & 1u, abort_flag);
       if (!ok) break;
       tc_fence_after();
@@ -503,9 +509,11 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         }
         const int nc = min(32, o.nt - c * 32), n = o.n0 + c * 32;
         if (g.to == kToC) {
-          uint32_t valid = 0xffffffffu;
-          if (g.columns) valid = __ballot_sync(0xffffffffu, lane >= nc || (unsigned)g.columns[n + min(lane, nc - 1)] < (unsigned)g.N);
-          store_columns<BF16>(acc, reinterpret_cast<T*>(g.C) + (long long)n * g.ldc, g.ldc, m, g.M, nc, g.pairs != 0, valid);
+          uint32_t gone = 0u;
+#pragma unroll
+          for (int q = 0; q < NT / 32; ++q)
+            if (q == c) gone = none[q];
+          store_columns<BF16>(acc, reinterpret_cast<T*>(g.C) + (long long)n * g.ldc, g.ldc, m, g.M, nc, g.pairs != 0, ~gone);
         } else if (g.to == kToParts) {
           float* out = reinterpret_cast<float*>(g.C) + ((long long)o.split * g.runs.R + n) * g.M + m;
           if (m < g.M) {
@@ -896,34 +904,46 @@ cudaError_t launch_bwd(const CUtensorMap& r, const CUtensorMap& c, GradArgs g, c
   return cudaGetLastError();
 }
 
+// Rows and columns of a tile.
 struct Shape {
-  int mh, nt;
+  int mh, cap;
   long long most;                        // column tiles that there can be
+  int nt() const { return cap > 128 ? 256 : cap > 64 ? 128 : cap > 32 ? 64 : 32; }
 };
-// Rows and columns of a tile.  As many columns as the average run has (a tile is cut to a multiple of 16 at run time, so that
-// too wide a tile costs ring depth only); 256 rows where K is long enough to hide an epilogue that nothing overlaps with, and where
-// that still leaves every SM a tile.
 Shape shape_of(int M, int K, int R, int runs) {
-  const long long each = R / std::max(1, runs);
-  Shape s;
-  s.mh = 1;
-  s.nt = each > 128 ? 256 : each > 64 ? 128 : each > 32 ? 64 : 32;
-  auto most = [&](int nt) { return (long long)R / nt + std::min(R, runs) + 1; };
-  while (s.nt > 32 && most(s.nt) * ((M + 127) / 128) < 120) s.nt /= 2;
-  if (s.nt == 256 && M > 128 && K > 512 && (R / 256) * ((M + 255) / 256) >= 148) s.mh = 2;
-  s.most = most(s.nt);
-  return s;
+  const int sms = 148, each = std::max(1, (R + runs - 1) / std::max(1, runs)), nkb = (K + kBK - 1) / kBK;
+  Shape best{1, 32, 0};
+  double least = 1e300;
+  for (int mh = 1; mh <= 2; ++mh) {
+    if (mh == 2 && M <= 128) break;
+    for (int cap = mh == 2 ? 144 : 16; cap <= 256; cap += 16) {
+      const int w = tile_width(each, cap);
+      if (w != cap && cap != 256) continue;            // the same tiles as a smaller cap's
+      const double tiles = (double)tile_count(each, cap) * std::min(runs, R) * ((M + 128 * mh - 1) / (128 * mh)) / sms;
+      const double waves = runs == 1 ? std::ceil(tiles) : std::max(1.0, tiles + 0.5);
+      const double block = std::max(4.0 * mh * std::max(90, w / 2) + 100, (16384.0 * mh + 128.0 * w) / 64);
+      const double end = 3000 + (mh == 2 ? 8000.0 * w / 256 : 0);
+      const double cost = waves * (nkb * block + end);
+      if (cost < least) {
+        least = cost;
+        best.mh = mh;
+        best.cap = cap;
+      }
+    }
+  }
+  best.most = (long long)R / best.cap + std::min(R, runs) + 1;
+  return best;
 }
 
 template <bool BF16>
 cudaError_t fwd(const Shape& s, const CUtensorMap& a, const CUtensorMap& x, const CUtensorMap& b, const CUtensorMap& t, const FwdArgs& g, cudaStream_t st) {
   if (s.mh == 2) return launch_fwd<BF16, 2, 256>(a, x, b, t, g, s.most, st);
-  if (s.nt == 256) return launch_fwd<BF16, 1, 256>(a, x, b, t, g, s.most, st);
-  if (s.nt == 128) return launch_fwd<BF16, 1, 128>(a, x, b, t, g, s.most, st);
-  if (s.nt == 64) return launch_fwd<BF16, 1, 64>(a, x, b, t, g, s.most, st);
+  if (s.nt() == 256) return launch_fwd<BF16, 1, 256>(a, x, b, t, g, s.most, st);
+  if (s.nt() == 128) return launch_fwd<BF16, 1, 128>(a, x, b, t, g, s.most, st);
+  if (s.nt() == 64) return launch_fwd<BF16, 1, 64>(a, x, b, t, g, s.most, st);
   return launch_fwd<BF16, 1, 32>(a, x, b, t, g, s.most, st);
 }
-int box_of(const Shape& s) { return s.nt >= 128 ? 64 : 16; }
+int box_of(const Shape& s) { return s.nt() >= 128 ? 64 : 16; }
 
 Operand matrices(const void* p, bool trans, int M, int K, long long ld, long long stride, int count) {
   return trans ? Operand{p, K, M, ld, stride, count, nullptr, 0} : Operand{p, M, K, ld, stride, count, nullptr, 0};
@@ -935,7 +955,7 @@ Operand columns_of(const void* X, int K, int N, long long ld, const int* columns
 // Whether the copy engine gathers: it takes some 65 cycles for every four columns and 64 features, for each tile of rows anew, so
 // only while all columns are few; a copy of them, gathered once, costs a launch (8192 tokens twice, 14336 x 4096: 4.5 ms, 1.5 with the copy).
 bool gathers_in_place(const Operand& x, const Shape& s) {
-  return s.nt <= 32 && Operand{x.p, x.wide, x.deep, x.ld, x.stride, x.count, nullptr, 0}.fits();
+  return s.nt() <= 32 && Operand{x.p, x.wide, x.deep, x.ld, x.stride, x.count, nullptr, 0}.fits();
 }
 
 }  // namespace
@@ -969,6 +989,7 @@ cudaError_t grouped_umma(const GroupedArgs& g, int dtype, bool to_low, void* wor
   f.ids = g.ids;
   f.columns = g.columns;
   f.gather = in_place;
+  f.cap = s.cap;
   f.C = g.C;
   f.ldc = g.ldc;
   f.scale = g.scale;
