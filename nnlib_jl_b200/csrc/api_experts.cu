@@ -231,23 +231,25 @@ bool adapter_on_umma(const Adapters& a, int dtype) {
 }
 bool has_pairs(const Adapters& a) { return a.first.G > 0 && a.first.mats > 0 && a.first.K > 0; }
 size_t low_bytes(const Adapters& a, bool umma) {
-  return round256((size_t)a.first.R * (umma ? 2 * (size_t)low_width(a.first.M) : 4 * (size_t)a.first.M));
+  return umma ? low_umma_bytes(a.first) : round256((size_t)a.first.R * 4 * (size_t)a.first.M);
 }
-// A X (or B^T dC) into `low`, then the product that adds B times it (A^T times it); `ws`: for both
-cudaError_t adapter_products(Adapters& a, int dtype, bool umma, void* low, void* ws, cudaStream_t st) {
+// A X (or B^T dC) into `low`, then the product that adds B times it (A^T times it); `ws`: adapter_ws() bytes.  keep: `low` is read behind it.
+cudaError_t adapter_products(Adapters& a, int dtype, bool umma, bool keep, void* low, void* ws, cudaStream_t st) {
+  if (!has_pairs(a)) a.main.low.r = 0;
+  if (umma) return adapter_umma(a.first, a.main, dtype, keep, low, ws, st);
   a.first.C = low;
   a.first.ldc = a.first.M;
   a.main.low.T = low;
-  a.main.low.ldt = umma ? low_width(a.first.M) : a.first.M;
-  if (!has_pairs(a)) a.main.low.r = 0;
+  a.main.low.ldt = a.first.M;
   if (has_pairs(a)) {
-    const cudaError_t e = umma ? grouped_umma(a.first, dtype, true, ws, st) : grouped_fma(a.first, dtype, true, st);
+    const cudaError_t e = grouped_fma(a.first, dtype, true, st);
     if (e != cudaSuccess) return e;
   }
-  return umma ? grouped_umma(a.main, dtype, false, ws, st) : grouped_fma(a.main, dtype, false, st);
+  return grouped_fma(a.main, dtype, false, st);
 }
-size_t adapter_ws(const Adapters& a, bool umma) {
-  return umma ? std::max(grouped_umma_workspace_bytes(a.first), grouped_umma_workspace_bytes(a.main)) : 0;
+size_t adapter_ws(Adapters& a, bool umma, bool keep) {
+  if (!has_pairs(a)) a.main.low.r = 0;
+  return umma ? adapter_umma_workspace_bytes(a.first, a.main, keep) : 0;
 }
 
 // Gradients of the pairs: dA = (scale B^T dC) X^T, dB = dC (scale A X)^T.  `other`: A X for them.
@@ -319,7 +321,7 @@ int nnlib_b200_grouped_gemm(const nnlib_b200_grouped_params* p, void* workspace,
   if ((rc = check_grouped_arrays(a))) return rc;
   if (log_calls())
     std::fprintf(stderr, "[nnlib_b200] grouped_gemm M=%d K=%d G=%d N=%d R=%d -> %s\n", a.M, a.K, a.G, a.N, a.R, umma ? "tcgen05" : "cuda-core");
-  return finish(umma ? grouped_umma(a, p->dtype, false, workspace, (cudaStream_t)stream) : grouped_fma(a, p->dtype, false, (cudaStream_t)stream));
+  return finish(umma ? grouped_umma(a, p->dtype, workspace, (cudaStream_t)stream) : grouped_fma(a, p->dtype, false, (cudaStream_t)stream));
 }
 size_t nnlib_b200_grouped_gemm_grad_workspace_bytes(const nnlib_b200_grouped_params* p) {
   GroupedArgs a;
@@ -360,7 +362,7 @@ size_t nnlib_b200_adapter_gemm_workspace_bytes(const nnlib_b200_adapter_params* 
   Adapters a;
   if (resolve_adapter(p, false, &a)) return 0;
   const bool umma = adapter_on_umma(a, p->dtype);
-  return low_bytes(a, umma) + adapter_ws(a, umma);
+  return low_bytes(a, umma) + adapter_ws(a, umma, false);
 }
 int nnlib_b200_adapter_gemm(const nnlib_b200_adapter_params* p, void* workspace, size_t workspace_bytes, void* stream) {
   Adapters a;
@@ -368,22 +370,22 @@ int nnlib_b200_adapter_gemm(const nnlib_b200_adapter_params* p, void* workspace,
   if (rc || a.main.M == 0 || a.main.N == 0) return rc;
   const bool umma = adapter_on_umma(a, p->dtype);
   const size_t low = low_bytes(a, umma);
-  if ((rc = workspace_ok(workspace, workspace_bytes, low + adapter_ws(a, umma)))) return rc;
+  if ((rc = workspace_ok(workspace, workspace_bytes, low + adapter_ws(a, umma, false)))) return rc;
   const void* all[] = {p->C, p->X, p->W, p->A, p->B, p->offsets, p->ids, p->scale, p->status};
   if ((rc = check_arrays(all, 2, 9))) return rc;
   if (log_calls())
     std::fprintf(stderr, "[nnlib_b200] adapter_gemm M=%d K=%d N=%d r=%d runs=%d -> %s\n", a.main.M, a.main.K, a.main.N, a.first.M, a.first.G,
                  umma ? "tcgen05" : "cuda-core");
-  return finish(adapter_products(a, p->dtype, umma, workspace, static_cast<char*>(workspace) + low, (cudaStream_t)stream));
+  return finish(adapter_products(a, p->dtype, umma, false, workspace, static_cast<char*>(workspace) + low, (cudaStream_t)stream));
 }
 size_t nnlib_b200_adapter_bwd_workspace_bytes(const nnlib_b200_adapter_params* p) {
   Adapters a;
   if (resolve_adapter(p, true, &a)) return 0;
   const bool umma = adapter_on_umma(a, p->dtype);
-  size_t rest = adapter_ws(a, umma);
+  size_t rest = adapter_ws(a, umma, true);
   if (umma && p->dA) {
     const PairGrads g = pair_grads(p, a, true);
-    rest = std::max({rest, grouped_umma_workspace_bytes(g.first), grouped_umma_grad_workspace_bytes(g.a, 1), grouped_umma_grad_workspace_bytes(g.b, 2)});
+    rest = std::max({rest, low_umma_workspace_bytes(g.first), grouped_umma_grad_workspace_bytes(g.a, 1), grouped_umma_grad_workspace_bytes(g.b, 2)});
   }
   return 2 * low_bytes(a, umma) + rest;
 }
@@ -400,7 +402,7 @@ int nnlib_b200_adapter_bwd(const nnlib_b200_adapter_params* p, void* workspace, 
   char* of_dC = static_cast<char*>(workspace);             // scale * B^T dC
   char* of_X = of_dC + low;                                // scale * A X
   char* ws = of_X + low;
-  if ((rc = finish(adapter_products(a, p->dtype, umma, of_dC, ws, st)))) return rc;
+  if ((rc = finish(adapter_products(a, p->dtype, umma, true, of_dC, ws, st)))) return rc;
   if (!p->dA || !p->dB || a.first.mats == 0) return NNLIB_B200_OK;
   PairGrads g = pair_grads(p, a, umma);
   g.first.C = of_X;
@@ -411,7 +413,7 @@ int nnlib_b200_adapter_bwd(const nnlib_b200_adapter_params* p, void* workspace, 
     if ((rc = finish(grouped_fma_grad(g.a, p->dtype, true, false, st)))) return rc;
     return finish(grouped_fma_grad(g.b, p->dtype, false, true, st));
   }
-  if (has_pairs(a) && (rc = finish(grouped_umma(g.first, p->dtype, true, ws, st)))) return rc;
+  if (has_pairs(a) && (rc = finish(low_umma(g.first, p->dtype, of_X, ws, st)))) return rc;
   if ((rc = finish(grouped_umma_grad(g.a, p->dtype, 1, ws, st)))) return rc;
   return finish(grouped_umma_grad(g.b, p->dtype, 2, ws, st));
 }

@@ -278,6 +278,33 @@ __device__ __forceinline__ void store_columns(const uint32_t (&acc)[32], void* o
   }
 }
 
+// Chunks of 32 columns from..to, every STEP-th, of this warp's rows of an accumulator through put(values, chunk): the next chunk is on
+// its way out of tensor memory while one is put.  Then the accumulator is free as far as this warp goes.
+template <int STEP, typename F>
+__device__ __forceinline__ void drain_columns(uint32_t taddr, int c, int chunks, uint64_t* empty, F put) {
+  uint32_t a[32], b[32];
+  auto free = [&] {
+    tc_fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(empty);
+  };
+  if (c >= chunks) {
+    free();
+    return;
+  }
+  tmem_ld32(taddr + c * 32, a);
+  while (true) {
+    tmem_wait_ld();
+    if (c + STEP < chunks) tmem_ld32(taddr + (c + STEP) * 32, b); else free();
+    put(a, c);
+    if ((c += STEP) >= chunks) break;
+    tmem_wait_ld();
+    if (c + STEP < chunks) tmem_ld32(taddr + (c + STEP) * 32, a); else free();
+    put(b, c);
+    if ((c += STEP) >= chunks) break;
+  }
+}
+
 template <bool BF16, int MH, int NT>
 __global__ void __launch_bounds__(kThreads, 1)
 grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_b,
@@ -343,14 +370,14 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
       if (lane == 0) {
         if (at.round > 0) good = mbar_wait(&bars->empty[s], (uint32_t)(at.round - 1) & 1u, abort_flag) ? 1 : 0;
         if (good) {
-          const int boxes = (o.nt + C::kBox - 1) / C::kBox;
-          mbar_arrive_expect_tx(&bars->full[s], C::kA + (gather ? round16(o.nt) * 128 : boxes * C::kBox * 128));
+          // (rows of shared memory behind the last row of the matrix keep what they have: no row sees another)
+          const int boxes = (o.nt + C::kBox - 1) / C::kBox, rows = min(MH * 128, g.M - o.m0);
+          const int of_a = kmaj ? (rows + 127) / 128 : (rows + 63) / 64, bytes_a = of_a * (kmaj ? kHalfBytes : kHalfBytes / 2);
+          mbar_arrive_expect_tx(&bars->full[s], bytes_a + (gather ? round16(o.nt) * 128 : boxes * C::kBox * 128));
           if (kmaj) {
-#pragma unroll
-            for (int i = 0; i < MH; ++i) tma_load_3d(da + i * kHalfBytes, ma, &bars->full[s], ka, o.m0 + i * 128, za);
+            for (int i = 0; i < of_a; ++i) tma_load_3d(da + i * kHalfBytes, ma, &bars->full[s], ka, o.m0 + i * 128, za);
           } else {
-#pragma unroll
-            for (int i = 0; i < 2 * MH; ++i) tma_load_3d(da + i * (kHalfBytes / 2), ma, &bars->full[s], o.m0 + i * 64, ka, za);
+            for (int i = 0; i < of_a; ++i) tma_load_3d(da + i * (kHalfBytes / 2), ma, &bars->full[s], o.m0 + i * 64, ka, za);
           }
           if (!gather)
             for (int i = 0; i < boxes; ++i) tma_load_2d(dx + i * C::kBox * 128, mx, &bars->full[s], kx, o.n0 + i * C::kBox);
@@ -409,6 +436,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
       const int ab = ti % C::kAccBufs;
       const uint32_t acc = tmem + ab * C::kAccCols;
       const uint32_t id_main = idesc_of(BF16, round16(o.nt), !g.a_kmaj, false);
+      const bool upper = MH == 2 && g.M - o.m0 > 128;      // the second 128 rows are there
       int good = 1;
       if (lane == 0) {
         if (ti >= C::kAccBufs) good = mbar_wait(&bars->acc_empty[ab], (uint32_t)((ti / C::kAccBufs) + 1) & 1u, abort_flag) ? 1 : 0;
@@ -425,7 +453,8 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
             if (kk < steps) {
 #pragma unroll
               for (int h = 0; h < MH; ++h)
-                umma_ss_lohi(acc + h * NT, a + h * (kHalfBytes >> 4) + kk * step, x + kk * 2, kDescHi, id_main, (kb > o.kb0 || kk > 0) ? 1u : 0u);
+                if (h == 0 || upper)
+                  umma_ss_lohi(acc + h * NT, a + h * (kHalfBytes >> 4) + kk * step, x + kk * 2, kDescHi, id_main, (kb > o.kb0 || kk > 0) ? 1u : 0u);
             }
           }
           umma_commit(&bars->empty[s]);
@@ -460,6 +489,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
               for (int kk = 0; kk < steps; ++kk) {
 #pragma unroll
                 for (int h = 0; h < MH; ++h) {
+                  if (h > 0 && !upper) continue;
                   umma_ss_lohi(acc + h * NT, a + h * (kHalfBytes >> 4) + kk * step, x + kk * 2, kDescHi, id_low, 1u);
                   if (!half) umma_ss_lohi(acc + h * NT, a + h * (kHalfBytes >> 4) + kk * step, x + kk * 2 + 4, kDescHi, id_low, 1u);
                 }
@@ -495,18 +525,10 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
       tc_fence_after();
       const int m = o.m0 + (MH == 2 ? part * 128 : 0) + wq * 32 + lane;
       const uint32_t taddr = tmem + (static_cast<uint32_t>(wq * 32) << 16) + ab * C::kAccCols + (MH == 2 ? part * NT : 0);
-      const int chunks = (o.nt + 31) / 32;
+      const int chunks = MH == 2 && part * 128 >= g.M - o.m0 ? 0 : (o.nt + 31) / 32;
       float scale = 1.f;
-      if (g.to == kToLow) scale = g.scale ? g.scale[o.mat] : g.scale0;
-      for (int c = MH == 2 ? 0 : part; c < chunks; c += kStep) {
-        uint32_t acc[32];
-        tmem_ld32(taddr + c * 32, acc);
-        tmem_wait_ld();
-        if (c + kStep >= chunks) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->acc_empty[ab]);
-        }
+      if (g.to != kToC) scale = g.scale ? g.scale[o.mat] : g.scale0;
+      auto put = [&](const uint32_t (&acc)[32], int c) {
         const int nc = min(32, o.nt - c * 32), n = o.n0 + c * 32;
         if (g.to == kToC) {
           uint32_t gone = 0u;
@@ -519,7 +541,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
           if (m < g.M) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (j < nc) out[(long long)j * g.M] = __uint_as_float(acc[j]);
+              if (j < nc) out[(long long)j * g.M] = scale * __uint_as_float(acc[j]);
           }
         } else if (m < g.low_step) {
           // T: what is left after rounding to 16 bits is the second term; zeros behind the rank
@@ -534,12 +556,8 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
             }
           }
         }
-      }
-      if (MH == 1 && part >= chunks) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->acc_empty[ab]);
-      }
+      };
+      drain_columns<kStep>(taddr, MH == 2 ? 0 : part, chunks, &bars->acc_empty[ab], put);
       ++ti;
     }
     if (g.zero_rest && ok) {
@@ -724,44 +742,37 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
       const int m = r0 + (MH == 2 ? part * 128 : 0) + wq * 32 + lane;
       const uint32_t taddr = tmem + (static_cast<uint32_t>(wq * 32) << 16) + ab * C::kAccCols + (MH == 2 ? part * NT : 0);
       T* base = reinterpret_cast<T*>(g.A) + (long long)a * g.stride;
-      const int width = g.fold ? g.fold_step : NT, chunks = width / 32;
-      for (int c = MH == 2 ? 0 : part; c < chunks; c += kStep) {
+      const int width = g.fold ? g.fold_step : min(NT, g.cols - c0), chunks = MH == 2 && part * 128 >= g.rows - r0 ? 0 : (width + 31) / 32;
+      auto put = [&](const uint32_t (&got)[32], int c) {
         uint32_t acc[32];
-        tmem_ld32(taddr + c * 32, acc);
-        if (g.fold) {
-          uint32_t more[32];
-          tmem_ld32(taddr + g.fold_step + c * 32, more);
-          tmem_wait_ld();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) acc[j] = __float_as_uint(__uint_as_float(acc[j]) + __uint_as_float(more[j]));
-        }
-        tmem_wait_ld();
-        if (c + kStep >= chunks) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->acc_empty[ab]);
-        }
-        if (!some) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) acc[j] = 0u;
-        }
+        for (int j = 0; j < 32; ++j) acc[j] = some ? got[j] : 0u;
         const int n = c0 + c * 32, nc = min(32, g.cols - n);
-        if (g.along) {
-          if (m < g.rows) {
-            T* out = base + (long long)m * g.ld + n;
+        if (!g.along) {
+          store_columns<BF16>(acc, base + (long long)n * g.ld, g.ld, m, g.rows, nc, g.pairs != 0, 0xffffffffu);
+        } else if (m < g.rows) {
+          T* out = base + (long long)m * g.ld + n;
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j < nc) out[j] = Elem<T>::from_f(__uint_as_float(acc[j]));
-          }
-          continue;
+          for (int j = 0; j < 32; ++j)
+            if (j < nc) out[j] = Elem<T>::from_f(__uint_as_float(acc[j]));
         }
-        store_columns<BF16>(acc, base + (long long)n * g.ld, g.ld, m, g.rows, nc, g.pairs != 0, 0xffffffffu);
+      };
+      if (!g.fold) {
+        drain_columns<kStep>(taddr, MH == 2 ? 0 : part, chunks, &bars->acc_empty[ab], put);
+        continue;
       }
-      if (MH == 1 && part >= chunks) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->acc_empty[ab]);
+      for (int c = part; c < chunks; c += 2) {
+        uint32_t acc[32], more[32];
+        tmem_ld32(taddr + c * 32, acc);
+        tmem_ld32(taddr + g.fold_step + c * 32, more);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) acc[j] = __float_as_uint(__uint_as_float(acc[j]) + __uint_as_float(more[j]));
+        put(acc, c);
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->acc_empty[ab]);
     }
   }
   tc_fence_before();
@@ -816,6 +827,87 @@ __global__ void __launch_bounds__(256) copy_rows_kernel(const __grid_constant__ 
       d[row * g.ld8 + i] = v;
     }
   }
+}
+
+// Parts of a product whose K was cut, added in their order: C, and for columns of low-rank pairs B T on top (few columns: a pair's
+// products are so little that they need no tensor cores).  A block takes a column and 256 rows.
+struct JoinArgs {
+  const float* parts;                    // (M, R, splits)
+  void* C;
+  long long ldc;
+  int splits, M, R, N, zero_rest;
+  Runs runs;
+  const int* columns;
+  const float* t;                        // (r, R, t_splits), r = 0: none
+  int t_splits, r, n, transB;
+  Runs low_runs;
+  const int* low_ids;
+  const void* B;
+  long long ldb, strideB;
+};
+template <typename T>
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ JoinArgs g) {
+  __shared__ float t[128];
+  __shared__ int pair;
+  const int n = blockIdx.x, m = (blockIdx.y * 128 + threadIdx.x) * 2;
+  T* out = reinterpret_cast<T*>(g.C) + (long long)n * g.ldc + m;
+  int in = 0;
+  for (int i = threadIdx.x; i < g.runs.runs; i += 128) in |= g.runs.begin(i) <= n && n < g.runs.end(i);
+  if (threadIdx.x == 0) pair = -1;
+  in = __syncthreads_or(in);
+  if (!in && !g.zero_rest) return;
+  float sum[2] = {0.f, 0.f};
+  if (in && (!g.columns || (unsigned)g.columns[n] < (unsigned)g.N)) {
+#pragma unroll 4
+    for (int s = 0; s < g.splits; ++s) {
+      const float* p = g.parts + ((long long)s * g.R + n) * g.M + m;
+      if (m < g.M) sum[0] += p[0];
+      if (m + 1 < g.M) sum[1] += p[1];
+    }
+  }
+  if (g.r > 0) {
+    for (int i = threadIdx.x; i < g.low_runs.runs; i += 128)
+      if (g.low_runs.begin(i) <= n && n < g.low_runs.end(i)) pair = g.low_ids[i];
+    __syncthreads();
+    const int id = pair;
+    if (id >= 0 && id < g.n) {
+      if (threadIdx.x < g.r) {
+        float v = 0.f;
+        for (int s = 0; s < g.t_splits; ++s) v += g.t[((long long)s * g.R + n) * g.r + threadIdx.x];
+        t[threadIdx.x] = v;
+      }
+      __syncthreads();
+      const T* B = reinterpret_cast<const T*>(g.B) + (long long)id * g.strideB;
+      const long long row = g.transB ? g.ldb : 1, col = g.transB ? 1 : g.ldb;
+      if (m < g.M) {
+        const T* b = B + m * row;
+        const bool two = m + 1 < g.M;
+#pragma unroll 8
+        for (int i = 0; i < g.r; ++i) {
+          sum[0] = fmaf(Elem<T>::to_f(b[i * col]), t[i], sum[0]);
+          if (two) sum[1] = fmaf(Elem<T>::to_f(b[row + i * col]), t[i], sum[1]);
+        }
+      }
+    }
+  }
+  if (m < g.M) out[0] = Elem<T>::from_f(sum[0]);
+  if (m + 1 < g.M) out[1] = Elem<T>::from_f(sum[1]);
+}
+// T from the parts of scale * A X: two 16-bit terms, zeros behind the rank
+template <typename T>
+__global__ void __launch_bounds__(256) join_low_kernel(const float* parts, int splits, int r, int R, T* out, int width) {
+  const int step = width / 2;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int n = (int)(i / step), c = (int)(i % step);
+  if (n >= R) return;
+  float v = 0.f;
+  if (c < r) {
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) v += parts[((long long)s * R + n) * r + c];
+  }
+  const T first = Elem<T>::from_f(v);
+  out[(long long)n * width + c] = first;
+  out[(long long)n * width + step + c] = Elem<T>::from_f(v - Elem<T>::to_f(first));
 }
 
 // A matrix (or several) that is read: where it lies, contiguous extent first.
@@ -906,31 +998,39 @@ cudaError_t launch_bwd(const CUtensorMap& r, const CUtensorMap& c, GradArgs g, c
 
 // Rows and columns of a tile.
 struct Shape {
-  int mh, cap;
+  int mh, cap, splits;
   long long most;                        // column tiles that there can be
   int nt() const { return cap > 128 ? 256 : cap > 64 ? 128 : cap > 32 ? 64 : 32; }
 };
-Shape shape_of(int M, int K, int R, int runs) {
+// The tile, and the cut of K into parts, of the fewest cycles, runs taken as equally long.  A K block costs its products (half a cycle
+// for each column, 90 at least to issue one, 128 rows each) or its copies (64 bytes a cycle), a tile of 256 x 256 the end that nothing overlaps with,
+// and K is cut (the parts are added up by another launch, 6000 cycles) only where tiles are fewer than SMs.  Measured against
+// the others at 2048 x 2048 x 8192: 256 x 224 tiles 59.5 us, 256 x 256 67.7, 128 x 256 70; 64 x 4096 by 6656 columns in 7 runs: 128 columns 31 us, 32 56.
+Shape shape_of(int M, int K, int R, int runs, bool may_split) {
   const int sms = 148, each = std::max(1, (R + runs - 1) / std::max(1, runs)), nkb = (K + kBK - 1) / kBK;
-  Shape best{1, 32, 0};
+  Shape best{1, 32, 1, 0};
   double least = 1e300;
   for (int mh = 1; mh <= 2; ++mh) {
     if (mh == 2 && M <= 128) break;
     for (int cap = mh == 2 ? 144 : 16; cap <= 256; cap += 16) {
       const int w = tile_width(each, cap);
-      if (w != cap && cap != 256) continue;            // the same tiles as a smaller cap's
+      if (w != cap) continue;                          // the same tiles as a smaller cap's
       const double tiles = (double)tile_count(each, cap) * std::min(runs, R) * ((M + 128 * mh - 1) / (128 * mh)) / sms;
-      const double waves = runs == 1 ? std::ceil(tiles) : std::max(1.0, tiles + 0.5);
       const double block = std::max(4.0 * mh * std::max(90, w / 2) + 100, (16384.0 * mh + 128.0 * w) / 64);
       const double end = 3000 + (mh == 2 ? 8000.0 * w / 256 : 0);
-      const double cost = waves * (nkb * block + end);
-      if (cost < least) {
-        least = cost;
-        best.mh = mh;
-        best.cap = cap;
+      for (int splits = 1; splits == 1 || (may_split && splits <= 8 && tiles * splits < 1.01 && nkb / splits >= 4); ++splits) {
+        const double all = tiles * splits, waves = runs == 1 ? std::ceil(all) : std::max(1.0, all + (all > 1 ? 0.5 : 0.0));
+        const double cost = waves * ((nkb + splits - 1) / splits * block + end) + (splits > 1 ? 6000 : 0);
+        if (cost < least) {
+          least = cost;
+          best.mh = mh;
+          best.cap = cap;
+          best.splits = splits;
+        }
       }
     }
   }
+  best.cap = std::max(best.cap, 32);
   best.most = (long long)R / best.cap + std::min(R, runs) + 1;
   return best;
 }
@@ -966,18 +1066,20 @@ bool grouped_umma_supports(const GroupedArgs& g, int dtype) {
   return (dtype == NNLIB_B200_F16 || dtype == NNLIB_B200_BF16) && g.M > 0 && g.K > 0 && g.N > 0 && g.R > 0 && g.G > 0 && (g.G <= kMaxRuns || !g.offsets) &&
          g.mats > 0 && encode_tiled_fn() != nullptr;
 }
-size_t grouped_umma_workspace_bytes(const GroupedArgs& g) {
+namespace {
+
+size_t copies_bytes(const GroupedArgs& g, const Shape& s) {
   const Operand a = matrices(g.A, g.transA != 0, g.M, g.K, g.lda, g.strideA, g.mats), x = columns_of(g.X, g.K, g.N, g.ldx, g.columns, g.R);
-  size_t n = padded(a.copy_bytes()) + (gathers_in_place(x, shape_of(g.M, g.K, g.R, g.G)) ? 0 : padded(x.copy_bytes()));
+  size_t n = padded(a.copy_bytes()) + (g.columns && gathers_in_place(x, s) ? 0 : padded(x.copy_bytes()));
   if (g.low.r > 0) n += padded(matrices(g.low.B, g.low.transB != 0, g.M, g.low.r, g.low.ldb, g.low.strideB, g.low.n).copy_bytes());
   return n;
 }
-// to_low: C is T of a following product, low_width(M) elements for each column
-cudaError_t grouped_umma(const GroupedArgs& g, int dtype, bool to_low, void* workspace, cudaStream_t st) {
-  char* ws = static_cast<char*>(workspace);
+size_t parts_bytes(const GroupedArgs& g, const Shape& s) { return padded((size_t)s.splits * g.R * g.M * sizeof(float)); }
+
+// One product; `to` and `out`: what it writes and where.  ws: copies_bytes().
+cudaError_t product(const GroupedArgs& g, int dtype, const Shape& s, int to, void* out, char* ws, cudaStream_t st) {
   Operand a = matrices(g.A, g.transA != 0, g.M, g.K, g.lda, g.strideA, g.mats), x = columns_of(g.X, g.K, g.N, g.ldx, g.columns, g.R);
   const Runs runs{g.offsets, g.run_len, g.G, g.R};
-  const Shape s = shape_of(g.M, g.K, g.R, g.G);
   const bool in_place = g.columns && gathers_in_place(x, s);
   if (in_place) x = columns_of(g.X, g.K, g.N, g.ldx, nullptr, 0);
   cudaError_t e = align_operand(a, ws, g.ids || !g.offsets ? nullptr : &runs, st);
@@ -990,17 +1092,17 @@ cudaError_t grouped_umma(const GroupedArgs& g, int dtype, bool to_low, void* wor
   f.columns = g.columns;
   f.gather = in_place;
   f.cap = s.cap;
-  f.C = g.C;
+  f.C = out;
   f.ldc = g.ldc;
   f.scale = g.scale;
   f.scale0 = g.scale0;
   f.M = g.M; f.K = g.K; f.G = g.G; f.N = g.N; f.mats = g.mats;
   f.a_kmaj = g.transA;
   f.a_same = g.mats > 1 && g.strideA == 0;
-  f.zero_rest = g.zero_rest;
-  f.splits = 1;
-  f.to = to_low ? kToLow : kToC;
-  f.pairs = (reinterpret_cast<uintptr_t>(g.C) & 3u) == 0 && g.ldc % 2 == 0 && g.M % 2 == 0;
+  f.zero_rest = g.zero_rest && to == kToC;
+  f.splits = s.splits;
+  f.to = to;
+  f.pairs = (reinterpret_cast<uintptr_t>(out) & 3u) == 0 && g.ldc % 2 == 0 && g.M % 2 == 0;
   f.low_width = low_width(g.M);
   f.low_step = f.low_width / 2;
   f.status = g.status;
@@ -1008,10 +1110,10 @@ cudaError_t grouped_umma(const GroupedArgs& g, int dtype, bool to_low, void* wor
   if (!encode_matrix(&ma, dtype, a, g.transA != 0) || !encode_columns(&mx, dtype, x, in_place ? 1 : box_of(s))) return cudaErrorInvalidValue;
   mb = ma;
   mt = mx;
-  if (g.low.r > 0 && g.low.n > 0 && g.low.runs > 0) {
+  if (g.low.r > 0 && to == kToC) {
     Operand b = matrices(g.low.B, g.low.transB != 0, g.M, g.low.r, g.low.ldb, g.low.strideB, g.low.n);
     if ((e = align_operand(b, ws, nullptr, st)) != cudaSuccess) return e;
-    const Operand t{g.low.T, low_width(g.low.r), g.R, g.low.ldt, 0, 1, nullptr, 0};
+    const Operand t{g.low.T, low_width(g.low.r), g.R, low_width(g.low.r), 0, 1, nullptr, 0};
     if (!encode_matrix(&mb, dtype, b, g.low.transB != 0) || !encode_columns(&mt, dtype, t, box_of(s))) return cudaErrorInvalidValue;
     f.low_runs = Runs{g.low.offsets, g.low.run_len, g.low.runs, g.R};
     f.low_ids = g.low.ids;
@@ -1019,6 +1121,97 @@ cudaError_t grouped_umma(const GroupedArgs& g, int dtype, bool to_low, void* wor
     f.low_kmaj = g.low.transB;
   }
   return dtype == NNLIB_B200_BF16 ? fwd<true>(s, ma, mx, mb, mt, f, st) : fwd<false>(s, ma, mx, mb, mt, f, st);
+}
+
+cudaError_t join(const GroupedArgs& g, int dtype, const Shape& s, const float* parts, const float* t, int t_splits, cudaStream_t st) {
+  JoinArgs j;
+  std::memset(&j, 0, sizeof(j));
+  j.parts = parts;
+  j.C = g.C;
+  j.ldc = g.ldc;
+  j.splits = s.splits; j.M = g.M; j.R = g.R; j.N = g.N; j.zero_rest = g.zero_rest;
+  j.runs = Runs{g.offsets, g.run_len, g.G, g.R};
+  j.columns = g.columns;
+  if (t) {
+    j.t = t;
+    j.t_splits = t_splits; j.r = g.low.r; j.n = g.low.n; j.transB = g.low.transB;
+    j.low_runs = Runs{g.low.offsets, g.low.run_len, g.low.runs, g.R};
+    j.low_ids = g.low.ids;
+    j.B = g.low.B;
+    j.ldb = g.low.ldb; j.strideB = g.low.strideB;
+  }
+  const dim3 grid((unsigned)g.R, (unsigned)((g.M + 255) / 256));
+  if (dtype == NNLIB_B200_BF16) join_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(j);
+  else join_kernel<__half><<<grid, 128, 0, st>>>(j);
+  count_launch();
+  return cudaGetLastError();
+}
+// K is cut for few columns only: parts of many cost more than the SMs that it fills
+bool few(int R, int M) { return R <= 512 && M <= 65535 * 256; }
+
+}  // namespace
+
+size_t grouped_umma_workspace_bytes(const GroupedArgs& g) {
+  const Shape s = shape_of(g.M, g.K, g.R, g.G, few(g.R, g.M));
+  return copies_bytes(g, s) + (s.splits > 1 ? parts_bytes(g, s) : 0);
+}
+cudaError_t grouped_umma(const GroupedArgs& g, int dtype, void* workspace, cudaStream_t st) {
+  char* ws = static_cast<char*>(workspace);
+  const Shape s = shape_of(g.M, g.K, g.R, g.G, few(g.R, g.M));
+  if (s.splits == 1) return product(g, dtype, s, kToC, g.C, ws, st);
+  char* parts = ws + copies_bytes(g, s);
+  const cudaError_t e = product(g, dtype, s, kToParts, parts, ws, st);
+  return e == cudaSuccess ? join(g, dtype, s, reinterpret_cast<const float*>(parts), nullptr, 0, st) : e;
+}
+
+// A X of low-rank pairs, as T or, `parts`, in Float32 parts
+static Shape first_shape(const GroupedArgs& f) { return shape_of(f.M, f.K, f.R, f.G, true); }
+size_t low_umma_workspace_bytes(const GroupedArgs& f) {
+  const Shape s = first_shape(f);
+  return copies_bytes(f, s) + (s.splits > 1 ? parts_bytes(f, s) : 0);
+}
+size_t low_umma_bytes(const GroupedArgs& f) { return padded((size_t)f.R * 2 * low_width(f.M)); }
+cudaError_t low_umma(const GroupedArgs& f, int dtype, void* T, void* workspace, cudaStream_t st) {
+  const Shape s = first_shape(f);
+  char* ws = static_cast<char*>(workspace);
+  if (s.splits == 1) return product(f, dtype, s, kToLow, T, ws, st);
+  char* parts = ws + copies_bytes(f, s);
+  const cudaError_t e = product(f, dtype, s, kToParts, parts, ws, st);
+  if (e != cudaSuccess) return e;
+  const int width = low_width(f.M);
+  const long long blocks = ((long long)f.R * (width / 2) + 255) / 256;
+  const float* p = reinterpret_cast<const float*>(parts);
+  if (dtype == NNLIB_B200_BF16) join_low_kernel<<<(unsigned)blocks, 256, 0, st>>>(p, s.splits, f.M, f.R, static_cast<__nv_bfloat16*>(T), width);
+  else join_low_kernel<<<(unsigned)blocks, 256, 0, st>>>(p, s.splits, f.M, f.R, static_cast<__half*>(T), width);
+  count_launch();
+  return cudaGetLastError();
+}
+
+// W X with the pairs' term; first.R columns.  keep: T of the columns is wanted behind it (the gradients read it), at `low`.
+static Shape main_shape(const GroupedArgs& m, bool keep) { return shape_of(m.M, m.K, m.R, 1, !keep && few(m.R, m.M)); }
+size_t adapter_umma_workspace_bytes(const GroupedArgs& first, const GroupedArgs& m, bool keep) {
+  const Shape s = main_shape(m, keep);
+  if (s.splits == 1) return std::max(m.low.r > 0 ? low_umma_workspace_bytes(first) : 0, copies_bytes(m, s));
+  const Shape f = first_shape(first);
+  return copies_bytes(m, s) + parts_bytes(m, s) + (m.low.r > 0 ? copies_bytes(first, f) + parts_bytes(first, f) : 0);
+}
+cudaError_t adapter_umma(const GroupedArgs& first, GroupedArgs m, int dtype, bool keep, void* low, void* workspace, cudaStream_t st) {
+  const Shape s = main_shape(m, keep);
+  char* ws = static_cast<char*>(workspace);
+  cudaError_t e = cudaSuccess;
+  if (s.splits == 1) {
+    if (m.low.r > 0) e = low_umma(first, dtype, low, ws, st);
+    m.low.T = low;
+    return e == cudaSuccess ? product(m, dtype, s, kToC, m.C, ws, st) : e;
+  }
+  // few columns: both products in parts, joined by one launch that multiplies by B
+  const Shape f = first_shape(first);
+  char* parts = ws + copies_bytes(m, s);
+  char* ws_first = parts + parts_bytes(m, s);
+  char* of_first = ws_first + (m.low.r > 0 ? copies_bytes(first, f) : 0);
+  if (m.low.r > 0) e = product(first, dtype, f, kToParts, of_first, ws_first, st);
+  if (e == cudaSuccess) e = product(m, dtype, s, kToParts, parts, ws, st);
+  return e == cudaSuccess ? join(m, dtype, s, reinterpret_cast<const float*>(parts), m.low.r > 0 ? reinterpret_cast<const float*>(of_first) : nullptr, f.splits, st) : e;
 }
 
 size_t grouped_umma_grad_workspace_bytes(const GroupedGradArgs& g, int fold) {
