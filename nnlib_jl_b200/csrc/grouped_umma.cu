@@ -844,6 +844,11 @@ struct JoinArgs {
   const int* low_ids;
   const void* B;
   long long ldb, strideB;
+  int b_pairs;                           // rows of B come in pairs at 4-byte addresses
+};
+template <typename T>
+struct alignas(4) Two {
+  T x, y;
 };
 template <typename T>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ JoinArgs g) {
@@ -851,11 +856,31 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ JoinA
   __shared__ int pair;
   const int n = blockIdx.x, m = (blockIdx.y * 128 + threadIdx.x) * 2;
   T* out = reinterpret_cast<T*>(g.C) + (long long)n * g.ldc + m;
-  int in = 0;
-  for (int i = threadIdx.x; i < g.runs.runs; i += 128) in |= g.runs.begin(i) <= n && n < g.runs.end(i);
-  if (threadIdx.x == 0) pair = -1;
-  in = __syncthreads_or(in);
-  if (!in && !g.zero_rest) return;
+  int in = 1;
+  if (g.runs.offsets) {
+    in = 0;
+    for (int i = threadIdx.x; i < g.runs.runs; i += 128) in |= g.runs.begin(i) <= n && n < g.runs.end(i);
+    in = __syncthreads_or(in);
+    if (!in && !g.zero_rest) return;
+  }
+  if (g.r > 0) {
+    if (g.low_runs.offsets) {
+      if (threadIdx.x == 0) pair = -1;
+      __syncthreads();
+      for (int i = threadIdx.x; i < g.low_runs.runs; i += 128)
+        if (g.low_runs.begin(i) <= n && n < g.low_runs.end(i)) pair = g.low_ids[i];
+    } else if (threadIdx.x == 0) {
+      const long long i = g.low_runs.len > 0 ? n / g.low_runs.len : g.low_runs.runs;
+      pair = i < g.low_runs.runs ? g.low_ids[i] : -1;
+    }
+    if (threadIdx.x < g.r) {
+      float v = 0.f;
+#pragma unroll 4
+      for (int s = 0; s < g.t_splits; ++s) v += g.t[((long long)s * g.R + n) * g.r + threadIdx.x];
+      t[threadIdx.x] = v;
+    }
+    __syncthreads();
+  }
   float sum[2] = {0.f, 0.f};
   if (in && (!g.columns || (unsigned)g.columns[n] < (unsigned)g.N)) {
 #pragma unroll 4
@@ -865,28 +890,25 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ JoinA
       if (m + 1 < g.M) sum[1] += p[1];
     }
   }
-  if (g.r > 0) {
-    for (int i = threadIdx.x; i < g.low_runs.runs; i += 128)
-      if (g.low_runs.begin(i) <= n && n < g.low_runs.end(i)) pair = g.low_ids[i];
-    __syncthreads();
-    const int id = pair;
-    if (id >= 0 && id < g.n) {
-      if (threadIdx.x < g.r) {
-        float v = 0.f;
-        for (int s = 0; s < g.t_splits; ++s) v += g.t[((long long)s * g.R + n) * g.r + threadIdx.x];
-        t[threadIdx.x] = v;
-      }
-      __syncthreads();
-      const T* B = reinterpret_cast<const T*>(g.B) + (long long)id * g.strideB;
-      const long long row = g.transB ? g.ldb : 1, col = g.transB ? 1 : g.ldb;
-      if (m < g.M) {
-        const T* b = B + m * row;
-        const bool two = m + 1 < g.M;
+  const int id = g.r > 0 ? pair : -1;
+  if (id >= 0 && id < g.n && m < g.M) {
+    const T* B = reinterpret_cast<const T*>(g.B) + (long long)id * g.strideB;
+    const bool two = m + 1 < g.M;
+    if (!g.transB && two && g.b_pairs) {
+      const Two<T>* b = reinterpret_cast<const Two<T>*>(B + m);
 #pragma unroll 8
-        for (int i = 0; i < g.r; ++i) {
-          sum[0] = fmaf(Elem<T>::to_f(b[i * col]), t[i], sum[0]);
-          if (two) sum[1] = fmaf(Elem<T>::to_f(b[row + i * col]), t[i], sum[1]);
-        }
+      for (int i = 0; i < g.r; ++i) {
+        const Two<T> v = b[i * (g.ldb / 2)];
+        sum[0] = fmaf(Elem<T>::to_f(v.x), t[i], sum[0]);
+        sum[1] = fmaf(Elem<T>::to_f(v.y), t[i], sum[1]);
+      }
+    } else {
+      const long long row = g.transB ? g.ldb : 1, col = g.transB ? 1 : g.ldb;
+      const T* b = B + m * row;
+#pragma unroll 8
+      for (int i = 0; i < g.r; ++i) {
+        sum[0] = fmaf(Elem<T>::to_f(b[i * col]), t[i], sum[0]);
+        if (two) sum[1] = fmaf(Elem<T>::to_f(b[row + i * col]), t[i], sum[1]);
       }
     }
   }
@@ -1139,6 +1161,7 @@ cudaError_t join(const GroupedArgs& g, int dtype, const Shape& s, const float* p
     j.low_ids = g.low.ids;
     j.B = g.low.B;
     j.ldb = g.low.ldb; j.strideB = g.low.strideB;
+    j.b_pairs = (reinterpret_cast<uintptr_t>(g.low.B) & 3u) == 0 && g.low.ldb % 2 == 0 && g.low.strideB % 2 == 0;
   }
   const dim3 grid((unsigned)g.R, (unsigned)((g.M + 255) / 256));
   if (dtype == NNLIB_B200_BF16) join_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(j);

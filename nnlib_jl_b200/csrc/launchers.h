@@ -190,7 +190,7 @@ struct RouteArgs {
   void* dlogits;
   int* ws;                   // counts (G, blocks), totals (G)
   int G, N, k, normalize;
-  int blocks, per_block;     // filled in by the launcher
+  int blocks, per_block, vec, k_up;   // filled in by the launcher
 };
 size_t route_workspace_bytes(const RouteArgs& a);
 cudaError_t route(RouteArgs a, int dtype, cudaStream_t st);

@@ -1,9 +1,9 @@
 // The router of a layer of experts and the sum that ends it (include/nnlib_b200.h: nnlib_b200_route, nnlib_b200_combine).
 //
 // route: S_t = the k largest of l_t + b; w = softmax(l) over S_t or over all; then a stable counting sort of the chosen
-// (token, expert) pairs by expert.  A warp takes a token, its G logits as order-preserving integers in registers, and picks
-// the largest k times (redux.sync gives a warp's largest; the first lane that has it has the lowest expert, since lanes hold
-// neighbouring experts).  A block counts its tokens' choices; a second launch turns the counts of all blocks into each
+// (token, expert) pairs by expert.  A warp takes a token: its G logits are order-preserving integers in registers, in falling order in
+// each lane, and k times the largest head is taken (redux.sync gives a warp's largest; the first lane that has it has the lowest expert, since
+// lanes hold neighbouring experts).  A block counts its tokens' choices; a second launch turns the counts of all blocks into each
 // block's first number for each expert; a third gives every pair its number: a token picks an expert at most once, so the
 // pair's place among its block's is the number of earlier tokens in the expert's bit mask.  Nothing depends on the order in
 // which warps run.  Few tokens take one block and one launch.
@@ -11,6 +11,7 @@
 // combine: HBM bound, 16 bytes a thread and column.
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "common.cuh"
 #include "launchers.h"
@@ -19,14 +20,52 @@ namespace nb200 {
 namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
-constexpr int kChooseWarps = 16;
+
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+  T v[VEC];
+};
+constexpr int kChooseWarps = 8;
 constexpr int kMaxPerBlock = 256;        // tokens whose choices one block numbers: the masks of an expert are 8 words
 
-// Larger floats are larger integers; -0 like +0; NaN below everything, 0 for what cannot be chosen.
+// Larger floats are larger integers; -0 like +0; NaN below everything; 0 for what cannot be chosen.
 __device__ __forceinline__ unsigned sortable(float x) {
   if (isnan(x)) return 1u;
   const unsigned u = __float_as_uint(x + 0.f);
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+// What an expert is chosen by, unlike any other's: its logit, then the lower expert.  A 16-bit logit fits one word with the
+// expert's number.
+__device__ __forceinline__ unsigned packed_key(unsigned bits, unsigned infinity, int e) {
+  const unsigned size = bits & 0x7fffu;
+  unsigned k = (bits & 0x8000u) ? 0x8000u - size : 0x8000u + size;      // -0 like +0
+  if (size > infinity) k = 0u;                                          // NaN
+  return k << 16 | (0xffffu - (unsigned)e);
+}
+template <typename T> __device__ __forceinline__ unsigned raw_bits(T v) { return 0u; }
+template <> __device__ __forceinline__ unsigned raw_bits(__half v) { return __half_as_ushort(v); }
+template <> __device__ __forceinline__ unsigned raw_bits(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
+__device__ __forceinline__ unsigned long long wide_key(float x, int e) {
+  return (unsigned long long)sortable(x) << 32 | (0xffffffffu - (unsigned)e);
+}
+// in falling order: Batcher's odd-even merge sort
+template <int V, typename K>
+__device__ __forceinline__ void sort_falling(K (&a)[V]) {
+#pragma unroll
+  for (int p = 1; p < V; p *= 2) {
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2) {
+#pragma unroll
+      for (int i = 0; i + k < V; ++i) {
+        const bool in = i >= k % p && ((i - k % p) / k) % 2 == 0 && i / (2 * p) == (i + k) / (2 * p);
+        if (in) {
+          const K lo = a[i] < a[i + k] ? a[i] : a[i + k], hi = a[i] < a[i + k] ? a[i + k] : a[i];
+          a[i] = hi;
+          a[i + k] = lo;
+        }
+      }
+    }
+  }
 }
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
@@ -39,13 +78,23 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// V neighbouring logits of a token for each lane; -Inf where there is no expert
+// V neighbouring logits of a token for each lane; -Inf where there is no expert.  vec: as many as fit 16 bytes at a time
 template <typename T, int V>
-__device__ __forceinline__ void load_logits(const T* row, int G, int lane, float (&x)[V]) {
+__device__ __forceinline__ void load_logits(const T* row, int G, int lane, bool vec, T (&x)[V]) {
+  constexpr int W = V * sizeof(T) <= 16 ? V : 16 / sizeof(T);
+  if (vec && lane * V + V <= G) {
+#pragma unroll
+    for (int v = 0; v < V; v += W) {
+      const Pack<T, W> p = *reinterpret_cast<const Pack<T, W>*>(row + lane * V + v);
+#pragma unroll
+      for (int w = 0; w < W; ++w) x[v + w] = p.v[w];
+    }
+    return;
+  }
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int e = lane * V + v;
-    x[v] = e < G ? Elem<T>::to_f(row[e]) : __int_as_float(0xff800000);
+    x[v] = e < G ? row[e] : Elem<T>::from_f(__int_as_float(0xff800000));
   }
 }
 // the exponential of a logit relative to the largest: the slow branch of the softmax for +Inf
@@ -54,56 +103,65 @@ __device__ __forceinline__ float share_of(float x, float mx) {
   return expf(x - mx);
 }
 
-template <typename T, int V>
+template <typename T, int V, bool PACKED>
 __device__ void choose_token(const RouteArgs& a, int t, int lane, int* count) {
   const bool live = !a.mask || a.mask[t];
   int mine = -1;                          // lane j: the j-th expert of the token
   float w = 0.f;
   if (live) {
-    float x[V];
-    load_logits<T, V>(reinterpret_cast<const T*>(a.logits) + (long long)t * a.stride, a.G, lane, x);
-    unsigned key[V], best = 0u;
-    int at = 0;
+    const T* row = reinterpret_cast<const T*>(a.logits) + (long long)t * a.stride;
+    T x[V];
+    load_logits<T, V>(row, a.G, lane, a.vec != 0, x);
+    // every lane's experts in falling order: the warp's best is the best of their heads
+    typename std::conditional<PACKED, unsigned, unsigned long long>::type key[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int e = lane * V + v;
-      key[v] = e < a.G ? sortable(a.bias ? x[v] + a.bias[e] : x[v]) : 0u;
-      if (key[v] > best) { best = key[v]; at = v; }
-    }
-    float logit = 0.f;
-    for (int j = 0; j < a.k; ++j) {
-      const unsigned top = __reduce_max_sync(kFull, best);
-      const int src = __ffs(__ballot_sync(kFull, best == top)) - 1;
-      float mylogit = 0.f;
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        if (v == at) mylogit = x[v];
-      const int e = __shfl_sync(kFull, lane * V + at, src);
-      const float l = __shfl_sync(kFull, mylogit, src);
-      if (lane == j) { mine = e; logit = l; }
-      if (lane == src) {
-        best = 0u;
-        const int gone = at;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          if (v == gone) key[v] = 0u;
-          if (key[v] > best) { best = key[v]; at = v; }
-        }
+      if constexpr (PACKED) {
+        key[v] = e < a.G ? packed_key(raw_bits(x[v]), std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u, e) : 0u;
+      } else {
+        const float f = Elem<T>::to_f(x[v]);
+        key[v] = e < a.G ? wide_key(a.bias ? f + a.bias[e] : f, e) : 0ull;
       }
     }
-    float mx, part = 0.f;
-    if (a.normalize) {
-      mx = warp_max(lane < a.k ? logit : __int_as_float(0xff800000));
-      if (lane < a.k) part = share_of(logit, mx);
-      w = part / warp_sum(part);
-    } else {
-      mx = x[0];
+    sort_falling<V>(key);
+    for (int j = 0; j < a.k; ++j) {
+      int e;
+      bool win;
+      if constexpr (PACKED) {
+        const unsigned top = __reduce_max_sync(kFull, key[0]);
+        e = (int)(0xffffu - (top & 0xffffu));
+        win = key[0] == top;
+      } else {
+        const unsigned head = (unsigned)(key[0] >> 32), top = __reduce_max_sync(kFull, head);
+        const int src = __ffs(__ballot_sync(kFull, head == top)) - 1;      // (lanes hold neighbouring experts)
+        e = (int)(0xffffffffu - __shfl_sync(kFull, (unsigned)key[0], src));
+        win = lane == src;
+      }
+      if (lane == j) mine = e;
+      if (win) {
 #pragma unroll
-      for (int v = 1; v < V; ++v) mx = fmaxf(mx, x[v]);
+        for (int v = 0; v + 1 < V; ++v) key[v] = key[v + 1];
+        key[V - 1] = 0;
+      }
+    }
+    const float logit = lane < a.k ? Elem<T>::to_f(row[mine]) : 0.f;
+    if (a.normalize) {
+      // over the first lanes only: as many steps as k has bits
+      float mx = lane < a.k ? logit : __int_as_float(0xff800000);
+      for (int o = a.k_up / 2; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, o));
+      const float part = lane < a.k ? share_of(logit, mx) : 0.f;
+      float sum = part;
+      for (int o = a.k_up / 2; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+      w = part / sum;
+    } else {
+      float mx = Elem<T>::to_f(x[0]), part = 0.f;
+#pragma unroll
+      for (int v = 1; v < V; ++v) mx = fmaxf(mx, Elem<T>::to_f(x[v]));
       mx = warp_max(mx);
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        if (lane * V + v < a.G) part += share_of(x[v], mx);
+        if (lane * V + v < a.G) part += share_of(Elem<T>::to_f(x[v]), mx);
       w = share_of(logit, mx) / warp_sum(part);
     }
     if (count && lane < a.k) atomicAdd(&count[mine], 1);
@@ -172,17 +230,17 @@ __device__ void end_of_order(const RouteArgs& a, int total, long long i0, long l
 }
 
 // shared memory: G counts or bases, then the masks
-template <typename T, int V, bool ALONE>
-__global__ void __launch_bounds__(32 * kChooseWarps) route_choose_kernel(const RouteArgs a) {
+template <typename T, int V, bool PACKED, bool ALONE, int W>
+__global__ void __launch_bounds__(32 * W) route_choose_kernel(const RouteArgs a) {
   extern __shared__ int sm[];
-  __shared__ int part[kChooseWarps];
+  __shared__ int part[W];
   const int t0 = blockIdx.x * a.per_block, t1 = min(a.N, t0 + a.per_block);
   for (int i = threadIdx.x; i < a.G; i += blockDim.x) sm[i] = 0;
   __syncthreads();
-  for (int t = t0 + (threadIdx.x >> 5); t < t1; t += kChooseWarps) choose_token<T, V>(a, t, threadIdx.x & 31, sm);
+  for (int t = t0 + (threadIdx.x >> 5); t < t1; t += W) choose_token<T, V, PACKED>(a, t, threadIdx.x & 31, sm);
   __syncthreads();
   if constexpr (ALONE) {
-    const int total = block_scan<kChooseWarps>(sm, a.G, part);
+    const int total = block_scan<W>(sm, a.G, part);
     for (int i = threadIdx.x; i < a.G; i += blockDim.x) a.offsets[i] = sm[i];
     if (threadIdx.x == 0) a.offsets[a.G] = total;
     number_pairs(a, t0, t1, sm, reinterpret_cast<unsigned*>(sm + a.G));
@@ -198,27 +256,40 @@ __global__ void __launch_bounds__(256) route_scan_kernel(const RouteArgs a) {
   if (e >= a.G) return;
   int* c = a.ws + (long long)e * a.blocks;
   int carry = 0;
-  for (int i0 = 0; i0 < a.blocks; i0 += 32) {
-    const int own = i0 + lane < a.blocks ? c[i0 + lane] : 0;
-    int s = own;
+  for (int i0 = 0; i0 < a.blocks; i0 += 256) {             // eight neighbours a lane: all on their way at once
+    int own[8], sum = 0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int i = i0 + lane * 8 + u;
+      own[u] = i < a.blocks ? c[i] : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) sum += own[u];
+    int s = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(kFull, s, o);
       if (lane >= o) s += u;
     }
-    if (i0 + lane < a.blocks) c[i0 + lane] = carry + s - own;
+    int before = carry + s - sum;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int i = i0 + lane * 8 + u;
+      if (i < a.blocks) c[i] = before;
+      before += own[u];
+    }
     carry += __shfl_sync(kFull, s, 31);
   }
   if (lane == 0) a.ws[(long long)a.G * a.blocks + e] = carry;
 }
 
-__global__ void __launch_bounds__(512) route_number_kernel(const RouteArgs a) {
+__global__ void __launch_bounds__(256) route_number_kernel(const RouteArgs a) {
   extern __shared__ int sm[];
-  __shared__ int part[16];
+  __shared__ int part[8];
   const int* totals = a.ws + (long long)a.G * a.blocks;
   for (int i = threadIdx.x; i < a.G; i += blockDim.x) sm[i] = totals[i];
   __syncthreads();
-  const int total = block_scan<16>(sm, a.G, part);
+  const int total = block_scan<8>(sm, a.G, part);
   if (blockIdx.x == 0) {
     for (int i = threadIdx.x; i < a.G; i += blockDim.x) a.offsets[i] = sm[i];
     if (threadIdx.x == 0) a.offsets[a.G] = total;
@@ -257,8 +328,11 @@ __global__ void __launch_bounds__(256) route_bwd_kernel(const RouteArgs a) {
       if (v == at) d[v] = val;
   }
   if (!a.normalize && live) {
+    T raw[V];
     float x[V], mx, part = 0.f;
-    load_logits<T, V>(reinterpret_cast<const T*>(a.logits) + (long long)t * a.stride, a.G, lane, x);
+    load_logits<T, V>(reinterpret_cast<const T*>(a.logits) + (long long)t * a.stride, a.G, lane, a.vec != 0, raw);
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[v] = Elem<T>::to_f(raw[v]);
     mx = x[0];
 #pragma unroll
     for (int v = 1; v < V; ++v) mx = fmaxf(mx, x[v]);
@@ -279,29 +353,39 @@ __global__ void __launch_bounds__(256) route_bwd_kernel(const RouteArgs a) {
 }
 
 void plan(RouteArgs& a) {
-  // one block while its warps have few tokens each; then as many blocks as keep every SM busy, in whole mask words
+  // one block while its warps have few tokens each; then as many blocks as make full waves, in whole mask words
   if (a.N <= 128) {
     a.per_block = 128;
   } else {
-    a.per_block = std::min(kMaxPerBlock, std::max(32, (a.N / 296 + 31) / 32 * 32));
+    // (seven blocks of eight warps an SM: 32768 tokens of 256 experts 23 us)
+    a.per_block = std::min(kMaxPerBlock, std::max(32, (a.N / 1036 + 31) / 32 * 32));
   }
   a.blocks = (a.N + a.per_block - 1) / a.per_block;
 }
 
-template <typename T, int V>
-cudaError_t launch_route(RouteArgs a, cudaStream_t st) {
+template <typename T, int V, bool PACKED>
+cudaError_t launch_choose(RouteArgs a, cudaStream_t st) {
+  // (64 registers to a thread are enough for up to 256 experts)
+  constexpr int kAlone = V <= 8 ? 32 : 8;
   const size_t counts = sizeof(int) * a.G, masks = sizeof(unsigned) * a.G * (kMaxPerBlock / 32);
   if (a.blocks <= 1) {
     a.blocks = 1;
-    route_choose_kernel<T, V, true><<<1, 32 * kChooseWarps, counts + masks, st>>>(a);
+    route_choose_kernel<T, V, PACKED, true, kAlone><<<1, 32 * kAlone, counts + masks, st>>>(a);
     count_launch();
     return cudaGetLastError();
   }
-  route_choose_kernel<T, V, false><<<a.blocks, 32 * kChooseWarps, counts, st>>>(a);
+  route_choose_kernel<T, V, PACKED, false, kChooseWarps><<<a.blocks, 32 * kChooseWarps, counts, st>>>(a);
   route_scan_kernel<<<(a.G + 7) / 8, 256, 0, st>>>(a);
-  route_number_kernel<<<a.blocks, 512, counts + masks, st>>>(a);
+  route_number_kernel<<<a.blocks, 256, counts + masks, st>>>(a);
   count_launch(3);
   return cudaGetLastError();
+}
+template <typename T, int V>
+cudaError_t launch_route(const RouteArgs& a, cudaStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (!a.bias) return launch_choose<T, V, true>(a, st);
+  }
+  return launch_choose<T, V, false>(a, st);
 }
 template <typename T, int V>
 cudaError_t launch_route_bwd(const RouteArgs& a, cudaStream_t st) {
@@ -311,33 +395,51 @@ cudaError_t launch_route_bwd(const RouteArgs& a, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------------------------------------- combine
-template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Pack {
-  T v[VEC];
-};
-
-template <typename T, int VEC>
-__global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
-  const int per = a.E / VEC;               // packets of a column
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (long long)per * a.N) return;
-  const int t = (int)(i / per), c = (int)(i % per) * VEC;
-  float acc[VEC];
+// A block takes 256 P packets of a token's column, P to a thread, two of the token's pairs at a time: 2 P loads under way.
+template <typename T, int VEC, int P>
+__global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a, int chunks) {
+  const int t = blockIdx.x / chunks, c0 = (blockIdx.x % chunks) * (256 * P) + threadIdx.x, per = a.E / VEC;
+  if (c0 >= per) return;
+  const int* position = a.position + (long long)t * a.k;
+  const float* weights = a.weights ? a.weights + (long long)t * a.k : nullptr;
+  const Pack<T, VEC>* Y = reinterpret_cast<const Pack<T, VEC>*>(a.Y);
+  const long long ld = a.Y_stride / VEC;
+  float acc[P][VEC];
 #pragma unroll
-  for (int v = 0; v < VEC; ++v) acc[v] = 0.f;
-#pragma unroll 4
-  for (int j = 0; j < a.k; ++j) {
-    const int p = a.position[(long long)t * a.k + j];
-    if (p < 0 || p >= a.R) continue;
-    const float w = a.weights ? a.weights[(long long)t * a.k + j] : 1.f;
-    const Pack<T, VEC> y = *reinterpret_cast<const Pack<T, VEC>*>(reinterpret_cast<const T*>(a.Y) + (long long)p * a.Y_stride + c);
+  for (int p = 0; p < P; ++p)
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) acc[v] = fmaf(w, Elem<T>::to_f(y.v[v]), acc[v]);
+    for (int v = 0; v < VEC; ++v) acc[p][v] = 0.f;
+  for (int j = 0; j < a.k; j += 2) {
+    Pack<T, VEC> y[2][P];
+    float w[2];
+    bool there[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int at = j + u < a.k ? position[j + u] : -1;
+      there[u] = at >= 0 && at < a.R;
+      w[u] = there[u] && weights ? weights[j + u] : 1.f;
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+        if (there[u] && c0 + 256 * p < per) y[u][p] = Y[(long long)at * ld + c0 + 256 * p];
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (!there[u]) continue;
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) acc[p][v] = fmaf(w[u], Elem<T>::to_f(y[u][p].v[v]), acc[p][v]);
+    }
   }
-  Pack<T, VEC> out;
+  Pack<T, VEC>* out = reinterpret_cast<Pack<T, VEC>*>(reinterpret_cast<T*>(a.y) + (long long)t * a.y_stride);
 #pragma unroll
-  for (int v = 0; v < VEC; ++v) out.v[v] = Elem<T>::from_f(acc[v]);
-  *reinterpret_cast<Pack<T, VEC>*>(reinterpret_cast<T*>(a.y) + (long long)t * a.y_stride + c) = out;
+  for (int p = 0; p < P; ++p) {
+    if (c0 + 256 * p >= per) continue;
+    Pack<T, VEC> o;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) o.v[v] = Elem<T>::from_f(acc[p][v]);
+    out[c0 + 256 * p] = o;
+  }
 }
 
 // A warp takes a column of Y: its token, the weight that names it, the gradient of both.
@@ -397,9 +499,11 @@ bool packets(const void* p, long long stride, int bytes, int esize) {
 template <typename T, int VEC>
 cudaError_t launch_combine(const CombineArgs& a, bool bwd, cudaStream_t st) {
   if (!bwd) {
-    const long long n = (long long)(a.E / VEC) * a.N, blocks = (n + 255) / 256;
+    const int per = a.E / VEC, P = per > 256 ? 2 : 1, chunks = (per + 256 * P - 1) / (256 * P);
+    const long long blocks = (long long)chunks * a.N;
     if (blocks > INT_MAX) return cudaErrorInvalidConfiguration;
-    combine_kernel<T, VEC><<<(unsigned)blocks, 256, 0, st>>>(a);
+    if (P == 2) combine_kernel<T, VEC, 2><<<(unsigned)blocks, 256, 0, st>>>(a, chunks);
+    else combine_kernel<T, VEC, 1><<<(unsigned)blocks, 256, 0, st>>>(a, chunks);
     count_launch();
   } else {
     if (a.R) combine_bwd_kernel<T, VEC><<<(a.R + 7) / 8, 256, 0, st>>>(a);
@@ -418,7 +522,12 @@ cudaError_t combine_of(const CombineArgs& a, bool bwd, cudaStream_t st) {
 }
 
 template <typename T>
-cudaError_t route_of(const RouteArgs& a, bool bwd, cudaStream_t st) {
+cudaError_t route_of(RouteArgs a, bool bwd, cudaStream_t st) {
+  int v = 1;
+  while (32 * v < a.G) v *= 2;
+  a.k_up = 1;
+  while (a.k_up < a.k) a.k_up *= 2;
+  a.vec = packets(a.logits, a.stride, std::min<int>(16, v * sizeof(T)), sizeof(T));
 #define NB_V(VV)                                                                          \
   if (a.G <= 32 * VV) return bwd ? launch_route_bwd<T, VV>(a, st) : launch_route<T, VV>(a, st)
   NB_V(1);
