@@ -48,19 +48,20 @@ struct Table {
   int cum[kMaxRuns + 8], begin[kMaxRuns], end[kMaxRuns];
 };
 constexpr int kTableBytes = sizeof(Table);
+constexpr int kOutBytes = 8 * 2048;      // a box of 32 rows x 32 columns for each warp of the epilogue
 
 template <int MH, int NT>
 struct Cfg {
   static constexpr int kA = MH * kHalfBytes, kX = NT * 128, kStage = kA + kX;
-  static constexpr int kRoom = 226 * 1024 - kTableBytes - 512;
+  static constexpr int kRoom = 226 * 1024 - kTableBytes - kOutBytes - 512;
   static constexpr int kStages = kRoom / kStage > 10 ? 10 : kRoom / kStage;
   static constexpr int kAccCols = MH * NT, kAccBufs = kAccCols <= 256 ? 2 : 1;
   static constexpr int kTmemCols = kAccCols * kAccBufs < 32 ? 32 : kAccCols * kAccBufs;
   static constexpr int kBox = NT >= 128 ? 64 : 16;       // columns of X that one copy brings
-  static constexpr int kTableOff = kStages * kStage, kBarOff = kTableOff + kTableBytes;
+  static constexpr int kOutOff = kStages * kStage, kTableOff = kOutOff + kOutBytes, kBarOff = kTableOff + kTableBytes;
   static constexpr int kSmem = kBarOff + 512 + 1024;
 };
-static_assert(Cfg<2, 256>::kStages == 3 && Cfg<1, 256>::kStages == 4 && Cfg<1, 32>::kStages == 10, "ring depth");
+static_assert(Cfg<2, 256>::kStages == 3 && Cfg<1, 256>::kStages == 4 && Cfg<1, 32>::kStages == 9, "ring depth");
 static_assert(Cfg<2, 256>::kSmem <= 232448 && Cfg<1, 256>::kSmem <= 232448 && Cfg<1, 128>::kSmem <= 232448 && Cfg<1, 64>::kSmem <= 232448 &&
               Cfg<1, 32>::kSmem <= 232448, "shared memory budget");
 
@@ -84,7 +85,7 @@ struct FwdArgs {
   float scale0;
   int M, K, G, N, mats;
   int cap;                               // columns of a tile, at most NT
-  int a_kmaj, a_same, zero_rest, splits, tiles_m, to, pairs, gather;
+  int a_kmaj, a_same, zero_rest, splits, tiles_m, to, vec, gather;
   int low_width, low_step;               // kToLow: elements of T for a column, from the first term to the second
   Runs low_runs;                         // kToC: low-rank pairs, r = 0: none
   const int* low_ids;
@@ -234,47 +235,103 @@ struct Pairs {
 // K blocks that a pair adds: rank up to 32: both terms of T in one; above: the first terms' blocks, then the second ones'
 __device__ __forceinline__ int low_blocks(int r) { return r <= 32 ? 1 : 2 * ((r + 63) / 64); }
 
-// 32 columns of row m (32 neighbouring rows to a warp) to a column-major array: out + column * ld + row.  `pairs`: an even number of rows
-// at 4-byte addresses, two lanes exchange halves: the even one has a column of rows m, m + 1, the odd one the next column.  Nothing
-// but predicates between the stores: with a branch for each a tile of 256 x 256 took 17000 cycles to write.
+// 16 lanes x 32 columns of tensor memory in the fragment layout of a matrix product: register 4 j + 2 s + e of lane l is row 8 s + l / 4,
+// column 8 j + 2 (l % 4) + e
+__device__ __forceinline__ void tmem_ld_frag32(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+// four 8 x 8 matrices to shared memory, transposed: lane 8 m + i gives the place of column i of matrix m
+__device__ __forceinline__ void stmatrix_x4_trans(uint32_t saddr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(saddr), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
+}
+
+// 32 rows x 32 columns of results of a warp of the epilogue to a column-major array.  The accumulator comes out of tensor memory in the
+// fragment layout, which stmatrix transposes into a box of shared memory (a column's 32 rows are 64 bytes, whose 16-byte pieces trade
+// places by column so that eight columns meet all banks); from there a warp stores eight columns of 64 bytes at a time.  f[0]: rows 0 .. 15,
+// f[1]: 16 .. 31 of m..; columns n.., of which `wide` are written; bits of `gone`: zeros; vec: 16-byte stores are possible.
+// (256 x 256: with stores of two rows, halves exchanged by shuffles, 8000 cycles; with boxes of 1 KB sent off by the copy engine 11500, for a
+// fence and a copy each.)
 template <bool BF16>
-__device__ __forceinline__ void store_columns(const uint32_t (&acc)[32], void* out_, long long ld, int m, int rows, int nc, bool pairs, uint32_t valid) {
+__device__ __forceinline__ void put_fragments(uint32_t (&f)[2][16], uint8_t* box, void* base, long long ld, int m, int n, int rows, int wide, uint32_t gone, bool vec) {
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-  T* out = reinterpret_cast<T*>(out_);
-  const bool odd = threadIdx.x & 1;
-  uint32_t v[16];
+  const int lane = threadIdx.x & 31;
+  if (m >= rows) return;
+  if (gone) {
+    const uint32_t bits = gone >> (2 * (lane & 3));
 #pragma unroll
-  for (int j = 0; j < 32; j += 2) {
-    float lo = __uint_as_float(acc[j]), hi = __uint_as_float(acc[j + 1]);
-    if (valid != 0xffffffffu) {
-      if (!((valid >> j) & 1u)) lo = 0.f;
-      if (!((valid >> (j + 1)) & 1u)) hi = 0.f;
-    }
-    v[j / 2] = pack2<BF16>(lo, hi);
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if ((bits >> (8 * (i >> 2) + (i & 1))) & 1u) f[h][i] = 0u;
   }
-  if (pairs) {
+  // a lane's place in the first box half: matrices are rows 0 .. 7 and 8 .. 15 of columns 0 .. 7, then of 8 .. 15
+  const int col = (lane & 7) + ((lane >> 4) << 3), piece = (lane >> 3) & 1, turn = (col >> 1) & 3;
+  const uint32_t at = smem_u32(box) + col * 64;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const uint32_t other = __shfl_xor_sync(0xffffffffu, v[j], 1);
-      v[j] = odd ? __byte_perm(other, v[j], 0x7632) : __byte_perm(v[j], other, 0x5410);
-    }
-    if (m < rows) {
-      T* dst = out + (m & ~1) + (odd ? ld : 0);
-      if (nc >= 32) {
+  for (int q = 0; q < 2; ++q) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j, dst += 2 * ld) *reinterpret_cast<uint32_t*>(dst) = v[j];
-      } else {
-        const int last = nc - (odd ? 1 : 0);
+    for (int h = 0; h < 2; ++h) {
+      uint32_t v[4];
 #pragma unroll
-        for (int j = 0; j < 16; ++j, dst += 2 * ld)
-          if (2 * j < last) *reinterpret_cast<uint32_t*>(dst) = v[j];
+      for (int x = 0; x < 4; ++x) {
+        const int i = 4 * (2 * q + (x >> 1)) + 2 * (x & 1);
+        v[x] = pack2<BF16>(__uint_as_float(f[h][i]), __uint_as_float(f[h][i + 1]));
       }
+      stmatrix_x4_trans(at + q * 1024 + (((2 * h + piece) ^ turn) << 4), v[0], v[1], v[2], v[3]);
     }
-  } else if (m < rows) {
-    unsigned short* dst = reinterpret_cast<unsigned short*>(out) + m;
+  }
+  __syncwarp();
+  const int c = lane >> 2, r = (lane & 3) * 8;
+  T* out = reinterpret_cast<T*>(base) + (long long)(n + c) * ld + m + r;
+  const uint8_t* from = box + c * 64 + (((lane & 3) ^ ((c >> 1) & 3)) << 4);
+  const bool whole = vec && m + r + 8 <= rows;
 #pragma unroll
-    for (int j = 0; j < 32; ++j, dst += ld)
-      if (j < nc) *dst = (unsigned short)(v[j / 2] >> (j & 1 ? 16 : 0));
+  for (int i = 0; i < 4; ++i, out += 8 * ld) {
+    if (i * 8 + c >= wide) continue;
+    const uint4 v = *reinterpret_cast<const uint4*>(from + i * 512);
+    if (whole) {
+      *reinterpret_cast<uint4*>(out) = v;
+    } else {
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (m + r + e < rows) reinterpret_cast<unsigned short*>(out)[e] = (unsigned short)(w[e >> 1] >> (e & 1 ? 16 : 0));
+    }
+  }
+  __syncwarp();
+}
+// Chunks of 32 columns through put(values, chunk), like drain_columns, in that layout
+template <int STEP, typename F>
+__device__ __forceinline__ void drain_fragments(uint32_t taddr, int c, int chunks, uint64_t* empty, F put) {
+  uint32_t a[2][16], b[2][16];
+  auto load = [&](uint32_t (&r)[2][16], int i) {
+    tmem_ld_frag32(taddr + i * 32, r[0]);
+    tmem_ld_frag32(taddr + (16u << 16) + i * 32, r[1]);
+  };
+  auto free = [&] {
+    tc_fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(empty);
+  };
+  if (c >= chunks) {
+    free();
+    return;
+  }
+  load(a, c);
+  while (true) {
+    tmem_wait_ld();
+    if (c + STEP < chunks) load(b, c + STEP); else free();
+    put(a, c);
+    if ((c += STEP) >= chunks) break;
+    tmem_wait_ld();
+    if (c + STEP < chunks) load(a, c + STEP); else free();
+    put(b, c);
+    if ((c += STEP) >= chunks) break;
   }
 }
 
@@ -509,6 +566,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     constexpr int kStep = MH == 2 ? 1 : 2;
     bool ok = true;
     int ti = 0;
+    uint8_t* box = smem + C::kOutOff + (warp - 2) * 2048;
     for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
       const Tile o = tile_of<MH>(g, tab, t, nkb);
       if (o.nt <= 0) continue;
@@ -528,15 +586,21 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
       const int chunks = MH == 2 && part * 128 >= g.M - o.m0 ? 0 : (o.nt + 31) / 32;
       float scale = 1.f;
       if (g.to != kToC) scale = g.scale ? g.scale[o.mat] : g.scale0;
-      auto put = [&](const uint32_t (&acc)[32], int c) {
-        const int nc = min(32, o.nt - c * 32), n = o.n0 + c * 32;
-        if (g.to == kToC) {
+      if (g.to == kToC) {
+        auto put = [&](uint32_t (&f)[2][16], int c) {
           uint32_t gone = 0u;
 #pragma unroll
           for (int q = 0; q < NT / 32; ++q)
             if (q == c) gone = none[q];
-          store_columns<BF16>(acc, reinterpret_cast<T*>(g.C) + (long long)n * g.ldc, g.ldc, m, g.M, nc, g.pairs != 0, ~gone);
-        } else if (g.to == kToParts) {
+          put_fragments<BF16>(f, box, g.C, g.ldc, m - lane, o.n0 + c * 32, g.M, o.nt - c * 32, gone, g.vec != 0);
+        };
+        drain_fragments<kStep>(taddr, MH == 2 ? 0 : part, chunks, &bars->acc_empty[ab], put);
+        ++ti;
+        continue;
+      }
+      auto put = [&](const uint32_t (&acc)[32], int c) {
+        const int nc = min(32, o.nt - c * 32), n = o.n0 + c * 32;
+        if (g.to == kToParts) {
           float* out = reinterpret_cast<float*>(g.C) + ((long long)o.split * g.runs.R + n) * g.M + m;
           if (m < g.M) {
 #pragma unroll
@@ -595,7 +659,7 @@ struct GradArgs {
   void* A;
   long long ld, stride;                  // between columns and matrices of the result
   int rows, cols, G, mats;
-  int tiles_r, tiles_c, pairs;
+  int tiles_r, tiles_c, vec;
   int fold, fold_step, along;            // fold: columns fold_step apart are the two terms of one; along: a row's columns are contiguous
   int* status;
 };
@@ -730,6 +794,7 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
     constexpr int kStep = MH == 2 ? 1 : 2;
     bool ok = true;
     int ti = 0;
+    uint8_t* box = smem + C::kOutOff + (warp - 2) * 2048;
     for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++ti) {
       const int a = (int)(t / each), q = (int)(t % each);
       const int r0 = (q % g.tiles_r) * (MH * 128), c0 = (q / g.tiles_r) * NT;
@@ -743,22 +808,11 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
       const uint32_t taddr = tmem + (static_cast<uint32_t>(wq * 32) << 16) + ab * C::kAccCols + (MH == 2 ? part * NT : 0);
       T* base = reinterpret_cast<T*>(g.A) + (long long)a * g.stride;
       const int width = g.fold ? g.fold_step : min(NT, g.cols - c0), chunks = MH == 2 && part * 128 >= g.rows - r0 ? 0 : (width + 31) / 32;
-      auto put = [&](const uint32_t (&got)[32], int c) {
-        uint32_t acc[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) acc[j] = some ? got[j] : 0u;
-        const int n = c0 + c * 32, nc = min(32, g.cols - n);
-        if (!g.along) {
-          store_columns<BF16>(acc, base + (long long)n * g.ld, g.ld, m, g.rows, nc, g.pairs != 0, 0xffffffffu);
-        } else if (m < g.rows) {
-          T* out = base + (long long)m * g.ld + n;
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (j < nc) out[j] = Elem<T>::from_f(__uint_as_float(acc[j]));
-        }
-      };
       if (!g.fold) {
-        drain_columns<kStep>(taddr, MH == 2 ? 0 : part, chunks, &bars->acc_empty[ab], put);
+        auto put = [&](uint32_t (&f)[2][16], int c) {
+          put_fragments<BF16>(f, box, base, g.ld, m - lane, c0 + c * 32, g.rows, g.cols - c0 - c * 32, some ? 0u : 0xffffffffu, g.vec != 0);
+        };
+        drain_fragments<kStep>(taddr, MH == 2 ? 0 : part, chunks, &bars->acc_empty[ab], put);
         continue;
       }
       for (int c = part; c < chunks; c += 2) {
@@ -767,11 +821,19 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
         tmem_ld32(taddr + g.fold_step + c * 32, more);
         tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) acc[j] = __float_as_uint(__uint_as_float(acc[j]) + __uint_as_float(more[j]));
-        put(acc, c);
+        for (int j = 0; j < 32; ++j) acc[j] = __float_as_uint(some ? __uint_as_float(acc[j]) + __uint_as_float(more[j]) : 0.f);
+        const int n = c0 + c * 32, nc = min(32, g.cols - n);
+        if (m < g.rows) {
+          T* dst = base + (g.along ? (long long)m * g.ld + n : (long long)n * g.ld + m);
+          const long long step = g.along ? 1 : g.ld;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (j < nc) dst[j * step] = Elem<T>::from_f(__uint_as_float(acc[j]));
+        }
+        __syncwarp();
       }
-      tc_fence_before();
       __syncwarp();
+      tc_fence_before();
       if (lane == 0) mbar_arrive(&bars->acc_empty[ab]);
     }
   }
@@ -992,15 +1054,19 @@ int sm_count() {
   return n;
 }
 
+struct Maps {
+  CUtensorMap a, x, b, t;
+};
+
 template <bool BF16, int MH, int NT>
-cudaError_t launch_fwd(const CUtensorMap& a, const CUtensorMap& x, const CUtensorMap& b, const CUtensorMap& t, FwdArgs g, long long most, cudaStream_t st) {
+cudaError_t launch_fwd(const Maps& m, FwdArgs g, long long most, cudaStream_t st) {
   using C = Cfg<MH, NT>;
   auto kern = grouped_umma_kernel<BF16, MH, NT>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (e != cudaSuccess) return e;
   g.tiles_m = (g.M + MH * 128 - 1) / (MH * 128);
   const long long grid = std::max<long long>(1, std::min<long long>(most * g.tiles_m * g.splits, sm_count()));
-  kern<<<(unsigned)grid, kThreads, C::kSmem, st>>>(a, x, b, t, g);
+  kern<<<(unsigned)grid, kThreads, C::kSmem, st>>>(m.a, m.x, m.b, m.t, g);
   count_launch();
   return cudaGetLastError();
 }
@@ -1058,12 +1124,12 @@ Shape shape_of(int M, int K, int R, int runs, bool may_split) {
 }
 
 template <bool BF16>
-cudaError_t fwd(const Shape& s, const CUtensorMap& a, const CUtensorMap& x, const CUtensorMap& b, const CUtensorMap& t, const FwdArgs& g, cudaStream_t st) {
-  if (s.mh == 2) return launch_fwd<BF16, 2, 256>(a, x, b, t, g, s.most, st);
-  if (s.nt() == 256) return launch_fwd<BF16, 1, 256>(a, x, b, t, g, s.most, st);
-  if (s.nt() == 128) return launch_fwd<BF16, 1, 128>(a, x, b, t, g, s.most, st);
-  if (s.nt() == 64) return launch_fwd<BF16, 1, 64>(a, x, b, t, g, s.most, st);
-  return launch_fwd<BF16, 1, 32>(a, x, b, t, g, s.most, st);
+cudaError_t fwd(const Shape& s, const Maps& m, const FwdArgs& g, cudaStream_t st) {
+  if (s.mh == 2) return launch_fwd<BF16, 2, 256>(m, g, s.most, st);
+  if (s.nt() == 256) return launch_fwd<BF16, 1, 256>(m, g, s.most, st);
+  if (s.nt() == 128) return launch_fwd<BF16, 1, 128>(m, g, s.most, st);
+  if (s.nt() == 64) return launch_fwd<BF16, 1, 64>(m, g, s.most, st);
+  return launch_fwd<BF16, 1, 32>(m, g, s.most, st);
 }
 int box_of(const Shape& s) { return s.nt() >= 128 ? 64 : 16; }
 
@@ -1124,25 +1190,24 @@ cudaError_t product(const GroupedArgs& g, int dtype, const Shape& s, int to, voi
   f.zero_rest = g.zero_rest && to == kToC;
   f.splits = s.splits;
   f.to = to;
-  f.pairs = (reinterpret_cast<uintptr_t>(out) & 3u) == 0 && g.ldc % 2 == 0 && g.M % 2 == 0;
   f.low_width = low_width(g.M);
   f.low_step = f.low_width / 2;
   f.status = g.status;
-  CUtensorMap ma, mx, mb, mt;
-  if (!encode_matrix(&ma, dtype, a, g.transA != 0) || !encode_columns(&mx, dtype, x, in_place ? 1 : box_of(s))) return cudaErrorInvalidValue;
-  mb = ma;
-  mt = mx;
+  Maps m;
+  if (!encode_matrix(&m.a, dtype, a, g.transA != 0) || !encode_columns(&m.x, dtype, x, in_place ? 1 : box_of(s))) return cudaErrorInvalidValue;
+  m.b = m.t = m.a;
+  f.vec = aligned16(out) && g.ldc % 8 == 0;
   if (g.low.r > 0 && to == kToC) {
     Operand b = matrices(g.low.B, g.low.transB != 0, g.M, g.low.r, g.low.ldb, g.low.strideB, g.low.n);
     if ((e = align_operand(b, ws, nullptr, st)) != cudaSuccess) return e;
     const Operand t{g.low.T, low_width(g.low.r), g.R, low_width(g.low.r), 0, 1, nullptr, 0};
-    if (!encode_matrix(&mb, dtype, b, g.low.transB != 0) || !encode_columns(&mt, dtype, t, box_of(s))) return cudaErrorInvalidValue;
+    if (!encode_matrix(&m.b, dtype, b, g.low.transB != 0) || !encode_columns(&m.t, dtype, t, box_of(s))) return cudaErrorInvalidValue;
     f.low_runs = Runs{g.low.offsets, g.low.run_len, g.low.runs, g.R};
     f.low_ids = g.low.ids;
     f.r = g.low.r; f.n = g.low.n;
     f.low_kmaj = g.low.transB;
   }
-  return dtype == NNLIB_B200_BF16 ? fwd<true>(s, ma, mx, mb, mt, f, st) : fwd<false>(s, ma, mx, mb, mt, f, st);
+  return dtype == NNLIB_B200_BF16 ? fwd<true>(s, m, f, st) : fwd<false>(s, m, f, st);
 }
 
 cudaError_t join(const GroupedArgs& g, int dtype, const Shape& s, const float* parts, const float* t, int t_splits, cudaStream_t st) {
@@ -1267,12 +1332,12 @@ cudaError_t grouped_umma_grad(const GroupedGradArgs& g, int dtype, int fold, voi
   a.fold = fold != 0;
   a.fold_step = fold ? low_width(a.cols) / 2 : 0;
   a.along = fold && (fold == 1) == (g.transA == 0);
-  a.pairs = (reinterpret_cast<uintptr_t>(g.A) & 3u) == 0 && g.lda % 2 == 0 && g.strideA % 2 == 0 && a.rows % 2 == 0;
   const int nt = fold ? low_width(a.cols) : 256;
   // 256 rows where the runs are long enough to hide an epilogue that nothing overlaps with
   const int mh = !fold && a.rows > 128 && g.R / std::max(1, g.mats) > 1024 ? 2 : 1;
   CUtensorMap mc, mx;
   if (!encode_columns(&mc, dtype, c, 64) || !encode_columns(&mx, dtype, x, 64)) return cudaErrorInvalidValue;
+  a.vec = aligned16(g.A) && g.lda % 8 == 0 && g.strideA % 8 == 0;
   const CUtensorMap& r = x_rows ? mx : mc;
   const CUtensorMap& q = x_rows ? mc : mx;
   const bool bf16 = dtype == NNLIB_B200_BF16;
