@@ -43,7 +43,8 @@ constexpr int kMaxRuns = 1024;
 constexpr int kAhead = 8;                // column tiles that a band of row tiles shares
 constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);   // 8-row groups 1024 bytes apart, 128-byte swizzle
 
-// The runs of a call with offsets, in shared memory: column tiles of the runs before run i, its first column, the column behind it.
+// Runs in shared memory: the product's own where they have offsets (column tiles of the runs before run i, its first column, the column
+// behind it), else those of low-rank pairs (cum: the pair).  From global memory a tile's search for its pairs took 7000 cycles.
 struct Table {
   int cum[kMaxRuns + 8], begin[kMaxRuns], end[kMaxRuns];
 };
@@ -124,7 +125,17 @@ __host__ __device__ __forceinline__ int tile_count(int n, int cap) {
 
 // Fills the table (runs of one length need none).  By the whole block.
 __device__ void count_tiles(const FwdArgs& g, Table& tab, RunSearch& s) {
-  if (!g.runs.offsets) return;
+  if (!g.runs.offsets) {
+    if (g.r > 0 && g.low_runs.runs <= kMaxRuns) {
+      for (int i = threadIdx.x; i < g.low_runs.runs; i += kThreads) {
+        tab.cum[i] = g.low_ids[i];
+        tab.begin[i] = g.low_runs.begin(i);
+        tab.end[i] = g.low_runs.end(i);
+      }
+      __syncthreads();
+    }
+    return;
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int carry = 0;
   for (int i0 = 0; i0 < g.G; i0 += kThreads) {
@@ -210,23 +221,27 @@ __device__ __forceinline__ Tile tile_of(const FwdArgs& g, const Table& tab, long
 
 // Runs of low-rank pairs that have columns in a tile, neighbours of the same pair as one.
 struct Pairs {
+  const Table* tab;                      // NULL: more runs than it holds
   int b, end, id, lo, hi;
-  __device__ __forceinline__ Pairs(const FwdArgs& g, int n0, int nt) : end(n0 + nt) {
+  __device__ __forceinline__ int first_of(const FwdArgs& g, int i) const { return tab ? tab->begin[i] : g.low_runs.begin(i); }
+  __device__ __forceinline__ int end_of(const FwdArgs& g, int i) const { return tab ? tab->end[i] : g.low_runs.end(i); }
+  __device__ __forceinline__ int id_of(const FwdArgs& g, int i) const { return tab ? tab->cum[i] : g.low_ids[i]; }
+  __device__ __forceinline__ Pairs(const FwdArgs& g, const Table& t, int n0, int nt) : tab(g.low_runs.runs <= kMaxRuns ? &t : nullptr), end(n0 + nt) {
     int a = 0, c = g.low_runs.runs;                        // the first run that ends behind n0
     while (a < c) {
       const int mid = (a + c) >> 1;
-      if (g.low_runs.end(mid) > n0) c = mid; else a = mid + 1;
+      if (end_of(g, mid) > n0) c = mid; else a = mid + 1;
     }
     b = a;
   }
   __device__ __forceinline__ bool next(const FwdArgs& g, int n0) {
     for (; b < g.low_runs.runs; ++b) {
-      lo = max(g.low_runs.begin(b), n0);
+      lo = max(first_of(g, b), n0);
       if (lo >= end) return false;
-      hi = min(g.low_runs.end(b), end);
-      id = g.low_ids[b];
+      hi = min(end_of(g, b), end);
+      id = id_of(g, b);
       if (lo >= hi || id < 0 || id >= g.n) continue;
-      for (++b; b < g.low_runs.runs && hi < end && g.low_ids[b] == id && g.low_runs.begin(b) == hi; ++b) hi = max(hi, min(g.low_runs.end(b), end));
+      for (++b; b < g.low_runs.runs && hi < end && id_of(g, b) == id && first_of(g, b) == hi; ++b) hi = max(hi, min(end_of(g, b), end));
       return true;
     }
     return false;
@@ -466,7 +481,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         for (int kb = o.kb0; kb < o.kb1 && ok; ++kb)
           ok = fill(&tm_a, kb * kBK, g.a_same ? 0 : o.mat, g.a_kmaj != 0, &tm_x, kb * kBK, o, g.gather != 0, four);
         if (g.r > 0 && ok) {
-          Pairs p(g, o.n0, o.nt);
+          Pairs p(g, tab, o.n0, o.nt);
           const int blocks = low_blocks(g.r), half = blocks / 2;
           while (ok && p.next(g, o.n0))
             for (int q = 0; q < blocks && ok; ++q) ok = fill(&tm_b, (half ? q % half : 0) * kBK, p.id, g.low_kmaj != 0, &tm_t, q * kBK, o, false, four);
@@ -522,7 +537,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
       at.s = __shfl_sync(0xffffffffu, at.s, 0);
       at.round = __shfl_sync(0xffffffffu, at.round, 0);
       if (g.r > 0 && ok) {
-        Pairs p(g, o.n0, o.nt);
+        Pairs p(g, tab, o.n0, o.nt);
         const int blocks = low_blocks(g.r), half = blocks / 2;
         const uint32_t id_low = idesc_of(BF16, round16(o.nt), !g.low_kmaj, false), step = g.low_kmaj ? 32 >> 4 : 2048 >> 4;
         while (ok && p.next(g, o.n0)) {
@@ -672,6 +687,7 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   Bars* bars = reinterpret_cast<Bars*>(smem + C::kBarOff);
+  Table& tab = *reinterpret_cast<Table*>(smem + C::kTableOff);
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -690,15 +706,26 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
     tmem_alloc(&bars->tmem_base, C::kTmemCols);
     tmem_relinquish();
   }
+  const bool held = g.G <= kMaxRuns;
+  if (held) {
+    for (int i = threadIdx.x; i < g.G; i += kThreads) {
+      tab.cum[i] = g.ids ? g.ids[i] : i;
+      tab.begin[i] = g.runs.begin(i);
+      tab.end[i] = g.runs.end(i);
+    }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
   const bool start_ok = (*abort_flag == 0);
   const long long each = (long long)g.tiles_r * g.tiles_c, tiles = each * g.mats;
-  // blocks of a tile, run by run: begin(b), end(b) of the runs b of matrix a
+  // blocks of a tile, run by run: the runs of matrix a
   auto first_run = [&](int a) { return g.ids ? 0 : a; };
   auto last_run = [&](int a) { return g.ids ? g.G : min(a + 1, g.G); };
+  auto is_of = [&](int b, int a) { return !g.ids || (held ? tab.cum[b] : g.ids[b]) == a; };
+  auto begin_of = [&](int b) { return held ? tab.begin[b] : g.runs.begin(b); };
+  auto end_of = [&](int b) { return held ? tab.end[b] : g.runs.end(b); };
 
   if (start_ok && (warp == 0 || warp >= 10)) {
     const int me = warp == 0 ? 0 : warp - 9;
@@ -712,9 +739,9 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
         const int a = (int)(t / each), q = (int)(t % each);
         const int r0 = (q % g.tiles_r) * (MH * 128), c0 = (q / g.tiles_r) * NT;
         for (int b = first_run(a); b < last_run(a) && ok; ++b) {
-          if (g.ids && g.ids[b] != a) continue;
-          const int end = g.runs.end(b);
-          for (int i0 = g.runs.begin(b); i0 < end; i0 += kBK, at.next()) {
+          if (!is_of(b, a)) continue;
+          const int end = end_of(b);
+          for (int i0 = begin_of(b); i0 < end; i0 += kBK, at.next()) {
             const bool mine = turn == me;
             if (++turn == kProducers) turn = 0;
             if (!mine) continue;
@@ -754,36 +781,51 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
       tc_fence_after();
       bool begun = false;
       for (int b = first_run(a); b < last_run(a) && ok; ++b) {
-        if (g.ids && g.ids[b] != a) continue;
-        const int end = g.runs.end(b);
-        for (int i0 = g.runs.begin(b); i0 < end; i0 += kBK, at.next()) {
-          const int s = at.s, here = min(kBK, end - i0), steps = (here + 15) >> 4;
-          ok = mbar_wait_warp(&bars->full[s], (uint32_t)at.round & 1u, abort_flag);
+        if (!is_of(b, a)) continue;
+        const int end = end_of(b);
+        const int begin = begin_of(b);
+        // a block of which the first `here` columns are the run's
+        auto multiply = [&](int here) {
+          tc_fence_after();
+          const uint32_t r = base + at.s * (C::kStage >> 4), c = r + (C::kA >> 4);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            if (kk * 16 < here) {
+#pragma unroll
+              for (int h = 0; h < MH; ++h)
+                umma_ss_lohi(acc + h * NT, r + h * (kHalfBytes >> 4) + kk * (2048 >> 4), c + kk * (2048 >> 4), kDescHi, idesc, (begun || kk > 0) ? 1u : 0u);
+            }
+          }
+          umma_commit(&bars->empty[at.s]);
+          begun = true;
+        };
+        // whole blocks are one lane's, a last one is the warp's
+        const int whole = (end - begin) / kBK, rest = (end - begin) % kBK;
+        int good = 1;
+        if (lane == 0) {
+          for (int i = 0; i < whole; ++i, at.next()) {
+            if (!mbar_wait(&bars->full[at.s], (uint32_t)at.round & 1u, abort_flag)) { good = 0; break; }
+            multiply(kBK);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, good, 0) != 0;
+        at.s = __shfl_sync(0xffffffffu, at.s, 0);
+        at.round = __shfl_sync(0xffffffffu, at.round, 0);
+        if (ok && rest) {
+          ok = mbar_wait_warp(&bars->full[at.s], (uint32_t)at.round & 1u, abort_flag);
           if (!ok) break;
-          if (here & 15) {                                 // another run's columns, or nobody's
+          if (rest & 15) {                                 // another run's columns, or nobody's
             __syncwarp();
-            for (int i = here * 8 + lane; i < steps * 16 * 8; i += 32) {
+            for (int i = rest * 8 + lane; i < round16(rest) * 8; i += 32) {
 #pragma unroll
               for (int x = 0; x < C::kStage / (kHalfBytes / 2); ++x)
-                *reinterpret_cast<uint4*>(smem + s * C::kStage + x * (kHalfBytes / 2) + i * 16) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(smem + at.s * C::kStage + x * (kHalfBytes / 2) + i * 16) = make_uint4(0, 0, 0, 0);
             }
             fence_proxy_async_smem();
             __syncwarp();
           }
-          if (lane == 0) {
-            tc_fence_after();
-            const uint32_t r = base + s * (C::kStage >> 4), c = r + (C::kA >> 4);
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-              if (kk < steps) {
-#pragma unroll
-                for (int h = 0; h < MH; ++h)
-                  umma_ss_lohi(acc + h * NT, r + h * (kHalfBytes >> 4) + kk * (2048 >> 4), c + kk * (2048 >> 4), kDescHi, idesc, (begun || kk > 0) ? 1u : 0u);
-              }
-            }
-            umma_commit(&bars->empty[s]);
-          }
-          begun = true;
+          if (lane == 0) multiply(rest);
+          at.next();
           __syncwarp();
         }
       }
@@ -800,7 +842,7 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
       const int r0 = (q % g.tiles_r) * (MH * 128), c0 = (q / g.tiles_r) * NT;
       const int ab = ti % C::kAccBufs;
       bool some = false;                                   // a matrix that no column met is zeros
-      for (int b = first_run(a); b < last_run(a) && !some; ++b) some = (!g.ids || g.ids[b] == a) && g.runs.end(b) > g.runs.begin(b);
+      for (int b = first_run(a); b < last_run(a) && !some; ++b) some = is_of(b, a) && end_of(b) > begin_of(b);
       ok = mbar_wait_warp(&bars->acc_full[ab], (uint32_t)(ti / C::kAccBufs) & 1u, abort_flag);
       if (!ok) break;
       tc_fence_after();
