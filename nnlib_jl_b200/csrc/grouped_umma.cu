@@ -51,23 +51,27 @@ struct Table {
 constexpr int kTableBytes = sizeof(Table);
 constexpr int kOutBytes = 8 * 2048;      // a box of 32 rows x 32 columns for each warp of the epilogue
 
-template <int MH, int NT>
+// PAIR: two CTAs of a cluster on one tile, 128 rows and half of the columns' operand each
+template <int NT, bool PAIR>
 struct Cfg {
-  static constexpr int kA = MH * kHalfBytes, kX = NT * 128, kStage = kA + kX;
+  // K blocks of 64 in a stage: a pair's products are as short as half a tile's, and each wait, commit and turn of the loop takes the thread that
+  // issues them 370 cycles
+  static constexpr int kSub = PAIR ? 2 : 1;
+  static constexpr int kA = kHalfBytes, kX = NT * 128 / (PAIR ? 2 : 1), kXOff = kSub * kA, kStage = kSub * (kA + kX);
   static constexpr int kRoom = 226 * 1024 - kTableBytes - kOutBytes - 512;
   static constexpr int kStages = kRoom / kStage > 10 ? 10 : kRoom / kStage;
-  static constexpr int kAccCols = MH * NT, kAccBufs = kAccCols <= 256 ? 2 : 1;
-  static constexpr int kTmemCols = kAccCols * kAccBufs < 32 ? 32 : kAccCols * kAccBufs;
+  static constexpr int kTmemCols = 2 * NT;               // two accumulators
   static constexpr int kBox = NT >= 128 ? 64 : 16;       // columns of X that one copy brings
   static constexpr int kOutOff = kStages * kStage, kTableOff = kOutOff + kOutBytes, kBarOff = kTableOff + kTableBytes;
   static constexpr int kSmem = kBarOff + 512 + 1024;
 };
-static_assert(Cfg<2, 256>::kStages == 3 && Cfg<1, 256>::kStages == 4 && Cfg<1, 32>::kStages == 9, "ring depth");
-static_assert(Cfg<2, 256>::kSmem <= 232448 && Cfg<1, 256>::kSmem <= 232448 && Cfg<1, 128>::kSmem <= 232448 && Cfg<1, 64>::kSmem <= 232448 &&
-              Cfg<1, 32>::kSmem <= 232448, "shared memory budget");
+static_assert(Cfg<256, true>::kStages == 3 && Cfg<256, false>::kStages == 4 && Cfg<32, false>::kStages == 9, "ring depth");
+static_assert(Cfg<256, true>::kSmem <= 232448 && Cfg<256, false>::kSmem <= 232448 && Cfg<128, false>::kSmem <= 232448 && Cfg<64, false>::kSmem <= 232448 &&
+              Cfg<32, false>::kSmem <= 232448, "shared memory budget");
 
 struct Bars {
   uint64_t full[10], empty[10], acc_full[2], acc_empty[2];
+  uint64_t side[6];                      // PAIR, stages of which columns are to be cleared: the second CTA's copies are there; in the first CTA: are cleared
   uint32_t tmem_base;
   int abort_flag;
   RunSearch search;
@@ -107,11 +111,182 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* m, uin
                : "memory");
 }
 __device__ __forceinline__ uint32_t desc_lo(uint32_t addr) { return ((addr & 0x3FFFFu) >> 4) | ((uint32_t)((kHalfBytes / 2) >> 4) << 16); }
+// ---- two CTAs as one
+__device__ __forceinline__ int cluster_rank() {
+  int r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// an arrival at the first CTA's barrier
+__device__ __forceinline__ void arrive_first(uint64_t* bar) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(bar)));
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
+}
+// copies of a pair: their bytes count at the first CTA's barrier, whose address this is in the cluster
+__device__ __forceinline__ uint32_t first_barrier(uint64_t* bar) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(bar)));
+  return a;
+}
+__device__ __forceinline__ void pair_load_2d(void* dst, const CUtensorMap* m, uint32_t bar, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+               "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1)
+               : "memory");
+}
+__device__ __forceinline__ void pair_load_3d(void* dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+               "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+// mbar_wait for a barrier that the other CTA arrives at
+__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  auto look = [&] {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t"
+        "}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+  };
+#pragma unroll 1
+  for (int it = 0; it < 4096; ++it)
+    if (look()) return true;
+  const unsigned long long t0 = globaltimer_ns();
+#pragma unroll 1
+  while (true) {
+#pragma unroll 1
+    for (int it = 0; it < 32; ++it)
+      if (look()) return true;
+    if (*abort_flag) return false;
+    if (globaltimer_ns() - t0 > kWaitLimitNs) {
+      *abort_flag = 1;
+      return false;
+    }
+  }
+}
+template <bool PAIR>
+__device__ __forceinline__ bool wait_of(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, PAIR ? wait_cluster(bar, parity, abort_flag) : mbar_wait(bar, parity, abort_flag)) != 0;
+}
+// One thread's instructions, called by a whole warp in step: what they take is then computed in uniform registers, where the instruction
+// wants it.
+template <bool PAIR>
+__device__ __forceinline__ void multiply_add(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+#define NB_MMA(GROUP)                                                                                    \
+  asm volatile(                                                                                          \
+      "{\n\t"                                                                                            \
+      ".reg .pred p, one;\n\t"                                                                           \
+      ".reg .b64 da, db;\n\t"                                                                            \
+      "mov.b64 da, {%1, %3};\n\t"                                                                        \
+      "mov.b64 db, {%2, %3};\n\t"                                                                        \
+      "setp.ne.b32 p, %5, 0;\n\t"                                                                        \
+      "elect.sync _|one, 0xffffffff;\n\t"                                                                \
+      "@one tcgen05.mma.cta_group::" GROUP ".kind::f16 [%0], da, db, %4, p;\n\t"                         \
+      "}" ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(accumulate)                      \
+      : "memory")
+  if constexpr (PAIR) NB_MMA("2");
+  else NB_MMA("1");
+#undef NB_MMA
+}
+// an arrival (PAIR: at both CTAs' barriers) when what was issued so far has completed
+template <bool PAIR>
+__device__ __forceinline__ void commit_to(uint64_t* bar) {
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n\t"
+        ".reg .pred one;\n\t"
+        "elect.sync _|one, 0xffffffff;\n\t"
+        "@one tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t"
+        "}" ::"r"(smem_u32(bar)), "h"((unsigned short)3)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t"
+        ".reg .pred one;\n\t"
+        "elect.sync _|one, 0xffffffff;\n\t"
+        "@one tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t"
+        "}" ::"r"(smem_u32(bar))
+        : "memory");
+}
+// a wait of a warp in step
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0;
+}
+template <bool PAIR>
+__device__ __forceinline__ void take_tmem(uint32_t* result, uint32_t columns) {
+  if constexpr (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(result)), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    tmem_alloc(result, columns);
+    tmem_relinquish();
+  }
+}
+template <bool PAIR>
+__device__ __forceinline__ void give_tmem(uint32_t addr, uint32_t columns) {
+  if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(columns));
+  else tmem_dealloc(addr, columns);
+}
+template <bool PAIR>
+__device__ __forceinline__ void sync_all() {
+  if constexpr (PAIR) {
+    __syncwarp();
+    cluster_sync();
+  } else {
+    __syncthreads();
+  }
+}
+// barriers, tensor memory and the abort flag of a CTA; the whole block's
+template <int NT, bool PAIR>
+__device__ __forceinline__ void set_up(Bars* bars) {
+  using C = Cfg<NT, PAIR>;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 1);
+      if (PAIR) mbar_init(&bars->side[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars->acc_full[s], 1);
+      mbar_init(&bars->acc_empty[s], PAIR ? 16 : 8);
+    }
+    bars->abort_flag = *reinterpret_cast<volatile int*>(&g_grouped_abort);
+    fence_mbar_init();
+  }
+  if ((threadIdx.x >> 5) == 1) take_tmem<PAIR>(&bars->tmem_base, C::kTmemCols);
+}
+template <int NT, bool PAIR>
+__device__ __forceinline__ void tear_down(Bars* bars, uint32_t tmem, int* status) {
+  tc_fence_before();
+  sync_all<PAIR>();                                       // (the first CTA's products read the other's shared memory)
+  if ((threadIdx.x >> 5) == 1) {
+    tc_fence_after();
+    give_tmem<PAIR>(tmem, Cfg<NT, PAIR>::kTmemCols);
+  }
+  if (threadIdx.x == 0 && *reinterpret_cast<volatile int*>(&bars->abort_flag)) {
+    atomicExch(&g_grouped_abort, 1);
+    if (status) atomicExch(status, NNLIB_B200_TIMEOUT);
+  }
+  sync_all<PAIR>();
+}
+template <bool PAIR>
 __device__ __forceinline__ uint32_t idesc_of(bool bf16, int n, bool a_mn, bool b_mn) {
   return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
-         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+         ((uint32_t)(n >> 3) << 17) | ((uint32_t)((PAIR ? 256 : 128) >> 4) << 24);
 }
 __device__ __forceinline__ int round16(int n) { return (n + 15) & ~15; }
+// columns that a product of n takes (PAIR: half of them from each CTA)
+template <bool PAIR>
+__device__ __forceinline__ int product_columns(int n) { return PAIR ? (n + 31) & ~31 : round16(n); }
 
 // Width of the tiles of a run of n columns, and their number: at most cap (a multiple of 16) and as even as multiples of 16 allow.
 __host__ __device__ __forceinline__ int tile_width(int n, int cap) {
@@ -175,12 +350,17 @@ struct Ring {
   __device__ __forceinline__ void next() {
     if (++s == N) { s = 0; ++round; }
   }
+  __device__ __forceinline__ void skip(int n) {
+    s += n;
+    round += s / N;
+    s %= N;
+  }
 };
 
 struct Tile {
   int run, mat, n0, nt, m0, kb0, kb1, split;
 };
-template <int MH>
+template <bool PAIR>
 __device__ __forceinline__ Tile tile_of(const FwdArgs& g, const Table& tab, long long t, int nkb) {
   Tile o;
   o.split = (int)(t % g.splits);
@@ -211,7 +391,7 @@ __device__ __forceinline__ Tile tile_of(const FwdArgs& g, const Table& tab, long
   const int w = tile_width(end - begin, g.cap);
   o.run = run;
   o.mat = g.ids ? g.ids[run] : run;
-  o.m0 = (in / wide) * (MH * 128);
+  o.m0 = (in / wide) * (PAIR ? 256 : 128);
   o.n0 = begin + (band * kAhead + in % wide) * w;
   o.nt = o.mat >= 0 && o.mat < g.mats ? min(w, end - o.n0) : 0;      // (0: nothing to do)
   o.kb0 = (int)((long long)nkb * o.split / g.splits);
@@ -321,8 +501,9 @@ __device__ __forceinline__ void put_fragments(uint32_t (&f)[2][16], uint8_t* box
   __syncwarp();
 }
 // Chunks of 32 columns through put(values, chunk), like drain_columns, in that layout
-template <int STEP, typename F>
+template <bool PAIR, typename F>
 __device__ __forceinline__ void drain_fragments(uint32_t taddr, int c, int chunks, uint64_t* empty, F put) {
+  constexpr int STEP = 2;
   uint32_t a[2][16], b[2][16];
   auto load = [&](uint32_t (&r)[2][16], int i) {
     tmem_ld_frag32(taddr + i * 32, r[0]);
@@ -331,7 +512,10 @@ __device__ __forceinline__ void drain_fragments(uint32_t taddr, int c, int chunk
   auto free = [&] {
     tc_fence_before();
     __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(empty);
+    if ((threadIdx.x & 31) == 0) {
+      if (PAIR) arrive_first(empty);
+      else mbar_arrive(empty);
+    }
   };
   if (c >= chunks) {
     free();
@@ -350,15 +534,19 @@ __device__ __forceinline__ void drain_fragments(uint32_t taddr, int c, int chunk
   }
 }
 
-// Chunks of 32 columns from..to, every STEP-th, of this warp's rows of an accumulator through put(values, chunk): the next chunk is on
+// Chunks c, c + 2, ... of 32 columns of this warp's rows of an accumulator through put(values, chunk): the next chunk is on
 // its way out of tensor memory while one is put.  Then the accumulator is free as far as this warp goes.
-template <int STEP, typename F>
+template <bool PAIR, typename F>
 __device__ __forceinline__ void drain_columns(uint32_t taddr, int c, int chunks, uint64_t* empty, F put) {
+  constexpr int STEP = 2;
   uint32_t a[32], b[32];
   auto free = [&] {
     tc_fence_before();
     __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(empty);
+    if ((threadIdx.x & 31) == 0) {
+      if (PAIR) arrive_first(empty);
+      else mbar_arrive(empty);
+    }
   };
   if (c >= chunks) {
     free();
@@ -377,11 +565,11 @@ __device__ __forceinline__ void drain_columns(uint32_t taddr, int c, int chunks,
   }
 }
 
-template <bool BF16, int MH, int NT>
+template <bool BF16, int NT, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_b,
                     const __grid_constant__ CUtensorMap tm_t, const __grid_constant__ FwdArgs g) {
-  using C = Cfg<MH, NT>;
+  using C = Cfg<NT, PAIR>;
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -391,27 +579,13 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int nkb = (g.K + kBK - 1) / kBK;
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(&bars->full[s], 1);
-      mbar_init(&bars->empty[s], 1);
-    }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&bars->acc_full[s], 1);
-      mbar_init(&bars->acc_empty[s], 8);
-    }
-    bars->abort_flag = *reinterpret_cast<volatile int*>(&g_grouped_abort);
-    fence_mbar_init();
-  }
-  if (warp == 1) {
-    tmem_alloc(&bars->tmem_base, C::kTmemCols);
-    tmem_relinquish();
-  }
+  const int rank = PAIR ? cluster_rank() : 0, worker = PAIR ? blockIdx.x >> 1 : blockIdx.x, workers = PAIR ? gridDim.x >> 1 : gridDim.x;
+  set_up<NT, PAIR>(bars);
   count_tiles(g, tab, bars->search);
   tc_fence_before();
-  __syncthreads();
+  sync_all<PAIR>();
   tc_fence_after();
-  const uint32_t tmem = bars->tmem_base;
+  const uint32_t tmem = __reduce_or_sync(0xffffffffu, bars->tmem_base);     // (in a uniform register)
   const bool start_ok = (*abort_flag == 0);
   const long long columns = g.runs.offsets ? tab.cum[g.G] : (long long)g.G * tile_count((int)g.runs.len, g.cap);
   const long long tiles = columns * g.tiles_m * g.splits;
@@ -428,7 +602,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     int turn = 0;
     // One stage, if it is this warp's turn: the boxes of the matrix (map ma, block ka of matrix za) and of the columns (map mx, block kx).  Lane 0 issues them all;
     // gathered columns are the other lanes' too, four each.
-    auto fill = [&](const CUtensorMap* ma, int ka, int za, bool kmaj, const CUtensorMap* mx, int kx, const Tile& o, bool gather, const int4& four) {
+    auto fill = [&](const CUtensorMap* ma, int ka, int za, bool kmaj, const CUtensorMap* mx, int kx, const Tile& o, bool gather, const int4& four, bool side, int subs) {
       const bool mine = turn == me;
       if (++turn == kProducers) turn = 0;
       if (!mine) {
@@ -437,22 +611,34 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
       }
       const int s = at.s;
       uint8_t* da = smem + s * C::kStage;
-      uint8_t* dx = da + C::kA;
+      uint8_t* dx = da + C::kXOff;
       int good = 1;
       if (lane == 0) {
         if (at.round > 0) good = mbar_wait(&bars->empty[s], (uint32_t)(at.round - 1) & 1u, abort_flag) ? 1 : 0;
         if (good) {
           // (rows of shared memory behind the last row of the matrix keep what they have: no row sees another)
-          const int boxes = (o.nt + C::kBox - 1) / C::kBox, rows = min(MH * 128, g.M - o.m0);
-          const int of_a = kmaj ? (rows + 127) / 128 : (rows + 63) / 64, bytes_a = of_a * (kmaj ? kHalfBytes : kHalfBytes / 2);
-          mbar_arrive_expect_tx(&bars->full[s], bytes_a + (gather ? round16(o.nt) * 128 : boxes * C::kBox * 128));
-          if (kmaj) {
-            for (int i = 0; i < of_a; ++i) tma_load_3d(da + i * kHalfBytes, ma, &bars->full[s], ka, o.m0 + i * 128, za);
+          const int mine = PAIR ? product_columns<true>(o.nt) / 2 : o.nt, n0 = o.n0 + rank * mine, m0 = o.m0 + rank * 128;
+          const int boxes = (mine + C::kBox - 1) / C::kBox;
+          auto of_a = [&](int first) {
+            const int rows = max(0, min(128, g.M - first));
+            return kmaj ? (rows + 127) / 128 : (rows + 63) / 64;
+          };
+          const int n_a = of_a(m0), box_a = kmaj ? kHalfBytes : kHalfBytes / 2;
+          const int bytes = n_a * box_a + (gather ? round16(o.nt) * 128 : boxes * C::kBox * 128);
+          if (!PAIR || side) {
+            uint64_t* bar = PAIR && rank ? &bars->side[s] : &bars->full[s];
+            mbar_arrive_expect_tx(bar, bytes);             // (one block: such stages of a pair are low-rank pairs')
+            for (int i = 0; i < n_a; ++i) tma_load_3d(da + i * box_a, ma, bar, kmaj ? ka : m0 + i * 64, kmaj ? m0 : ka, za);
+            if (!gather)
+              for (int i = 0; i < boxes; ++i) tma_load_2d(dx + i * C::kBox * 128, mx, bar, kx, n0 + i * C::kBox);
           } else {
-            for (int i = 0; i < of_a; ++i) tma_load_3d(da + i * (kHalfBytes / 2), ma, &bars->full[s], o.m0 + i * 64, ka, za);
+            if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], subs * (bytes + of_a(m0 + 128) * box_a + boxes * C::kBox * 128));
+            const uint32_t bar = first_barrier(&bars->full[s]);
+            for (int u = 0; u < subs; ++u, ka += kBK, kx += kBK) {
+              for (int i = 0; i < n_a; ++i) pair_load_3d(da + u * C::kA + i * box_a, ma, bar, kmaj ? ka : m0 + i * 64, kmaj ? m0 : ka, za);
+              for (int i = 0; i < boxes; ++i) pair_load_2d(dx + u * C::kX + i * C::kBox * 128, mx, bar, kx, n0 + i * C::kBox);
+            }
           }
-          if (!gather)
-            for (int i = 0; i < boxes; ++i) tma_load_2d(dx + i * C::kBox * 128, mx, &bars->full[s], kx, o.n0 + i * C::kBox);
         }
       }
       at.next();
@@ -464,8 +650,8 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     };
     // (all lanes stay together where columns are gathered; elsewhere the others have nothing to do)
     if (g.gather || lane == 0) {
-      for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-        const Tile o = tile_of<MH>(g, tab, t, nkb);
+      for (long long t = worker; t < tiles && ok; t += workers) {
+        const Tile o = tile_of<PAIR>(g, tab, t, nkb);
         if (o.nt <= 0) continue;
         int4 four = make_int4(0, 0, 0, 0);
         if (g.gather) {
@@ -478,13 +664,15 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
           }
           four = make_int4(c[0], c[1], c[2], c[3]);
         }
-        for (int kb = o.kb0; kb < o.kb1 && ok; ++kb)
-          ok = fill(&tm_a, kb * kBK, g.a_same ? 0 : o.mat, g.a_kmaj != 0, &tm_x, kb * kBK, o, g.gather != 0, four);
+        for (int kb = o.kb0; kb < o.kb1 && ok; kb += C::kSub)
+          ok = fill(&tm_a, kb * kBK, g.a_same ? 0 : o.mat, g.a_kmaj != 0, &tm_x, kb * kBK, o, g.gather != 0, four, false, min(C::kSub, o.kb1 - kb));
         if (g.r > 0 && ok) {
           Pairs p(g, tab, o.n0, o.nt);
           const int blocks = low_blocks(g.r), half = blocks / 2;
-          while (ok && p.next(g, o.n0))
-            for (int q = 0; q < blocks && ok; ++q) ok = fill(&tm_b, (half ? q % half : 0) * kBK, p.id, g.low_kmaj != 0, &tm_t, q * kBK, o, false, four);
+          while (ok && p.next(g, o.n0)) {
+            const bool side = p.lo > o.n0 || p.hi < o.n0 + product_columns<PAIR>(o.nt);
+            for (int q = 0; q < blocks && ok; ++q) ok = fill(&tm_b, (half ? q % half : 0) * kBK, p.id, g.low_kmaj != 0, &tm_t, q * kBK, o, false, four, side, 1);
+          }
         }
       }
     }
@@ -497,95 +685,90 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
       }
     }
   } else if (start_ok && warp == 1) {
-    // -------------------------------------------------------------- MMA issuer
+    // -------------------------------------------------------------- MMA issuer; in the second CTA of a pair what clears its columns of a stage and says so
     bool ok = true;
     Ring<C::kStages> at;
     int ti = 0;
     const uint32_t base = desc_lo(smem_u32(smem));
-    for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const Tile o = tile_of<MH>(g, tab, t, nkb);
+    const bool issues = !PAIR || rank == 0;
+    uint32_t sides = 0u;                                   // phases of the barriers `side`
+    for (long long t = worker; t < tiles && ok; t += workers) {
+      const Tile o = tile_of<PAIR>(g, tab, t, nkb);
       if (o.nt <= 0) continue;
-      const int ab = ti % C::kAccBufs;
-      const uint32_t acc = tmem + ab * C::kAccCols;
-      const uint32_t id_main = idesc_of(BF16, round16(o.nt), !g.a_kmaj, false);
-      const bool upper = MH == 2 && g.M - o.m0 > 128;      // the second 128 rows are there
-      int good = 1;
-      if (lane == 0) {
-        if (ti >= C::kAccBufs) good = mbar_wait(&bars->acc_empty[ab], (uint32_t)((ti / C::kAccBufs) + 1) & 1u, abort_flag) ? 1 : 0;
+      const int ab = ti & 1, wide = product_columns<PAIR>(o.nt);
+      const uint32_t acc = tmem + ab * NT;
+      if (issues) {
+        const uint32_t id_main = idesc_of<PAIR>(BF16, wide, !g.a_kmaj, false);
+        if (ti >= 2) ok = wait_of<PAIR>(&bars->acc_empty[ab], (uint32_t)((ti >> 1) + 1) & 1u, abort_flag);
         tc_fence_after();
         const uint32_t step = g.a_kmaj ? 32 >> 4 : 2048 >> 4;
-        for (int kb = o.kb0; kb < o.kb1 && good; ++kb) {
+        for (int kb = o.kb0; kb < o.kb1 && ok; kb += C::kSub) {
           const int s = at.s;
-          if (!mbar_wait(&bars->full[s], (uint32_t)at.round & 1u, abort_flag)) { good = 0; break; }
+          ok = warp_wait(&bars->full[s], (uint32_t)at.round & 1u, abort_flag);
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t a = base + s * (C::kStage >> 4), x = a + (C::kA >> 4);
-          const int steps = min(4, (g.K - kb * kBK + 15) >> 4);
+          const uint32_t a = base + s * (C::kStage >> 4), x = a + (C::kXOff >> 4);
+          const int steps = (min(g.K, o.kb1 * kBK) - kb * kBK + 15) >> 4;    // of 16, four to a block
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            if (kk < steps) {
-#pragma unroll
-              for (int h = 0; h < MH; ++h)
-                if (h == 0 || upper)
-                  umma_ss_lohi(acc + h * NT, a + h * (kHalfBytes >> 4) + kk * step, x + kk * 2, kDescHi, id_main, (kb > o.kb0 || kk > 0) ? 1u : 0u);
-            }
-          }
-          umma_commit(&bars->empty[s]);
+          for (int kk = 0; kk < 4 * C::kSub; ++kk)
+            if (kk < steps)
+              multiply_add<PAIR>(acc, a + (kk >> 2) * (C::kA >> 4) + (kk & 3) * step, x + (kk >> 2) * (C::kX >> 4) + (kk & 3) * 2, id_main, (kb > o.kb0 || kk > 0) ? 1u : 0u);
+          commit_to<PAIR>(&bars->empty[s]);
           at.next();
         }
+      } else {
+        at.skip((o.kb1 - o.kb0 + C::kSub - 1) / C::kSub);
       }
-      ok = __shfl_sync(0xffffffffu, good, 0) != 0;
-      at.s = __shfl_sync(0xffffffffu, at.s, 0);
-      at.round = __shfl_sync(0xffffffffu, at.round, 0);
       if (g.r > 0 && ok) {
         Pairs p(g, tab, o.n0, o.nt);
         const int blocks = low_blocks(g.r), half = blocks / 2;
-        const uint32_t id_low = idesc_of(BF16, round16(o.nt), !g.low_kmaj, false), step = g.low_kmaj ? 32 >> 4 : 2048 >> 4;
+        const uint32_t id_low = idesc_of<PAIR>(BF16, wide, !g.low_kmaj, false), step = g.low_kmaj ? 32 >> 4 : 2048 >> 4;
+        const int mine = PAIR ? wide / 2 : wide, n0 = o.n0 + rank * mine;
         while (ok && p.next(g, o.n0)) {
-          const int lo = p.lo - o.n0, hi = p.hi - o.n0, all = round16(o.nt);
+          const int lo = p.lo - n0, hi = p.hi - n0;
+          const bool side = p.lo > o.n0 || p.hi < o.n0 + wide;      // columns of other runs take no part
           for (int q = 0; q < blocks; ++q, at.next()) {
             const int s = at.s;
-            ok = mbar_wait_warp(&bars->full[s], (uint32_t)at.round & 1u, abort_flag);
+            uint8_t* tx = smem + s * C::kStage + C::kXOff;
+            if (!issues && !side) continue;
+            ok = issues ? warp_wait(&bars->full[s], (uint32_t)at.round & 1u, abort_flag) : warp_wait(&bars->side[s], (sides >> s) & 1u, abort_flag);
             if (!ok) break;
-            __syncwarp();
-            uint8_t* tx = smem + s * C::kStage + C::kA;
-            if (lo > 0 || hi < all) {                      // columns of other runs take no part
-              for (int i = lane; i < all * 8; i += 32)
+            if (side) {
+              for (int i = lane; i < mine * 8; i += 32)
                 if ((i >> 3) < lo || (i >> 3) >= hi) *reinterpret_cast<uint4*>(tx + i * 16) = make_uint4(0, 0, 0, 0);
               fence_proxy_async_smem();
               __syncwarp();
+              if (PAIR && !issues && lane == 0) arrive_first(&bars->side[s]);
+              if (PAIR && issues) ok = wait_of<PAIR>(&bars->side[s], (sides >> s) & 1u, abort_flag);
+              sides ^= 1u << s;
+              if (!ok) break;
             }
-            if (lane == 0) {
+            if (issues) {
               tc_fence_after();
-              const uint32_t a = desc_lo(smem_u32(smem + s * C::kStage)), x = desc_lo(smem_u32(tx));
+              const uint32_t a = base + s * (C::kStage >> 4), x = a + (C::kXOff >> 4);
               const int left = half ? g.r - (q % half) * kBK : g.r, steps = min(4, (left + 15) >> 4);
               for (int kk = 0; kk < steps; ++kk) {
-#pragma unroll
-                for (int h = 0; h < MH; ++h) {
-                  if (h > 0 && !upper) continue;
-                  umma_ss_lohi(acc + h * NT, a + h * (kHalfBytes >> 4) + kk * step, x + kk * 2, kDescHi, id_low, 1u);
-                  if (!half) umma_ss_lohi(acc + h * NT, a + h * (kHalfBytes >> 4) + kk * step, x + kk * 2 + 4, kDescHi, id_low, 1u);
-                }
+                multiply_add<PAIR>(acc, a + kk * step, x + kk * 2, id_low, 1u);
+                if (!half) multiply_add<PAIR>(acc, a + kk * step, x + kk * 2 + 4, id_low, 1u);
               }
-              umma_commit(&bars->empty[s]);
+              commit_to<PAIR>(&bars->empty[s]);
             }
-            __syncwarp();
           }
         }
       }
-      if (ok && lane == 0) umma_commit(&bars->acc_full[ab]);
+      if (ok && issues) commit_to<PAIR>(&bars->acc_full[ab]);
       ++ti;
     }
   } else if (start_ok && warp >= 2 && warp < 10) {
     // ----------------------------------------------------------------- epilogue
-    const int wq = warp & 3, part = (warp - 2) >> 2;       // TMEM lane quarter; MH = 2: half of the rows, 1: every other 32 columns
-    constexpr int kStep = MH == 2 ? 1 : 2;
+    const int wq = warp & 3, part = (warp - 2) >> 2;       // TMEM lane quarter; every other 32 columns
     bool ok = true;
     int ti = 0;
     uint8_t* box = smem + C::kOutOff + (warp - 2) * 2048;
-    for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const Tile o = tile_of<MH>(g, tab, t, nkb);
+    for (long long t = worker; t < tiles && ok; t += workers) {
+      const Tile o = tile_of<PAIR>(g, tab, t, nkb);
       if (o.nt <= 0) continue;
-      const int ab = ti % C::kAccBufs;
+      const int ab = ti & 1;
       uint32_t none[NT / 32];                              // columns whose column of X does not exist, a bit each
 #pragma unroll
       for (int c = 0; c < NT / 32; ++c) {
@@ -593,12 +776,12 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         if (g.columns && c * 32 < o.nt)
           none[c] = __ballot_sync(0xffffffffu, c * 32 + lane < o.nt && (unsigned)g.columns[o.n0 + min(c * 32 + lane, o.nt - 1)] >= (unsigned)g.N);
       }
-      ok = mbar_wait_warp(&bars->acc_full[ab], (uint32_t)(ti / C::kAccBufs) & 1u, abort_flag);
+      ok = mbar_wait_warp(&bars->acc_full[ab], (uint32_t)(ti >> 1) & 1u, abort_flag);
       if (!ok) break;
       tc_fence_after();
-      const int m = o.m0 + (MH == 2 ? part * 128 : 0) + wq * 32 + lane;
-      const uint32_t taddr = tmem + (static_cast<uint32_t>(wq * 32) << 16) + ab * C::kAccCols + (MH == 2 ? part * NT : 0);
-      const int chunks = MH == 2 && part * 128 >= g.M - o.m0 ? 0 : (o.nt + 31) / 32;
+      const int m = o.m0 + rank * 128 + wq * 32 + lane;
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(wq * 32) << 16) + ab * NT;
+      const int chunks = m - lane < g.M ? (o.nt + 31) / 32 : 0;
       float scale = 1.f;
       if (g.to != kToC) scale = g.scale ? g.scale[o.mat] : g.scale0;
       if (g.to == kToC) {
@@ -609,7 +792,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
             if (q == c) gone = none[q];
           put_fragments<BF16>(f, box, g.C, g.ldc, m - lane, o.n0 + c * 32, g.M, o.nt - c * 32, gone, g.vec != 0);
         };
-        drain_fragments<kStep>(taddr, MH == 2 ? 0 : part, chunks, &bars->acc_empty[ab], put);
+        drain_fragments<PAIR>(taddr, part, chunks, &bars->acc_empty[ab], put);
         ++ti;
         continue;
       }
@@ -636,7 +819,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
           }
         }
       };
-      drain_columns<kStep>(taddr, MH == 2 ? 0 : part, chunks, &bars->acc_empty[ab], put);
+      drain_columns<PAIR>(taddr, part, chunks, &bars->acc_empty[ab], put);
       ++ti;
     }
     if (g.zero_rest && ok) {
@@ -650,17 +833,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     }
   }
 
-  // ---------------------------------------------------------------- teardown
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem, C::kTmemCols);
-  }
-  if (threadIdx.x == 0 && *abort_flag) {
-    atomicExch(&g_grouped_abort, 1);
-    if (g.status) atomicExch(g.status, NNLIB_B200_TIMEOUT);
-  }
+  tear_down<NT, PAIR>(bars, tmem, g.status);
 }
 
 // ------------------------------------------------------------------------------------------------- gradient
@@ -679,10 +852,11 @@ struct GradArgs {
   int* status;
 };
 
-template <bool BF16, int MH, int NT>
+template <bool BF16, int NT, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_constant__ CUtensorMap tm_c, const __grid_constant__ GradArgs g) {
-  using C = Cfg<MH, NT>;
+  using C = Cfg<NT, PAIR>;
+  constexpr int kBlock = kBK * C::kSub;                    // columns of a stage
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -690,22 +864,8 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
   Table& tab = *reinterpret_cast<Table*>(smem + C::kTableOff);
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(&bars->full[s], 1);
-      mbar_init(&bars->empty[s], 1);
-    }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&bars->acc_full[s], 1);
-      mbar_init(&bars->acc_empty[s], 8);
-    }
-    bars->abort_flag = *reinterpret_cast<volatile int*>(&g_grouped_abort);
-    fence_mbar_init();
-  }
-  if (warp == 1) {
-    tmem_alloc(&bars->tmem_base, C::kTmemCols);
-    tmem_relinquish();
-  }
+  const int rank = PAIR ? cluster_rank() : 0, worker = PAIR ? blockIdx.x >> 1 : blockIdx.x, workers = PAIR ? gridDim.x >> 1 : gridDim.x;
+  set_up<NT, PAIR>(bars);
   const bool held = g.G <= kMaxRuns;
   if (held) {
     for (int i = threadIdx.x; i < g.G; i += kThreads) {
@@ -715,9 +875,9 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
     }
   }
   tc_fence_before();
-  __syncthreads();
+  sync_all<PAIR>();
   tc_fence_after();
-  const uint32_t tmem = bars->tmem_base;
+  const uint32_t tmem = __reduce_or_sync(0xffffffffu, bars->tmem_base);     // (in a uniform register)
   const bool start_ok = (*abort_flag == 0);
   const long long each = (long long)g.tiles_r * g.tiles_c, tiles = each * g.mats;
   // blocks of a tile, run by run: the runs of matrix a
@@ -735,13 +895,14 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
       bool ok = true;
       Ring<C::kStages> at;
       int turn = 0;
-      for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      for (long long t = worker; t < tiles && ok; t += workers) {
         const int a = (int)(t / each), q = (int)(t % each);
-        const int r0 = (q % g.tiles_r) * (MH * 128), c0 = (q / g.tiles_r) * NT;
+        const int r0 = (q % g.tiles_r) * (PAIR ? 256 : 128) + rank * 128, left = g.cols - (q / g.tiles_r) * NT;
+        const int c0 = (q / g.tiles_r) * NT + (PAIR ? rank * (product_columns<true>(min(NT, left)) / 2) : 0);
         for (int b = first_run(a); b < last_run(a) && ok; ++b) {
           if (!is_of(b, a)) continue;
           const int end = end_of(b);
-          for (int i0 = begin_of(b); i0 < end; i0 += kBK, at.next()) {
+          for (int i0 = begin_of(b); i0 < end; i0 += kBlock, at.next()) {
             const bool mine = turn == me;
             if (++turn == kProducers) turn = 0;
             if (!mine) continue;
@@ -749,11 +910,27 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
             if (at.round > 0) ok = mbar_wait(&bars->empty[s], (uint32_t)(at.round - 1) & 1u, abort_flag);
             if (!ok) break;
             uint8_t* d = smem + s * C::kStage;
-            mbar_arrive_expect_tx(&bars->full[s], C::kStage);
+            const bool side = ((end - i0) & 15) && end - i0 < kBlock;
+            const int subs = min(C::kSub, (end - i0 + kBK - 1) / kBK);
+            if (!PAIR || side) {
+              uint64_t* bar = PAIR && rank ? &bars->side[s] : &bars->full[s];
+              mbar_arrive_expect_tx(bar, subs * (C::kA + C::kX));
+              for (int u = 0; u < subs; ++u) {
 #pragma unroll
-            for (int x = 0; x < 2 * MH; ++x) tma_load_2d(d + x * (kHalfBytes / 2), &tm_r, &bars->full[s], r0 + x * 64, i0);
+                for (int x = 0; x < 2; ++x) tma_load_2d(d + u * C::kA + x * (kHalfBytes / 2), &tm_r, bar, r0 + x * 64, i0 + u * kBK);
 #pragma unroll
-            for (int x = 0; x < NT / 64; ++x) tma_load_2d(d + C::kA + x * (kHalfBytes / 2), &tm_c, &bars->full[s], c0 + x * 64, i0);
+                for (int x = 0; x < C::kX / (kHalfBytes / 2); ++x) tma_load_2d(d + C::kXOff + u * C::kX + x * (kHalfBytes / 2), &tm_c, bar, c0 + x * 64, i0 + u * kBK);
+              }
+            } else {
+              if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], 2 * subs * (C::kA + C::kX));
+              const uint32_t bar = first_barrier(&bars->full[s]);
+              for (int u = 0; u < subs; ++u) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) pair_load_2d(d + u * C::kA + x * (kHalfBytes / 2), &tm_r, bar, r0 + x * 64, i0 + u * kBK);
+#pragma unroll
+                for (int x = 0; x < C::kX / (kHalfBytes / 2); ++x) pair_load_2d(d + C::kXOff + u * C::kX + x * (kHalfBytes / 2), &tm_c, bar, c0 + x * 64, i0 + u * kBK);
+              }
+            }
           }
         }
       }
@@ -769,15 +946,15 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
     Ring<C::kStages> at;
     int ti = 0;
     const uint32_t base = desc_lo(smem_u32(smem));
-    for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++ti) {
+    const bool issues = !PAIR || rank == 0;
+    uint32_t sides = 0u;                                   // phases of the barriers `side`
+    for (long long t = worker; t < tiles && ok; t += workers, ++ti) {
       const int a = (int)(t / each), left = g.cols - (int)((t % each) / g.tiles_r) * NT;
-      const int ab = ti % C::kAccBufs;
-      const uint32_t acc = tmem + ab * C::kAccCols;
-      const uint32_t idesc = idesc_of(BF16, g.fold || left > NT ? NT : round16(left), true, true);
-      if (ti >= C::kAccBufs) {
-        ok = mbar_wait_warp(&bars->acc_empty[ab], (uint32_t)((ti / C::kAccBufs) + 1) & 1u, abort_flag);
-        if (!ok) break;
-      }
+      const int ab = ti & 1;
+      const uint32_t acc = tmem + ab * NT;
+      const uint32_t idesc = idesc_of<PAIR>(BF16, g.fold ? NT : product_columns<PAIR>(min(NT, left)), true, true);
+      if (ti >= 2 && issues) ok = wait_of<PAIR>(&bars->acc_empty[ab], (uint32_t)((ti >> 1) + 1) & 1u, abort_flag);
+      if (!ok) break;
       tc_fence_after();
       bool begun = false;
       for (int b = first_run(a); b < last_run(a) && ok; ++b) {
@@ -787,74 +964,74 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
         // a block of which the first `here` columns are the run's
         auto multiply = [&](int here) {
           tc_fence_after();
-          const uint32_t r = base + at.s * (C::kStage >> 4), c = r + (C::kA >> 4);
+          const uint32_t r = base + at.s * (C::kStage >> 4), c = r + (C::kXOff >> 4);
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            if (kk * 16 < here) {
-#pragma unroll
-              for (int h = 0; h < MH; ++h)
-                umma_ss_lohi(acc + h * NT, r + h * (kHalfBytes >> 4) + kk * (2048 >> 4), c + kk * (2048 >> 4), kDescHi, idesc, (begun || kk > 0) ? 1u : 0u);
-            }
-          }
-          umma_commit(&bars->empty[at.s]);
+          for (int kk = 0; kk < 4 * C::kSub; ++kk)
+            if (kk * 16 < here)
+              multiply_add<PAIR>(acc, r + (kk >> 2) * (C::kA >> 4) + (kk & 3) * (2048 >> 4), c + (kk >> 2) * (C::kX >> 4) + (kk & 3) * (2048 >> 4), idesc, (begun || kk > 0) ? 1u : 0u);
+          commit_to<PAIR>(&bars->empty[at.s]);
           begun = true;
         };
-        // whole blocks are one lane's, a last one is the warp's
-        const int whole = (end - begin) / kBK, rest = (end - begin) % kBK;
-        int good = 1;
-        if (lane == 0) {
-          for (int i = 0; i < whole; ++i, at.next()) {
-            if (!mbar_wait(&bars->full[at.s], (uint32_t)at.round & 1u, abort_flag)) { good = 0; break; }
-            multiply(kBK);
+        const int whole = (end - begin) / kBlock, rest = (end - begin) % kBlock;
+        if (issues) {
+          for (int i = 0; i < whole && ok; ++i) {
+            ok = warp_wait(&bars->full[at.s], (uint32_t)at.round & 1u, abort_flag);
+            if (!ok) break;
+            multiply(kBlock);
+            at.next();
           }
+        } else {
+          at.skip(whole);
         }
-        ok = __shfl_sync(0xffffffffu, good, 0) != 0;
-        at.s = __shfl_sync(0xffffffffu, at.s, 0);
-        at.round = __shfl_sync(0xffffffffu, at.round, 0);
-        if (ok && rest) {
-          ok = mbar_wait_warp(&bars->full[at.s], (uint32_t)at.round & 1u, abort_flag);
+        const bool side = rest & 15;                       // behind the run's end: another run's columns, or nobody's
+        if (ok && rest && (issues || side)) {
+          ok = issues ? warp_wait(&bars->full[at.s], (uint32_t)at.round & 1u, abort_flag) : warp_wait(&bars->side[at.s], (sides >> at.s) & 1u, abort_flag);
           if (!ok) break;
-          if (rest & 15) {                                 // another run's columns, or nobody's
-            __syncwarp();
-            for (int i = rest * 8 + lane; i < round16(rest) * 8; i += 32) {
+          if (side) {
+            const int u = rest / kBK, in = rest % kBK;     // (a part of 16: in one block)
+            for (int i = in * 8 + lane; i < round16(in) * 8; i += 32) {
 #pragma unroll
-              for (int x = 0; x < C::kStage / (kHalfBytes / 2); ++x)
-                *reinterpret_cast<uint4*>(smem + at.s * C::kStage + x * (kHalfBytes / 2) + i * 16) = make_uint4(0, 0, 0, 0);
+              for (int x = 0; x < 2; ++x) *reinterpret_cast<uint4*>(smem + at.s * C::kStage + u * C::kA + x * (kHalfBytes / 2) + i * 16) = make_uint4(0, 0, 0, 0);
+#pragma unroll
+              for (int x = 0; x < C::kX / (kHalfBytes / 2); ++x)
+                *reinterpret_cast<uint4*>(smem + at.s * C::kStage + C::kXOff + u * C::kX + x * (kHalfBytes / 2) + i * 16) = make_uint4(0, 0, 0, 0);
             }
             fence_proxy_async_smem();
             __syncwarp();
+            if (PAIR && !issues && lane == 0) arrive_first(&bars->side[at.s]);
+            if (PAIR && issues) ok = wait_of<PAIR>(&bars->side[at.s], (sides >> at.s) & 1u, abort_flag);
+            sides ^= 1u << at.s;
+            if (!ok) break;
           }
-          if (lane == 0) multiply(rest);
-          at.next();
-          __syncwarp();
+          if (issues) multiply(rest);
         }
+        if (rest) at.next();
       }
-      if (ok && lane == 0) umma_commit(&bars->acc_full[ab]);
+      if (ok && issues) commit_to<PAIR>(&bars->acc_full[ab]);
     }
   } else if (start_ok && warp >= 2 && warp < 10) {
     const int wq = warp & 3, part = (warp - 2) >> 2;
-    constexpr int kStep = MH == 2 ? 1 : 2;
     bool ok = true;
     int ti = 0;
     uint8_t* box = smem + C::kOutOff + (warp - 2) * 2048;
-    for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++ti) {
+    for (long long t = worker; t < tiles && ok; t += workers, ++ti) {
       const int a = (int)(t / each), q = (int)(t % each);
-      const int r0 = (q % g.tiles_r) * (MH * 128), c0 = (q / g.tiles_r) * NT;
-      const int ab = ti % C::kAccBufs;
+      const int r0 = (q % g.tiles_r) * (PAIR ? 256 : 128) + rank * 128, c0 = (q / g.tiles_r) * NT;
+      const int ab = ti & 1;
       bool some = false;                                   // a matrix that no column met is zeros
       for (int b = first_run(a); b < last_run(a) && !some; ++b) some = is_of(b, a) && end_of(b) > begin_of(b);
-      ok = mbar_wait_warp(&bars->acc_full[ab], (uint32_t)(ti / C::kAccBufs) & 1u, abort_flag);
+      ok = mbar_wait_warp(&bars->acc_full[ab], (uint32_t)(ti >> 1) & 1u, abort_flag);
       if (!ok) break;
       tc_fence_after();
-      const int m = r0 + (MH == 2 ? part * 128 : 0) + wq * 32 + lane;
-      const uint32_t taddr = tmem + (static_cast<uint32_t>(wq * 32) << 16) + ab * C::kAccCols + (MH == 2 ? part * NT : 0);
+      const int m = r0 + wq * 32 + lane;
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(wq * 32) << 16) + ab * NT;
       T* base = reinterpret_cast<T*>(g.A) + (long long)a * g.stride;
-      const int width = g.fold ? g.fold_step : min(NT, g.cols - c0), chunks = MH == 2 && part * 128 >= g.rows - r0 ? 0 : (width + 31) / 32;
+      const int width = g.fold ? g.fold_step : min(NT, g.cols - c0), chunks = m - lane < g.rows ? (width + 31) / 32 : 0;
       if (!g.fold) {
         auto put = [&](uint32_t (&f)[2][16], int c) {
           put_fragments<BF16>(f, box, base, g.ld, m - lane, c0 + c * 32, g.rows, g.cols - c0 - c * 32, some ? 0u : 0xffffffffu, g.vec != 0);
         };
-        drain_fragments<kStep>(taddr, MH == 2 ? 0 : part, chunks, &bars->acc_empty[ab], put);
+        drain_fragments<PAIR>(taddr, part, chunks, &bars->acc_empty[ab], put);
         continue;
       }
       for (int c = part; c < chunks; c += 2) {
@@ -879,16 +1056,7 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
       if (lane == 0) mbar_arrive(&bars->acc_empty[ab]);
     }
   }
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem, C::kTmemCols);
-  }
-  if (threadIdx.x == 0 && *abort_flag) {
-    atomicExch(&g_grouped_abort, 1);
-    if (g.status) atomicExch(g.status, NNLIB_B200_TIMEOUT);
-  }
+  tear_down<NT, PAIR>(bars, tmem, g.status);
 }
 
 // ------------------------------------------------------------------------------------------------- copies, host
@@ -1100,60 +1268,66 @@ struct Maps {
   CUtensorMap a, x, b, t;
 };
 
-template <bool BF16, int MH, int NT>
-cudaError_t launch_fwd(const Maps& m, FwdArgs g, long long most, cudaStream_t st) {
-  using C = Cfg<MH, NT>;
-  auto kern = grouped_umma_kernel<BF16, MH, NT>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+template <bool PAIR, typename K, typename... Args>
+cudaError_t launch(K kern, long long workers, int smem, cudaStream_t st, const Args&... args) {
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  g.tiles_m = (g.M + MH * 128 - 1) / (MH * 128);
-  const long long grid = std::max<long long>(1, std::min<long long>(most * g.tiles_m * g.splits, sm_count()));
-  kern<<<(unsigned)grid, kThreads, C::kSmem, st>>>(m.a, m.x, m.b, m.t, g);
+  const long long most = sm_count() / (PAIR ? 2 : 1);
+  const unsigned grid = (unsigned)std::max<long long>(1, std::min(workers, most)) * (PAIR ? 2 : 1);
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3(grid);
+  c.blockDim = dim3(kThreads);
+  c.dynamicSmemBytes = smem;
+  c.stream = st;
+  cudaLaunchAttribute a[1];
+  a[0].id = cudaLaunchAttributeClusterDimension;
+  a[0].val.clusterDim.x = 2;
+  a[0].val.clusterDim.y = a[0].val.clusterDim.z = 1;
+  c.attrs = a;
+  c.numAttrs = PAIR ? 1 : 0;
+  e = cudaLaunchKernelEx(&c, kern, args...);
   count_launch();
-  return cudaGetLastError();
+  return e == cudaSuccess ? cudaGetLastError() : e;
 }
-template <bool BF16, int MH, int NT>
+template <bool BF16, int NT, bool PAIR>
+cudaError_t launch_fwd(const Maps& m, FwdArgs g, long long most, cudaStream_t st) {
+  g.tiles_m = (g.M + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128);
+  return launch<PAIR>(grouped_umma_kernel<BF16, NT, PAIR>, most * g.tiles_m * g.splits, Cfg<NT, PAIR>::kSmem, st, m.a, m.x, m.b, m.t, g);
+}
+template <bool BF16, int NT, bool PAIR>
 cudaError_t launch_bwd(const CUtensorMap& r, const CUtensorMap& c, GradArgs g, cudaStream_t st) {
-  using C = Cfg<MH, NT>;
-  auto kern = grouped_grad_umma_kernel<BF16, MH, NT>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
-  if (e != cudaSuccess) return e;
-  g.tiles_r = (g.rows + MH * 128 - 1) / (MH * 128);
+  g.tiles_r = (g.rows + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128);
   g.tiles_c = g.fold ? 1 : (g.cols + NT - 1) / NT;
-  const long long grid = std::min<long long>((long long)g.tiles_r * g.tiles_c * g.mats, sm_count());
-  kern<<<(unsigned)grid, kThreads, C::kSmem, st>>>(r, c, g);
-  count_launch();
-  return cudaGetLastError();
+  return launch<PAIR>(grouped_grad_umma_kernel<BF16, NT, PAIR>, (long long)g.tiles_r * g.tiles_c * g.mats, Cfg<NT, PAIR>::kSmem, st, r, c, g);
 }
 
 // Rows and columns of a tile.
 struct Shape {
-  int mh, cap, splits;
+  bool pair;
+  int cap, splits;
   long long most;                        // column tiles that there can be
   int nt() const { return cap > 128 ? 256 : cap > 64 ? 128 : cap > 32 ? 64 : 32; }
 };
 // The tile, and the cut of K into parts, of the fewest cycles, runs taken as equally long.  A K block costs its products (half a cycle
-// for each column, 90 at least to issue one, 128 rows each) or its copies (64 bytes a cycle), a tile of 256 x 256 the end that nothing overlaps with,
-// and K is cut (the parts are added up by another launch, 6000 cycles) only where tiles are fewer than SMs.  Measured against
-// the others at 2048 x 2048 x 8192: 256 x 224 tiles 59.5 us, 256 x 256 67.7, 128 x 256 70; 64 x 4096 by 6656 columns in 7 runs: 128 columns 31 us, 32 56.
+// for each column, 90 at least to issue one, 128 rows) or its copies (64 bytes a cycle and SM, which is where a pair of CTAs, each with half of
+// the columns, gains); K is cut (the parts are added up by another launch, 6000 cycles) only where tiles are fewer than SMs.
 Shape shape_of(int M, int K, int R, int runs, bool may_split) {
   const int sms = 148, each = std::max(1, (R + runs - 1) / std::max(1, runs)), nkb = (K + kBK - 1) / kBK;
-  Shape best{1, 32, 1, 0};
+  Shape best{false, 32, 1, 0};
   double least = 1e300;
-  for (int mh = 1; mh <= 2; ++mh) {
-    if (mh == 2 && M <= 128) break;
-    for (int cap = mh == 2 ? 144 : 16; cap <= 256; cap += 16) {
+  for (int pair = 0; pair <= 1; ++pair) {
+    if (pair && M <= 128) break;
+    for (int cap = pair ? 144 : 16; cap <= 256; cap += 16) {
       const int w = tile_width(each, cap);
       if (w != cap) continue;                          // the same tiles as a smaller cap's
-      const double tiles = (double)tile_count(each, cap) * std::min(runs, R) * ((M + 128 * mh - 1) / (128 * mh)) / sms;
-      const double block = std::max(4.0 * mh * std::max(90, w / 2) + 100, (16384.0 * mh + 128.0 * w) / 64);
-      const double end = 3000 + (mh == 2 ? 8000.0 * w / 256 : 0);
-      for (int splits = 1; splits == 1 || (may_split && splits <= 8 && tiles * splits < 1.01 && nkb / splits >= 4); ++splits) {
+      const double tiles = (double)tile_count(each, cap) * std::min(runs, R) * ((M + 127 + 128 * pair) / (128 + 128 * pair)) / (pair ? sms / 2 : sms);
+      const double block = std::max(4.0 * std::max(90, w / 2) + 60, (16384 + (pair ? 64.0 : 128.0) * w) / 64);
+      for (int splits = 1; splits == 1 || (may_split && !pair && splits <= 8 && tiles * splits < 1.01 && nkb / splits >= 4); ++splits) {
         const double all = tiles * splits, waves = runs == 1 ? std::ceil(all) : std::max(1.0, all + (all > 1 ? 0.5 : 0.0));
-        const double cost = waves * ((nkb + splits - 1) / splits * block + end) + (splits > 1 ? 6000 : 0);
+        const double cost = waves * (std::max((nkb + splits - 1) / splits * block, 3500.0 * w / 256) + 500) + (splits > 1 ? 6000 : 0);
         if (cost < least) {
           least = cost;
-          best.mh = mh;
+          best.pair = pair;
           best.cap = cap;
           best.splits = splits;
         }
@@ -1167,11 +1341,11 @@ Shape shape_of(int M, int K, int R, int runs, bool may_split) {
 
 template <bool BF16>
 cudaError_t fwd(const Shape& s, const Maps& m, const FwdArgs& g, cudaStream_t st) {
-  if (s.mh == 2) return launch_fwd<BF16, 2, 256>(m, g, s.most, st);
-  if (s.nt() == 256) return launch_fwd<BF16, 1, 256>(m, g, s.most, st);
-  if (s.nt() == 128) return launch_fwd<BF16, 1, 128>(m, g, s.most, st);
-  if (s.nt() == 64) return launch_fwd<BF16, 1, 64>(m, g, s.most, st);
-  return launch_fwd<BF16, 1, 32>(m, g, s.most, st);
+  if (s.pair) return launch_fwd<BF16, 256, true>(m, g, s.most, st);
+  if (s.nt() == 256) return launch_fwd<BF16, 256, false>(m, g, s.most, st);
+  if (s.nt() == 128) return launch_fwd<BF16, 128, false>(m, g, s.most, st);
+  if (s.nt() == 64) return launch_fwd<BF16, 64, false>(m, g, s.most, st);
+  return launch_fwd<BF16, 32, false>(m, g, s.most, st);
 }
 int box_of(const Shape& s) { return s.nt() >= 128 ? 64 : 16; }
 
@@ -1375,18 +1549,17 @@ cudaError_t grouped_umma_grad(const GroupedGradArgs& g, int dtype, int fold, voi
   a.fold_step = fold ? low_width(a.cols) / 2 : 0;
   a.along = fold && (fold == 1) == (g.transA == 0);
   const int nt = fold ? low_width(a.cols) : 256;
-  // 256 rows where the runs are long enough to hide an epilogue that nothing overlaps with
-  const int mh = !fold && a.rows > 128 && g.R / std::max(1, g.mats) > 1024 ? 2 : 1;
+  const bool pair = !fold && a.rows > 128 && a.cols > 128;
   CUtensorMap mc, mx;
   if (!encode_columns(&mc, dtype, c, 64) || !encode_columns(&mx, dtype, x, 64)) return cudaErrorInvalidValue;
   a.vec = aligned16(g.A) && g.lda % 8 == 0 && g.strideA % 8 == 0;
   const CUtensorMap& r = x_rows ? mx : mc;
   const CUtensorMap& q = x_rows ? mc : mx;
   const bool bf16 = dtype == NNLIB_B200_BF16;
-  if (mh == 2) return bf16 ? launch_bwd<true, 2, 256>(r, q, a, st) : launch_bwd<false, 2, 256>(r, q, a, st);
-  if (nt == 256) return bf16 ? launch_bwd<true, 1, 256>(r, q, a, st) : launch_bwd<false, 1, 256>(r, q, a, st);
-  if (nt == 128) return bf16 ? launch_bwd<true, 1, 128>(r, q, a, st) : launch_bwd<false, 1, 128>(r, q, a, st);
-  return bf16 ? launch_bwd<true, 1, 64>(r, q, a, st) : launch_bwd<false, 1, 64>(r, q, a, st);
+  if (pair) return bf16 ? launch_bwd<true, 256, true>(r, q, a, st) : launch_bwd<false, 256, true>(r, q, a, st);
+  if (nt == 256) return bf16 ? launch_bwd<true, 256, false>(r, q, a, st) : launch_bwd<false, 256, false>(r, q, a, st);
+  if (nt == 128) return bf16 ? launch_bwd<true, 128, false>(r, q, a, st) : launch_bwd<false, 128, false>(r, q, a, st);
+  return bf16 ? launch_bwd<true, 64, false>(r, q, a, st) : launch_bwd<false, 64, false>(r, q, a, st);
 }
 
 // Reads and clears the sticky "a bounded wait ran out" flag of these kernels on the current device.
