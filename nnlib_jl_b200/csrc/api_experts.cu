@@ -337,7 +337,7 @@ int nnlib_b200_grouped_gemm_grad(const nnlib_b200_grouped_params* p, void* works
   const bool umma = on_umma(g, p->dtype);
   if (umma && (rc = workspace_ok(workspace, workspace_bytes, grouped_umma_grad_workspace_bytes(g, 0)))) return rc;
   if ((rc = check_grouped_arrays(a))) return rc;
-  return finish(umma ? grouped_umma_grad(g, p->dtype, 0, workspace, (cudaStream_t)stream)
+  return finish(umma ? grouped_umma_grad(g, p->dtype, 0, workspace, false, (cudaStream_t)stream)
                      : grouped_fma_grad(g, p->dtype, false, false, (cudaStream_t)stream));
 }
 
@@ -413,9 +413,9 @@ int nnlib_b200_adapter_bwd(const nnlib_b200_adapter_params* p, void* workspace, 
     if ((rc = finish(grouped_fma_grad(g.a, p->dtype, true, false, st)))) return rc;
     return finish(grouped_fma_grad(g.b, p->dtype, false, true, st));
   }
-  if (has_pairs(a) && (rc = finish(low_umma(g.first, p->dtype, of_X, ws, st)))) return rc;
-  if ((rc = finish(grouped_umma_grad(g.a, p->dtype, 1, ws, st)))) return rc;
-  return finish(grouped_umma_grad(g.b, p->dtype, 2, ws, st));
+  if (has_pairs(a) && (rc = finish(low_umma(g.first, p->dtype, of_X, ws, true, st)))) return rc;
+  if ((rc = finish(grouped_umma_grad(g.a, p->dtype, 1, ws, true, st)))) return rc;
+  return finish(grouped_umma_grad(g.b, p->dtype, 2, ws, true, st));
 }
 
 }  // extern "C"

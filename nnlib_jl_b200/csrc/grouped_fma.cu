@@ -15,12 +15,11 @@
 namespace nb200 {
 namespace {
 
-constexpr int kGK = 16;
-
 // acc[i][j] += Q[k][i] * P[k][j] for a stage of BT + 4 wide rows
 template <int BT>
 struct Tile {
-  static constexpr int R = BT / 16, G = R < 4 ? R : 4, LD = BT + 4, NL = BT * kGK / 256;
+  static constexpr int KG = 16;
+  static constexpr int R = BT / 16, G = R < 4 ? R : 4, LD = BT + 4, NL = BT * KG / 256;
   float acc[R][R];                           // [column side][row side]
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -54,19 +53,19 @@ struct Tile {
 
 template <int BT>
 struct Stages {
-  float p[2][kGK][Tile<BT>::LD], q[2][kGK][Tile<BT>::LD];
+  float p[2][Tile<BT>::KG][Tile<BT>::LD], q[2][Tile<BT>::KG][Tile<BT>::LD];
 };
 
 // One contraction of K terms: P(k, row) and Q(k, column) give the elements (0 where there is none); `pk`: P's neighbours in
 // memory are along k
 template <int BT, typename FP, typename FQ>
 __device__ __forceinline__ void contract(Tile<BT>& t, Stages<BT>& s, int K, bool pk, bool qk, FP P, FQ Q) {
-  constexpr int NL = Tile<BT>::NL;
+  constexpr int NL = Tile<BT>::NL, KG = Tile<BT>::KG;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   float rp[NL], rq[NL];
   auto at = [&](int e, bool along, int& k, int& r) {
     const int c = e * 256 + threadIdx.x;
-    if (along) { k = c % kGK; r = c / kGK; } else { r = c % BT; k = c / BT; }
+    if (along) { k = c % KG; r = c / KG; } else { r = c % BT; k = c / BT; }
   };
   auto fetch = [&](int k0) {
 #pragma unroll
@@ -93,13 +92,13 @@ __device__ __forceinline__ void contract(Tile<BT>& t, Stages<BT>& s, int K, bool
   __syncthreads();                           // (an earlier contraction's last stage has been read)
   stage(0);
   __syncthreads();
-  for (int k0 = 0, b = 0; k0 < K; k0 += kGK, b ^= 1) {
-    const bool more = k0 + kGK < K;
-    if (more) fetch(k0 + kGK);
-    const int kn = min(kGK, K - k0);         // the padding is not multiplied: 0 * Inf would be a NaN
-    if (kn == kGK) {
+  for (int k0 = 0, b = 0; k0 < K; k0 += KG, b ^= 1) {
+    const bool more = k0 + KG < K;
+    if (more) fetch(k0 + KG);
+    const int kn = min(KG, K - k0);         // the padding is not multiplied: 0 * Inf would be a NaN
+    if (kn == KG) {
 #pragma unroll
-      for (int k = 0; k < kGK; ++k) t.step(s.p[b][k], s.q[b][k], tx, ty);
+      for (int k = 0; k < KG; ++k) t.step(s.p[b][k], s.q[b][k], tx, ty);
     } else {
       for (int k = 0; k < kn; ++k) t.step(s.p[b][k], s.q[b][k], tx, ty);
     }
@@ -227,14 +226,15 @@ cudaError_t launch(const GroupedArgs& g, cudaStream_t st) {
   count_launch();
   return cudaGetLastError();
 }
-// The largest tile that is not mostly padding for runs of the average length and still gives every SM a block.
+// The largest tile that is not mostly padding for runs of the average length and still gives most SMs a block: a tile of 32 reads twice as
+// much shared memory for its products as one of 64 (333 x 200 by 1200 columns in 5 runs: 20 us in tiles of 32, 17 in tiles of 64).
 template <typename T, typename TC>
 cudaError_t launch_of(const GroupedArgs& g, cudaStream_t st) {
   if (g.M < 1 || g.R < 1) return cudaSuccess;
   const long long each = g.R / std::max(1, g.G);
   auto blocks = [&](long long bt) { return (g.R / bt + 1) * ((g.M + bt - 1) / bt); };
   if (each > 64 && g.M > 64 && blocks(128) >= 148) return launch<T, TC, 128>(g, st);
-  if (each > 32 && g.M > 32 && blocks(64) >= 148) return launch<T, TC, 64>(g, st);
+  if (each > 32 && g.M > 32 && blocks(64) >= 100) return launch<T, TC, 64>(g, st);
   return launch<T, TC, 32>(g, st);
 }
 
@@ -246,6 +246,7 @@ cudaError_t launch_grad(const GroupedGradArgs& g, cudaStream_t st) {
   count_launch();
   return cudaGetLastError();
 }
+// (there the sums are the runs', which a tile of 64 walks as long as one of 32: 25 us and 40)
 template <typename TC, typename TX, typename TA>
 cudaError_t launch_grad_of(const GroupedGradArgs& g, cudaStream_t st) {
   if (g.M < 1 || g.K < 1 || g.mats < 1) return cudaSuccess;

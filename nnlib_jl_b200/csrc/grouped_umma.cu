@@ -24,6 +24,7 @@
 #include <cstring>
 
 #include "common.cuh"
+#include "early.cuh"
 #include "grouped_runs.cuh"
 #include "launchers.h"
 #include "umma.cuh"
@@ -79,6 +80,7 @@ struct Bars {
 static_assert(sizeof(Bars) <= 512, "barrier block");
 
 enum { kToC, kToParts, kToLow };         // what the epilogue writes
+enum { kWaitNone, kWaitData, kWaitEnd }; // launched early: what the kernel before writes is read from the start, or not at all
 
 struct FwdArgs {
   Runs runs;
@@ -95,6 +97,7 @@ struct FwdArgs {
   Runs low_runs;                         // kToC: low-rank pairs, r = 0: none
   const int* low_ids;
   int r, n, low_kmaj;
+  int wait;
   int* status;
 };
 
@@ -580,8 +583,10 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
   const int nkb = (g.K + kBK - 1) / kBK;
 
   const int rank = PAIR ? cluster_rank() : 0, worker = PAIR ? blockIdx.x >> 1 : blockIdx.x, workers = PAIR ? gridDim.x >> 1 : gridDim.x;
+  let_next();
   set_up<NT, PAIR>(bars);
   count_tiles(g, tab, bars->search);
+  if (g.wait == kWaitData) wait_before();
   tc_fence_before();
   sync_all<PAIR>();
   tc_fence_after();
@@ -833,6 +838,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     }
   }
 
+  if (g.wait == kWaitEnd) wait_before();
   tear_down<NT, PAIR>(bars, tmem, g.status);
 }
 
@@ -848,6 +854,7 @@ struct GradArgs {
   long long ld, stride;                  // between columns and matrices of the result
   int rows, cols, G, mats;
   int tiles_r, tiles_c, vec;
+  int wait;                              // launched early
   int fold, fold_step, along;            // fold: columns fold_step apart are the two terms of one; along: a row's columns are contiguous
   int* status;
 };
@@ -865,7 +872,9 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = PAIR ? cluster_rank() : 0, worker = PAIR ? blockIdx.x >> 1 : blockIdx.x, workers = PAIR ? gridDim.x >> 1 : gridDim.x;
+  let_next();
   set_up<NT, PAIR>(bars);
+  if (g.wait) wait_before();
   const bool held = g.G <= kMaxRuns;
   if (held) {
     for (int i = threadIdx.x; i < g.G; i += kThreads) {
@@ -1072,6 +1081,8 @@ struct CopyArgs {
 };
 __global__ void __launch_bounds__(256) copy_rows_kernel(const __grid_constant__ CopyArgs g) {
   const int mat = blockIdx.z;
+  let_next();
+  wait_before();
   if (g.of.offsets && g.of.end(mat) <= g.of.begin(mat)) return;
   const unsigned short* s = g.src + (long long)mat * g.stride;
   uint4* d = g.dst + (long long)mat * g.deep * g.ld8;
@@ -1126,6 +1137,8 @@ template <typename T>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ JoinArgs g) {
   __shared__ float t[128];
   __shared__ int pair;
+  let_next();
+  wait_before();
   const int n = blockIdx.x, m = (blockIdx.y * 128 + threadIdx.x) * 2;
   T* out = reinterpret_cast<T*>(g.C) + (long long)n * g.ldc + m;
   int in = 1;
@@ -1187,10 +1200,109 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ JoinA
   if (m < g.M) out[0] = Elem<T>::from_f(sum[0]);
   if (m + 1 < g.M) out[1] = Elem<T>::from_f(sum[1]);
 }
+// scale * A X of columns that hardly share a pair, in parts as the products leave them: a block takes a column and kLowK of K.  What bounds it is
+// reading A, so it needs no tensor cores (64 requests of one column, rank 16, K = 4096: 20 us as a product, 8.6 so).
+constexpr int kLowK = 1024;
+struct LowFewArgs {
+  const void* A;
+  const void* X;
+  float* parts;                          // (r, R, splits)
+  long long lda, strideA, ldx;
+  const float* scale;
+  float scale0;
+  Runs runs;
+  const int* ids;
+  int transA, r, K, R, mats, vec;        // vec: 16-byte packets of A along what is contiguous
+};
+template <typename T>
+__global__ void __launch_bounds__(256) low_few_kernel(const __grid_constant__ LowFewArgs g) {
+  __shared__ float x[kLowK];
+  __shared__ float part[256 * 8], sums[256];
+  __shared__ int pair;
+  let_next();
+  const int n = blockIdx.x, k0 = blockIdx.y * kLowK, nk = min(kLowK, g.K - k0), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    pair = -1;
+    if (!g.runs.offsets) {
+      const long long i = g.runs.len > 0 ? n / g.runs.len : g.runs.runs;
+      if (i < g.runs.runs) pair = g.ids[i];
+    }
+  }
+  __syncthreads();
+  if (g.runs.offsets) {
+    for (int i = threadIdx.x; i < g.runs.runs; i += 256)
+      if (g.runs.begin(i) <= n && n < g.runs.end(i)) pair = g.ids[i];
+  }
+  const T* X = reinterpret_cast<const T*>(g.X) + (long long)n * g.ldx + k0;
+  for (int k = threadIdx.x; k < nk; k += 256) x[k] = Elem<T>::to_f(X[k]);
+  __syncthreads();
+  const int id = pair;
+  if (id < 0 || id >= g.mats) return;
+  const float scale = g.scale ? g.scale[id] : g.scale0;
+  const T* A = reinterpret_cast<const T*>(g.A) + (long long)id * g.strideA;
+  float* out = g.parts + ((long long)blockIdx.y * g.R + n) * g.r;
+  if (g.transA) {                        // K contiguous: a warp a row
+    for (int i = warp; i < g.r; i += 8) {
+      const T* a = A + (long long)i * g.lda + k0;
+      float sum = 0.f;
+      if (g.vec) {
+#pragma unroll 4
+        for (int k = lane * 8; k < nk; k += 256) {
+          const uint4 v = *reinterpret_cast<const uint4*>(a + k);
+          const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) sum = fmaf(Elem<T>::to_f(e[u]), x[k + u], sum);
+        }
+      } else {
+#pragma unroll 4
+        for (int k = lane; k < nk; k += 32) sum = fmaf(Elem<T>::to_f(a[k]), x[k], sum);
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) out[i] = scale * sum;
+    }
+    return;
+  }
+  // the rank contiguous: eight (or one) of it to a thread, every L-th of K
+  const int each = g.vec ? 8 : 1, groups = g.r / each, L = 256 / groups, group = threadIdx.x % groups, kl = threadIdx.x / groups;
+  float acc[8] = {};
+  if (kl < L) {
+    const T* a = A + (long long)k0 * g.lda + group * each;
+    if (g.vec) {
+#pragma unroll 8
+      for (int k = kl; k < nk; k += L) {
+        const uint4 v = *reinterpret_cast<const uint4*>(a + (long long)k * g.lda);
+        const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) acc[u] = fmaf(Elem<T>::to_f(e[u]), x[k], acc[u]);
+      }
+    } else {
+#pragma unroll 8
+      for (int k = kl; k < nk; k += L) acc[0] = fmaf(Elem<T>::to_f(a[(long long)k * g.lda]), x[k], acc[0]);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 8; ++u) part[u * 256 + threadIdx.x] = acc[u];
+  __syncthreads();
+  // element i of the rank is component i % each of threads i / each + groups * (0 .. L - 1): cut into P, then P into one
+  const int P = 256 / g.r, i = threadIdx.x % g.r, p = threadIdx.x / g.r;
+  float sum = 0.f;
+  if (p < P)
+    for (int q = p; q < L; q += P) sum += part[(i % each) * 256 + i / each + groups * q];
+  sums[threadIdx.x] = sum;
+  __syncthreads();
+  if (threadIdx.x < g.r) {
+    sum = 0.f;
+    for (int q = 0; q < P; ++q) sum += sums[q * g.r + threadIdx.x];
+    out[threadIdx.x] = scale * sum;
+  }
+}
 // T from the parts of scale * A X: two 16-bit terms, zeros behind the rank
 template <typename T>
 __global__ void __launch_bounds__(256) join_low_kernel(const float* parts, int splits, int r, int R, T* out, int width) {
   const int step = width / 2;
+  let_next();
+  wait_before();
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
   const int n = (int)(i / step), c = (int)(i % step);
   if (n >= R) return;
@@ -1213,7 +1325,7 @@ struct Operand {
   bool fits() const { return aligned16(p) && stride_ok(ld) && (count <= 1 || stride == 0 || stride_ok(stride)); }
   size_t copy_bytes() const { return (fits() && !columns) || wide == 0 || deep == 0 || count == 0 ? 0 : (size_t)((wide + 7) / 8 * 16) * deep * count; }
 };
-cudaError_t align_operand(Operand& o, char*& ws, const Runs* of, cudaStream_t st) {
+cudaError_t align_operand(Operand& o, char*& ws, const Runs* of, bool& behind, cudaStream_t st) {
   const size_t bytes = o.copy_bytes();
   if (!bytes) return cudaSuccess;
   CopyArgs c;
@@ -1227,8 +1339,16 @@ cudaError_t align_operand(Operand& o, char*& ws, const Runs* of, cudaStream_t st
   c.columns = o.columns;
   c.of = of ? *of : Runs{nullptr, 0, 0, 0};
   const long long blocks = std::min<long long>((o.deep + 7) / 8, 1 << 20);
-  copy_rows_kernel<<<dim3((unsigned)blocks, 1, (unsigned)o.count), 256, 0, st>>>(c);
+  // (behind: a kernel of this call is before it in the stream)
+  const dim3 grid((unsigned)blocks, 1, (unsigned)o.count);
+  if (behind) {
+    const cudaError_t e = launch_early(copy_rows_kernel, grid, dim3(256), 0, st, c);
+    if (e != cudaSuccess) return e;
+  } else {
+    copy_rows_kernel<<<grid, 256, 0, st>>>(c);
+  }
   count_launch();
+  behind = true;
   o.p = ws;
   o.ld = (long long)c.ld8 * 8;
   o.stride = o.ld * o.deep;
@@ -1269,7 +1389,7 @@ struct Maps {
 };
 
 template <bool PAIR, typename K, typename... Args>
-cudaError_t launch(K kern, long long workers, int smem, cudaStream_t st, const Args&... args) {
+cudaError_t launch(K kern, long long workers, int smem, bool early, cudaStream_t st, const Args&... args) {
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   const long long most = sm_count() / (PAIR ? 2 : 1);
@@ -1279,12 +1399,19 @@ cudaError_t launch(K kern, long long workers, int smem, cudaStream_t st, const A
   c.blockDim = dim3(kThreads);
   c.dynamicSmemBytes = smem;
   c.stream = st;
-  cudaLaunchAttribute a[1];
-  a[0].id = cudaLaunchAttributeClusterDimension;
-  a[0].val.clusterDim.x = 2;
-  a[0].val.clusterDim.y = a[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute a[2];
   c.attrs = a;
-  c.numAttrs = PAIR ? 1 : 0;
+  if (PAIR) {
+    a[c.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    a[c.numAttrs].val.clusterDim.x = 2;
+    a[c.numAttrs].val.clusterDim.y = a[c.numAttrs].val.clusterDim.z = 1;
+    ++c.numAttrs;
+  }
+  if (early) {
+    a[c.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    a[c.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++c.numAttrs;
+  }
   e = cudaLaunchKernelEx(&c, kern, args...);
   count_launch();
   return e == cudaSuccess ? cudaGetLastError() : e;
@@ -1292,13 +1419,13 @@ cudaError_t launch(K kern, long long workers, int smem, cudaStream_t st, const A
 template <bool BF16, int NT, bool PAIR>
 cudaError_t launch_fwd(const Maps& m, FwdArgs g, long long most, cudaStream_t st) {
   g.tiles_m = (g.M + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128);
-  return launch<PAIR>(grouped_umma_kernel<BF16, NT, PAIR>, most * g.tiles_m * g.splits, Cfg<NT, PAIR>::kSmem, st, m.a, m.x, m.b, m.t, g);
+  return launch<PAIR>(grouped_umma_kernel<BF16, NT, PAIR>, most * g.tiles_m * g.splits, Cfg<NT, PAIR>::kSmem, g.wait != kWaitNone, st, m.a, m.x, m.b, m.t, g);
 }
 template <bool BF16, int NT, bool PAIR>
 cudaError_t launch_bwd(const CUtensorMap& r, const CUtensorMap& c, GradArgs g, cudaStream_t st) {
   g.tiles_r = (g.rows + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128);
   g.tiles_c = g.fold ? 1 : (g.cols + NT - 1) / NT;
-  return launch<PAIR>(grouped_grad_umma_kernel<BF16, NT, PAIR>, (long long)g.tiles_r * g.tiles_c * g.mats, Cfg<NT, PAIR>::kSmem, st, r, c, g);
+  return launch<PAIR>(grouped_grad_umma_kernel<BF16, NT, PAIR>, (long long)g.tiles_r * g.tiles_c * g.mats, Cfg<NT, PAIR>::kSmem, g.wait != 0, st, r, c, g);
 }
 
 // Rows and columns of a tile.
@@ -1380,15 +1507,19 @@ size_t copies_bytes(const GroupedArgs& g, const Shape& s) {
 }
 size_t parts_bytes(const GroupedArgs& g, const Shape& s) { return padded((size_t)s.splits * g.R * g.M * sizeof(float)); }
 
-// One product; `to` and `out`: what it writes and where.  ws: copies_bytes().
-cudaError_t product(const GroupedArgs& g, int dtype, const Shape& s, int to, void* out, char* ws, cudaStream_t st) {
+// One product; `to` and `out`: what it writes and where.  ws: copies_bytes().  before: what of this call was launched before it (kWaitData:
+// it reads that; kWaitEnd: it does not).
+cudaError_t product(const GroupedArgs& g, int dtype, const Shape& s, int to, void* out, char* ws, int before, cudaStream_t st) {
+  bool behind = before != kWaitNone, copied = false;
   Operand a = matrices(g.A, g.transA != 0, g.M, g.K, g.lda, g.strideA, g.mats), x = columns_of(g.X, g.K, g.N, g.ldx, g.columns, g.R);
   const Runs runs{g.offsets, g.run_len, g.G, g.R};
   const bool in_place = g.columns && gathers_in_place(x, s);
   if (in_place) x = columns_of(g.X, g.K, g.N, g.ldx, nullptr, 0);
-  cudaError_t e = align_operand(a, ws, g.ids || !g.offsets ? nullptr : &runs, st);
-  if (e == cudaSuccess) e = align_operand(x, ws, nullptr, st);
+  const size_t copies = a.copy_bytes() + x.copy_bytes();
+  cudaError_t e = align_operand(a, ws, g.ids || !g.offsets ? nullptr : &runs, behind, st);
+  if (e == cudaSuccess) e = align_operand(x, ws, nullptr, behind, st);
   if (e != cudaSuccess) return e;
+  copied = copies > 0;
   FwdArgs f;
   std::memset(&f, 0, sizeof(f));
   f.runs = runs;
@@ -1415,7 +1546,8 @@ cudaError_t product(const GroupedArgs& g, int dtype, const Shape& s, int to, voi
   f.vec = aligned16(out) && g.ldc % 8 == 0;
   if (g.low.r > 0 && to == kToC) {
     Operand b = matrices(g.low.B, g.low.transB != 0, g.M, g.low.r, g.low.ldb, g.low.strideB, g.low.n);
-    if ((e = align_operand(b, ws, nullptr, st)) != cudaSuccess) return e;
+    copied = copied || b.copy_bytes() > 0;
+    if ((e = align_operand(b, ws, nullptr, behind, st)) != cudaSuccess) return e;
     const Operand t{g.low.T, low_width(g.low.r), g.R, low_width(g.low.r), 0, 1, nullptr, 0};
     if (!encode_matrix(&m.b, dtype, b, g.low.transB != 0) || !encode_columns(&m.t, dtype, t, box_of(s))) return cudaErrorInvalidValue;
     f.low_runs = Runs{g.low.offsets, g.low.run_len, g.low.runs, g.R};
@@ -1423,6 +1555,7 @@ cudaError_t product(const GroupedArgs& g, int dtype, const Shape& s, int to, voi
     f.r = g.low.r; f.n = g.low.n;
     f.low_kmaj = g.low.transB;
   }
+  f.wait = copied ? kWaitData : before;
   return dtype == NNLIB_B200_BF16 ? fwd<true>(s, m, f, st) : fwd<false>(s, m, f, st);
 }
 
@@ -1445,10 +1578,8 @@ cudaError_t join(const GroupedArgs& g, int dtype, const Shape& s, const float* p
     j.b_pairs = (reinterpret_cast<uintptr_t>(g.low.B) & 3u) == 0 && g.low.ldb % 2 == 0 && g.low.strideB % 2 == 0;
   }
   const dim3 grid((unsigned)g.R, (unsigned)((g.M + 255) / 256));
-  if (dtype == NNLIB_B200_BF16) join_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(j);
-  else join_kernel<__half><<<grid, 128, 0, st>>>(j);
   count_launch();
-  return cudaGetLastError();
+  return dtype == NNLIB_B200_BF16 ? launch_early(join_kernel<__nv_bfloat16>, grid, dim3(128), 0, st, j) : launch_early(join_kernel<__half>, grid, dim3(128), 0, st, j);
 }
 // K is cut for few columns only: parts of many cost more than the SMs that it fills
 bool few(int R, int M) { return R <= 512 && M <= 65535 * 256; }
@@ -1462,9 +1593,9 @@ size_t grouped_umma_workspace_bytes(const GroupedArgs& g) {
 cudaError_t grouped_umma(const GroupedArgs& g, int dtype, void* workspace, cudaStream_t st) {
   char* ws = static_cast<char*>(workspace);
   const Shape s = shape_of(g.M, g.K, g.R, g.G, few(g.R, g.M));
-  if (s.splits == 1) return product(g, dtype, s, kToC, g.C, ws, st);
+  if (s.splits == 1) return product(g, dtype, s, kToC, g.C, ws, kWaitNone, st);
   char* parts = ws + copies_bytes(g, s);
-  const cudaError_t e = product(g, dtype, s, kToParts, parts, ws, st);
+  const cudaError_t e = product(g, dtype, s, kToParts, parts, ws, kWaitNone, st);
   return e == cudaSuccess ? join(g, dtype, s, reinterpret_cast<const float*>(parts), nullptr, 0, st) : e;
 }
 
@@ -1475,47 +1606,78 @@ size_t low_umma_workspace_bytes(const GroupedArgs& f) {
   return copies_bytes(f, s) + (s.splits > 1 ? parts_bytes(f, s) : 0);
 }
 size_t low_umma_bytes(const GroupedArgs& f) { return padded((size_t)f.R * 2 * low_width(f.M)); }
-cudaError_t low_umma(const GroupedArgs& f, int dtype, void* T, void* workspace, cudaStream_t st) {
+// behind: a kernel of this call is before it in the stream, whose results it does not read but whose workspace it may write
+cudaError_t low_umma(const GroupedArgs& f, int dtype, void* T, void* workspace, bool behind, cudaStream_t st) {
+  const int before = behind ? kWaitData : kWaitNone;
   const Shape s = first_shape(f);
   char* ws = static_cast<char*>(workspace);
-  if (s.splits == 1) return product(f, dtype, s, kToLow, T, ws, st);
+  if (s.splits == 1) return product(f, dtype, s, kToLow, T, ws, before, st);
   char* parts = ws + copies_bytes(f, s);
-  const cudaError_t e = product(f, dtype, s, kToParts, parts, ws, st);
+  const cudaError_t e = product(f, dtype, s, kToParts, parts, ws, before, st);
   if (e != cudaSuccess) return e;
   const int width = low_width(f.M);
   const long long blocks = ((long long)f.R * (width / 2) + 255) / 256;
   const float* p = reinterpret_cast<const float*>(parts);
-  if (dtype == NNLIB_B200_BF16) join_low_kernel<<<(unsigned)blocks, 256, 0, st>>>(p, s.splits, f.M, f.R, static_cast<__nv_bfloat16*>(T), width);
-  else join_low_kernel<<<(unsigned)blocks, 256, 0, st>>>(p, s.splits, f.M, f.R, static_cast<__half*>(T), width);
   count_launch();
-  return cudaGetLastError();
+  const dim3 grid((unsigned)blocks);
+  if (dtype == NNLIB_B200_BF16) return launch_early(join_low_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, p, s.splits, f.M, f.R, static_cast<__nv_bfloat16*>(T), width);
+  return launch_early(join_low_kernel<__half>, grid, dim3(256), 0, st, p, s.splits, f.M, f.R, static_cast<__half*>(T), width);
 }
 
 // W X with the pairs' term; first.R columns.  keep: T of the columns is wanted behind it (the gradients read it), at `low`.
 static Shape main_shape(const GroupedArgs& m, bool keep) { return shape_of(m.M, m.K, m.R, 1, !keep && few(m.R, m.M)); }
+// (a pair is read anew for each of its columns)
+static bool first_by_column(const GroupedArgs& f) { return f.R <= 4 * f.G && f.K <= 64 * kLowK; }
 size_t adapter_umma_workspace_bytes(const GroupedArgs& first, const GroupedArgs& m, bool keep) {
   const Shape s = main_shape(m, keep);
   if (s.splits == 1) return std::max(m.low.r > 0 ? low_umma_workspace_bytes(first) : 0, copies_bytes(m, s));
-  const Shape f = first_shape(first);
-  return copies_bytes(m, s) + parts_bytes(m, s) + (m.low.r > 0 ? copies_bytes(first, f) + parts_bytes(first, f) : 0);
+  Shape f = first_shape(first);
+  const size_t own = copies_bytes(m, s) + parts_bytes(m, s);
+  if (m.low.r == 0) return own;
+  if (!first_by_column(first)) return own + copies_bytes(first, f) + parts_bytes(first, f);
+  f.splits = (first.K + kLowK - 1) / kLowK;
+  return own + parts_bytes(first, f);
 }
 cudaError_t adapter_umma(const GroupedArgs& first, GroupedArgs m, int dtype, bool keep, void* low, void* workspace, cudaStream_t st) {
   const Shape s = main_shape(m, keep);
   char* ws = static_cast<char*>(workspace);
   cudaError_t e = cudaSuccess;
   if (s.splits == 1) {
-    if (m.low.r > 0) e = low_umma(first, dtype, low, ws, st);
+    if (m.low.r > 0) e = low_umma(first, dtype, low, ws, false, st);
     m.low.T = low;
-    return e == cudaSuccess ? product(m, dtype, s, kToC, m.C, ws, st) : e;
+    return e == cudaSuccess ? product(m, dtype, s, kToC, m.C, ws, m.low.r > 0 ? kWaitData : kWaitNone, st) : e;
   }
-  // few columns: both products in parts, joined by one launch that multiplies by B
-  const Shape f = first_shape(first);
+  // few columns: both products in parts, joined by one launch that multiplies by B.  W X does not wait for A X, its end does.
+  Shape f = first_shape(first);
   char* parts = ws + copies_bytes(m, s);
-  char* ws_first = parts + parts_bytes(m, s);
-  char* of_first = ws_first + (m.low.r > 0 ? copies_bytes(first, f) : 0);
-  if (m.low.r > 0) e = product(first, dtype, f, kToParts, of_first, ws_first, st);
-  if (e == cudaSuccess) e = product(m, dtype, s, kToParts, parts, ws, st);
-  return e == cudaSuccess ? join(m, dtype, s, reinterpret_cast<const float*>(parts), m.low.r > 0 ? reinterpret_cast<const float*>(of_first) : nullptr, f.splits, st) : e;
+  char* rest = parts + parts_bytes(m, s);
+  if (m.low.r == 0) {
+    e = product(m, dtype, s, kToParts, parts, ws, kWaitNone, st);
+    return e == cudaSuccess ? join(m, dtype, s, reinterpret_cast<const float*>(parts), nullptr, 0, st) : e;
+  }
+  char* of_first = rest;
+  if (first_by_column(first)) {
+    LowFewArgs l;
+    l.A = first.A; l.X = first.X;
+    l.parts = reinterpret_cast<float*>(of_first);
+    l.lda = first.lda; l.strideA = first.strideA; l.ldx = first.ldx;
+    l.scale = first.scale; l.scale0 = first.scale0;
+    l.runs = Runs{first.offsets, first.run_len, first.G, first.R};
+    l.ids = first.ids;
+    l.transA = first.transA; l.r = first.M; l.K = first.K; l.R = first.R; l.mats = first.mats;
+    l.vec = aligned16(first.A) && first.lda % 8 == 0 && first.strideA % 8 == 0 && (first.transA ? first.K : first.M) % 8 == 0;
+    f.splits = (first.K + kLowK - 1) / kLowK;
+    const dim3 grid((unsigned)first.R, (unsigned)f.splits);
+    if (dtype == NNLIB_B200_BF16) low_few_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(l);
+    else low_few_kernel<__half><<<grid, 256, 0, st>>>(l);
+    count_launch();
+    e = cudaGetLastError();
+  } else {
+    of_first = rest + copies_bytes(first, f);
+    e = product(first, dtype, f, kToParts, of_first, rest, kWaitNone, st);
+  }
+  if (e == cudaSuccess) e = product(m, dtype, s, kToParts, parts, ws, kWaitEnd, st);
+  return e == cudaSuccess ? join(m, dtype, s, reinterpret_cast<const float*>(parts), reinterpret_cast<const float*>(of_first), f.splits, st) : e;
 }
 
 size_t grouped_umma_grad_workspace_bytes(const GroupedGradArgs& g, int fold) {
@@ -1526,12 +1688,12 @@ bool grouped_umma_grad_supports(const GroupedGradArgs& g, int dtype) {
   return (dtype == NNLIB_B200_F16 || dtype == NNLIB_B200_BF16) && g.M > 0 && g.K > 0 && g.N > 0 && g.R > 0 && g.mats > 0 && encode_tiled_fn() != nullptr;
 }
 // fold: 0: none; 1: C is T, M its rank; 2: X is T, K its rank
-cudaError_t grouped_umma_grad(const GroupedGradArgs& g, int dtype, int fold, void* workspace, cudaStream_t st) {
+cudaError_t grouped_umma_grad(const GroupedGradArgs& g, int dtype, int fold, void* workspace, bool behind, cudaStream_t st) {
   char* ws = static_cast<char*>(workspace);
   Operand c = columns_of(g.C, fold == 1 ? low_width(g.M) : g.M, g.R, g.ldc, nullptr, 0),
           x = columns_of(g.X, fold == 2 ? low_width(g.K) : g.K, g.N, g.ldx, g.columns, g.R);
-  cudaError_t e = align_operand(c, ws, nullptr, st);
-  if (e == cudaSuccess) e = align_operand(x, ws, nullptr, st);
+  cudaError_t e = align_operand(c, ws, nullptr, behind, st);
+  if (e == cudaSuccess) e = align_operand(x, ws, nullptr, behind, st);
   if (e != cudaSuccess) return e;
   GradArgs a;
   std::memset(&a, 0, sizeof(a));
@@ -1541,6 +1703,7 @@ cudaError_t grouped_umma_grad(const GroupedGradArgs& g, int dtype, int fold, voi
   a.ld = g.lda; a.stride = g.strideA;
   a.G = g.G; a.mats = g.mats;
   a.status = g.status;
+  a.wait = behind;
   // the folded side's terms are neighbours in a row of tensor memory; otherwise the side that is contiguous in the result is in its lanes
   const bool x_rows = fold ? fold == 1 : g.transA != 0;
   a.rows = x_rows ? g.K : g.M;

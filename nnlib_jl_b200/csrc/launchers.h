@@ -261,12 +261,13 @@ cudaError_t grouped_umma(const GroupedArgs& g, int dtype, void* workspace, cudaS
 int low_width(int r);                                     // 16-bit elements of T for a column
 size_t low_umma_bytes(const GroupedArgs& first);          // T of all columns
 size_t low_umma_workspace_bytes(const GroupedArgs& first);
-cudaError_t low_umma(const GroupedArgs& first, int dtype, void* T, void* workspace, cudaStream_t st);
+cudaError_t low_umma(const GroupedArgs& first, int dtype, void* T, void* workspace, bool behind, cudaStream_t st);
 size_t adapter_umma_workspace_bytes(const GroupedArgs& first, const GroupedArgs& main, bool keep);
 cudaError_t adapter_umma(const GroupedArgs& first, GroupedArgs main, int dtype, bool keep, void* low, void* workspace, cudaStream_t st);
 bool grouped_umma_grad_supports(const GroupedGradArgs& g, int dtype);
 size_t grouped_umma_grad_workspace_bytes(const GroupedGradArgs& g, int fold);
-cudaError_t grouped_umma_grad(const GroupedGradArgs& g, int dtype, int fold, void* workspace, cudaStream_t st);   // fold: C (1) or X (2) is T
+// fold: C (1) or X (2) is T; behind: a kernel of this call is before it in the stream
+cudaError_t grouped_umma_grad(const GroupedGradArgs& g, int dtype, int fold, void* workspace, bool behind, cudaStream_t st);
 cudaError_t grouped_take_abort(int* out, cudaStream_t st);
 
 }  // namespace nb200

@@ -14,6 +14,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "early.cuh"
 #include "launchers.h"
 
 namespace nb200 {
@@ -235,6 +236,7 @@ __global__ void __launch_bounds__(32 * W) route_choose_kernel(const RouteArgs a)
   extern __shared__ int sm[];
   __shared__ int part[W];
   const int t0 = blockIdx.x * a.per_block, t1 = min(a.N, t0 + a.per_block);
+  let_next();
   for (int i = threadIdx.x; i < a.G; i += blockDim.x) sm[i] = 0;
   __syncthreads();
   for (int t = t0 + (threadIdx.x >> 5); t < t1; t += W) choose_token<T, V, PACKED>(a, t, threadIdx.x & 31, sm);
@@ -253,6 +255,8 @@ __global__ void __launch_bounds__(32 * W) route_choose_kernel(const RouteArgs a)
 // counts of each expert, block by block, to the number of its pairs in earlier blocks; a warp an expert
 __global__ void __launch_bounds__(256) route_scan_kernel(const RouteArgs a) {
   const int e = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  let_next();
+  wait_before();
   if (e >= a.G) return;
   int* c = a.ws + (long long)e * a.blocks;
   int carry = 0;
@@ -286,6 +290,7 @@ __global__ void __launch_bounds__(256) route_scan_kernel(const RouteArgs a) {
 __global__ void __launch_bounds__(256) route_number_kernel(const RouteArgs a) {
   extern __shared__ int sm[];
   __shared__ int part[8];
+  wait_before();
   const int* totals = a.ws + (long long)a.G * a.blocks;
   for (int i = threadIdx.x; i < a.G; i += blockDim.x) sm[i] = totals[i];
   __syncthreads();
@@ -375,10 +380,11 @@ cudaError_t launch_choose(RouteArgs a, cudaStream_t st) {
     return cudaGetLastError();
   }
   route_choose_kernel<T, V, PACKED, false, kChooseWarps><<<a.blocks, 32 * kChooseWarps, counts, st>>>(a);
-  route_scan_kernel<<<(a.G + 7) / 8, 256, 0, st>>>(a);
-  route_number_kernel<<<a.blocks, 256, counts + masks, st>>>(a);
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) e = launch_early(route_scan_kernel, dim3((a.G + 7) / 8), dim3(256), 0, st, a);
+  if (e == cudaSuccess) e = launch_early(route_number_kernel, dim3(a.blocks), dim3(256), counts + masks, st, a);
   count_launch(3);
-  return cudaGetLastError();
+  return e;
 }
 template <typename T, int V>
 cudaError_t launch_route(const RouteArgs& a, cudaStream_t st) {
