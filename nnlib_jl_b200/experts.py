@@ -103,15 +103,24 @@ def _columns(t: torch.Tensor, E: int, N: int) -> torch.Tensor:
     return t.new_empty_strided((E, N), (1, E or 1))
 
 
+_entries: dict = {}
+
+
 def _run(entry: str, p, dev, works: bool = True):
-    lib = _lib.load()
+    """The library's entry point of that name, with a workspace where it wants one."""
+    fns = _entries.get(entry)
+    if fns is None:
+        lib = _lib.load()
+        fns = _entries[entry] = (getattr(lib, "nnlib_b200_" + entry), getattr(lib, f"nnlib_b200_{entry}_workspace_bytes") if works else None)
+    call, size = fns
+    ref = C.byref(p)
     with _on_device(dev):
-        if not works:
-            _check(getattr(lib, "nnlib_b200_" + entry)(C.byref(p), _stream()), entry)
+        if size is None:
+            _check(call(ref, _stream()), entry)
             return
-        need = getattr(lib, f"nnlib_b200_{entry}_workspace_bytes")(C.byref(p))
+        need = size(ref)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        _check(getattr(lib, "nnlib_b200_" + entry)(C.byref(p), ws.data_ptr() if need else None, need, _stream()), entry)
+        _check(call(ref, ws.data_ptr() if need else None, need, _stream()), entry)
 
 
 # ------------------------------------------------------------------------------------------------- router
