@@ -118,6 +118,20 @@ int workspace_ok(const void* ws, size_t bytes, size_t need) {
   return need && (!ws || bytes < need || !aligned(ws, 16)) ? NNLIB_B200_WORKSPACE_TOO_SMALL : NNLIB_B200_OK;
 }
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+// On the CUDA cores, K in parts where that pays (ws: fma_ws() bytes); f32_out: C is Float32, whatever A and X are
+size_t fma_ws(const GroupedArgs& a) {
+  const int splits = a.M && a.R ? grouped_fma_splits(a) : 1;
+  return splits > 1 ? round256(sizeof(float) * splits * (size_t)a.R * a.M) : 0;
+}
+cudaError_t fma_product(GroupedArgs a, int dtype, bool f32_out, void* ws, cudaStream_t st) {
+  const int splits = a.M && a.R ? grouped_fma_splits(a) : 1;
+  if (splits == 1) return grouped_fma(a, dtype, f32_out, nullptr, st);
+  const float* t = a.low.r > 0 ? static_cast<const float*>(a.low.T) : nullptr;
+  GroupedArgs main = a;
+  main.low.r = 0;
+  const cudaError_t e = grouped_fma(main, dtype, f32_out, static_cast<float*>(ws), st);
+  return e != cudaSuccess ? e : join_parts(a, f32_out ? NNLIB_B200_F32 : dtype, splits, static_cast<const float*>(ws), t, 1, st);
+}
 
 int check_grouped_arrays(const GroupedArgs& a) {
   const void* all[] = {a.C, a.X, a.A, a.offsets, a.columns, a.status};
@@ -242,14 +256,14 @@ cudaError_t adapter_products(Adapters& a, int dtype, bool umma, bool keep, void*
   a.main.low.T = low;
   a.main.low.ldt = a.first.M;
   if (has_pairs(a)) {
-    const cudaError_t e = grouped_fma(a.first, dtype, true, st);
+    const cudaError_t e = fma_product(a.first, dtype, true, ws, st);
     if (e != cudaSuccess) return e;
   }
-  return grouped_fma(a.main, dtype, false, st);
+  return fma_product(a.main, dtype, false, ws, st);
 }
 size_t adapter_ws(Adapters& a, bool umma, bool keep) {
   if (!has_pairs(a)) a.main.low.r = 0;
-  return umma ? adapter_umma_workspace_bytes(a.first, a.main, keep) : 0;
+  return umma ? adapter_umma_workspace_bytes(a.first, a.main, keep) : std::max(fma_ws(a.first), fma_ws(a.main));
 }
 
 // Gradients of the pairs: dA = (scale B^T dC) X^T, dB = dC (scale A X)^T.  `other`: A X for them.
@@ -310,18 +324,18 @@ int nnlib_b200_route_bwd(const nnlib_b200_route_params* p, void* stream) {
 size_t nnlib_b200_grouped_gemm_workspace_bytes(const nnlib_b200_grouped_params* p) {
   GroupedArgs a;
   if (resolve_grouped(p, &a)) return 0;
-  return on_umma(a, p->dtype) ? grouped_umma_workspace_bytes(a) : 0;
+  return on_umma(a, p->dtype) ? grouped_umma_workspace_bytes(a) : fma_ws(a);
 }
 int nnlib_b200_grouped_gemm(const nnlib_b200_grouped_params* p, void* workspace, size_t workspace_bytes, void* stream) {
   GroupedArgs a;
   int rc = resolve_grouped(p, &a);
   if (rc || a.M == 0 || a.R == 0) return rc;
   const bool umma = on_umma(a, p->dtype);
-  if (umma && (rc = workspace_ok(workspace, workspace_bytes, grouped_umma_workspace_bytes(a)))) return rc;
+  if ((rc = workspace_ok(workspace, workspace_bytes, umma ? grouped_umma_workspace_bytes(a) : fma_ws(a)))) return rc;
   if ((rc = check_grouped_arrays(a))) return rc;
   if (log_calls())
     std::fprintf(stderr, "[nnlib_b200] grouped_gemm M=%d K=%d G=%d N=%d R=%d -> %s\n", a.M, a.K, a.G, a.N, a.R, umma ? "tcgen05" : "cuda-core");
-  return finish(umma ? grouped_umma(a, p->dtype, workspace, (cudaStream_t)stream) : grouped_fma(a, p->dtype, false, (cudaStream_t)stream));
+  return finish(umma ? grouped_umma(a, p->dtype, workspace, (cudaStream_t)stream) : fma_product(a, p->dtype, false, workspace, (cudaStream_t)stream));
 }
 size_t nnlib_b200_grouped_gemm_grad_workspace_bytes(const nnlib_b200_grouped_params* p) {
   GroupedArgs a;
@@ -383,6 +397,7 @@ size_t nnlib_b200_adapter_bwd_workspace_bytes(const nnlib_b200_adapter_params* p
   if (resolve_adapter(p, true, &a)) return 0;
   const bool umma = adapter_on_umma(a, p->dtype);
   size_t rest = adapter_ws(a, umma, true);
+  if (!umma && p->dA) rest = std::max(rest, fma_ws(pair_grads(p, a, false).first));
   if (umma && p->dA) {
     const PairGrads g = pair_grads(p, a, true);
     rest = std::max({rest, low_umma_workspace_bytes(g.first), grouped_umma_grad_workspace_bytes(g.a, 1), grouped_umma_grad_workspace_bytes(g.b, 2)});
@@ -409,7 +424,7 @@ int nnlib_b200_adapter_bwd(const nnlib_b200_adapter_params* p, void* workspace, 
   g.a.C = of_dC;
   g.b.X = of_X;
   if (!umma) {
-    if ((rc = finish(grouped_fma(g.first, p->dtype, true, st)))) return rc;
+    if ((rc = finish(fma_product(g.first, p->dtype, true, ws, st)))) return rc;
     if ((rc = finish(grouped_fma_grad(g.a, p->dtype, true, false, st)))) return rc;
     return finish(grouped_fma_grad(g.b, p->dtype, false, true, st));
   }

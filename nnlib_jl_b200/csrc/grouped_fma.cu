@@ -1,124 +1,220 @@
-// Products of ragged groups of columns on the CUDA cores, exact fp32 in ascending k, any element type, size and stride.
+// Products of ragged groups of columns on the CUDA cores, exact fp32 in ascending k, any element type, size and stride: Float32 arrays, and
+// what of the 16-bit ones grouped_umma.cu does not take.
 //
 //   grouped_fma_kernel   C[:, i] = A_g X[:, columns[i]] for the columns i of run g, and, for low-rank pairs, + B_a T[:, i]
+//   grouped_narrow_kernel  the same for runs of up to four columns
 //   grouped_grad_kernel  A_a = sum over the columns i of the runs of matrix a of C[:, i] X[:, columns[i]]^T
 //
-// Tiles and their shared-memory stages are gemm_fma.cu's: 256 threads, BT x BT, k in steps of 16, two stages.  A block's slot
-// number is turned into (run, first column) by counting the tiles of all runs, since their sizes are on the device only; slots
-// that no run needs end at once.  FMA bound: BT = 128 reads four 16-byte words of shared memory for 64 multiply-adds.
+// 256 threads compute 128 rows x BN columns, k in steps of 16 or 32 through two shared-memory stages [k][row]: while one is multiplied the next
+// one's elements are on their way into registers, four neighbours at a time.  A thread owns 8 rows and BN / 16 columns, its products are
+// packed pairs of rows.  A block's slot number is turned into (run, first column) by counting the tiles of all runs, since their sizes
+// are on the device only; slots that no run needs end at once.  Few tiles: K is cut and the parts are added by another launch
+// (join_columns).  What bounds it: the FMA pipe and shared memory where columns are many (2048 x 2048, 4096 columns in 8 runs: FWD_BIG),
+// reading A where they are few.
 #include <algorithm>
 
 #include "common.cuh"
 #include "grouped_runs.cuh"
 #include "launchers.h"
+#include "umma.cuh"
 
 namespace nb200 {
 namespace {
 
-// acc[i][j] += Q[k][i] * P[k][j] for a stage of BT + 4 wide rows
-template <int BT>
+using ptx::pair_fma;
+using ptx::pair_of;
+using ptx::pair_unpack;
+
+constexpr int kRows = 128;                   // rows to a tile
+
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    return *reinterpret_cast<const float4*>(p);
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    const T* e = reinterpret_cast<const T*>(&v);
+    return make_float4(Elem<T>::to_f(e[0]), Elem<T>::to_f(e[1]), Elem<T>::to_f(e[2]), Elem<T>::to_f(e[3]));
+  }
+}
+
+// One side of a contraction: elements (k, r) of W rows r, as they lie in memory.
+//   along:  k contiguous; row r begins at base + row(r) * ld, or is none (row(r) < 0: zeros)
+//   else    r contiguous; step k begins at base + step(k) * ld, or is none (zeros); `rows` of them are there
+template <typename T>
+struct Side {
+  const T* base;
+  long long ld;
+  bool along, vec;                           // vec: four neighbours at an address of their size's multiple
+  int rows;
+  const int* table;                          // along: row(r), in shared memory, or NULL: r < rows; else step(k) of the whole contraction, or NULL: k
+  int limit;                                 // else, with a table: its entries below this are there
+};
+
+// k to a stage: narrow tiles are there to read A, 16 KB of it at a time
+__host__ __device__ constexpr int step_of(int bn) { return bn <= 32 ? 32 : 16; }
+
+template <typename T, int W, int KS>
+struct Loader {
+  static constexpr int NV = W * KS >= 1024 ? W * KS / 1024 : 1, kThreads = W * KS / 4 / NV;   // of 256 threads, these load
+  const Side<T>& s;
+  float4 v[NV];
+  __device__ __forceinline__ Loader(const Side<T>& side) : s(side) {}
+  __device__ __forceinline__ void fetch(int k0, int K) {
+#pragma unroll
+    for (int e = 0; e < NV; ++e) {
+      const int q = threadIdx.x + 256 * e;
+      v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (kThreads < 256 && threadIdx.x >= kThreads) continue;
+      float* f = reinterpret_cast<float*>(&v[e]);
+      if (s.along) {
+        const int k = k0 + (q % (KS / 4)) * 4, r = q / (KS / 4), row = s.table ? s.table[r] : (r < s.rows ? r : -1);
+        if (row < 0) continue;
+        const T* p = s.base + row * s.ld + k;
+        if (s.vec && k + 4 <= K) {
+          v[e] = load4(p);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (k + i < K) f[i] = Elem<T>::to_f(p[i]);
+        }
+      } else {
+        const int r = (q % (W / 4)) * 4, k = k0 + q / (W / 4);
+        if (k >= K || r >= s.rows) continue;
+        const int step = s.table ? s.table[k] : k;
+        if (s.table && (unsigned)step >= (unsigned)s.limit) continue;
+        const T* p = s.base + step * s.ld + r;
+        if (s.vec && r + 4 <= s.rows) {
+          v[e] = load4(p);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (r + i < s.rows) f[i] = Elem<T>::to_f(p[i]);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void stage(float (*t)[W + 4]) {
+#pragma unroll
+    for (int e = 0; e < NV; ++e) {
+      const int q = threadIdx.x + 256 * e;
+      if (kThreads < 256 && threadIdx.x >= kThreads) continue;
+      if (s.along) {
+        const int k = (q % (KS / 4)) * 4, r = q / (KS / 4);
+        t[k][r] = v[e].x;
+        t[k + 1][r] = v[e].y;
+        t[k + 2][r] = v[e].z;
+        t[k + 3][r] = v[e].w;
+      } else {
+        *reinterpret_cast<float4*>(&t[q / (W / 4)][(q % (W / 4)) * 4]) = v[e];
+      }
+    }
+  }
+};
+
+template <int BN>
+struct Stages {
+  static constexpr int kStep = step_of(BN);
+  float p[2][kStep][kRows + 4], q[2][kStep][BN + 4];
+};
+
+// a thread's part of a 128 x BN tile: rows row(j), columns column(i)
+template <int BN>
 struct Tile {
-  static constexpr int KG = 16;
-  static constexpr int R = BT / 16, G = R < 4 ? R : 4, LD = BT + 4, NL = BT * KG / 256;
-  float acc[R][R];                           // [column side][row side]
+  static constexpr int R = BN / 16, G = R < 4 ? R : 4;
+  unsigned long long acc[R][4];              // pairs of rows
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int i = 0; i < R; ++i)
 #pragma unroll
-      for (int j = 0; j < R; ++j) acc[i][j] = 0.f;
+      for (int j = 0; j < 4; ++j) acc[i][j] = 0ull;
   }
-  __device__ __forceinline__ void step(const float* p, const float* q, int tx, int ty) {
-    float am[R], bn[R];
+  __device__ __forceinline__ void step(const float* p, const float* q) {
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    unsigned long long a[4];
 #pragma unroll
-    for (int r = 0; r < R; r += G) {
+    for (int h = 0; h < 2; ++h) {
+      const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p + tx * 4 + h * 64);
+      a[2 * h] = v.x;
+      a[2 * h + 1] = v.y;
+    }
+    float b[R];
+#pragma unroll
+    for (int i = 0; i < R; i += G) {
       if constexpr (G == 4) {
-        const float4 va = *reinterpret_cast<const float4*>(p + tx * 4 + r * 16);
-        const float4 vb = *reinterpret_cast<const float4*>(q + ty * 4 + r * 16);
-        am[r] = va.x; am[r + 1] = va.y; am[r + 2] = va.z; am[r + 3] = va.w;
-        bn[r] = vb.x; bn[r + 1] = vb.y; bn[r + 2] = vb.z; bn[r + 3] = vb.w;
+        const float4 v = *reinterpret_cast<const float4*>(q + ty * 4 + i * 16);
+        b[i] = v.x; b[i + 1] = v.y; b[i + 2] = v.z; b[i + 3] = v.w;
       } else {
-        const float2 va = *reinterpret_cast<const float2*>(p + tx * 2);
-        const float2 vb = *reinterpret_cast<const float2*>(q + ty * 2);
-        am[0] = va.x; am[1] = va.y;
-        bn[0] = vb.x; bn[1] = vb.y;
+#pragma unroll
+        for (int u = 0; u < G; ++u) b[u] = q[ty * G + u];
       }
     }
 #pragma unroll
-    for (int i = 0; i < R; ++i)
+    for (int i = 0; i < R; ++i) {
+      const unsigned long long bb = pair_of(b[i]);
 #pragma unroll
-      for (int j = 0; j < R; ++j) acc[i][j] = fmaf(am[j], bn[i], acc[i][j]);
+      for (int j = 0; j < 4; ++j) acc[i][j] = pair_fma(a[j], bb, acc[i][j]);
+    }
   }
-  static __device__ __forceinline__ int place(int t, int i) { return t * G + (i / G) * 16 * G + i % G; }
+  __device__ __forceinline__ void values(int i, float (&v)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) pair_unpack(acc[i][j], v[2 * j], v[2 * j + 1]);
+  }
+  static __device__ __forceinline__ int row(int j) { return (threadIdx.x & 15) * 4 + (j >> 2) * 64 + (j & 3); }
+  static __device__ __forceinline__ int column(int i) { return (threadIdx.x >> 4) * G + (i / G) * 16 * G + i % G; }
 };
 
-template <int BT>
-struct Stages {
-  float p[2][Tile<BT>::KG][Tile<BT>::LD], q[2][Tile<BT>::KG][Tile<BT>::LD];
-};
-
-// One contraction of K terms: P(k, row) and Q(k, column) give the elements (0 where there is none); `pk`: P's neighbours in
-// memory are along k
-template <int BT, typename FP, typename FQ>
-__device__ __forceinline__ void contract(Tile<BT>& t, Stages<BT>& s, int K, bool pk, bool qk, FP P, FQ Q) {
-  constexpr int NL = Tile<BT>::NL, KG = Tile<BT>::KG;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float rp[NL], rq[NL];
-  auto at = [&](int e, bool along, int& k, int& r) {
-    const int c = e * 256 + threadIdx.x;
-    if (along) { k = c % KG; r = c / KG; } else { r = c % BT; k = c / BT; }
-  };
-  auto fetch = [&](int k0) {
-#pragma unroll
-    for (int e = 0; e < NL; ++e) {
-      int k, r;
-      at(e, pk, k, r);
-      rp[e] = k0 + k < K ? P(k0 + k, r) : 0.f;
-      at(e, qk, k, r);
-      rq[e] = k0 + k < K ? Q(k0 + k, r) : 0.f;
-    }
-  };
-  auto stage = [&](int b) {
-#pragma unroll
-    for (int e = 0; e < NL; ++e) {
-      int k, r;
-      at(e, pk, k, r);
-      s.p[b][k][r] = rp[e];
-      at(e, qk, k, r);
-      s.q[b][k][r] = rq[e];
-    }
-  };
-  if (K <= 0) return;
-  fetch(0);
+// One contraction over k0 .. K - 1 (k0 a multiple of 4)
+template <int BN, typename TP, typename TQ>
+__device__ __forceinline__ void contract(Tile<BN>& t, Stages<BN>& s, int k0, int K, const Side<TP>& P, const Side<TQ>& Q) {
+  constexpr int kStep = step_of(BN);
+  if (K <= k0) return;
+  Loader<TP, kRows, kStep> p(P);
+  Loader<TQ, BN, kStep> q(Q);
+  p.fetch(k0, K);
+  q.fetch(k0, K);
   __syncthreads();                           // (an earlier contraction's last stage has been read)
-  stage(0);
+  p.stage(s.p[0]);
+  q.stage(s.q[0]);
   __syncthreads();
-  for (int k0 = 0, b = 0; k0 < K; k0 += KG, b ^= 1) {
-    const bool more = k0 + KG < K;
-    if (more) fetch(k0 + KG);
-    const int kn = min(KG, K - k0);         // the padding is not multiplied: 0 * Inf would be a NaN
-    if (kn == KG) {
-#pragma unroll
-      for (int k = 0; k < KG; ++k) t.step(s.p[b][k], s.q[b][k], tx, ty);
-    } else {
-      for (int k = 0; k < kn; ++k) t.step(s.p[b][k], s.q[b][k], tx, ty);
+  for (int b = 0; k0 < K; k0 += kStep, b ^= 1) {
+    const bool more = k0 + kStep < K;
+    if (more) {
+      p.fetch(k0 + kStep, K);
+      q.fetch(k0 + kStep, K);
     }
-    if (more) stage(b ^ 1);
+    const int kn = min(kStep, K - k0);       // the padding is not multiplied: 0 * Inf would be a NaN
+    if (kn == kStep) {
+#pragma unroll
+      for (int k = 0; k < kStep; ++k) t.step(s.p[b][k], s.q[b][k]);
+    } else {
+      for (int k = 0; k < kn; ++k) t.step(s.p[b][k], s.q[b][k]);
+    }
+    if (more) {
+      p.stage(s.p[b ^ 1]);
+      q.stage(s.q[b ^ 1]);
+    }
     __syncthreads();
   }
 }
 
-template <typename T, typename TC, int BT>
-__global__ void __launch_bounds__(256) grouped_fma_kernel(const GroupedArgs g) {
-  __shared__ __align__(16) Stages<BT> st;
+template <typename T>
+__host__ __device__ __forceinline__ bool fours(const T* p, long long a, long long b) {
+  return (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)) == 0 && a % 4 == 0 && b % 4 == 0;
+}
+
+// blockIdx: (slot of columns, tile of rows, part of K).  parts: Float32 (M, R, parts) instead of C
+template <typename T, typename TC, int BN>
+__global__ void __launch_bounds__(256) grouped_fma_kernel(const __grid_constant__ GroupedArgs g, float* parts) {
+  __shared__ __align__(16) Stages<BN> st;
   __shared__ RunSearch search;
-  __shared__ int cols[BT];
-  const RunTile run = find_run(Runs{g.offsets, g.run_len, g.G, g.R}, g.zero_rest, BT, blockIdx.x, search);
+  __shared__ int cols[BN];
+  const RunTile run = find_run(Runs{g.offsets, g.run_len, g.G, g.R}, g.zero_rest && !parts, BN, blockIdx.x, search);
   if (run.run == kNoRun) return;
-  const int m0 = blockIdx.y * BT, n0 = run.first, nn = min(BT, run.end - n0);
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int m0 = blockIdx.y * kRows, n0 = run.first, nn = min(BN, run.end - n0);
   const int mat = run.run < 0 ? -1 : (g.ids ? g.ids[run.run] : run.run);
   const bool have = mat >= 0 && mat < g.mats;
-  for (int i = threadIdx.x; i < BT; i += 256) {
+  for (int i = threadIdx.x; i < BN; i += 256) {
     int c = -1;
     if (have && i < nn) {
       c = g.columns ? g.columns[n0 + i] : n0 + i;
@@ -127,143 +223,293 @@ __global__ void __launch_bounds__(256) grouped_fma_kernel(const GroupedArgs g) {
     cols[i] = c;
   }
   __syncthreads();
-  Tile<BT> t;
+  Tile<BN> t;
   t.clear();
-  const T* X = reinterpret_cast<const T*>(g.X);
+  const int rows = min(kRows, g.M - m0);
   if (have) {
-    const T* A = reinterpret_cast<const T*>(g.A) + (long long)mat * g.strideA;
-    contract<BT>(t, st, g.K, g.transA != 0, true,
-                 [&](int k, int r) { return m0 + r < g.M ? Elem<T>::to_f(g.transA ? A[(long long)(m0 + r) * g.lda + k] : A[(long long)k * g.lda + m0 + r]) : 0.f; },
-                 [&](int k, int r) { return cols[r] >= 0 ? Elem<T>::to_f(X[(long long)cols[r] * g.ldx + k]) : 0.f; });
+    const T* A = reinterpret_cast<const T*>(g.A) + (long long)mat * g.strideA + (g.transA ? (long long)m0 * g.lda : m0);
+    const T* X = reinterpret_cast<const T*>(g.X);
+    const int each = ((g.K + gridDim.z - 1) / gridDim.z + 31) / 32 * 32, k0 = blockIdx.z * each;
+    contract<BN>(t, st, k0, min(g.K, k0 + each), Side<T>{A, g.lda, g.transA != 0, fours(A, g.lda, 0), rows, nullptr, 0},
+                 Side<T>{X, g.ldx, true, fours(X, g.ldx, 0), BN, cols, 0});
   }
   const float scale = !have ? 0.f : (g.scale ? g.scale[mat] : g.scale0);
-  if (scale != 1.f) {
+  float c[Tile<BN>::R][8];
 #pragma unroll
-    for (int i = 0; i < Tile<BT>::R; ++i)
+  for (int i = 0; i < Tile<BN>::R; ++i) {
+    t.values(i, c[i]);
 #pragma unroll
-      for (int j = 0; j < Tile<BT>::R; ++j) t.acc[i][j] *= scale;
+    for (int j = 0; j < 8; ++j) c[i][j] *= scale;
   }
   if (g.low.r > 0) {
     // the runs of pairs that have columns here, one after the other; columns of other runs take no part
     const Runs of{g.low.offsets, g.low.run_len, g.low.runs, g.R};
     const float* low = reinterpret_cast<const float*>(g.low.T);
+    __shared__ int mine[BN];
     for (int b = 0; b < g.low.runs; ++b) {
       const int lo = max(of.begin(b), n0), hi = min(of.end(b), n0 + nn), id = g.low.ids[b];
       if (lo >= hi || id < 0 || id >= g.low.n) continue;
-      const T* B = reinterpret_cast<const T*>(g.low.B) + (long long)id * g.low.strideB;
-      Tile<BT> u;
-      u.clear();
-      contract<BT>(u, st, g.low.r, g.low.transB != 0, true,
-                   [&](int k, int r) { return m0 + r < g.M ? Elem<T>::to_f(g.low.transB ? B[(long long)(m0 + r) * g.low.ldb + k] : B[(long long)k * g.low.ldb + m0 + r]) : 0.f; },
-                   [&](int k, int r) { return n0 + r >= lo && n0 + r < hi ? low[(long long)(n0 + r) * g.low.ldt + k] : 0.f; });
+      const T* B = reinterpret_cast<const T*>(g.low.B) + (long long)id * g.low.strideB + (g.low.transB ? (long long)m0 * g.low.ldb : m0);
+      __syncthreads();
+      for (int i = threadIdx.x; i < BN; i += 256) mine[i] = n0 + i >= lo && n0 + i < hi ? n0 + i : -1;
+      __syncthreads();
+      t.clear();
+      contract<BN>(t, st, 0, g.low.r, Side<T>{B, g.low.ldb, g.low.transB != 0, fours(B, g.low.ldb, 0), rows, nullptr, 0},
+                   Side<float>{low, g.low.ldt, true, fours(low, g.low.ldt, 0), BN, mine, 0});
 #pragma unroll
-      for (int i = 0; i < Tile<BT>::R; ++i) {
-        const int n = n0 + Tile<BT>::place(ty, i);
+      for (int i = 0; i < Tile<BN>::R; ++i) {
+        const int n = n0 + Tile<BN>::column(i);
         if (n < lo || n >= hi) continue;     // (0 * Inf of another pair's matrix)
+        float v[8];
+        t.values(i, v);
 #pragma unroll
-        for (int j = 0; j < Tile<BT>::R; ++j) t.acc[i][j] += u.acc[i][j];
+        for (int j = 0; j < 8; ++j) c[i][j] += v[j];
       }
     }
   }
-  TC* C = reinterpret_cast<TC*>(g.C);
 #pragma unroll
-  for (int i = 0; i < Tile<BT>::R; ++i) {
-    const int c = Tile<BT>::place(ty, i);
-    if (c >= nn) continue;
-    const bool zero = cols[c] < 0;           // (a padding column's 0 times an infinity of A)
+  for (int i = 0; i < Tile<BN>::R; ++i) {
+    const int n = Tile<BN>::column(i);
+    if (n >= nn) continue;
+    const bool zero = cols[n] < 0;           // (a padding column's 0 times an infinity of A)
+    if (parts) {
+      float* out = parts + ((long long)blockIdx.z * g.R + n0 + n) * g.M + m0;
 #pragma unroll
-    for (int j = 0; j < Tile<BT>::R; ++j) {
-      const int m = m0 + Tile<BT>::place(tx, j);
-      if (m < g.M) C[(long long)(n0 + c) * g.ldc + m] = Elem<TC>::from_f(zero ? 0.f : t.acc[i][j]);
+      for (int j = 0; j < 8; ++j)
+        if (Tile<BN>::row(j) < rows) out[Tile<BN>::row(j)] = c[i][j];
+    } else {
+      TC* out = reinterpret_cast<TC*>(g.C) + (long long)(n0 + n) * g.ldc + m0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (Tile<BN>::row(j) < rows) out[Tile<BN>::row(j)] = Elem<TC>::from_f(zero ? 0.f : c[i][j]);
+    }
+  }
+}
+
+// Runs of a few columns: nothing of A is read twice, so none of it goes through shared memory.  128 rows and up to kNarrow columns to a block.
+// Rows contiguous: a lane has four rows, every eighth k is a warp's; k contiguous: a warp has 16 rows, a lane every 32nd four of k.
+// (a token of 32 columns, 8 of 128 matrices of 1536 x 2048 each: NARROW_US, in tiles of 16 columns 1148 us)
+constexpr int kNarrow = 4, kChunk = 1024;
+template <typename T, typename TC>
+__global__ void __launch_bounds__(256, 2) grouped_narrow_kernel(const __grid_constant__ GroupedArgs g, float* parts) {
+  __shared__ __align__(16) float x[kNarrow][kChunk];
+  __shared__ __align__(16) float sums[8][kNarrow][kRows];
+  __shared__ RunSearch search;
+  const RunTile run = find_run(Runs{g.offsets, g.run_len, g.G, g.R}, g.zero_rest && !parts, kNarrow, blockIdx.x, search);
+  if (run.run == kNoRun) return;
+  const int m0 = blockIdx.y * kRows, n0 = run.first, nn = min(kNarrow, run.end - n0), rows = min(kRows, g.M - m0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int mat = run.run < 0 ? -1 : (g.ids ? g.ids[run.run] : run.run);
+  const bool have = mat >= 0 && mat < g.mats;
+  int col[kNarrow];
+#pragma unroll
+  for (int c = 0; c < kNarrow; ++c) {
+    col[c] = have && c < nn ? (g.columns ? g.columns[n0 + c] : n0 + c) : -1;
+    if (col[c] >= g.N) col[c] = -1;
+  }
+  float acc[16][kNarrow];                    // rows contiguous: the first four rows; else the warp's 16
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+#pragma unroll
+    for (int c = 0; c < kNarrow; ++c) acc[i][c] = 0.f;
+  const int each = ((g.K + gridDim.z - 1) / gridDim.z + 31) / 32 * 32, k1 = have ? min(g.K, (int)(blockIdx.z + 1) * each) : 0;
+  const T* A = reinterpret_cast<const T*>(g.A) + (long long)(have ? mat : 0) * g.strideA + (g.transA ? (long long)m0 * g.lda : m0);
+  const bool vec = fours(A, g.lda, 0);
+  for (int k0 = blockIdx.z * each; k0 < k1; k0 += kChunk) {
+    const int nk = min(kChunk, k1 - k0);
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < kNarrow; ++c)
+      for (int k = threadIdx.x; k < nk; k += 256)
+        x[c][k] = col[c] >= 0 ? Elem<T>::to_f(reinterpret_cast<const T*>(g.X)[(long long)col[c] * g.ldx + k0 + k]) : 0.f;
+    __syncthreads();
+    if (!g.transA) {
+      const int r = lane * 4;
+      const T* a = A + (long long)k0 * g.lda + r;
+#pragma unroll 8
+      for (int k = warp; k < nk; k += 8) {
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        const T* p = a + (long long)k * g.lda;
+        if (vec && r + 4 <= rows) {
+          const float4 f = load4(p);
+          v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (r + i < rows) v[i] = Elem<T>::to_f(p[i]);
+        }
+#pragma unroll
+        for (int c = 0; c < kNarrow; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[i][c] = fmaf(v[i], x[c][k], acc[i][c]);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {          // four rows at a time
+#pragma unroll 2
+        for (int k = lane * 4; k < nk; k += 128) {
+          float4 v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = warp * 16 + q * 4 + i;
+            v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r >= rows) continue;
+            const T* p = A + r * g.lda + k0 + k;
+            if (vec && k + 4 <= nk) {
+              v[i] = load4(p);
+            } else {
+              float* f = reinterpret_cast<float*>(&v[i]);
+#pragma unroll
+              for (int u = 0; u < 4; ++u)
+                if (k + u < nk) f[u] = Elem<T>::to_f(p[u]);
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < kNarrow; ++c) {
+            float4 b = *reinterpret_cast<const float4*>(&x[c][k]);
+            if (k + 4 > nk) {                // (what is behind the end of the chunk is an older one's)
+              if (k + 1 >= nk) b.y = 0.f;
+              if (k + 2 >= nk) b.z = 0.f;
+              b.w = 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              acc[q * 4 + i][c] = fmaf(v[i].x, b.x, fmaf(v[i].y, b.y, fmaf(v[i].z, b.z, fmaf(v[i].w, b.w, acc[q * 4 + i][c]))));
+          }
+        }
+      }
+    }
+  }
+  // to sums[w][c][row]: w = 8 warps of every row, or one
+  if (!g.transA) {
+#pragma unroll
+    for (int c = 0; c < kNarrow; ++c) *reinterpret_cast<float4*>(&sums[warp][c][lane * 4]) = make_float4(acc[0][c], acc[1][c], acc[2][c], acc[3][c]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+      for (int c = 0; c < kNarrow; ++c) {
+        float v = acc[i][c];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (lane == 0) sums[0][c][warp * 16 + i] = v;
+      }
+  }
+  __syncthreads();
+  const float scale = !have ? 0.f : (g.scale ? g.scale[mat] : g.scale0);
+  for (int i = threadIdx.x; i < kNarrow * kRows; i += 256) {
+    const int c = i / kRows, r = i % kRows;
+    if (c >= nn || r >= rows) continue;
+    float v = sums[0][c][r];
+    if (!g.transA)
+      for (int w = 1; w < 8; ++w) v += sums[w][c][r];
+    v *= scale;
+    if (parts) parts[((long long)blockIdx.z * g.R + n0 + c) * g.M + m0 + r] = v;
+    else {
+      const int from = have ? (g.columns ? g.columns[n0 + c] : n0 + c) : -1;
+      reinterpret_cast<TC*>(g.C)[(long long)(n0 + c) * g.ldc + m0 + r] = Elem<TC>::from_f((unsigned)from < (unsigned)g.N ? v : 0.f);
     }
   }
 }
 
 // blockIdx: (column tile of A, row tile of A, matrix).  Rows of A are C's, columns X's.
-template <typename TC, typename TX, typename TA, int BT>
-__global__ void __launch_bounds__(256) grouped_grad_kernel(const GroupedGradArgs g) {
-  __shared__ __align__(16) Stages<BT> st;
-  const int k0 = blockIdx.x * BT, m0 = blockIdx.y * BT, a = blockIdx.z;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const TC* C = reinterpret_cast<const TC*>(g.C);
-  const TX* X = reinterpret_cast<const TX*>(g.X);
+template <typename TC, typename TX, typename TA, int BN>
+__global__ void __launch_bounds__(256) grouped_grad_kernel(const __grid_constant__ GroupedGradArgs g) {
+  __shared__ __align__(16) Stages<BN> st;
+  const int k0 = blockIdx.x * BN, m0 = blockIdx.y * kRows, a = blockIdx.z, rows = min(kRows, g.M - m0), cols = min(BN, g.K - k0);
   const Runs of{g.offsets, g.run_len, g.G, g.R};
-  Tile<BT> t;
+  Tile<BN> t;
   t.clear();
   for (int b = g.ids ? 0 : a; b < (g.ids ? g.G : min(a + 1, g.G)); ++b) {
     if (g.ids && g.ids[b] != a) continue;
     const int lo = of.begin(b), n = of.end(b) - lo;
-    contract<BT>(t, st, n, false, false,
-                 [&](int i, int r) {
-                   if (m0 + r >= g.M) return 0.f;
-                   if (g.columns && (unsigned)g.columns[lo + i] >= (unsigned)g.N) return 0.f;
-                   return Elem<TC>::to_f(C[(long long)(lo + i) * g.ldc + m0 + r]);
-                 },
-                 [&](int i, int r) {
-                   if (k0 + r >= g.K) return 0.f;
-                   const int c = g.columns ? g.columns[lo + i] : lo + i;
-                   return (unsigned)c < (unsigned)g.N ? Elem<TX>::to_f(X[(long long)c * g.ldx + k0 + r]) : 0.f;
-                 });
+    const TC* C = reinterpret_cast<const TC*>(g.C) + (long long)lo * g.ldc + m0;
+    const TX* X = reinterpret_cast<const TX*>(g.X) + (g.columns ? 0 : (long long)lo * g.ldx) + k0;
+    contract<BN>(t, st, 0, n, Side<TC>{C, g.ldc, false, fours(C, g.ldc, 0), rows, nullptr, 0},
+                 Side<TX>{X, g.ldx, false, fours(X, g.ldx, 0), cols, g.columns ? g.columns + lo : nullptr, g.N});
   }
   TA* A = reinterpret_cast<TA*>(g.A) + (long long)a * g.strideA;
 #pragma unroll
-  for (int i = 0; i < Tile<BT>::R; ++i) {
-    const int k = k0 + Tile<BT>::place(ty, i);
+  for (int i = 0; i < Tile<BN>::R; ++i) {
+    const int k = k0 + Tile<BN>::column(i);
     if (k >= g.K) continue;
+    float v[8];
+    t.values(i, v);
 #pragma unroll
-    for (int j = 0; j < Tile<BT>::R; ++j) {
-      const int m = m0 + Tile<BT>::place(tx, j);
-      if (m < g.M) A[g.transA ? (long long)m * g.lda + k : (long long)k * g.lda + m] = Elem<TA>::from_f(t.acc[i][j]);
+    for (int j = 0; j < 8; ++j) {
+      const int m = m0 + Tile<BN>::row(j);
+      if (m < g.M) A[g.transA ? (long long)m * g.lda + k : (long long)k * g.lda + m] = Elem<TA>::from_f(v[j]);
     }
   }
 }
 
-template <typename T, typename TC, int BT>
-cudaError_t launch(const GroupedArgs& g, cudaStream_t st) {
-  const long long slots = run_slots(g.R, g.G, BT), rows = (g.M + BT - 1) / BT;
-  if (slots > 0x7fffffffLL || rows > 65535) return cudaErrorInvalidConfiguration;
-  grouped_fma_kernel<T, TC, BT><<<dim3((unsigned)slots, (unsigned)rows), 256, 0, st>>>(g);
-  count_launch();
-  return cudaGetLastError();
-}
-// The largest tile that is not mostly padding for runs of the average length and still gives most SMs a block: a tile of 32 reads twice as
-// much shared memory for its products as one of 64 (333 x 200 by 1200 columns in 5 runs: 20 us in tiles of 32, 17 in tiles of 64).
-template <typename T, typename TC>
-cudaError_t launch_of(const GroupedArgs& g, cudaStream_t st) {
-  if (g.M < 1 || g.R < 1) return cudaSuccess;
-  const long long each = g.R / std::max(1, g.G);
-  auto blocks = [&](long long bt) { return (g.R / bt + 1) * ((g.M + bt - 1) / bt); };
-  if (each > 64 && g.M > 64 && blocks(128) >= 148) return launch<T, TC, 128>(g, st);
-  if (each > 32 && g.M > 32 && blocks(64) >= 100) return launch<T, TC, 64>(g, st);
-  return launch<T, TC, 32>(g, st);
+struct FmaShape {
+  int bn, splits;
+};
+// As many columns to a tile as the average run has, fewer where that leaves SMs without a tile (333 x 200 by 1200 columns in 5 runs: RAGGED128
+// in tiles of 128 columns, RAGGED32 of 32), and K cut into parts of at least 128 while tiles are fewer than two to an SM and the parts are few.
+FmaShape fma_shape(const GroupedArgs& g) {
+  const long long each = std::max<long long>(1, g.R / std::max(1, g.G)), rows = (g.M + kRows - 1) / kRows;
+  FmaShape s;
+  s.bn = each > 64 ? 128 : each > 32 ? 64 : each > 16 ? 32 : each > kNarrow ? 16 : kNarrow;
+  auto tiles = [&] { return ((each + s.bn - 1) / s.bn) * std::min(g.G, g.R) * rows; };
+  auto cut = [&] {
+    int splits = 1;
+    while (splits < 32 && tiles() * splits < 296 && g.K / (2 * splits) >= 128 && (g.R <= 512 || 8ll * splits * g.R * g.M <= (16ll << 20))) splits *= 2;
+    return splits;
+  };
+  while (s.bn > 32 && tiles() * cut() < 148) s.bn /= 2;
+  s.splits = cut();
+  if (s.bn == kNarrow && g.low.r > 0 && s.splits == 1) s.bn = 16;      // (low-rank pairs: in the wider tiles, or by the launch that adds the parts)
+  return s;
 }
 
-template <typename TC, typename TX, typename TA, int BT>
-cudaError_t launch_grad(const GroupedGradArgs& g, cudaStream_t st) {
-  const long long rows = (g.M + BT - 1) / BT;
-  if (rows > 65535 || g.mats > 65535) return cudaErrorInvalidConfiguration;
-  grouped_grad_kernel<TC, TX, TA, BT><<<dim3((unsigned)((g.K + BT - 1) / BT), (unsigned)rows, (unsigned)g.mats), 256, 0, st>>>(g);
+template <typename T, typename TC>
+cudaError_t launch_of(const GroupedArgs& g, const FmaShape& s, float* parts, cudaStream_t st) {
+  const long long slots = run_slots(g.R, g.G, s.bn), rows = (g.M + kRows - 1) / kRows;
+  if (slots > 0x7fffffffLL || rows > 65535) return cudaErrorInvalidConfiguration;
+  const dim3 grid((unsigned)slots, (unsigned)rows, (unsigned)s.splits);
+  switch (s.bn) {
+    case 128: grouped_fma_kernel<T, TC, 128><<<grid, 256, 0, st>>>(g, parts); break;
+    case 64:  grouped_fma_kernel<T, TC, 64><<<grid, 256, 0, st>>>(g, parts); break;
+    case 32:  grouped_fma_kernel<T, TC, 32><<<grid, 256, 0, st>>>(g, parts); break;
+    case 16:  grouped_fma_kernel<T, TC, 16><<<grid, 256, 0, st>>>(g, parts); break;
+    default:  grouped_narrow_kernel<T, TC><<<grid, 256, 0, st>>>(g, parts); break;
+  }
   count_launch();
   return cudaGetLastError();
 }
-// (there the sums are the runs', which a tile of 64 walks as long as one of 32: 25 us and 40)
+
 template <typename TC, typename TX, typename TA>
 cudaError_t launch_grad_of(const GroupedGradArgs& g, cudaStream_t st) {
   if (g.M < 1 || g.K < 1 || g.mats < 1) return cudaSuccess;
-  auto blocks = [&](long long bt) { return ((g.K + bt - 1) / bt) * ((g.M + bt - 1) / bt) * g.mats; };
-  if (g.M > 64 && g.K > 64 && blocks(128) >= 148) return launch_grad<TC, TX, TA, 128>(g, st);
-  if (g.M > 32 && g.K > 32 && blocks(64) >= 148) return launch_grad<TC, TX, TA, 64>(g, st);
-  return launch_grad<TC, TX, TA, 32>(g, st);
+  const long long rows = (g.M + kRows - 1) / kRows;
+  if (rows > 65535 || g.mats > 65535) return cudaErrorInvalidConfiguration;
+  auto blocks = [&](long long bn) { return ((g.K + bn - 1) / bn) * rows * g.mats; };
+  const int bn = g.K > 64 && blocks(128) >= 148 ? 128 : g.K > 32 && blocks(64) >= 148 ? 64 : g.K > 16 ? 32 : 16;
+  const dim3 grid((unsigned)((g.K + bn - 1) / bn), (unsigned)rows, (unsigned)g.mats);
+  switch (bn) {
+    case 128: grouped_grad_kernel<TC, TX, TA, 128><<<grid, 256, 0, st>>>(g); break;
+    case 64:  grouped_grad_kernel<TC, TX, TA, 64><<<grid, 256, 0, st>>>(g); break;
+    case 32:  grouped_grad_kernel<TC, TX, TA, 32><<<grid, 256, 0, st>>>(g); break;
+    default:  grouped_grad_kernel<TC, TX, TA, 16><<<grid, 256, 0, st>>>(g); break;
+  }
+  count_launch();
+  return cudaGetLastError();
 }
 
 }  // namespace
 
-// low: C is Float32, whatever A and X are
-cudaError_t grouped_fma(const GroupedArgs& g, int dtype, bool f32_out, cudaStream_t st) {
+// parts: Float32 (M, R, grouped_fma_splits(g)) instead of C
+int grouped_fma_splits(const GroupedArgs& g) { return fma_shape(g).splits; }
+cudaError_t grouped_fma(const GroupedArgs& g, int dtype, bool f32_out, float* parts, cudaStream_t st) {
+  if (g.M < 1 || g.R < 1) return cudaSuccess;
+  FmaShape s = fma_shape(g);
+  if (!parts) s.splits = 1;
   switch (dtype) {
-    case NNLIB_B200_F16:  return f32_out ? launch_of<__half, float>(g, st) : launch_of<__half, __half>(g, st);
-    case NNLIB_B200_BF16: return f32_out ? launch_of<__nv_bfloat16, float>(g, st) : launch_of<__nv_bfloat16, __nv_bfloat16>(g, st);
-    default:              return launch_of<float, float>(g, st);
+    case NNLIB_B200_F16:  return f32_out ? launch_of<__half, float>(g, s, parts, st) : launch_of<__half, __half>(g, s, parts, st);
+    case NNLIB_B200_BF16: return f32_out ? launch_of<__nv_bfloat16, float>(g, s, parts, st) : launch_of<__nv_bfloat16, __nv_bfloat16>(g, s, parts, st);
+    default:              return launch_of<float, float>(g, s, parts, st);
   }
 }
 // f32_rows / f32_cols: C / X are Float32, whatever A is

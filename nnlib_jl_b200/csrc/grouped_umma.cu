@@ -1127,10 +1127,10 @@ struct JoinArgs {
   const int* low_ids;
   const void* B;
   long long ldb, strideB;
-  int b_pairs;                           // rows of B come in pairs at 4-byte addresses
+  int b_pairs;                           // rows of B come in pairs at an address of their size's multiple
 };
 template <typename T>
-struct alignas(4) Two {
+struct alignas(2 * sizeof(T)) Two {
   T x, y;
 };
 template <typename T>
@@ -1559,13 +1559,19 @@ cudaError_t product(const GroupedArgs& g, int dtype, const Shape& s, int to, voi
   return dtype == NNLIB_B200_BF16 ? fwd<true>(s, m, f, st) : fwd<false>(s, m, f, st);
 }
 
-cudaError_t join(const GroupedArgs& g, int dtype, const Shape& s, const float* parts, const float* t, int t_splits, cudaStream_t st) {
+// K is cut for few columns only: parts of many cost more than the SMs that it fills
+bool few(int R, int M) { return R <= 512 && M <= 65535 * 256; }
+
+}  // namespace
+
+// parts: Float32 (M, R, splits); t: A X of g.low's pairs, Float32 (r, R, t_splits), or NULL
+cudaError_t join_parts(const GroupedArgs& g, int dtype, int splits, const float* parts, const float* t, int t_splits, cudaStream_t st) {
   JoinArgs j;
   std::memset(&j, 0, sizeof(j));
   j.parts = parts;
   j.C = g.C;
   j.ldc = g.ldc;
-  j.splits = s.splits; j.M = g.M; j.R = g.R; j.N = g.N; j.zero_rest = g.zero_rest;
+  j.splits = splits; j.M = g.M; j.R = g.R; j.N = g.N; j.zero_rest = g.zero_rest;
   j.runs = Runs{g.offsets, g.run_len, g.G, g.R};
   j.columns = g.columns;
   if (t) {
@@ -1575,17 +1581,16 @@ cudaError_t join(const GroupedArgs& g, int dtype, const Shape& s, const float* p
     j.low_ids = g.low.ids;
     j.B = g.low.B;
     j.ldb = g.low.ldb; j.strideB = g.low.strideB;
-    j.b_pairs = (reinterpret_cast<uintptr_t>(g.low.B) & 3u) == 0 && g.low.ldb % 2 == 0 && g.low.strideB % 2 == 0;
+    j.b_pairs = reinterpret_cast<uintptr_t>(g.low.B) % (dtype == NNLIB_B200_F32 ? 8 : 4) == 0 && g.low.ldb % 2 == 0 && g.low.strideB % 2 == 0;
   }
   const dim3 grid((unsigned)g.R, (unsigned)((g.M + 255) / 256));
   count_launch();
-  return dtype == NNLIB_B200_BF16 ? launch_early(join_kernel<__nv_bfloat16>, grid, dim3(128), 0, st, j) : launch_early(join_kernel<__half>, grid, dim3(128), 0, st, j);
+  switch (dtype) {
+    case NNLIB_B200_F16:  return launch_early(join_kernel<__half>, grid, dim3(128), 0, st, j);
+    case NNLIB_B200_BF16: return launch_early(join_kernel<__nv_bfloat16>, grid, dim3(128), 0, st, j);
+    default:              return launch_early(join_kernel<float>, grid, dim3(128), 0, st, j);
+  }
 }
-// K is cut for few columns only: parts of many cost more than the SMs that it fills
-bool few(int R, int M) { return R <= 512 && M <= 65535 * 256; }
-
-}  // namespace
-
 size_t grouped_umma_workspace_bytes(const GroupedArgs& g) {
   const Shape s = shape_of(g.M, g.K, g.R, g.G, few(g.R, g.M));
   return copies_bytes(g, s) + (s.splits > 1 ? parts_bytes(g, s) : 0);
@@ -1596,7 +1601,7 @@ cudaError_t grouped_umma(const GroupedArgs& g, int dtype, void* workspace, cudaS
   if (s.splits == 1) return product(g, dtype, s, kToC, g.C, ws, kWaitNone, st);
   char* parts = ws + copies_bytes(g, s);
   const cudaError_t e = product(g, dtype, s, kToParts, parts, ws, kWaitNone, st);
-  return e == cudaSuccess ? join(g, dtype, s, reinterpret_cast<const float*>(parts), nullptr, 0, st) : e;
+  return e == cudaSuccess ? join_parts(g, dtype, s.splits, reinterpret_cast<const float*>(parts), nullptr, 0, st) : e;
 }
 
 // A X of low-rank pairs, as T or, `parts`, in Float32 parts
@@ -1653,7 +1658,7 @@ cudaError_t adapter_umma(const GroupedArgs& first, GroupedArgs m, int dtype, boo
   char* rest = parts + parts_bytes(m, s);
   if (m.low.r == 0) {
     e = product(m, dtype, s, kToParts, parts, ws, kWaitNone, st);
-    return e == cudaSuccess ? join(m, dtype, s, reinterpret_cast<const float*>(parts), nullptr, 0, st) : e;
+    return e == cudaSuccess ? join_parts(m, dtype, s.splits, reinterpret_cast<const float*>(parts), nullptr, 0, st) : e;
   }
   char* of_first = rest;
   if (first_by_column(first)) {
@@ -1677,7 +1682,7 @@ cudaError_t adapter_umma(const GroupedArgs& first, GroupedArgs m, int dtype, boo
     e = product(first, dtype, f, kToParts, of_first, rest, kWaitNone, st);
   }
   if (e == cudaSuccess) e = product(m, dtype, s, kToParts, parts, ws, kWaitEnd, st);
-  return e == cudaSuccess ? join(m, dtype, s, reinterpret_cast<const float*>(parts), reinterpret_cast<const float*>(of_first), f.splits, st) : e;
+  return e == cudaSuccess ? join_parts(m, dtype, s.splits, reinterpret_cast<const float*>(parts), reinterpret_cast<const float*>(of_first), f.splits, st) : e;
 }
 
 size_t grouped_umma_grad_workspace_bytes(const GroupedGradArgs& g, int fold) {

@@ -252,7 +252,10 @@ struct GroupedGradArgs {
   int M, K, G, N, R, mats;
   int* status;
 };
-cudaError_t grouped_fma(const GroupedArgs& g, int dtype, bool f32_out, cudaStream_t st);
+// CUDA cores (grouped_fma.cu): everything.  parts: Float32 (M, R, grouped_fma_splits(g)) instead of C, for join_parts
+int grouped_fma_splits(const GroupedArgs& g);
+cudaError_t grouped_fma(const GroupedArgs& g, int dtype, bool f32_out, float* parts, cudaStream_t st);
+cudaError_t join_parts(const GroupedArgs& g, int dtype, int splits, const float* parts, const float* t, int t_splits, cudaStream_t st);   // (grouped_umma.cu)
 cudaError_t grouped_fma_grad(const GroupedGradArgs& g, int dtype, bool f32_rows, bool f32_cols, cudaStream_t st);
 // tcgen05 (grouped_umma.cu): 16-bit arrays
 bool grouped_umma_supports(const GroupedArgs& g, int dtype);

@@ -96,6 +96,39 @@ def test_more_runs_than_a_table_holds(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("M,K,G,N", [(300, 1200, 20, 40), (127, 1027, 9, 30), (64, 2500, 3, 4), (1030, 65, 50, 70), (5, 3000, 2, 5), (512, 640, 6, 300)])
+def test_a_few_columns_to_a_run_in_float32(M, K, G, N, turned):
+    gen = np.random.default_rng(M + K)
+    A, X = _matrices(gen, M, K, G, F32, turned), _cols(gen.standard_normal((K, 17)))
+    o = np.sort(gen.integers(0, N + 1, G + 1))
+    c = gen.integers(0, 17, N)
+    c[N // 2] = 99                                           # no column
+    X[:, 5] = float("inf")
+    none = torch.empty(0, device=DEV)
+    r = nb.Routing(none, none, _ints(o), _ints(c), none)
+    a, x = _f64(A), _f64(X)
+    fine = np.flatnonzero(c != 5)
+    x[:, 5] = 0
+    want, size = R.grouped(a, x, o, c), _bound(K, F32) * R.grouped(np.abs(a), np.abs(x), o, c)
+    for run in range(2):
+        got = nb.grouped_mul(A, X, r) if run else nb.grouped_mul_(_cols(np.full((M, N), 3.0)), A, X, r)
+        keep = fine if run else fine[(fine >= o[0]) & (fine < o[-1])]
+        _close(got[:, _ints(keep).long()], want[:, keep], F32, size[:, keep])
+        if not run:
+            assert (got[:, :o[0]] == 3).all() and (got[:, o[-1]:] == 3).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("turn", [(0, 0, 0), (1, 1, 1)])
+@pytest.mark.parametrize("M,K,r,n,N", [(320, 1024, 16, 7, 20), (131, 1500, 5, 3, 9), (512, 5000, 128, 4, 3), (64, 1024, 3, 2, 500), (40, 100, 8, 70, 64)])
+def test_single_columns_in_float32(turn, M, K, r, n, N):
+    ids = [(5 * i) % (n + 2) - 1 for i in range(N)]
+    for given in (False, True):
+        _adapter_case(F32, M, K, r, n, np.arange(N + 1), ids, N, turn, given)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", SIXTEEN)
 def test_one_matrix_for_every_run(dtype):
     gen = np.random.default_rng(4)
