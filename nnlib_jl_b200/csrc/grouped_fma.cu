@@ -290,8 +290,8 @@ __global__ void __launch_bounds__(256) grouped_fma_kernel(const __grid_constant_
 // Rows contiguous: a lane has four rows, every eighth k is a warp's; k contiguous: a warp has 16 rows, a lane every 32nd four of k.
 // (a token of 32 columns, 8 of 128 matrices of 1536 x 2048 each: NARROW_US, in tiles of 16 columns 1148 us)
 constexpr int kNarrow = 4, kChunk = 1024;
-template <typename T, typename TC>
-__global__ void __launch_bounds__(256, 2) grouped_narrow_kernel(const __grid_constant__ GroupedArgs g, float* parts) {
+template <typename T, typename TC, bool TURNED>
+__global__ void __launch_bounds__(256, TURNED ? 2 : 3) grouped_narrow_kernel(const __grid_constant__ GroupedArgs g, float* parts) {
   __shared__ __align__(16) float x[kNarrow][kChunk];
   __shared__ __align__(16) float sums[8][kNarrow][kRows];
   __shared__ RunSearch search;
@@ -307,13 +307,14 @@ __global__ void __launch_bounds__(256, 2) grouped_narrow_kernel(const __grid_con
     col[c] = have && c < nn ? (g.columns ? g.columns[n0 + c] : n0 + c) : -1;
     if (col[c] >= g.N) col[c] = -1;
   }
-  float acc[16][kNarrow];                    // rows contiguous: the first four rows; else the warp's 16
+  constexpr int kMine = TURNED ? 16 : 4;
+  float acc[kMine][kNarrow];
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
+  for (int i = 0; i < kMine; ++i)
 #pragma unroll
     for (int c = 0; c < kNarrow; ++c) acc[i][c] = 0.f;
   const int each = ((g.K + gridDim.z - 1) / gridDim.z + 31) / 32 * 32, k1 = have ? min(g.K, (int)(blockIdx.z + 1) * each) : 0;
-  const T* A = reinterpret_cast<const T*>(g.A) + (long long)(have ? mat : 0) * g.strideA + (g.transA ? (long long)m0 * g.lda : m0);
+  const T* A = reinterpret_cast<const T*>(g.A) + (long long)(have ? mat : 0) * g.strideA + (TURNED ? (long long)m0 * g.lda : m0);
   const bool vec = fours(A, g.lda, 0);
   for (int k0 = blockIdx.z * each; k0 < k1; k0 += kChunk) {
     const int nk = min(kChunk, k1 - k0);
@@ -323,7 +324,7 @@ __global__ void __launch_bounds__(256, 2) grouped_narrow_kernel(const __grid_con
       for (int k = threadIdx.x; k < nk; k += 256)
         x[c][k] = col[c] >= 0 ? Elem<T>::to_f(reinterpret_cast<const T*>(g.X)[(long long)col[c] * g.ldx + k0 + k]) : 0.f;
     __syncthreads();
-    if (!g.transA) {
+    if constexpr (!TURNED) {
       const int r = lane * 4;
       const T* a = A + (long long)k0 * g.lda + r;
 #pragma unroll 8
@@ -381,12 +382,12 @@ __global__ void __launch_bounds__(256, 2) grouped_narrow_kernel(const __grid_con
     }
   }
   // to sums[w][c][row]: w = 8 warps of every row, or one
-  if (!g.transA) {
+  if constexpr (!TURNED) {
 #pragma unroll
     for (int c = 0; c < kNarrow; ++c) *reinterpret_cast<float4*>(&sums[warp][c][lane * 4]) = make_float4(acc[0][c], acc[1][c], acc[2][c], acc[3][c]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+    for (int i = 0; i < kMine; ++i)
 #pragma unroll
       for (int c = 0; c < kNarrow; ++c) {
         float v = acc[i][c];
@@ -401,7 +402,7 @@ __global__ void __launch_bounds__(256, 2) grouped_narrow_kernel(const __grid_con
     const int c = i / kRows, r = i % kRows;
     if (c >= nn || r >= rows) continue;
     float v = sums[0][c][r];
-    if (!g.transA)
+    if (!TURNED)
       for (int w = 1; w < 8; ++w) v += sums[w][c][r];
     v *= scale;
     if (parts) parts[((long long)blockIdx.z * g.R + n0 + c) * g.M + m0 + r] = v;
@@ -412,33 +413,47 @@ __global__ void __launch_bounds__(256, 2) grouped_narrow_kernel(const __grid_con
   }
 }
 
-// blockIdx: (column tile of A, row tile of A, matrix).  Rows of A are C's, columns X's.
-template <typename TC, typename TX, typename TA, int BN>
+// blockIdx: (tile of A's shorter way, tile of its contiguous one, matrix).  The tile's rows are those along which A is contiguous, so that it is
+// stored in long pieces: A's own (sums over C's rows), or, turned, its columns (X's rows).
+template <typename TP, typename TQ, typename TA, int BN>
 __global__ void __launch_bounds__(256) grouped_grad_kernel(const __grid_constant__ GroupedGradArgs g) {
   __shared__ __align__(16) Stages<BN> st;
-  const int k0 = blockIdx.x * BN, m0 = blockIdx.y * kRows, a = blockIdx.z, rows = min(kRows, g.M - m0), cols = min(BN, g.K - k0);
+  const bool turned = g.transA != 0;
+  const int P = turned ? g.K : g.M, Q = turned ? g.M : g.K;
+  const int q0 = blockIdx.x * BN, p0 = blockIdx.y * kRows, a = blockIdx.z, rows = min(kRows, P - p0), cols = min(BN, Q - q0);
+  const void *p_base = turned ? g.X : g.C, *q_base = turned ? g.C : g.X;
+  const long long ldp = turned ? g.ldx : g.ldc, ldq = turned ? g.ldc : g.ldx;
   const Runs of{g.offsets, g.run_len, g.G, g.R};
   Tile<BN> t;
   t.clear();
   for (int b = g.ids ? 0 : a; b < (g.ids ? g.G : min(a + 1, g.G)); ++b) {
     if (g.ids && g.ids[b] != a) continue;
     const int lo = of.begin(b), n = of.end(b) - lo;
-    const TC* C = reinterpret_cast<const TC*>(g.C) + (long long)lo * g.ldc + m0;
-    const TX* X = reinterpret_cast<const TX*>(g.X) + (g.columns ? 0 : (long long)lo * g.ldx) + k0;
-    contract<BN>(t, st, 0, n, Side<TC>{C, g.ldc, false, fours(C, g.ldc, 0), rows, nullptr, 0},
-                 Side<TX>{X, g.ldx, false, fours(X, g.ldx, 0), cols, g.columns ? g.columns + lo : nullptr, g.N});
+    const int* table = g.columns ? g.columns + lo : nullptr;
+    const int *p_table = turned ? table : nullptr, *q_table = turned ? nullptr : table;
+    const TP* p = reinterpret_cast<const TP*>(p_base) + (p_table ? 0 : (long long)lo * ldp) + p0;
+    const TQ* q = reinterpret_cast<const TQ*>(q_base) + (q_table ? 0 : (long long)lo * ldq) + q0;
+    contract<BN>(t, st, 0, n, Side<TP>{p, ldp, false, fours(p, ldp, 0), rows, p_table, g.N}, Side<TQ>{q, ldq, false, fours(q, ldq, 0), cols, q_table, g.N});
   }
-  TA* A = reinterpret_cast<TA*>(g.A) + (long long)a * g.strideA;
+  TA* A = reinterpret_cast<TA*>(g.A) + (long long)a * g.strideA + p0;
+  const bool vec = fours(A, g.lda, 0);
 #pragma unroll
   for (int i = 0; i < Tile<BN>::R; ++i) {
-    const int k = k0 + Tile<BN>::column(i);
-    if (k >= g.K) continue;
+    const int c = Tile<BN>::column(i);
+    if (c >= cols) continue;
     float v[8];
     t.values(i, v);
+    TA* out = A + (long long)(q0 + c) * g.lda;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int m = m0 + Tile<BN>::row(j);
-      if (m < g.M) A[g.transA ? (long long)m * g.lda + k : (long long)k * g.lda + m] = Elem<TA>::from_f(v[j]);
+    for (int h = 0; h < 8; h += 4) {
+      const int r = Tile<BN>::row(h);
+      if (vec && sizeof(TA) == 4 && r + 4 <= rows) {
+        *reinterpret_cast<float4*>(out + r) = make_float4(v[h], v[h + 1], v[h + 2], v[h + 3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (r + j < rows) out[r + j] = Elem<TA>::from_f(v[h + j]);
+      }
     }
   }
 }
@@ -474,28 +489,35 @@ cudaError_t launch_of(const GroupedArgs& g, const FmaShape& s, float* parts, cud
     case 64:  grouped_fma_kernel<T, TC, 64><<<grid, 256, 0, st>>>(g, parts); break;
     case 32:  grouped_fma_kernel<T, TC, 32><<<grid, 256, 0, st>>>(g, parts); break;
     case 16:  grouped_fma_kernel<T, TC, 16><<<grid, 256, 0, st>>>(g, parts); break;
-    default:  grouped_narrow_kernel<T, TC><<<grid, 256, 0, st>>>(g, parts); break;
+    default:
+      if (g.transA) grouped_narrow_kernel<T, TC, true><<<grid, 256, 0, st>>>(g, parts);
+      else grouped_narrow_kernel<T, TC, false><<<grid, 256, 0, st>>>(g, parts);
+      break;
   }
   count_launch();
   return cudaGetLastError();
 }
 
-template <typename TC, typename TX, typename TA>
-cudaError_t launch_grad_of(const GroupedGradArgs& g, cudaStream_t st) {
-  if (g.M < 1 || g.K < 1 || g.mats < 1) return cudaSuccess;
-  const long long rows = (g.M + kRows - 1) / kRows;
+template <typename TP, typename TQ, typename TA>
+cudaError_t launch_grad_tiles(const GroupedGradArgs& g, cudaStream_t st) {
+  const long long P = g.transA ? g.K : g.M, Q = g.transA ? g.M : g.K, rows = (P + kRows - 1) / kRows;
   if (rows > 65535 || g.mats > 65535) return cudaErrorInvalidConfiguration;
-  auto blocks = [&](long long bn) { return ((g.K + bn - 1) / bn) * rows * g.mats; };
-  const int bn = g.K > 64 && blocks(128) >= 148 ? 128 : g.K > 32 && blocks(64) >= 148 ? 64 : g.K > 16 ? 32 : 16;
-  const dim3 grid((unsigned)((g.K + bn - 1) / bn), (unsigned)rows, (unsigned)g.mats);
+  auto blocks = [&](long long bn) { return ((Q + bn - 1) / bn) * rows * g.mats; };
+  const int bn = Q > 64 && blocks(128) >= 148 ? 128 : Q > 32 && blocks(64) >= 148 ? 64 : Q > 16 ? 32 : 16;
+  const dim3 grid((unsigned)((Q + bn - 1) / bn), (unsigned)rows, (unsigned)g.mats);
   switch (bn) {
-    case 128: grouped_grad_kernel<TC, TX, TA, 128><<<grid, 256, 0, st>>>(g); break;
-    case 64:  grouped_grad_kernel<TC, TX, TA, 64><<<grid, 256, 0, st>>>(g); break;
-    case 32:  grouped_grad_kernel<TC, TX, TA, 32><<<grid, 256, 0, st>>>(g); break;
-    default:  grouped_grad_kernel<TC, TX, TA, 16><<<grid, 256, 0, st>>>(g); break;
+    case 128: grouped_grad_kernel<TP, TQ, TA, 128><<<grid, 256, 0, st>>>(g); break;
+    case 64:  grouped_grad_kernel<TP, TQ, TA, 64><<<grid, 256, 0, st>>>(g); break;
+    case 32:  grouped_grad_kernel<TP, TQ, TA, 32><<<grid, 256, 0, st>>>(g); break;
+    default:  grouped_grad_kernel<TP, TQ, TA, 16><<<grid, 256, 0, st>>>(g); break;
   }
   count_launch();
   return cudaGetLastError();
+}
+template <typename TC, typename TX, typename TA>
+cudaError_t launch_grad_of(const GroupedGradArgs& g, cudaStream_t st) {
+  if (g.M < 1 || g.K < 1 || g.mats < 1) return cudaSuccess;
+  return g.transA ? launch_grad_tiles<TX, TC, TA>(g, st) : launch_grad_tiles<TC, TX, TA>(g, st);
 }
 
 }  // namespace
