@@ -1,16 +1,16 @@
-// Products of ragged groups of columns on the CUDA cores, exact fp32 in ascending k, any element type, size and stride: Float32 arrays, and
+// Products of ragged groups of columns on the CUDA cores, products and sums in fp32, any element type, size and stride: Float32 arrays, and
 // what of the 16-bit ones grouped_umma.cu does not take.
 //
-//   grouped_fma_kernel   C[:, i] = A_g X[:, columns[i]] for the columns i of run g, and, for low-rank pairs, + B_a T[:, i]
+//   grouped_fma_kernel     C[:, i] = A_g X[:, columns[i]] for the columns i of run g, and, for low-rank pairs, + B_a T[:, i]
 //   grouped_narrow_kernel  the same for runs of up to four columns
-//   grouped_grad_kernel  A_a = sum over the columns i of the runs of matrix a of C[:, i] X[:, columns[i]]^T
+//   grouped_grad_kernel    A_a = sum over the columns i of the runs of matrix a of C[:, i] X[:, columns[i]]^T
 //
 // 256 threads compute 128 rows x BN columns, k in steps of 16 or 32 through two shared-memory stages [k][row]: while one is multiplied the next
 // one's elements are on their way into registers, four neighbours at a time.  A thread owns 8 rows and BN / 16 columns, its products are
 // packed pairs of rows.  A block's slot number is turned into (run, first column) by counting the tiles of all runs, since their sizes
-// are on the device only; slots that no run needs end at once.  Few tiles: K is cut and the parts are added by another launch
-// (join_columns).  What bounds it: the FMA pipe and shared memory where columns are many (2048 x 2048, 4096 columns in 8 runs: FWD_BIG),
-// reading A where they are few.
+// are on the device only; slots that no run needs end at once.  Few tiles: K is cut and the parts are added by another launch (join_parts).
+// What bounds it: the FMA pipe and the shared memory that feeds it where columns are many (2048 x 2048, 4096 columns in 8 runs: 880 us,
+// 39 TFLOP/s; the gradient of the matrices 1074 us), reading A where they are few (6248 x 6680, 64 columns in 3 runs: 378 us, 1.3 TB/s).
 #include <algorithm>
 
 #include "common.cuh"
@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(256) grouped_fma_kernel(const __grid_constant_
 
 // Runs of a few columns: nothing of A is read twice, so none of it goes through shared memory.  128 rows and up to kNarrow columns to a block.
 // Rows contiguous: a lane has four rows, every eighth k is a warp's; k contiguous: a warp has 16 rows, a lane every 32nd four of k.
-// (a token of 32 columns, 8 of 128 matrices of 1536 x 2048 each: NARROW_US, in tiles of 16 columns 1148 us)
+// (two columns to each of 128 matrices of 1536 x 2048: 430 us, 3.7 TB/s, turned; 522 us not; in tiles of 16 columns 1148 us)
 constexpr int kNarrow = 4, kChunk = 1024;
 template <typename T, typename TC, bool TURNED>
 __global__ void __launch_bounds__(256, TURNED ? 2 : 3) grouped_narrow_kernel(const __grid_constant__ GroupedArgs g, float* parts) {
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(256, TURNED ? 2 : 3) grouped_narrow_kernel(con
 }
 
 // blockIdx: (tile of A's shorter way, tile of its contiguous one, matrix).  The tile's rows are those along which A is contiguous, so that it is
-// stored in long pieces: A's own (sums over C's rows), or, turned, its columns (X's rows).
+// stored in long pieces: C's rows, or, turned, X's.  (64 columns in 3 runs, 6248 x 6680, turned: 291 us, 558 us with C's rows)
 template <typename TP, typename TQ, typename TA, int BN>
 __global__ void __launch_bounds__(256) grouped_grad_kernel(const __grid_constant__ GroupedGradArgs g) {
   __shared__ __align__(16) Stages<BN> st;
@@ -461,8 +461,8 @@ __global__ void __launch_bounds__(256) grouped_grad_kernel(const __grid_constant
 struct FmaShape {
   int bn, splits;
 };
-// As many columns to a tile as the average run has, fewer where that leaves SMs without a tile (333 x 200 by 1200 columns in 5 runs: RAGGED128
-// in tiles of 128 columns, RAGGED32 of 32), and K cut into parts of at least 128 while tiles are fewer than two to an SM and the parts are few.
+// As many columns to a tile as the average run has, fewer where that leaves SMs without a tile (333 x 200 by 1200 columns in 5 runs: 36 us
+// in tiles of 128 columns, 20 us of 32), and K cut into parts of at least 128 while tiles are fewer than two to an SM and the parts are few.
 FmaShape fma_shape(const GroupedArgs& g) {
   const long long each = std::max<long long>(1, g.R / std::max(1, g.G)), rows = (g.M + kRows - 1) / kRows;
   FmaShape s;
