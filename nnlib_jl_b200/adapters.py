@@ -88,7 +88,8 @@ def adapter_mul(W: torch.Tensor, X: torch.Tensor, A: torch.Tensor, B: torch.Tens
     - 1`` (Int32, one more than requests, on the device; a column in no run gets ``W * X``; runs must not overlap), or, without
     ``offsets``, single columns.  ``scale``: a number, or Float32, one per pair.  Ranks from 1 to 128.
 
-    Both terms are summed in Float32 and rounded once.  In between, ``scale * A * X`` is kept as two terms of the element type."""
+    Both terms are summed in Float32 and rounded once.  In between, ``scale * A * X`` is kept as two terms of the element type or in Float32:
+    with Float16 arrays it may be infinite beyond 65504, whatever ``B`` makes of it."""
     p, X2 = _params(W, X, A, B, adapters, offsets, scale)
     out = _columns(X2, W.shape[0], X2.shape[1])
     p.C, p.ldc = out.data_ptr(), W.shape[0] or 1

@@ -7,16 +7,20 @@
 // columns along its columns.  That way round a tile's number of columns can be any multiple of 16 (the instruction's N is its own), so
 // that a run of 300 is two tiles of 160 and 140 and not 256 and 44, and one of 3 is padded to 16 and not to 128.
 //
-// One CTA owns an (MH*128 rows) x (at most NT columns) tile and walks over K in blocks of 64; the grid is persistent.
+// A CTA owns a tile of 128 rows x at most NT columns, a pair of CTAs (cta_group::2) one of 256 x 256, and walks over K in blocks of 64; the
+// grid is persistent.
 //   prologue    every CTA counts the tiles of all runs (at most kMaxRuns) into a table in shared memory
-//   warps 0, 10, 11  TMA producers, every third stage each: a ring of stages, each a K block of the matrix (K- or MN-major, as it
-//               is stored) and of the columns (K-major); gathered columns arrive four at a time (tile::gather4), their numbers in
+//   warps 0, 10, 11  TMA producers, every third stage each: a ring of stages, each a K block (of a pair two) of the matrix (K- or MN-major,
+//               as it is stored) and of the columns (K-major); gathered columns arrive four at a time (tile::gather4), their numbers in
 //               the lanes' registers.  One thread takes some 125 cycles for a copy: with a single producer a stage took 765 cycles,
 //               148 of them 4.2 TB/s
 //   warp 1      allocates tensor memory, issues every tcgen05.mma; for low-rank pairs it clears the rows of T that belong to
 //               other runs before it multiplies
-//   warps 2-9   epilogue: tensor memory -> registers -> C; two lanes exchange halves so that a store is two rows of a column
-// With MH*NT <= 256 two accumulators alternate, so that the epilogue of one tile overlaps the products of the next.
+//   warps 2-9   epilogue: tensor memory -> registers -> shared memory, transposed -> C
+// Two accumulators alternate, so that the epilogue of one tile overlaps the products of the next.
+//
+// What bounds it: reading the matrices while a run is a few columns (8 experts of 14336 x 4096 for 16 columns: 99 us, 1.2 of what reading those
+// in use takes at 6.55 TB/s), the tensor cores under the power limit where it is hundreds (8192 tokens twice: 1361 us, 1413 TFLOP/s).
 #include <cuda.h>
 
 #include <algorithm>
@@ -55,8 +59,7 @@ constexpr int kOutBytes = 8 * 2048;      // a box of 32 rows x 32 columns for ea
 // PAIR: two CTAs of a cluster on one tile, 128 rows and half of the columns' operand each
 template <int NT, bool PAIR>
 struct Cfg {
-  // K blocks of 64 in a stage: a pair's products are as short as half a tile's, and each wait, commit and turn of the loop takes the thread that
-  // issues them 370 cycles
+  // K blocks of 64 in a stage: a wait, a commit and a turn of the loop took the issuing thread 370 cycles, a pair's products of a block 512
   static constexpr int kSub = PAIR ? 2 : 1;
   static constexpr int kA = kHalfBytes, kX = NT * 128 / (PAIR ? 2 : 1), kXOff = kSub * kA, kStage = kSub * (kA + kX);
   static constexpr int kRoom = 226 * 1024 - kTableBytes - kOutBytes - 512;
@@ -285,6 +288,12 @@ template <bool PAIR>
 __device__ __forceinline__ uint32_t idesc_of(bool bf16, int n, bool a_mn, bool b_mn) {
   return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)((PAIR ? 256 : 128) >> 4) << 24);
+}
+// T is kept as two terms of 16 bits, together 16 (BFloat16) or 22 bits of it: one alone would be off by what the result is rounded by.  Nothing
+// is left of what is infinite: Inf - Inf would be a NaN.
+template <typename T>
+__device__ __forceinline__ T left_of(float v, T first) {
+  return Elem<T>::from_f(fabsf(Elem<T>::to_f(first)) < INFINITY ? v - Elem<T>::to_f(first) : 0.f);
 }
 __device__ __forceinline__ int round16(int n) { return (n + 15) & ~15; }
 // columns that a product of n takes (PAIR: half of them from each CTA)
@@ -811,7 +820,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
               if (j < nc) out[(long long)j * g.M] = scale * __uint_as_float(acc[j]);
           }
         } else if (m < g.low_step) {
-          // T: what is left after rounding to 16 bits is the second term; zeros behind the rank
+          // T; zeros behind the rank
           T* out = reinterpret_cast<T*>(g.C) + (long long)n * g.low_width + m;
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
@@ -819,7 +828,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
             const T first = Elem<T>::from_f(v);
             if (j < nc) {
               out[(long long)j * g.low_width] = first;
-              out[(long long)j * g.low_width + g.low_step] = Elem<T>::from_f(v - Elem<T>::to_f(first));
+              out[(long long)j * g.low_width + g.low_step] = left_of(v, first);
             }
           }
         }
@@ -1313,7 +1322,7 @@ __global__ void __launch_bounds__(256) join_low_kernel(const float* parts, int s
   }
   const T first = Elem<T>::from_f(v);
   out[(long long)n * width + c] = first;
-  out[(long long)n * width + step + c] = Elem<T>::from_f(v - Elem<T>::to_f(first));
+  out[(long long)n * width + step + c] = left_of(v, first);
 }
 
 // A matrix (or several) that is read: where it lies, contiguous extent first.

@@ -204,7 +204,8 @@ def _grouped(A, X, runs, dims=3):
 
 
 def grouped_mul_(Cm: torch.Tensor, A: torch.Tensor, X: torch.Tensor, runs: Union[torch.Tensor, Routing]) -> torch.Tensor:
-    """:func:`grouped_mul` into ``Cm``, ``(rows, columns)`` with adjacent rows; its columns in no run are left as they are."""
+    """:func:`grouped_mul` into ``Cm``, ``(rows, columns)`` with adjacent rows that shares no memory with
+    the arguments; its columns in no run are left as they are."""
     p, M, R = _grouped(A, X, runs)
     p.ldc = _matrix("C", Cm, X)
     if tuple(Cm.shape) != (M, R):

@@ -186,3 +186,21 @@ def test_refusals():
                 lambda: nb.adapter_mul(W, X, nb.jl_zeros((130, 16, 2), F32, DEV), nb.jl_zeros((8, 130, 2), F32, DEV), ids)):
         with pytest.raises(nb.ArgumentError):
             bad()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("N", [5, 700])
+def test_an_infinite_column_stays_infinite(dtype, N):
+    """Everything is positive, so that an infinity of X is one of its column's result, and no other's."""
+    M, K, r, n = 136, 72, 8, 2
+    W, A, B = (_cols(np.full(s, 0.125), dtype) for s in ((M, K), (r, K, n), (M, r, n)))
+    X = _cols(np.ones((K, N)), dtype)
+    X[40, 2] = float("inf")
+    for how in ({}, {"offsets": _ints([0, 3, N])}):
+        ids = _ints([0, 1] if how else [i % 2 for i in range(N)])
+        y, back = nb.adapter_mul_pullback(W, X, A, B, ids, **how)
+        assert torch.isinf(y[:, 2]).all() and torch.isfinite(y[:, :2]).all() and torch.isfinite(y[:, 3:]).all()
+        dY = _cols(np.full((M, N), 0.125), dtype)
+        dX, dA, dB = back(dY)
+        assert torch.isinf(dB[:, :, 0]).all() and torch.isfinite(dB[:, :, 1]).all() and torch.isfinite(dX).all()
