@@ -6,11 +6,11 @@
 //   grouped_grad_kernel    A_a = sum over the columns i of the runs of matrix a of C[:, i] X[:, columns[i]]^T
 //
 // 256 threads compute 128 rows x BN columns, k in steps of 16 or 32 through two shared-memory stages [k][row]: while one is multiplied the next
-// one's elements are on their way into registers, four neighbours at a time.  A thread owns 8 rows and BN / 16 columns, its products are
-// packed pairs of rows.  A block's slot number is turned into (run, first column) by counting the tiles of all runs, since their sizes
+// one's elements are on their way into registers, four neighbours at a time.  A thread multiplies 8 rows and 8 columns as packed pairs of
+// rows, in narrow tiles of every 128 / BN-th k.  A block's slot number is turned into (run, first column) by counting the tiles of all runs, since their sizes
 // are on the device only; slots that no run needs end at once.  Few tiles: K is cut and the parts are added by another launch (join_parts).
 // What bounds it: the FMA pipe and the shared memory that feeds it where columns are many (2048 x 2048, 4096 columns in 8 runs: 880 us,
-// 39 TFLOP/s; the gradient of the matrices 1074 us), reading A where they are few (6248 x 6680, 64 columns in 3 runs: 378 us, 1.3 TB/s).
+// 39 TFLOP/s; the gradient of the matrices 1086 us), reading A where they are few (6248 x 6680, 64 columns in 3 runs: 295 us, 1.7 TB/s).
 #include <algorithm>
 
 #include "common.cuh"
@@ -21,6 +21,7 @@
 namespace nb200 {
 namespace {
 
+using ptx::pair_add;
 using ptx::pair_fma;
 using ptx::pair_of;
 using ptx::pair_unpack;
@@ -51,8 +52,8 @@ struct Side {
   int limit;                                 // else, with a table: its entries below this are there
 };
 
-// k to a stage: narrow tiles are there to read A, 16 KB of it at a time
-__host__ __device__ constexpr int step_of(int bn) { return bn <= 32 ? 32 : 16; }
+// k to a stage: the narrowest tiles are there to read A, 16 KB of it at a time (of 32 columns: 309 us instead of 295, spilled)
+__host__ __device__ constexpr int step_of(int bn) { return bn <= 16 ? 32 : 16; }
 
 template <typename T, int W, int KS>
 struct Loader {
@@ -112,25 +113,25 @@ struct Loader {
   }
 };
 
-template <int BN>
-struct Stages {
-  static constexpr int kStep = step_of(BN);
-  float p[2][kStep][kRows + 4], q[2][kStep][BN + 4];
-};
-
-// a thread's part of a 128 x BN tile: rows row(j), columns column(i)
+// A thread's part of a 128 x BN tile: 8 rows row(j) and 8 columns, of every kParts-th k, so that a step's four 16-byte reads of shared memory feed 64
+// products whatever the tile is (with 8 x 2 of every k tiles of 32 columns took 378 us where these take 295: 6248 x 6680,
+// 64 columns in 3 runs).  join()
+// adds the parts, in their order; then the thread has all of k for kOwn columns, column(i).
 template <int BN>
 struct Tile {
-  static constexpr int R = BN / 16, G = R < 4 ? R : 4;
-  unsigned long long acc[R][4];              // pairs of rows
+  static constexpr int kParts = 128 / BN, kOwn = 8 / kParts, kLanes = 256 / kParts;
+  static constexpr int kJoin = kParts > 1 ? 4 * kOwn * (kParts - 1) * kLanes : 1;      // pairs of rows that join() has in shared memory
+  unsigned long long acc[8][4], own[kParts > 1 ? kOwn : 1][4];              // pairs of rows
+  static __device__ __forceinline__ int part() { return threadIdx.x / kLanes; }
+  static __device__ __forceinline__ int lane() { return threadIdx.x % kLanes; }
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < R; ++i)
+    for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = 0ull;
   }
   __device__ __forceinline__ void step(const float* p, const float* q) {
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int tx = lane() & 15, ty = lane() >> 4;
     unsigned long long a[4];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -138,30 +139,66 @@ struct Tile {
       a[2 * h] = v.x;
       a[2 * h + 1] = v.y;
     }
-    float b[R];
 #pragma unroll
-    for (int i = 0; i < R; i += G) {
-      if constexpr (G == 4) {
-        const float4 v = *reinterpret_cast<const float4*>(q + ty * 4 + i * 16);
-        b[i] = v.x; b[i + 1] = v.y; b[i + 2] = v.z; b[i + 3] = v.w;
-      } else {
+    for (int h = 0; h < 2; ++h) {
+      const float4 v = *reinterpret_cast<const float4*>(q + ty * 4 + h * (BN / 2));
+      const float b[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int u = 0; u < G; ++u) b[u] = q[ty * G + u];
+      for (int i = 0; i < 4; ++i) {
+        const unsigned long long bb = pair_of(b[i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[h * 4 + i][j] = pair_fma(a[j], bb, acc[h * 4 + i][j]);
       }
     }
+  }
+  // by the whole block, behind a barrier; leaves one behind itself
+  __device__ __forceinline__ void join(unsigned long long* room) {
+    if constexpr (kParts > 1) {
+      const int me = part(), t = lane();
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const unsigned long long bb = pair_of(b[i]);
+      for (int d = 0; d < kParts; ++d) {
+        if (me != d) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = pair_fma(a[j], bb, acc[i][j]);
+          for (int i = 0; i < kOwn; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) room[((i * 4 + j) * (kParts - 1) + me - (me > d ? 1 : 0)) * kLanes + t] = acc[d * kOwn + i][j];
+        }
+        __syncthreads();
+        if (me == d) {
+#pragma unroll
+          for (int i = 0; i < kOwn; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              unsigned long long v = acc[d * kOwn + i][j];
+#pragma unroll
+              for (int q = 0; q + 1 < kParts; ++q) v = pair_add(v, room[((i * 4 + j) * (kParts - 1) + q) * kLanes + t]);
+              own[i][j] = v;
+            }
+        }
+        __syncthreads();
+      }
     }
   }
   __device__ __forceinline__ void values(int i, float (&v)[8]) const {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) pair_unpack(acc[i][j], v[2 * j], v[2 * j + 1]);
+    for (int j = 0; j < 4; ++j) pair_unpack(kParts > 1 ? own[kParts > 1 ? i : 0][j] : acc[i][j], v[2 * j], v[2 * j + 1]);
   }
-  static __device__ __forceinline__ int row(int j) { return (threadIdx.x & 15) * 4 + (j >> 2) * 64 + (j & 3); }
-  static __device__ __forceinline__ int column(int i) { return (threadIdx.x >> 4) * G + (i / G) * 16 * G + i % G; }
+  static __device__ __forceinline__ int row(int j) { return (lane() & 15) * 4 + (j >> 2) * 64 + (j & 3); }
+  static __device__ __forceinline__ int column(int i) {
+    const int c = part() * kOwn + i;
+    return (lane() >> 4) * 4 + (c >> 2) * (BN / 2) + (c & 3);
+  }
+};
+
+template <int BN>
+struct Stages {
+  static constexpr int kStep = step_of(BN);
+  float p[2][kStep][kRows + 4], q[2][kStep][BN + 4];
+};
+template <int BN>
+union alignas(16) Shared {
+  Stages<BN> stages;
+  unsigned long long joined[Tile<BN>::kJoin];
 };
 
 // One contraction over k0 .. K - 1 (k0 a multiple of 4)
@@ -186,9 +223,9 @@ __device__ __forceinline__ void contract(Tile<BN>& t, Stages<BN>& s, int k0, int
     const int kn = min(kStep, K - k0);       // the padding is not multiplied: 0 * Inf would be a NaN
     if (kn == kStep) {
 #pragma unroll
-      for (int k = 0; k < kStep; ++k) t.step(s.p[b][k], s.q[b][k]);
+      for (int k = 0; k < kStep; k += Tile<BN>::kParts) t.step(s.p[b][k + Tile<BN>::part()], s.q[b][k + Tile<BN>::part()]);
     } else {
-      for (int k = 0; k < kn; ++k) t.step(s.p[b][k], s.q[b][k]);
+      for (int k = Tile<BN>::part(); k < kn; k += Tile<BN>::kParts) t.step(s.p[b][k], s.q[b][k]);
     }
     if (more) {
       p.stage(s.p[b ^ 1]);
@@ -205,8 +242,9 @@ __host__ __device__ __forceinline__ bool fours(const T* p, long long a, long lon
 
 // blockIdx: (slot of columns, tile of rows, part of K).  parts: Float32 (M, R, parts) instead of C
 template <typename T, typename TC, int BN>
-__global__ void __launch_bounds__(256) grouped_fma_kernel(const __grid_constant__ GroupedArgs g, float* parts) {
-  __shared__ __align__(16) Stages<BN> st;
+__global__ void __launch_bounds__(256, BN == 128 ? 1 : 2) grouped_fma_kernel(const __grid_constant__ GroupedArgs g, float* parts) {
+  __shared__ Shared<BN> shared;
+  Stages<BN>& st = shared.stages;
   __shared__ RunSearch search;
   __shared__ int cols[BN];
   const RunTile run = find_run(Runs{g.offsets, g.run_len, g.G, g.R}, g.zero_rest && !parts, BN, blockIdx.x, search);
@@ -233,10 +271,11 @@ __global__ void __launch_bounds__(256) grouped_fma_kernel(const __grid_constant_
     contract<BN>(t, st, k0, min(g.K, k0 + each), Side<T>{A, g.lda, g.transA != 0, fours(A, g.lda, 0), rows, nullptr, 0},
                  Side<T>{X, g.ldx, true, fours(X, g.ldx, 0), BN, cols, 0});
   }
+  t.join(shared.joined);
   const float scale = !have ? 0.f : (g.scale ? g.scale[mat] : g.scale0);
-  float c[Tile<BN>::R][8];
+  float c[Tile<BN>::kOwn][8];
 #pragma unroll
-  for (int i = 0; i < Tile<BN>::R; ++i) {
+  for (int i = 0; i < Tile<BN>::kOwn; ++i) {
     t.values(i, c[i]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) c[i][j] *= scale;
@@ -256,8 +295,9 @@ __global__ void __launch_bounds__(256) grouped_fma_kernel(const __grid_constant_
       t.clear();
       contract<BN>(t, st, 0, g.low.r, Side<T>{B, g.low.ldb, g.low.transB != 0, fours(B, g.low.ldb, 0), rows, nullptr, 0},
                    Side<float>{low, g.low.ldt, true, fours(low, g.low.ldt, 0), BN, mine, 0});
+      t.join(shared.joined);
 #pragma unroll
-      for (int i = 0; i < Tile<BN>::R; ++i) {
+      for (int i = 0; i < Tile<BN>::kOwn; ++i) {
         const int n = n0 + Tile<BN>::column(i);
         if (n < lo || n >= hi) continue;     // (0 * Inf of another pair's matrix)
         float v[8];
@@ -268,7 +308,7 @@ __global__ void __launch_bounds__(256) grouped_fma_kernel(const __grid_constant_
     }
   }
 #pragma unroll
-  for (int i = 0; i < Tile<BN>::R; ++i) {
+  for (int i = 0; i < Tile<BN>::kOwn; ++i) {
     const int n = Tile<BN>::column(i);
     if (n >= nn) continue;
     const bool zero = cols[n] < 0;           // (a padding column's 0 times an infinity of A)
@@ -414,10 +454,11 @@ __global__ void __launch_bounds__(256, TURNED ? 2 : 3) grouped_narrow_kernel(con
 }
 
 // blockIdx: (tile of A's shorter way, tile of its contiguous one, matrix).  The tile's rows are those along which A is contiguous, so that it is
-// stored in long pieces: C's rows, or, turned, X's.  (64 columns in 3 runs, 6248 x 6680, turned: 291 us, 558 us with C's rows)
+// stored in long pieces: C's rows, or, turned, X's.  (64 columns in 3 runs, 6248 x 6680, turned: 258 us; 558 us with C's rows, in tiles of 128 columns)
 template <typename TP, typename TQ, typename TA, int BN>
-__global__ void __launch_bounds__(256) grouped_grad_kernel(const __grid_constant__ GroupedGradArgs g) {
-  __shared__ __align__(16) Stages<BN> st;
+__global__ void __launch_bounds__(256, BN == 128 ? 1 : 2) grouped_grad_kernel(const __grid_constant__ GroupedGradArgs g) {
+  __shared__ Shared<BN> shared;
+  Stages<BN>& st = shared.stages;
   const bool turned = g.transA != 0;
   const int P = turned ? g.K : g.M, Q = turned ? g.M : g.K;
   const int q0 = blockIdx.x * BN, p0 = blockIdx.y * kRows, a = blockIdx.z, rows = min(kRows, P - p0), cols = min(BN, Q - q0);
@@ -435,10 +476,11 @@ __global__ void __launch_bounds__(256) grouped_grad_kernel(const __grid_constant
     const TQ* q = reinterpret_cast<const TQ*>(q_base) + (q_table ? 0 : (long long)lo * ldq) + q0;
     contract<BN>(t, st, 0, n, Side<TP>{p, ldp, false, fours(p, ldp, 0), rows, p_table, g.N}, Side<TQ>{q, ldq, false, fours(q, ldq, 0), cols, q_table, g.N});
   }
+  t.join(shared.joined);
   TA* A = reinterpret_cast<TA*>(g.A) + (long long)a * g.strideA + p0;
   const bool vec = fours(A, g.lda, 0);
 #pragma unroll
-  for (int i = 0; i < Tile<BN>::R; ++i) {
+  for (int i = 0; i < Tile<BN>::kOwn; ++i) {
     const int c = Tile<BN>::column(i);
     if (c >= cols) continue;
     float v[8];
@@ -462,7 +504,7 @@ struct FmaShape {
   int bn, splits;
 };
 // As many columns to a tile as the average run has, fewer where that leaves SMs without a tile (333 x 200 by 1200 columns in 5 runs: 36 us
-// in tiles of 128 columns, 20 us of 32), and K cut into parts of at least 128 while tiles are fewer than two to an SM and the parts are few.
+// in tiles of 128 columns, 19 us of 32), and K cut into parts of at least 128 while tiles are fewer than two to an SM and the parts are few.
 FmaShape fma_shape(const GroupedArgs& g) {
   const long long each = std::max<long long>(1, g.R / std::max(1, g.G)), rows = (g.M + kRows - 1) / kRows;
   FmaShape s;
@@ -503,7 +545,10 @@ cudaError_t launch_grad_tiles(const GroupedGradArgs& g, cudaStream_t st) {
   const long long P = g.transA ? g.K : g.M, Q = g.transA ? g.M : g.K, rows = (P + kRows - 1) / kRows;
   if (rows > 65535 || g.mats > 65535) return cudaErrorInvalidConfiguration;
   auto blocks = [&](long long bn) { return ((Q + bn - 1) / bn) * rows * g.mats; };
-  const int bn = Q > 64 && blocks(128) >= 148 ? 128 : Q > 32 && blocks(64) >= 148 ? 64 : Q > 16 ? 32 : 16;
+  // short runs: a block's time is the loads of its first columns and its results, so that two to an SM are better than one of twice the tile
+  // (8 matrices of 1024 x 1024, 64 columns each: 40 us in tiles of 64, 47 of 128; 100 each: 56 and 67)
+  const bool brief = g.R / std::max(1, g.mats) < 128;
+  const int bn = Q > 64 && blocks(128) >= 148 && !brief ? 128 : Q > 32 && blocks(64) >= 148 ? 64 : Q > 16 ? 32 : 16;
   const dim3 grid((unsigned)((Q + bn - 1) / bn), (unsigned)rows, (unsigned)g.mats);
   switch (bn) {
     case 128: grouped_grad_kernel<TP, TQ, TA, 128><<<grid, 256, 0, st>>>(g); break;
