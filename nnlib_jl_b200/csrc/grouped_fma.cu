@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(256, BN == 128 ? 1 : 2) grouped_fma_kernel(con
 
 // Runs of a few columns: nothing of A is read twice, so none of it goes through shared memory.  128 rows and up to kNarrow columns to a block.
 // Rows contiguous: a lane has four rows, every eighth k is a warp's; k contiguous: a warp has 16 rows, a lane every 32nd four of k.
-// (two columns to each of 128 matrices of 1536 x 2048: 430 us, 3.7 TB/s, turned; 522 us not; in tiles of 16 columns 1148 us)
+// (two columns to each of 128 matrices of 1536 x 2048: 427 us, 3.8 TB/s, turned; 512 us not; in tiles of 16 columns 1148 us)
 constexpr int kNarrow = 4, kChunk = 1024;
 template <typename T, typename TC, bool TURNED>
 __global__ void __launch_bounds__(256, TURNED ? 2 : 3) grouped_narrow_kernel(const __grid_constant__ GroupedArgs g, float* parts) {
@@ -504,16 +504,23 @@ struct FmaShape {
   int bn, splits;
 };
 // As many columns to a tile as the average run has, fewer where that leaves SMs without a tile (333 x 200 by 1200 columns in 5 runs: 36 us
-// in tiles of 128 columns, 19 us of 32), and K cut into parts of at least 128 while tiles are fewer than two to an SM and the parts are few.
+// in tiles of 128 columns, 19 us of 32), and K cut into parts of at least 128, while these are few, where full waves of blocks gain a tenth by it: a block costs its k and
+// some 96 more, the launch that adds the parts about 50 k (6680 x 6248 by 64 columns in 3 runs, 159 blocks: 432 us in 2 parts, 309 in more).
 FmaShape fma_shape(const GroupedArgs& g) {
   const long long each = std::max<long long>(1, g.R / std::max(1, g.G)), rows = (g.M + kRows - 1) / kRows;
   FmaShape s;
   s.bn = each > 64 ? 128 : each > 32 ? 64 : each > 16 ? 32 : each > kNarrow ? 16 : kNarrow;
   auto tiles = [&] { return ((each + s.bn - 1) / s.bn) * std::min(g.G, g.R) * rows; };
   auto cut = [&] {
-    int splits = 1;
-    while (splits < 32 && tiles() * splits < 296 && g.K / (2 * splits) >= 128 && (g.R <= 512 || 8ll * splits * g.R * g.M <= (16ll << 20))) splits *= 2;
-    return splits;
+    const long long slots = s.bn == 128 ? 148 : 296;
+    long long least = 0;
+    int best = 1;
+    for (int n = 1; n <= 32 && (n == 1 || g.K / n >= 128); n *= 2) {
+      if (n > 1 && g.R > 512 && 8ll * n * g.R * g.M > (16ll << 20)) break;
+      const long long cost = ((tiles() * n + slots - 1) / slots) * (g.K / n + 96) + (n > 1 ? 40 + 8 * n : 0);
+      if (n == 1 || 10 * cost < 9 * least) { least = cost; best = n; }
+    }
+    return best;
   };
   while (s.bn > 32 && tiles() * cut() < 148) s.bn /= 2;
   s.splits = cut();
