@@ -467,8 +467,21 @@ __global__ void __launch_bounds__(256, BN == 128 ? 1 : 2) grouped_grad_kernel(co
   const Runs of{g.offsets, g.run_len, g.G, g.R};
   Tile<BN> t;
   t.clear();
-  for (int b = g.ids ? 0 : a; b < (g.ids ? g.G : min(a + 1, g.G)); ++b) {
-    if (g.ids && g.ids[b] != a) continue;
+  // the runs of matrix a: a warp looks at 32 at a time, and every warp finds the same
+  int b = g.ids ? -1 : a - 1, at = -32;
+  unsigned found = 0u;
+  while (true) {
+    if (!g.ids) {
+      if (++b > a || b >= g.G) break;
+    } else {
+      while (found == 0u && (at += 32) < g.G) {
+        const int i = at + (int)(threadIdx.x & 31);
+        found = __ballot_sync(0xffffffffu, i < g.G && g.ids[i] == a);
+      }
+      if (found == 0u) break;
+      b = at + __ffs(found) - 1;
+      found &= found - 1u;
+    }
     const int lo = of.begin(b), n = of.end(b) - lo;
     const int* table = g.columns ? g.columns + lo : nullptr;
     const int *p_table = turned ? table : nullptr, *q_table = turned ? nullptr : table;
