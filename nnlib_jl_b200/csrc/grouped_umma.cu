@@ -501,10 +501,22 @@ __device__ __forceinline__ void put_fragments(uint32_t (&f)[2][16], uint8_t* box
   for (int i = 0; i < 4; ++i, out += 8 * ld) {
     if (i * 8 + c >= wide) continue;
     const uint4 v = *reinterpret_cast<const uint4*>(from + i * 512);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     if (whole) {
       *reinterpret_cast<uint4*>(out) = v;
+    } else if (m + r + 8 <= rows) {
+      // columns that begin at no multiple of 16 bytes: words, where a column of odd length begins between two of them put together anew
+      // (dA of 10 matrices of 12343 x 2728: 1623 us element by element, 528 so)
+      if (reinterpret_cast<uintptr_t>(out) & 2) {
+        reinterpret_cast<unsigned short*>(out)[0] = (unsigned short)w[0];
+#pragma unroll
+        for (int e = 0; e < 3; ++e) *reinterpret_cast<uint32_t*>(reinterpret_cast<unsigned short*>(out) + 1 + 2 * e) = __funnelshift_r(w[e], w[e + 1], 16);
+        reinterpret_cast<unsigned short*>(out)[7] = (unsigned short)(w[3] >> 16);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) reinterpret_cast<uint32_t*>(out)[e] = w[e];
+      }
     } else {
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (m + r + e < rows) reinterpret_cast<unsigned short*>(out)[e] = (unsigned short)(w[e >> 1] >> (e & 1 ? 16 : 0));
