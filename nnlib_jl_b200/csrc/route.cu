@@ -6,9 +6,11 @@
 // lanes hold neighbouring experts).  A block counts its tokens' choices; a second launch turns the counts of all blocks into each
 // block's first number for each expert; a third gives every pair its number: a token picks an expert at most once, so the
 // pair's place among its block's is the number of earlier tokens in the expert's bit mask.  Nothing depends on the order in
-// which warps run.  Few tokens take one block and one launch.
+// which warps run.  Few tokens take one block and one launch.  What bounds it is instructions, 547 a token of 256 experts and 8 choices (32768 such
+// tokens, bf16: 26 + 8 + 10 us).
 //
-// combine: HBM bound, 16 bytes a thread and column.
+// combine: HBM bound, 16 bytes a thread and column (8192 tokens of 2 columns of 4096, bf16: 42 us, 4.7 TB/s; the pullback of 4096 tokens of 6
+// columns of 2048: 40 us, 5.4 TB/s).
 #include <algorithm>
 #include <climits>
 #include <type_traits>
