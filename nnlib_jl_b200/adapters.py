@@ -15,7 +15,7 @@ import torch
 from . import _lib
 from .attention import _DTYPES, ArgumentError, _status_word
 from .experts import _columns, _factor, _matrix, _run, _vector
-from .layout import is_column_major, jl_reshape
+from .layout import is_column_major
 
 __all__ = ["adapter_mul", "adapter_mul_pullback"]
 
@@ -25,10 +25,10 @@ _blank = bytes(_lib.AdapterParams())
 def _flat(name: str, X, like=None):
     """A (features, columns) view of X and the columns of a request, or None where X has but columns."""
     if isinstance(X, torch.Tensor) and X.ndim == 3:
-        if not is_column_major(X):
+        if X.numel() and not is_column_major(X):
             raise TypeError(f"{name}: a 3-d array must be dense and column-major (strides {X.stride()} for size {tuple(X.shape)})")
         L = X.shape[1]
-        X = jl_reshape(X, (X.shape[0], X.shape[1] * X.shape[2]))
+        X = X.as_strided((X.shape[0], L * X.shape[2]), (1, X.shape[0] or 1))
         _matrix(name, X, like)
         return X, L
     _matrix(name, X, like)

@@ -255,7 +255,7 @@ cudaError_t adapter_products(Adapters& a, int dtype, bool umma, bool keep, void*
   a.first.ldc = a.first.M;
   a.main.low.T = low;
   a.main.low.ldt = a.first.M;
-  if (has_pairs(a)) {
+  if (a.first.G > 0 && a.first.mats > 0) {             // (without features too: the gradients read it, as zeros)
     const cudaError_t e = fma_product(a.first, dtype, true, ws, st);
     if (e != cudaSuccess) return e;
   }
@@ -397,8 +397,9 @@ size_t nnlib_b200_adapter_bwd_workspace_bytes(const nnlib_b200_adapter_params* p
   if (resolve_adapter(p, true, &a)) return 0;
   const bool umma = adapter_on_umma(a, p->dtype);
   size_t rest = adapter_ws(a, umma, true);
-  if (!umma && p->dA) rest = std::max(rest, fma_ws(pair_grads(p, a, false).first));
-  if (umma && p->dA) {
+  const bool pairs = p->dA || p->dB;                       // (of no elements: NULL)
+  if (!umma && pairs) rest = std::max(rest, fma_ws(pair_grads(p, a, false).first));
+  if (umma && pairs) {
     const PairGrads g = pair_grads(p, a, true);
     rest = std::max({rest, low_umma_workspace_bytes(g.first), grouped_umma_grad_workspace_bytes(g.a, 1), grouped_umma_grad_workspace_bytes(g.b, 2)});
   }
@@ -418,7 +419,7 @@ int nnlib_b200_adapter_bwd(const nnlib_b200_adapter_params* p, void* workspace, 
   char* of_X = of_dC + low;                                // scale * A X
   char* ws = of_X + low;
   if ((rc = finish(adapter_products(a, p->dtype, umma, true, of_dC, ws, st)))) return rc;
-  if (!p->dA || !p->dB || a.first.mats == 0) return NNLIB_B200_OK;
+  if ((!p->dA && !p->dB) || a.first.mats == 0) return NNLIB_B200_OK;
   PairGrads g = pair_grads(p, a, umma);
   g.first.C = of_X;
   g.a.C = of_dC;

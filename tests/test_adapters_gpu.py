@@ -204,3 +204,18 @@ def test_an_infinite_column_stays_infinite(dtype, N):
         dY = _cols(np.full((M, N), 0.125), dtype)
         dX, dA, dB = back(dY)
         assert torch.isinf(dB[:, :, 0]).all() and torch.isfinite(dB[:, :, 1]).all() and torch.isfinite(dX).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_empty_arrays(dtype):
+    for M, K, n, N in ((0, 8, 2, 5), (8, 0, 2, 5), (8, 8, 0, 5), (8, 8, 2, 0), (0, 0, 0, 0)):
+        W, A, B, X = (nb.jl_zeros(s, dtype, DEV) for s in ((M, K), (4, K, n), (M, 4, n), (K, N)))
+        y, back = nb.adapter_mul_pullback(W, X, A, B, torch.zeros(N, dtype=torch.int32, device=DEV))
+        assert tuple(y.shape) == (M, N) and (y == 0).all()
+        for t, s in zip(back(nb.jl_zeros((M, N), dtype, DEV)), ((K, N), (4, K, n), (M, 4, n))):
+            assert tuple(t.shape) == s and (t == 0).all()
+    W, A, B = (nb.jl_zeros(s, dtype, DEV) for s in ((8, 8), (4, 8, 2), (8, 4, 2)))
+    for L, R in ((0, 3), (3, 0)):
+        y, back = nb.adapter_mul_pullback(W, torch.zeros(R, L, 8, dtype=dtype, device=DEV).permute(2, 1, 0), A, B, torch.zeros(R, dtype=torch.int32, device=DEV))
+        assert tuple(y.shape) == (8, L, R) and [tuple(t.shape) for t in back(y)] == [(8, L, R), (4, 8, 2), (8, 4, 2)]
