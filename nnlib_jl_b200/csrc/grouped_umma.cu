@@ -877,6 +877,8 @@ struct GradArgs {
   int tiles_r, tiles_c, vec;
   int wait;                              // launched early
   int fold, fold_step, along;            // fold: columns fold_step apart are the two terms of one; along: a row's columns are contiguous
+  float* parts;                          // fold, in parts of the columns: (rows, cols, mats, splits) instead of A
+  int splits;
   int* status;
 };
 
@@ -909,14 +911,15 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
   tc_fence_after();
   const uint32_t tmem = __reduce_or_sync(0xffffffffu, bars->tmem_base);     // (in a uniform register)
   const bool start_ok = (*abort_flag == 0);
-  const long long each = (long long)g.tiles_r * g.tiles_c, tiles = each * g.mats;
+  const long long each = (long long)g.tiles_r * g.tiles_c * g.splits, tiles = each * g.mats;
   auto begin_of = [&](int b) { return held ? tab.begin[b] : g.runs.begin(b); };
   auto end_of = [&](int b) { return held ? tab.end[b] : g.runs.end(b); };
   // The runs of matrix a that have columns, one after the other, -1: no more.  A warp looks at 32 at a time (64 runs of 64 pairs, 4096 x 16: one
-  // at a time each tile took 17000 cycles to find its own, 121 us for what takes 29 so).
+  // at a time each tile took 17000 cycles to find its own, 121 us for what takes 35 so).
   struct Walk {
     int at = -32;
     unsigned found = 0u;
+    int pos = 0, lo = 0, hi = 0x7fffffff;                  // blocks of columns gone by, and those that are wanted
   };
   auto next_run = [&](Walk& w, int a) {
     if (!g.ids) {
@@ -933,6 +936,35 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
     w.found &= w.found - 1u;
     return b;
   };
+  // part `split` of the blocks of matrix a
+  auto walk_of = [&](int a, int split) {
+    Walk w;
+    if (g.splits > 1) {
+      Walk all;
+      int n = 0;
+      for (int b = next_run(all, a); b >= 0; b = next_run(all, a)) n += (end_of(b) - begin_of(b) + kBlock - 1) / kBlock;
+      w.lo = (int)((long long)n * split / g.splits);
+      w.hi = (int)((long long)n * (split + 1) / g.splits);
+    }
+    return w;
+  };
+  // the next columns of a run that are wanted: false: no more
+  auto next_piece = [&](Walk& w, int a, int& begin, int& end) {
+    while (w.pos < w.hi) {
+      const int b = next_run(w, a);
+      if (b < 0) return false;
+      begin = begin_of(b);
+      end = end_of(b);
+      if (g.splits == 1) return true;
+      const int n = (end - begin + kBlock - 1) / kBlock, first = max(0, w.lo - w.pos), last = min(n, w.hi - w.pos);
+      w.pos += n;
+      if (first >= last) continue;
+      if (last < n) end = begin + last * kBlock;
+      begin += first * kBlock;
+      return true;
+    }
+    return false;
+  };
 
   if (start_ok && (warp == 0 || warp >= 10)) {
     const int me = warp == 0 ? 0 : warp - 9;
@@ -945,13 +977,13 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
     Ring<C::kStages> at;
     int turn = 0;
     for (long long t = worker; t < tiles && ok; t += workers) {
-      const int a = (int)(t / each), q = (int)(t % each);
+      const int a = (int)(t / each), in = (int)(t - a * each), q = g.splits > 1 ? in / g.splits : in, split = in - q * g.splits;
       const int r0 = (q % g.tiles_r) * (PAIR ? 256 : 128) + rank * 128, left = g.cols - (q / g.tiles_r) * NT;
       const int c0 = (q / g.tiles_r) * NT + (PAIR ? rank * (product_columns<true>(min(NT, left)) / 2) : 0);
-      Walk walk;
-      for (int b = next_run(walk, a); b >= 0 && ok; b = next_run(walk, a)) {
-        const int end = end_of(b);
-        for (int i0 = begin_of(b); i0 < end; i0 += kBlock, at.next()) {
+      Walk walk = walk_of(a, split);
+      int begin, end;
+      while (ok && next_piece(walk, a, begin, end)) {
+        for (int i0 = begin; i0 < end; i0 += kBlock, at.next()) {
           const bool mine = turn == me;
           if (++turn == kProducers) turn = 0;
           if (!mine) continue;
@@ -1002,7 +1034,7 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
     const bool issues = !PAIR || rank == 0;
     uint32_t sides = 0u;                                   // phases of the barriers `side`
     for (long long t = worker; t < tiles && ok; t += workers, ++ti) {
-      const int a = (int)(t / each), left = g.cols - (int)((t % each) / g.tiles_r) * NT;
+      const int a = (int)(t / each), in = (int)(t - a * each), q = g.splits > 1 ? in / g.splits : in, split = in - q * g.splits, left = g.cols - q / g.tiles_r * NT;
       const int ab = ti & 1;
       const uint32_t acc = tmem + ab * NT;
       const uint32_t idesc = idesc_of<PAIR>(BF16, g.fold ? NT : product_columns<PAIR>(min(NT, left)), true, true);
@@ -1010,10 +1042,9 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
       if (!ok) break;
       tc_fence_after();
       bool begun = false;
-      Walk walk;
-      for (int b = next_run(walk, a); b >= 0 && ok; b = next_run(walk, a)) {
-        const int end = end_of(b);
-        const int begin = begin_of(b);
+      Walk walk = walk_of(a, split);
+      int begin, end;
+      while (ok && next_piece(walk, a, begin, end)) {
         // a block of which the first `here` columns are the run's
         auto multiply = [&](int here) {
           tc_fence_after();
@@ -1041,8 +1072,8 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
           ok = issues ? warp_wait(&bars->full[at.s], (uint32_t)at.round & 1u, abort_flag) : warp_wait(&bars->side[at.s], (sides >> at.s) & 1u, abort_flag);
           if (!ok) break;
           if (side) {
-            const int u = rest / kBK, in = rest % kBK;     // (a part of 16: in one block)
-            for (int i = in * 8 + lane; i < round16(in) * 8; i += 32) {
+            const int u = rest / kBK, there = rest % kBK;  // (a part of 16: in one block)
+            for (int i = there * 8 + lane; i < round16(there) * 8; i += 32) {
 #pragma unroll
               for (int x = 0; x < 2; ++x) *reinterpret_cast<uint4*>(smem + at.s * C::kStage + u * C::kA + x * (kHalfBytes / 2) + i * 16) = make_uint4(0, 0, 0, 0);
 #pragma unroll
@@ -1068,11 +1099,12 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
     int ti = 0;
     uint8_t* box = smem + C::kOutOff + (warp - 2) * 2048;
     for (long long t = worker; t < tiles && ok; t += workers, ++ti) {
-      const int a = (int)(t / each), q = (int)(t % each);
+      const int a = (int)(t / each), in = (int)(t - a * each), q = g.splits > 1 ? in / g.splits : in, split = in - q * g.splits;
       const int r0 = (q % g.tiles_r) * (PAIR ? 256 : 128) + rank * 128, c0 = (q / g.tiles_r) * NT;
       const int ab = ti & 1;
-      Walk walk;
-      const bool some = next_run(walk, a) >= 0;            // a matrix that no column met is zeros
+      Walk walk = walk_of(a, split);
+      int begin, end;
+      const bool some = next_piece(walk, a, begin, end);   // a matrix that no column met is zeros
       ok = mbar_wait_warp(&bars->acc_full[ab], (uint32_t)(ti >> 1) & 1u, abort_flag);
       if (!ok) break;
       tc_fence_after();
@@ -1090,7 +1122,7 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
       // (46 pairs of rank 128 and 5984 rows, stored along the rank: 468 us with stores of an element, 213 so)
       for (int c = part; c < chunks; c += 2) {
         const int n = c0 + c * 32;
-        if (!g.along) {
+        if (!g.along && !g.parts) {
           uint32_t f[2][16], more[2][16];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -1110,6 +1142,16 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
         tmem_ld32(taddr + g.fold_step + c * 32, more);
         tmem_wait_ld();
         const int nc = min(32, g.cols - n);
+        if (g.parts) {
+          float* out = g.parts + (((long long)split * g.mats + a) * g.cols + n) * g.rows + m;
+          if (m < g.rows) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < nc) out[(long long)j * g.rows] = some ? __uint_as_float(acc[j]) + __uint_as_float(more[j]) : 0.f;
+          }
+          __syncwarp();
+          continue;
+        }
         if (m < g.rows) {
           T* dst = base + (long long)m * g.ld + n;
 #pragma unroll
@@ -1134,6 +1176,41 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
     }
   }
   tear_down<NT, PAIR>(bars, tmem, g.status);
+}
+
+// The parts of such a gradient, added in their order.  A block takes 32 rows of a matrix and 32 columns at a time, turned in shared memory where a row's
+// columns are contiguous.
+struct JoinGradArgs {
+  const float* parts;
+  void* A;
+  long long ld, stride;
+  int rows, cols, mats, splits, along;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) join_grad_kernel(const __grid_constant__ JoinGradArgs g) {
+  __shared__ float tile[32][33];
+  let_next();
+  wait_before();
+  const int m0 = blockIdx.x * 32, a = blockIdx.y, x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  T* A = reinterpret_cast<T*>(g.A) + (long long)a * g.stride;
+  for (int n0 = 0; n0 < g.cols; n0 += 32) {
+    __syncthreads();
+#pragma unroll
+    for (int i = y; i < 32; i += 8) {
+      float v = 0.f;
+      if (n0 + i < g.cols && m0 + x < g.rows) {
+#pragma unroll 4
+        for (int s = 0; s < g.splits; ++s) v += g.parts[(((long long)s * g.mats + a) * g.cols + n0 + i) * g.rows + m0 + x];
+        if (!g.along) A[(long long)(n0 + i) * g.ld + m0 + x] = Elem<T>::from_f(v);
+      }
+      if (g.along) tile[i][x] = v;
+    }
+    if (!g.along) continue;
+    __syncthreads();
+#pragma unroll
+    for (int i = y; i < 32; i += 8)
+      if (m0 + i < g.rows && n0 + x < g.cols) A[(long long)(m0 + i) * g.ld + n0 + x] = Elem<T>::from_f(tile[x][i]);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------- copies, host
@@ -1511,7 +1588,7 @@ template <bool BF16, int NT, bool PAIR>
 cudaError_t launch_bwd(const CUtensorMap& r, const CUtensorMap& c, GradArgs g, cudaStream_t st) {
   g.tiles_r = (g.rows + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128);
   g.tiles_c = g.fold ? 1 : (g.cols + NT - 1) / NT;
-  return launch<PAIR>(grouped_grad_umma_kernel<BF16, NT, PAIR>, (long long)g.tiles_r * g.tiles_c * g.mats, Cfg<NT, PAIR>::kSmem, g.wait != 0, st, r, c, g);
+  return launch<PAIR>(grouped_grad_umma_kernel<BF16, NT, PAIR>, (long long)g.tiles_r * g.tiles_c * g.splits * g.mats, Cfg<NT, PAIR>::kSmem, g.wait != 0, st, r, c, g);
 }
 
 // Rows and columns of a tile.
@@ -1771,9 +1848,19 @@ cudaError_t adapter_umma(const GroupedArgs& first, GroupedArgs m, int dtype, boo
   return e == cudaSuccess ? join_parts(m, dtype, s.splits, reinterpret_cast<const float*>(parts), reinterpret_cast<const float*>(of_first), f.splits, st) : e;
 }
 
+// Parts of the columns that a pair's gradient is cut into: as many as there are SMs for, where that takes away 48 of a tile's blocks or more: the launch that
+// adds them is some 5 us (one pair, 4096 x 16, 32768 columns: 50 us in four parts, 112 in one; 2048 columns in two parts: 4 us more than in one).
+static int grad_splits(const GroupedGradArgs& g, int fold) {
+  if (!fold) return 1;
+  const long long tiles = (long long)(((fold == 1 ? g.K : g.M) + 127) / 128) * g.mats, blocks = g.R / 64 / g.mats;
+  const long long splits = std::max<long long>(1, std::min({148 / tiles, blocks / 8, 16ll}));
+  return blocks - blocks / splits < 48 ? 1 : (int)splits;
+}
 size_t grouped_umma_grad_workspace_bytes(const GroupedGradArgs& g, int fold) {
   const Operand c = columns_of(g.C, g.M, g.R, g.ldc, nullptr, 0), x = columns_of(g.X, g.K, g.N, g.ldx, g.columns, g.R);
-  return (fold == 1 ? 0 : padded(c.copy_bytes())) + (fold == 2 ? 0 : padded(x.copy_bytes()));
+  const int splits = grad_splits(g, fold);
+  return (fold == 1 ? 0 : padded(c.copy_bytes())) + (fold == 2 ? 0 : padded(x.copy_bytes())) +
+         (splits > 1 ? padded(sizeof(float) * splits * (size_t)g.mats * g.M * g.K) : 0);
 }
 bool grouped_umma_grad_supports(const GroupedGradArgs& g, int dtype) {
   return (dtype == NNLIB_B200_F16 || dtype == NNLIB_B200_BF16) && g.M > 0 && g.K > 0 && g.N > 0 && g.R > 0 && g.mats > 0 && encode_tiled_fn() != nullptr;
@@ -1810,10 +1897,24 @@ cudaError_t grouped_umma_grad(const GroupedGradArgs& g, int dtype, int fold, voi
   const CUtensorMap& r = x_rows ? mx : mc;
   const CUtensorMap& q = x_rows ? mc : mx;
   const bool bf16 = dtype == NNLIB_B200_BF16;
-  if (pair) return bf16 ? launch_bwd<true, 256, true>(r, q, a, st) : launch_bwd<false, 256, true>(r, q, a, st);
-  if (nt == 256) return bf16 ? launch_bwd<true, 256, false>(r, q, a, st) : launch_bwd<false, 256, false>(r, q, a, st);
-  if (nt == 128) return bf16 ? launch_bwd<true, 128, false>(r, q, a, st) : launch_bwd<false, 128, false>(r, q, a, st);
-  return bf16 ? launch_bwd<true, 64, false>(r, q, a, st) : launch_bwd<false, 64, false>(r, q, a, st);
+  a.splits = grad_splits(g, fold);
+  if (a.splits > 1) a.parts = reinterpret_cast<float*>(ws);       // (behind the copies)
+  auto run = [&] {
+    if (pair) return bf16 ? launch_bwd<true, 256, true>(r, q, a, st) : launch_bwd<false, 256, true>(r, q, a, st);
+    if (nt == 256) return bf16 ? launch_bwd<true, 256, false>(r, q, a, st) : launch_bwd<false, 256, false>(r, q, a, st);
+    if (nt == 128) return bf16 ? launch_bwd<true, 128, false>(r, q, a, st) : launch_bwd<false, 128, false>(r, q, a, st);
+    return bf16 ? launch_bwd<true, 64, false>(r, q, a, st) : launch_bwd<false, 64, false>(r, q, a, st);
+  };
+  if ((e = run()) != cudaSuccess || !a.parts) return e;
+  JoinGradArgs j;
+  std::memset(&j, 0, sizeof(j));
+  j.parts = a.parts;
+  j.A = a.A;
+  j.ld = a.ld; j.stride = a.stride;
+  j.rows = a.rows; j.cols = a.cols; j.mats = a.mats; j.splits = a.splits; j.along = a.along;
+  count_launch();
+  const dim3 grid((unsigned)((a.rows + 31) / 32), (unsigned)a.mats);
+  return bf16 ? launch_early(join_grad_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, j) : launch_early(join_grad_kernel<__half>, grid, dim3(256), 0, st, j);
 }
 
 // Reads and clears the sticky "a bounded wait ran out" flag of these kernels on the current device.

@@ -173,6 +173,15 @@ def test_single_columns(dtype, turn, M, K, r, n, N):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", SIXTEEN)
+@pytest.mark.parametrize("turn", [(0, 0, 0), (1, 1, 1)])
+@pytest.mark.parametrize("M,K,r,n,lens,ids", [(200, 136, 8, 1, [6000], [0]), (130, 264, 40, 1, [1000, 3, 2050, 64, 1900], [0, 0, -1, 0, 0]),
+                                              (300, 128, 128, 2, [4000, 10, 5000, 0, 77], [1, 0, 1, 0, 1]), (65, 33, 16, 3, [4500, 4500, 4500], [0, 2, 2])])
+def test_gradients_of_few_pairs_and_many_columns(dtype, turn, M, K, r, n, lens, ids):
+    _adapter_case(dtype, M, K, r, n, np.concatenate(([0], np.cumsum(lens))), ids, sum(lens), turn)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("given", [False, True])
 def test_more_requests_than_a_table_holds(dtype, given):
