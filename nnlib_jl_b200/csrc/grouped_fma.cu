@@ -9,8 +9,8 @@
 // one's elements are on their way into registers, four neighbours at a time.  A thread multiplies 8 rows and 8 columns as packed pairs of
 // rows, in narrow tiles of every 128 / BN-th k.  A block's slot number is turned into (run, first column) by counting the tiles of all runs, since their sizes
 // are on the device only; slots that no run needs end at once.  Few tiles: K is cut and the parts are added by another launch (join_parts).
-// What bounds it: the FMA pipe and the shared memory that feeds it where columns are many (2048 x 2048, 4096 columns in 8 runs: 880 us,
-// 39 TFLOP/s; the gradient of the matrices 1086 us), reading A where they are few (6248 x 6680, 64 columns in 3 runs: 295 us, 1.7 TB/s).
+// What bounds it: the FMA pipe and the shared memory that feeds it where columns are many (2048 x 2048, 4096 columns in 8 runs: 807 us,
+// 43 TFLOP/s, with two blocks to an SM and 128 registers; 883 with one; the gradient of the matrices 802 and 1086), reading A where they are few (6248 x 6680, 64 columns in 3 runs: 277 us, 1.8 TB/s).
 #include <algorithm>
 
 #include "common.cuh"
@@ -114,7 +114,7 @@ struct Loader {
 };
 
 // A thread's part of a 128 x BN tile: 8 rows row(j) and 8 columns, of every kParts-th k, so that a step's four 16-byte reads of shared memory feed 64
-// products whatever the tile is (with 8 x 2 of every k tiles of 32 columns took 378 us where these take 295: 6248 x 6680,
+// products whatever the tile is (with 8 x 2 of every k tiles of 32 columns took 378 us where these take 277: 6248 x 6680,
 // 64 columns in 3 runs).  join()
 // adds the parts, in their order; then the thread has all of k for kOwn columns, column(i).
 template <int BN>
@@ -124,6 +124,9 @@ struct Tile {
   unsigned long long acc[8][4], own[kParts > 1 ? kOwn : 1][4];              // pairs of rows
   static __device__ __forceinline__ int part() { return threadIdx.x / kLanes; }
   static __device__ __forceinline__ int lane() { return threadIdx.x % kLanes; }
+  // a warp's lanes: 8 fours of rows by 4 fours of columns
+  static __device__ __forceinline__ int tx() { return BN > 16 ? (lane() & 7) + ((lane() >> 5) & 1) * 8 : lane() & 15; }
+  static __device__ __forceinline__ int ty() { return BN > 16 ? ((lane() >> 3) & 3) + (lane() >> 6) * 4 : lane() >> 4; }
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -131,17 +134,16 @@ struct Tile {
       for (int j = 0; j < 4; ++j) acc[i][j] = 0ull;
   }
   __device__ __forceinline__ void step(const float* p, const float* q) {
-    const int tx = lane() & 15, ty = lane() >> 4;
     unsigned long long a[4];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p + tx * 4 + h * 64);
+      const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p + tx() * 4 + h * 64);
       a[2 * h] = v.x;
       a[2 * h + 1] = v.y;
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float4 v = *reinterpret_cast<const float4*>(q + ty * 4 + h * (BN / 2));
+      const float4 v = *reinterpret_cast<const float4*>(q + ty() * 4 + h * (BN / 2));
       const float b[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -183,10 +185,10 @@ struct Tile {
 #pragma unroll
     for (int j = 0; j < 4; ++j) pair_unpack(kParts > 1 ? own[kParts > 1 ? i : 0][j] : acc[i][j], v[2 * j], v[2 * j + 1]);
   }
-  static __device__ __forceinline__ int row(int j) { return (lane() & 15) * 4 + (j >> 2) * 64 + (j & 3); }
+  static __device__ __forceinline__ int row(int j) { return tx() * 4 + (j >> 2) * 64 + (j & 3); }
   static __device__ __forceinline__ int column(int i) {
     const int c = part() * kOwn + i;
-    return (lane() >> 4) * 4 + (c >> 2) * (BN / 2) + (c & 3);
+    return ty() * 4 + (c >> 2) * (BN / 2) + (c & 3);
   }
 };
 
@@ -242,7 +244,7 @@ __host__ __device__ __forceinline__ bool fours(const T* p, long long a, long lon
 
 // blockIdx: (slot of columns, tile of rows, part of K).  parts: Float32 (M, R, parts) instead of C
 template <typename T, typename TC, int BN>
-__global__ void __launch_bounds__(256, BN == 128 ? 1 : 2) grouped_fma_kernel(const __grid_constant__ GroupedArgs g, float* parts) {
+__global__ void __launch_bounds__(256, 2) grouped_fma_kernel(const __grid_constant__ GroupedArgs g, float* parts) {
   __shared__ Shared<BN> shared;
   Stages<BN>& st = shared.stages;
   __shared__ RunSearch search;
@@ -454,9 +456,9 @@ __global__ void __launch_bounds__(256, TURNED ? 2 : 3) grouped_narrow_kernel(con
 }
 
 // blockIdx: (tile of A's shorter way, tile of its contiguous one, matrix).  The tile's rows are those along which A is contiguous, so that it is
-// stored in long pieces: C's rows, or, turned, X's.  (64 columns in 3 runs, 6248 x 6680, turned: 258 us; 558 us with C's rows, in tiles of 128 columns)
+// stored in long pieces: C's rows, or, turned, X's.  (64 columns in 3 runs, 6248 x 6680, turned: 210 us; 298 with one block to an SM; 558 with that and C's rows)
 template <typename TP, typename TQ, typename TA, int BN>
-__global__ void __launch_bounds__(256, BN == 128 ? 1 : 2) grouped_grad_kernel(const __grid_constant__ GroupedGradArgs g) {
+__global__ void __launch_bounds__(256, 2) grouped_grad_kernel(const __grid_constant__ GroupedGradArgs g) {
   __shared__ Shared<BN> shared;
   Stages<BN>& st = shared.stages;
   const bool turned = g.transA != 0;
@@ -516,20 +518,22 @@ __global__ void __launch_bounds__(256, BN == 128 ? 1 : 2) grouped_grad_kernel(co
 struct FmaShape {
   int bn, splits;
 };
-// As many columns to a tile as the average run has, fewer where that leaves SMs without a tile (333 x 200 by 1200 columns in 5 runs: 36 us
+// As many columns to a tile as the average run has (64 instead of 128 where that pads a tenth less: 8107 x 6384 by 165 columns 561 us, 620 of 128),
+// fewer where that leaves SMs without a tile (333 x 200 by 1200 columns in 5 runs: 36 us
 // in tiles of 128 columns, 19 us of 32), and K cut into parts of at least 128, while these are few, where full waves of blocks gain a tenth by it: a block costs its k and
 // some 96 more, the launch that adds the parts about 50 k (6680 x 6248 by 64 columns in 3 runs, 159 blocks: 432 us in 2 parts, 309 in more).
 FmaShape fma_shape(const GroupedArgs& g) {
   const long long each = std::max<long long>(1, g.R / std::max(1, g.G)), rows = (g.M + kRows - 1) / kRows;
   FmaShape s;
-  s.bn = each > 64 ? 128 : each > 32 ? 64 : each > 16 ? 32 : each > kNarrow ? 16 : kNarrow;
+  auto padded = [&](int bn) { return (each + bn - 1) / bn * bn; };
+  s.bn = each > 64 ? (10 * padded(64) < 9 * padded(128) ? 64 : 128) : each > 32 ? 64 : each > 16 ? 32 : each > kNarrow ? 16 : kNarrow;
   auto tiles = [&] { return ((each + s.bn - 1) / s.bn) * std::min(g.G, g.R) * rows; };
   auto cut = [&] {
-    const long long slots = s.bn == 128 ? 148 : 296;
+    const long long slots = 296;
     long long least = 0;
     int best = 1;
     for (int n = 1; n <= 32 && (n == 1 || g.K / n >= 128); n *= 2) {
-      if (n > 1 && g.R > 512 && 8ll * n * g.R * g.M > (16ll << 20)) break;
+      if (n > 1 && g.R > 512 && 8ll * n * g.R * g.M > (32ll << 20)) break;
       const long long cost = ((tiles() * n + slots - 1) / slots) * (g.K / n + 96) + (n > 1 ? 40 + 8 * n : 0);
       if (n == 1 || 10 * cost < 9 * least) { least = cost; best = n; }
     }
@@ -565,10 +569,7 @@ cudaError_t launch_grad_tiles(const GroupedGradArgs& g, cudaStream_t st) {
   const long long P = g.transA ? g.K : g.M, Q = g.transA ? g.M : g.K, rows = (P + kRows - 1) / kRows;
   if (rows > 65535 || g.mats > 65535) return cudaErrorInvalidConfiguration;
   auto blocks = [&](long long bn) { return ((Q + bn - 1) / bn) * rows * g.mats; };
-  // short runs: a block's time is the loads of its first columns and its results, so that two to an SM are better than one of twice the tile
-  // (8 matrices of 1024 x 1024, 64 columns each: 40 us in tiles of 64, 47 of 128; 100 each: 56 and 67)
-  const bool brief = g.R / std::max(1, g.mats) < 128;
-  const int bn = Q > 64 && blocks(128) >= 148 && !brief ? 128 : Q > 32 && blocks(64) >= 148 ? 64 : Q > 16 ? 32 : 16;
+  const int bn = Q > 64 && blocks(128) >= 148 ? 128 : Q > 32 && blocks(64) >= 148 ? 64 : Q > 16 ? 32 : 16;
   const dim3 grid((unsigned)((Q + bn - 1) / bn), (unsigned)rows, (unsigned)g.mats);
   switch (bn) {
     case 128: grouped_grad_kernel<TP, TQ, TA, 128><<<grid, 256, 0, st>>>(g); break;
