@@ -118,19 +118,23 @@ int workspace_ok(const void* ws, size_t bytes, size_t need) {
   return need && (!ws || bytes < need || !aligned(ws, 16)) ? NNLIB_B200_WORKSPACE_TOO_SMALL : NNLIB_B200_OK;
 }
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
-// On the CUDA cores, K in parts where that pays (ws: fma_ws() bytes); f32_out: C is Float32, whatever A and X are
-size_t fma_ws(const GroupedArgs& a) {
-  const int splits = a.M && a.R ? grouped_fma_splits(a) : 1;
-  return splits > 1 ? round256(sizeof(float) * splits * (size_t)a.R * a.M) : 0;
+// On the CUDA cores, by way of Float32 parts of K where that pays (ws: fma_ws() bytes).  They are also the way for low-rank pairs that few columns
+// share: the launch that adds the parts takes each column's pair by itself, a tile all of its columns' pairs one after the other (24 single
+// columns, 304 x 160, rank 128: 20 us, 211 in the tile).  f32_out: C is Float32, whatever A and X are
+int fma_parts(const GroupedArgs& a) {
+  if (a.M == 0 || a.R == 0) return 0;
+  const int splits = grouped_fma_splits(a);
+  return splits > 1 || (a.low.r > 0 && a.R <= 512 && a.R <= 8ll * a.low.runs) ? splits : 0;
 }
+size_t fma_ws(const GroupedArgs& a) { return round256(sizeof(float) * fma_parts(a) * (size_t)a.R * a.M); }
 cudaError_t fma_product(GroupedArgs a, int dtype, bool f32_out, void* ws, cudaStream_t st) {
-  const int splits = a.M && a.R ? grouped_fma_splits(a) : 1;
-  if (splits == 1) return grouped_fma(a, dtype, f32_out, nullptr, st);
+  const int parts = fma_parts(a);
+  if (parts == 0) return grouped_fma(a, dtype, f32_out, nullptr, st);
   const float* t = a.low.r > 0 ? static_cast<const float*>(a.low.T) : nullptr;
   GroupedArgs main = a;
   main.low.r = 0;
   const cudaError_t e = grouped_fma(main, dtype, f32_out, static_cast<float*>(ws), st);
-  return e != cudaSuccess ? e : join_parts(a, f32_out ? NNLIB_B200_F32 : dtype, splits, static_cast<const float*>(ws), t, 1, st);
+  return e != cudaSuccess ? e : join_parts(a, f32_out ? NNLIB_B200_F32 : dtype, parts, static_cast<const float*>(ws), t, 1, st);
 }
 
 int check_grouped_arrays(const GroupedArgs& a) {
