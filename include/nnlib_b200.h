@@ -577,7 +577,9 @@ NNLIB_B200_API int nnlib_b200_combine_bwd(const nnlib_b200_combine_params* p, vo
 
 /* C = W * X + scale[a] * B[:, :, a] * (A[:, :, a] * X) for the columns of the runs whose id a is a pair's number; a run with
    another id, and a column in no run, gets W * X alone.  scale * A * X is rounded to two terms of the element type (Float32: not
-   at all) and multiplied by B into the same Float32 sum as W * X. */
+   at all) and multiplied by B into the same Float32 sum as W * X; a Float16 one may be infinite
+   beyond 65504.  The workspace holds them, parts of sums, and copies of arrays that TMA cannot address (odd leading dimensions, addresses
+   that are no multiples of 16 bytes). */
 typedef struct nnlib_b200_adapter_params {
   size_t struct_size;        /* = sizeof(nnlib_b200_adapter_params) */
   int32_t dtype;
