@@ -247,8 +247,8 @@ def grouped_mul_pullback(A: torch.Tensor, X: torch.Tensor, runs: Union[torch.Ten
         At = A.transpose(0, 1)
         if not isinstance(runs, Routing):
             return dA, grouped_mul(At, dC, runs)
-        dX = _combine(grouped_mul_(_columns(X, K, R), At, dC, runs.offsets), runs, None, ones=True)
-        return dA, dX
+        # (zeros for the pairs of experts whose part of the offsets is not here)
+        return dA, _combine(grouped_mul(At, dC, runs.offsets), runs, None, ones=True)
 
     return out, back
 

@@ -1,0 +1,37 @@
+"""Calls of grouped products that their documentation allows and that went wrong once: a routing of which some experts are held, a
+routing of other tokens, one matrix for every run that has to be copied, offsets that fall, a column's place in its tile.  Tolerances as in test_experts_gpu.py."""
+import numpy as np
+import pytest
+import torch
+
+import nnlib_jl_b200 as nb
+from oracle import experts_oracle as R
+from test_experts_gpu import BF16, DEV, F16, F32, _bound, _close, _cols, _f64, _ints, _matrices
+
+
+def _poison(n):
+    """What the allocator gives out next is full of NaN."""
+    junk = [torch.full((n,), float("nan"), device=DEV) for _ in range(3)]
+    torch.cuda.synchronize()
+    del junk
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_gathered_gradients_where_some_of_the_experts_are_held(dtype):
+    """A part of the offsets, and the matrices of that part: pairs of other experts add nothing to the columns' gradient."""
+    gen = np.random.default_rng(1)
+    M, K, G, k, N = 72, 136, 6, 3, 100
+    r = nb.route_topk(_cols(gen.standard_normal((G, N))), k)
+    held = r._replace(offsets=r.offsets[2:5])
+    o, c = held.offsets.cpu().numpy(), r.columns.cpu().numpy()
+    A, X, dC = _matrices(gen, M, K, 2, dtype, False), _cols(gen.standard_normal((K, N)), dtype), _cols(gen.standard_normal((M, k * N)), dtype)
+    out, back = nb.grouped_mul_pullback(A, X, held)
+    _poison(K * k * N // 2 if dtype != F32 else K * k * N)
+    dA, dX = back(dC)
+    a, x, d = _f64(A), _f64(X), _f64(dC)
+    wA, wX = R.grouped_back(a, x, o, d, c)
+    sA, sX = R.grouped_back(np.abs(a), np.abs(x), o, np.abs(d), c)
+    _close(out, R.grouped(a, x, o, c), dtype, _bound(K, dtype) * R.grouped(np.abs(a), np.abs(x), o, c), "C")
+    _close(dA, wA, dtype, _bound(k * N, dtype) * sA, "dA")
+    _close(dX, wX, dtype, (_bound(M, dtype) + torch.finfo(dtype).eps / 2 * 1.01) * sX + (k * 2.0 ** -25 if dtype == F16 else 0), "dX")
