@@ -231,8 +231,11 @@ def grouped_mul(A: torch.Tensor, X: torch.Tensor, runs: Union[torch.Tensor, Rout
 def grouped_mul_pullback(A: torch.Tensor, X: torch.Tensor, runs: Union[torch.Tensor, Routing]):
     """``rrule``-style forward of :func:`grouped_mul`: ``(C, back)`` where ``back(dC)`` gives ``(dA, dX)``.  Nothing but the
     arguments is kept, so none of them may be written to in between.  ``dA`` is stored as ``A`` is, zeros for an empty run.
-    The gradients of columns that a :class:`Routing` gathers several times are rounded before they are added."""
+    The gradients of columns that a :class:`Routing` gathers several times are rounded before they are added; its ``position`` must be
+    that of the columns of ``X``, and the inverse of its ``columns``."""
     out = grouped_mul(A, X, runs)
+    if isinstance(runs, Routing):
+        _pairs("position", runs.position, torch.int32, None, X.shape[1], X.device)
 
     def back(dC: torch.Tensor):
         p, M, R = _grouped(A, X, runs)

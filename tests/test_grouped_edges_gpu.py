@@ -35,3 +35,15 @@ def test_gathered_gradients_where_some_of_the_experts_are_held(dtype):
     _close(out, R.grouped(a, x, o, c), dtype, _bound(K, dtype) * R.grouped(np.abs(a), np.abs(x), o, c), "C")
     _close(dA, wA, dtype, _bound(k * N, dtype) * sA, "dA")
     _close(dX, wX, dtype, (_bound(M, dtype) + torch.finfo(dtype).eps / 2 * 1.01) * sX + (k * 2.0 ** -25 if dtype == F16 else 0), "dX")
+
+
+@pytest.mark.gpu
+def test_a_routing_of_other_tokens_has_no_gradient():
+    r = nb.route_topk(nb.jl_zeros((4, 10), F32, DEV), 2)
+    A = nb.jl_zeros((8, 16, 4), F32, DEV)
+    for N in (9, 11):
+        with pytest.raises(nb.ArgumentError):
+            nb.grouped_mul_pullback(A, nb.jl_zeros((16, N), F32, DEV), r)
+    with pytest.raises(TypeError):
+        nb.grouped_mul_pullback(A, nb.jl_zeros((16, 10), F32, DEV), r._replace(position=r.position.long()))
+    nb.grouped_mul_pullback(A, nb.jl_zeros((16, 10), F32, DEV), r)
