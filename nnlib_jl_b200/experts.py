@@ -275,8 +275,9 @@ def _combine_params(Y, r, weights, ones=False):
 def _combine(Y, r, weights, ones=False):
     p, E, N, R = _combine_params(Y, r, weights, ones)
     y = _columns(Y, E, N)
-    p.y = y.data_ptr()
-    _run("combine", p, Y.device, works=False)
+    if E:
+        p.y = y.data_ptr()
+        _run("combine", p, Y.device, works=False)
     return y
 
 
@@ -300,6 +301,8 @@ def combine_pullback(Y: torch.Tensor, r: Routing, weights: Optional[torch.Tensor
             raise ArgumentError(f"dy must be of size {(E, N)}, got {tuple(dy.shape)}")
         p.columns = _vector("columns", r.columns, torch.int32, R, Y.device)
         dY, dw = _columns(Y, E, R), Y.new_empty_strided(r.position.shape, (1, r.position.shape[0]), dtype=torch.float32)
+        if not E:
+            return dY, dw.zero_()
         p.dy, p.dY, p.dweights = dy.data_ptr(), dY.data_ptr(), dw.data_ptr()
         _run("combine_bwd", p, Y.device, works=False)
         return dY, dw

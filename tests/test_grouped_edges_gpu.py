@@ -47,3 +47,17 @@ def test_a_routing_of_other_tokens_has_no_gradient():
     with pytest.raises(TypeError):
         nb.grouped_mul_pullback(A, nb.jl_zeros((16, 10), F32, DEV), r._replace(position=r.position.long()))
     nb.grouped_mul_pullback(A, nb.jl_zeros((16, 10), F32, DEV), r)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gathered_arrays_without_features(dtype):
+    r = nb.route_topk(nb.jl_zeros((4, 10), F32, DEV), 2)
+    for M, K in ((8, 0), (0, 8), (0, 0)):
+        out, back = nb.grouped_mul_pullback(nb.jl_zeros((M, K, 4), dtype, DEV), nb.jl_zeros((K, 10), dtype, DEV), r)
+        dA, dX = back(nb.jl_zeros((M, 20), dtype, DEV))
+        assert tuple(out.shape) == (M, 20) and tuple(dA.shape) == (M, K, 4) and tuple(dX.shape) == (K, 10)
+        assert (out == 0).all() and (dX == 0).all()
+    y, back = nb.combine_pullback(nb.jl_zeros((0, 20), dtype, DEV), r)
+    dY, dw = back(nb.jl_zeros((0, 10), dtype, DEV))
+    assert tuple(y.shape) == (0, 10) and tuple(dY.shape) == (0, 20) and (dw == 0).all() and tuple(dw.shape) == (2, 10)
