@@ -99,7 +99,7 @@ struct FwdArgs {
   int low_width, low_step;               // kToLow: elements of T for a column, from the first term to the second
   Runs low_runs;                         // kToC: low-rank pairs, r = 0: none
   const int* low_ids;
-  int r, n, low_kmaj;
+  int r, n, low_kmaj, low_same;          // same: one matrix for all pairs
   int wait;
   int* status;
 };
@@ -697,7 +697,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
           const int blocks = low_blocks(g.r), half = blocks / 2;
           while (ok && p.next(g, o.n0)) {
             const bool side = p.lo > o.n0 || p.hi < o.n0 + product_columns<PAIR>(o.nt);
-            for (int q = 0; q < blocks && ok; ++q) ok = fill(&tm_b, (half ? q % half : 0) * kBK, p.id, g.low_kmaj != 0, &tm_t, q * kBK, o, false, four, side, 1);
+            for (int q = 0; q < blocks && ok; ++q) ok = fill(&tm_b, (half ? q % half : 0) * kBK, g.low_same ? 0 : p.id, g.low_kmaj != 0, &tm_t, q * kBK, o, false, four, side, 1);
           }
         }
       }
@@ -1730,6 +1730,7 @@ cudaError_t product(const GroupedArgs& g, int dtype, const Shape& s, int to, voi
     f.low_ids = g.low.ids;
     f.r = g.low.r; f.n = g.low.n;
     f.low_kmaj = g.low.transB;
+    f.low_same = g.low.n > 1 && g.low.strideB == 0;
   }
   f.wait = copied ? kWaitData : before;
   return dtype == NNLIB_B200_BF16 ? fwd<true>(s, m, f, st) : fwd<false>(s, m, f, st);
