@@ -1495,11 +1495,12 @@ __global__ void __launch_bounds__(256) join_low_kernel(const float* parts, int s
 // A matrix (or several) that is read: where it lies, contiguous extent first.
 struct Operand {
   const void* p;
-  long long wide, deep, ld, stride, count;
+  long long wide, deep, ld, stride, count;               // stride 0: all are one, which is copied once
   const int* columns;                    // rows `deep` of them are gathered from these of `rows`; NULL: as they lie
   long long rows;
   bool fits() const { return aligned16(p) && stride_ok(ld) && (count <= 1 || stride == 0 || stride_ok(stride)); }
-  size_t copy_bytes() const { return (fits() && !columns) || wide == 0 || deep == 0 || count == 0 ? 0 : (size_t)((wide + 7) / 8 * 16) * deep * count; }
+  long long different() const { return stride ? count : std::min(count, 1ll); }
+  size_t copy_bytes() const { return (fits() && !columns) || wide == 0 || deep == 0 || count == 0 ? 0 : (size_t)((wide + 7) / 8 * 16) * deep * different(); }
 };
 cudaError_t align_operand(Operand& o, char*& ws, const Runs* of, bool& behind, cudaStream_t st) {
   const size_t bytes = o.copy_bytes();
@@ -1513,10 +1514,10 @@ cudaError_t align_operand(Operand& o, char*& ws, const Runs* of, bool& behind, c
   c.vec = o.fits() && o.wide % 8 == 0;
   c.rows = (int)o.rows;
   c.columns = o.columns;
-  c.of = of ? *of : Runs{nullptr, 0, 0, 0};
+  c.of = of && o.stride ? *of : Runs{nullptr, 0, 0, 0};
   const long long blocks = std::min<long long>((o.deep + 7) / 8, 1 << 20);
   // (behind: a kernel of this call is before it in the stream)
-  const dim3 grid((unsigned)blocks, 1, (unsigned)o.count);
+  const dim3 grid((unsigned)blocks, 1, (unsigned)o.different());
   if (behind) {
     const cudaError_t e = launch_early(copy_rows_kernel, grid, dim3(256), 0, st, c);
     if (e != cudaSuccess) return e;
@@ -1527,7 +1528,7 @@ cudaError_t align_operand(Operand& o, char*& ws, const Runs* of, bool& behind, c
   behind = true;
   o.p = ws;
   o.ld = (long long)c.ld8 * 8;
-  o.stride = o.ld * o.deep;
+  if (o.stride) o.stride = o.ld * o.deep;
   o.columns = nullptr;
   ws += (bytes + 255) / 256 * 256;
   return cudaGetLastError();

@@ -61,3 +61,31 @@ def test_gathered_arrays_without_features(dtype):
     y, back = nb.combine_pullback(nb.jl_zeros((0, 20), dtype, DEV), r)
     dY, dw = back(nb.jl_zeros((0, 10), dtype, DEV))
     assert tuple(y.shape) == (0, 10) and tuple(dY.shape) == (0, 20) and (dw == 0).all() and tuple(dw.shape) == (2, 10)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("M,K", [(137, 64), (136, 67), (137, 67)])
+def test_one_matrix_for_every_run_that_is_copied(dtype, turned, M, K):
+    """The first run is empty: the one copy of the matrix is not its alone."""
+    gen = np.random.default_rng(M + K)
+    G, N = 5, 400
+    one = _matrices(gen, M, K, 1, dtype, turned)
+    X, dC, o = _cols(gen.standard_normal((K, N)), dtype), _cols(gen.standard_normal((M, N)), dtype), _ints([0, 0, 100, 250, 390, 400])
+    each = _matrices(gen, M, K, G, dtype, turned).copy_(one.expand(M, K, G))
+    want = nb.grouped_mul(each, X, o)
+    dA, dX = nb.grouped_mul_pullback(each, X, o)[1](dC)
+    _poison(M * K * G)
+    out, back = nb.grouped_mul_pullback(one.expand(M, K, G), X, o)
+    assert (out == want).all()
+    _poison(M * K * G)
+    gA, gX = back(dC)
+    assert (gX == dX).all() and (gA == dA).all()
+    few = _ints([0, 0, 3, 5, 9, 12])                        # (gathered, K in parts)
+    c = _ints(gen.integers(0, N, 12))
+    none = torch.empty(0, device=DEV)
+    r = nb.Routing(none, none, few, c, none)
+    want = nb.grouped_mul(each, X, r)
+    _poison(M * K * G)
+    assert (nb.grouped_mul(one.expand(M, K, G), X, r) == want).all()
