@@ -171,9 +171,11 @@ struct Tile {
           for (int i = 0; i < kOwn; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              unsigned long long v = acc[d * kOwn + i][j];
+              // (part 0 first, whoever adds: a column's sum is the same in every place)
+              auto part_of = [&](int q) { return q == d ? acc[d * kOwn + i][j] : room[((i * 4 + j) * (kParts - 1) + q - (q > d ? 1 : 0)) * kLanes + t]; };
+              unsigned long long v = part_of(0);
 #pragma unroll
-              for (int q = 0; q + 1 < kParts; ++q) v = pair_add(v, room[((i * 4 + j) * (kParts - 1) + q) * kLanes + t]);
+              for (int q = 1; q < kParts; ++q) v = pair_add(v, part_of(q));
               own[i][j] = v;
             }
         }

@@ -89,3 +89,16 @@ def test_one_matrix_for_every_run_that_is_copied(dtype, turned, M, K):
     want = nb.grouped_mul(each, X, r)
     _poison(M * K * G)
     assert (nb.grouped_mul(one.expand(M, K, G), X, r) == want).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("M,K,N", [(136, 64, 400), (300, 1000, 70), (72, 333, 40), (520, 130, 20), (264, 96, 9), (96, 70, 3)])
+def test_a_columns_result_does_not_depend_on_its_place(M, K, N, turned):
+    """Bit by bit, in Float32, whatever the tile: the parts of a sum are added in one order."""
+    gen = np.random.default_rng(M + N)
+    A, X = _matrices(gen, M, K, 1, F32, turned), _cols(gen.standard_normal((K, N)))
+    out = nb.grouped_mul(A, X, _ints([0, N]))
+    for by in (1, 2, 5, 8, 19):
+        moved = nb.grouped_mul(A, nb.as_column_major(torch.roll(X, by, 1)), _ints([0, N]))
+        assert (moved == torch.roll(out, by, 1)).all(), by
