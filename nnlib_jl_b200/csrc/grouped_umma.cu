@@ -14,9 +14,13 @@
 //               as it is stored) and of the columns (K-major); gathered columns arrive four at a time (tile::gather4), their numbers in
 //               the lanes' registers.  One thread takes some 125 cycles for a copy: with a single producer a stage took 765 cycles,
 //               148 of them 4.2 TB/s
-//   warp 1      allocates tensor memory, issues every tcgen05.mma; for low-rank pairs it clears the rows of T that belong to
-//               other runs before it multiplies
+//   warp 1      allocates tensor memory, issues every tcgen05.mma; a low-rank pair's are of the 16 columns (PAIR: 32) that its runs are in, where
+//               it first clears the rows of T that belong to other runs
 //   warps 2-9   epilogue: tensor memory -> registers -> shared memory, transposed -> C
+// A matrix B_a with infinities or NaN may meet neither those cleared rows nor the second terms of T, which can have the other sign: zero times
+// infinity, and infinity minus infinity, would be NaN in columns of other requests and in its own.  So the product A X, whose epilogue has
+// nothing to do at first, looks through the B_a in use and leaves a byte for each 128 rows of each, and where one is set the pair is
+// added by the epilogue in Float32.  (6160 columns in 8 runs, 4096 x 4096, rank 64: 194 us; 205 where the issuing warp looks through the blocks as they arrive.)
 // Two accumulators alternate, so that the epilogue of one tile overlaps the products of the next.
 //
 // What bounds it: reading the matrices while a run is a few columns (8 experts of 14336 x 4096 for 16 columns: 99 us, 1.2 of what reading those
@@ -78,6 +82,7 @@ struct Bars {
   uint64_t side[6];                      // PAIR, stages of which columns are to be cleared: the second CTA's copies are there; in the first CTA: are cleared
   uint32_t tmem_base;
   int abort_flag;
+  int odd;                               // sticky: a pair was left to the epilogue
   RunSearch search;
 };
 static_assert(sizeof(Bars) <= 512, "barrier block");
@@ -96,9 +101,14 @@ struct FwdArgs {
   int M, K, G, N, mats;
   int cap;                               // columns of a tile, at most NT
   int a_kmaj, a_same, zero_rest, splits, tiles_m, to, vec, gather;
-  int low_width, low_step;               // kToLow: elements of T for a column, from the first term to the second
+  int low_width, low_step;               // elements of T for a column, from the first term to the second
   Runs low_runs;                         // kToC: low-rank pairs, r = 0: none
   const int* low_ids;
+  const void* low_B;                     // as the caller has it
+  long long low_ldb, low_strideB;
+  const void* low_T;
+  unsigned char* odd;                    // (n, 128s of rows of B): whether there are infinities or NaN; read, or, look_r > 0, found out
+  int look_r, look_m;                    // rank of B, its rows
   int r, n, low_kmaj, low_same;          // same: one matrix for all pairs
   int wait;
   int* status;
@@ -266,6 +276,7 @@ __device__ __forceinline__ void set_up(Bars* bars) {
       mbar_init(&bars->acc_empty[s], PAIR ? 16 : 8);
     }
     bars->abort_flag = *reinterpret_cast<volatile int*>(&g_grouped_abort);
+    bars->odd = 0;
     fence_mbar_init();
   }
   if ((threadIdx.x >> 5) == 1) take_tmem<PAIR>(&bars->tmem_base, C::kTmemCols);
@@ -296,9 +307,10 @@ __device__ __forceinline__ T left_of(float v, T first) {
   return Elem<T>::from_f(fabsf(Elem<T>::to_f(first)) < INFINITY ? v - Elem<T>::to_f(first) : 0.f);
 }
 __device__ __forceinline__ int round16(int n) { return (n + 15) & ~15; }
-// columns that a product of n takes (PAIR: half of them from each CTA)
+// columns that a product takes are so many at a time (PAIR: half of them from each CTA)
+template <bool PAIR> constexpr int kGrain = PAIR ? 32 : 16;
 template <bool PAIR>
-__device__ __forceinline__ int product_columns(int n) { return PAIR ? (n + 31) & ~31 : round16(n); }
+__device__ __forceinline__ int product_columns(int n) { return (n + kGrain<PAIR> - 1) & ~(kGrain<PAIR> - 1); }
 
 // Width of the tiles of a run of n columns, and their number: at most cap (a multiple of 16) and as even as multiples of 16 allow.
 __host__ __device__ __forceinline__ int tile_width(int n, int cap) {
@@ -439,8 +451,88 @@ struct Pairs {
     return false;
   }
 };
+// The part of a tile that a pair's columns are in, in whole grains: a tile of its own; whether columns of other runs are there too.
+template <bool PAIR>
+__device__ __forceinline__ Tile part_of(const Tile& o, const Pairs& p, bool& shared) {
+  Tile t = o;
+  t.n0 = o.n0 + ((p.lo - o.n0) & ~(kGrain<PAIR> - 1));
+  t.nt = product_columns<PAIR>(p.hi - t.n0);
+  shared = p.lo > t.n0 || p.hi < min(t.n0 + t.nt, o.n0 + o.nt);
+  return t;
+}
+// whether the pair is left to the epilogue (for the tile; PAIR: both CTAs' rows)
+template <bool PAIR>
+__device__ __forceinline__ bool odd_pair(const FwdArgs& g, const Tile& o, int id) {
+  const unsigned char* f = g.odd + (long long)(o.m0 >> 7) * g.n + id;
+  return (f[0] | (PAIR && o.m0 + 128 < g.M ? f[g.n] : 0)) != 0;
+}
 // K blocks that a pair adds: rank up to 32: both terms of T in one; above: the first terms' blocks, then the second ones'
 __device__ __forceinline__ int low_blocks(int r) { return r <= 32 ? 1 : 2 * ((r + 63) / 64); }
+
+// Looks for infinities and NaN in the matrices of pairs that runs name, 128 rows of one to a warp: warp `w` of `warps`.
+template <bool BF16>
+__device__ __forceinline__ void look_for_odd(const FwdArgs& g, long long w, long long warps) {
+  constexpr uint32_t kExponent = BF16 ? 0x7f807f80u : 0x7c007c00u, kOne = BF16 ? 0x00800080u : 0x04000400u;
+  auto high = [](uint32_t v) { return ((v & kExponent) + kOne) & 0x80008000u; };           // an exponent of ones runs over into the sign's place
+  const int lane = threadIdx.x & 31, runs = g.low_runs.runs;
+  const bool vec = ((reinterpret_cast<uintptr_t>(g.low_B) & 15) | ((g.low_ldb | g.low_strideB) & 7)) == 0;
+  const long long units = (long long)runs * ((g.look_m + 127) >> 7);
+  for (long long u = w; u < units; u += warps) {
+    const int rb = units <= 0x7fffffff ? (int)u / runs : (int)(u / runs), b = (int)(u - (long long)rb * runs), id = g.low_ids[b];
+    if (id < 0 || id >= g.n) continue;
+    bool again = false;                                    // an earlier run has the pair
+    for (int i = 0; i < b && !again; i += 32) again = __any_sync(0xffffffffu, i + lane < b && g.low_ids[i + lane] == id);
+    if (again) continue;
+    const int rows = min(128, g.look_m - rb * 128), inner = g.low_kmaj ? g.look_r : rows, outer = g.low_kmaj ? rows : g.look_r;
+    const unsigned short* p = reinterpret_cast<const unsigned short*>(g.low_B) + id * g.low_strideB + rb * 128ll * (g.low_kmaj ? g.low_ldb : 1);
+    const int pieces = vec ? inner >> 3 : 0;               // at most 16: 2^wide lanes to a line
+    const int wide = pieces > 8 ? 4 : pieces > 4 ? 3 : pieces > 2 ? 2 : pieces > 1 ? 1 : 0, c = lane & ((1 << wide) - 1);
+    uint32_t found = 0u;
+    if (c < pieces) {
+      const unsigned short* q = p + c * 8;
+#pragma unroll 8
+      for (int i = lane >> wide; i < outer; i += 32 >> wide) {
+        const uint4 v = *reinterpret_cast<const uint4*>(q + i * g.low_ldb);
+        found |= high(v.x) | high(v.y) | high(v.z) | high(v.w);
+      }
+    }
+    if (inner > pieces * 8) {
+#pragma unroll 4
+      for (int i = 0; i < outer; ++i)
+        for (int e = pieces * 8 + lane; e < inner; e += 32) found |= high(p[i * g.low_ldb + e]);
+    }
+    const int any = __any_sync(0xffffffffu, found != 0u);
+    if (lane == 0) g.odd[(long long)rb * g.n + id] = any ? 1 : 0;
+  }
+}
+// Adds to a tile of products, in tensor memory, what the pairs that the tensor cores left out give: this warp's rows, every other 32 columns.  Hardly
+// ever called.
+template <bool BF16, bool PAIR>
+__device__ __noinline__ void add_odd(const FwdArgs& g, const Table& tab, const Tile& o, int m, int part, uint32_t taddr) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  Pairs p(g, tab, o.n0, o.nt);
+  while (p.next(g, o.n0)) {
+    if (!odd_pair<PAIR>(g, o, p.id)) continue;
+    const T* b = reinterpret_cast<const T*>(g.low_B) + (long long)p.id * g.low_strideB + (g.low_kmaj ? (long long)m * g.low_ldb : m);
+    const long long step = g.low_kmaj ? 1 : g.low_ldb;
+    for (int n = p.lo; n < p.hi; ++n) {
+      const int c = n - o.n0;
+      if (((c >> 5) & 1) != part) continue;
+      const T* t = reinterpret_cast<const T*>(g.low_T) + (long long)n * g.low_width;
+      float v = 0.f;
+      if (m < g.M) {
+#pragma unroll 4
+        for (int k = 0; k < g.r; ++k) v = fmaf(Elem<T>::to_f(b[k * step]), Elem<T>::to_f(t[k]) + Elem<T>::to_f(t[g.low_step + k]), v);
+      }
+      __syncwarp();
+      uint32_t a;
+      asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(a) : "r"(taddr + c) : "memory");
+      tmem_wait_ld();
+      asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr + c), "r"(__float_as_uint(__uint_as_float(a) + v)) : "memory");
+      tmem_wait_st();
+    }
+  }
+}
 
 // 16 lanes x 32 columns of tensor memory in the fragment layout of a matrix product: register 4 j + 2 s + e of lane l is row 8 s + l / 4,
 // column 8 j + 2 (l % 4) + e
@@ -696,8 +788,10 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
           Pairs p(g, tab, o.n0, o.nt);
           const int blocks = low_blocks(g.r), half = blocks / 2;
           while (ok && p.next(g, o.n0)) {
-            const bool side = p.lo > o.n0 || p.hi < o.n0 + product_columns<PAIR>(o.nt);
-            for (int q = 0; q < blocks && ok; ++q) ok = fill(&tm_b, (half ? q % half : 0) * kBK, g.low_same ? 0 : p.id, g.low_kmaj != 0, &tm_t, q * kBK, o, false, four, side, 1);
+            if (odd_pair<PAIR>(g, o, p.id)) continue;
+            bool shared;
+            const Tile own = part_of<PAIR>(o, p, shared);
+            for (int q = 0; q < blocks && ok; ++q) ok = fill(&tm_b, (half ? q % half : 0) * kBK, g.low_same ? 0 : p.id, g.low_kmaj != 0, &tm_t, q * kBK, own, false, four, shared, 1);
           }
         }
       }
@@ -748,11 +842,16 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
       if (g.r > 0 && ok) {
         Pairs p(g, tab, o.n0, o.nt);
         const int blocks = low_blocks(g.r), half = blocks / 2;
-        const uint32_t id_low = idesc_of<PAIR>(BF16, wide, !g.low_kmaj, false), step = g.low_kmaj ? 32 >> 4 : 2048 >> 4;
-        const int mine = PAIR ? wide / 2 : wide, n0 = o.n0 + rank * mine;
+        const uint32_t step = g.low_kmaj ? 32 >> 4 : 2048 >> 4;
         while (ok && p.next(g, o.n0)) {
-          const int lo = p.lo - n0, hi = p.hi - n0;
-          const bool side = p.lo > o.n0 || p.hi < o.n0 + wide;      // columns of other runs take no part
+          if (odd_pair<PAIR>(g, o, p.id)) {
+            if (lane == 0) *reinterpret_cast<volatile int*>(&bars->odd) = 1;
+            continue;
+          }
+          bool side;                                       // columns of other runs take no part
+          const Tile own = part_of<PAIR>(o, p, side);
+          const int mine = PAIR ? own.nt / 2 : own.nt, n0 = own.n0 + rank * mine, lo = p.lo - n0, hi = p.hi - n0;
+          const uint32_t id_low = idesc_of<PAIR>(BF16, own.nt, !g.low_kmaj, false), d = acc + (own.n0 - o.n0);
           for (int q = 0; q < blocks; ++q, at.next()) {
             const int s = at.s;
             uint8_t* tx = smem + s * C::kStage + C::kXOff;
@@ -774,8 +873,8 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
               const uint32_t a = base + s * (C::kStage >> 4), x = a + (C::kXOff >> 4);
               const int left = half ? g.r - (q % half) * kBK : g.r, steps = min(4, (left + 15) >> 4);
               for (int kk = 0; kk < steps; ++kk) {
-                multiply_add<PAIR>(acc, a + kk * step, x + kk * 2, id_low, 1u);
-                if (!half) multiply_add<PAIR>(acc, a + kk * step, x + kk * 2 + 4, id_low, 1u);
+                multiply_add<PAIR>(d, a + kk * step, x + kk * 2, id_low, 1u);
+                if (!half) multiply_add<PAIR>(d, a + kk * step, x + kk * 2 + 4, id_low, 1u);
               }
               commit_to<PAIR>(&bars->empty[s]);
             }
@@ -791,6 +890,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     bool ok = true;
     int ti = 0;
     uint8_t* box = smem + C::kOutOff + (warp - 2) * 2048;
+    if (g.look_r > 0) look_for_odd<BF16>(g, (gridDim.x - 1 - blockIdx.x) * 8ll + warp - 2, gridDim.x * 8ll);      // (the last CTAs have the fewest tiles)
     for (long long t = worker; t < tiles && ok; t += workers) {
       const Tile o = tile_of<PAIR>(g, tab, t, nkb);
       if (o.nt <= 0) continue;
@@ -811,6 +911,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
       float scale = 1.f;
       if (g.to != kToC) scale = g.scale ? g.scale[o.mat] : g.scale0;
       if (g.to == kToC) {
+        if (g.r > 0 && chunks > 0 && *reinterpret_cast<volatile int*>(&bars->odd)) add_odd<BF16, PAIR>(g, tab, o, m, part, taddr);
         auto put = [&](uint32_t (&f)[2][16], int c) {
           uint32_t gone = 0u;
 #pragma unroll
@@ -1596,7 +1697,9 @@ cudaError_t launch(K kern, long long workers, int smem, bool early, cudaStream_t
 template <bool BF16, int NT, bool PAIR>
 cudaError_t launch_fwd(const Maps& m, FwdArgs g, long long most, cudaStream_t st) {
   g.tiles_m = (g.M + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128);
-  return launch<PAIR>(grouped_umma_kernel<BF16, NT, PAIR>, most * g.tiles_m * g.splits, Cfg<NT, PAIR>::kSmem, g.wait != kWaitNone, st, m.a, m.x, m.b, m.t, g);
+  // (as many CTAs as look through the pairs' matrices in one go, be the tiles few)
+  const long long looks = g.look_r > 0 ? ((long long)g.low_runs.runs * ((g.look_m + 127) / 128) + 7) / 8 : 0;
+  return launch<PAIR>(grouped_umma_kernel<BF16, NT, PAIR>, most * g.tiles_m * g.splits + looks, Cfg<NT, PAIR>::kSmem, g.wait != kWaitNone, st, m.a, m.x, m.b, m.t, g);
 }
 template <bool BF16, int NT, bool PAIR>
 cudaError_t launch_bwd(const CUtensorMap& r, const CUtensorMap& c, GradArgs g, cudaStream_t st) {
@@ -1686,7 +1789,9 @@ size_t parts_bytes(const GroupedArgs& g, const Shape& s) { return padded((size_t
 
 // One product; `to` and `out`: what it writes and where.  ws: copies_bytes().  before: what of this call was launched before it (kWaitData:
 // it reads that; kWaitEnd: it does not).
-cudaError_t product(const GroupedArgs& g, int dtype, const Shape& s, int to, void* out, char* ws, int before, cudaStream_t st) {
+// odd: bytes of the pairs' matrices, read with g.low; look: the product whose pairs they are, whose matrices are looked through.
+cudaError_t product(const GroupedArgs& g, int dtype, const Shape& s, int to, void* out, char* ws, int before, cudaStream_t st, unsigned char* odd = nullptr,
+                    const GroupedArgs* look = nullptr) {
   bool behind = before != kWaitNone, copied = false;
   Operand a = matrices(g.A, g.transA != 0, g.M, g.K, g.lda, g.strideA, g.mats), x = columns_of(g.X, g.K, g.N, g.ldx, g.columns, g.R);
   const Runs runs{g.offsets, g.run_len, g.G, g.R};
@@ -1714,7 +1819,7 @@ cudaError_t product(const GroupedArgs& g, int dtype, const Shape& s, int to, voi
   f.zero_rest = g.zero_rest && to == kToC;
   f.splits = s.splits;
   f.to = to;
-  f.low_width = low_width(g.M);
+  f.low_width = low_width(to == kToLow ? g.M : g.low.r);
   f.low_step = f.low_width / 2;
   f.status = g.status;
   Maps m;
@@ -1727,11 +1832,24 @@ cudaError_t product(const GroupedArgs& g, int dtype, const Shape& s, int to, voi
     if ((e = align_operand(b, ws, nullptr, behind, st)) != cudaSuccess) return e;
     const Operand t{g.low.T, low_width(g.low.r), g.R, low_width(g.low.r), 0, 1, nullptr, 0};
     if (!encode_matrix(&m.b, dtype, b, g.low.transB != 0) || !encode_columns(&m.t, dtype, t, box_of(s))) return cudaErrorInvalidValue;
-    f.low_runs = Runs{g.low.offsets, g.low.run_len, g.low.runs, g.R};
-    f.low_ids = g.low.ids;
-    f.r = g.low.r; f.n = g.low.n;
-    f.low_kmaj = g.low.transB;
+    f.r = g.low.r;
     f.low_same = g.low.n > 1 && g.low.strideB == 0;
+  }
+  const GroupedArgs* of = look ? look : f.r > 0 ? &g : nullptr;
+  if (of) {
+    const LowRank& l = of->low;
+    f.low_runs = Runs{l.offsets, l.run_len, l.runs, of->R};
+    f.low_ids = l.ids;
+    f.n = l.n;
+    f.low_B = l.B;
+    f.low_ldb = l.ldb; f.low_strideB = l.strideB;
+    f.low_kmaj = l.transB;
+    f.low_T = l.T;
+    f.odd = odd;
+  }
+  if (look) {
+    f.look_r = look->low.r;
+    f.look_m = look->M;
   }
   f.wait = copied ? kWaitData : before;
   return dtype == NNLIB_B200_BF16 ? fwd<true>(s, m, f, st) : fwd<false>(s, m, f, st);
@@ -1792,13 +1910,13 @@ size_t low_umma_workspace_bytes(const GroupedArgs& f) {
 }
 size_t low_umma_bytes(const GroupedArgs& f) { return padded((size_t)f.R * 2 * low_width(f.M)); }
 // behind: a kernel of this call is before it in the stream, whose results it does not read but whose workspace it may write
-cudaError_t low_umma(const GroupedArgs& f, int dtype, void* T, void* workspace, bool behind, cudaStream_t st) {
+cudaError_t low_umma(const GroupedArgs& f, int dtype, void* T, void* workspace, bool behind, cudaStream_t st, unsigned char* odd, const GroupedArgs* look) {
   const int before = behind ? kWaitData : kWaitNone;
   const Shape s = first_shape(f);
   char* ws = static_cast<char*>(workspace);
-  if (s.splits == 1) return product(f, dtype, s, kToLow, T, ws, before, st);
+  if (s.splits == 1) return product(f, dtype, s, kToLow, T, ws, before, st, odd, look);
   char* parts = ws + copies_bytes(f, s);
-  const cudaError_t e = product(f, dtype, s, kToParts, parts, ws, before, st);
+  const cudaError_t e = product(f, dtype, s, kToParts, parts, ws, before, st, odd, look);
   if (e != cudaSuccess) return e;
   const int width = low_width(f.M);
   const long long blocks = ((long long)f.R * (width / 2) + 255) / 256;
@@ -1813,9 +1931,10 @@ cudaError_t low_umma(const GroupedArgs& f, int dtype, void* T, void* workspace, 
 static Shape main_shape(const GroupedArgs& m, bool keep) { return shape_of(m.M, m.K, m.R, 1, !keep && few(m.R, m.M)); }
 // (a pair is read anew for each of its columns)
 static bool first_by_column(const GroupedArgs& f) { return f.R <= 4 * f.G && f.K <= 64 * kLowK; }
+static size_t odd_bytes(const GroupedArgs& m) { return m.low.r > 0 ? padded((size_t)m.low.n * ((m.M + 127) / 128)) : 0; }
 size_t adapter_umma_workspace_bytes(const GroupedArgs& first, const GroupedArgs& m, bool keep) {
   const Shape s = main_shape(m, keep);
-  if (s.splits == 1) return std::max(m.low.r > 0 ? low_umma_workspace_bytes(first) : 0, copies_bytes(m, s));
+  if (s.splits == 1) return odd_bytes(m) + std::max(m.low.r > 0 ? low_umma_workspace_bytes(first) : 0, copies_bytes(m, s));
   Shape f = first_shape(first);
   const size_t own = copies_bytes(m, s) + parts_bytes(m, s);
   if (m.low.r == 0) return own;
@@ -1828,9 +1947,11 @@ cudaError_t adapter_umma(const GroupedArgs& first, GroupedArgs m, int dtype, boo
   char* ws = static_cast<char*>(workspace);
   cudaError_t e = cudaSuccess;
   if (s.splits == 1) {
-    if (m.low.r > 0) e = low_umma(first, dtype, low, ws, false, st);
+    unsigned char* odd = static_cast<unsigned char*>(workspace);
+    ws += odd_bytes(m);
+    if (m.low.r > 0) e = low_umma(first, dtype, low, ws, false, st, odd, &m);
     m.low.T = low;
-    return e == cudaSuccess ? product(m, dtype, s, kToC, m.C, ws, m.low.r > 0 ? kWaitData : kWaitNone, st) : e;
+    return e == cudaSuccess ? product(m, dtype, s, kToC, m.C, ws, m.low.r > 0 ? kWaitData : kWaitNone, st, odd) : e;
   }
   // few columns: both products in parts, joined by one launch that multiplies by B.  W X does not wait for A X, its end does.
   Shape f = first_shape(first);

@@ -264,7 +264,9 @@ cudaError_t grouped_umma(const GroupedArgs& g, int dtype, void* workspace, cudaS
 int low_width(int r);                                     // 16-bit elements of T for a column
 size_t low_umma_bytes(const GroupedArgs& first);          // T of all columns
 size_t low_umma_workspace_bytes(const GroupedArgs& first);
-cudaError_t low_umma(const GroupedArgs& first, int dtype, void* T, void* workspace, bool behind, cudaStream_t st);
+// odd, look: where it is noted which matrices of the pairs of `look` have infinities or NaN
+cudaError_t low_umma(const GroupedArgs& first, int dtype, void* T, void* workspace, bool behind, cudaStream_t st, unsigned char* odd = nullptr,
+                     const GroupedArgs* look = nullptr);
 size_t adapter_umma_workspace_bytes(const GroupedArgs& first, const GroupedArgs& main, bool keep);
 cudaError_t adapter_umma(const GroupedArgs& first, GroupedArgs main, int dtype, bool keep, void* low, void* workspace, cudaStream_t st);
 bool grouped_umma_grad_supports(const GroupedGradArgs& g, int dtype);

@@ -32,3 +32,54 @@ def test_a_factor_that_all_pairs_share(dtype, turn, M, K, r, N):
         _close(y, R.adapters(w, x, p, q, ids, offsets, s), dtype, sizes[0], "Y")
         for got, want, size, what in zip(back(dY), R.adapters_back(w, x, p, q, ids, offsets, s, d), sizes[1:], ("dX", "dA", "dB")):
             _close(got, want, dtype, size, what)
+
+
+def _same_kind(got, want, base, others, near, size, dtype, what):
+    """NaN and the infinities where the definition has them; in columns of other requests the bits of a call without them, in the pair's own rows without
+    them what the definition gives (near: with zeros in their place)."""
+    assert (got[:, others] == base[:, others]).all(), what
+    got = _f64(got)
+    assert (np.isnan(got) == np.isnan(want)).all(), what
+    for s in (np.inf, -np.inf):
+        assert ((got == s) == (want == s)).all(), what
+    fine = np.isfinite(want)
+    _close(torch.from_numpy(np.where(fine, got, near)), near, dtype, size, what)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("turn", [(0, 0, 0), (1, 1, 1)])
+@pytest.mark.parametrize("M,K,r,lens", [
+    (136, 64, 16, [10, 50, 1, 39, 50, 17, 33]), (100, 200, 40, [7, 9, 20]), (512, 328, 16, [300, 5, 129, 64, 20, 240, 1]),
+    (320, 136, 100, [64, 32, 16, 500, 3, 40, 200]), (264, 1024, 8, [1] * 24), (512, 200, 64, [512, 256, 256]), (300, 72, 5, [31, 33, 600])])
+def test_a_pair_with_infinities_reaches_its_own_columns_alone(dtype, turn, M, K, r, lens):
+    """Whatever the other requests of a tile are; the pullback's dX is the same product."""
+    gen = np.random.default_rng(M + K)
+    n = 6
+    W, A, B = _factors(gen, M, K, r, n, dtype, turn)
+    N = sum(lens)
+    X, dY = _cols(gen.standard_normal((K, N)), dtype), _cols(gen.standard_normal((M, N)), dtype)
+    ids, offsets = [(2, 0, 5, 1, -1, 3)[i % 6] for i in range(len(lens))], np.concatenate(([0], np.cumsum(lens))).astype(int)
+    how = {"offsets": _ints(offsets)}
+    run = lambda: (lambda y, back: (y, *back(dY)))(*nb.adapter_mul_pullback(W, X, A, B, _ints(ids), **how))
+    base = run()
+    inf = float("inf")
+    B[M // 2, r // 2, 0], B[3, 0, 5], B[min(M - 1, 70), r - 1, 5] = inf, float("nan"), -inf
+    B[M - 1, 0, 2], B[M - 1, r - 1, 2] = inf, inf
+    got = run()
+    w, x, a, b, d, s = _f64(W), _f64(X), _f64(A), _f64(B), _f64(dY), np.ones(n)
+    others = [i for (p, q), e in zip(R.runs(offsets, N), ids) if e in (1, 3, -1) for i in range(p, q)]
+    zeros = lambda v: np.where(np.isfinite(v), v, 0.0)
+    with np.errstate(invalid="ignore"):
+        _same_kind(got[0], R.adapters(w, x, a, b, ids, offsets, s), base[0], others, R.adapters(w, x, a, zeros(b), ids, offsets, s),
+                   _sizes(w, x, a, zeros(b), ids, offsets, s, dtype), dtype, "Y")
+    B[:] = _cols(np.where(np.isfinite(b), b, 0.25), dtype)
+    base = run()
+    A[0, K // 2, 0], A[r - 1, K - 1, 5], A[r // 2, 0, 5] = inf, float("nan"), -inf
+    got = run()
+    a, b = _f64(A), _f64(B)
+    others = [i for (p, q), e in zip(R.runs(offsets, N), ids) if e not in (0, 5) for i in range(p, q)]
+    with np.errstate(invalid="ignore"):
+        _same_kind(got[1], R.adapters_back(w, x, a, b, ids, offsets, s, d)[0], base[1], others, R.adapters_back(w, x, zeros(a), b, ids, offsets, s, d)[0],
+                   _sizes(w, x, zeros(a), b, ids, offsets, s, dtype, d)[1], dtype, "dX")
+    assert (got[2] == base[2]).all()                         # (dA = scale B^T dY X^T)
