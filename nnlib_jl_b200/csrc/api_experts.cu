@@ -248,8 +248,8 @@ bool adapter_on_umma(const Adapters& a, int dtype) {
   return on_umma(a.main, dtype) && on_umma(f, dtype);
 }
 bool has_pairs(const Adapters& a) { return a.first.G > 0 && a.first.mats > 0 && a.first.K > 0; }
-size_t low_bytes(const Adapters& a, bool umma) {
-  return umma ? low_umma_bytes(a.first) : round256((size_t)a.first.R * 4 * (size_t)a.first.M);
+size_t low_bytes(const Adapters& a, int dtype, bool umma) {
+  return umma ? low_umma_bytes(a.first, dtype) : round256((size_t)a.first.R * 4 * (size_t)a.first.M);
 }
 // A X (or B^T dC) into `low`, then the product that adds B times it (A^T times it); `ws`: adapter_ws() bytes.  keep: `low` is read behind it.
 cudaError_t adapter_products(Adapters& a, int dtype, bool umma, bool keep, void* low, void* ws, cudaStream_t st) {
@@ -281,7 +281,7 @@ PairGrads pair_grads(const nnlib_b200_adapter_params* p, const Adapters& a, bool
   o.first.A = p->A; o.first.lda = p->lda; o.first.strideA = p->strideA; o.first.transA = p->transA ? 1 : 0;
   o.first.K = (int)p->K;
   o.first.X = p->X; o.first.ldx = p->ldx;
-  const long long wide = umma ? low_width((int)p->r) : p->r;
+  const long long wide = umma ? low_width((int)p->r, p->dtype) : p->r;
   o.a = grad_of(o.first);
   o.a.A = p->dA; o.a.lda = p->transA ? p->K : p->r; o.a.strideA = p->r * p->K;
   o.a.C = nullptr; o.a.ldc = wide;
@@ -380,14 +380,14 @@ size_t nnlib_b200_adapter_gemm_workspace_bytes(const nnlib_b200_adapter_params* 
   Adapters a;
   if (resolve_adapter(p, false, &a)) return 0;
   const bool umma = adapter_on_umma(a, p->dtype);
-  return low_bytes(a, umma) + adapter_ws(a, umma, false);
+  return low_bytes(a, p->dtype, umma) + adapter_ws(a, umma, false);
 }
 int nnlib_b200_adapter_gemm(const nnlib_b200_adapter_params* p, void* workspace, size_t workspace_bytes, void* stream) {
   Adapters a;
   int rc = resolve_adapter(p, false, &a);
   if (rc || a.main.M == 0 || a.main.N == 0) return rc;
   const bool umma = adapter_on_umma(a, p->dtype);
-  const size_t low = low_bytes(a, umma);
+  const size_t low = low_bytes(a, p->dtype, umma);
   if ((rc = workspace_ok(workspace, workspace_bytes, low + adapter_ws(a, umma, false)))) return rc;
   const void* all[] = {p->C, p->X, p->W, p->A, p->B, p->offsets, p->ids, p->scale, p->status};
   if ((rc = check_arrays(all, 2, 9))) return rc;
@@ -407,14 +407,14 @@ size_t nnlib_b200_adapter_bwd_workspace_bytes(const nnlib_b200_adapter_params* p
     const PairGrads g = pair_grads(p, a, true);
     rest = std::max({rest, low_umma_workspace_bytes(g.first), grouped_umma_grad_workspace_bytes(g.a, 1), grouped_umma_grad_workspace_bytes(g.b, 2)});
   }
-  return 2 * low_bytes(a, umma) + rest;
+  return 2 * low_bytes(a, p->dtype, umma) + rest;
 }
 int nnlib_b200_adapter_bwd(const nnlib_b200_adapter_params* p, void* workspace, size_t workspace_bytes, void* stream) {
   Adapters a;
   int rc = resolve_adapter(p, true, &a);
   if (rc) return rc;
   const bool umma = adapter_on_umma(a, p->dtype);
-  const size_t low = low_bytes(a, umma);
+  const size_t low = low_bytes(a, p->dtype, umma);
   if ((rc = workspace_ok(workspace, workspace_bytes, nnlib_b200_adapter_bwd_workspace_bytes(p)))) return rc;
   const void* all[] = {p->dX, p->dC, p->X, p->W, p->A, p->B, p->offsets, p->ids, p->scale, p->status, p->dA, p->dB};
   if ((rc = check_arrays(all, 2, 12))) return rc;

@@ -101,7 +101,7 @@ struct FwdArgs {
   int M, K, G, N, mats;
   int cap;                               // columns of a tile, at most NT
   int a_kmaj, a_same, zero_rest, splits, tiles_m, to, vec, gather;
-  int low_width, low_step;               // elements of T for a column, from the first term to the second
+  int low_width, low_step;               // elements of T for a column, of each of its terms
   Runs low_runs;                         // kToC: low-rank pairs, r = 0: none
   const int* low_ids;
   const void* low_B;                     // as the caller has it
@@ -300,11 +300,19 @@ __device__ __forceinline__ uint32_t idesc_of(bool bf16, int n, bool a_mn, bool b
   return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)((PAIR ? 256 : 128) >> 4) << 24);
 }
-// T is kept as two terms of 16 bits, together 16 (BFloat16) or 22 bits of it: one alone would be off by what the result is rounded by.  Nothing
-// is left of what is infinite: Inf - Inf would be a NaN.
+// T of a column is kept as two terms of 16 bits, together 16 (BFloat16) or 22 bits of it: one alone would be off by what the result is rounded by.
+// Float16 has no such bits below 2^-14: what is left of a T of 1e-4 is off by 1.7e-4 of T, of 1e-6 by 2 %.  A product is so off by at most 2^-25
+// times the magnitudes in a row of B, where its own result's smallest steps are 2^-24; but the gradients add up many such T.  They take the second
+// term 2^11 times as large, from a third place (at most 2^15: what is left of the largest numbers is 2^4): its step is 2^-35.
+// Nothing is left of what is infinite: Inf - Inf would be a NaN.
+constexpr float kScaled = 2048.f;
 template <typename T>
-__device__ __forceinline__ T left_of(float v, T first) {
-  return Elem<T>::from_f(fabsf(Elem<T>::to_f(first)) < INFINITY ? v - Elem<T>::to_f(first) : 0.f);
+__device__ __forceinline__ void put_terms(T* out, int step, float v) {
+  const T first = Elem<T>::from_f(v);
+  const float left = fabsf(Elem<T>::to_f(first)) < INFINITY ? v - Elem<T>::to_f(first) : 0.f;
+  out[0] = Elem<T>::from_f(left);
+  out[step] = first;
+  if constexpr (std::is_same<T, __half>::value) out[2 * step] = Elem<T>::from_f(left * kScaled);
 }
 __device__ __forceinline__ int round16(int n) { return (n + 15) & ~15; }
 // columns that a product takes are so many at a time (PAIR: half of them from each CTA)
@@ -466,7 +474,7 @@ __device__ __forceinline__ bool odd_pair(const FwdArgs& g, const Tile& o, int id
   const unsigned char* f = g.odd + (long long)(o.m0 >> 7) * g.n + id;
   return (f[0] | (PAIR && o.m0 + 128 < g.M ? f[g.n] : 0)) != 0;
 }
-// K blocks that a pair adds: rank up to 32: both terms of T in one; above: the first terms' blocks, then the second ones'
+// K blocks that a pair adds: rank up to 32: both terms of T in one; above: the blocks of what the first terms leave, then those of the first terms
 __device__ __forceinline__ int low_blocks(int r) { return r <= 32 ? 1 : 2 * ((r + 63) / 64); }
 
 // Looks for infinities and NaN in the matrices of pairs that runs name, 128 rows of one to a warp: warp `w` of `warps`.
@@ -937,12 +945,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
           T* out = reinterpret_cast<T*>(g.C) + (long long)n * g.low_width + m;
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            const float v = m < g.M ? scale * __uint_as_float(acc[j]) : 0.f;
-            const T first = Elem<T>::from_f(v);
-            if (j < nc) {
-              out[(long long)j * g.low_width] = first;
-              out[(long long)j * g.low_width + g.low_step] = left_of(v, first);
-            }
+            if (j < nc) put_terms(out + (long long)j * g.low_width, g.low_step, m < g.M ? scale * __uint_as_float(acc[j]) : 0.f);
           }
         }
       };
@@ -977,7 +980,8 @@ struct GradArgs {
   int rows, cols, G, mats;
   int tiles_r, tiles_c, vec;
   int wait;                              // launched early
-  int fold, fold_step, along;            // fold: columns fold_step apart are the two terms of one; along: a row's columns are contiguous
+  int fold, fold_at, fold_step, along;   // fold: columns fold_step apart, from fold_at on, are the two terms of one; along: a row's columns are contiguous
+  float fold_scale;                      // of the second of them
   float* parts;                          // fold, in parts of the columns: (rows, cols, mats, splits) instead of A
   int splits;
   int* status;
@@ -1080,7 +1084,7 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
     for (long long t = worker; t < tiles && ok; t += workers) {
       const int a = (int)(t / each), in = (int)(t - a * each), q = g.splits > 1 ? in / g.splits : in, split = in - q * g.splits;
       const int r0 = (q % g.tiles_r) * (PAIR ? 256 : 128) + rank * 128, left = g.cols - (q / g.tiles_r) * NT;
-      const int c0 = (q / g.tiles_r) * NT + (PAIR ? rank * (product_columns<true>(min(NT, left)) / 2) : 0);
+      const int c0 = g.fold_at + (q / g.tiles_r) * NT + (PAIR ? rank * (product_columns<true>(min(NT, left)) / 2) : 0);
       Walk walk = walk_of(a, split);
       int begin, end;
       while (ok && next_piece(walk, a, begin, end)) {
@@ -1234,7 +1238,7 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) f[h][i] = __float_as_uint(__uint_as_float(f[h][i]) + __uint_as_float(more[h][i]));
+            for (int i = 0; i < 16; ++i) f[h][i] = __float_as_uint(fmaf(g.fold_scale, __uint_as_float(more[h][i]), __uint_as_float(f[h][i])));
           put_fragments<BF16>(f, box, base, g.ld, m - lane, n, g.rows, g.cols - n, some ? 0u : 0xffffffffu, g.vec != 0);
           continue;
         }
@@ -1248,7 +1252,7 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
           if (m < g.rows) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (j < nc) out[(long long)j * g.rows] = some ? __uint_as_float(acc[j]) + __uint_as_float(more[j]) : 0.f;
+              if (j < nc) out[(long long)j * g.rows] = some ? fmaf(g.fold_scale, __uint_as_float(more[j]), __uint_as_float(acc[j])) : 0.f;
           }
           __syncwarp();
           continue;
@@ -1259,7 +1263,7 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
           for (int j = 0; j < 32; j += 8) {
             float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = some ? __uint_as_float(acc[j + e]) + __uint_as_float(more[j + e]) : 0.f;
+            for (int e = 0; e < 8; ++e) v[e] = some ? fmaf(g.fold_scale, __uint_as_float(more[j + e]), __uint_as_float(acc[j + e])) : 0.f;
             if (g.vec && j + 8 <= nc) {
               *reinterpret_cast<uint4*>(dst + j) = make_uint4(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]), pack2<BF16>(v[4], v[5]), pack2<BF16>(v[6], v[7]));
             } else {
@@ -1576,8 +1580,7 @@ __global__ void __launch_bounds__(256) low_few_kernel(const __grid_constant__ Lo
 }
 // T from the parts of scale * A X: two 16-bit terms, zeros behind the rank
 template <typename T>
-__global__ void __launch_bounds__(256) join_low_kernel(const float* parts, int splits, int r, int R, T* out, int width) {
-  const int step = width / 2;
+__global__ void __launch_bounds__(256) join_low_kernel(const float* parts, int splits, int r, int R, T* out, int width, int step) {
   let_next();
   wait_before();
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -1588,9 +1591,7 @@ __global__ void __launch_bounds__(256) join_low_kernel(const float* parts, int s
 #pragma unroll 4
     for (int s = 0; s < splits; ++s) v += parts[((long long)s * R + n) * r + c];
   }
-  const T first = Elem<T>::from_f(v);
-  out[(long long)n * width + c] = first;
-  out[(long long)n * width + step + c] = left_of(v, first);
+  put_terms(out + (long long)n * width + c, step, v);
 }
 
 // A matrix (or several) that is read: where it lies, contiguous extent first.
@@ -1771,7 +1772,8 @@ bool gathers_in_place(const Operand& x, const Shape& s) {
 
 }  // namespace
 
-int low_width(int r) { return r <= 32 ? 64 : 128 * ((r + 63) / 64); }
+static int low_step(int r) { return r <= 32 ? 32 : 64 * ((r + 63) / 64); }
+int low_width(int r, int dtype) { return (dtype == NNLIB_B200_F16 ? 3 : 2) * low_step(r); }
 
 bool grouped_umma_supports(const GroupedArgs& g, int dtype) {
   return (dtype == NNLIB_B200_F16 || dtype == NNLIB_B200_BF16) && g.M > 0 && g.K > 0 && g.N > 0 && g.R > 0 && g.G > 0 && (g.G <= kMaxRuns || !g.offsets) &&
@@ -1819,8 +1821,8 @@ cudaError_t product(const GroupedArgs& g, int dtype, const Shape& s, int to, voi
   f.zero_rest = g.zero_rest && to == kToC;
   f.splits = s.splits;
   f.to = to;
-  f.low_width = low_width(to == kToLow ? g.M : g.low.r);
-  f.low_step = f.low_width / 2;
+  f.low_width = low_width(to == kToLow ? g.M : g.low.r, dtype);
+  f.low_step = low_step(to == kToLow ? g.M : g.low.r);
   f.status = g.status;
   Maps m;
   if (!encode_matrix(&m.a, dtype, a, g.transA != 0) || !encode_columns(&m.x, dtype, x, in_place ? 1 : box_of(s))) return cudaErrorInvalidValue;
@@ -1830,7 +1832,7 @@ cudaError_t product(const GroupedArgs& g, int dtype, const Shape& s, int to, voi
     Operand b = matrices(g.low.B, g.low.transB != 0, g.M, g.low.r, g.low.ldb, g.low.strideB, g.low.n);
     copied = copied || b.copy_bytes() > 0;
     if ((e = align_operand(b, ws, nullptr, behind, st)) != cudaSuccess) return e;
-    const Operand t{g.low.T, low_width(g.low.r), g.R, low_width(g.low.r), 0, 1, nullptr, 0};
+    const Operand t{g.low.T, f.low_width, g.R, f.low_width, 0, 1, nullptr, 0};
     if (!encode_matrix(&m.b, dtype, b, g.low.transB != 0) || !encode_columns(&m.t, dtype, t, box_of(s))) return cudaErrorInvalidValue;
     f.r = g.low.r;
     f.low_same = g.low.n > 1 && g.low.strideB == 0;
@@ -1908,7 +1910,7 @@ size_t low_umma_workspace_bytes(const GroupedArgs& f) {
   const Shape s = first_shape(f);
   return copies_bytes(f, s) + (s.splits > 1 ? parts_bytes(f, s) : 0);
 }
-size_t low_umma_bytes(const GroupedArgs& f) { return padded((size_t)f.R * 2 * low_width(f.M)); }
+size_t low_umma_bytes(const GroupedArgs& f, int dtype) { return padded((size_t)f.R * 2 * low_width(f.M, dtype)); }
 // behind: a kernel of this call is before it in the stream, whose results it does not read but whose workspace it may write
 cudaError_t low_umma(const GroupedArgs& f, int dtype, void* T, void* workspace, bool behind, cudaStream_t st, unsigned char* odd, const GroupedArgs* look) {
   const int before = behind ? kWaitData : kWaitNone;
@@ -1918,13 +1920,13 @@ cudaError_t low_umma(const GroupedArgs& f, int dtype, void* T, void* workspace, 
   char* parts = ws + copies_bytes(f, s);
   const cudaError_t e = product(f, dtype, s, kToParts, parts, ws, before, st, odd, look);
   if (e != cudaSuccess) return e;
-  const int width = low_width(f.M);
-  const long long blocks = ((long long)f.R * (width / 2) + 255) / 256;
+  const int width = low_width(f.M, dtype), step = low_step(f.M);
+  const long long blocks = ((long long)f.R * step + 255) / 256;
   const float* p = reinterpret_cast<const float*>(parts);
   count_launch();
   const dim3 grid((unsigned)blocks);
-  if (dtype == NNLIB_B200_BF16) return launch_early(join_low_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, p, s.splits, f.M, f.R, static_cast<__nv_bfloat16*>(T), width);
-  return launch_early(join_low_kernel<__half>, grid, dim3(256), 0, st, p, s.splits, f.M, f.R, static_cast<__half*>(T), width);
+  if (dtype == NNLIB_B200_BF16) return launch_early(join_low_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, p, s.splits, f.M, f.R, static_cast<__nv_bfloat16*>(T), width, step);
+  return launch_early(join_low_kernel<__half>, grid, dim3(256), 0, st, p, s.splits, f.M, f.R, static_cast<__half*>(T), width, step);
 }
 
 // W X with the pairs' term; first.R columns.  keep: T of the columns is wanted behind it (the gradients read it), at `low`.
@@ -2003,11 +2005,11 @@ size_t grouped_umma_grad_workspace_bytes(const GroupedGradArgs& g, int fold) {
 bool grouped_umma_grad_supports(const GroupedGradArgs& g, int dtype) {
   return (dtype == NNLIB_B200_F16 || dtype == NNLIB_B200_BF16) && g.M > 0 && g.K > 0 && g.N > 0 && g.R > 0 && g.mats > 0 && encode_tiled_fn() != nullptr;
 }
-// fold: 0: none; 1: C is T, M its rank; 2: X is T, K its rank
+// fold: 0: none; 1: C is T, M its rank; 2: X is T, K its rank.  (The first term and what it leaves, Float16: that 2^11 times as large)
 cudaError_t grouped_umma_grad(const GroupedGradArgs& g, int dtype, int fold, void* workspace, bool behind, cudaStream_t st) {
   char* ws = static_cast<char*>(workspace);
-  Operand c = columns_of(g.C, fold == 1 ? low_width(g.M) : g.M, g.R, g.ldc, nullptr, 0),
-          x = columns_of(g.X, fold == 2 ? low_width(g.K) : g.K, g.N, g.ldx, g.columns, g.R);
+  Operand c = columns_of(g.C, fold == 1 ? low_width(g.M, dtype) : g.M, g.R, g.ldc, nullptr, 0),
+          x = columns_of(g.X, fold == 2 ? low_width(g.K, dtype) : g.K, g.N, g.ldx, g.columns, g.R);
   cudaError_t e = align_operand(c, ws, nullptr, behind, st);
   if (e == cudaSuccess) e = align_operand(x, ws, nullptr, behind, st);
   if (e != cudaSuccess) return e;
@@ -2025,9 +2027,11 @@ cudaError_t grouped_umma_grad(const GroupedGradArgs& g, int dtype, int fold, voi
   a.rows = x_rows ? g.K : g.M;
   a.cols = x_rows ? g.M : g.K;
   a.fold = fold != 0;
-  a.fold_step = fold ? low_width(a.cols) / 2 : 0;
+  a.fold_step = fold ? low_step(a.cols) : 0;
+  a.fold_at = dtype == NNLIB_B200_F16 ? a.fold_step : 0;
+  a.fold_scale = dtype == NNLIB_B200_F16 ? 1.f / kScaled : 1.f;
   a.along = fold && (fold == 1) == (g.transA == 0);
-  const int nt = fold ? low_width(a.cols) : 256;
+  const int nt = fold ? 2 * a.fold_step : 256;
   const bool pair = !fold && a.rows > 128 && a.cols > 128;
   CUtensorMap mc, mx;
   if (!encode_columns(&mc, dtype, c, 64) || !encode_columns(&mx, dtype, x, 64)) return cudaErrorInvalidValue;

@@ -261,8 +261,8 @@ cudaError_t grouped_fma_grad(const GroupedGradArgs& g, int dtype, bool f32_rows,
 bool grouped_umma_supports(const GroupedArgs& g, int dtype);
 size_t grouped_umma_workspace_bytes(const GroupedArgs& g);
 cudaError_t grouped_umma(const GroupedArgs& g, int dtype, void* workspace, cudaStream_t st);
-int low_width(int r);                                     // 16-bit elements of T for a column
-size_t low_umma_bytes(const GroupedArgs& first);          // T of all columns
+int low_width(int r, int dtype);                          // 16-bit elements of T for a column
+size_t low_umma_bytes(const GroupedArgs& first, int dtype);   // T of all columns
 size_t low_umma_workspace_bytes(const GroupedArgs& first);
 // odd, look: where it is noted which matrices of the pairs of `look` have infinities or NaN
 cudaError_t low_umma(const GroupedArgs& first, int dtype, void* T, void* workspace, bool behind, cudaStream_t st, unsigned char* odd = nullptr,

@@ -83,3 +83,32 @@ def test_a_pair_with_infinities_reaches_its_own_columns_alone(dtype, turn, M, K,
         _same_kind(got[1], R.adapters_back(w, x, a, b, ids, offsets, s, d)[0], base[1], others, R.adapters_back(w, x, zeros(a), b, ids, offsets, s, d)[0],
                    _sizes(w, x, zeros(a), b, ids, offsets, s, dtype, d)[1], dtype, "dX")
     assert (got[2] == base[2]).all()                         # (dA = scale B^T dY X^T)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("turn", [(0, 0, 0), (1, 1, 1)])
+@pytest.mark.parametrize("M,K,r,lens", [(256, 136, 16, [300, 300]), (264, 200, 48, [700, 3, 500]), (130, 72, 100, [2000]), (128, 1024, 8, [1] * 40), (64, 33, 16, [9000])])
+def test_gradients_of_small_float16_numbers(turn, M, K, r, lens):
+    """scale * B^T dY of a training step is of some 1e-6, and scale * A X of small columns too: what is kept of them may not be what the gradients are off by.
+    Two Float16 terms, the second 2^11 times as large: |T| * 2^-22, and 2^-36, half a step of Float16's smallest numbers (2^-25) / 2^11."""
+    gen = np.random.default_rng(M + r)
+    N, n = sum(lens), 3
+    offsets, ids = np.concatenate(([0], np.cumsum(lens))).astype(int), [i % n for i in range(len(lens))]
+    W, A, B = _factors(gen, M, K, r, n, F16, turn)
+    w, a, b, s = _f64(W), _f64(A), _f64(B), np.full(n, 0.5)
+    for of_x, of_d in ((1.0, 1e-6), (1e-6, 1.0), (1.0, 2e-5)):
+        X, dY = _cols(of_x * gen.standard_normal((K, N)), F16), _cols(of_d * gen.standard_normal((M, N)), F16)
+        y, back = nb.adapter_mul_pullback(W, X, A, B, _ints(ids), offsets=_ints(offsets), scale=0.5)
+        x, d = _f64(X), _f64(dY)
+        _close(y, R.adapters(w, x, a, b, ids, offsets, s), F16, _sizes(w, x, a, b, ids, offsets, s, F16), "Y")
+        dX, dA, dB = R.adapters_back(*(np.abs(v) for v in (w, x, a, b)), ids, offsets, s, np.abs(d))
+        kept, u = 2.0 ** -22 * 1.01, 2.0 ** -23
+        sA, sB = ((N + M + r + 4) * u * 2 + kept) * dA, ((N + K + r + 4) * u * 2 + kept) * dB
+        for (p, q), i in zip(R.runs(offsets, N), ids):
+            sA[:, :, i] += 2.0 ** -36 * np.abs(x[:, p:q]).sum(1)
+            sB[:, :, i] += 2.0 ** -36 * np.abs(d[:, p:q]).sum(1, keepdims=True)
+        want = R.adapters_back(w, x, a, b, ids, offsets, s, d)
+        got = back(dY)
+        _close(got[0], want[0], F16, _sizes(w, x, a, b, ids, offsets, s, F16, d)[1], "dX")
+        _close(got[1], want[1], F16, sA, "dA")
+        _close(got[2], want[2], F16, sB, "dB")
