@@ -251,9 +251,14 @@ __global__ void __launch_bounds__(256, 2) grouped_fma_kernel(const __grid_consta
   Stages<BN>& st = shared.stages;
   __shared__ RunSearch search;
   __shared__ int cols[BN];
-  const RunTile run = find_run(Runs{g.offsets, g.run_len, g.G, g.R}, g.zero_rest && !parts, BN, blockIdx.x, search);
+  const Runs runs{g.offsets, g.run_len, g.G, g.R};
+  const RunTile run = find_run(runs, g.zero_rest && !parts, BN, blockIdx.x, gridDim.x, search);
   if (run.run == kNoRun) return;
   const int m0 = blockIdx.y * kRows, n0 = run.first, nn = min(BN, run.end - n0);
+  if (run.run == kScattered) {
+    clear_scattered(runs, run, reinterpret_cast<TC*>(g.C), g.ldc, m0, min(kRows, g.M - m0), search);
+    return;
+  }
   const int mat = run.run < 0 ? -1 : (g.ids ? g.ids[run.run] : run.run);
   const bool have = mat >= 0 && mat < g.mats;
   for (int i = threadIdx.x; i < BN; i += 256) {
@@ -339,9 +344,14 @@ __global__ void __launch_bounds__(256, TURNED ? 2 : 3) grouped_narrow_kernel(con
   __shared__ __align__(16) float x[kNarrow][kChunk];
   __shared__ __align__(16) float sums[8][kNarrow][kRows];
   __shared__ RunSearch search;
-  const RunTile run = find_run(Runs{g.offsets, g.run_len, g.G, g.R}, g.zero_rest && !parts, kNarrow, blockIdx.x, search);
+  const Runs runs{g.offsets, g.run_len, g.G, g.R};
+  const RunTile run = find_run(runs, g.zero_rest && !parts, kNarrow, blockIdx.x, gridDim.x, search);
   if (run.run == kNoRun) return;
   const int m0 = blockIdx.y * kRows, n0 = run.first, nn = min(kNarrow, run.end - n0), rows = min(kRows, g.M - m0);
+  if (run.run == kScattered) {
+    clear_scattered(runs, run, reinterpret_cast<TC*>(g.C), g.ldc, m0, rows, search);
+    return;
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int mat = run.run < 0 ? -1 : (g.ids ? g.ids[run.run] : run.run);
   const bool have = mat >= 0 && mat < g.mats;

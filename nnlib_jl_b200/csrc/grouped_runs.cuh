@@ -8,6 +8,7 @@ namespace {
 
 constexpr int kRest = -1;                // a tile of columns in no run, before the first or behind the last
 constexpr int kNoRun = -2;               // no tile at all
+constexpr int kScattered = -3;           // offsets fall somewhere: what columns are in no run is seen column by column
 
 struct Runs {
   const int* offsets;                    // (runs + 1); NULL: len columns each
@@ -29,18 +30,20 @@ struct RunSearch {
   RunTile found;
 };
 
-// Tile number `slot` when the columns before the first run (rest), of every run in turn and behind the last one (rest) are
-// cut into tiles of bt columns.  Called by a whole block of whole warps.
-__device__ inline RunTile find_run(const Runs& of, bool rest, int bt, int slot, RunSearch& s) {
+// Tile number `slot` of `slots` when the columns of every run in turn, before the first one and behind the last one (rest) are
+// cut into tiles of bt columns.  Where offsets fall, the slots behind the runs' tiles are {kScattered, number, how many}.  Called by a whole block of whole warps.
+__device__ inline RunTile find_run(const Runs& of, bool rest, int bt, int slot, int slots, RunSearch& s) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  if (threadIdx.x == 0) s.found = {kNoRun, 0, 0};
   int carry = 0;
-  for (int i0 = -1; i0 <= of.runs; i0 += blockDim.x) {
+  bool falls = false;
+  for (int i0 = 0; i0 < of.runs; i0 += blockDim.x) {
     const int i = i0 + (int)threadIdx.x;
     int first = 0, end = 0;
-    if (i == -1) { if (rest) end = of.runs > 0 ? of.at(0) : of.R; }
-    else if (i < of.runs) { first = of.begin(i); end = of.end(i); }
-    else if (i == of.runs && rest && of.runs > 0) { first = of.at(of.runs); end = of.R; }
+    if (i < of.runs) {
+      first = of.begin(i);
+      end = of.end(i);
+      falls = falls || (rest && of.at(i + 1) < first);
+    }
     const int own = end > first ? (end - first + bt - 1) / bt : 0;
     int sum = own;
 #pragma unroll
@@ -56,12 +59,36 @@ __device__ inline RunTile find_run(const Runs& of, bool rest, int bt, int slot, 
       all += s.part[q];
     }
     const int at = slot - (before + sum - own);
-    if (at >= 0 && at < own) s.found = {i < 0 || i >= of.runs ? kRest : i, first + at * bt, end};
+    if (at >= 0 && at < own) s.found = {i, first + at * bt, end};
     carry = all;
     __syncthreads();
-    if (slot < carry) break;             // (the same for every thread)
+    if (slot < carry) return s.found;    // (the same for every thread)
   }
-  return s.found;
+  if (!rest) return {kNoRun, 0, 0};
+  if (__syncthreads_or(falls)) return {kScattered, slot - carry, slots - carry};
+  const int first = of.runs > 0 ? of.at(0) : of.R, last = of.runs > 0 ? of.at(of.runs) : of.R, before = (first + bt - 1) / bt;
+  if (slot - carry < before) return {kRest, (slot - carry) * bt, first};
+  const long long at = last + (slot - carry - before) * (long long)bt;
+  if (at < of.R) return {kRest, (int)at, of.R};
+  return {kNoRun, 0, 0};
+}
+
+// Zeros for the rows m0 .. m0 + rows - 1 of the columns in no run: chunk t.first, t.first + t.end, ... of 32 columns.  By the whole block.  (There is such a
+// slot whenever there is such a column, see run_slots.)
+template <typename T>
+__device__ inline void clear_scattered(const Runs& of, const RunTile& t, T* C, long long ldc, int m0, int rows, RunSearch& s) {
+  for (long long c0 = t.first * 32ll; c0 < of.R; c0 += t.end * 32ll) {
+    if (threadIdx.x < 32) s.part[threadIdx.x] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < of.runs; i += blockDim.x)
+      for (int n = max(of.begin(i), (int)c0); n < of.end(i) && n < c0 + 32; ++n) s.part[n - c0] = 1;
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * rows; i += blockDim.x) {
+      const int n = i / rows, m = i % rows;
+      if (c0 + n < of.R && !s.part[n]) C[(c0 + n) * ldc + m0 + m] = T(0.f);
+    }
+    __syncthreads();
+  }
 }
 
 // tiles that R columns in `runs` runs can make, with the rest before and behind

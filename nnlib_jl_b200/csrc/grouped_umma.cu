@@ -330,8 +330,8 @@ __host__ __device__ __forceinline__ int tile_count(int n, int cap) {
   return (n + w - 1) / w;
 }
 
-// Fills the table (runs of one length need none).  By the whole block.
-__device__ void count_tiles(const FwdArgs& g, Table& tab, RunSearch& s) {
+// Fills the table (runs of one length need none).  By the whole block.  Whether offsets fall somewhere.
+__device__ bool count_tiles(const FwdArgs& g, Table& tab, RunSearch& s) {
   if (!g.runs.offsets) {
     if (g.r > 0 && g.low_runs.runs <= kMaxRuns) {
       for (int i = threadIdx.x; i < g.low_runs.runs; i += kThreads) {
@@ -341,10 +341,11 @@ __device__ void count_tiles(const FwdArgs& g, Table& tab, RunSearch& s) {
       }
       __syncthreads();
     }
-    return;
+    return false;
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int carry = 0;
+  bool falls = false;
   for (int i0 = 0; i0 < g.G; i0 += kThreads) {
     const int i = i0 + (int)threadIdx.x;
     int own = 0;
@@ -353,6 +354,7 @@ __device__ void count_tiles(const FwdArgs& g, Table& tab, RunSearch& s) {
       if (mat >= 0 && mat < g.mats) own = tile_count(end - begin, g.cap);
       tab.begin[i] = begin;
       tab.end[i] = end;
+      falls = falls || g.runs.at(i + 1) < begin;
     }
     int sum = own;
 #pragma unroll
@@ -372,7 +374,7 @@ __device__ void count_tiles(const FwdArgs& g, Table& tab, RunSearch& s) {
     __syncthreads();
   }
   if (threadIdx.x == 0) tab.cum[g.G] = carry;
-  __syncthreads();
+  return __syncthreads_or(falls) != 0;
 }
 
 // Place in a ring of N stages: no divisions, which cost as much as a stage's copies do.
@@ -706,7 +708,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
   const int rank = PAIR ? cluster_rank() : 0, worker = PAIR ? blockIdx.x >> 1 : blockIdx.x, workers = PAIR ? gridDim.x >> 1 : gridDim.x;
   let_next();
   set_up<NT, PAIR>(bars);
-  count_tiles(g, tab, bars->search);
+  const bool falls = count_tiles(g, tab, bars->search);
   if (g.wait == kWaitData) wait_before();
   tc_fence_before();
   sync_all<PAIR>();
@@ -953,10 +955,14 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
       ++ti;
     }
     if (g.zero_rest && ok) {
-      // columns in no run
-      const int first = tab.begin[0], last = g.runs.at(g.G);
+      // columns in no run: those before the first and behind the last one, or, where offsets fall, what a look at all of them says
+      const int first = falls ? g.runs.R : tab.begin[0], last = falls ? g.runs.R : g.runs.at(g.G);
       const int rest = first + g.runs.R - last;
       for (int i = blockIdx.x * 8 + warp - 2; i < rest; i += gridDim.x * 8) {
+        bool in = false;
+        if (falls)
+          for (int b = 0; b < g.G && !in; b += 32) in = __any_sync(0xffffffffu, b + lane < g.G && tab.begin[b + lane] <= i && i < tab.end[b + lane]);
+        if (in) continue;
         T* out = reinterpret_cast<T*>(g.C) + (long long)(i < first ? i : last + i - first) * g.ldc;
         for (int m = lane; m < g.M; m += 32) out[m] = Elem<T>::from_f(0.f);
       }

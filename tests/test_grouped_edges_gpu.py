@@ -102,3 +102,28 @@ def test_a_columns_result_does_not_depend_on_its_place(M, K, N, turned):
     for by in (1, 2, 5, 8, 19):
         moved = nb.grouped_mul(A, nb.as_column_major(torch.roll(X, by, 1)), _ints([0, N]))
         assert (moved == torch.roll(out, by, 1)).all(), by
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("M,K,G,N", [(136, 72, 4, 90), (512, 256, 4, 900), (40, 2048, 4, 30), (264, 64, 4, 5000)])
+def test_offsets_that_fall(dtype, M, K, G, N):
+    """A run that ends before it begins is empty; what no other run has becomes zeros, and nothing else does."""
+    gen = np.random.default_rng(M + N)
+    A, X, dC = _matrices(gen, M, K, G, dtype, False), _cols(gen.standard_normal((K, N)), dtype), _cols(gen.standard_normal((M, N)), dtype)
+    a, x, d = _f64(A), _f64(X), _f64(dC)
+    u = lambda v: int(round(v * N))
+    for o in ([1.0, 0.0, 0.4, 0.9, 0.8], [0.9, 0.2, 0.5, 0.5, 0.9], [0.6, 0.9, 0.1, 0.3, 0.0], [0.0, 0.5, -3.0, 0.0, 0.0], [0.5, 9.0, 0.1, 0.4, -1.0], [0.8, 0.6, 0.4, 0.2, 0.0]):
+        o = [u(v) for v in o]
+        out, back = nb.grouped_mul_pullback(A, X, _ints(o))
+        want, size = R.grouped(a, x, o), _bound(K, dtype) * R.grouped(np.abs(a), np.abs(x), o)
+        _close(out, want, dtype, size, o)
+        dA, dX = back(dC)
+        wA, wX = R.grouped_back(a, x, o, d)
+        sA, sX = R.grouped_back(np.abs(a), np.abs(x), o, np.abs(d))
+        _close(dA, wA, dtype, _bound(N, dtype) * sA, o)
+        _close(dX, wX, dtype, _bound(M, dtype) * sX, o)
+        keep = _cols(np.full((M, N), 7.0), dtype)
+        nb.grouped_mul_(keep, A, X, _ints(o))
+        want = R.grouped(a, x, o, rest=7.0)
+        _close(keep, want, dtype, size, o)
