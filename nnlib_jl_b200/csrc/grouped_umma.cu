@@ -333,15 +333,15 @@ __host__ __device__ __forceinline__ int tile_count(int n, int cap) {
 // Fills the table (runs of one length need none).  By the whole block.  Whether offsets fall somewhere.
 __device__ bool count_tiles(const FwdArgs& g, Table& tab, RunSearch& s) {
   if (!g.runs.offsets) {
-    if (g.r > 0 && g.low_runs.runs <= kMaxRuns) {
-      for (int i = threadIdx.x; i < g.low_runs.runs; i += kThreads) {
-        tab.cum[i] = g.low_ids[i];
-        tab.begin[i] = g.low_runs.begin(i);
-        tab.end[i] = g.low_runs.end(i);
-      }
-      __syncthreads();
+    if (g.r == 0 || g.low_runs.runs > kMaxRuns) return false;          // (more have no offsets)
+    bool falls = false;
+    for (int i = threadIdx.x; i < g.low_runs.runs; i += kThreads) {
+      tab.cum[i] = g.low_ids[i];
+      tab.begin[i] = g.low_runs.begin(i);
+      tab.end[i] = g.low_runs.end(i);
+      falls = falls || g.low_runs.at(i + 1) < g.low_runs.at(i);
     }
-    return false;
+    return __syncthreads_or(falls) != 0;
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int carry = 0;
@@ -433,15 +433,16 @@ __device__ __forceinline__ Tile tile_of(const FwdArgs& g, const Table& tab, long
   return o;
 }
 
-// Runs of low-rank pairs that have columns in a tile, neighbours of the same pair as one.
+// Runs of low-rank pairs that have columns in a tile, neighbours of the same pair as one.  Where offsets rise, the first is found by halving.
 struct Pairs {
   const Table* tab;                      // NULL: more runs than it holds
+  bool falls;
   int b, end, id, lo, hi;
   __device__ __forceinline__ int first_of(const FwdArgs& g, int i) const { return tab ? tab->begin[i] : g.low_runs.begin(i); }
   __device__ __forceinline__ int end_of(const FwdArgs& g, int i) const { return tab ? tab->end[i] : g.low_runs.end(i); }
   __device__ __forceinline__ int id_of(const FwdArgs& g, int i) const { return tab ? tab->cum[i] : g.low_ids[i]; }
-  __device__ __forceinline__ Pairs(const FwdArgs& g, const Table& t, int n0, int nt) : tab(g.low_runs.runs <= kMaxRuns ? &t : nullptr), end(n0 + nt) {
-    int a = 0, c = g.low_runs.runs;                        // the first run that ends behind n0
+  __device__ __forceinline__ Pairs(const FwdArgs& g, const Table& t, int n0, int nt, bool fall) : tab(g.low_runs.runs <= kMaxRuns ? &t : nullptr), falls(fall), end(n0 + nt) {
+    int a = 0, c = falls ? 0 : g.low_runs.runs;            // the first run that ends behind n0
     while (a < c) {
       const int mid = (a + c) >> 1;
       if (end_of(g, mid) > n0) c = mid; else a = mid + 1;
@@ -451,7 +452,7 @@ struct Pairs {
   __device__ __forceinline__ bool next(const FwdArgs& g, int n0) {
     for (; b < g.low_runs.runs; ++b) {
       lo = max(first_of(g, b), n0);
-      if (lo >= end) return false;
+      if (lo >= end && !falls) return false;
       hi = min(end_of(g, b), end);
       id = id_of(g, b);
       if (lo >= hi || id < 0 || id >= g.n) continue;
@@ -518,9 +519,9 @@ __device__ __forceinline__ void look_for_odd(const FwdArgs& g, long long w, long
 // Adds to a tile of products, in tensor memory, what the pairs that the tensor cores left out give: this warp's rows, every other 32 columns.  Hardly
 // ever called.
 template <bool BF16, bool PAIR>
-__device__ __noinline__ void add_odd(const FwdArgs& g, const Table& tab, const Tile& o, int m, int part, uint32_t taddr) {
+__device__ __noinline__ void add_odd(const FwdArgs& g, const Table& tab, bool falls, const Tile& o, int m, int part, uint32_t taddr) {
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-  Pairs p(g, tab, o.n0, o.nt);
+  Pairs p(g, tab, o.n0, o.nt, falls);
   while (p.next(g, o.n0)) {
     if (!odd_pair<PAIR>(g, o, p.id)) continue;
     const T* b = reinterpret_cast<const T*>(g.low_B) + (long long)p.id * g.low_strideB + (g.low_kmaj ? (long long)m * g.low_ldb : m);
@@ -795,7 +796,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         for (int kb = o.kb0; kb < o.kb1 && ok; kb += C::kSub)
           ok = fill(&tm_a, kb * kBK, g.a_same ? 0 : o.mat, g.a_kmaj != 0, &tm_x, kb * kBK, o, g.gather != 0, four, false, min(C::kSub, o.kb1 - kb));
         if (g.r > 0 && ok) {
-          Pairs p(g, tab, o.n0, o.nt);
+          Pairs p(g, tab, o.n0, o.nt, falls);
           const int blocks = low_blocks(g.r), half = blocks / 2;
           while (ok && p.next(g, o.n0)) {
             if (odd_pair<PAIR>(g, o, p.id)) continue;
@@ -850,7 +851,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         at.skip((o.kb1 - o.kb0 + C::kSub - 1) / C::kSub);
       }
       if (g.r > 0 && ok) {
-        Pairs p(g, tab, o.n0, o.nt);
+        Pairs p(g, tab, o.n0, o.nt, falls);
         const int blocks = low_blocks(g.r), half = blocks / 2;
         const uint32_t step = g.low_kmaj ? 32 >> 4 : 2048 >> 4;
         while (ok && p.next(g, o.n0)) {
@@ -921,7 +922,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
       float scale = 1.f;
       if (g.to != kToC) scale = g.scale ? g.scale[o.mat] : g.scale0;
       if (g.to == kToC) {
-        if (g.r > 0 && chunks > 0 && *reinterpret_cast<volatile int*>(&bars->odd)) add_odd<BF16, PAIR>(g, tab, o, m, part, taddr);
+        if (g.r > 0 && chunks > 0 && *reinterpret_cast<volatile int*>(&bars->odd)) add_odd<BF16, PAIR>(g, tab, falls, o, m, part, taddr);
         auto put = [&](uint32_t (&f)[2][16], int c) {
           uint32_t gone = 0u;
 #pragma unroll

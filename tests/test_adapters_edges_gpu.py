@@ -51,7 +51,7 @@ def _same_kind(got, want, base, others, near, size, dtype, what):
 @pytest.mark.parametrize("turn", [(0, 0, 0), (1, 1, 1)])
 @pytest.mark.parametrize("M,K,r,lens", [
     (136, 64, 16, [10, 50, 1, 39, 50, 17, 33]), (100, 200, 40, [7, 9, 20]), (512, 328, 16, [300, 5, 129, 64, 20, 240, 1]),
-    (320, 136, 100, [64, 32, 16, 500, 3, 40, 200]), (264, 1024, 8, [1] * 24), (512, 200, 64, [512, 256, 256]), (300, 72, 5, [31, 33, 600])])
+    (320, 136, 100, [64, 32, 16, 500, 3, 40, 200]), (264, 1024, 8, [1] * 24), (512, 200, 64, [512, 256, 256]), (300, 72, 5, [31, 33, 600]), (136, 64, 8, [1] * 900)])
 def test_a_pair_with_infinities_reaches_its_own_columns_alone(dtype, turn, M, K, r, lens):
     """Whatever the other requests of a tile are; the pullback's dX is the same product."""
     gen = np.random.default_rng(M + K)
@@ -112,3 +112,21 @@ def test_gradients_of_small_float16_numbers(turn, M, K, r, lens):
         _close(got[0], want[0], F16, _sizes(w, x, a, b, ids, offsets, s, F16, d)[1], "dX")
         _close(got[1], want[1], F16, sA, "dA")
         _close(got[2], want[2], F16, sB, "dB")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("N", [40, 200, 1500])
+def test_offsets_of_requests_that_fall(dtype, N):
+    gen = np.random.default_rng(N)
+    M, K, r, n = 264, 136, 16, 4
+    W, A, B = _factors(gen, M, K, r, n, dtype)
+    X, dY = _cols(gen.standard_normal((K, N)), dtype), _cols(gen.standard_normal((M, N)), dtype)
+    w, x, a, b, d, s = _f64(W), _f64(X), _f64(A), _f64(B), _f64(dY), np.ones(n)
+    for o in ([1.0, 0.0, 0.4, 0.9, 0.8], [0.9, 0.2, 0.5, 0.5, 0.9], [0.6, 0.9, 0.1, 0.3, 0.0], [0.5, 9.0, 0.1, 0.4, -1.0], [0.8, 0.6, 0.4, 0.2, 0.0]):
+        offsets, ids = [int(round(v * N)) for v in o], [1, 3, 0, 2]
+        y, back = nb.adapter_mul_pullback(W, X, A, B, _ints(ids), offsets=_ints(offsets))
+        sizes = _sizes(w, x, a, b, ids, offsets, s, dtype, d)
+        _close(y, R.adapters(w, x, a, b, ids, offsets, s), dtype, sizes[0], o)
+        for got, want, size, what in zip(back(dY), R.adapters_back(w, x, a, b, ids, offsets, s, d), sizes[1:], ("dX", "dA", "dB")):
+            _close(got, want, dtype, size, (what, o))
