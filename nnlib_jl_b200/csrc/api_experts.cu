@@ -18,6 +18,8 @@ bool dtype_ok(int dt) { return dt == NNLIB_B200_F16 || dt == NNLIB_B200_BF16 || 
 int esize(int dt) { return dt == NNLIB_B200_F32 ? 4 : 2; }
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 bool extent(int64_t n) { return n >= 0 && n <= kMost; }
+// the kernels' indexes are 32 bits wide and go up to a tile, or a block's share, beyond an extent
+bool countable(int64_t n) { return n <= kMost - 65536; }
 
 // the arrays of a call: the first `always` are looked up on every call, the rest under NNLIB_B200_CHECK_POINTERS
 int check_arrays(const void* const* ptrs, int always, int n) {
@@ -44,6 +46,7 @@ int resolve_route(const nnlib_b200_route_params* p, bool bwd, RouteArgs* out) {
   if (p->G < 1 || p->N < 0 || p->k < 1 || p->k > p->G || p->logits_stride < 0) return NNLIB_B200_INVALID_ARG;
   if (p->G > 1024 || p->k > 32) return NNLIB_B200_UNSUPPORTED_SHAPE;
   if (p->N > kMost / p->k) return NNLIB_B200_INVALID_ARG;
+  if (!countable(p->N * p->k)) return NNLIB_B200_UNSUPPORTED_SHAPE;
   RouteArgs a;
   std::memset(&a, 0, sizeof(a));
   a.logits = p->logits;
@@ -78,7 +81,7 @@ int resolve_route(const nnlib_b200_route_params* p, bool bwd, RouteArgs* out) {
 int resolve_grouped(const nnlib_b200_grouped_params* p, GroupedArgs* out) {
   if (!p || p->struct_size != sizeof(*p) || !dtype_ok(p->dtype)) return NNLIB_B200_INVALID_ARG;
   if (!extent(p->M) || !extent(p->K) || !extent(p->N) || !extent(p->R) || p->G < 0) return NNLIB_B200_INVALID_ARG;
-  if (p->G > 32767 || p->R > kMost - 65536) return NNLIB_B200_UNSUPPORTED_SHAPE;
+  if (p->G > 32767 || !countable(p->M) || !countable(p->K) || !countable(p->N) || !countable(p->R)) return NNLIB_B200_UNSUPPORTED_SHAPE;
   const int z = esize(p->dtype);
   if (!matrix_ok(p->A, p->M, p->K, p->lda, p->strideA, p->G, p->transA != 0, z) || !matrix_ok(p->X, p->K, p->N, p->ldx, 0, 1, false, z) ||
       !matrix_ok(p->C, p->M, p->R, p->ldc, 0, 1, false, z))
@@ -148,6 +151,7 @@ int resolve_combine(const nnlib_b200_combine_params* p, bool bwd, CombineArgs* o
   if (p->E < 1 || !extent(p->E) || !extent(p->N) || !extent(p->R) || p->k < 1) return NNLIB_B200_INVALID_ARG;
   if (p->k > 32) return NNLIB_B200_UNSUPPORTED_SHAPE;
   if (p->N > kMost / p->k || p->R > kMost - 8) return NNLIB_B200_INVALID_ARG;
+  if (!countable(p->E) || !countable(p->R)) return NNLIB_B200_UNSUPPORTED_SHAPE;
   CombineArgs a;
   std::memset(&a, 0, sizeof(a));
   a.Y = p->Y; a.y = p->y; a.dy = p->dy; a.dY = p->dY;
@@ -184,7 +188,7 @@ struct Adapters {
 int resolve_adapter(const nnlib_b200_adapter_params* p, bool bwd, Adapters* out) {
   if (!p || p->struct_size != sizeof(*p) || !dtype_ok(p->dtype)) return NNLIB_B200_INVALID_ARG;
   if (!extent(p->M) || !extent(p->K) || !extent(p->N) || p->r < 1 || p->n < 0 || p->runs < 0 || p->run_len < 0) return NNLIB_B200_INVALID_ARG;
-  if (p->r > 128 || p->n > 32767 || p->runs > (1 << 20) || p->N > kMost - 65536) return NNLIB_B200_UNSUPPORTED_SHAPE;
+  if (p->r > 128 || p->n > 32767 || p->runs > (1 << 20) || !countable(p->M) || !countable(p->K) || !countable(p->N)) return NNLIB_B200_UNSUPPORTED_SHAPE;
   if (p->run_len > kMost) return NNLIB_B200_INVALID_ARG;
   const int z = esize(p->dtype);
   if (!matrix_ok(p->W, p->M, p->K, p->ldw, 0, 1, p->transW != 0, z) || !matrix_ok(p->A, p->r, p->K, p->lda, p->strideA, p->n, p->transA != 0, z) ||
