@@ -533,7 +533,7 @@ typedef struct nnlib_b200_grouped_params {
   int64_t M, K, G;
   int64_t N, R;              /* columns of X and of C */
   void* A;                   /* (M, K, G); written by grouped_gemm_grad */
-  int64_t lda, strideA;      /* elements between columns and between matrices */
+  int64_t lda, strideA;      /* elements between columns and between matrices (0: one for all runs; not where A is written) */
   const void* X;             /* (K, N) */
   int64_t ldx;
   void* C;                   /* (M, R); read by grouped_gemm_grad */

@@ -355,6 +355,7 @@ int nnlib_b200_grouped_gemm_grad(const nnlib_b200_grouped_params* p, void* works
   GroupedArgs a;
   int rc = resolve_grouped(p, &a);
   if (rc || a.M == 0 || a.K == 0 || a.G == 0) return rc;
+  if (a.G > 1 && a.strideA == 0) return NNLIB_B200_INVALID_ARG;        // (one matrix for all runs is read, not written)
   const GroupedGradArgs g = grad_of(a);
   const bool umma = on_umma(g, p->dtype);
   if (umma && (rc = workspace_ok(workspace, workspace_bytes, grouped_umma_grad_workspace_bytes(g, 0)))) return rc;

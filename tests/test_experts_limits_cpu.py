@@ -23,3 +23,9 @@ def test_extents_near_what_32_bits_count(lib, n):
         assert f(_combine(R=n), None) == (_lib.INVALID_ARG if n > NEAR - 8 else _lib.UNSUPPORTED_SHAPE)
     assert lib.nnlib_b200_route(_route(N=n, k=1), 0x1000, BIG, None) == lib.nnlib_b200_route_bwd(_route(N=n, k=1), None) == _lib.UNSUPPORTED_SHAPE
     assert lib.nnlib_b200_route_workspace_bytes(_route(N=n, k=1)) == 0
+
+
+def test_gradients_that_would_be_written_to_one_matrix(lib):
+    """strideA = 0: one matrix for all runs is read, not written."""
+    f = lambda **kw: lib.nnlib_b200_grouped_gemm_grad(_grouped(strideA=0, **kw), 0x1000, BIG, None)
+    assert f() == _lib.INVALID_ARG and f(M=0) == _lib.OK
