@@ -360,6 +360,8 @@ int nnlib_b200_grouped_gemm_grad(const nnlib_b200_grouped_params* p, void* works
   const bool umma = on_umma(g, p->dtype);
   if (umma && (rc = workspace_ok(workspace, workspace_bytes, grouped_umma_grad_workspace_bytes(g, 0)))) return rc;
   if ((rc = check_grouped_arrays(a))) return rc;
+  if (log_calls())
+    std::fprintf(stderr, "[nnlib_b200] grouped_gemm_grad M=%d K=%d G=%d N=%d R=%d -> %s\n", a.M, a.K, a.G, a.N, a.R, umma ? "tcgen05" : "cuda-core");
   return finish(umma ? grouped_umma_grad(g, p->dtype, 0, workspace, false, (cudaStream_t)stream)
                      : grouped_fma_grad(g, p->dtype, false, false, (cudaStream_t)stream));
 }
@@ -423,6 +425,9 @@ int nnlib_b200_adapter_bwd(const nnlib_b200_adapter_params* p, void* workspace, 
   if ((rc = workspace_ok(workspace, workspace_bytes, nnlib_b200_adapter_bwd_workspace_bytes(p)))) return rc;
   const void* all[] = {p->dX, p->dC, p->X, p->W, p->A, p->B, p->offsets, p->ids, p->scale, p->status, p->dA, p->dB};
   if ((rc = check_arrays(all, 2, 12))) return rc;
+  if (log_calls())
+    std::fprintf(stderr, "[nnlib_b200] adapter_bwd M=%lld K=%lld N=%lld r=%lld runs=%lld -> %s\n", (long long)p->M, (long long)p->K, (long long)p->N,
+                 (long long)p->r, (long long)p->runs, umma ? "tcgen05" : "cuda-core");
   cudaStream_t st = (cudaStream_t)stream;
   char* of_dC = static_cast<char*>(workspace);             // scale * B^T dC
   char* of_X = of_dC + low;                                // scale * A X

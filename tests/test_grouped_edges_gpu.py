@@ -1,5 +1,9 @@
 """Calls of grouped products that their documentation allows and that went wrong once: a routing of which some experts are held, a
 routing of other tokens, one matrix for every run that has to be copied, offsets that fall, a column's place in its tile.  Tolerances as in test_experts_gpu.py."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -127,3 +131,17 @@ def test_offsets_that_fall(dtype, M, K, G, N):
         nb.grouped_mul_(keep, A, X, _ints(o))
         want = R.grouped(a, x, o, rest=7.0)
         _close(keep, want, dtype, size, o)
+
+
+@pytest.mark.gpu
+def test_the_log_names_the_way_of_every_product_and_gradient():
+    code = ("import torch, nnlib_jl_b200 as nb\n"
+            "for t in (torch.bfloat16, torch.float32):\n"
+            "    z = lambda *s: nb.jl_zeros(s, t, torch.device('cuda:0'))\n"
+            "    i = lambda *v: torch.tensor(v, dtype=torch.int32, device='cuda')\n"
+            "    out, back = nb.grouped_mul_pullback(z(64, 32, 2), z(32, 40), i(0, 20, 40)); back(out)\n"
+            "    y, back = nb.adapter_mul_pullback(z(64, 32), z(32, 40), z(8, 32, 2), z(64, 8, 2), i(0, 1), offsets=i(0, 20, 40)); back(y)\n")
+    r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, NNLIB_B200_LOG="1"), capture_output=True, text=True)
+    lines = [(l.split()[1], l.split("->")[1].strip()) for l in r.stderr.splitlines() if l.startswith("[nnlib_b200]")]
+    calls = ["grouped_gemm", "grouped_gemm_grad", "grouped_gemm", "adapter_gemm", "adapter_bwd"]
+    assert lines == [(c, way) for way in ("tcgen05", "cuda-core") for c in calls], r.stderr
