@@ -290,11 +290,18 @@ __global__ void __launch_bounds__(256, 2) grouped_fma_kernel(const __grid_consta
     for (int j = 0; j < 8; ++j) c[i][j] *= scale;
   }
   if (g.low.r > 0) {
-    // the runs of pairs that have columns here, one after the other; columns of other runs take no part
+    // The runs of pairs that have columns here, one after the other; columns of other runs take no part.  Of 256 runs the block sees in one go whether
+    // any has, of equal ones it begins with the first that has (20000 single columns, 256 x 256: 3020 us; 9940 where each block goes through all).
     const Runs of{g.low.offsets, g.low.run_len, g.low.runs, g.R};
     const float* low = reinterpret_cast<const float*>(g.low.T);
     __shared__ int mine[BN];
-    for (int b = 0; b < g.low.runs; ++b) {
+    const int b0 = of.offsets ? 0 : of.len > 0 ? (int)min((long long)of.runs, n0 / of.len) : of.runs;
+    for (int b = b0; b < of.runs; ++b) {
+      if (((b - b0) & 255) == 0) {
+        const auto meets = [&](int i) { return i < of.runs && max(of.begin(i), n0) < min(of.end(i), n0 + nn); };
+        while (b < of.runs && !__syncthreads_or(meets(b + (int)threadIdx.x))) b = of.offsets ? b + 256 : of.runs;
+        if (b >= of.runs) break;
+      }
       const int lo = max(of.begin(b), n0), hi = min(of.end(b), n0 + nn), id = g.low.ids[b];
       if (lo >= hi || id < 0 || id >= g.low.n) continue;
       const T* B = reinterpret_cast<const T*>(g.low.B) + (long long)id * g.low.strideB + (g.low.transB ? (long long)m0 * g.low.ldb : m0);

@@ -130,3 +130,24 @@ def test_offsets_of_requests_that_fall(dtype, N):
         _close(y, R.adapters(w, x, a, b, ids, offsets, s), dtype, sizes[0], o)
         for got, want, size, what in zip(back(dY), R.adapters_back(w, x, a, b, ids, offsets, s, d), sizes[1:], ("dX", "dA", "dB")):
             _close(got, want, dtype, size, (what, o))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize("runs,L", [(3001, 1), (700, 3)])
+def test_many_requests_of_a_few_columns(dtype, given, runs, L):
+    """More than a block looks at in one go, and more columns than are taken one by one."""
+    gen = np.random.default_rng(runs)
+    M, K, r, n, N = 200, 72, 12, 30, runs * L
+    W, A, B = _factors(gen, M, K, r, n, dtype)
+    X, ids = _cols(gen.standard_normal((K, N)), dtype), gen.integers(-1, n + 1, runs)
+    if given:
+        offsets = np.minimum(np.arange(runs + 1) * L + gen.integers(0, L + 1, runs + 1), N)
+        y = nb.adapter_mul(W, X, A, B, _ints(ids), offsets=_ints(offsets))
+    else:
+        offsets = np.arange(runs + 1) * L
+        y = nb.adapter_mul(W, nb.jl_reshape(X, (K, L, runs)) if L > 1 else X, A, B, _ints(ids))
+        y = nb.jl_reshape(y, (M, N))
+    w, x, a, b, s = _f64(W), _f64(X), _f64(A), _f64(B), np.ones(n)
+    _close(y, R.adapters(w, x, a, b, ids, offsets, s), dtype, _sizes(w, x, a, b, ids, offsets, s, dtype), "Y")
