@@ -310,9 +310,18 @@ template <typename T>
 __device__ __forceinline__ void put_terms(T* out, int step, float v) {
   const T first = Elem<T>::from_f(v);
   const float left = fabsf(Elem<T>::to_f(first)) < INFINITY ? v - Elem<T>::to_f(first) : 0.f;
-  out[0] = Elem<T>::from_f(left);
-  out[step] = first;
-  if constexpr (std::is_same<T, __half>::value) out[2 * step] = Elem<T>::from_f(left * kScaled);
+  constexpr bool kThree = std::is_same<T, __half>::value;
+  out[kThree ? step : 0] = first;
+  out[kThree ? 0 : step] = Elem<T>::from_f(left);
+  if constexpr (kThree) out[2 * step] = Elem<T>::from_f(left * kScaled);
+}
+// A gradient's sum from those of the first and the second terms.  A first that is infinite met an infinity of the other array, whose product with the second
+// term, a zero or of the other sign, would make a NaN of it.
+__device__ __forceinline__ float both_terms(uint32_t first, uint32_t second, float scale) {
+  const float v = fmaf(scale, __uint_as_float(second), __uint_as_float(first));
+  float r;
+  asm("{\n\t.reg .pred p;\n\tsetp.nan.f32 p, %1, %1;\n\tselp.f32 %0, %2, %1, p;\n\t}" : "=f"(r) : "f"(v), "f"(__uint_as_float(first)));
+  return r;
 }
 __device__ __forceinline__ int round16(int n) { return (n + 15) & ~15; }
 // columns that a product takes are so many at a time (PAIR: half of them from each CTA)
@@ -477,7 +486,7 @@ __device__ __forceinline__ bool odd_pair(const FwdArgs& g, const Tile& o, int id
   const unsigned char* f = g.odd + (long long)(o.m0 >> 7) * g.n + id;
   return (f[0] | (PAIR && o.m0 + 128 < g.M ? f[g.n] : 0)) != 0;
 }
-// K blocks that a pair adds: rank up to 32: both terms of T in one; above: the blocks of what the first terms leave, then those of the first terms
+// K blocks that a pair adds: rank up to 32: both terms of T in one; above: the blocks of one, then those of the other
 __device__ __forceinline__ int low_blocks(int r) { return r <= 32 ? 1 : 2 * ((r + 63) / 64); }
 
 // Looks for infinities and NaN in the matrices of pairs that runs name, 128 rows of one to a warp: warp `w` of `warps`.
@@ -1245,7 +1254,7 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) f[h][i] = __float_as_uint(fmaf(g.fold_scale, __uint_as_float(more[h][i]), __uint_as_float(f[h][i])));
+            for (int i = 0; i < 16; ++i) f[h][i] = __float_as_uint(both_terms(f[h][i], more[h][i], g.fold_scale));
           put_fragments<BF16>(f, box, base, g.ld, m - lane, n, g.rows, g.cols - n, some ? 0u : 0xffffffffu, g.vec != 0);
           continue;
         }
@@ -1259,7 +1268,7 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
           if (m < g.rows) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (j < nc) out[(long long)j * g.rows] = some ? fmaf(g.fold_scale, __uint_as_float(more[j]), __uint_as_float(acc[j])) : 0.f;
+              if (j < nc) out[(long long)j * g.rows] = some ? both_terms(acc[j], more[j], g.fold_scale) : 0.f;
           }
           __syncwarp();
           continue;
@@ -1270,7 +1279,7 @@ grouped_grad_umma_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_
           for (int j = 0; j < 32; j += 8) {
             float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = some ? fmaf(g.fold_scale, __uint_as_float(more[j + e]), __uint_as_float(acc[j + e])) : 0.f;
+            for (int e = 0; e < 8; ++e) v[e] = some ? both_terms(acc[j + e], more[j + e], g.fold_scale) : 0.f;
             if (g.vec && j + 8 <= nc) {
               *reinterpret_cast<uint4*>(dst + j) = make_uint4(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]), pack2<BF16>(v[4], v[5]), pack2<BF16>(v[6], v[7]));
             } else {

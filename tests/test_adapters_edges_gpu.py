@@ -151,3 +151,31 @@ def test_many_requests_of_a_few_columns(dtype, given, runs, L):
         y = nb.jl_reshape(y, (M, N))
     w, x, a, b, s = _f64(W), _f64(X), _f64(A), _f64(B), np.ones(n)
     _close(y, R.adapters(w, x, a, b, ids, offsets, s), dtype, _sizes(w, x, a, b, ids, offsets, s, dtype), "Y")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("turn", [(0, 0, 0), (1, 1, 1)])
+@pytest.mark.parametrize("M,K,r,lens", [(136, 72, 8, [200, 90, 300]), (256, 200, 64, [600, 40, 7]), (130, 264, 16, [4000, 3, 700])])
+def test_gradients_of_infinite_columns_are_infinite(dtype, turn, M, K, r, lens):
+    """An infinity of X or of dY is one of its pair's gradients, of the sign of what it meets, and no NaN unless it meets a zero or another's sign."""
+    gen = np.random.default_rng(M + r)
+    n, N = 4, sum(lens)
+    W, A, B = _factors(gen, M, K, r, n, dtype, turn)
+    ids, offsets = [1, 3, 0], np.concatenate(([0], np.cumsum(lens))).astype(int)
+    X, dY = _cols(gen.standard_normal((K, N)), dtype), _cols(gen.standard_normal((M, N)), dtype)
+    a, b, s = _f64(A), _f64(B), np.full(n, 0.5)
+    for of_x in (True, False):
+        x, d = X.clone(), dY.clone()
+        if of_x:
+            x[5, 17], x[K - 1, lens[0] + 2], x[5, 30] = float("inf"), -float("inf"), float("inf")
+        else:
+            d[7, 17], d[M - 1, lens[0] + 2], d[7, 40] = float("inf"), -float("inf"), float("inf")
+        dX, dA, dB = nb.adapter_mul_pullback(W, x, A, B, _ints(ids), offsets=_ints(offsets), scale=0.5)[1](d)
+        with np.errstate(invalid="ignore"):
+            _, wA, wB = R.adapters_back(_f64(W), _f64(x), a, b, ids, offsets, s, _f64(d))
+        for got, want, what in ((dA, wA, "dA"), (dB, wB, "dB")):
+            got = _f64(got)
+            for e in (np.inf, -np.inf):
+                assert ((got == e) == (want == e)).all(), (what, of_x)
+            assert (np.isnan(got) == np.isnan(want)).all() and np.isinf(want).any(), (what, of_x)
