@@ -485,8 +485,8 @@ NNLIB_B200_API int nnlib_b200_cache_attn_path(const nnlib_b200_cache* c, const n
 
 /* Products of ragged groups of columns: what a router, its experts and the low-rank pairs of many requests need.  Sizes of
    groups are on the device only: offsets (runs + 1) says that run g is columns offsets[g] .. offsets[g+1] - 1.  An offset
-   outside 0 .. R counts as the nearer of the two, a run that ends before it begins as empty; runs that overlap leave their
-   common columns undefined. */
+   outside 0 .. R counts as the nearer of the two, a run that ends before it begins as empty (offsets may fall); runs that overlap
+   leave their common columns undefined.  Extents go up to 2^31 - 65537. */
 
 /* Each token's k best of G experts (1 <= k <= min(G, 32), G <= 1024) and the tokens' order by expert.
    Chosen are the k largest of logits + bias (in Float32; ties: the lower expert first; a NaN is below everything), in falling order; their
@@ -496,7 +496,7 @@ NNLIB_B200_API int nnlib_b200_cache_attn_path(const nnlib_b200_cache* c, const n
      offsets  (G + 1)  expert g has numbers offsets[g] .. offsets[g+1] - 1
      columns  (k*N)    the token of each number, -1 from offsets[G] on
      position (k, N)   the number of each pair
-   N * k < 2^31. */
+   N * k <= 2^31 - 65537. */
 typedef struct nnlib_b200_route_params {
   size_t struct_size;        /* = sizeof(nnlib_b200_route_params) */
   int32_t dtype;             /* element type of logits and dlogits */
@@ -576,9 +576,10 @@ NNLIB_B200_API int nnlib_b200_combine(const nnlib_b200_combine_params* p, void* 
 NNLIB_B200_API int nnlib_b200_combine_bwd(const nnlib_b200_combine_params* p, void* stream);
 
 /* C = W * X + scale[a] * B[:, :, a] * (A[:, :, a] * X) for the columns of the runs whose id a is a pair's number; a run with
-   another id, and a column in no run, gets W * X alone.  scale * A * X is rounded to two terms of the element type (Float32: not
-   at all) and multiplied by B into the same Float32 sum as W * X; a Float16 one may be infinite
-   beyond 65504.  The workspace holds them, parts of sums, and copies of arrays that TMA cannot address (odd leading dimensions, addresses
+   another id, and a column in no run, gets W * X alone.  scale * A * X is rounded to two terms of the element type (Float32, and
+   some calls of few columns: not at all) and multiplied by B into the same Float32 sum as W * X; a Float16 one may be infinite
+   beyond 65504 and is off by up to 2^-25 (the gradients of A and B take it to 2^-36).  Infinities and NaN of a pair are in its own
+   columns alone.  strideA, strideB = 0: one matrix for all pairs.  The workspace holds the terms, parts of sums, and copies of arrays that TMA cannot address (odd leading dimensions, addresses
    that are no multiples of 16 bytes). */
 typedef struct nnlib_b200_adapter_params {
   size_t struct_size;        /* = sizeof(nnlib_b200_adapter_params) */

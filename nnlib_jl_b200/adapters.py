@@ -85,11 +85,14 @@ def adapter_mul(W: torch.Tensor, X: torch.Tensor, A: torch.Tensor, B: torch.Tens
     ``adapters``, Int32, one per request, from 0; one outside the pairs (-1, say) has none and gets ``W * X``.
 
     The requests are the last dimension of a 3-d ``X``.  For a 2-d one they are runs of columns, ``offsets[b] .. offsets[b + 1]
-    - 1`` (Int32, one more than requests, on the device; a column in no run gets ``W * X``; runs must not overlap), or, without
-    ``offsets``, single columns.  ``scale``: a number, or Float32, one per pair.  Ranks from 1 to 128.
+    - 1`` (Int32, one more than requests, on the device; a column in no run gets ``W * X``; a run that ends before it begins is empty; runs must not
+    overlap), or, without ``offsets``, single columns.  More than 1024 requests with ``offsets`` are computed on the CUDA cores, at a thirtieth of the
+    rate: without them, or as a 3-d ``X``, they are not.  ``scale``: a number, or Float32, one per pair.  Ranks from 1 to 128.  Pairs may share a
+    matrix (``expand``).
 
-    Both terms are summed in Float32 and rounded once.  In between, ``scale * A * X`` is kept as two terms of the element type or in Float32:
-    with Float16 arrays it may be infinite beyond 65504, whatever ``B`` makes of it."""
+    Both terms are summed in Float32 and rounded once.  In between, ``scale * A * X`` is kept as two terms of the element type or in Float32 (few
+    columns).  With Float16 arrays it may so be infinite beyond 65504, whatever ``B`` makes of it, and is off by up to 2^-25, half a step of the smallest
+    numbers, which makes 2^-25 of the magnitudes in a row of ``B``.  Infinities and NaN of a pair are in the columns of its requests alone."""
     p, X2 = _params(W, X, A, B, adapters, offsets, scale)
     out = _columns(X2, W.shape[0], X2.shape[1])
     p.C, p.ldc = out.data_ptr(), W.shape[0] or 1
@@ -101,7 +104,8 @@ def adapter_mul_pullback(W: torch.Tensor, X: torch.Tensor, A: torch.Tensor, B: t
                          offsets: Optional[torch.Tensor] = None, scale: Union[float, torch.Tensor] = 1.0):
     """``rrule``-style forward of :func:`adapter_mul`: ``(Y, back)`` where ``back(dY)`` gives ``(dX, dA, dB)``; ``W`` is taken
     as fixed.  ``dA`` and ``dB`` are stored as ``A`` and ``B`` are, zeros for a pair that no request names; requests that
-    share a pair add to it in their order.  Nothing but the arguments is kept, so none of them may be written to in between."""
+    share a pair add to it in their order.  They take ``scale * A * X`` and ``scale * B' * dY`` with 16 (BFloat16) or 22 bits, in Float16 down to
+    2^-36.  Nothing but the arguments is kept, so none of them may be written to in between."""
     y = adapter_mul(W, X, A, B, adapters, offsets=offsets, scale=scale)
 
     def back(dY: torch.Tensor):

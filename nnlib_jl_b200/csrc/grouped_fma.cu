@@ -9,8 +9,9 @@
 // one's elements are on their way into registers, four neighbours at a time.  A thread multiplies 8 rows and 8 columns as packed pairs of
 // rows, in narrow tiles of every 128 / BN-th k.  A block's slot number is turned into (run, first column) by counting the tiles of all runs, since their sizes
 // are on the device only; slots that no run needs end at once.  Few tiles: K is cut and the parts are added by another launch (join_parts).
-// What bounds it: the FMA pipe and the shared memory that feeds it where columns are many (2048 x 2048, 4096 columns in 8 runs: 807 us,
-// 43 TFLOP/s, with two blocks to an SM and 128 registers; 883 with one; the gradient of the matrices 802 and 1086), reading A where they are few (6248 x 6680, 64 columns in 3 runs: 277 us, 1.8 TB/s).
+// What bounds it: the FMA pipe and the shared memory that feeds it where columns are many (2048 x 2048, 4096 columns in 8 runs: 822 us,
+// 42 TFLOP/s, with two blocks to an SM and 128 registers; 883 with one; the gradient of the matrices 802 and 1086), reading A where they are few (6248 x 6680, 64 columns in 3 runs: 288 us, 1.7 TB/s).
+// (Of these, 15 and 10 us are what the compiler makes of 128 registers since a block also sees to columns in no run where offsets fall.)
 #include <algorithm>
 
 #include "common.cuh"

@@ -175,7 +175,7 @@ bool cache_umma_parts(const CacheAttnArgs& a, int dtype, int splits);         //
 cudaError_t cache_umma(const CacheAttnArgs& a, int dtype, int splits, cudaStream_t st);   // partial results only, if splits > 1
 cudaError_t cache_umma_take_abort(int* out, cudaStream_t st);
 
-// ---- ragged groups of columns (api_experts.cu checks, experts.cu and grouped_*.cu compute) ----
+// ---- ragged groups of columns (api_experts.cu checks, route.cu and grouped_*.cu compute) ----
 struct RouteArgs {
   const void* logits;
   long long stride;

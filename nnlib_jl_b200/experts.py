@@ -180,7 +180,7 @@ def route_topk_pullback(logits: torch.Tensor, k: int, *, bias: Optional[torch.Te
 
 
 # ------------------------------------------------------------------------------------------------- products
-def _grouped(A, X, runs, dims=3):
+def _grouped(A, X, runs):
     """The struct of a product, without its result."""
     p = _lib.GroupedParams.from_buffer_copy(_blank_grouped)
     p.ldx = _matrix("X", X)
@@ -219,8 +219,9 @@ def grouped_mul(A: torch.Tensor, X: torch.Tensor, runs: Union[torch.Tensor, Rout
     """``C[:, i] = A[:, :, g] * X[:, i]`` for the columns ``i`` of run ``g``: ``A`` is ``(M, K, G)``, ``X`` ``(K, N)`` with
     adjacent features, ``runs`` the ``G + 1`` Int32 offsets of the runs, ``offsets[g] .. offsets[g + 1] - 1``, on the device.
     With a :class:`Routing` the columns of ``X`` are gathered: column ``i`` of the result is of column ``routing.columns[i]``.
-    Columns of the result in no run are zeros.  Sums are Float32, results rounded once.  Offsets beyond the columns count as
-    their end; a run that ends before it begins is empty; runs must not overlap."""
+    Columns of the result in no run are zeros, and so are those whose column of ``X`` does not exist.  Sums are Float32, results rounded once.  Offsets beyond
+    the columns count as their end; a run that ends before it begins is empty, so offsets may fall; runs must not overlap.  One matrix for all
+    runs may be ``A.expand(M, K, G)``."""
     p, M, R = _grouped(A, X, runs)
     out = _columns(X, M, R)
     p.C, p.ldc, p.zero_rest = out.data_ptr(), M or 1, 1
@@ -231,8 +232,9 @@ def grouped_mul(A: torch.Tensor, X: torch.Tensor, runs: Union[torch.Tensor, Rout
 def grouped_mul_pullback(A: torch.Tensor, X: torch.Tensor, runs: Union[torch.Tensor, Routing]):
     """``rrule``-style forward of :func:`grouped_mul`: ``(C, back)`` where ``back(dC)`` gives ``(dA, dX)``.  Nothing but the
     arguments is kept, so none of them may be written to in between.  ``dA`` is stored as ``A`` is, zeros for an empty run.
-    The gradients of columns that a :class:`Routing` gathers several times are rounded before they are added; its ``position`` must be
-    that of the columns of ``X``, and the inverse of its ``columns``."""
+    The gradients of columns that a :class:`Routing` gathers several times are rounded before they are added, in Float32, and their sum is rounded
+    again: 1.4 times one rounding (Float32 ones would be twice the bytes to write and to read).  Its ``position`` must be
+    that of the columns of ``X``, and the inverse of its ``columns``; pairs in no run, those of experts that are not among its offsets, add nothing."""
     out = grouped_mul(A, X, runs)
     if isinstance(runs, Routing):
         _pairs("position", runs.position, torch.int32, None, X.shape[1], X.device)
