@@ -141,7 +141,7 @@ def test_the_log_names_the_way_of_every_product_and_gradient():
             "    i = lambda *v: torch.tensor(v, dtype=torch.int32, device='cuda')\n"
             "    out, back = nb.grouped_mul_pullback(z(64, 32, 2), z(32, 40), i(0, 20, 40)); back(out)\n"
             "    y, back = nb.adapter_mul_pullback(z(64, 32), z(32, 40), z(8, 32, 2), z(64, 8, 2), i(0, 1), offsets=i(0, 20, 40)); back(y)\n")
-    r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, NNLIB_B200_LOG="1"), capture_output=True, text=True)
+    r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, NNLIB_B200_LOG="1", NNLIB_B200_FORCE_SIMT="0"), capture_output=True, text=True)
     lines = [(l.split()[1], l.split("->")[1].strip()) for l in r.stderr.splitlines() if l.startswith("[nnlib_b200]")]
     calls = ["grouped_gemm", "grouped_gemm_grad", "grouped_gemm", "adapter_gemm", "adapter_bwd"]
     assert lines == [(c, way) for way in ("tcgen05", "cuda-core") for c in calls], r.stderr
