@@ -73,6 +73,8 @@ def _factor(name: str, t: torch.Tensor):
         trans, ld = 1, (s0 if r > 1 else c)
     elif (r <= 1 or s0 == 1) and (c <= 1 or s1 >= r):
         trans, ld = 0, (s1 if c > 1 else max(r, 1))
+    elif c == 1 and s0 > 1:
+        trans, ld = 1, s0                            # (a column of a matrix whose rows are adjacent)
     else:
         raise TypeError(f"{name}: rows or columns must be adjacent (strides {t.stride()} for size {tuple(t.shape)})")
     return trans, ld, (s2 if n > 1 else 0)

@@ -145,3 +145,19 @@ def test_the_log_names_the_way_of_every_product_and_gradient():
     lines = [(l.split()[1], l.split("->")[1].strip()) for l in r.stderr.splitlines() if l.startswith("[nnlib_b200]")]
     calls = ["grouped_gemm", "grouped_gemm_grad", "grouped_gemm", "adapter_gemm", "adapter_bwd"]
     assert lines == [(c, way) for way in ("tcgen05", "cuda-core") for c in calls], r.stderr
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_matrices_of_one_column_of_wider_ones(dtype):
+    gen = np.random.default_rng(8)
+    for M in (40, 137, 1):
+        A, X, dC = _matrices(gen, M, 9, 3, dtype, True)[:, 3:4], _cols(gen.standard_normal((1, 50)), dtype), _cols(gen.standard_normal((M, 50)), dtype)
+        o = [0, 20, 20, 50]
+        out, back = nb.grouped_mul_pullback(A, X, _ints(o))
+        dA, dX = back(dC)
+        a, x, d = _f64(A), _f64(X), _f64(dC)
+        _close(out, R.grouped(a, x, o), dtype, _bound(1, dtype) * R.grouped(np.abs(a), np.abs(x), o))
+        (wA, wX), (sA, sX) = R.grouped_back(a, x, o, d), R.grouped_back(np.abs(a), np.abs(x), o, np.abs(d))
+        _close(dA, wA, dtype, _bound(50, dtype) * sA)
+        _close(dX, wX, dtype, _bound(M, dtype) * sX)
