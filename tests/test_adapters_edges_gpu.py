@@ -179,3 +179,34 @@ def test_gradients_of_infinite_columns_are_infinite(dtype, turn, M, K, r, lens):
             for e in (np.inf, -np.inf):
                 assert ((got == e) == (want == e)).all(), (what, of_x)
             assert (np.isnan(got) == np.isnan(want)).all() and np.isinf(want).any(), (what, of_x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_a_captured_call_follows_what_the_pairs_hold(dtype):
+    """Whether a pair has infinities is found out on every replay, here by two graphs in turn."""
+    gen = np.random.default_rng(9)
+    M, K, r, n, N = 264, 136, 16, 3, 800
+    W, A, B = _factors(gen, M, K, r, n, dtype)
+    X, dY = _cols(gen.standard_normal((K, N)), dtype), _cols(gen.standard_normal((M, N)), dtype)
+    ids, offsets = _ints([0, 1, 2]), _ints([0, 300, 310, N])
+    run = lambda: (lambda y, back: (y, *back(dY)))(*nb.adapter_mul_pullback(W, X, A, B, ids, offsets=offsets))
+    clean, graphs, outs = run(), [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(run())
+        graphs.append(g)
+    was = B[5, 3, 1].clone()
+    for value in (was, torch.full_like(was, float("inf")), was):
+        B[5, 3, 1] = value
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        want = run()
+        for out in outs:
+            for a, b, c in zip(out, want, clean):
+                assert torch.equal(torch.nan_to_num(a, 7.0, 8.0, 9.0), torch.nan_to_num(b, 7.0, 8.0, 9.0))
+                assert value.isinf() or (a == c).all()
+        assert value.isfinite() or (torch.isinf(outs[0][0][5, 300:310]).all() and torch.isfinite(outs[0][0][:, :300]).all())
+    nb.device_health(DEV)
