@@ -489,40 +489,44 @@ __device__ __forceinline__ bool odd_pair(const FwdArgs& g, const Tile& o, int id
 // K blocks that a pair adds: rank up to 32: both terms of T in one; above: the blocks of one, then those of the other
 __device__ __forceinline__ int low_blocks(int r) { return r <= 32 ? 1 : 2 * ((r + 63) / 64); }
 
-// Looks for infinities and NaN in the matrices of pairs that runs name, 128 rows of one to a warp: warp `w` of `warps`.
+// Looks for infinities and NaN in the matrices of pairs that runs name, 128 rows of one to a warp: warp `w` of `warps`.  Where there are as many runs as pairs, in
+// all pairs (200000 single columns of 20000 pairs: whether an earlier run has the pair took 9 ms).
 template <bool BF16>
 __device__ __forceinline__ void look_for_odd(const FwdArgs& g, long long w, long long warps) {
   constexpr uint32_t kExponent = BF16 ? 0x7f807f80u : 0x7c007c00u, kOne = BF16 ? 0x00800080u : 0x04000400u;
   auto high = [](uint32_t v) { return ((v & kExponent) + kOne) & 0x80008000u; };           // an exponent of ones runs over into the sign's place
-  const int lane = threadIdx.x & 31, runs = g.low_runs.runs;
+  const bool all = g.low_runs.runs >= g.n;
+  const int lane = threadIdx.x & 31, count = all ? g.n : g.low_runs.runs, blocks = (g.look_m + 127) >> 7;
   const bool vec = ((reinterpret_cast<uintptr_t>(g.low_B) & 15) | ((g.low_ldb | g.low_strideB) & 7)) == 0;
-  const long long units = (long long)runs * ((g.look_m + 127) >> 7);
-  for (long long u = w; u < units; u += warps) {
-    const int rb = units <= 0x7fffffff ? (int)u / runs : (int)(u / runs), b = (int)(u - (long long)rb * runs), id = g.low_ids[b];
+  const int parts = (int)min((long long)blocks, max(1ll, warps / max(1, count)));          // warps to a pair
+  for (long long u = w; u < (long long)count * parts; u += warps) {
+    const int part = parts > 1 ? (int)u / count : 0, b = (int)(u - (long long)part * count), id = all ? b : g.low_ids[b];
     if (id < 0 || id >= g.n) continue;
     bool again = false;                                    // an earlier run has the pair
-    for (int i = 0; i < b && !again; i += 32) again = __any_sync(0xffffffffu, i + lane < b && g.low_ids[i + lane] == id);
+    for (int i = 0; i < b && !all && !again; i += 32) again = __any_sync(0xffffffffu, i + lane < b && g.low_ids[i + lane] == id);
     if (again) continue;
-    const int rows = min(128, g.look_m - rb * 128), inner = g.low_kmaj ? g.look_r : rows, outer = g.low_kmaj ? rows : g.look_r;
-    const unsigned short* p = reinterpret_cast<const unsigned short*>(g.low_B) + id * g.low_strideB + rb * 128ll * (g.low_kmaj ? g.low_ldb : 1);
-    const int pieces = vec ? inner >> 3 : 0;               // at most 16: 2^wide lanes to a line
-    const int wide = pieces > 8 ? 4 : pieces > 4 ? 3 : pieces > 2 ? 2 : pieces > 1 ? 1 : 0, c = lane & ((1 << wide) - 1);
-    uint32_t found = 0u;
-    if (c < pieces) {
-      const unsigned short* q = p + c * 8;
+    for (int rb = part; rb < blocks; rb += parts) {
+      const int rows = min(128, g.look_m - rb * 128), inner = g.low_kmaj ? g.look_r : rows, outer = g.low_kmaj ? rows : g.look_r;
+      const unsigned short* p = reinterpret_cast<const unsigned short*>(g.low_B) + id * g.low_strideB + rb * 128ll * (g.low_kmaj ? g.low_ldb : 1);
+      const int pieces = vec ? inner >> 3 : 0;             // at most 16: 2^wide lanes to a line
+      const int wide = pieces > 8 ? 4 : pieces > 4 ? 3 : pieces > 2 ? 2 : pieces > 1 ? 1 : 0, c = lane & ((1 << wide) - 1);
+      uint32_t found = 0u;
+      if (c < pieces) {
+        const unsigned short* q = p + c * 8;
 #pragma unroll 8
-      for (int i = lane >> wide; i < outer; i += 32 >> wide) {
-        const uint4 v = *reinterpret_cast<const uint4*>(q + i * g.low_ldb);
-        found |= high(v.x) | high(v.y) | high(v.z) | high(v.w);
+        for (int i = lane >> wide; i < outer; i += 32 >> wide) {
+          const uint4 v = *reinterpret_cast<const uint4*>(q + i * g.low_ldb);
+          found |= high(v.x) | high(v.y) | high(v.z) | high(v.w);
+        }
       }
-    }
-    if (inner > pieces * 8) {
+      if (inner > pieces * 8) {
 #pragma unroll 4
-      for (int i = 0; i < outer; ++i)
-        for (int e = pieces * 8 + lane; e < inner; e += 32) found |= high(p[i * g.low_ldb + e]);
+        for (int i = 0; i < outer; ++i)
+          for (int e = pieces * 8 + lane; e < inner; e += 32) found |= high(p[i * g.low_ldb + e]);
+      }
+      const int any = __any_sync(0xffffffffu, found != 0u);
+      if (lane == 0) g.odd[(long long)rb * g.n + id] = any ? 1 : 0;
     }
-    const int any = __any_sync(0xffffffffu, found != 0u);
-    if (lane == 0) g.odd[(long long)rb * g.n + id] = any ? 1 : 0;
   }
 }
 // Adds to a tile of products, in tensor memory, what the pairs that the tensor cores left out give: this warp's rows, every other 32 columns.  Hardly
@@ -1715,7 +1719,7 @@ template <bool BF16, int NT, bool PAIR>
 cudaError_t launch_fwd(const Maps& m, FwdArgs g, long long most, cudaStream_t st) {
   g.tiles_m = (g.M + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128);
   // (as many CTAs as look through the pairs' matrices in one go, be the tiles few)
-  const long long looks = g.look_r > 0 ? ((long long)g.low_runs.runs * ((g.look_m + 127) / 128) + 7) / 8 : 0;
+  const long long looks = g.look_r > 0 ? ((long long)std::min(g.low_runs.runs, g.n) * ((g.look_m + 127) / 128) + 7) / 8 : 0;
   return launch<PAIR>(grouped_umma_kernel<BF16, NT, PAIR>, most * g.tiles_m * g.splits + looks, Cfg<NT, PAIR>::kSmem, g.wait != kWaitNone, st, m.a, m.x, m.b, m.t, g);
 }
 template <bool BF16, int NT, bool PAIR>
