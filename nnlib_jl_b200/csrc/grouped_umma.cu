@@ -482,9 +482,9 @@ __device__ __forceinline__ Tile part_of(const Tile& o, const Pairs& p, bool& sha
 }
 // whether the pair is left to the epilogue (for the tile; PAIR: both CTAs' rows)
 template <bool PAIR>
-__device__ __forceinline__ bool odd_pair(const FwdArgs& g, const Tile& o, int id) {
-  const unsigned char* f = g.odd + (long long)(o.m0 >> 7) * g.n + id;
-  return (f[0] | (PAIR && o.m0 + 128 < g.M ? f[g.n] : 0)) != 0;
+__device__ __forceinline__ bool odd_pair(const FwdArgs& g, int m0, int id) {
+  const unsigned char* f = g.odd + (long long)(m0 >> 7) * g.n + id;
+  return (f[0] | (PAIR && m0 + 128 < g.M ? f[g.n] : 0)) != 0;
 }
 // K blocks that a pair adds: rank up to 32: both terms of T in one; above: the blocks of one, then those of the other
 __device__ __forceinline__ int low_blocks(int r) { return r <= 32 ? 1 : 2 * ((r + 63) / 64); }
@@ -532,15 +532,15 @@ __device__ __forceinline__ void look_for_odd(const FwdArgs& g, long long w, long
 // Adds to a tile of products, in tensor memory, what the pairs that the tensor cores left out give: this warp's rows, every other 32 columns.  Hardly
 // ever called.
 template <bool BF16, bool PAIR>
-__device__ __noinline__ void add_odd(const FwdArgs& g, const Table& tab, bool falls, const Tile& o, int m, int part, uint32_t taddr) {
+__device__ __noinline__ void add_odd(const FwdArgs& g, const Table& tab, bool falls, int n0, int nt, int m0, int m, int part, uint32_t taddr) {
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-  Pairs p(g, tab, o.n0, o.nt, falls);
-  while (p.next(g, o.n0)) {
-    if (!odd_pair<PAIR>(g, o, p.id)) continue;
+  Pairs p(g, tab, n0, nt, falls);
+  while (p.next(g, n0)) {
+    if (!odd_pair<PAIR>(g, m0, p.id)) continue;
     const T* b = reinterpret_cast<const T*>(g.low_B) + (long long)p.id * g.low_strideB + (g.low_kmaj ? (long long)m * g.low_ldb : m);
     const long long step = g.low_kmaj ? 1 : g.low_ldb;
     for (int n = p.lo; n < p.hi; ++n) {
-      const int c = n - o.n0;
+      const int c = n - n0;
       if (((c >> 5) & 1) != part) continue;
       const T* t = reinterpret_cast<const T*>(g.low_T) + (long long)n * g.low_width;
       float v = 0.f;
@@ -812,7 +812,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
           Pairs p(g, tab, o.n0, o.nt, falls);
           const int blocks = low_blocks(g.r), half = blocks / 2;
           while (ok && p.next(g, o.n0)) {
-            if (odd_pair<PAIR>(g, o, p.id)) continue;
+            if (odd_pair<PAIR>(g, o.m0, p.id)) continue;
             bool shared;
             const Tile own = part_of<PAIR>(o, p, shared);
             for (int q = 0; q < blocks && ok; ++q) ok = fill(&tm_b, (half ? q % half : 0) * kBK, g.low_same ? 0 : p.id, g.low_kmaj != 0, &tm_t, q * kBK, own, false, four, shared, 1);
@@ -868,7 +868,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         const int blocks = low_blocks(g.r), half = blocks / 2;
         const uint32_t step = g.low_kmaj ? 32 >> 4 : 2048 >> 4;
         while (ok && p.next(g, o.n0)) {
-          if (odd_pair<PAIR>(g, o, p.id)) {
+          if (odd_pair<PAIR>(g, o.m0, p.id)) {
             if (lane == 0) *reinterpret_cast<volatile int*>(&bars->odd) = 1;
             continue;
           }
@@ -935,7 +935,7 @@ grouped_umma_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
       float scale = 1.f;
       if (g.to != kToC) scale = g.scale ? g.scale[o.mat] : g.scale0;
       if (g.to == kToC) {
-        if (g.r > 0 && chunks > 0 && *reinterpret_cast<volatile int*>(&bars->odd)) add_odd<BF16, PAIR>(g, tab, falls, o, m, part, taddr);
+        if (g.r > 0 && chunks > 0 && *reinterpret_cast<volatile int*>(&bars->odd)) add_odd<BF16, PAIR>(g, tab, falls, o.n0, o.nt, o.m0, m, part, taddr);
         auto put = [&](uint32_t (&f)[2][16], int c) {
           uint32_t gone = 0u;
 #pragma unroll
